@@ -65,6 +65,18 @@ PROTOTYPES = {
     "fk_paged_decode_attn_planned": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64,
                                             _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32,
                                             _vp, _sz, _vp, _vp]),
+    "fk_shared_prefix_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "fk_shared_prefix_attn": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _vp,
+                                     _vp, _i64, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32,
+                                     _i32, _vp, _sz, _vp, _vp]),
+    "fk_key_bounds": (_i32, [_vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i64,
+                             _i64, _vp, _i32, _i32, _vp, _vp]),
+    "fk_select_blocks": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i32,
+                                _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "fk_selected_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "fk_selected_attn": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp,
+                                _vp, _i64, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
+                                _f32, _vp, _sz, _vp, _vp]),
     "fk_rmsnorm": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _f32, _i64, _i64,
                           _vp]),
     "fk_fused_add_rmsnorm": (_i32, [_vp, _i64, _vp, _i64, _vp, _f32, _i64, _i64, _vp]),
@@ -186,7 +198,8 @@ PROTOTYPES = {
 # Parts of the library that a partial build may leave out (build.COMPONENT_SOURCES),
 # by the symbols they export; a part is there with all of them or not at all.
 COMPONENTS = {
-    "decode_attn": [n for n in PROTOTYPES if n.startswith("fk_paged_decode_attn")],
+    "decode_attn": [n for n in PROTOTYPES if n.startswith(("fk_paged_decode_attn", "fk_shared_",
+                                                           "fk_key_", "fk_select"))],
     "delta": [n for n in PROTOTYPES if n.startswith("fk_delta_")],
     "latent": [n for n in PROTOTYPES if n.startswith("fk_latent_")],
     "mlstm": [n for n in PROTOTYPES if n.startswith("fk_mlstm_")],

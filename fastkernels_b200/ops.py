@@ -286,6 +286,232 @@ def merge_attn_states(output, prefix_output, prefix_lse, suffix_output, suffix_l
         _stream()), "fk_merge_attn_states")
 
 
+# ------------------------------------------------- decode attention that reads less of the cache
+def _need_here(t: torch.Tensor, dtype, name: str) -> None:
+    """`_need`, and on the device whose stream the kernels go to."""
+    _need(t, dtype, name)
+    if t.device.index != torch.cuda.current_device():
+        raise _lib.FkError(f"{name} is on {t.device}, the current device is "
+                           f"cuda:{torch.cuda.current_device()}")
+
+
+def _need_ints(t: torch.Tensor, numel, name: str) -> None:
+    _need_here(t, torch.int32, name)
+    if t.dim() != 1 or not t.is_contiguous():
+        raise _lib.FkError(f"{name} must be a dense vector")
+    if numel is not None and t.numel() != numel:
+        raise _lib.FkError(f"{name} must have {numel} entries, got {t.numel()}")
+
+
+def _need_tables(block_tables) -> tuple[int, int, int]:
+    """(stride, columns, rows) of page tables; rows may be one row expanded."""
+    _need_here(block_tables, torch.int32, "block_tables")
+    if block_tables.dim() != 2 or block_tables.stride(1) != 1 and block_tables.shape[1] > 1 \
+            and block_tables.shape[0]:
+        raise _lib.FkError("block_tables must be [rows, pages] with dense rows")
+    rows, cols = block_tables.shape
+    return block_tables.stride(0) if rows > 1 else cols, cols, rows
+
+
+def _need_cache(cache, kv_layout, name, like=None) -> tuple[int, int, int, int, int]:
+    """(pages, page size, KV heads, head size, page stride) of a paged pool."""
+    _need_here(cache, BF16, name)
+    if kv_layout not in ("NHD", "HND"):
+        raise _lib.FkError("kv_layout must be 'NHD' or 'HND'")
+    if cache.dim() != 4:
+        raise _lib.FkError(f"{name} must have four dimensions")
+    if kv_layout == "NHD":
+        pages, page, hkv, d = cache.shape
+        dense = (hkv * d, d, 1)
+    else:
+        pages, hkv, page, d = cache.shape
+        dense = (page * d, d, 1)
+    if cache.stride()[1:] != dense:
+        raise _lib.FkError(f"{name} must be dense within a page")
+    if like is not None and (cache.shape != like.shape or cache.stride() != like.stride()):
+        raise _lib.FkError("cache shape mismatch")
+    return pages, page, hkv, d, cache.stride(0) if pages > 1 else page * hkv * d
+
+
+def _need_rows(t, like, name) -> int:
+    """Token stride of q or out, [tokens, heads, D] with dense heads."""
+    _need_here(t, BF16, name)
+    if t.dim() != 3 or like is not None and t.shape != like.shape:
+        raise _lib.FkError(f"{name} must be [tokens, heads, D]")
+    n, heads, d = t.shape
+    if n and (t.stride(2) != 1 and d > 1 or t.stride(1) != d and heads > 1):
+        raise _lib.FkError(f"{name} heads must be dense")
+    return t.stride(0) if n > 1 else heads * d
+
+
+def _workspace(workspace, need: int, like) -> torch.Tensor:
+    if workspace is None:
+        return torch.empty(max(need, 1), dtype=torch.uint8, device=like.device)
+    if not workspace.is_cuda or workspace.device != like.device or not workspace.is_contiguous():
+        raise _lib.FkError("the workspace must be dense and on the device of q")
+    return workspace
+
+
+def shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, head_dim,
+                                  max_splits) -> int:
+    return int(lib.fk_shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads,
+                                                    head_dim, max_splits))
+
+
+def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_starts, prefix_lens,
+                       softmax_scale, workspace=None, max_splits=None, out=None, status=None,
+                       kv_layout="NHD"):
+    """paged_decode_attn for a batch whose rows group_starts[g] .. group_starts[g + 1] - 1 list the
+    same pages for their first prefix_lens[g] tokens: that part is read once for all of them.
+
+    group_starts int32 [groups + 1] ascends from 0 on, prefix_lens int32 [groups]; of a prefix that
+    ends inside a page the whole pages are taken together.  Rows outside of all groups have nothing
+    in common.  context_lens count all tokens of a row, the common ones too.  GQA ratios up to 16.
+    A workspace of shared_prefix_workspace_bytes holds the schedule and partial results of one call
+    at a time; without one it is allocated here."""
+    pages, page, hkv, d2, stride = _need_cache(k_cache, kv_layout, "k_cache")
+    _need_cache(v_cache, kv_layout, "v_cache", k_cache)
+    qs = _need_rows(q, None, "q")
+    b, hq, d = q.shape
+    if d2 != d:
+        raise _lib.FkError("cache shape mismatch")
+    _need_ints(context_lens, b, "context_lens")
+    ts, cols, rows = _need_tables(block_tables)
+    if rows != b:
+        raise _lib.FkError(f"block_tables must have {b} rows, got {rows}")
+    groups = prefix_lens.numel()
+    _need_ints(prefix_lens, groups, "prefix_lens")
+    _need_ints(group_starts, groups + 1, "group_starts")
+    if out is None:
+        out = torch.empty((b, hq, d), dtype=BF16, device=q.device)
+    os_ = _need_rows(out, q, "out")
+    if max_splits is None:
+        max_splits = max_splits_for(cols * page)
+    workspace = _workspace(workspace, shared_prefix_workspace_bytes(b, groups, hq, hkv, d,
+                                                                    max_splits), q)
+    check(lib.fk_shared_prefix_attn(
+        _ptr(q), qs, _ptr(out), os_, _ptr(k_cache), _ptr(v_cache), pages, page, stride,
+        int(kv_layout == "HND"), _ptr(context_lens), _ptr(block_tables), ts, cols,
+        _ptr(group_starts), _ptr(prefix_lens), groups, b, hq, hkv, d, float(softmax_scale),
+        int(max_splits), _ptr(workspace), workspace.numel() * workspace.element_size(),
+        _status_ptr(status, q), _stream()), "fk_shared_prefix_attn")
+    return out
+
+
+def new_key_bounds(k_cache, block, kv_layout="NHD") -> torch.Tensor:
+    """Bounds of all blocks of `block` tokens of a pool, [pages, Hkv, page // block, 2, D], zeroed;
+    key_bounds fills in those of the blocks that hold tokens."""
+    pages, page, hkv, d, _ = _need_cache(k_cache, kv_layout, "k_cache")
+    if block < 1 or page % block:
+        raise _lib.FkError(f"a page of {page} tokens is not a whole number of blocks of {block}")
+    return torch.zeros((pages, hkv, page // block, 2, d), dtype=BF16, device=k_cache.device)
+
+
+def _need_bounds(bounds) -> None:
+    _need_here(bounds, BF16, "bounds")
+    if bounds.dim() != 5 or bounds.shape[3] != 2 or not bounds.is_contiguous():
+        raise _lib.FkError("bounds must be a contiguous [pages, Hkv, blocks of a page, 2, D]")
+
+
+def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new=1,
+               kv_layout="NHD", status=None):
+    """Smallest and largest key per channel, in place and exact, of the blocks that hold the newest
+    tokens of each sequence: the last one, or with cu_new (int32 [sequences + 1], as
+    cu_seqlens) the last cu_new[s + 1] - cu_new[s], at most max_new.  Call it after those tokens' keys
+    have been stored; context_lens count them.  A block that is not full yet has the bounds of the
+    keys in it.  A sequence (and so a page with new tokens) appears once in the batch."""
+    pages, page, hkv, d, stride = _need_cache(k_cache, kv_layout, "k_cache")
+    _need_bounds(bounds)
+    per = bounds.shape[2]
+    if tuple(bounds.shape) != (pages, hkv, per, 2, d) or per < 1 or page % per:
+        raise _lib.FkError("bounds do not fit the cache")
+    n = context_lens.numel()
+    _need_ints(context_lens, None, "context_lens")
+    ts, cols, rows = _need_tables(block_tables)
+    if rows != n:
+        raise _lib.FkError(f"block_tables must have {n} rows, got {rows}")
+    if cu_new is not None:
+        _need_ints(cu_new, n + 1, "cu_new")
+    check(lib.fk_key_bounds(
+        _ptr(k_cache), pages, page, stride, int(kv_layout == "HND"), hkv, d, _ptr(bounds),
+        page // per, _ptr(context_lens), _ptr(block_tables), ts, cols, _ptr(cu_new), n,
+        int(max_new), _status_ptr(status, k_cache), _stream()), "fk_key_bounds")
+    return bounds
+
+
+def select_blocks(q, bounds, context_lens, block_tables, block, count, keep_first=1, keep_last=1,
+                  table_rows=None, out=None, status=None):
+    """Blocks of `block` tokens for each query token and KV head, int32 [tokens, Hkv, count] in
+    ascending order, -1 behind the last: the first keep_first, the last keep_last (the last of all
+    holds the token itself), and those whose bounds allow the largest logit of any query head of
+    the KV head, max_h sum_d max(q_hd lo_d, q_hd hi_d); the lower index on ties.
+
+    context_lens int32 [tokens]: keys that a token sees, itself among them.  table_rows int32
+    [tokens]: its row of block_tables (None: its own number).  Bounds of a token's last block are
+    not read; all others before it must be there."""
+    qs = _need_rows(q, None, "q")
+    _need_bounds(bounds)
+    n, hq, d = q.shape
+    pages, hkv, per, _, d2 = bounds.shape
+    if d2 != d:
+        raise _lib.FkError("bounds do not fit q")
+    _need_ints(context_lens, n, "context_lens")
+    ts, cols, rows = _need_tables(block_tables)
+    if table_rows is not None:
+        _need_ints(table_rows, n, "table_rows")
+    if out is None:
+        out = torch.empty((n, hkv, count), dtype=torch.int32, device=q.device)
+    _need_here(out, torch.int32, "out")
+    if tuple(out.shape) != (n, hkv, count) or not out.is_contiguous():
+        raise _lib.FkError("out must be a contiguous [tokens, Hkv, count]")
+    check(lib.fk_select_blocks(
+        _ptr(q), qs, _ptr(bounds), pages, per * block, block, _ptr(context_lens),
+        _ptr(table_rows), _ptr(block_tables), ts, cols, rows, n, hq, hkv, d, int(count),
+        int(keep_first), int(keep_last), _ptr(out), _status_ptr(status, q), _stream()),
+        "fk_select_blocks")
+    return out
+
+
+def selected_attn_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, head_dim, count,
+                                  block) -> int:
+    return int(lib.fk_selected_attn_workspace_bytes(num_tokens, num_q_heads, num_kv_heads,
+                                                    head_dim, count, block))
+
+
+def selected_attn(q, k_cache, v_cache, context_lens, block_tables, selected, block, softmax_scale,
+                  table_rows=None, workspace=None, out=None, status=None, kv_layout="NHD"):
+    """Attention of each query token over the blocks in selected [tokens, Hkv, count] (int32, as
+    select_blocks gives them), at positions below its context_lens.  Entries below 0 or past the
+    context hold no keys, and one that is listed twice counts twice; a token without keys gets
+    zeros.  table_rows as in select_blocks; GQA ratios up to 16."""
+    pages, page, hkv, d2, stride = _need_cache(k_cache, kv_layout, "k_cache")
+    _need_cache(v_cache, kv_layout, "v_cache", k_cache)
+    qs = _need_rows(q, None, "q")
+    n, hq, d = q.shape
+    if d2 != d:
+        raise _lib.FkError("cache shape mismatch")
+    _need_ints(context_lens, n, "context_lens")
+    ts, cols, rows = _need_tables(block_tables)
+    if table_rows is not None:
+        _need_ints(table_rows, n, "table_rows")
+    _need_here(selected, torch.int32, "selected")
+    if selected.dim() != 3 or selected.shape[:2] != (n, hkv) or not selected.is_contiguous():
+        raise _lib.FkError("selected must be a contiguous [tokens, Hkv, count]")
+    count = selected.shape[2]
+    if out is None:
+        out = torch.empty((n, hq, d), dtype=BF16, device=q.device)
+    os_ = _need_rows(out, q, "out")
+    workspace = _workspace(workspace, selected_attn_workspace_bytes(n, hq, hkv, d, count, block),
+                           q)
+    check(lib.fk_selected_attn(
+        _ptr(q), qs, _ptr(out), os_, _ptr(k_cache), _ptr(v_cache), pages, page, stride,
+        int(kv_layout == "HND"), _ptr(context_lens), _ptr(table_rows), _ptr(block_tables), ts,
+        cols, rows, _ptr(selected), count, int(block), n, hq, hkv, d, float(softmax_scale),
+        _ptr(workspace), workspace.numel() * workspace.element_size(), _status_ptr(status, q),
+        _stream()), "fk_selected_attn")
+    return out
+
+
 # --------------------------------------------------------------------------- norms
 def rmsnorm(x, weight, eps, out=None):
     """out = bf16(x * rsqrt(mean(x^2)+eps) * w); x is [..., cols], last dim dense.

@@ -178,6 +178,88 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
                                  int32_t* status, fk_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Decode attention that reads less of the paged cache (no counterpart in the
+ * reference).  Caches, block tables, context_lens and softmax_scale as in
+ * fk_paged_decode_attn, with any num_q_heads / num_kv_heads up to 16, bf16,
+ * head_dim 128; block_table_cols = entries of a table's row that may be read
+ * (a context beyond them is cut there and flagged FK_DEV_BAD_PAGE).  A page id
+ * outside the pool is flagged FK_DEV_BAD_PAGE; nothing is read in its place (its
+ * keys are left out of fk_selected_attn, and zeros in fk_shared_prefix_attn).
+ *
+ * fk_shared_prefix_attn: out as fk_paged_decode_attn, for a batch in which the
+ * rows group_starts[g] .. group_starts[g + 1] - 1 list the same pages for their
+ * first prefix_lens[g] tokens (whole pages of them).  That part is read through
+ * the table of the group's first row, once for all rows of the group: their
+ * query heads are the rows of one product per KV head.  group_starts
+ * [num_groups + 1] ascends; rows outside of all groups, and groups of one row, have
+ * nothing in common.  A row's context may end inside the common part.
+ * max_splits: upper bound of KV splits of what each row has for itself.
+ *
+ * fk_key_bounds: bounds[page][head][i][0 / 1][d] = smallest / largest key of
+ * channel d over the cached tokens of the i-th run of `block` positions of a page,
+ * i in [0, page_size / block), for the blocks that hold the last
+ * cu_new[s + 1] - cu_new[s] tokens of sequence s (cu_new NULL: one token each),
+ * at most max_new each.  context_lens count the new tokens, whose keys are in the
+ * cache already.  Bounds of other blocks stay as they are.  A sequence appears
+ * once.  No-number keys give no-number bounds.
+ *
+ * fk_select_blocks: for query token i and KV head, of the n = ceil(context_lens[i]
+ * / block) blocks that it sees, in ascending order: the first keep_first, the last
+ * keep_last (>= 1: the block that holds the token itself, whose bounds are not
+ * read) and those with the largest
+ *   max over the query heads h of the KV head of sum_d max(q_hd lo_d, q_hd hi_d),
+ * count in all, the lower index on ties, -1 behind the last where n < count.  The
+ * choice is that of 64-bit sums.  A score that is no number counts as the largest,
+ * a block whose page id is bad as the smallest.  table_rows[i] is the table of token
+ * i (NULL: i itself), so several tokens of a prompt may select with one table.
+ * At most 16384 blocks per table.
+ *
+ * fk_selected_attn: attention of query token i over the keys of selected[i][head]
+ * [0 .. count) at positions below context_lens[i]; entries below 0 or at or past
+ * the context's end hold no keys, and a block that is listed twice counts twice.
+ * A token without keys gets zeros.
+ * ---------------------------------------------------------------------- */
+size_t fk_shared_prefix_workspace_bytes(int batch, int num_groups, int num_q_heads,
+                                        int num_kv_heads, int head_dim, int max_splits);
+
+int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
+                          int64_t out_stride_token, const void* k_cache, const void* v_cache,
+                          int64_t num_pages, int page_size, int64_t kv_page_stride, int kv_layout,
+                          const int32_t* context_lens, const int32_t* block_tables,
+                          int64_t block_table_stride, int64_t block_table_cols,
+                          const int32_t* group_starts, const int32_t* prefix_lens, int num_groups,
+                          int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                          float softmax_scale, int max_splits, void* workspace,
+                          size_t workspace_bytes, int32_t* status, fk_stream_t stream);
+
+int fk_key_bounds(const void* k_cache, int64_t num_pages, int page_size, int64_t kv_page_stride,
+                  int kv_layout, int num_kv_heads, int head_dim, void* bounds, int block,
+                  const int32_t* context_lens, const int32_t* block_tables,
+                  int64_t block_table_stride, int64_t block_table_cols, const int32_t* cu_new,
+                  int num_seqs, int max_new, int32_t* status, fk_stream_t stream);
+
+int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, int64_t num_pages,
+                     int page_size, int block, const int32_t* context_lens,
+                     const int32_t* table_rows, const int32_t* block_tables,
+                     int64_t block_table_stride, int64_t block_table_cols, int num_tables,
+                     int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int count,
+                     int keep_first, int keep_last, int32_t* selected, int32_t* status,
+                     fk_stream_t stream);
+
+size_t fk_selected_attn_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads,
+                                        int head_dim, int count, int block);
+
+int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t out_stride_token,
+                     const void* k_cache, const void* v_cache, int64_t num_pages, int page_size,
+                     int64_t kv_page_stride, int kv_layout, const int32_t* context_lens,
+                     const int32_t* table_rows, const int32_t* block_tables,
+                     int64_t block_table_stride, int64_t block_table_cols, int num_tables,
+                     const int32_t* selected, int count, int block, int num_tokens,
+                     int num_q_heads, int num_kv_heads, int head_dim, float softmax_scale,
+                     void* workspace, size_t workspace_bytes, int32_t* status,
+                     fk_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * RMSNorm and fused residual-add + RMSNorm.
  * Replace RMSNorm.forward(x, residual=None)
  * (fastkernels/tasks/baseline/L1/rms_norm.py:153-164; kernels

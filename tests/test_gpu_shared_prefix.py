@@ -1,0 +1,196 @@
+"""Decode attention of batches whose sequences begin with the same pages, on the GPU."""
+import numpy as np
+import pytest
+import torch
+
+import selected_oracle as S
+from gpu_util import dev, host_f32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from fastkernels_b200 import ops as _ops
+    return _ops
+
+
+def ints(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+
+def build(seed, groups, page, layout, hq, hkv, extra_rows=()):
+    """groups: (prefix tokens, [tokens behind it of each row]).  Rows of a group share the whole
+    pages of its prefix.  extra_rows: lengths of rows behind the last group.  What is behind
+    a row's last token, and in nobody's pages, is no number."""
+    rng = np.random.default_rng(seed)
+    lens, starts, prefix = [], [0], []
+    plan = []                                     # (shared pages, own pages) of each row
+    for p, own in groups:
+        prefix.append(p)
+        starts.append(starts[-1] + len(own))
+        whole = p // page
+        for s in own:
+            n = max(0, p + s)
+            lens.append(n)
+            plan.append((whole, max(0, -(-n // page) - whole)))
+    for n in extra_rows:
+        lens.append(n)
+        plan.append((0, -(-n // page)))
+    total = sum(p // page for p, _ in groups) + sum(o for _, o in plan) + 2
+    order = rng.permutation(total).astype(np.int32)
+    cols = max(s + o for s, o in plan) + 1
+    table = np.full((len(lens), cols), -1, np.int32)
+    at, row = 0, 0
+    live = np.zeros((total, page), bool)
+    for p, own in groups:
+        common = order[at:at + p // page]
+        at += len(common)
+        live[common] = True
+        for _ in own:
+            table[row, :len(common)] = common
+            row += 1
+    for i, (shared, own) in enumerate(plan):
+        table[i, shared:shared + own] = order[at:at + own]
+        at += own
+        for pos in range(shared * page, lens[i]):
+            live[table[i, pos // page], pos % page] = True
+    kc, vc = (S.pool(rng, total, page, hkv, layout) for _ in range(2))
+    for c in (kc, vc):
+        (c if layout == "NHD" else c.swapaxes(1, 2))[~live] = np.nan
+    q = S.bf16(rng.standard_normal((len(lens), hq, S.D)))
+    return q, kc, vc, np.array(lens, np.int32), table, starts, prefix
+
+
+def run(ops, case, layout, status=None, **kw):
+    q, kc, vc, lens, table, starts, prefix = case
+    return ops.shared_prefix_attn(dev(q), dev(kc), dev(vc), ints(lens), ints(table), ints(starts),
+                                  ints(prefix), S.SCALE, kv_layout=layout, status=status, **kw)
+
+
+def check(ops, case, page, layout, hkv, **kw):
+    q, kc, vc, lens, table, _, _ = case
+    st = ops.new_status("cuda")
+    got = run(ops, case, layout, st, **kw)
+    out, mass = S.over_positions(q, kc, vc, lens, table, page, layout, hkv,
+                                 lambda i, h: range(lens[i]))
+    d = np.abs(host_f32(got).astype(np.float64) - out)
+    over = d - S.tolerance(out, mass)
+    assert (over <= 0).all(), (over.max(), np.unravel_index(over.argmax(), over.shape))
+    assert int(st.item()) == 0
+    return got
+
+
+@pytest.mark.parametrize("page,layout,hq,hkv", [(64, "NHD", 8, 2), (16, "HND", 16, 2),
+                                                (256, "NHD", 4, 4), (32, "NHD", 10, 2),
+                                                (64, "HND", 16, 1), (16, "NHD", 7, 1),
+                                                (192, "NHD", 6, 2)])
+def test_groups_of_all_kinds(ops, page, layout, hq, hkv):
+    groups = [(4 * page, [1, 5, page, page + 1]),        # ordinary
+              (page, [3]),                               # alone
+              (0, [7, 300]),                             # nothing in common
+              (9 * page, [0, 1, 2 * page + 3]),          # a row that ends with the common part
+              (5 * page, [-page - 3, 2, -5 * page, 1]),  # rows that end inside it, one empty
+              (2 * page + 5, [20, 30]),                  # ends inside a page
+              (page - 1, [page, 9])]                     # not one whole page
+    check(ops, build(page + hq, groups, page, layout, hq, hkv, extra_rows=[70, 0, 1]), page, layout,
+          hkv)
+
+
+@pytest.mark.parametrize("rows,hq,hkv", [(2, 2, 2), (33, 4, 1), (32, 8, 2), (40, 16, 1),
+                                         (130, 2, 2), (65, 12, 3), (26, 10, 2), (129, 2, 1),
+                                         (17, 32, 2)])
+def test_rows_of_a_group_over_tiles(ops, rows, hq, hkv):
+    """Numbers of rows times query heads around and past the tiles of a product."""
+    case = build(rows + hq, [(320, [i % 70 for i in range(rows)])], 64, "NHD", hq, hkv)
+    check(ops, case, 64, "NHD", hkv)
+
+
+@pytest.mark.parametrize("prefix", [16, 112, 128, 144, 2048, 12304])
+def test_lengths_of_the_common_part(ops, prefix):
+    case = build(prefix, [(prefix, [5, 300, 1]), (prefix + 160, [1, 2])], 16, "HND", 4, 2)
+    check(ops, case, 16, "HND", 2)
+
+
+def test_many_groups(ops):
+    rng = np.random.default_rng(2)
+    groups = [(int(rng.integers(0, 9)) * 16, [int(x) for x in rng.integers(1, 60, rng.integers(1, 5))])
+              for _ in range(90)]
+    check(ops, build(1, groups, 16, "NHD", 4, 2), 16, "NHD", 2)
+
+
+def test_no_groups_and_one_row(ops):
+    check(ops, build(1, [], 64, "NHD", 8, 2, extra_rows=[1, 700, 64, 0]), 64, "NHD", 2)
+    check(ops, build(2, [(640, [11])], 64, "NHD", 8, 2), 64, "NHD", 2)
+    check(ops, build(3, [(1280, [1, 1])], 64, "NHD", 8, 2), 64, "NHD", 2, max_splits=1)
+
+
+def test_large_scores(ops):
+    """Scores of some hundreds, the largest in either part."""
+    case = build(8, [(1024, [200, 300, 1]), (64, [700, 3])], 64, "NHD", 8, 2)
+    q, kc, vc, lens, table = case[:5]
+    q[:] = S.bf16(q * 60)
+    got = run(ops, case, "NHD")
+    out, mass = S.over_positions(q, kc, vc, lens, table, 64, "NHD", 2, lambda i, h: range(lens[i]))
+    # scores off by at most 2^-17 of the sum of |q k| (below 2^9): 2^-8
+    d = np.abs(host_f32(got) - out)
+    assert (d <= S.tolerance(out, mass) + 2 * 2.0 ** -8 * mass).all()
+
+
+def test_strided_rows_and_neighbours_of_the_result(ops):
+    case = build(5, [(256, [5, 9, 70])], 64, "NHD", 8, 2)
+    packed = torch.zeros((3, 12 * 128), dtype=torch.bfloat16, device="cuda")
+    packed[:, :1024] = dev(case[0]).view(3, 1024)
+    out = torch.full((5, 10, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    q, kc, vc, lens, table, starts, prefix = case
+    ops.shared_prefix_attn(packed[:, :1024].view(3, 8, 128), dev(kc), dev(vc), ints(lens),
+                           ints(table), ints(starts), ints(prefix), S.SCALE, out=out[:3, :8])
+    assert torch.equal(out[:3, :8], run(ops, case, "NHD"))
+    assert (out[3:] == 3.0).all() and (out[:, 8:] == 3.0).all()
+
+
+def test_bad_pages_are_flagged_and_left_out(ops):
+    case = build(6, [(256, [5, 9, 70]), (128, [3, 4])], 64, "NHD", 8, 2)
+    q, kc, vc, lens, table, starts, prefix = case
+    good = host_f32(run(ops, case, "NHD"))
+    broken = table.copy()
+    broken[0, 1], broken[4, 2] = 10 ** 6, -7
+    st = ops.new_status("cuda")
+    got = host_f32(run(ops, (q, kc, vc, lens, broken, starts, prefix), "NHD", st))
+    assert int(st.item()) == 2
+    assert np.isfinite(got).all() and (got[3] == good[3]).all()
+
+
+def test_in_a_graph_with_other_lengths(ops):
+    """Captured once; replayed with other lengths, groups and queries in the same buffers."""
+    rng = np.random.default_rng(9)
+    case = build(9, [(640, [400, 500, 600]), (320, [100, 900])], 64, "NHD", 8, 2)
+    q, kc, vc, lens, table, starts, prefix = case
+    kc, vc = np.nan_to_num(kc), np.nan_to_num(vc)
+    a = [dev(q), dev(kc), dev(vc), ints(lens), ints(table), ints(starts), ints(prefix)]
+    ws = torch.empty(ops.shared_prefix_workspace_bytes(5, 2, 8, 2, 128, 16), dtype=torch.uint8,
+                     device="cuda")
+    ops.shared_prefix_attn(*a, S.SCALE, workspace=ws, max_splits=16)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.shared_prefix_attn(*a, S.SCALE, workspace=ws, max_splits=16)
+    for step in range(3):
+        q = S.bf16(rng.standard_normal(q.shape))
+        lens = (lens - rng.integers(0, 90, 5)).astype(np.int32)
+        shorter = [640 - 64 * step, 320 - 128 * step]
+        a[0].copy_(dev(q))
+        a[3].copy_(ints(lens))
+        a[6].copy_(ints(shorter))
+        g.replay()
+        want, mass = S.over_positions(q, kc, vc, lens, table, 64, "NHD", 2,
+                                      lambda i, h: range(lens[i]))
+        d = np.abs(host_f32(out) - want)
+        assert (d <= S.tolerance(want, mass)).all()
+
+
+def test_same_bits_every_time(ops):
+    case = build(10, [(4096, [40, 50, 60, 1000] * 4), (320, [100, 900])], 64, "NHD", 8, 2)
+    first = run(ops, case, "NHD")
+    for _ in range(3):
+        assert torch.equal(run(ops, case, "NHD"), first)
