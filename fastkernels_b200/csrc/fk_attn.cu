@@ -27,17 +27,15 @@
 // HBM traffic per call = the algorithmic bytes (K and V of every live token
 // once, q, out, lens, block tables) + split partials (fp32, < 4 % at the chosen
 // split sizes).
-#include "fk_common.cuh"
+#include "fk_attn.cuh"
 
 #include <mutex>
 #include <unordered_map>
 
 namespace fk {
 
-constexpr int ATT_D = 128;                  // head_dim
 constexpr int ATT_NW = 8;                   // consumer warps
-constexpr int ATT_TILE = ATT_NW * 16;       // tokens per pipeline stage
-constexpr int ATT_BOX = 64;                 // tokens per TMA box
+static_assert(ATT_TILE == ATT_NW * 16, "a consumer warp takes 16 tokens of a tile");
 constexpr int ATT_STAGES = 3;
 constexpr int ATT_THREADS = (ATT_NW + 1) * 32;
 constexpr int ATT_BOX_BYTES = ATT_BOX * 128;          // 64 tokens x 64 bf16
@@ -50,7 +48,8 @@ constexpr int ATT_PLAN_HDR = 8;                       // ints before chunk_start
 enum : int { TILE_FIRST = 1, TILE_LAST = 2, TILE_END = 4 };
 
 struct TileMeta {
-  int seq, kvh, split, nsplits, n_valid, flags, pad0, pad1;
+  int seq, kvh, split, nsplits, n_valid, flags;
+  uint32_t valid[2];        // selected blocks: valid tokens of each 16-token slab, a byte each
 };
 
 struct AttnSmem {
@@ -65,27 +64,6 @@ struct AttnSmem {
   static constexpr int kAlloc = kTotal + 1024;  // manual 1024-byte alignment
 };
 static_assert(AttnSmem::kAlloc <= 232448, "shared memory budget");
-
-struct AttnParams {
-  const uint16_t* q; int64_t q_stride;
-  uint16_t* out; int64_t out_stride;
-  const int32_t* context_lens;
-  const int32_t* block_tables; int64_t bt_stride;
-  int batch, hq, hkv, g;
-  int block_size; int num_blocks;
-  int sub_tokens;     // tokens per TMA copy = min(block_size, 64)
-  int fused16;        // 16-token pages: one 5-D copy brings both 64-dim halves of a page
-  int bs_shift;       // log2(block_size) when it is a power of two, else -1
-  int hnd;            // 1: pool is [blocks, Hkv, block, D]; 0: [blocks, block, Hkv, D]
-  float scale_log2;
-  int max_splits;
-  int direct;         // 1: no plan, no splits: CTA b handles (sequence, KV head) item b whole
-  int* plan;          // header + chunk_start[batch+1]
-  int4* chunk_info;   // per chunk: {seq, split | nsplits << 16, tok_begin, tok_end}
-  float* part_o;      // [batch, hq, max_splits, D]
-  float2* part_ml;    // [batch, hq, max_splits]
-  int32_t* status;
-};
 
 __device__ __forceinline__ uint64_t global_ns() {
   uint64_t t;
@@ -254,11 +232,158 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(
 }
 
 // ---------------------------------------------------------------------------
+// producer of selected blocks
+// ---------------------------------------------------------------------------
+// The tiles of all tokens and KV heads, `tiles` each, are one sequence of which every CTA takes a run
+// of `unit`: what falls into one run is a split of its token and head.  The whole warp resolves 32
+// listed blocks at a time (block, page, valid tokens), a lane each, and issues a tile's pieces of
+// `sub_tokens` as the producer of whole contexts does.  Pieces without keys are not copied and
+// tiles without keys not sent; a tile is held back until the next one is known, since the last one
+// of a split says so.
+__device__ __forceinline__ void att_produce_selected(
+    const CUtensorMap& tmap_k, const CUtensorMap& tmap_v, const AttnParams& p, uint8_t* stages,
+    uint8_t* qslots, TileMeta* metas, uint64_t* full, uint64_t* empty, volatile int* abort_flag,
+    int lane) {
+  const int st = p.sub_tokens, block = p.sel_block;
+  const int64_t total = (int64_t)p.batch * p.hkv * p.tiles;
+  int64_t at = (int64_t)blockIdx.x * p.unit;
+  const int64_t end = at + p.unit < total ? at + p.unit : total;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  while (ok && at < end) {
+    const int64_t item = at / p.tiles;
+    const int t0 = (int)(at - item * p.tiles);
+    const int t1 = end - at < p.tiles - t0 ? t0 + (int)(end - at) : p.tiles;
+    at += t1 - t0;
+    const int token = (int)(item / p.hkv), kvh = (int)(item - (int64_t)token * p.hkv);
+    int first_cta, last_cta;
+    selected_ctas(item, p.tiles, p.unit, &first_cta, &last_cta);
+    const int split = (int)blockIdx.x - first_cta, nsplits = last_cta - first_cta + 1;
+    const int row = p.rows ? p.rows[token] : token;
+    int64_t len64 = p.context_lens[token];
+    const bool bad_row = row < 0 || row >= p.num_tables || len64 > p.capacity;
+    if (bad_row && lane == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+    if (len64 > p.capacity) len64 = p.capacity;
+    const int len = row < 0 || row >= p.num_tables || len64 < 0 ? 0 : (int)len64;
+    const int32_t* sel = p.selected + item * p.count;
+    const int32_t* table = p.block_tables + (int64_t)row * p.bt_stride;
+    // this lane's entry of the batch of 32: page (-1: none), position of its first token, tokens
+    int base = t0 * ATT_TILE / block, page = -1, pos = 0, keys = 0;
+    auto listed = [&](int e) -> int { return e < p.count ? sel[e] : -1; };
+    auto resolve = [&](int b) {
+      page = -1; pos = 0; keys = 0;
+      if (b < 0 || (int64_t)b * block >= len) return;
+      pos = b * block;
+      page = table[pos / p.block_size];
+      if (page < 0 || page >= p.num_blocks) {
+        page = -1;
+        if (p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+        return;
+      }
+      keys = min(block, len - pos);
+    };
+    resolve(listed(base + lane));
+    int ahead = listed(base + 32 + lane);
+    bool have = false;                         // a tile is held back
+    int h_page = 0, h_off = 0, h_keys = 0, flags = TILE_FIRST;
+    auto send = [&](bool last) -> bool {
+      int pass = 1;
+      if (lane == 0) pass = att_wait(&empty[stage], phase ^ 1, abort_flag, p.status) ? 1 : 0;
+      pass = __shfl_sync(0xffffffffu, pass, 0);
+      if (!pass) return false;
+      const int slab = (lane & 7) * 16;
+      int v = __shfl_sync(0xffffffffu, h_keys, slab / st) - slab % st;
+      v = min(16, max(0, v)) << ((lane & 3) * 8);
+      const uint32_t v0 = __reduce_or_sync(0xffffffffu, lane < 4 ? (uint32_t)v : 0u);
+      const uint32_t v1 = __reduce_or_sync(0xffffffffu, lane >= 4 && lane < 8 ? (uint32_t)v : 0u);
+      const uint32_t pieces = __ballot_sync(0xffffffffu, h_keys > 0);
+      if (last) flags |= TILE_LAST;
+      if (lane == 0) {
+        TileMeta m;
+        m.seq = token; m.kvh = kvh; m.split = split; m.nsplits = nsplits;
+        m.n_valid = ATT_TILE;
+        m.flags = flags;
+        m.valid[0] = v0; m.valid[1] = v1;
+        metas[stage] = m;
+        uint32_t bytes = (uint32_t)__popc(pieces) * 4u * (uint32_t)st * 128u;
+        if (flags & TILE_FIRST) bytes += (uint32_t)p.g * ATT_D * 2u;
+        mbar_arrive_expect_tx(&full[stage], bytes);
+        if (flags & TILE_FIRST)
+          bulk_load(qslots + stage * ATT_QSLOT_BYTES,
+                    p.q + (int64_t)token * p.q_stride + (int64_t)kvh * p.g * ATT_D,
+                    (uint32_t)p.g * ATT_D * 2u, &full[stage]);
+      }
+      __syncwarp();
+      if (h_keys > 0) {
+        uint8_t* kdst = stages + stage * ATT_STAGE_BYTES;
+        uint8_t* vdst = kdst + ATT_KV_BYTES;
+        if (p.fused16) {
+          tma_load_5d(kdst + lane * 4096, &tmap_k, &full[stage], 0, h_off, 0, kvh, h_page);
+          tma_load_5d(vdst + lane * 4096, &tmap_v, &full[stage], 0, h_off, 0, kvh, h_page);
+        } else {
+          const int my = lane * st, b = my / ATT_BOX, r0 = my % ATT_BOX;
+          const int c1 = p.hnd ? h_off : kvh, c2 = p.hnd ? kvh : h_off;
+#pragma unroll
+          for (int dh = 0; dh < 2; ++dh) {
+            const int dsto = (b * 2 + dh) * ATT_BOX_BYTES + r0 * 128;
+            tma_load_4d(kdst + dsto, &tmap_k, &full[stage], dh * 64, c1, c2, h_page);
+            tma_load_4d(vdst + dsto, &tmap_v, &full[stage], dh * 64, c1, c2, h_page);
+          }
+        }
+      }
+      flags = 0;
+      if (++stage == ATT_STAGES) { stage = 0; phase ^= 1; }
+      return true;
+    };
+    for (int t = t0; t < t1 && ok; ++t) {
+      if ((t * ATT_TILE + ATT_TILE - 1) / block >= base + 32) {
+        const int to = t * ATT_TILE / block;
+        resolve(to == base + 32 ? ahead : listed(to + lane));
+        base = to;
+        ahead = listed(base + 32 + lane);
+      }
+      const int my = t * ATT_TILE + (lane * st & (ATT_TILE - 1));
+      const int e = my / block, in = my - e * block;
+      const int n_page = __shfl_sync(0xffffffffu, page, e - base);
+      const int n_pos = __shfl_sync(0xffffffffu, pos, e - base) + in;
+      int n_keys = __shfl_sync(0xffffffffu, keys, e - base) - in;
+      n_keys = lane * st < ATT_TILE ? min(st, max(0, n_keys)) : 0;
+      if (!__any_sync(0xffffffffu, n_keys > 0)) continue;
+      if (have) ok = send(false);
+      have = true;
+      h_page = n_page;
+      h_off = n_pos % p.block_size;
+      h_keys = n_keys;
+    }
+    if (!ok) break;
+    if (have) {
+      ok = send(true);
+    } else if (nsplits == 1) {
+      uint4* dst = reinterpret_cast<uint4*>(p.out + (int64_t)token * p.out_stride +
+                                            (int64_t)kvh * p.g * ATT_D);
+      for (int i = lane; i < p.g * ATT_D / 8; i += 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+    } else if (lane < p.g) {
+      p.part_ml[((int64_t)token * p.hq + kvh * p.g + lane) * p.max_splits + split] =
+          make_float2(-INFINITY, 0.f);
+    }
+  }
+  if (lane == 0) {
+    if (att_wait(&empty[stage], phase ^ 1, abort_flag, p.status)) {
+      TileMeta m{};
+      m.flags = TILE_END;
+      metas[stage] = m;
+      mbar_arrive(&full[stage]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // main kernel
 // ---------------------------------------------------------------------------
 // SPLIT: the softmax weights enter P V as two bf16 parts (16 significant bits) instead
-// of one.
-template <bool G16, bool SPLIT>
+// of one.  SEL: over selected blocks.
+template <bool G16, bool SPLIT, bool SEL>
 __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
     const __grid_constant__ CUtensorMap tmap_k,
     const __grid_constant__ CUtensorMap tmap_v, const AttnParams p) {
@@ -303,6 +428,10 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
     if (lane == 0) {
       tma_prefetch_desc(&tmap_k);
       tma_prefetch_desc(&tmap_v);
+    }
+    if constexpr (SEL) {
+      att_produce_selected(tmap_k, tmap_v, p, stages, qslots, metas, full, empty, abort_flag, lane);
+      return;
     }
     const int total_items = p.direct ? p.batch * p.hkv : plan[0] * p.hkv;
     int* counter = const_cast<int*>(plan) + 2;
@@ -388,7 +517,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
           m.seq = seq; m.kvh = kvh; m.split = split; m.nsplits = nsplits;
           m.n_valid = n_valid;
           m.flags = flags;
-          m.pad0 = m.pad1 = 0;
+          m.valid[0] = m.valid[1] = 0;
           metas[stage] = m;
           uint32_t bytes = (uint32_t)ncopy * 4u * (uint32_t)st * 128u;
           if (flags & TILE_FIRST) bytes += (uint32_t)p.g * ATT_D * 2u;
@@ -491,7 +620,9 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
       for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
 
-    const int nv = min(16, meta.n_valid - w * 16);  // valid tokens in my slab
+    // valid tokens in my slab
+    const int nv = SEL ? (int)(meta.valid[w >> 2] >> ((w & 3) * 8) & 255u)
+                       : min(16, meta.n_valid - w * 16);
     if (nv > 0) {
       const uint32_t kbase = smem_u32(stages + stage * ATT_STAGE_BYTES) + slab_off;
       const uint32_t vbase = kbase + ATT_KV_BYTES;
@@ -778,28 +909,27 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const AttnParams p) {
 // host: tensor-map cache
 // ---------------------------------------------------------------------------
 struct MapKey {
-  const void* ptr; int64_t num_blocks; int block_size; int hkv; int64_t stride; int hnd;
+  const void* ptr; int64_t num_blocks; int block_size; int hkv; int64_t stride; int hnd; int sub;
   bool operator==(const MapKey& o) const {
     return ptr == o.ptr && num_blocks == o.num_blocks &&
            block_size == o.block_size && hkv == o.hkv && stride == o.stride &&
-           hnd == o.hnd;
+           hnd == o.hnd && sub == o.sub;
   }
 };
 struct MapKeyHash {
   size_t operator()(const MapKey& k) const {
     size_t h = std::hash<const void*>()(k.ptr);
     h ^= std::hash<int64_t>()(k.num_blocks * 1315423911ll + k.block_size * 2654435761ll +
-                              k.hkv * 97ll + k.stride + k.hnd * 7919ll);
+                              k.hkv * 97ll + k.stride + k.hnd * 7919ll + k.sub * 31ll);
     return h;
   }
 };
 static std::mutex g_map_mu;
 static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> g_maps;
 
-static int get_kv_map(const void* cache, int64_t num_blocks, int block_size,
-                      int hkv, int64_t block_stride, int hnd, int fused,
-                      CUtensorMap* out) {
-  MapKey key{cache, num_blocks, block_size, hkv, block_stride, hnd + 2 * fused};
+int get_kv_map(const void* cache, int64_t num_blocks, int block_size, int hkv,
+               int64_t block_stride, int hnd, int sub, int fused, CUtensorMap* out) {
+  MapKey key{cache, num_blocks, block_size, hkv, block_stride, hnd + 2 * fused, sub};
   std::lock_guard<std::mutex> lk(g_map_mu);
   auto it = g_maps.find(key);
   if (it != g_maps.end()) {
@@ -812,7 +942,6 @@ static int get_kv_map(const void* cache, int64_t num_blocks, int block_size,
   // One copy = `sub` tokens x 64 dims of one KV head inside one page.
   //   NHD pool [blocks, block, Hkv, D]: dims (D, Hkv, token, block)
   //   HND pool [blocks, Hkv, block, D]: dims (D, token, Hkv, block)
-  const cuuint32_t sub = (cuuint32_t)(block_size < ATT_BOX ? block_size : ATT_BOX);
   cuuint64_t dims[4], strides[3];
   cuuint32_t box[4];
   dims[0] = ATT_D; dims[3] = (cuuint64_t)num_blocks;
@@ -822,26 +951,26 @@ static int get_kv_map(const void* cache, int64_t num_blocks, int block_size,
     dims[1] = (cuuint64_t)block_size; dims[2] = (cuuint64_t)hkv;
     strides[0] = (cuuint64_t)ATT_D * 2;
     strides[1] = (cuuint64_t)block_size * ATT_D * 2;
-    box[1] = sub; box[2] = 1;
+    box[1] = (cuuint32_t)sub; box[2] = 1;
   } else {
     dims[1] = (cuuint64_t)hkv; dims[2] = (cuuint64_t)block_size;
     strides[0] = (cuuint64_t)ATT_D * 2;
     strides[1] = (cuuint64_t)hkv * ATT_D * 2;
-    box[1] = 1; box[2] = sub;
+    box[1] = 1; box[2] = (cuuint32_t)sub;
   }
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUtensorMap m;
   CUresult r;
   if (fused) {
-    // Pages of fewer than 64 tokens: the two 64-dim halves of a head become a
+    // Copies of fewer than 64 tokens: the two 64-dim halves of a head become a
     // dimension of their own, (64 dims, token, dim half, head, page), so that one
-    // copy of box (64, page tokens, 2, 1, 1) lands as [dim half][token][128 B].
+    // copy of box (64, sub, 2, 1, 1) lands as [dim half][token][128 B].
     const cuuint64_t tok_stride = hnd ? (cuuint64_t)ATT_D * 2 : (cuuint64_t)hkv * ATT_D * 2;
     const cuuint64_t head_stride =
         hnd ? (cuuint64_t)block_size * ATT_D * 2 : (cuuint64_t)ATT_D * 2;
     cuuint64_t d5[5] = {64, (cuuint64_t)block_size, 2, (cuuint64_t)hkv, (cuuint64_t)num_blocks};
     cuuint64_t s5[4] = {tok_stride, 128, head_stride, (cuuint64_t)block_stride * 2};
-    cuuint32_t b5[5] = {64, (cuuint32_t)block_size, 2, 1, 1};
+    cuuint32_t b5[5] = {64, (cuuint32_t)sub, 2, 1, 1};
     r = enc(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(cache), d5, s5, b5,
             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -856,6 +985,23 @@ static int get_kv_map(const void* cache, int64_t num_blocks, int block_size,
   g_maps.emplace(key, m);
   *out = m;
   return FK_OK;
+}
+
+cudaError_t launch_decode(bool g16, bool split, bool selected, int grid, const CUtensorMap& mk,
+                          const CUtensorMap& mv, const AttnParams& p, cudaStream_t s) {
+  static PerDeviceOnce once[6];
+  auto go = [&](PerDeviceOnce& o, auto kernel) {
+    const cudaError_t e = set_max_dynamic_smem(o, kernel, AttnSmem::kAlloc);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(kernel, dim3(grid), dim3(ATT_THREADS), (size_t)AttnSmem::kAlloc, s, mk,
+                         mv, p);
+  };
+  if (selected) return g16 ? go(once[5], attn_decode_kernel<true, false, true>)
+                           : go(once[4], attn_decode_kernel<false, false, true>);
+  if (g16) return split ? go(once[3], attn_decode_kernel<true, true, false>)
+                        : go(once[1], attn_decode_kernel<true, false, false>);
+  return split ? go(once[2], attn_decode_kernel<false, true, false>)
+               : go(once[0], attn_decode_kernel<false, false, false>);
 }
 
 static size_t plan_hdr_bytes(int batch) {
@@ -880,23 +1026,6 @@ size_t fk_paged_decode_attn_workspace_bytes(int batch, int num_q_heads,
   const size_t parts = (size_t)batch * num_q_heads * max_splits;
   return plan_bytes(batch, max_splits) + parts * head_dim * sizeof(float) +
          parts * sizeof(float2);
-}
-
-// launch of the main kernel: 16 query heads per KV head or fewer, weights in one part
-// or two
-static cudaError_t launch_decode(bool g16, bool split, int grid, const CUtensorMap& mk,
-                                 const CUtensorMap& mv, const AttnParams& p, cudaStream_t s) {
-  static PerDeviceOnce once[4];
-  auto go = [&](PerDeviceOnce& o, auto kernel) {
-    const cudaError_t e = set_max_dynamic_smem(o, kernel, AttnSmem::kAlloc);
-    if (e != cudaSuccess) return e;
-    return launch_kernel(kernel, dim3(grid), dim3(ATT_THREADS), (size_t)AttnSmem::kAlloc, s, mk,
-                         mv, p);
-  };
-  if (g16) return split ? go(once[3], attn_decode_kernel<true, true>)
-                        : go(once[1], attn_decode_kernel<true, false>);
-  return split ? go(once[2], attn_decode_kernel<false, true>)
-               : go(once[0], attn_decode_kernel<false, false>);
 }
 
 static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token, void* out,
@@ -959,22 +1088,23 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
   // copies per 128-token tile held the kernel at 0.74 of the HBM peak).  If the
   // driver refuses the 5-D map, the per-half copies are used.
   int fused16 = block_size == 16 ? 1 : 0;
+  const int sub = block_size < ATT_BOX ? block_size : ATT_BOX;
   if (mode != 1) {
     int rc = FK_OK;
     if (fused16) {
       rc = get_kv_map(k_cache, num_blocks, block_size, num_kv_heads, kv_block_stride,
-                      kv_layout, 1, &mk);
+                      kv_layout, sub, 1, &mk);
       if (rc == FK_OK)
         rc = get_kv_map(v_cache, num_blocks, block_size, num_kv_heads, kv_block_stride,
-                        kv_layout, 1, &mv);
+                        kv_layout, sub, 1, &mv);
       if (rc != FK_OK) fused16 = 0;
     }
     if (!fused16) {
       rc = get_kv_map(k_cache, num_blocks, block_size, num_kv_heads, kv_block_stride,
-                      kv_layout, 0, &mk);
+                      kv_layout, sub, 0, &mk);
       if (rc != FK_OK) return rc;
       rc = get_kv_map(v_cache, num_blocks, block_size, num_kv_heads, kv_block_stride,
-                      kv_layout, 0, &mv);
+                      kv_layout, sub, 0, &mv);
       if (rc != FK_OK) return rc;
     }
   }
@@ -987,7 +1117,7 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
   p.block_tables = block_tables; p.bt_stride = block_table_stride;
   p.batch = batch; p.hq = num_q_heads; p.hkv = num_kv_heads; p.g = g;
   p.block_size = block_size; p.num_blocks = (int)num_blocks;
-  p.sub_tokens = block_size < ATT_BOX ? block_size : ATT_BOX;
+  p.sub_tokens = sub;
   p.fused16 = fused16;
   p.hnd = kv_layout;
   p.bs_shift = -1;
@@ -1014,7 +1144,7 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
 
   if (direct) {
     const int dgrid = batch * num_kv_heads;
-    FK_CUDA_OK(launch_decode(g > 8, split, dgrid, mk, mv, p, s));
+    FK_CUDA_OK(launch_decode(g > 8, split, false, dgrid, mk, mv, p, s));
     count_launch(1);
     return FK_OK;
   }
@@ -1028,7 +1158,7 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
     FK_CUDA_OK(cudaGetLastError());
     return FK_OK;
   }
-  FK_CUDA_OK(launch_decode(g > 8, split, grid, mk, mv, p, s));
+  FK_CUDA_OK(launch_decode(g > 8, split, false, grid, mk, mv, p, s));
   const int warps = batch * num_q_heads;
   FK_LAUNCH(attn_merge_kernel, dim3((warps * 32 + 255) / 256), dim3(256), 0, s, p);
   count_launch(2);

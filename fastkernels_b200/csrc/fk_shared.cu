@@ -4,111 +4,915 @@
 //   fk_shared_prefix_attn  attention of a batch whose sequences begin with the same pages in groups
 //
 // Both are one softmax per query head over a set of keys, out = sum_t e^(s q.k_t) v_t / sum_t
-// e^(s q.k_t).
-#include "fk_common.cuh"
+// e^(s q.k_t), cut into parts that are joined by their maxima and sums.  Selected blocks, and what the
+// rows of a group have for themselves, go through the decode attention kernel (fk_attn.cu).  What
+// the rows have in common goes through prefix_attn_kernel: with n rows of G query heads per KV head,
+// every key and value is used by n G query rows, which makes a matrix product of it.
+//
+// Four launches of fk_shared_prefix_attn: shared_plan_kernel (schedule of both parts, 1 CTA),
+// prefix_attn_kernel, attn_decode_kernel, shared_join_kernel.
+#include "fk_attn.cuh"
+#include "fk_tcgen05.cuh"
 #include "fk_types.cuh"
+
+#include <mutex>
+#include <unordered_map>
 
 namespace fk {
 
 constexpr int SH_D = 128;
 constexpr int SH_MAX_G = 16;
-constexpr int SH_THREADS = 256;
 
+// Checked arguments that both calls have.
 struct RowsParams {
   const uint16_t* q; int64_t q_stride;
   uint16_t* out; int64_t out_stride;
-  const uint16_t* k; const uint16_t* v; int64_t page_stride;
-  const int32_t* context_lens;
-  const int32_t* rows;
-  const int32_t* tables; int64_t table_stride;
-  int64_t capacity;
-  const int32_t* selected; int count;      // null: all blocks
-  int num_tables, num_pages, page, block, hkv, g, hnd;
+  int64_t capacity;                    // tokens that a table's row has pages for
+  int g;
   float scale_log2;
+};
+
+// ---------------------------------------------------------------------------
+// splits of a token and head joined: out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M)
+// ---------------------------------------------------------------------------
+// A lane has the (max, sum) of splits lane, lane + 32, ..., so all of them are one round of loads, and
+// four partial rows are on the way at a time.  A split without keys has a sum of zero; its row was not
+// written and is not read.
+struct JoinRow {
+  float4 acc;
+  float l;
+};
+__device__ __forceinline__ float join_max(const float2* ml, int n, int lane) {
+  float m = -INFINITY;
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, ml[s].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+__device__ __forceinline__ void join_add(JoinRow& r, const float* part_o, const float2* ml, int n,
+                                         float top, int lane) {
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    const float2 mlv = s0 + lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+    const float fl = mlv.y > 0.f ? fast_exp2(mlv.x - top) : 0.f;
+    const int cnt = min(32, n - s0);
+    const float4* src = reinterpret_cast<const float4*>(part_o + (int64_t)s0 * SH_D) + lane;
+    for (int s = 0; s < cnt; s += 4) {
+      float4 v[4];
+      float f[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = __shfl_sync(0xffffffffu, fl, s + i);
+        l[i] = __shfl_sync(0xffffffffu, mlv.y, s + i);
+        v[i] = s + i < cnt && l[i] > 0.f ? src[(s + i) * (SH_D / 4)]
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (s + i >= cnt) break;
+        r.l = fmaf(l[i], f[i], r.l);
+        r.acc = r.acc + v[i] * f[i];
+      }
+    }
+  }
+}
+
+// a warp per (token, query head)
+__global__ void __launch_bounds__(256) selected_join_kernel(const AttnParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t gw = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (gw >= (int64_t)p.batch * p.hq) return;
+  const int token = (int)(gw / p.hq), head = (int)(gw - (int64_t)token * p.hq);
+  int first, last;
+  selected_ctas((int64_t)token * p.hkv + head / p.g, p.tiles, p.unit, &first, &last);
+  const int n = last - first + 1;
+  if (n == 1) return;                        // written by the attention kernel
+  const float2* ml = p.part_ml + gw * p.max_splits;
+  const float top = join_max(ml, n, lane);
+  JoinRow r{make_float4(0.f, 0.f, 0.f, 0.f), 0.f};
+  join_add(r, p.part_o + gw * p.max_splits * SH_D, ml, n, top == -INFINITY ? 0.f : top, lane);
+  Elem<uint16_t>::store4(p.out + (int64_t)token * p.out_stride + (int64_t)head * SH_D + lane * 4,
+                         r.acc * (r.l > 0.f ? 1.0f / r.l : 0.f));
+}
+
+// How the tiles of all tokens and KV heads fall on CTAs.
+struct SelectedSchedule {
+  int tiles, splits, grid;
+  int64_t unit;
+};
+static SelectedSchedule selected_schedule(int64_t items, int count, int block) {
+  SelectedSchedule s;
+  const int sms = sm_count();
+  s.tiles = (int)(((int64_t)count * block + ATT_TILE - 1) / ATT_TILE);
+  const int64_t total = items * s.tiles;
+  s.unit = (total + sms - 1) / sms;
+  // many items: whole ones, at most an eighth more on some CTAs than on others
+  if (items >= 8ll * sms) s.unit = (items + sms - 1) / sms * s.tiles;
+  s.grid = (int)((total + s.unit - 1) / s.unit);
+  // an item's tiles lie in at most this many runs
+  const bool whole = s.unit % s.tiles == 0;
+  s.splits = whole ? 1 : (int)((s.tiles - 2 + s.unit) / s.unit) + 1;
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// schedule of a batch with common prefixes
+// ---------------------------------------------------------------------------
+// Up to two tiles of 128 query rows share the keys of an item.
+struct PrefixItem {
+  int row0, rows;      // batch rows
+  int table;           // the row whose table is read: the one with the longest context
+  int keys;            // whole pages, all of them below that row's context
+  int start;           // its first tile of 128 keys among those of all items and KV heads
+  int tiles;           // per KV head
+  int pad0, pad1;
+};
+
+enum : int { PLAN_CHUNKS = 0, PLAN_COUNTER = 2, PLAN_ITEMS = 4, PLAN_TILES = 5, PLAN_UNIT = 6,
+             PLAN_HDR = 8 };
+
+struct SharedPlan {
+  int* hdr;            // see above; chunk_start[batch + 1] behind it, as the decode kernel has it
+  int* row_item;       // [batch] item that holds a row, -1: none
+  int* row_from;       // [batch] tokens of a row that its item covers
+  PrefixItem* items;   // [batch]
+  int4* chunks;        // chunks of what each row has for itself
+};
+
+struct SharedPlanParams {
+  const int32_t* lens; const int32_t* starts; const int32_t* prefix;
+  int batch, groups, hkv, page, per_tile, max_splits, ctas, min_unit;
+  int64_t capacity;
+  SharedPlan plan;
   int32_t* status;
 };
 
-// One CTA per (token, KV head); its warps take blocks in turn, a lane has four channels, and every
-// warp keeps a running maximum and sum of its own, which are joined at the end.
-__global__ void __launch_bounds__(SH_THREADS) attn_rows_kernel(const RowsParams p) {
-  __shared__ float o_part[SH_D];
-  __shared__ float m_part[8], l_part[8];
+constexpr int PLAN_THREADS = 1024;
+
+__device__ __forceinline__ int plan_sum(int v, int* red) {     // over the block, for all
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  v = red[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// sum of the threads before this one
+__device__ __forceinline__ int plan_before(int v, int* red, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = upto;
+  __syncthreads();
+  int w = red[lane], wi = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, wi, o);
+    if (lane >= o) wi += u;
+  }
+  *total = __shfl_sync(0xffffffffu, wi, 31);
+  return __shfl_sync(0xffffffffu, wi - w, warp) + upto - v;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedPlanParams p) {
+  __shared__ int red[32];
+  __shared__ int s_keys[PLAN_THREADS], s_table[PLAN_THREADS], s_item[PLAN_THREADS],
+      s_start[PLAN_THREADS];
+  const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  const int token = blockIdx.x, kvh = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t len = p.context_lens[token];
-  const int row = p.rows ? p.rows[token] : token;
-  bool bad = len > p.capacity;
-  if (len < 0) len = 0;
-  if (len > p.capacity) len = p.capacity;
-  if (row < 0 || row >= p.num_tables) { len = 0; bad = true; }
-  if (bad && threadIdx.x == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-  const int n = (int)((len + p.block - 1) / p.block);
-  const int units = p.selected ? p.count : n;
-  const int32_t* sel = p.selected ? p.selected + ((int64_t)token * p.hkv + kvh) * p.count : nullptr;
-  const int32_t* table = p.tables + (int64_t)row * p.table_stride;
-  for (int h = 0; h < p.g; ++h) {
-    const int64_t at = (int64_t)(kvh * p.g + h) * SH_D;
-    const float4 q = Elem<uint16_t>::load4(p.q + (int64_t)token * p.q_stride + at + lane * 4);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = -INFINITY, l = 0.f;
-    for (int u = warp; u < units; u += SH_THREADS / 32) {
-      const int b = sel ? sel[u] : u;
-      if (b < 0 || b >= n) continue;
-      const int64_t pos = (int64_t)b * p.block;
-      const int page = table[pos / p.page];
-      if (page < 0 || page >= p.num_pages) {
-        if (lane == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-        continue;
+  auto len_of = [&](int i) -> int {
+    const int64_t len = p.lens[i];
+    return len < 0 ? 0 : (int)(len > p.capacity ? p.capacity : len);
+  };
+  bool cut = false;
+  for (int i = tid; i < p.batch; i += PLAN_THREADS) {
+    cut |= (int64_t)p.lens[i] > p.capacity;
+    p.plan.row_item[i] = -1;
+    p.plan.row_from[i] = 0;
+  }
+  if (cut && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+  __syncthreads();
+
+  // Groups into items, 1024 groups at a time: a warp looks for the longest row of a group, a thread
+  // per group adds up, a warp per group writes.  Starts that do not ascend within the batch: nobody
+  // has anything in common then.
+  bool odd = false;
+  for (int g = tid; g < p.groups; g += PLAN_THREADS)
+    odd |= p.starts[g] < 0 || p.starts[g + 1] < p.starts[g] || p.starts[g + 1] > p.batch;
+  odd = __syncthreads_or(odd);
+  if (odd && tid == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_POSITION);
+  const int groups = odd ? 0 : p.groups;
+  const int warp = tid >> 5, lane = tid & 31;
+  int items = 0, tiles = 0;                    // of the groups before
+  for (int g0 = 0; g0 < groups; g0 += PLAN_THREADS) {
+    const int here = min(PLAN_THREADS, groups - g0);
+    for (int i = warp; i < here; i += PLAN_THREADS / 32) {
+      const int a = p.starts[g0 + i], b = p.starts[g0 + i + 1];
+      int longest = 0, table = a;
+      for (int r = a + lane; r < b; r += 32) {
+        const int n = len_of(r);
+        if (n > longest) { longest = n; table = r; }
       }
-      const int off = (int)(pos % p.page);
-      const int keys = (int)(len - pos < p.block ? len - pos : p.block);
-      const int64_t step = p.hnd ? SH_D : (int64_t)p.hkv * SH_D;
-      const int64_t base = (int64_t)page * p.page_stride + lane * 4 +
-                           (p.hnd ? ((int64_t)kvh * p.page + off) * SH_D
-                                  : (int64_t)off * p.hkv * SH_D + (int64_t)kvh * SH_D);
-      for (int t = 0; t < keys; ++t) {
-        const float4 k = Elem<uint16_t>::load4(p.k + base + t * step);
-        const float s = warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * p.scale_log2;
-        const float4 v = Elem<uint16_t>::load4(p.v + base + t * step);
-        const float mn = fmaxf(m, s);
-        const float keep = m == -INFINITY ? 0.f : exp2f(m - mn);
-        const float e = mn == -INFINITY ? 0.f : exp2f(s - mn);
-        m = mn;
-        l = l * keep + e;
-        o = o * keep + v * e;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const int n = __shfl_xor_sync(0xffffffffu, longest, o);
+        const int r = __shfl_xor_sync(0xffffffffu, table, o);
+        if (n > longest || (n == longest && r < table)) { longest = n; table = r; }
+      }
+      if (lane == 0) {
+        s_keys[i] = b - a < 2 ? 0 : max(0, min(p.prefix[g0 + i], longest)) / p.page * p.page;
+        s_table[i] = table;
       }
     }
-    if (lane == 0) { m_part[warp] = m; l_part[warp] = l; }
-    if (threadIdx.x < SH_D) o_part[threadIdx.x] = 0.f;
     __syncthreads();
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, m_part[w]);
-    for (int w = 0; w < 8; ++w)
-      sum += m_part[w] == -INFINITY ? 0.f : l_part[w] * exp2f(m_part[w] - top);
-    const float f = m == -INFINITY ? 0.f : exp2f(m - top);
-    for (int w = 0; w < 8; ++w) {              // in order
-      if (w == warp) {
-        float4* d = reinterpret_cast<float4*>(o_part) + lane;
-        *d = *d + o * f;
+    const int span = 2 * p.per_tile;
+    const int keys = tid < here ? s_keys[tid] : 0;
+    const int mine = keys > 0 ? (p.starts[g0 + tid + 1] - p.starts[g0 + tid] + span - 1) / span : 0;
+    const int per_item = (keys + ATT_TILE - 1) / ATT_TILE;
+    int n_items, n_tiles;
+    s_item[tid] = items + plan_before(mine, red, &n_items);
+    s_start[tid] = tiles + plan_before(mine * per_item * p.hkv, red, &n_tiles);
+    items += n_items;
+    tiles += n_tiles;
+    __syncthreads();
+    for (int i = warp; i < here; i += PLAN_THREADS / 32) {
+      const int keys_i = s_keys[i];
+      if (keys_i == 0) continue;
+      // the rows of a group evenly over its items
+      const int a = p.starts[g0 + i], n = p.starts[g0 + i + 1] - a;
+      const int m = (n + span - 1) / span, each = (n + m - 1) / m;
+      const int tiles_i = (keys_i + ATT_TILE - 1) / ATT_TILE;
+      for (int j = lane; j < m; j += 32)
+        p.plan.items[s_item[i] + j] =
+            PrefixItem{a + j * each, min(each, n - j * each), s_table[i], keys_i,
+                       s_start[i] + j * tiles_i * p.hkv, tiles_i, 0, 0};
+      for (int r = lane; r < n; r += 32) {
+        p.plan.row_item[a + r] = s_item[i] + r / each;
+        p.plan.row_from[a + r] = keys_i;
       }
-      __syncthreads();
-    }
-    if (warp == 0) {
-      const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-      Elem<uint16_t>::store4(p.out + (int64_t)token * p.out_stride + at + lane * 4,
-                             reinterpret_cast<float4*>(o_part)[lane] * inv);
     }
     __syncthreads();
   }
+  __syncthreads();
+
+  // What each row has for itself, in chunks of one length: long ones, but enough of them for every
+  // CTA, and at most max_splits a row.
+  auto rest_of = [&](int i) -> int { return max(0, len_of(i) - p.plan.row_from[i]); };
+  int longest = 0;
+  for (int i = tid; i < p.batch; i += PLAN_THREADS) longest = max(longest, rest_of(i));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  if ((tid & 31) == 0) red[tid >> 5] = longest;
+  __syncthreads();
+  longest = red[tid & 31];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  int least = ATT_TILE;
+  while ((int64_t)least * p.max_splits < longest) least <<= 1;
+  int chunk = max(1024, least);
+  for (;;) {
+    int n = 0;
+    for (int i = tid; i < p.batch; i += PLAN_THREADS) n += (rest_of(i) + chunk - 1) / chunk;
+    if (plan_sum(n, red) * p.hkv >= 4 * p.ctas || (chunk >> 1) < least) break;
+    chunk >>= 1;
+  }
+  int* chunk_start = p.plan.hdr + PLAN_HDR;
+  int run = 0;
+  for (int i0 = 0; i0 < p.batch; i0 += PLAN_THREADS) {
+    const int i = i0 + tid;
+    const int from = i < p.batch ? p.plan.row_from[i] : 0;
+    const int len = i < p.batch ? len_of(i) : 0;
+    const int n = (max(0, len - from) + chunk - 1) / chunk;
+    int all;
+    const int at = run + plan_before(n, red, &all);
+    run += all;
+    if (i >= p.batch) continue;
+    chunk_start[i] = at;
+    // one chunk and nothing before it: the decode kernel writes the result itself
+    const int parts = n + (from > 0 ? 2 : 0);
+    for (int c = 0; c < n; ++c)
+      p.plan.chunks[at + c] = make_int4(i, c | parts << 16, from + c * chunk,
+                                        min(len, from + (c + 1) * chunk));
+  }
+  if (tid == 0) {
+    chunk_start[p.batch] = run;
+    p.plan.hdr[PLAN_CHUNKS] = run;
+    p.plan.hdr[PLAN_COUNTER] = 0;
+    p.plan.hdr[PLAN_ITEMS] = items;
+    p.plan.hdr[PLAN_TILES] = tiles;
+    p.plan.hdr[PLAN_UNIT] = max(p.min_unit, (tiles + p.ctas - 1) / p.ctas);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the common part
+// ---------------------------------------------------------------------------
+// One persistent CTA per SM takes a run of `unit` tiles of 128 keys from the items' tiles, one after
+// another; each item and KV head in it is a split.  Rows of an item are (batch row, query head of the
+// KV head): 128 / G batch rows make a tile of query rows, and an item has one or two.
+//
+//   warp 8        TMA: query tiles, then K_0 V_0 K_1 V_1 ... through a ring of five 32 KiB slots
+//   warp 9        tensor memory and products: S_t = Q_t K_j^T into columns [128 t, 128 t + 128),
+//                 O_t += P_t V_j into [256 + 128 t, ...), P_t read from the first 64 columns of S_t.
+//                 The two tiles take turns, so that the softmax of one runs beside the
+//                 products of the other.
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a thread per query row: maximum, exponentials, sum;
+//                 weights are rounded to bf16 for the product with the values (their sum is of
+//                 what was before), O is scaled when a maximum grew by more than 2^8.
+//
+// Bounds: the bytes of the common part up to some 250 query rows a KV head, the products and
+// exponentials beyond.  Waits end after two seconds, as in the other attention kernels.
+constexpr int PX_SLOTS = 5;
+constexpr int PX_HALF_BYTES = 128 * 128;
+constexpr int PX_TILE_BYTES = 2 * PX_HALF_BYTES;
+constexpr int PX_THREADS = 320;
+constexpr int PX_WARP_TMA = 8, PX_WARP_MMA = 9;
+constexpr int PX_OFF_Q = 0;
+constexpr int PX_OFF_KV = 2 * PX_TILE_BYTES;
+constexpr int PX_OFF_BAR = PX_OFF_KV + PX_SLOTS * PX_TILE_BYTES;
+constexpr int PX_SMEM_ALLOC = PX_OFF_BAR + 256 + 1024;
+constexpr int PX_TMEM_COLS = 512;
+constexpr float PX_RESCALE_LOG2 = 8.0f;
+static_assert(PX_SMEM_ALLOC <= 232448, "shared memory budget");
+static_assert(tmem_alone(PX_SMEM_ALLOC), "two CTAs could wait for one another's tensor memory");
+
+struct PrefixParams {
+  const int* hdr; const PrefixItem* items;
+  const int32_t* lens;
+  const int32_t* tables; int64_t table_stride;
+  int hq, hkv, g, per_tile;            // batch rows of a query tile
+  int hnd, block_size, sub_tokens, num_blocks;
+  float scale_log2;
+  int64_t capacity;
+  float* part_o; float2* part_ml;      // [batch, hq, splits]
+  int splits;
+  int32_t* status;
+};
+
+__device__ __forceinline__ uint64_t px_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool px_poll(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                        int32_t* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = px_ns();
+  for (;;) {
+    for (int i = 0; i < 128; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (px_ns() - t0 > 2000000000ull) {
+      *abort_flag = 1;
+      if (status) atomicOr(status, FK_DEV_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+}
+// By whole warps: one answer for all lanes.
+__device__ __forceinline__ bool px_wait_warp(uint64_t* bar, uint32_t parity,
+                                             volatile int* abort_flag, int32_t* status) {
+  return __all_sync(0xffffffffu, px_poll(bar, parity, abort_flag, status) ? 1 : 0) != 0;
+}
+
+// packed fp32 pairs and the three-input maximum
+__device__ __forceinline__ uint64_t px_pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void px_unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t px_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t px_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float px_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// One split: tiles t0 .. t1 - 1 of an item and KV head.
+struct PrefixSeg {
+  int row0, rows, table, keys, kvh, t0, t1, split, two;
+};
+// The split that holds tile `at` of all; ends at `end` or with its item and head.
+__device__ __forceinline__ PrefixSeg px_segment(const PrefixParams& p, int items, int unit, int at,
+                                                int end) {
+  int lo = 0, hi = items;                      // the last item that starts at or before `at`
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.items[mid].start <= at) lo = mid; else hi = mid;
+  }
+  const PrefixItem it = p.items[lo];
+  PrefixSeg s;
+  s.row0 = it.row0; s.rows = it.rows; s.table = it.table; s.keys = it.keys;
+  const int in = at - it.start;
+  s.kvh = in / it.tiles;
+  s.t0 = in - s.kvh * it.tiles;
+  s.t1 = min(it.tiles, s.t0 + end - at);
+  s.split = (int)blockIdx.x - (it.start + s.kvh * it.tiles) / unit;
+  s.two = it.rows > p.per_tile ? 1 : 0;
+  return s;
+}
+
+__global__ void __launch_bounds__(PX_THREADS, 1)
+prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
+                   const __grid_constant__ CUtensorMap tmap_k,
+                   const __grid_constant__ CUtensorMap tmap_v, const PrefixParams p) {
+  extern __shared__ uint8_t px_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(px_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + PX_OFF_BAR);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* slot_full = q_full + 2;
+  uint64_t* slot_empty = slot_full + PX_SLOTS;
+  uint64_t* s_full = slot_empty + PX_SLOTS;          // [2]
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* o_empty = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(o_empty + 3);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < PX_SLOTS; ++i) {
+      mbar_init(&slot_full[i], 1);
+      mbar_init(&slot_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+      mbar_init(&o_empty[t], 4);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == PX_WARP_TMA && lane == 0) {
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == PX_WARP_MMA) tmem_alloc(tmem_slot, PX_TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // all 512 columns: they start at column 0
+  const uint32_t tmem_got = *tmem_slot;
+  constexpr uint32_t tmem_base = 0;
+  pdl_wait();     // the schedule, q and the cache may come from earlier kernels
+  const int items = p.hdr[PLAN_ITEMS], unit = p.hdr[PLAN_UNIT], total = p.hdr[PLAN_TILES];
+  const int64_t from = (int64_t)blockIdx.x * unit;
+  const int begin = (int)(from < total ? from : total);
+  const int end = tmem_got != 0 ? begin : min(total - begin, unit) + begin;
+  if (tmem_got != 0 && threadIdx.x == 0 && p.status) atomicOr(p.status, FK_DEV_TMEM_BASE);
+
+  if (warp == PX_WARP_TMA) {
+    const int st = p.sub_tokens, npieces = 128 / st;
+    int kv_idx = 0, q_loads = 0;
+    bool ok = true;
+    for (int at = begin; ok && at < end;) {
+      const PrefixSeg sg = px_segment(p, items, unit, at, end);
+      at += sg.t1 - sg.t0;
+      int pass = 1;
+      if (lane == 0) {
+        if (q_loads > 0)
+          pass = px_poll(q_empty, (uint32_t)(q_loads - 1) & 1u, abort_flag, p.status) ? 1 : 0;
+        if (pass) {
+          mbar_arrive_expect_tx(q_full, (uint32_t)(1 + sg.two) * 2u * 128u *
+                                            (uint32_t)(p.g * p.per_tile));
+          for (int t = 0; t <= sg.two; ++t)
+            for (int dh = 0; dh < 2; ++dh)
+              tma_load_4d(smem + PX_OFF_Q + t * PX_TILE_BYTES + dh * PX_HALF_BYTES, &tmap_q, q_full,
+                          dh * 64, sg.kvh * p.g, sg.row0 + t * p.per_tile, 0);
+        }
+      }
+      pass = __shfl_sync(0xffffffffu, pass, 0);
+      if (!pass) { ok = false; break; }
+      ++q_loads;
+      const int32_t* bt = p.tables + (int64_t)sg.table * p.table_stride;
+      for (int i = 2 * sg.t0; i < 2 * sg.t1; ++i, ++kv_idx) {
+        const int slot = kv_idx % PX_SLOTS;
+        const uint32_t lap = (uint32_t)(kv_idx / PX_SLOTS) & 1u;
+        const int tok = (i >> 1) * 128 + lane * st;
+        int page = p.num_blocks;               // past the end: the copy reads the zero fill
+        if (lane < npieces && tok < sg.keys) {
+          page = bt[tok / p.block_size];
+          if (page < 0 || page >= p.num_blocks) {
+            page = p.num_blocks;
+            if (p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+          }
+        }
+        pass = 1;
+        if (lane == 0) pass = px_poll(&slot_empty[slot], lap ^ 1, abort_flag, p.status) ? 1 : 0;
+        pass = __shfl_sync(0xffffffffu, pass, 0);
+        if (!pass) { ok = false; break; }
+        if (lane == 0) mbar_arrive_expect_tx(&slot_full[slot], PX_TILE_BYTES);
+        __syncwarp();
+        if (lane < npieces) {
+          uint8_t* dst = smem + PX_OFF_KV + slot * PX_TILE_BYTES + lane * st * 128;
+          const CUtensorMap* map = i & 1 ? &tmap_v : &tmap_k;
+          const int off = tok % p.block_size;
+          const int c1 = p.hnd ? off : sg.kvh, c2 = p.hnd ? sg.kvh : off;
+          tma_load_4d(dst, map, &slot_full[slot], 0, c1, c2, page);
+          tma_load_4d(dst + PX_HALF_BYTES, map, &slot_full[slot], 64, c1, c2, page);
+        }
+      }
+    }
+  } else if (warp == PX_WARP_MMA) {
+    constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) |
+                                 ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t idesc_pv = idesc_s | (1u << 16);   // B (= V) is MN-major
+    const uint32_t q_addr = smem_u32(smem + PX_OFF_Q);
+    const uint32_t kv_addr = smem_u32(smem + PX_OFF_KV);
+    auto issue_s = [&](int t, int slot) {
+      const uint32_t a = q_addr + t * PX_TILE_BYTES;
+      const uint32_t b = kv_addr + slot * PX_TILE_BYTES;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < SH_D / 16; ++kk) {
+          const uint32_t o = (kk >> 2) * PX_HALF_BYTES + (kk & 3) * 32;
+          tc_mma_bf16(tmem_base + t * 128, smem_desc_sw128(a + o), smem_desc_sw128(b + o), idesc_s,
+                      kk > 0 ? 1u : 0u);
+        }
+      }
+      __syncwarp();
+    };
+    auto issue_pv = [&](int t, int slot, bool acc) {
+      const uint32_t a = tmem_base + t * 128;
+      const uint32_t b = kv_addr + slot * PX_TILE_BYTES;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          tc_mma_bf16_ts(tmem_base + 256 + t * SH_D, a + kk * 8,
+                         smem_desc_sw128_mn(b + kk * 2048, PX_HALF_BYTES, 1024), idesc_pv,
+                         (acc || kk > 0) ? 1u : 0u);
+      }
+      __syncwarp();
+    };
+    int kv_base = 0, segs = 0;
+    uint32_t n_sp[2] = {0, 0}, n_o[2] = {0, 0};   // hand-overs and splits per query tile so far
+    bool ok = true;
+    for (int at = begin; ok && at < end;) {
+      const PrefixSeg sg = px_segment(p, items, unit, at, end);
+      const int n = sg.t1 - sg.t0, qt = 1 + sg.two;
+      at += n;
+      ok = px_wait_warp(q_full, (uint32_t)segs & 1u, abort_flag, p.status) &&
+           px_wait_warp(&slot_full[kv_base % PX_SLOTS], (uint32_t)(kv_base / PX_SLOTS) & 1u,
+                        abort_flag, p.status);
+      if (!ok) break;
+      tc_fence_after();
+      for (int t = 0; t < qt; ++t) {
+        issue_s(t, kv_base % PX_SLOTS);
+        tc_commit_elect(&s_full[t]);
+      }
+      tc_commit_elect(&slot_empty[kv_base % PX_SLOTS]);
+      if (n == 1) tc_commit_elect(q_empty);
+      for (int j = 0; j < n && ok; ++j) {
+        const int vi = kv_base + 2 * j + 1, ki = vi + 1;
+        const int vslot = vi % PX_SLOTS, kslot = ki % PX_SLOTS;
+        ok = px_wait_warp(&slot_full[vslot], (uint32_t)(vi / PX_SLOTS) & 1u, abort_flag, p.status);
+        bool k_ready = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || t >= qt) break;
+          if (j == 0 && n_o[t] > 0) {
+            // O_t holds the split before until its rows have been read
+            ok = px_wait_warp(&o_empty[t], (n_o[t] - 1) & 1u, abort_flag, p.status);
+            if (!ok) break;
+          }
+          ok = px_wait_warp(&p_full[t], (n_sp[t] + (uint32_t)j) & 1u, abort_flag, p.status);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(t, vslot, j > 0);
+          if (j == n - 1) tc_commit_elect(&o_full[t]);
+          if (j + 1 < n) {
+            if (!k_ready) {
+              ok = px_wait_warp(&slot_full[kslot], (uint32_t)(ki / PX_SLOTS) & 1u, abort_flag,
+                                p.status);
+              if (!ok) break;
+              tc_fence_after();
+              k_ready = true;
+            }
+            issue_s(t, kslot);
+            tc_commit_elect(&s_full[t]);
+          }
+        }
+        if (!ok) break;
+        tc_commit_elect(&slot_empty[vslot]);
+        if (k_ready) tc_commit_elect(&slot_empty[kslot]);
+        if (j + 2 == n) tc_commit_elect(q_empty);   // the last S products have been issued
+      }
+      kv_base += 2 * n;
+      ++segs;
+      for (int t = 0; t < qt; ++t) {
+        n_sp[t] += (uint32_t)n;
+        ++n_o[t];
+      }
+    }
+  } else {
+    const int t = warp >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
+    const uint32_t s_addr = lane_addr + t * 128;
+    const uint32_t o_addr = lane_addr + 256 + t * SH_D;
+    const float sc = p.scale_log2;
+    const uint64_t sc2 = px_pack2(sc, sc);
+    const int in_tile = row / p.g, head_in = row - in_tile * p.g;
+    uint32_t n_sp = 0, n_o = 0;
+    bool ok = true;
+    for (int at = begin; ok && at < end;) {
+      int n, lim, kpos;
+      int64_t part;                            // of this row's results, -1: no row
+      {
+        const PrefixSeg sg = px_segment(p, items, unit, at, end);
+        n = sg.t1 - sg.t0;
+        at += n;
+        if (t > sg.two) continue;
+        const int i = t * p.per_tile + in_tile;
+        lim = 0;
+        part = -1;
+        if (in_tile < p.per_tile && i < sg.rows) {
+          const int64_t len = p.lens[sg.row0 + i];
+          lim = (int)(len < 0 ? 0 : len < sg.keys ? len : sg.keys);
+          part = ((int64_t)(sg.row0 + i) * p.hq + sg.kvh * p.g + head_in) * p.splits + sg.split;
+        }
+        kpos = sg.t0 * 128;
+      }
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, kpos += 128) {
+        if (!px_wait_warp(&s_full[t], (n_sp + (uint32_t)j) & 1u, abort_flag, p.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        // The row is read twice, half by half: registers for all of it at once would spill.
+        auto half_row = [&](int half, uint32_t (&v)[64]) {
+          tc_ld32(s_addr + half * 64, v);
+          tc_ld32(s_addr + half * 64 + 32, v + 32);
+          tc_wait_ld();
+          const int first = kpos + half * 64;
+          if (first + 64 > lim) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (first + c >= lim) v[c] = 0xff800000u;   // -inf
+          }
+        };
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[64];
+          half_row(half, v);
+#pragma unroll
+          for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mx4[i] = px_max3(mx4[i], __uint_as_float(v[c + i]), __uint_as_float(v[c + 4 + i]));
+          }
+          __syncwarp();
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+        if (j == 0) {
+          m_used = mx;
+        } else {
+          const bool grow = mx > m_used + PX_RESCALE_LOG2;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float alpha = grow ? fast_exp2(m_used - mx) : 1.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tc_ld32(o_addr + c * 32, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tc_st32(o_addr + c * 32, o);
+            }
+            tc_wait_st();
+            if (grow) {
+              l *= alpha;
+              m_used = mx;
+            }
+          }
+        }
+        const float neg_mu = m_used == -INFINITY ? 0.f : -m_used;
+        const uint64_t nm2 = px_pack2(neg_mu, neg_mu);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[64];
+          half_row(half, v);
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float t0, t1, t2, t3;
+            px_unpack2(px_fma2(px_pack2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
+                               sc2, nm2), t0, t1);
+            px_unpack2(px_fma2(px_pack2(__uint_as_float(v[2 * c + 2]),
+                                        __uint_as_float(v[2 * c + 3])), sc2, nm2), t2, t3);
+            const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
+            const float e2 = fast_exp2(t2), e3 = fast_exp2(t3);
+            sum2[0] = px_add2(sum2[0], px_pack2(e0, e1));
+            sum2[1] = px_add2(sum2[1], px_pack2(e2, e3));
+            v[c] = pack_bf16(e0, e1);
+            v[c + 1] = pack_bf16(e2, e3);
+          }
+          // over columns of S that have been read
+          __syncwarp();
+          tc_st32(s_addr + half * 32, v);
+        }
+        {
+          float a0, a1, a2, a3;
+          px_unpack2(sum2[0], a0, a1);
+          px_unpack2(sum2[1], a2, a3);
+          l += (a0 + a1) + (a2 + a3);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      if (!px_wait_warp(&o_full[t], n_o & 1u, abort_flag, p.status)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (m_used == -INFINITY) l = 0.f;        // no key: the sum says that there is no row
+      float4* dst = reinterpret_cast<float4*>(p.part_o + part * SH_D);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        tc_ld32(o_addr + c * 32, o);
+        tc_wait_ld();
+        if (c == 3) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[t]);
+        }
+        if (part >= 0 && l > 0.f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            dst[c * 8 + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                         __uint_as_float(o[4 * i + 2]),
+                                         __uint_as_float(o[4 * i + 3]));
+        }
+        __syncwarp();
+      }
+      if (part >= 0) p.part_ml[part] = make_float2(m_used, l);
+      n_sp += (uint32_t)n;
+      ++n_o;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == PX_WARP_MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem_got, PX_TMEM_COLS);
+  }
+}
+
+// a warp per (row, query head): the splits of its common part, then its own
+struct SharedJoinParams {
+  const int* hdr; const int* row_item; const PrefixItem* items;
+  int* counter;
+  uint16_t* out; int64_t out_stride;
+  const float* pre_o; const float2* pre_ml; int pre_splits;
+  const float* own_o; const float2* own_ml; int own_splits;
+  int batch, hq, g;
+};
+__global__ void __launch_bounds__(256) shared_join_kernel(const SharedJoinParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  // the decode kernel has ended: its work counter is ready for the next layer
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0;
+  const int64_t gw = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (gw >= (int64_t)p.batch * p.hq) return;
+  const int row = (int)(gw / p.hq), head = (int)(gw - (int64_t)row * p.hq);
+  const int* chunk_start = p.hdr + PLAN_HDR;
+  const int n_own = chunk_start[row + 1] - chunk_start[row];
+  const int item = p.row_item[row];
+  int n_pre = 0;
+  if (item >= 0) {
+    const int tiles = p.items[item].tiles, unit = p.hdr[PLAN_UNIT];
+    const int first = p.items[item].start + head / p.g * tiles;
+    n_pre = (first + tiles - 1) / unit - first / unit + 1;
+  }
+  if (n_pre == 0 && n_own == 1) return;        // written by the decode kernel
+  const float2* pre_ml = p.pre_ml + gw * p.pre_splits;
+  const float2* own_ml = p.own_ml + gw * p.own_splits;
+  float top = fmaxf(join_max(pre_ml, n_pre, lane), join_max(own_ml, n_own, lane));
+  if (top == -INFINITY) top = 0.f;
+  JoinRow r{make_float4(0.f, 0.f, 0.f, 0.f), 0.f};
+  join_add(r, p.pre_o + gw * p.pre_splits * SH_D, pre_ml, n_pre, top, lane);
+  join_add(r, p.own_o + gw * p.own_splits * SH_D, own_ml, n_own, top, lane);
+  Elem<uint16_t>::store4(p.out + (int64_t)row * p.out_stride + (int64_t)head * SH_D + lane * 4,
+                         r.acc * (r.l > 0.f ? 1.0f / r.l : 0.f));
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+// Tensor map of q for query tiles: (64 channels, g heads, per_tile batch rows) a copy.
+struct QMapKey {
+  const void* q; int64_t stride; int batch, hq, g, per_tile;
+  bool operator==(const QMapKey& o) const {
+    return q == o.q && stride == o.stride && batch == o.batch && hq == o.hq && g == o.g &&
+           per_tile == o.per_tile;
+  }
+};
+struct QMapHash {
+  size_t operator()(const QMapKey& k) const {
+    return std::hash<const void*>()(k.q) ^
+           std::hash<int64_t>()(k.stride * 31 + k.batch * 1000003ll + k.hq * 97ll + k.g);
+  }
+};
+static int get_q_map(const QMapKey& key, CUtensorMap* out) {
+  static std::mutex mu;
+  static std::unordered_map<QMapKey, CUtensorMap, QMapHash> maps;
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = maps.find(key);
+  if (it != maps.end()) {
+    *out = it->second;
+    return FK_OK;
+  }
+  tensormap_encode_fn enc = get_tensormap_encode();
+  FK_REQUIRE(enc != nullptr, FK_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+  const cuuint64_t dims[4] = {SH_D, (cuuint64_t)key.hq, (cuuint64_t)key.batch, 1};
+  const cuuint64_t strides[3] = {SH_D * 2, (cuuint64_t)key.stride * 2,
+                                 (cuuint64_t)key.stride * 2 * (cuuint64_t)key.batch};
+  const cuuint32_t box[4] = {64, (cuuint32_t)key.g, (cuuint32_t)key.per_tile, 1};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(key.q), dims,
+                         strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FK_REQUIRE(r == CUDA_SUCCESS, FK_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  if (maps.size() > 4096) maps.clear();
+  maps.emplace(key, *out);
+  return FK_OK;
+}
+
+// fewest 128-key tiles of the common part that a CTA takes
+constexpr int PREFIX_MIN_UNIT = 2;
+
+struct SharedLayout {
+  size_t row_item, row_from, items, chunks, pre_o, pre_ml, own_o, own_ml, total;
+  int pre_splits;
+};
+static SharedLayout shared_layout(int64_t batch, int hq, int hkv, int max_splits) {
+  SharedLayout s;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at = (at + bytes + 255) & ~size_t(255);
+    return here;
+  };
+  take((PLAN_HDR + batch + 1) * sizeof(int));
+  s.row_item = take(batch * sizeof(int));
+  s.row_from = take(batch * sizeof(int));
+  s.items = take(batch * sizeof(PrefixItem));
+  s.chunks = take((size_t)batch * max_splits * sizeof(int4));
+  // A CTA takes at least 1 / ctas of all tiles, those of all KV heads of an item among them, so that
+  // an item and head falls on at most ctas / hkv CTAs and one more on either side.
+  s.pre_splits = sm_count() / hkv + 2;
+  const size_t rows = (size_t)batch * hq;
+  s.pre_o = take(rows * s.pre_splits * SH_D * sizeof(float));
+  s.pre_ml = take(rows * s.pre_splits * sizeof(float2));
+  s.own_o = take(rows * max_splits * SH_D * sizeof(float));
+  s.own_ml = take(rows * max_splits * sizeof(float2));
+  s.total = at;
+  return s;
 }
 
 static int rows_args(const char* what, RowsParams& p, const void* q, int64_t q_stride, void* out,
                      int64_t out_stride, const void* k, const void* v, int64_t num_pages, int page,
                      int64_t page_stride, int layout, const int32_t* lens, const int32_t* tables,
-                     int64_t table_stride, int64_t table_cols, int hq, int hkv, int d, int block,
-                     float scale, int32_t* status) {
+                     int64_t table_stride, int64_t table_cols, int hq, int hkv, int d,
+                     float scale) {
   FK_REQUIRE(q && out && k && v && lens && tables, FK_ERR_INVALID_ARG, "%s: null pointer", what);
   FK_REQUIRE(d == SH_D, FK_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (128 only)", what, d);
   FK_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, FK_ERR_INVALID_ARG,
@@ -129,14 +933,9 @@ static int rows_args(const char* what, RowsParams& p, const void* q, int64_t q_s
              FK_ERR_ALIGNMENT, "%s: 16-byte alignment required", what);
   p.q = static_cast<const uint16_t*>(q); p.q_stride = q_stride;
   p.out = static_cast<uint16_t*>(out); p.out_stride = out_stride;
-  p.k = static_cast<const uint16_t*>(k); p.v = static_cast<const uint16_t*>(v);
-  p.page_stride = page_stride;
-  p.context_lens = lens;
-  p.tables = tables; p.table_stride = table_stride; p.capacity = table_cols * page;
-  p.num_pages = (int)num_pages; p.page = page; p.block = block; p.hkv = hkv; p.g = hq / hkv;
-  p.hnd = layout;
+  p.capacity = table_cols * page;
+  p.g = hq / hkv;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.status = status;
   return FK_OK;
 }
 
@@ -148,10 +947,12 @@ extern "C" {
 
 size_t fk_selected_attn_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads,
                                         int head_dim, int count, int block) {
-  return num_tokens > 0 && num_q_heads > 0 && num_kv_heads > 0 && head_dim > 0 && count > 0 &&
-                 block > 0
-             ? 256
-             : 0;
+  if (num_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || count <= 0 ||
+      block <= 0)
+    return 0;
+  const SelectedSchedule s = selected_schedule((int64_t)num_tokens * num_kv_heads, count, block);
+  if (s.splits == 1) return 0;
+  return (size_t)num_tokens * num_q_heads * s.splits * (head_dim * sizeof(float) + sizeof(float2));
 }
 
 int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t out_stride_token,
@@ -169,7 +970,7 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
   const int rc = rows_args("fk_selected_attn", p, q, q_stride_token, out, out_stride_token, k_cache,
                            v_cache, num_pages, page_size, kv_page_stride, kv_layout, context_lens,
                            block_tables, block_table_stride, block_table_cols, num_q_heads,
-                           num_kv_heads, head_dim, block, softmax_scale, status);
+                           num_kv_heads, head_dim, softmax_scale);
   if (rc != FK_OK) return rc;
   FK_REQUIRE(selected != nullptr && count > 0, FK_ERR_INVALID_ARG,
              "fk_selected_attn: no selected blocks");
@@ -180,27 +981,62 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
              page_size, block);
   FK_REQUIRE(table_rows != nullptr || num_tables >= num_tokens, FK_ERR_INVALID_ARG,
              "fk_selected_attn: %d tables for %d tokens", num_tables, num_tokens);
+  FK_REQUIRE((int64_t)count * block <= (1 << 30), FK_ERR_UNSUPPORTED,
+             "fk_selected_attn: %d blocks of %d tokens", count, block);
   const size_t need = fk_selected_attn_workspace_bytes(num_tokens, num_q_heads, num_kv_heads,
                                                        head_dim, count, block);
-  FK_REQUIRE(workspace != nullptr && workspace_bytes >= need &&
-                 (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
+  FK_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need &&
+                           (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0),
              FK_ERR_WORKSPACE,
              "fk_selected_attn: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
              workspace_bytes);
-  p.rows = table_rows; p.num_tables = num_tables;
-  p.selected = selected; p.count = count;
-  FK_CUDA_OK(launch_kernel(attn_rows_kernel, dim3((unsigned)num_tokens, (unsigned)num_kv_heads),
-                           dim3(SH_THREADS), (size_t)0, static_cast<cudaStream_t>(stream), p));
+  const SelectedSchedule s = selected_schedule((int64_t)num_tokens * num_kv_heads, count, block);
+  AttnParams a{};
+  a.q = p.q; a.q_stride = p.q_stride;
+  a.out = p.out; a.out_stride = p.out_stride;
+  a.context_lens = context_lens;
+  a.block_tables = block_tables; a.bt_stride = block_table_stride;
+  a.batch = num_tokens; a.hq = num_q_heads; a.hkv = num_kv_heads; a.g = p.g;
+  a.block_size = page_size; a.num_blocks = (int)num_pages;
+  a.sub_tokens = block < ATT_BOX ? block : ATT_BOX;
+  a.fused16 = block == 16;
+  a.bs_shift = -1;
+  a.hnd = kv_layout;
+  a.scale_log2 = p.scale_log2;
+  a.max_splits = s.splits;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)num_tokens * num_q_heads * s.splits *
+                                                       head_dim);
+  a.status = status;
+  a.selected = selected; a.rows = table_rows;
+  a.count = count; a.sel_block = block; a.num_tables = num_tables;
+  a.capacity = p.capacity;
+  a.tiles = s.tiles; a.unit = s.unit;
+  CUtensorMap mk, mv;
+  int rc2 = get_kv_map(k_cache, num_pages, page_size, num_kv_heads, kv_page_stride, kv_layout,
+                       a.sub_tokens, a.fused16, &mk);
+  if (rc2 == FK_OK)
+    rc2 = get_kv_map(v_cache, num_pages, page_size, num_kv_heads, kv_page_stride, kv_layout,
+                     a.sub_tokens, a.fused16, &mv);
+  if (rc2 != FK_OK) return rc2;
+  FK_CUDA_OK(launch_decode(p.g > 8, false, true, s.grid, mk, mv, a,
+                           static_cast<cudaStream_t>(stream)));
   count_launch(1);
+  if (s.splits > 1) {
+    const int64_t warps = (int64_t)num_tokens * num_q_heads;
+    FK_CUDA_OK(launch_kernel(selected_join_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256),
+                             (size_t)0, static_cast<cudaStream_t>(stream), a));
+    count_launch(1);
+  }
   return FK_OK;
 }
 
 size_t fk_shared_prefix_workspace_bytes(int batch, int num_groups, int num_q_heads,
                                         int num_kv_heads, int head_dim, int max_splits) {
-  return batch > 0 && num_groups >= 0 && num_q_heads > 0 && num_kv_heads > 0 && head_dim > 0 &&
-                 max_splits > 0
-             ? 256
-             : 0;
+  if (batch <= 0 || num_groups < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      max_splits <= 0)
+    return 0;
+  return shared_layout(batch, num_q_heads, num_kv_heads, max_splits).total;
 }
 
 int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
@@ -215,26 +1051,119 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   FK_REQUIRE(batch >= 0 && num_groups >= 0, FK_ERR_INVALID_ARG,
              "fk_shared_prefix_attn: negative size");
   if (batch == 0) return FK_OK;
-  RowsParams p{};
-  const int rc = rows_args("fk_shared_prefix_attn", p, q, q_stride_token, out, out_stride_token,
-                           k_cache, v_cache, num_pages, page_size, kv_page_stride, kv_layout,
-                           context_lens, block_tables, block_table_stride, block_table_cols,
-                           num_q_heads, num_kv_heads, head_dim, page_size, softmax_scale, status);
+  RowsParams r{};
+  int rc = rows_args("fk_shared_prefix_attn", r, q, q_stride_token, out, out_stride_token, k_cache,
+                     v_cache, num_pages, page_size, kv_page_stride, kv_layout, context_lens,
+                     block_tables, block_table_stride, block_table_cols, num_q_heads, num_kv_heads,
+                     head_dim, softmax_scale);
   if (rc != FK_OK) return rc;
   FK_REQUIRE(num_groups == 0 || (group_starts && prefix_lens), FK_ERR_INVALID_ARG,
              "fk_shared_prefix_attn: null pointer");
-  FK_REQUIRE(max_splits > 0, FK_ERR_INVALID_ARG, "fk_shared_prefix_attn: max_splits < 1");
-  const size_t need = fk_shared_prefix_workspace_bytes(batch, num_groups, num_q_heads,
-                                                       num_kv_heads, head_dim, max_splits);
-  FK_REQUIRE(workspace != nullptr && workspace_bytes >= need &&
+  FK_REQUIRE(max_splits > 0 && max_splits < (1 << 14), FK_ERR_INVALID_ARG,
+             "fk_shared_prefix_attn: %d splits", max_splits);
+  FK_REQUIRE(softmax_scale > 0.f, FK_ERR_INVALID_ARG,
+             "fk_shared_prefix_attn: softmax_scale must be above zero");
+  FK_REQUIRE((int64_t)batch * num_kv_heads * ((r.capacity + ATT_TILE - 1) / ATT_TILE) <
+                 (1ll << 31) - (1 << 20),
+             FK_ERR_UNSUPPORTED, "fk_shared_prefix_attn: batch and tables too large");
+  const SharedLayout w = shared_layout(batch, num_q_heads, num_kv_heads, max_splits);
+  FK_REQUIRE(workspace != nullptr && workspace_bytes >= w.total &&
                  (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
              FK_ERR_WORKSPACE,
-             "fk_shared_prefix_attn: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
-             workspace_bytes);
-  p.num_tables = batch;
-  FK_CUDA_OK(launch_kernel(attn_rows_kernel, dim3((unsigned)batch, (unsigned)num_kv_heads),
-                           dim3(SH_THREADS), (size_t)0, static_cast<cudaStream_t>(stream), p));
+             "fk_shared_prefix_attn: workspace needs %zu bytes, 256-byte aligned (got %zu)",
+             w.total, workspace_bytes);
+  const int g = r.g, sms = sm_count(), per_tile = 128 / g;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+  SharedPlanParams pl{};
+  pl.lens = context_lens; pl.starts = group_starts; pl.prefix = prefix_lens;
+  pl.batch = batch; pl.groups = num_groups; pl.hkv = num_kv_heads; pl.page = page_size;
+  pl.per_tile = per_tile; pl.max_splits = max_splits; pl.ctas = sms;
+  pl.min_unit = PREFIX_MIN_UNIT;
+  pl.capacity = r.capacity;
+  pl.plan.hdr = reinterpret_cast<int*>(ws);
+  pl.plan.row_item = reinterpret_cast<int*>(ws + w.row_item);
+  pl.plan.row_from = reinterpret_cast<int*>(ws + w.row_from);
+  pl.plan.items = reinterpret_cast<PrefixItem*>(ws + w.items);
+  pl.plan.chunks = reinterpret_cast<int4*>(ws + w.chunks);
+  pl.status = status;
+
+  const int sub = page_size < ATT_BOX ? page_size : ATT_BOX;
+  const int fused16 = page_size == 16;
+  CUtensorMap mq, mk, mv, dk, dv;
+  rc = get_q_map(QMapKey{q, q_stride_token, batch, num_q_heads, g, per_tile}, &mq);
+  if (rc == FK_OK)
+    rc = get_kv_map(k_cache, num_pages, page_size, num_kv_heads, kv_page_stride, kv_layout, sub, 0,
+                    &mk);
+  if (rc == FK_OK)
+    rc = get_kv_map(v_cache, num_pages, page_size, num_kv_heads, kv_page_stride, kv_layout, sub, 0,
+                    &mv);
+  dk = mk; dv = mv;
+  if (rc == FK_OK && fused16) {
+    rc = get_kv_map(k_cache, num_pages, page_size, num_kv_heads, kv_page_stride, kv_layout, sub, 1,
+                    &dk);
+    if (rc == FK_OK)
+      rc = get_kv_map(v_cache, num_pages, page_size, num_kv_heads, kv_page_stride, kv_layout, sub,
+                      1, &dv);
+  }
+  if (rc != FK_OK) return rc;
+
+  PrefixParams px{};
+  px.hdr = pl.plan.hdr; px.items = pl.plan.items;
+  px.lens = context_lens;
+  px.tables = block_tables; px.table_stride = block_table_stride;
+  px.hq = num_q_heads; px.hkv = num_kv_heads; px.g = g; px.per_tile = per_tile;
+  px.hnd = kv_layout; px.block_size = page_size; px.sub_tokens = sub;
+  px.num_blocks = (int)num_pages;
+  px.scale_log2 = r.scale_log2;
+  px.capacity = r.capacity;
+  px.part_o = reinterpret_cast<float*>(ws + w.pre_o);
+  px.part_ml = reinterpret_cast<float2*>(ws + w.pre_ml);
+  px.splits = w.pre_splits;
+  px.status = status;
+
+  AttnParams a{};
+  a.q = r.q; a.q_stride = r.q_stride;
+  a.out = r.out; a.out_stride = r.out_stride;
+  a.context_lens = context_lens;
+  a.block_tables = block_tables; a.bt_stride = block_table_stride;
+  a.batch = batch; a.hq = num_q_heads; a.hkv = num_kv_heads; a.g = g;
+  a.block_size = page_size; a.num_blocks = (int)num_pages;
+  a.sub_tokens = sub;
+  a.fused16 = fused16;
+  a.hnd = kv_layout;
+  a.bs_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
+  a.scale_log2 = r.scale_log2;
+  a.max_splits = max_splits;
+  a.plan = pl.plan.hdr;
+  a.chunk_info = pl.plan.chunks;
+  a.part_o = reinterpret_cast<float*>(ws + w.own_o);
+  a.part_ml = reinterpret_cast<float2*>(ws + w.own_ml);
+  a.status = status;
+
+  SharedJoinParams jn{};
+  jn.hdr = pl.plan.hdr; jn.row_item = pl.plan.row_item; jn.items = pl.plan.items;
+  jn.counter = pl.plan.hdr + PLAN_COUNTER;
+  jn.out = r.out; jn.out_stride = r.out_stride;
+  jn.pre_o = px.part_o; jn.pre_ml = px.part_ml; jn.pre_splits = w.pre_splits;
+  jn.own_o = a.part_o; jn.own_ml = a.part_ml; jn.own_splits = max_splits;
+  jn.batch = batch; jn.hq = num_q_heads; jn.g = g;
+
+  FK_CUDA_OK(launch_kernel(shared_plan_kernel, dim3(1), dim3(PLAN_THREADS), (size_t)0, s, pl));
   count_launch(1);
+  if (num_groups > 0) {
+    static PerDeviceOnce once;
+    FK_CUDA_OK(set_max_dynamic_smem(once, prefix_attn_kernel, PX_SMEM_ALLOC));
+    FK_CUDA_OK(launch_kernel(prefix_attn_kernel, dim3((unsigned)sms), dim3(PX_THREADS),
+                             (size_t)PX_SMEM_ALLOC, s, mq, mk, mv, px));
+    count_launch(1);
+  }
+  FK_CUDA_OK(launch_decode(g > 8, false, false, sms, dk, dv, a, s));
+  const int64_t warps = (int64_t)batch * num_q_heads;
+  FK_CUDA_OK(launch_kernel(shared_join_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256),
+                           (size_t)0, s, jn));
+  count_launch(2);
   return FK_OK;
 }
 

@@ -161,6 +161,19 @@ def test_bad_pages_are_flagged_and_left_out(ops):
     assert np.isfinite(got).all() and (got[3] == good[3]).all()
 
 
+def test_groups_that_do_not_fit_the_batch(ops):
+    """Starts past the batch or below the one before are flagged; nobody has anything in common
+    then, and all rows have their results."""
+    case = build(7, [(128, [5, 9, 70]), (64, [3, 4])], 64, "NHD", 4, 2)
+    q, kc, vc, lens, table, _, prefix = case
+    good = host_f32(run(ops, case, "NHD"))
+    for starts in ([0, 3, 99], [-4, 3, 5], [0, 3, 1]):
+        st = ops.new_status("cuda")
+        got = host_f32(run(ops, (q, kc, vc, lens, table, starts, prefix), "NHD", st))
+        assert int(st.item()) == 8
+        assert np.abs(got - good).max() <= 2.0 ** -6
+
+
 def test_in_a_graph_with_other_lengths(ops):
     """Captured once; replayed with other lengths, groups and queries in the same buffers."""
     rng = np.random.default_rng(9)

@@ -125,6 +125,10 @@ def test_attend_refusals():
 def test_shared_refusals():
     assert shared(groups=-1) == INVALID and shared(starts=None) == INVALID
     assert shared(prefix=None) == INVALID and shared(splits=0) == INVALID
+    for scale in (0.0, -0.1, float("nan")):
+        assert shared(scale=scale) == INVALID and "scale" in err()
+    assert shared(splits=1 << 14) == INVALID
+    assert shared(n=1 << 20, cols=1 << 20) == UNSUPPORTED
     assert shared(page=48, kv_stride=48 * 2 * 128) == UNSUPPORTED and "block_size" in err()
     need = L.fk_shared_prefix_workspace_bytes(3, 1, 8, 2, 128, 4)
     assert need > 0
