@@ -125,156 +125,425 @@ struct SelectParams {
   const int32_t* rows;                // table row of each token, null: its own number
   const int32_t* tables; int64_t table_stride;
   int64_t capacity;
-  int num_tables, num_pages, page, block, hkv, g;
+  int num_tokens, num_tables, num_pages, page, block, hkv, g;
   int count, keep_first, keep_last;
+  int together;                       // tokens of a CTA: 1, or up to 16 / g (a power of two)
+  int most;                           // blocks that a table's row has pages for
   int32_t* selected;                  // [tokens, hkv, count]
   int32_t* status;
 };
 
-// Doubles in an order of whole numbers: equal values (both zeros) alike, no-number above all.
+// Numbers in an order of whole numbers: equal values (both zeros) alike, no-number above all.  Zero
+// is below all of them.
 __device__ __forceinline__ uint64_t order_of(double v) {
   if (v != v) return ~0ull;
   const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
   return b >> 63 ? ~b : b | (1ull << 63);
 }
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b >> 31 ? ~b : b | (1u << 31);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
 
-// One CTA per (token, KV head).  Scores are sums in 64 bits: products of two bf16 are exact in
-// fp32, and 128 of them all but always in a 64-bit sum, so that the choice between two blocks does
-// not hang on the order of additions.
-__global__ void __launch_bounds__(SEL_THREADS) select_blocks_kernel(const SelectParams p) {
-  extern __shared__ uint64_t keys[];         // of the blocks between the kept ends
-  __shared__ float qs[SEL_MAX_G][SEL_D];
-  __shared__ int hist[256];
-  __shared__ int s_digit, s_left, s_eq[8], s_gt[8];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int token = blockIdx.x, kvh = blockIdx.y;
+struct SelectShared {
+  int hist[256];
+  int digit, left;
+  int eq[8], gt[8];
+  float q_sum[16];                    // of each token: largest sum of |q| of its query heads
+  uint32_t most[8];                   // largest |bound|, as bf16 bits
+  uint32_t lo[8], hi[8];
+};
+
+// The want-th largest of n keys (want >= 1), and in s.left how many of the keys equal to it are
+// among the want largest.  All threads; ends behind a barrier.
+template <typename KEY>
+__device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int top_shift,
+                                         KEY fixed, SelectShared& s) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int32_t* out = p.selected + ((int64_t)token * p.hkv + kvh) * p.count;
-  int64_t len = p.context_lens[token];
-  const int row = p.rows ? p.rows[token] : token;
-  bool bad = len > p.capacity;
-  if (len < 0) len = 0;
-  if (len > p.capacity) len = p.capacity;
-  if (row < 0 || row >= p.num_tables) { len = 0; bad = true; }
-  if (bad && tid == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-  const int n = (int)((len + p.block - 1) / p.block);
-  if (n <= p.count) {
-    for (int i = tid; i < p.count; i += SEL_THREADS) out[i] = i < n ? i : -1;
-    return;
-  }
-  const int32_t* table = p.tables + (int64_t)row * p.table_stride;
-  const int middle = n - p.keep_first - p.keep_last;
-  const int want = p.count - p.keep_first - p.keep_last;     // of the middle ones
-  const int per = p.page / p.block;
-  for (int i = tid; i < p.g * SEL_D; i += SEL_THREADS)
-    qs[i / SEL_D][i % SEL_D] =
-        bf16_bits_to_float(p.q[(int64_t)token * p.q_stride + (int64_t)kvh * p.g * SEL_D + i]);
-  __syncthreads();
-  for (int i = warp; i < middle; i += SEL_THREADS / 32) {
-    const int b = p.keep_first + i;
-    int page = table[b / per];
-    if (page < 0 || page >= p.num_pages) {
-      if (lane == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-      if (lane == 0) keys[i] = 0ull;          // the last to be taken
-      continue;
-    }
-    const uint16_t* at = p.bounds +
-                         (((int64_t)page * p.hkv + kvh) * per + b % per) * 2 * SEL_D + lane * 4;
-    const uint2 lo = *reinterpret_cast<const uint2*>(at);
-    const uint2 hi = *reinterpret_cast<const uint2*>(at + SEL_D);
-    const double l[4] = {bf16lo(lo.x), bf16hi(lo.x), bf16lo(lo.y), bf16hi(lo.y)};
-    const double u[4] = {bf16lo(hi.x), bf16hi(hi.x), bf16lo(hi.y), bf16hi(hi.y)};
-    double best = -INFINITY;
-    bool nan = false;
-    for (int h = 0; h < p.g; ++h) {
-      double sum = 0.0;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const double q = qs[h][lane * 4 + d];
-        const double a = q * l[d], c = q * u[d];
-        sum += a != a || c != c ? a + c : fmax(a, c);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      nan |= sum != sum;
-      best = fmax(best, sum);
-    }
-    if (lane == 0) keys[i] = nan ? ~0ull : order_of(best);
-  }
-  if (tid == 0) s_left = want;
-  uint64_t border = 0;                       // digits of the want-th largest key found so far
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    hist[tid] = 0;
+  constexpr int kBits = 8 * sizeof(KEY);
+  if (tid == 0) s.left = want;
+  KEY border = fixed;                        // the digits above that all keys share
+  for (int shift = top_shift; shift >= 0; shift -= 8) {
+    s.hist[tid] = 0;
     __syncthreads();
-    const uint64_t mask = shift == 56 ? 0ull : ~0ull << (shift + 8);
-    for (int i = tid; i < middle; i += SEL_THREADS)
-      if ((keys[i] & mask) == border) atomicAdd(&hist[(keys[i] >> shift) & 255], 1);
+    const KEY mask = shift + 8 >= kBits ? (KEY)0 : (KEY)(~(KEY)0 << (shift + 8));
+    for (int i = tid; i < n; i += SEL_THREADS)
+      if ((keys[i] & mask) == border) atomicAdd(&s.hist[(int)(keys[i] >> shift) & 255], 1);
     __syncthreads();
     if (warp == 0) {
       // digits from the largest down, eight a lane
       int own[8], sum = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += own[j] = hist[255 - lane * 8 - j];
+      for (int j = 0; j < 8; ++j) sum += own[j] = s.hist[255 - lane * 8 - j];
       int upto = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
-      const int left = s_left;
+      const int left = s.left;
       int before = upto - sum;
       __syncwarp();
       if (before < left && left <= upto) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (before < left && left <= before + own[j]) {
-            s_digit = 255 - lane * 8 - j;
-            s_left = left - before;
+            s.digit = 255 - lane * 8 - j;
+            s.left = left - before;
           }
           before += own[j];
         }
       }
     }
     __syncthreads();
-    if (want > 0) border |= (uint64_t)s_digit << shift;
+    border |= (KEY)s.digit << shift;
   }
-  // `s_left` of the blocks at the border are taken, the first ones.  Each warp has a run of blocks.
-  const int run = ((middle + 7) / 8 + 31) / 32 * 32;
-  const int from = min(warp * run, middle), to = min(from + run, middle);
-  int eq = 0, gt = 0;
-  for (int i = from + lane; i < to; i += 32) {
-    eq += keys[i] == border ? 1 : 0;
-    gt += keys[i] > border ? 1 : 0;
-  }
+  return border;
+}
+
+// Score of a block in 64 bits, by a warp: the largest over the query heads.  Products of two bf16 are
+// exact in fp32, and 128 of them all but always in a 64-bit sum.
+__device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int token, int kvh,
+                                                const uint16_t* at, int lane) {
+  const uint2 lo = *reinterpret_cast<const uint2*>(at + lane * 4);
+  const uint2 hi = *reinterpret_cast<const uint2*>(at + SEL_D + lane * 4);
+  const double l[4] = {bf16lo(lo.x), bf16hi(lo.x), bf16lo(lo.y), bf16hi(lo.y)};
+  const double u[4] = {bf16lo(hi.x), bf16hi(hi.x), bf16lo(hi.y), bf16hi(hi.y)};
+  const uint16_t* qp = p.q + (int64_t)token * p.q_stride + (int64_t)kvh * p.g * SEL_D + lane * 4;
+  double best = -INFINITY;
+  bool nan = false;
+  for (int h = 0; h < p.g; ++h) {
+    const uint2 qv = *reinterpret_cast<const uint2*>(qp + h * SEL_D);
+    const double q[4] = {bf16lo(qv.x), bf16hi(qv.x), bf16lo(qv.y), bf16hi(qv.y)};
+    double sum = 0.0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    eq += __shfl_xor_sync(0xffffffffu, eq, o);
-    gt += __shfl_xor_sync(0xffffffffu, gt, o);
-  }
-  if (lane == 0) { s_eq[warp] = eq; s_gt[warp] = gt; }
-  __syncthreads();
-  const int ties = want > 0 ? s_left : 0;
-  int seen = 0, at = 0;                      // at the border, and taken, ahead of this warp's run
-  for (int w = 0; w < warp; ++w) { seen += s_eq[w]; at += s_gt[w]; }
-  at += min(seen, ties);
-  if (want > 0) {
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const int i = i0 + lane;
-      const uint64_t key = i < to ? keys[i] : 0ull;
-      const bool is_eq = i < to && key == border;
-      const uint32_t eqs = __ballot_sync(0xffffffffu, is_eq), below = (1u << lane) - 1u;
-      const bool take = i < to && (key > border ||
-                                   (is_eq && seen + __popc(eqs & below) < ties));
-      const uint32_t takes = __ballot_sync(0xffffffffu, take);
-      if (take) out[p.keep_first + at + __popc(takes & below)] = p.keep_first + i;
-      seen += __popc(eqs);
-      at += __popc(takes);
+    for (int d = 0; d < 4; ++d) {
+      const double a = q[d] * l[d], c = q[d] * u[d];
+      sum += a != a || c != c ? a + c : fmax(a, c);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    nan |= sum != sum;
+    best = fmax(best, sum);
   }
-  for (int i = tid; i < p.keep_first; i += SEL_THREADS) out[i] = i;
-  for (int i = tid; i < p.keep_last; i += SEL_THREADS)
-    out[p.count - p.keep_last + i] = n - p.keep_last + i;
+  return nan ? ~0ull : order_of(best);
+}
+
+// One CTA per KV head and token, or several tokens of one table.
+//
+// Scores: sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with the positive and negative parts of
+// q, a product of 16 rows (query heads, of several tokens where they fit) by 8 blocks by 256 on the
+// tensor cores, the blocks' bounds straight from memory: a lane loads 16 bytes, which are operands of
+// two instructions when q's channels are taken in the same order.  Sums in fp32 are off by at most
+// e = 2^-15 sum |q| max |bound| (16 instructions of 17 terms, each off by at most 2^-23 of the sums
+// of absolute values: 2^-15.9).  Of the blocks between the kept ends those above the want-th largest
+// score by more than 2 e are taken, those below it by more are not, and those between are scored
+// again in 64 bits if they do not all fit.  So the choice is that of 64 bits, ties to the lower
+// index.
+//
+// Bounds: the bytes of the bounds when there are many tokens (8 loads of 16 bytes are under way per
+// lane, two CTAs on an SM), else the latency of the steps behind the scores.
+__global__ void __launch_bounds__(SEL_THREADS, 2) select_blocks_kernel(const SelectParams p) {
+  extern __shared__ uint64_t sel_smem[];
+  __shared__ SelectShared s;
+  uint64_t* exact = sel_smem;                                       // [most]
+  uint32_t* scores = reinterpret_cast<uint32_t*>(exact + p.most);   // [together][most], ordered
+  uint16_t* band = reinterpret_cast<uint16_t*>(scores + p.together * p.most);   // [most]
+  pdl_launch_dependents();
+  pdl_wait();
+  const int kvh = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = p.page / p.block;
+  auto length = [&](int token, int row) -> int {
+    const int64_t len = p.context_lens[token];
+    if (len <= 0 || row < 0 || row >= p.num_tables) return 0;
+    return (int)(len > p.capacity ? p.capacity : len);
+  };
+  auto bounds_at = [&](int page, int b) -> const uint16_t* {
+    return p.bounds + (((int64_t)page * p.hkv + kvh) * per + b % per) * 2 * SEL_D;
+  };
+
+  // runs of tokens with one table
+  const int last_token = min(p.num_tokens, ((int)blockIdx.x + 1) * p.together);
+  for (int t0 = blockIdx.x * p.together; t0 < last_token;) {
+    const int row = p.rows ? p.rows[t0] : t0;
+    int t1 = t0 + 1;
+    while (t1 < last_token && p.rows[t1] == row) ++t1;
+    int longest = 0;
+    bool bad = row < 0 || row >= p.num_tables;
+    for (int t = t0; t < t1; ++t) {
+      bad |= p.context_lens[t] > p.capacity;
+      longest = max(longest, length(t, row));
+    }
+    if (bad && tid == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+    const int32_t* table = p.tables + (int64_t)row * p.table_stride;
+    // scores of blocks keep_first .. of the longest context; a shorter one uses fewer of them
+    const int blocks = (longest + p.block - 1) / p.block;
+    const int scored = blocks > p.count ? blocks - p.keep_first - p.keep_last : 0;
+    if (scored > 0) {
+      // rows lane / 4 and lane / 4 + 8 of q, channels 32 j + 8 (lane % 4) + 0 .. 7
+      uint32_t qp[4][8], qm[4][8];
+      const int r0 = lane >> 2, quad = lane & 3;
+      float abs0 = 0.f, abs1 = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = r0 + half * 8, t = t0 + r / p.g;
+        const bool live = t < t1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (live)
+            v = *reinterpret_cast<const uint4*>(
+                p.q + (int64_t)t * p.q_stride + ((int64_t)kvh * p.g + r % p.g) * SEL_D + j * 32 +
+                quad * 8);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            qp[j][half * 4 + i] = max2_nan(w[i], 0u);
+            qm[j][half * 4 + i] = min2_nan(w[i], 0u);
+            const float a = fabsf(bf16lo(w[i])) + fabsf(bf16hi(w[i]));
+            if (half) abs1 += a; else abs0 += a;
+          }
+        }
+      }
+      abs0 += __shfl_xor_sync(0xffffffffu, abs0, 1); abs1 += __shfl_xor_sync(0xffffffffu, abs1, 1);
+      abs0 += __shfl_xor_sync(0xffffffffu, abs0, 2); abs1 += __shfl_xor_sync(0xffffffffu, abs1, 2);
+      if (tid < 16) s.q_sum[tid] = 0.f;
+      __syncthreads();
+      if (warp == 0 && quad == 0) {
+        // not a number counts as infinite; whole numbers order floats above zero
+        auto put = [&](int r, float a) {
+          if (r / p.g < p.together)
+            atomicMax(reinterpret_cast<int*>(&s.q_sum[r / p.g]),
+                      __float_as_int(a < INFINITY ? a : INFINITY));
+        };
+        put(r0, abs0);
+        put(r0 + 8, abs1);
+      }
+      uint32_t most = 0u;                      // largest |bound|, two channels at once
+      for (int b0 = warp * 8; b0 < scored; b0 += 8 * (SEL_THREADS / 32)) {
+        const int mine = b0 + r0, b = p.keep_first + mine;
+        int page = mine < scored ? table[b / per] : -1;
+        if (mine < scored && (page < 0 || page >= p.num_pages)) {
+          if (p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+          page = -1;
+        }
+        const bool have = page >= 0;
+        uint4 lo[4], hi[4];
+        const uint16_t* at = bounds_at(have ? page : 0, have ? b : 0) + quad * 8;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          hi[j] = lo[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (have) {
+            hi[j] = *reinterpret_cast<const uint4*>(at + SEL_D + j * 32);
+            lo[j] = *reinterpret_cast<const uint4*>(at + j * 32);
+          }
+        }
+        float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t pa[4] = {qp[j][0], qp[j][4], qp[j][1], qp[j][5]};
+          const uint32_t pb[4] = {qp[j][2], qp[j][6], qp[j][3], qp[j][7]};
+          const uint32_t ma[4] = {qm[j][0], qm[j][4], qm[j][1], qm[j][5]};
+          const uint32_t mb[4] = {qm[j][2], qm[j][6], qm[j][3], qm[j][7]};
+          mma_bf16_16816(c0, pa, hi[j].x, hi[j].y);
+          mma_bf16_16816(c1, ma, lo[j].x, lo[j].y);
+          mma_bf16_16816(c0, pb, hi[j].z, hi[j].w);
+          mma_bf16_16816(c1, mb, lo[j].z, lo[j].w);
+          most = max2_nan(most, max2_nan(max2_nan(hi[j].x & 0x7fff7fffu, hi[j].y & 0x7fff7fffu),
+                                         max2_nan(hi[j].z & 0x7fff7fffu, hi[j].w & 0x7fff7fffu)));
+          most = max2_nan(most, max2_nan(max2_nan(lo[j].x & 0x7fff7fffu, lo[j].y & 0x7fff7fffu),
+                                         max2_nan(lo[j].z & 0x7fff7fffu, lo[j].w & 0x7fff7fffu)));
+        }
+        // rows r0 and r0 + 8 of blocks b0 + 2 quad + 0, 1: the largest of each token's rows
+        float v[4] = {c0[0] + c1[0], c0[1] + c1[1], c0[2] + c1[2], c0[3] + c1[3]};
+        const uint32_t bads = __ballot_sync(0xffffffffu, mine < scored && !have);
+        if (p.together == 1) {
+          if (r0 >= p.g) v[0] = v[1] = -INFINITY;
+          if (r0 + 8 >= p.g) v[2] = v[3] = -INFINITY;
+          v[0] = v[2] = fmaxf(v[0], v[2]);
+          v[1] = v[3] = fmaxf(v[1], v[3]);
+        }
+        const int across = p.together == 1 ? 8 : p.g;
+        for (int o = 1; o < across; o <<= 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = fmaxf(v[i], __shfl_xor_sync(0xffffffffu, v[i], o * 4));
+        }
+        if (r0 % across == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int col = quad * 2 + (i & 1);
+            const int tq = p.together == 1 ? 0 : (r0 + (i >> 1) * 8) / p.g;
+            if ((p.together == 1 && i > 1) || b0 + col >= scored || tq >= p.together) continue;
+            scores[tq * p.most + b0 + col] = bads >> (col * 4) & 1u ? 0u : order_of(v[i]);
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = max2_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (lane == 0) s.most[warp] = most;
+      __syncthreads();
+    }
+
+    for (int token = t0; token < t1; ++token) {
+      int32_t* out = p.selected + ((int64_t)token * p.hkv + kvh) * p.count;
+      const int n = (length(token, row) + p.block - 1) / p.block;
+      if (n <= p.count) {
+        for (int i = tid; i < p.count; i += SEL_THREADS) out[i] = i < n ? i : -1;
+        continue;
+      }
+      const int middle = n - p.keep_first - p.keep_last;
+      const int want = p.count - p.keep_first - p.keep_last;     // of the middle ones
+      for (int i = tid; i < p.keep_first; i += SEL_THREADS) out[i] = i;
+      for (int i = tid; i < p.keep_last; i += SEL_THREADS)
+        out[p.count - p.keep_last + i] = n - p.keep_last + i;
+      if (want == 0) continue;
+      uint32_t* keys = scores + (token - t0) * p.most;
+      uint32_t most = s.most[0];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) most = max2_nan(most, s.most[w]);
+      const float reach = s.q_sum[token - t0] * __uint_as_float(max(most << 16, most & 0xffff0000u));
+      // scores past fp32's range, products below it, and what is not a number: all in 64 bits
+      const bool all = !(reach < INFINITY) || (reach > 0.f && reach < 7.9e-31f);
+      uint32_t above, least;                 // keys above are taken, keys below `least` are not
+      bool same = false;                     // keys between are equal in truth
+      if (all) {
+        above = ~0u; least = 0u;
+      } else {
+        // digits that all keys share need no pass
+        uint32_t lo = ~0u, hi = 0u;
+        for (int i = tid; i < middle; i += SEL_THREADS) {
+          lo = min(lo, keys[i]);
+          hi = max(hi, keys[i]);
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        __syncthreads();
+        if (lane == 0) { s.lo[warp] = lo; s.hi[warp] = hi; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) { lo = min(lo, s.lo[w]); hi = max(hi, s.hi[w]); }
+        const int shift = lo == hi ? 0 : (31 - __clz(lo ^ hi)) / 8 * 8;
+        const uint32_t border = border_of<uint32_t>(
+            keys, middle, want, shift, shift == 24 ? 0u : hi & ~0u << (shift + 8), s);
+        const float v = value_of(border), e2 = reach * (2.f / 32768.f);
+        same = border == 0u || reach == 0.f;
+        above = same ? border : order_of(v + e2);
+        least = same ? border : order_of(v - e2);
+      }
+      // how many are above, and between
+      int eq = 0, gt = 0;
+      const int run = ((middle + 7) / 8 + 31) / 32 * 32;       // blocks of a warp
+      const int from = min(warp * run, middle), to = min(from + run, middle);
+      for (int i = from + lane; i < to; i += 32) {
+        gt += keys[i] > above ? 1 : 0;
+        eq += keys[i] >= least && keys[i] <= above ? 1 : 0;
+      }
+      eq = __reduce_add_sync(0xffffffffu, eq);
+      gt = __reduce_add_sync(0xffffffffu, gt);
+      __syncthreads();
+      if (lane == 0) { s.eq[warp] = eq; s.gt[warp] = gt; }
+      __syncthreads();
+      int eqs = 0, gts = 0, eq_before = 0, gt_before = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        if (w == warp) { eq_before = eqs; gt_before = gts; }
+        eqs += s.eq[w];
+        gts += s.gt[w];
+      }
+      int ties = want - gts;                 // of those between, the first ones if they are equal
+      if (!same && eqs > ties) {
+        // score those between again; their keys become "taken" or "not"
+        int at = eq_before;
+        for (int i0 = from; i0 < to; i0 += 32) {
+          const int i = i0 + lane;
+          const bool is = i < to && keys[i] >= least && keys[i] <= above;
+          const uint32_t votes = __ballot_sync(0xffffffffu, is);
+          if (is) band[at + __popc(votes & ((1u << lane) - 1u))] = (uint16_t)i;
+          at += __popc(votes);
+        }
+        __syncthreads();
+        for (int c = warp; c < eqs; c += 8) {
+          const int b = p.keep_first + band[c];
+          uint64_t key = 0ull;               // without a page
+          if (keys[band[c]] != 0u)
+            key = exact_score(p, token, kvh, bounds_at(table[b / per], b), lane);
+          if (lane == 0) exact[c] = key;
+        }
+        __syncthreads();
+        if (eqs <= 32) {
+          // a lane per block: its rank, the lower index first among equals
+          if (warp == 0) {
+            const uint64_t key = lane < eqs ? exact[lane] : 0ull;
+            int rank = 0;
+            for (int j = 0; j < eqs; ++j) {
+              const uint64_t other = __shfl_sync(0xffffffffu, key, j);
+              rank += other > key || (other == key && j < lane) ? 1 : 0;
+            }
+            if (lane < eqs) keys[band[lane]] = rank < ties ? ~0u : 0u;
+          }
+          __syncthreads();
+        } else {
+          const uint64_t edge = border_of<uint64_t>(exact, eqs, ties, 56, 0ull, s);
+          const int left = s.left;
+          // equal ones in order: a warp has a run of them, as above
+          const int run_c = ((eqs + 7) / 8 + 31) / 32 * 32;
+          const int fc = min(warp * run_c, eqs), tc = min(fc + run_c, eqs);
+          int n_eq = 0;
+          for (int c = fc + lane; c < tc; c += 32) n_eq += exact[c] == edge ? 1 : 0;
+          n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+          __syncthreads();
+          if (lane == 0) s.eq[warp] = n_eq;
+          __syncthreads();
+          int seen = 0;
+          for (int w = 0; w < warp; ++w) seen += s.eq[w];
+          for (int c0 = fc; c0 < tc; c0 += 32) {
+            const int c = c0 + lane;
+            const bool is = c < tc && exact[c] == edge;
+            const uint32_t votes = __ballot_sync(0xffffffffu, is);
+            if (c < tc)
+              keys[band[c]] = exact[c] > edge ||
+                                      (is && seen + __popc(votes & ((1u << lane) - 1u)) < left)
+                                  ? ~0u : 0u;
+            seen += __popc(votes);
+          }
+          __syncthreads();
+        }
+        // taken ones are above now, and nothing is between
+        above = min(above, ~0u - 1u);
+        least = ~0u;
+        gt = 0;
+        for (int i = from + lane; i < to; i += 32) gt += keys[i] > above ? 1 : 0;
+        gt = __reduce_add_sync(0xffffffffu, gt);
+        __syncthreads();
+        if (lane == 0) s.gt[warp] = gt;
+        __syncthreads();
+        gt_before = 0;
+        for (int w = 0; w < warp; ++w) gt_before += s.gt[w];
+        eq_before = 0;
+        ties = 0;
+      }
+      // taken ones in order
+      int seen = eq_before, at = gt_before + min(eq_before, ties);
+      for (int i0 = from; i0 < to; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t key = i < to ? keys[i] : 0u;
+        const bool is_eq = ties > 0 && i < to && key >= least && key <= above;
+        const uint32_t votes = __ballot_sync(0xffffffffu, is_eq), below = (1u << lane) - 1u;
+        const bool take = i < to && (key > above || (is_eq && seen + __popc(votes & below) < ties));
+        const uint32_t takes = __ballot_sync(0xffffffffu, take);
+        if (take) out[p.keep_first + at + __popc(takes & below)] = p.keep_first + i;
+        seen += __popc(votes);
+        at += __popc(takes);
+      }
+      __syncthreads();
+    }
+    t0 = t1;
+  }
 }
 
 // what the entry points of this file have in common
@@ -380,17 +649,24 @@ int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, 
   p.context_lens = context_lens; p.rows = table_rows;
   p.tables = block_tables; p.table_stride = block_table_stride;
   p.capacity = block_table_cols * page_size;
-  p.num_tables = num_tables; p.num_pages = (int)num_pages; p.page = page_size; p.block = block;
+  p.num_tokens = num_tokens; p.num_tables = num_tables; p.num_pages = (int)num_pages;
+  p.page = page_size; p.block = block;
   p.hkv = num_kv_heads; p.g = num_q_heads / num_kv_heads;
   p.count = count; p.keep_first = keep_first; p.keep_last = keep_last;
+  p.most = (int)most;
+  // Tokens that may have one table share the scores' products, as far as their query heads fill the
+  // 16 rows and 32 KiB of scores leave several CTAs on an SM.
+  p.together = 1;
+  if (table_rows != nullptr && (p.g & (p.g - 1)) == 0)
+    while (p.together * 2 * p.g <= 16 && p.together * 2 * most * 4 <= 32768) p.together *= 2;
   p.selected = selected;
   p.status = status;
+  const int64_t ctas = ((int64_t)num_tokens + p.together - 1) / p.together;
+  const size_t smem = (size_t)most * (8 + 4 * (size_t)p.together + 2) + 16;
   static PerDeviceOnce once;
-  FK_CUDA_OK(set_max_dynamic_smem(once, select_blocks_kernel, SEL_MAX_BLOCKS * 8));
-  FK_CUDA_OK(launch_kernel(select_blocks_kernel,
-                           dim3((unsigned)num_tokens, (unsigned)num_kv_heads),
-                           dim3(SEL_THREADS), (size_t)(most < 1 ? 8 : most * 8),
-                           static_cast<cudaStream_t>(stream), p));
+  FK_CUDA_OK(set_max_dynamic_smem(once, select_blocks_kernel, SEL_MAX_BLOCKS * 14 + 16));
+  FK_CUDA_OK(launch_kernel(select_blocks_kernel, dim3((unsigned)ctas, (unsigned)num_kv_heads),
+                           dim3(SEL_THREADS), smem, static_cast<cudaStream_t>(stream), p));
   count_launch(1);
   return FK_OK;
 }
