@@ -72,7 +72,8 @@ PROTOTYPES = {
     "fk_key_bounds": (_i32, [_vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i64,
                              _i64, _vp, _i32, _i32, _vp, _vp]),
     "fk_select_blocks": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i32,
-                                _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+                                _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp, _vp]),
+    "fk_select_blocks_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i64]),
     "fk_selected_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "fk_selected_attn": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp,
                                 _vp, _i64, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32,

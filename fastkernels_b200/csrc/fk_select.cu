@@ -11,9 +11,9 @@
 namespace fk {
 
 constexpr int SEL_D = 128;                    // head_dim
-constexpr int SEL_THREADS = 256;
 constexpr int SEL_MAX_G = 16;                 // query heads per KV head
 constexpr int SEL_MAX_BLOCKS = 16384;         // of one context
+constexpr int SEL_WARP_BLOCKS = 1024;         // of one context, where a warp chooses
 
 // ---------------------------------------------------------------------------
 // bounds
@@ -127,8 +127,12 @@ struct SelectParams {
   int64_t capacity;
   int num_tokens, num_tables, num_pages, page, block, hkv, g;
   int count, keep_first, keep_last;
+  int per_shift;                      // log2 of the blocks of a page, -1: no power of two
   int together;                       // tokens of a CTA: 1, or up to 16 / g (a power of two)
   int most;                           // blocks that a table's row has pages for
+  int chunk, chunks;                  // blocks of a CTA of the scores, of those CTAs per token
+  uint32_t* scores;                   // [tokens, hkv, most], ordered
+  float* largest;                     // [groups of tokens, hkv, chunks] largest |bound| of a chunk
   int32_t* selected;                  // [tokens, hkv, count]
   int32_t* status;
 };
@@ -148,154 +152,415 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
 }
 
-struct SelectShared {
+// The threads that choose for one token: a warp, or all eight.
+template <int W>
+struct Team {
   int hist[256];
-  int digit, left;
-  int eq[8], gt[8];
-  float q_sum[16];                    // of each token: largest sum of |q| of its query heads
-  uint32_t most[8];                   // largest |bound|, as bf16 bits
-  uint32_t lo[8], hi[8];
+  int count;
+  int eq[W], gt[W];
+  uint64_t lo[W], hi[W];
+  uint64_t near[32];
+
+  static __device__ __forceinline__ int rank() { return W == 1 ? threadIdx.x & 31 : threadIdx.x; }
+  static __device__ __forceinline__ int warp() { return W == 1 ? 0 : threadIdx.x >> 5; }
+  static __device__ __forceinline__ void sync() {
+    if (W == 1) __syncwarp(); else __syncthreads();
+  }
 };
 
-// The want-th largest of n keys (want >= 1), and in s.left how many of the keys equal to it are
-// among the want largest.  All threads; ends behind a barrier.
-template <typename KEY>
-__device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int top_shift,
-                                         KEY fixed, SelectShared& s) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// The want-th largest of n keys (1 <= want <= n), and how many of the keys that equal it are among the
+// want largest.  Counts of 256 parts of the range of keys leave one part, which is the range of
+// the next round, until 32 keys are left, which are ranked, or all that are left are equal.
+template <int W, typename KEY>
+__device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int* left, Team<W>& s) {
+  const int tid = Team<W>::rank(), lane = threadIdx.x & 31;
   constexpr int kBits = 8 * sizeof(KEY);
-  if (tid == 0) s.left = want;
-  KEY border = fixed;                        // the digits above that all keys share
-  for (int shift = top_shift; shift >= 0; shift -= 8) {
-    s.hist[tid] = 0;
-    __syncthreads();
-    const KEY mask = shift + 8 >= kBits ? (KEY)0 : (KEY)(~(KEY)0 << (shift + 8));
-    for (int i = tid; i < n; i += SEL_THREADS)
-      if ((keys[i] & mask) == border) atomicAdd(&s.hist[(int)(keys[i] >> shift) & 255], 1);
-    __syncthreads();
-    if (warp == 0) {
-      // digits from the largest down, eight a lane
-      int own[8], sum = 0;
+  KEY lo = (KEY)~(KEY)0, hi = 0;
+  for (int i = tid; i < n; i += 32 * W) {
+    lo = min(lo, keys[i]);
+    hi = max(hi, keys[i]);
+  }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += own[j] = s.hist[255 - lane * 8 - j];
-      int upto = sum;
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (W > 1) {
+    if (lane == 0) { s.lo[Team<W>::warp()] = lo; s.hi[Team<W>::warp()] = hi; }
+    Team<W>::sync();
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      const int left = s.left;
-      int before = upto - sum;
-      __syncwarp();
-      if (before < left && left <= upto) {
+    for (int w = 0; w < W; ++w) {
+      lo = min(lo, (KEY)s.lo[w]);
+      hi = max(hi, (KEY)s.hi[w]);
+    }
+  }
+  while (lo != hi) {
+    const int used = kBits - (kBits == 64 ? __clzll((long long)(hi - lo)) : __clz((int)(hi - lo)));
+    const int shift = max(0, used - 8);
+    for (int i = tid; i < 256; i += 32 * W) s.hist[i] = 0;
+    if (tid == 0) s.count = 0;
+    Team<W>::sync();
+    for (int i = tid; i < n; i += 32 * W) {
+      const KEY k = keys[i];
+      if (k >= lo && k <= hi) atomicAdd(&s.hist[(int)((k - lo) >> shift)], 1);
+    }
+    Team<W>::sync();
+    // parts from the largest down, eight a lane; every warp looks for itself
+    const int4 p1 = reinterpret_cast<const int4*>(s.hist)[63 - lane * 2];
+    const int4 p0 = reinterpret_cast<const int4*>(s.hist)[62 - lane * 2];
+    const int own[8] = {p1.w, p1.z, p1.y, p1.x, p0.w, p0.z, p0.y, p0.x};
+    int sum = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (before < left && left <= before + own[j]) {
-            s.digit = 255 - lane * 8 - j;
-            s.left = left - before;
-          }
-          before += own[j];
+    for (int j = 0; j < 8; ++j) sum += own[j];
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    before -= sum;
+    const bool mine = before < want && want <= before + sum;
+    int part = 0, many = 0, ahead = 0;
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (before < want && want <= before + own[j]) {
+          part = 255 - lane * 8 - j;
+          many = own[j];
+          ahead = before;
         }
+        before += own[j];
       }
     }
-    __syncthreads();
-    border |= (KEY)s.digit << shift;
+    const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+    part = __shfl_sync(0xffffffffu, part, src);
+    many = __shfl_sync(0xffffffffu, many, src);
+    want -= __shfl_sync(0xffffffffu, ahead, src);
+    lo += (KEY)part << shift;
+    hi = min(hi, (KEY)(lo + (((KEY)1 << shift) - 1)));
+    if (shift == 0) break;                     // lo == hi
+    if (many <= 32) {
+      for (int i = tid; i < n; i += 32 * W) {
+        const KEY k = keys[i];
+        if (k >= lo && k <= hi) s.near[atomicAdd(&s.count, 1)] = k;
+      }
+      Team<W>::sync();
+      const KEY k = lane < many ? (KEY)s.near[lane] : (KEY)0;
+      int above = 0, equal = 0;
+      for (int j = 0; j < many; ++j) {
+        const KEY other = __shfl_sync(0xffffffffu, k, j);
+        above += other > k ? 1 : 0;
+        equal += other == k ? 1 : 0;
+      }
+      const bool is = lane < many && above < want && want <= above + equal;
+      const int at = __ffs(__ballot_sync(0xffffffffu, is)) - 1;
+      lo = __shfl_sync(0xffffffffu, k, at);
+      want -= __shfl_sync(0xffffffffu, above, at);
+      break;
+    }
+    Team<W>::sync();                           // the counts have been read
   }
-  return border;
+  Team<W>::sync();
+  *left = want;
+  return lo;
 }
 
-// Score of a block in 64 bits, by a warp: the largest over the query heads.  Products of two bf16 are
-// exact in fp32, and 128 of them all but always in a 64-bit sum.
+// Score of a block in 64 bits, by eight lanes: the largest over the query heads.  Products of two bf16
+// are exact in fp32, and 128 of them all but always in a 64-bit sum.
 __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int token, int kvh,
                                                 const uint16_t* at, int lane) {
-  const uint2 lo = *reinterpret_cast<const uint2*>(at + lane * 4);
-  const uint2 hi = *reinterpret_cast<const uint2*>(at + SEL_D + lane * 4);
-  const double l[4] = {bf16lo(lo.x), bf16hi(lo.x), bf16lo(lo.y), bf16hi(lo.y)};
-  const double u[4] = {bf16lo(hi.x), bf16hi(hi.x), bf16lo(hi.y), bf16hi(hi.y)};
-  const uint16_t* qp = p.q + (int64_t)token * p.q_stride + (int64_t)kvh * p.g * SEL_D + lane * 4;
-  double best = -INFINITY;
+  float l[16], u[16];
   bool nan = false;
-  for (int h = 0; h < p.g; ++h) {
-    const uint2 qv = *reinterpret_cast<const uint2*>(qp + h * SEL_D);
-    const double q[4] = {bf16lo(qv.x), bf16hi(qv.x), bf16lo(qv.y), bf16hi(qv.y)};
-    double sum = 0.0;
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const double a = q[d] * l[d], c = q[d] * u[d];
-      sum += a != a || c != c ? a + c : fmax(a, c);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    nan |= sum != sum;
-    best = fmax(best, sum);
+  for (int i = 0; i < 4; ++i) {
+    const uint2 a = reinterpret_cast<const uint2*>(at)[i * 8 + (lane & 7)];
+    const uint2 b = reinterpret_cast<const uint2*>(at + SEL_D)[i * 8 + (lane & 7)];
+    l[4 * i] = bf16lo(a.x); l[4 * i + 1] = bf16hi(a.x);
+    l[4 * i + 2] = bf16lo(a.y); l[4 * i + 3] = bf16hi(a.y);
+    u[4 * i] = bf16lo(b.x); u[4 * i + 1] = bf16hi(b.x);
+    u[4 * i + 2] = bf16lo(b.y); u[4 * i + 3] = bf16hi(b.y);
   }
-  return nan ? ~0ull : order_of(best);
+  bool odd = false;                            // an infinity, or no number
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    nan |= l[i] != l[i] || u[i] != u[i];
+    odd |= !(fabsf(l[i]) < INFINITY) || !(fabsf(u[i]) < INFINITY);
+  }
+  odd = __any_sync(0xffffffffu, odd);
+  const uint16_t* qp = p.q + (int64_t)token * p.q_stride + (int64_t)kvh * p.g * SEL_D;
+  double best = -INFINITY;
+#pragma unroll 2
+  for (int h = 0; h < p.g; ++h) {
+    double sum[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint2 v = reinterpret_cast<const uint2*>(qp + h * SEL_D)[i * 8 + (lane & 7)];
+      const float q[4] = {bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        sum[k & 1] += (double)q[k] * (double)(q[k] > 0.f ? u[4 * i + k] : l[4 * i + k]);
+        // zero times infinity is no number on either side
+        if (odd) nan |= q[k] == 0.f && (isinf(l[4 * i + k]) || isinf(u[4 * i + k]));
+      }
+    }
+    double all = sum[0] + sum[1];
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    nan |= all != all;
+    best = fmax(best, all);
+  }
+  const uint32_t nans = __ballot_sync(0xffffffffu, nan);
+  return nans >> (lane & 24) & 255u ? ~0ull : order_of(best);
 }
 
-// One CTA per KV head and token, or several tokens of one table.
+// The choice of one token, by a team: `keys` are the scores of its n - keep_first - keep_last blocks
+// in the middle, `reach` bounds sum |q| max |bound|.  exact and band: room for those blocks.
+template <int W>
+__device__ __forceinline__ void choose(const SelectParams& p, int token, int kvh, int n,
+                                       const int32_t* table, uint32_t* keys, float reach,
+                                       uint64_t* exact, uint16_t* band, Team<W>& s) {
+  const int tid = Team<W>::rank(), warp = Team<W>::warp(), lane = threadIdx.x & 31;
+  const uint32_t below = (1u << lane) - 1u;
+  const int per = p.page / p.block;
+  int32_t* out = p.selected + ((int64_t)token * p.hkv + kvh) * p.count;
+  if (n <= p.count) {
+    for (int i = tid; i < p.count; i += 32 * W) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int middle = n - p.keep_first - p.keep_last;
+  const int want = p.count - p.keep_first - p.keep_last;     // of the middle ones
+  for (int i = tid; i < p.keep_first; i += 32 * W) out[i] = i;
+  for (int i = tid; i < p.keep_last; i += 32 * W)
+    out[p.count - p.keep_last + i] = n - p.keep_last + i;
+  if (want == 0) return;
+  // scores past fp32's range, products below it, and what is no number: all in 64 bits
+  const bool all = !(reach < INFINITY) || (reach > 0.f && reach < 7.9e-31f);
+  uint32_t above = ~0u, least = 0u;            // keys above are taken, keys below `least` are not
+  bool same = false;                           // keys between are equal in truth
+  if (!all) {
+    int left;
+    const uint32_t border = border_of<W, uint32_t>(keys, middle, want, &left, s);
+    const float v = value_of(border), e2 = reach * (2.f / 262144.f);
+    same = border == 0u || reach == 0.f;
+    above = same ? border : order_of(v + e2);
+    least = same ? border : order_of(v - e2);
+  }
+  // how many are above, and between; each warp has a run of blocks
+  const int run = ((middle + W - 1) / W + 31) / 32 * 32;
+  const int from = min(warp * run, middle), to = min(from + run, middle);
+  auto count = [&](int* eqs, int* gts, int* eq_before, int* gt_before) {
+    int eq = 0, gt = 0;
+    for (int i = from + lane; i < to; i += 32) {
+      gt += keys[i] > above ? 1 : 0;
+      eq += keys[i] >= least && keys[i] <= above ? 1 : 0;
+    }
+    *eqs = __reduce_add_sync(0xffffffffu, eq);
+    *gts = __reduce_add_sync(0xffffffffu, gt);
+    *eq_before = *gt_before = 0;
+    if (W == 1) return;
+    Team<W>::sync();
+    if (lane == 0) { s.eq[warp] = *eqs; s.gt[warp] = *gts; }
+    Team<W>::sync();
+    *eqs = *gts = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w == warp) { *eq_before = *eqs; *gt_before = *gts; }
+      *eqs += s.eq[w];
+      *gts += s.gt[w];
+    }
+  };
+  int eqs, gts, eq_before, gt_before;
+  count(&eqs, &gts, &eq_before, &gt_before);
+  int ties = want - gts;                       // of those between, the first ones if they are equal
+  if (!same && eqs > ties) {
+    // score those between again; their keys become "taken" or "not"
+    int at = eq_before;
+    for (int i0 = from; i0 < to; i0 += 32) {
+      const int i = i0 + lane;
+      const bool is = i < to && keys[i] >= least && keys[i] <= above;
+      const uint32_t votes = __ballot_sync(0xffffffffu, is);
+      if (is) band[at + __popc(votes & below)] = (uint16_t)i;
+      at += __popc(votes);
+    }
+    Team<W>::sync();
+    for (int c0 = warp * 4; c0 < eqs; c0 += W * 4) {
+      const int c = min(c0 + (lane >> 3), eqs - 1);
+      const int b = p.keep_first + band[c];
+      const bool paged = keys[band[c]] != 0u;
+      const int64_t page = paged ? table[b / per] : 0;
+      const uint64_t key = exact_score(
+          p, token, kvh, p.bounds + ((page * p.hkv + kvh) * per + b % per) * 2 * SEL_D, lane);
+      if ((lane & 7) == 0 && c0 + (lane >> 3) < eqs) exact[c] = paged ? key : 0ull;
+    }
+    Team<W>::sync();
+    if (eqs <= 32) {
+      // a lane per block: its rank, the lower index first among equals
+      const uint64_t key = lane < eqs ? exact[lane] : 0ull;
+      int rank = 0;
+      for (int j = 0; j < eqs; ++j) {
+        const uint64_t other = __shfl_sync(0xffffffffu, key, j);
+        rank += other > key || (other == key && j < lane) ? 1 : 0;
+      }
+      if (warp == 0 && lane < eqs) keys[band[lane]] = rank < ties ? ~0u : 0u;
+    } else {
+      int left;
+      const uint64_t edge = border_of<W, uint64_t>(exact, eqs, ties, &left, s);
+      // equal ones in order: a warp has a run of them, as above
+      const int run_c = ((eqs + W - 1) / W + 31) / 32 * 32;
+      const int fc = min(warp * run_c, eqs), tc = min(fc + run_c, eqs);
+      int seen = 0;
+      if (W > 1) {
+        int n_eq = 0;
+        for (int c = fc + lane; c < tc; c += 32) n_eq += exact[c] == edge ? 1 : 0;
+        n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+        if (lane == 0) s.eq[warp] = n_eq;
+        Team<W>::sync();
+        for (int w = 0; w < warp; ++w) seen += s.eq[w];
+      }
+      for (int c0 = fc; c0 < tc; c0 += 32) {
+        const int c = c0 + lane;
+        const bool is = c < tc && exact[c] == edge;
+        const uint32_t votes = __ballot_sync(0xffffffffu, is);
+        if (c < tc)
+          keys[band[c]] =
+              exact[c] > edge || (is && seen + __popc(votes & below) < left) ? ~0u : 0u;
+        seen += __popc(votes);
+      }
+    }
+    Team<W>::sync();
+    // taken ones are above now, and nothing is between
+    above = min(above, ~0u - 1u);
+    least = ~0u;
+    count(&eqs, &gts, &eq_before, &gt_before);
+    ties = 0;
+    eq_before = 0;
+  }
+  // taken ones in order
+  int seen = eq_before, at = gt_before + min(eq_before, ties);
+  for (int i0 = from; i0 < to; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < to ? keys[i] : 0u;
+    const bool is_eq = ties > 0 && i < to && key >= least && key <= above;
+    const uint32_t votes = __ballot_sync(0xffffffffu, is_eq);
+    const bool take = i < to && (key > above || (is_eq && seen + __popc(votes & below) < ties));
+    const uint32_t takes = __ballot_sync(0xffffffffu, take);
+    if (take) out[p.keep_first + at + __popc(takes & below)] = p.keep_first + i;
+    seen += __popc(votes);
+    at += __popc(takes);
+  }
+}
+
+// a b with sums that begin at zero
+__device__ __forceinline__ void mma_from_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// two fp32 sums in one instruction
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr int SEL_STAGES = 3;                  // 8 blocks each of a warp's bounds under way
+constexpr int SEL_WARPS = 4;                   // of a CTA of the scores
+
+// 16 bytes into shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint4* dst, const uint16_t* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(have ? 16 : 0)
+               : "memory");
+}
+
+// ---- scores: a CTA per token (or several of one table), KV head and chunk of blocks
 //
-// Scores: sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with the positive and negative parts of
-// q, a product of 16 rows (query heads, of several tokens where they fit) by 8 blocks by 256 on the
-// tensor cores, the blocks' bounds straight from memory: a lane loads 16 bytes, which are operands of
-// two instructions when q's channels are taken in the same order.  Sums in fp32 are off by at most
-// e = 2^-15 sum |q| max |bound| (16 instructions of 17 terms, each off by at most 2^-23 of the sums
-// of absolute values: 2^-15.9).  Of the blocks between the kept ends those above the want-th largest
-// score by more than 2 e are taken, those below it by more are not, and those between are scored
-// again in 64 bits if they do not all fit.  So the choice is that of 64 bits, ties to the lower
-// index.
+// sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with the positive and negative parts of q: a
+// product of 16 rows (query heads, of several tokens where they fit) by 8 blocks by 256 on the tensor
+// cores.  A warp has 8 blocks at a time and three such on their way in shared memory; a lane copies
+// the 16-byte pieces that it uses itself, which are operands of two instructions when q's channels
+// are taken in the same order.  Sums in fp32 are off by at most e = 2^-18 sum |q| max |bound|: an
+// instruction adds 17 terms (its sum begins at zero), each off by at most 2^-23 of the sum of
+// absolute values, and a term goes through at most six further additions of 2^-24: 20 x 2^-23 =
+// 2^-18.7.
 //
-// Bounds: the bytes of the bounds when there are many tokens (8 loads of 16 bytes are under way per
-// lane, two CTAs on an SM), else the latency of the steps behind the scores.
-__global__ void __launch_bounds__(SEL_THREADS, 2) select_blocks_kernel(const SelectParams p) {
-  extern __shared__ uint64_t sel_smem[];
-  __shared__ SelectShared s;
-  uint64_t* exact = sel_smem;                                       // [most]
-  uint32_t* scores = reinterpret_cast<uint32_t*>(exact + p.most);   // [together][most], ordered
-  uint16_t* band = reinterpret_cast<uint16_t*>(scores + p.together * p.most);   // [most]
+// Bounds: the bytes of the bounds.
+__global__ void __launch_bounds__(32 * SEL_WARPS, 4)
+select_scores_kernel(const SelectParams p) {
+  __shared__ uint4 ring[SEL_WARPS * SEL_STAGES * 256];
   pdl_launch_dependents();
   pdl_wait();
   const int kvh = blockIdx.y;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = blockIdx.x / p.chunks, chunk = blockIdx.x - group * p.chunks;
   const int per = p.page / p.block;
-  auto length = [&](int token, int row) -> int {
-    const int64_t len = p.context_lens[token];
-    if (len <= 0 || row < 0 || row >= p.num_tables) return 0;
-    return (int)(len > p.capacity ? p.capacity : len);
-  };
-  auto bounds_at = [&](int page, int b) -> const uint16_t* {
-    return p.bounds + (((int64_t)page * p.hkv + kvh) * per + b % per) * 2 * SEL_D;
-  };
+  const int r0 = lane >> 2, quad = lane & 3;
 
   // runs of tokens with one table
-  const int last_token = min(p.num_tokens, ((int)blockIdx.x + 1) * p.together);
-  for (int t0 = blockIdx.x * p.together; t0 < last_token;) {
+  const int last_token = min(p.num_tokens, (group + 1) * p.together);
+  uint32_t top = 0u, low = 0u;                 // largest and smallest bound, two channels at once
+  for (int t0 = group * p.together; t0 < last_token;) {
     const int row = p.rows ? p.rows[t0] : t0;
     int t1 = t0 + 1;
     while (t1 < last_token && p.rows[t1] == row) ++t1;
-    int longest = 0;
-    bool bad = row < 0 || row >= p.num_tables;
-    for (int t = t0; t < t1; ++t) {
-      bad |= p.context_lens[t] > p.capacity;
-      longest = max(longest, length(t, row));
-    }
-    if (bad && tid == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+    int64_t longest = 0;
+    for (int t = t0; t < t1; ++t) longest = max(longest, (int64_t)p.context_lens[t]);
+    if (longest > p.capacity) longest = p.capacity;
+    if (row < 0 || row >= p.num_tables) longest = 0;
     const int32_t* table = p.tables + (int64_t)row * p.table_stride;
     // scores of blocks keep_first .. of the longest context; a shorter one uses fewer of them
-    const int blocks = (longest + p.block - 1) / p.block;
+    const int blocks = (int)((longest + p.block - 1) / p.block);
     const int scored = blocks > p.count ? blocks - p.keep_first - p.keep_last : 0;
-    if (scored > 0) {
+    const int begin = chunk * p.chunk, end = min(scored, begin + p.chunk);
+    if (begin < end) {
+      // pages of the blocks that this lane copies pieces of, three steps ahead
+      auto page_of = [&](int b0) -> int {
+        const int b = p.keep_first + b0 + r0;
+        return b0 + r0 < end ? table[p.per_shift >= 0 ? b >> p.per_shift : b / per] : -1;
+      };
+      uint32_t have = 0;                       // a bit per stage
+      auto copy = [&](int b0, int stage, int page) {
+        const bool ok = page >= 0 && page < p.num_pages;
+        if (!ok && b0 + r0 < end && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+        have = (have & ~(1u << stage)) | (ok ? 1u << stage : 0u);
+        const int b = p.keep_first + b0 + r0;
+        const int in = p.per_shift >= 0 ? b & (per - 1) : b % per;
+        const uint16_t* src =
+            p.bounds + (ok ? (((int64_t)page * p.hkv + kvh) * per + in) * 2 * SEL_D : 0) + quad * 8;
+        uint4* dst = ring + (warp * SEL_STAGES + stage) * 256 + lane;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) copy16(dst + j * 32, src + j * 32, ok);
+      };
+      constexpr int kStep = 8 * SEL_WARPS;
+      int ahead = begin + warp * 8;
+      {
+        int pages[SEL_STAGES];
+#pragma unroll
+        for (int i = 0; i < SEL_STAGES; ++i) pages[i] = page_of(ahead + i * kStep);
+#pragma unroll
+        for (int i = 0; i < SEL_STAGES; ++i, ahead += kStep) {
+          if (ahead < end) copy(ahead, i, pages[i]);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+      }
+      int next_page = page_of(ahead);
       // rows lane / 4 and lane / 4 + 8 of q, channels 32 j + 8 (lane % 4) + 0 .. 7
       uint32_t qp[4][8], qm[4][8];
-      const int r0 = lane >> 2, quad = lane & 3;
-      float abs0 = 0.f, abs1 = 0.f;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int r = r0 + half * 8, t = t0 + r / p.g;
-        const bool live = t < t1;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (live)
+          if (t < t1)
             v = *reinterpret_cast<const uint4*>(
                 p.q + (int64_t)t * p.q_stride + ((int64_t)kvh * p.g + r % p.g) * SEL_D + j * 32 +
                 quad * 8);
@@ -304,246 +569,179 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) select_blocks_kernel(const Sel
           for (int i = 0; i < 4; ++i) {
             qp[j][half * 4 + i] = max2_nan(w[i], 0u);
             qm[j][half * 4 + i] = min2_nan(w[i], 0u);
-            const float a = fabsf(bf16lo(w[i])) + fabsf(bf16hi(w[i]));
-            if (half) abs1 += a; else abs0 += a;
           }
         }
       }
-      abs0 += __shfl_xor_sync(0xffffffffu, abs0, 1); abs1 += __shfl_xor_sync(0xffffffffu, abs1, 1);
-      abs0 += __shfl_xor_sync(0xffffffffu, abs0, 2); abs1 += __shfl_xor_sync(0xffffffffu, abs1, 2);
-      if (tid < 16) s.q_sum[tid] = 0.f;
-      __syncthreads();
-      if (warp == 0 && quad == 0) {
-        // not a number counts as infinite; whole numbers order floats above zero
-        auto put = [&](int r, float a) {
-          if (r / p.g < p.together)
-            atomicMax(reinterpret_cast<int*>(&s.q_sum[r / p.g]),
-                      __float_as_int(a < INFINITY ? a : INFINITY));
-        };
-        put(r0, abs0);
-        put(r0 + 8, abs1);
-      }
-      uint32_t most = 0u;                      // largest |bound|, two channels at once
-      for (int b0 = warp * 8; b0 < scored; b0 += 8 * (SEL_THREADS / 32)) {
-        const int mine = b0 + r0, b = p.keep_first + mine;
-        int page = mine < scored ? table[b / per] : -1;
-        if (mine < scored && (page < 0 || page >= p.num_pages)) {
-          if (p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-          page = -1;
-        }
-        const bool have = page >= 0;
-        uint4 lo[4], hi[4];
-        const uint16_t* at = bounds_at(have ? page : 0, have ? b : 0) + quad * 8;
+      int stage = 0;
+      for (int b0 = begin + warp * 8; b0 < end; b0 += kStep) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(SEL_STAGES - 1) : "memory");
+        const uint4* src = ring + (warp * SEL_STAGES + stage) * 256 + lane;
+        const bool ok = have >> stage & 1u;
+        uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          hi[j] = lo[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (have) {
-            hi[j] = *reinterpret_cast<const uint4*>(at + SEL_D + j * 32);
-            lo[j] = *reinterpret_cast<const uint4*>(at + j * 32);
-          }
-        }
-        float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint4 lo = src[j * 32], hi = src[(4 + j) * 32];
+          float c[4][4];
+          mma_from_zero(c[0], qp[j][0], qp[j][4], qp[j][1], qp[j][5], hi.x, hi.y);
+          mma_from_zero(c[1], qm[j][0], qm[j][4], qm[j][1], qm[j][5], lo.x, lo.y);
+          mma_from_zero(c[2], qp[j][2], qp[j][6], qp[j][3], qp[j][7], hi.z, hi.w);
+          mma_from_zero(c[3], qm[j][2], qm[j][6], qm[j][3], qm[j][7], lo.z, lo.w);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t pa[4] = {qp[j][0], qp[j][4], qp[j][1], qp[j][5]};
-          const uint32_t pb[4] = {qp[j][2], qp[j][6], qp[j][3], qp[j][7]};
-          const uint32_t ma[4] = {qm[j][0], qm[j][4], qm[j][1], qm[j][5]};
-          const uint32_t mb[4] = {qm[j][2], qm[j][6], qm[j][3], qm[j][7]};
-          mma_bf16_16816(c0, pa, hi[j].x, hi[j].y);
-          mma_bf16_16816(c1, ma, lo[j].x, lo[j].y);
-          mma_bf16_16816(c0, pb, hi[j].z, hi[j].w);
-          mma_bf16_16816(c1, mb, lo[j].z, lo[j].w);
-          most = max2_nan(most, max2_nan(max2_nan(hi[j].x & 0x7fff7fffu, hi[j].y & 0x7fff7fffu),
-                                         max2_nan(hi[j].z & 0x7fff7fffu, hi[j].w & 0x7fff7fffu)));
-          most = max2_nan(most, max2_nan(max2_nan(lo[j].x & 0x7fff7fffu, lo[j].y & 0x7fff7fffu),
-                                         max2_nan(lo[j].z & 0x7fff7fffu, lo[j].w & 0x7fff7fffu)));
+          for (int i = 0; i < 2; ++i)
+            sum[i] = add_pair(sum[i], add_pair(add_pair(pair_of(c[0][2 * i], c[0][2 * i + 1]),
+                                                        pair_of(c[1][2 * i], c[1][2 * i + 1])),
+                                               add_pair(pair_of(c[2][2 * i], c[2][2 * i + 1]),
+                                                        pair_of(c[3][2 * i], c[3][2 * i + 1]))));
+          top = max2_nan(top, max2_nan(max2_nan(hi.x, hi.y), max2_nan(hi.z, hi.w)));
+          low = min2_nan(low, min2_nan(min2_nan(lo.x, lo.y), min2_nan(lo.z, lo.w)));
         }
+        // the stage has been read: its next blocks
+        const int page = next_page;
+        next_page = page_of(ahead + kStep);
+        if (ahead < end) copy(ahead, stage, page);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += kStep;
+        if (++stage == SEL_STAGES) stage = 0;
         // rows r0 and r0 + 8 of blocks b0 + 2 quad + 0, 1: the largest of each token's rows
-        float v[4] = {c0[0] + c1[0], c0[1] + c1[1], c0[2] + c1[2], c0[3] + c1[3]};
-        const uint32_t bads = __ballot_sync(0xffffffffu, mine < scored && !have);
+        const uint32_t bads = __ballot_sync(0xffffffffu, !ok);
+        uint32_t* scores = p.scores + ((int64_t)t0 * p.hkv + kvh) * p.most + b0;
+        float v[4];
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[0]), "=f"(v[1]) : "l"(sum[0]));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2]), "=f"(v[3]) : "l"(sum[1]));
         if (p.together == 1) {
-          if (r0 >= p.g) v[0] = v[1] = -INFINITY;
-          if (r0 + 8 >= p.g) v[2] = v[3] = -INFINITY;
-          v[0] = v[2] = fmaxf(v[0], v[2]);
-          v[1] = v[3] = fmaxf(v[1], v[3]);
-        }
-        const int across = p.together == 1 ? 8 : p.g;
-        for (int o = 1; o < across; o <<= 1) {
+          // rows of one token: a block's score is in the lanes of row 0
+          v[0] = fmaxf(r0 < p.g ? v[0] : -INFINITY, r0 + 8 < p.g ? v[2] : -INFINITY);
+          v[1] = fmaxf(r0 < p.g ? v[1] : -INFINITY, r0 + 8 < p.g ? v[3] : -INFINITY);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] = fmaxf(v[i], __shfl_xor_sync(0xffffffffu, v[i], o * 4));
-        }
-        if (r0 % across == 0) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int col = quad * 2 + (i & 1);
-            const int tq = p.together == 1 ? 0 : (r0 + (i >> 1) * 8) / p.g;
-            if ((p.together == 1 && i > 1) || b0 + col >= scored || tq >= p.together) continue;
-            scores[tq * p.most + b0 + col] = bads >> (col * 4) & 1u ? 0u : order_of(v[i]);
+          for (int o = 4; o < 32; o <<= 1) {
+            v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+            v[1] = fmaxf(v[1], __shfl_xor_sync(0xffffffffu, v[1], o));
           }
-        }
-      }
+          if (r0 == 0) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = max2_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (lane == 0) s.most[warp] = most;
-      __syncthreads();
-    }
-
-    for (int token = t0; token < t1; ++token) {
-      int32_t* out = p.selected + ((int64_t)token * p.hkv + kvh) * p.count;
-      const int n = (length(token, row) + p.block - 1) / p.block;
-      if (n <= p.count) {
-        for (int i = tid; i < p.count; i += SEL_THREADS) out[i] = i < n ? i : -1;
-        continue;
-      }
-      const int middle = n - p.keep_first - p.keep_last;
-      const int want = p.count - p.keep_first - p.keep_last;     // of the middle ones
-      for (int i = tid; i < p.keep_first; i += SEL_THREADS) out[i] = i;
-      for (int i = tid; i < p.keep_last; i += SEL_THREADS)
-        out[p.count - p.keep_last + i] = n - p.keep_last + i;
-      if (want == 0) continue;
-      uint32_t* keys = scores + (token - t0) * p.most;
-      uint32_t most = s.most[0];
-#pragma unroll
-      for (int w = 1; w < 8; ++w) most = max2_nan(most, s.most[w]);
-      const float reach = s.q_sum[token - t0] * __uint_as_float(max(most << 16, most & 0xffff0000u));
-      // scores past fp32's range, products below it, and what is not a number: all in 64 bits
-      const bool all = !(reach < INFINITY) || (reach > 0.f && reach < 7.9e-31f);
-      uint32_t above, least;                 // keys above are taken, keys below `least` are not
-      bool same = false;                     // keys between are equal in truth
-      if (all) {
-        above = ~0u; least = 0u;
-      } else {
-        // digits that all keys share need no pass
-        uint32_t lo = ~0u, hi = 0u;
-        for (int i = tid; i < middle; i += SEL_THREADS) {
-          lo = min(lo, keys[i]);
-          hi = max(hi, keys[i]);
-        }
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        hi = __reduce_max_sync(0xffffffffu, hi);
-        __syncthreads();
-        if (lane == 0) { s.lo[warp] = lo; s.hi[warp] = hi; }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 8; ++w) { lo = min(lo, s.lo[w]); hi = max(hi, s.hi[w]); }
-        const int shift = lo == hi ? 0 : (31 - __clz(lo ^ hi)) / 8 * 8;
-        const uint32_t border = border_of<uint32_t>(
-            keys, middle, want, shift, shift == 24 ? 0u : hi & ~0u << (shift + 8), s);
-        const float v = value_of(border), e2 = reach * (2.f / 32768.f);
-        same = border == 0u || reach == 0.f;
-        above = same ? border : order_of(v + e2);
-        least = same ? border : order_of(v - e2);
-      }
-      // how many are above, and between
-      int eq = 0, gt = 0;
-      const int run = ((middle + 7) / 8 + 31) / 32 * 32;       // blocks of a warp
-      const int from = min(warp * run, middle), to = min(from + run, middle);
-      for (int i = from + lane; i < to; i += 32) {
-        gt += keys[i] > above ? 1 : 0;
-        eq += keys[i] >= least && keys[i] <= above ? 1 : 0;
-      }
-      eq = __reduce_add_sync(0xffffffffu, eq);
-      gt = __reduce_add_sync(0xffffffffu, gt);
-      __syncthreads();
-      if (lane == 0) { s.eq[warp] = eq; s.gt[warp] = gt; }
-      __syncthreads();
-      int eqs = 0, gts = 0, eq_before = 0, gt_before = 0;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        if (w == warp) { eq_before = eqs; gt_before = gts; }
-        eqs += s.eq[w];
-        gts += s.gt[w];
-      }
-      int ties = want - gts;                 // of those between, the first ones if they are equal
-      if (!same && eqs > ties) {
-        // score those between again; their keys become "taken" or "not"
-        int at = eq_before;
-        for (int i0 = from; i0 < to; i0 += 32) {
-          const int i = i0 + lane;
-          const bool is = i < to && keys[i] >= least && keys[i] <= above;
-          const uint32_t votes = __ballot_sync(0xffffffffu, is);
-          if (is) band[at + __popc(votes & ((1u << lane) - 1u))] = (uint16_t)i;
-          at += __popc(votes);
-        }
-        __syncthreads();
-        for (int c = warp; c < eqs; c += 8) {
-          const int b = p.keep_first + band[c];
-          uint64_t key = 0ull;               // without a page
-          if (keys[band[c]] != 0u)
-            key = exact_score(p, token, kvh, bounds_at(table[b / per], b), lane);
-          if (lane == 0) exact[c] = key;
-        }
-        __syncthreads();
-        if (eqs <= 32) {
-          // a lane per block: its rank, the lower index first among equals
-          if (warp == 0) {
-            const uint64_t key = lane < eqs ? exact[lane] : 0ull;
-            int rank = 0;
-            for (int j = 0; j < eqs; ++j) {
-              const uint64_t other = __shfl_sync(0xffffffffu, key, j);
-              rank += other > key || (other == key && j < lane) ? 1 : 0;
-            }
-            if (lane < eqs) keys[band[lane]] = rank < ties ? ~0u : 0u;
+            for (int i = 0; i < 2; ++i)
+              if (b0 + quad * 2 + i < end)
+                scores[quad * 2 + i] = bads >> (quad * 8 + i * 4) & 1u ? 0u : order_of(v[i]);
           }
-          __syncthreads();
         } else {
-          const uint64_t edge = border_of<uint64_t>(exact, eqs, ties, 56, 0ull, s);
-          const int left = s.left;
-          // equal ones in order: a warp has a run of them, as above
-          const int run_c = ((eqs + 7) / 8 + 31) / 32 * 32;
-          const int fc = min(warp * run_c, eqs), tc = min(fc + run_c, eqs);
-          int n_eq = 0;
-          for (int c = fc + lane; c < tc; c += 32) n_eq += exact[c] == edge ? 1 : 0;
-          n_eq = __reduce_add_sync(0xffffffffu, n_eq);
-          __syncthreads();
-          if (lane == 0) s.eq[warp] = n_eq;
-          __syncthreads();
-          int seen = 0;
-          for (int w = 0; w < warp; ++w) seen += s.eq[w];
-          for (int c0 = fc; c0 < tc; c0 += 32) {
-            const int c = c0 + lane;
-            const bool is = c < tc && exact[c] == edge;
-            const uint32_t votes = __ballot_sync(0xffffffffu, is);
-            if (c < tc)
-              keys[band[c]] = exact[c] > edge ||
-                                      (is && seen + __popc(votes & ((1u << lane) - 1u)) < left)
-                                  ? ~0u : 0u;
-            seen += __popc(votes);
+          for (int o = 1; o < p.g; o <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i] = fmaxf(v[i], __shfl_xor_sync(0xffffffffu, v[i], o * 4));
           }
-          __syncthreads();
+          if (r0 % p.g == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int col = quad * 2 + (i & 1), of = (r0 + (i >> 1) * 8) / p.g;
+              if (b0 + col < end && t0 + of < t1)
+                scores[(int64_t)of * p.hkv * p.most + col] =
+                    bads >> (col * 4) & 1u ? 0u : order_of(v[i]);
+            }
+          }
         }
-        // taken ones are above now, and nothing is between
-        above = min(above, ~0u - 1u);
-        least = ~0u;
-        gt = 0;
-        for (int i = from + lane; i < to; i += 32) gt += keys[i] > above ? 1 : 0;
-        gt = __reduce_add_sync(0xffffffffu, gt);
-        __syncthreads();
-        if (lane == 0) s.gt[warp] = gt;
-        __syncthreads();
-        gt_before = 0;
-        for (int w = 0; w < warp; ++w) gt_before += s.gt[w];
-        eq_before = 0;
-        ties = 0;
       }
-      // taken ones in order
-      int seen = eq_before, at = gt_before + min(eq_before, ties);
-      for (int i0 = from; i0 < to; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t key = i < to ? keys[i] : 0u;
-        const bool is_eq = ties > 0 && i < to && key >= least && key <= above;
-        const uint32_t votes = __ballot_sync(0xffffffffu, is_eq), below = (1u << lane) - 1u;
-        const bool take = i < to && (key > above || (is_eq && seen + __popc(votes & below) < ties));
-        const uint32_t takes = __ballot_sync(0xffffffffu, take);
-        if (take) out[p.keep_first + at + __popc(takes & below)] = p.keep_first + i;
-        seen += __popc(votes);
-        at += __popc(takes);
-      }
-      __syncthreads();
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     t0 = t1;
   }
+  // the largest |bound| of either half: low <= high
+  uint32_t most = max2_nan(top, low ^ 0x80008000u);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max2_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  uint32_t* most_of = reinterpret_cast<uint32_t*>(ring);      // which has been read
+  __syncthreads();
+  if (lane == 0) most_of[warp] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < SEL_WARPS; ++w) most = max2_nan(most, most_of[w]);
+    p.largest[((int64_t)group * p.hkv + kvh) * p.chunks + chunk] =
+        __uint_as_float(max((most << 16) & 0x7fffffffu, most & 0x7fff0000u));
+  }
+}
+
+// ---- the choice: a team of W warps per token and KV head, 8 / W teams in a CTA
+//
+// Blocks above the want-th largest score by more than 2 e are taken, those below it by more are not,
+// and those between are scored again in 64 bits if they do not all fit.  So the choice is that of
+// 64 bits, ties to the lower index.
+//
+// Bounds: the latency of its steps, of which a warp has fewer instructions and a CTA the shorter
+// time: warps where there are many tokens.
+template <int W>
+__global__ void __launch_bounds__(256) select_choose_kernel(const SelectParams p) {
+  extern __shared__ __align__(16) uint8_t sel_smem[];
+  constexpr int kTeams = 8 / W;
+  __shared__ Team<W> teams[kTeams];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, team = (threadIdx.x >> 5) / W;
+  const int64_t item = (int64_t)blockIdx.x * kTeams + team;
+  if (item >= (int64_t)p.num_tokens * p.hkv) return;
+  const int token = (int)(item / p.hkv), kvh = (int)(item - (int64_t)token * p.hkv);
+  const int row = p.rows ? p.rows[token] : token;
+  int64_t len = p.context_lens[token];
+  if (row < 0 || row >= p.num_tables || len > p.capacity) {
+    if (Team<W>::rank() == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+    len = row < 0 || row >= p.num_tables ? 0 : p.capacity;
+  }
+  const int n = (int)((max(len, (int64_t)0) + p.block - 1) / p.block);
+  // [teams][most] each
+  uint64_t* exact = reinterpret_cast<uint64_t*>(sel_smem) + team * p.most;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(sel_smem + (size_t)kTeams * p.most * 8) +
+                   team * p.most;
+  uint16_t* band = reinterpret_cast<uint16_t*>(sel_smem + (size_t)kTeams * p.most * 12) +
+                   team * p.most;
+  float reach = 0.f;
+  if (n > p.count) {
+    const int middle = n - p.keep_first - p.keep_last;
+    const uint32_t* src = p.scores + item * p.most;
+    for (int i = Team<W>::rank(); i < middle; i += 32 * W) keys[i] = src[i];
+    // largest |bound|, and the largest sum of |q| of a query head; no number counts as infinite
+    const float* from = p.largest + ((int64_t)(token / p.together) * p.hkv + kvh) * p.chunks;
+    float largest = 0.f;
+    for (int i = lane; i < p.chunks; i += 32)
+      largest = fmaxf(largest, from[i] < INFINITY ? from[i] : INFINITY);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const uint16_t* q = p.q + (int64_t)token * p.q_stride + (int64_t)kvh * p.g * SEL_D + lane * 4;
+    for (int h = 0; h < p.g; ++h) {
+      const uint2 v = *reinterpret_cast<const uint2*>(q + h * SEL_D);
+      float a = fabsf(bf16lo(v.x)) + fabsf(bf16hi(v.x)) + fabsf(bf16lo(v.y)) + fabsf(bf16hi(v.y));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      reach = fmaxf(reach, a < INFINITY ? a : INFINITY);
+    }
+    reach *= largest;
+    Team<W>::sync();
+  }
+  choose<W>(p, token, kvh, n, p.tables + (int64_t)row * p.table_stride, keys, reach, exact, band,
+            teams[team]);
+}
+
+// Groups of tokens that share products, and what is in a workspace.
+struct SelectLayout {
+  int together, chunk, chunks;
+  int64_t groups;
+  size_t largest, total;              // bytes
+};
+static SelectLayout select_layout(int64_t tokens, int hkv, int g, bool rows, int64_t most) {
+  SelectLayout s;
+  // Tokens that may have one table share the scores' products, as far as their query heads fill the
+  // 16 rows.
+  s.together = 1;
+  if (rows && (g & (g - 1)) == 0)
+    while (s.together * 2 * g <= 16) s.together *= 2;
+  s.groups = (tokens + s.together - 1) / s.together;
+  // Long chunks for the pipeline's sake, unless that leaves SMs without work.
+  s.chunk = 256;
+  while (s.chunk > 32 && s.groups * hkv * ((most + s.chunk - 1) / s.chunk) < 4ll * sm_count())
+    s.chunk /= 2;
+  s.chunks = (int)((most + s.chunk - 1) / s.chunk);
+  s.largest = ((size_t)tokens * hkv * most * 4 + 255) & ~size_t(255);
+  s.total = s.largest + (size_t)s.groups * hkv * s.chunks * 4;
+  return s;
 }
 
 // what the entry points of this file have in common
@@ -609,13 +807,26 @@ int fk_key_bounds(const void* k_cache, int64_t num_pages, int page_size, int64_t
   return FK_OK;
 }
 
+size_t fk_select_blocks_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads,
+                                        int page_size, int block, int64_t block_table_cols) {
+  if (num_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads ||
+      block <= 0 || page_size < block || block_table_cols <= 0)
+    return 0;
+  // the larger of both ways to group tokens
+  const int64_t most = block_table_cols * (page_size / block);
+  const int g = num_q_heads / num_kv_heads;
+  const size_t a = select_layout(num_tokens, num_kv_heads, g, false, most).total;
+  const size_t b = select_layout(num_tokens, num_kv_heads, g, true, most).total;
+  return a > b ? a : b;
+}
+
 int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, int64_t num_pages,
                      int page_size, int block, const int32_t* context_lens,
                      const int32_t* table_rows, const int32_t* block_tables,
                      int64_t block_table_stride, int64_t block_table_cols, int num_tables,
                      int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int count,
-                     int keep_first, int keep_last, int32_t* selected, int32_t* status,
-                     fk_stream_t stream) {
+                     int keep_first, int keep_last, int32_t* selected, void* workspace,
+                     size_t workspace_bytes, int32_t* status, fk_stream_t stream) {
   FK_REQUIRE(num_tokens >= 0, FK_ERR_INVALID_ARG, "fk_select_blocks: negative size");
   if (num_tokens == 0) return FK_OK;
   FK_REQUIRE(q && bounds && context_lens && block_tables && selected, FK_ERR_INVALID_ARG,
@@ -654,19 +865,35 @@ int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, 
   p.hkv = num_kv_heads; p.g = num_q_heads / num_kv_heads;
   p.count = count; p.keep_first = keep_first; p.keep_last = keep_last;
   p.most = (int)most;
-  // Tokens that may have one table share the scores' products, as far as their query heads fill the
-  // 16 rows and 32 KiB of scores leave several CTAs on an SM.
-  p.together = 1;
-  if (table_rows != nullptr && (p.g & (p.g - 1)) == 0)
-    while (p.together * 2 * p.g <= 16 && p.together * 2 * most * 4 <= 32768) p.together *= 2;
+  const int per = page_size / block;
+  p.per_shift = (per & (per - 1)) == 0 ? __builtin_ctz(per) : -1;
   p.selected = selected;
   p.status = status;
-  const int64_t ctas = ((int64_t)num_tokens + p.together - 1) / p.together;
-  const size_t smem = (size_t)most * (8 + 4 * (size_t)p.together + 2) + 16;
-  static PerDeviceOnce once;
-  FK_CUDA_OK(set_max_dynamic_smem(once, select_blocks_kernel, SEL_MAX_BLOCKS * 14 + 16));
-  FK_CUDA_OK(launch_kernel(select_blocks_kernel, dim3((unsigned)ctas, (unsigned)num_kv_heads),
-                           dim3(SEL_THREADS), smem, static_cast<cudaStream_t>(stream), p));
+  const SelectLayout w =
+      select_layout(num_tokens, num_kv_heads, p.g, table_rows != nullptr, most);
+  FK_REQUIRE(workspace != nullptr && workspace_bytes >= w.total &&
+                 (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
+             FK_ERR_WORKSPACE,
+             "fk_select_blocks: workspace needs %zu bytes, 256-byte aligned (got %zu)", w.total,
+             workspace_bytes);
+  FK_REQUIRE(w.groups * w.chunks < (1ll << 31), FK_ERR_UNSUPPORTED,
+             "fk_select_blocks: too many tokens");
+  p.together = w.together; p.chunk = w.chunk; p.chunks = w.chunks;
+  p.scores = static_cast<uint32_t*>(workspace);
+  p.largest = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + w.largest);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  FK_CUDA_OK(launch_kernel(select_scores_kernel,
+                           dim3((unsigned)(w.groups * w.chunks), (unsigned)num_kv_heads),
+                           dim3(32 * SEL_WARPS), (size_t)0, s, p));
+  const int64_t items = (int64_t)num_tokens * num_kv_heads;
+  const bool many = items >= 16ll * sm_count() && most <= SEL_WARP_BLOCKS;
+  static PerDeviceOnce once[2];
+  auto kernel = many ? select_choose_kernel<1> : select_choose_kernel<8>;
+  FK_CUDA_OK(set_max_dynamic_smem(once[many], kernel,
+                                  (many ? 8 * SEL_WARP_BLOCKS : SEL_MAX_BLOCKS) * 14));
+  FK_CUDA_OK(launch_kernel(kernel, dim3((unsigned)(many ? (items + 7) / 8 : items)), dim3(256),
+                           (size_t)most * 14 * (many ? 8 : 1), s, p));
+  count_launch(1);
   count_launch(1);
   return FK_OK;
 }

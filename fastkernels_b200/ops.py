@@ -439,8 +439,14 @@ def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new
     return bounds
 
 
+def select_blocks_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, page_size, block,
+                                  table_cols) -> int:
+    return int(lib.fk_select_blocks_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, page_size,
+                                                    block, table_cols))
+
+
 def select_blocks(q, bounds, context_lens, block_tables, block, count, keep_first=1, keep_last=1,
-                  table_rows=None, out=None, status=None):
+                  table_rows=None, workspace=None, out=None, status=None):
     """Blocks of `block` tokens for each query token and KV head, int32 [tokens, Hkv, count] in
     ascending order, -1 behind the last: the first keep_first, the last keep_last (the last of all
     holds the token itself), and those whose bounds allow the largest logit of any query head of
@@ -464,10 +470,13 @@ def select_blocks(q, bounds, context_lens, block_tables, block, count, keep_firs
     _need_here(out, torch.int32, "out")
     if tuple(out.shape) != (n, hkv, count) or not out.is_contiguous():
         raise _lib.FkError("out must be a contiguous [tokens, Hkv, count]")
+    workspace = _workspace(workspace, select_blocks_workspace_bytes(n, hq, hkv, per * block, block,
+                                                                    cols), q)
     check(lib.fk_select_blocks(
         _ptr(q), qs, _ptr(bounds), pages, per * block, block, _ptr(context_lens),
         _ptr(table_rows), _ptr(block_tables), ts, cols, rows, n, hq, hkv, d, int(count),
-        int(keep_first), int(keep_last), _ptr(out), _status_ptr(status, q), _stream()),
+        int(keep_first), int(keep_last), _ptr(out), _ptr(workspace),
+        workspace.numel() * workspace.element_size(), _status_ptr(status, q), _stream()),
         "fk_select_blocks")
     return out
 

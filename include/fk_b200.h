@@ -211,7 +211,8 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  * keep_last (>= 1: the block that holds the token itself, whose bounds are not
  * read) and those with the largest
  *   max over the query heads h of the KV head of sum_d max(q_hd lo_d, q_hd hi_d),
- * count in all, the lower index on ties, -1 behind the last where n < count.  The
+ * (lo_d <= hi_d), count in all, the lower index on ties, -1 behind the last where
+ * n < count.  The
  * choice is that of 64-bit sums.  A score that is no number counts as the largest,
  * a block whose page id is bad as the smallest.  table_rows[i] is the table of token
  * i (NULL: i itself), so several tokens of a prompt may select with one table.
@@ -241,13 +242,16 @@ int fk_key_bounds(const void* k_cache, int64_t num_pages, int page_size, int64_t
                   int64_t block_table_stride, int64_t block_table_cols, const int32_t* cu_new,
                   int num_seqs, int max_new, int32_t* status, fk_stream_t stream);
 
+size_t fk_select_blocks_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads,
+                                        int page_size, int block, int64_t block_table_cols);
+
 int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, int64_t num_pages,
                      int page_size, int block, const int32_t* context_lens,
                      const int32_t* table_rows, const int32_t* block_tables,
                      int64_t block_table_stride, int64_t block_table_cols, int num_tables,
                      int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int count,
-                     int keep_first, int keep_last, int32_t* selected, int32_t* status,
-                     fk_stream_t stream);
+                     int keep_first, int keep_last, int32_t* selected, void* workspace,
+                     size_t workspace_bytes, int32_t* status, fk_stream_t stream);
 
 size_t fk_selected_attn_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads,
                                         int head_dim, int count, int block);

@@ -148,6 +148,16 @@ def test_select_rows_of_a_portion(ops):
     check_select(ops, q, bounds, lens, table, 32, 6, 1, 1, rows)
 
 
+@pytest.mark.parametrize("hq,hkv,n", [(8, 8, 301), (32, 4, 640), (10, 10, 250)])
+def test_select_many_tokens(ops, hq, hkv, n):
+    """As many tokens as let a warp choose for each; groups of tokens that end with a table."""
+    rows = [0] * 37 + [1] * (n - 38) + [2]
+    rng, q, bounds, table = select_case(hq + n, n, hq, hkv, 64, 16, 1500, rows)
+    lens = rng.integers(1, 1501, n)
+    q[5:9] = 0                                     # padded tokens
+    check_select(ops, q, bounds, lens, table, 16, 9, 1, 2, rows)
+
+
 @pytest.mark.parametrize("what", ["few values", "one block", "zero query", "equal blocks"])
 def test_select_takes_the_first_of_equals(ops, what):
     rng, q, bounds, table = select_case(13, 4, 8, 2, 64, 64, 64 * 700)

@@ -37,10 +37,10 @@ def bounds(**kw):
 
 def select(**kw):
     names = "q qs bounds num_pages page block lens rows tables ts cols num_tables n hq hkv d count " \
-            "first last sel status stream".split()
+            "first last sel ws wsb status stream".split()
     return call(L.fk_select_blocks, names,
                 dict(CACHE, q=P, qs=1024, bounds=P, block=64, rows=None, num_tables=3, n=3, hq=8,
-                     hkv=2, d=128, count=4, first=1, last=1, sel=P), kw)
+                     hkv=2, d=128, count=4, first=1, last=1, sel=P, ws=P, wsb=1 << 30), kw)
 
 
 def attend(**kw):
@@ -108,6 +108,11 @@ def test_select_refusals():
     assert select(num_tables=2) == INVALID and "tables" in err()
     assert select(cols=16385) == UNSUPPORTED and "16384" in err()
     assert select(sel=None) == INVALID and select(bounds=None) == INVALID
+    need = L.fk_select_blocks_workspace_bytes(3, 8, 2, 64, 64, 4)
+    assert need >= 3 * 2 * 4 * 4
+    assert select(wsb=16) == WORKSPACE and select(ws=None) == WORKSPACE
+    assert select(ws=P + 16) == WORKSPACE and "aligned" in err()
+    assert L.fk_select_blocks_workspace_bytes(3, 8, 2, 64, 128, 4) == 0
 
 
 def test_attend_refusals():
@@ -187,7 +192,8 @@ def test_prototypes_fit_the_header():
     kinds = {"int": ctypes.c_int, "int64_t": ctypes.c_int64, "float": ctypes.c_float,
              "size_t": ctypes.c_size_t}
     for name in ("fk_key_bounds", "fk_select_blocks", "fk_selected_attn", "fk_shared_prefix_attn",
-                 "fk_selected_attn_workspace_bytes", "fk_shared_prefix_workspace_bytes"):
+                 "fk_selected_attn_workspace_bytes", "fk_select_blocks_workspace_bytes",
+                 "fk_shared_prefix_workspace_bytes"):
         args = re.search(rf"\b{name}\s*\(([^)]*)\)", text).group(1).split(",")
         want = [ctypes.c_void_p if "*" in a or "fk_stream_t" in a else kinds[a.split()[0]]
                 for a in args]
