@@ -128,11 +128,13 @@ struct SelectParams {
   int num_tokens, num_tables, num_pages, page, block, hkv, g;
   int count, keep_first, keep_last;
   int per_shift;                      // log2 of the blocks of a page, -1: no power of two
-  int together;                       // tokens of a CTA: 1, or up to 16 / g (a power of two)
+  int together;                       // tokens of a CTA: 1, or 16 / g
+  int g_shift;                        // log2 of g where that is 16 / g
   int most;                           // blocks that a table's row has pages for
   int chunk, chunks;                  // blocks of a CTA of the scores, of those CTAs per token
   uint32_t* scores;                   // [tokens, hkv, most], ordered
   float* largest;                     // [groups of tokens, hkv, chunks] largest |bound| of a chunk
+  float* q_sum;                       // [tokens, hkv] largest sum of |q| of a query head
   int32_t* selected;                  // [tokens, hkv, count]
   int32_t* status;
 };
@@ -145,6 +147,7 @@ __device__ __forceinline__ uint64_t order_of(double v) {
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 __device__ __forceinline__ uint32_t order_of(float v) {
+  if (v != v) return ~0u;
   const uint32_t b = __float_as_uint(v + 0.0f);
   return b >> 31 ? ~b : b | (1u << 31);
 }
@@ -168,11 +171,12 @@ struct Team {
   }
 };
 
-// The want-th largest of n keys (1 <= want <= n), and how many of the keys that equal it are among the
+// The want-th largest of n keys (1 <= want <= n), the largest one, and how many of the keys that equal it are among the
 // want largest.  Counts of 256 parts of the range of keys leave one part, which is the range of
 // the next round, until 32 keys are left, which are ranked, or all that are left are equal.
 template <int W, typename KEY>
-__device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int* left, Team<W>& s) {
+__device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int* left, KEY* most,
+                                         Team<W>& s) {
   const int tid = Team<W>::rank(), lane = threadIdx.x & 31;
   constexpr int kBits = 8 * sizeof(KEY);
   KEY lo = (KEY)~(KEY)0, hi = 0;
@@ -194,6 +198,7 @@ __device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int* 
       hi = max(hi, (KEY)s.hi[w]);
     }
   }
+  *most = hi;
   while (lo != hi) {
     const int used = kBits - (kBits == 64 ? __clzll((long long)(hi - lo)) : __clz((int)(hi - lo)));
     const int shift = max(0, used - 8);
@@ -334,16 +339,18 @@ __device__ __forceinline__ void choose(const SelectParams& p, int token, int kvh
     out[p.count - p.keep_last + i] = n - p.keep_last + i;
   if (want == 0) return;
   // scores past fp32's range, products below it, and what is no number: all in 64 bits
-  const bool all = !(reach < INFINITY) || (reach > 0.f && reach < 7.9e-31f);
+  bool all = !(reach < INFINITY) || (reach > 0.f && reach < 7.9e-31f);
   uint32_t above = ~0u, least = 0u;            // keys above are taken, keys below `least` are not
   bool same = false;                           // keys between are equal in truth
   if (!all) {
     int left;
-    const uint32_t border = border_of<W, uint32_t>(keys, middle, want, &left, s);
+    uint32_t most;                             // the largest key
+    const uint32_t border = border_of<W, uint32_t>(keys, middle, want, &left, &most, s);
+    all = most == ~0u;
     const float v = value_of(border), e2 = reach * (2.f / 262144.f);
-    same = border == 0u || reach == 0.f;
-    above = same ? border : order_of(v + e2);
-    least = same ? border : order_of(v - e2);
+    same = !all && (border == 0u || reach == 0.f);
+    above = all ? ~0u : same ? border : order_of(v + e2);
+    least = all ? 0u : same ? border : order_of(v - e2);
   }
   // how many are above, and between; each warp has a run of blocks
   const int run = ((middle + W - 1) / W + 31) / 32 * 32;
@@ -404,7 +411,8 @@ __device__ __forceinline__ void choose(const SelectParams& p, int token, int kvh
       if (warp == 0 && lane < eqs) keys[band[lane]] = rank < ties ? ~0u : 0u;
     } else {
       int left;
-      const uint64_t edge = border_of<W, uint64_t>(exact, eqs, ties, &left, s);
+      uint64_t most;
+      const uint64_t edge = border_of<W, uint64_t>(exact, eqs, ties, &left, &most, s);
       // equal ones in order: a warp has a run of them, as above
       const int run_c = ((eqs + W - 1) / W + 31) / 32 * 32;
       const int fc = min(warp * run_c, eqs), tc = min(fc + run_c, eqs);
@@ -459,6 +467,12 @@ __device__ __forceinline__ void mma_from_zero(float (&d)[4], uint32_t a0, uint32
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+// the larger one, or no number where either is none
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // two fp32 sums in one instruction
 __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   uint64_t d;
@@ -471,8 +485,9 @@ __device__ __forceinline__ uint64_t pair_of(float a, float b) {
   return r;
 }
 
-constexpr int SEL_STAGES = 3;                  // 8 blocks each of a warp's bounds under way
+constexpr int SEL_STAGES = 2;                  // 16 blocks each of a warp's bounds under way
 constexpr int SEL_WARPS = 4;                   // of a CTA of the scores
+constexpr int SEL_RING_BYTES = SEL_WARPS * SEL_STAGES * 16 * 32 * 16;
 
 // 16 bytes into shared memory, or zeros.
 __device__ __forceinline__ void copy16(uint4* dst, const uint16_t* src, bool have) {
@@ -484,18 +499,21 @@ __device__ __forceinline__ void copy16(uint4* dst, const uint16_t* src, bool hav
 // ---- scores: a CTA per token (or several of one table), KV head and chunk of blocks
 //
 // sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with the positive and negative parts of q: a
-// product of 16 rows (query heads, of several tokens where they fit) by 8 blocks by 256 on the tensor
-// cores.  A warp has 8 blocks at a time and three such on their way in shared memory; a lane copies
-// the 16-byte pieces that it uses itself, which are operands of two instructions when q's channels
-// are taken in the same order.  Sums in fp32 are off by at most e = 2^-18 sum |q| max |bound|: an
-// instruction adds 17 terms (its sum begins at zero), each off by at most 2^-23 of the sum of
-// absolute values, and a term goes through at most six further additions of 2^-24: 20 x 2^-23 =
-// 2^-18.7.
+// product of 16 blocks by 8 or 16 columns (query heads, of several tokens where they fit) by 256 on
+// the tensor cores.  A warp has 16 blocks at a time and as many on their way in shared memory; a lane
+// copies the 16-byte pieces that it uses itself, which are operands of two instructions when q's
+// channels are taken in the same order.  Sums in fp32 are off by at most e = 2^-18 sum |q| max
+// |bound|: an instruction adds 17 terms (its sum begins at zero), each off by at most 2^-23 of the
+// sum of absolute values, and a term goes through at most six further additions of 2^-24: 20 x
+// 2^-23 = 2^-18.7.
 //
-// Bounds: the bytes of the bounds.
-__global__ void __launch_bounds__(32 * SEL_WARPS, 4)
+// Bounds: the bytes of the bounds, and the instructions around the products.  (Blocks as the 8
+// columns of a product, heads as its 16 rows, took twice as many of them.)
+template <int NT>                              // 8 columns each
+__global__ void __launch_bounds__(32 * SEL_WARPS, 3)
 select_scores_kernel(const SelectParams p) {
-  __shared__ uint4 ring[SEL_WARPS * SEL_STAGES * 256];
+  extern __shared__ __align__(16) uint8_t sel_smem[];
+  uint4* ring = reinterpret_cast<uint4*>(sel_smem);
   pdl_launch_dependents();
   pdl_wait();
   const int kvh = blockIdx.y;
@@ -504,178 +522,232 @@ select_scores_kernel(const SelectParams p) {
   const int per = p.page / p.block;
   const int r0 = lane >> 2, quad = lane & 3;
 
+  // tables and lengths of the group's tokens, a lane each
+  const int first_token = group * p.together;
+  const int tokens = min(p.together, p.num_tokens - first_token);
+  int my_row = -1, my_len = 0;
+  if (lane < tokens) {
+    my_row = p.rows ? p.rows[first_token + lane] : first_token + lane;
+    const int64_t len = p.context_lens[first_token + lane];
+    my_len = (int)(len > p.capacity ? p.capacity : len < 0 ? 0 : len);
+    if (my_row < 0 || my_row >= p.num_tables) my_len = 0;
+  }
+  // The largest upper bound and the smallest lower one, two channels at once, from below and above zero:
+  // bits of bf16 as signed numbers order those above zero, and as unsigned ones those below it, the
+  // most negative last.  (A bound that is no number makes a score that is none.)
+  uint32_t top = 0u, low = 0x80008000u;
   // runs of tokens with one table
-  const int last_token = min(p.num_tokens, (group + 1) * p.together);
-  uint32_t top = 0u, low = 0u;                 // largest and smallest bound, two channels at once
-  for (int t0 = group * p.together; t0 < last_token;) {
-    const int row = p.rows ? p.rows[t0] : t0;
-    int t1 = t0 + 1;
-    while (t1 < last_token && p.rows[t1] == row) ++t1;
-    int64_t longest = 0;
-    for (int t = t0; t < t1; ++t) longest = max(longest, (int64_t)p.context_lens[t]);
-    if (longest > p.capacity) longest = p.capacity;
-    if (row < 0 || row >= p.num_tables) longest = 0;
+  for (int i0 = 0; i0 < tokens;) {
+    const int row = __shfl_sync(0xffffffffu, my_row, i0);
+    const uint32_t others =
+        __ballot_sync(0xffffffffu, lane >= tokens || my_row != row) & (~0u << i0);
+    const int i1 = others ? __ffs(others) - 1 : 32;
+    const int t0 = first_token + i0, t1 = first_token + i1;
+    const int longest = __reduce_max_sync(0xffffffffu, lane >= i0 && lane < i1 ? my_len : 0);
+    i0 = i1;
     const int32_t* table = p.tables + (int64_t)row * p.table_stride;
     // scores of blocks keep_first .. of the longest context; a shorter one uses fewer of them
-    const int blocks = (int)((longest + p.block - 1) / p.block);
+    const int blocks = (int)(((int64_t)longest + p.block - 1) / p.block);
     const int scored = blocks > p.count ? blocks - p.keep_first - p.keep_last : 0;
     const int begin = chunk * p.chunk, end = min(scored, begin + p.chunk);
-    if (begin < end) {
-      // pages of the blocks that this lane copies pieces of, three steps ahead
-      auto page_of = [&](int b0) -> int {
-        const int b = p.keep_first + b0 + r0;
-        return b0 + r0 < end ? table[p.per_shift >= 0 ? b >> p.per_shift : b / per] : -1;
-      };
-      uint32_t have = 0;                       // a bit per stage
-      auto copy = [&](int b0, int stage, int page) {
+    if (begin >= end) continue;
+    // pages of the two blocks that this lane copies pieces of
+    auto page_of = [&](int at) -> int {
+      const int b = p.keep_first + at;
+      return at < end ? table[p.per_shift >= 0 ? b >> p.per_shift : b / per] : -1;
+    };
+    uint32_t have = 0;                         // two bits per stage
+    auto copy = [&](int b0, int stage, int page0, int page1) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int page = half ? page1 : page0, at = b0 + half * 8 + r0;
         const bool ok = page >= 0 && page < p.num_pages;
-        if (!ok && b0 + r0 < end && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-        have = (have & ~(1u << stage)) | (ok ? 1u << stage : 0u);
-        const int b = p.keep_first + b0 + r0;
+        if (!ok && at < end && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+        const uint32_t bit = 1u << (stage * 2 + half);
+        have = ok ? have | bit : have & ~bit;
+        const int b = p.keep_first + at;
         const int in = p.per_shift >= 0 ? b & (per - 1) : b % per;
         const uint16_t* src =
             p.bounds + (ok ? (((int64_t)page * p.hkv + kvh) * per + in) * 2 * SEL_D : 0) + quad * 8;
-        uint4* dst = ring + (warp * SEL_STAGES + stage) * 256 + lane;
+        uint4* dst = ring + ((warp * SEL_STAGES + stage) * 16 + half * 8) * 32 + lane;
 #pragma unroll
         for (int j = 0; j < 8; ++j) copy16(dst + j * 32, src + j * 32, ok);
-      };
-      constexpr int kStep = 8 * SEL_WARPS;
-      int ahead = begin + warp * 8;
-      {
-        int pages[SEL_STAGES];
+      }
+    };
+    constexpr int kStep = 16 * SEL_WARPS;
+    int ahead = begin + warp * 16;
 #pragma unroll
-        for (int i = 0; i < SEL_STAGES; ++i) pages[i] = page_of(ahead + i * kStep);
+    for (int i = 0; i < SEL_STAGES; ++i, ahead += kStep) {
+      if (ahead < end) copy(ahead, i, page_of(ahead + r0), page_of(ahead + 8 + r0));
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int page0 = page_of(ahead + r0), page1 = page_of(ahead + 8 + r0);
+    // column lane / 4 of 8: a query head of a token; channels 32 j + 8 (lane % 4) + 0 .. 7
+    uint32_t qp[NT][4][4], qm[NT][4][4];
+    float abs_sum[NT];
 #pragma unroll
-        for (int i = 0; i < SEL_STAGES; ++i, ahead += kStep) {
-          if (ahead < end) copy(ahead, i, pages[i]);
-          asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + r0;
+      const int t = t0 + (p.together == 1 ? (col < p.g ? 0 : 1) : col >> p.g_shift);
+      const int head = p.together == 1 ? col : col & (p.g - 1);
+      abs_sum[nt] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (t < t1)
+          v = *reinterpret_cast<const uint4*>(
+              p.q + (int64_t)t * p.q_stride + ((int64_t)kvh * p.g + head) * SEL_D + j * 32 + quad * 8);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          qp[nt][j][i] = max2_nan(w[i], 0u);
+          qm[nt][j][i] = min2_nan(w[i], 0u);
+          abs_sum[nt] += fabsf(bf16lo(w[i])) + fabsf(bf16hi(w[i]));
         }
       }
-      int next_page = page_of(ahead);
-      // rows lane / 4 and lane / 4 + 8 of q, channels 32 j + 8 (lane % 4) + 0 .. 7
-      uint32_t qp[4][8], qm[4][8];
+    }
+    if (chunk == 0 && warp == 0) {
+      // the largest sum of |q| of each token's heads; no number counts as infinite
+      float mine[NT];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = r0 + half * 8, t = t0 + r / p.g;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (t < t1)
-            v = *reinterpret_cast<const uint4*>(
-                p.q + (int64_t)t * p.q_stride + ((int64_t)kvh * p.g + r % p.g) * SEL_D + j * 32 +
-                quad * 8);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            qp[j][half * 4 + i] = max2_nan(w[i], 0u);
-            qm[j][half * 4 + i] = min2_nan(w[i], 0u);
-          }
-        }
+      for (int nt = 0; nt < NT; ++nt) {
+        float a = abs_sum[nt];
+        a += __shfl_xor_sync(0xffffffffu, a, 1);
+        a += __shfl_xor_sync(0xffffffffu, a, 2);
+        mine[nt] = a < INFINITY ? a : INFINITY;
       }
-      int stage = 0;
-      for (int b0 = begin + warp * 8; b0 < end; b0 += kStep) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(SEL_STAGES - 1) : "memory");
-        const uint4* src = ring + (warp * SEL_STAGES + stage) * 256 + lane;
-        const bool ok = have >> stage & 1u;
-        uint64_t sum[2] = {0ull, 0ull};
+      for (int t = t0; t < t1; ++t) {
+        float best = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 lo = src[j * 32], hi = src[(4 + j) * 32];
+        for (int nt = 0; nt < NT; ++nt)
+          if (p.together == 1 || t0 + ((nt * 8 + r0) >> p.g_shift) == t)
+            best = fmaxf(best, mine[nt]);
+        best = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(best)));
+        if (lane == 0) p.q_sum[(int64_t)t * p.hkv + kvh] = best;
+      }
+    }
+    int stage = 0;
+    for (int b0 = begin + warp * 16; b0 < end; b0 += kStep) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(SEL_STAGES - 1) : "memory");
+      const uint4* src = ring + (warp * SEL_STAGES + stage) * 512 + lane;
+      uint64_t sum[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = 0ull;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 l0 = src[j * 32], u0 = src[(4 + j) * 32];            // block r0
+        const uint4 l1 = src[(8 + j) * 32], u1 = src[(12 + j) * 32];     // block r0 + 8
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
           float c[4][4];
-          mma_from_zero(c[0], qp[j][0], qp[j][4], qp[j][1], qp[j][5], hi.x, hi.y);
-          mma_from_zero(c[1], qm[j][0], qm[j][4], qm[j][1], qm[j][5], lo.x, lo.y);
-          mma_from_zero(c[2], qp[j][2], qp[j][6], qp[j][3], qp[j][7], hi.z, hi.w);
-          mma_from_zero(c[3], qm[j][2], qm[j][6], qm[j][3], qm[j][7], lo.z, lo.w);
+          mma_from_zero(c[0], u0.x, u1.x, u0.y, u1.y, qp[nt][j][0], qp[nt][j][1]);
+          mma_from_zero(c[1], l0.x, l1.x, l0.y, l1.y, qm[nt][j][0], qm[nt][j][1]);
+          mma_from_zero(c[2], u0.z, u1.z, u0.w, u1.w, qp[nt][j][2], qp[nt][j][3]);
+          mma_from_zero(c[3], l0.z, l1.z, l0.w, l1.w, qm[nt][j][2], qm[nt][j][3]);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            sum[i] = add_pair(sum[i], add_pair(add_pair(pair_of(c[0][2 * i], c[0][2 * i + 1]),
-                                                        pair_of(c[1][2 * i], c[1][2 * i + 1])),
-                                               add_pair(pair_of(c[2][2 * i], c[2][2 * i + 1]),
-                                                        pair_of(c[3][2 * i], c[3][2 * i + 1]))));
-          top = max2_nan(top, max2_nan(max2_nan(hi.x, hi.y), max2_nan(hi.z, hi.w)));
-          low = min2_nan(low, min2_nan(min2_nan(lo.x, lo.y), min2_nan(lo.z, lo.w)));
+            sum[nt][i] = add_pair(
+                sum[nt][i], add_pair(add_pair(pair_of(c[0][2 * i], c[0][2 * i + 1]),
+                                              pair_of(c[1][2 * i], c[1][2 * i + 1])),
+                                     add_pair(pair_of(c[2][2 * i], c[2][2 * i + 1]),
+                                              pair_of(c[3][2 * i], c[3][2 * i + 1]))));
         }
-        // the stage has been read: its next blocks
-        const int page = next_page;
-        next_page = page_of(ahead + kStep);
-        if (ahead < end) copy(ahead, stage, page);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        ahead += kStep;
-        if (++stage == SEL_STAGES) stage = 0;
-        // rows r0 and r0 + 8 of blocks b0 + 2 quad + 0, 1: the largest of each token's rows
-        const uint32_t bads = __ballot_sync(0xffffffffu, !ok);
-        uint32_t* scores = p.scores + ((int64_t)t0 * p.hkv + kvh) * p.most + b0;
-        float v[4];
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[0]), "=f"(v[1]) : "l"(sum[0]));
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2]), "=f"(v[3]) : "l"(sum[1]));
-        if (p.together == 1) {
-          // rows of one token: a block's score is in the lanes of row 0
-          v[0] = fmaxf(r0 < p.g ? v[0] : -INFINITY, r0 + 8 < p.g ? v[2] : -INFINITY);
-          v[1] = fmaxf(r0 < p.g ? v[1] : -INFINITY, r0 + 8 < p.g ? v[3] : -INFINITY);
+        top = __vimax3_s16x2(top, u0.x, u0.y); top = __vimax3_s16x2(top, u0.z, u0.w);
+        top = __vimax3_s16x2(top, u1.x, u1.y); top = __vimax3_s16x2(top, u1.z, u1.w);
+        low = __vimax3_u16x2(low, l0.x, l0.y); low = __vimax3_u16x2(low, l0.z, l0.w);
+        low = __vimax3_u16x2(low, l1.x, l1.y); low = __vimax3_u16x2(low, l1.z, l1.w);
+      }
+      const bool ok0 = have >> (stage * 2) & 1u, ok1 = have >> (stage * 2 + 1) & 1u;
+      // the stage has been read: its next blocks
+      const int now0 = page0, now1 = page1;
+      page0 = page_of(ahead + kStep + r0);
+      page1 = page_of(ahead + kStep + 8 + r0);
+      if (ahead < end) copy(ahead, stage, now0, now1);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ahead += kStep;
+      if (++stage == SEL_STAGES) stage = 0;
+      // columns 2 quad + 0, 1 of blocks r0 (v[0], v[1]) and r0 + 8: the largest of a token's
+      float v[NT][4];
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
-            v[1] = fmaxf(v[1], __shfl_xor_sync(0xffffffffu, v[1], o));
+      for (int nt = 0; nt < NT; ++nt) {
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[nt][0]), "=f"(v[nt][1]) : "l"(sum[nt][0]));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[nt][2]), "=f"(v[nt][3]) : "l"(sum[nt][1]));
+      }
+      uint32_t* scores = p.scores + ((int64_t)t0 * p.hkv + kvh) * p.most + b0 + r0;
+      const bool in0 = b0 + r0 < end, in1 = b0 + 8 + r0 < end;
+      if (p.together == 1) {
+        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const bool live = nt * 8 + quad * 2 + i < p.g;
+            m0 = max_nan(m0, live ? v[nt][i] : -INFINITY);
+            m1 = max_nan(m1, live ? v[nt][2 + i] : -INFINITY);
           }
-          if (r0 == 0) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (b0 + quad * 2 + i < end)
-                scores[quad * 2 + i] = bads >> (quad * 8 + i * 4) & 1u ? 0u : order_of(v[i]);
+        for (int o = 1; o < 4; o <<= 1) {
+          m0 = max_nan(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+          m1 = max_nan(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+        }
+        if (quad == 0 && in0) scores[0] = ok0 ? order_of(m0) : 0u;
+        if (quad == 0 && in1) scores[8] = ok1 ? order_of(m1) : 0u;
+      } else {
+        // a power of two of heads: next columns, then next lanes
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (p.g > 1) {
+            v[nt][0] = v[nt][1] = max_nan(v[nt][0], v[nt][1]);
+            v[nt][2] = v[nt][3] = max_nan(v[nt][2], v[nt][3]);
           }
-        } else {
-          for (int o = 1; o < p.g; o <<= 1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[i] = fmaxf(v[i], __shfl_xor_sync(0xffffffffu, v[i], o * 4));
+          for (int o = 1; o < p.g / 2; o <<= 1) {
+            v[nt][0] = max_nan(v[nt][0], __shfl_xor_sync(0xffffffffu, v[nt][0], o));
+            v[nt][2] = max_nan(v[nt][2], __shfl_xor_sync(0xffffffffu, v[nt][2], o));
           }
-          if (r0 % p.g == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int col = quad * 2 + (i & 1), of = (r0 + (i >> 1) * 8) / p.g;
-              if (b0 + col < end && t0 + of < t1)
-                scores[(int64_t)of * p.hkv * p.most + col] =
-                    bads >> (col * 4) & 1u ? 0u : order_of(v[i]);
-            }
+          for (int i = 0; i < 2; ++i) {
+            const int col = nt * 8 + quad * 2 + i;
+            const int of = col >> p.g_shift;
+            if (of << p.g_shift != col || t0 + of >= t1) continue;
+            uint32_t* at = scores + (int64_t)of * p.hkv * p.most;
+            if (in0) at[0] = ok0 ? order_of(v[nt][i]) : 0u;
+            if (in1) at[8] = ok1 ? order_of(v[nt][2 + i]) : 0u;
           }
         }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    t0 = t1;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  // the largest |bound| of either half: low <= high
-  uint32_t most = max2_nan(top, low ^ 0x80008000u);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max2_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+  uint32_t most = max(max((top & 0xffffu) << 16, top & 0x7fff0000u),
+                      max((low & 0x7fffu) << 16, low & 0x7fff0000u));
+  most = __reduce_max_sync(0xffffffffu, most);
   uint32_t* most_of = reinterpret_cast<uint32_t*>(ring);      // which has been read
   __syncthreads();
   if (lane == 0) most_of[warp] = most;
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int w = 1; w < SEL_WARPS; ++w) most = max2_nan(most, most_of[w]);
-    p.largest[((int64_t)group * p.hkv + kvh) * p.chunks + chunk] =
-        __uint_as_float(max((most << 16) & 0x7fffffffu, most & 0x7fff0000u));
+    for (int w = 1; w < SEL_WARPS; ++w) most = max(most, most_of[w]);
+    p.largest[((int64_t)group * p.hkv + kvh) * p.chunks + chunk] = __uint_as_float(most);
   }
 }
 
-// ---- the choice: a team of W warps per token and KV head, 8 / W teams in a CTA
+// ---- the choice: a team of W warps per token and KV head, a CTA of its own or, of one warp, eight in one
 //
 // Blocks above the want-th largest score by more than 2 e are taken, those below it by more are not,
 // and those between are scored again in 64 bits if they do not all fit.  So the choice is that of
 // 64 bits, ties to the lower index.
 //
-// Bounds: the latency of its steps, of which a warp has fewer instructions and a CTA the shorter
-// time: warps where there are many tokens.
+// Bounds: the latency of its steps.  Eight warps take the shortest time over one, a single warp the
+// fewest instructions: the more there are to choose, the fewer warps for each.
 template <int W>
-__global__ void __launch_bounds__(256) select_choose_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) select_choose_kernel(const SelectParams p) {
   extern __shared__ __align__(16) uint8_t sel_smem[];
-  constexpr int kTeams = 8 / W;
+  constexpr int kTeams = W == 1 ? 8 : 1;
   __shared__ Team<W> teams[kTeams];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, team = (threadIdx.x >> 5) / W;
+  const int lane = threadIdx.x & 31, team = W == 1 ? threadIdx.x >> 5 : 0;
   const int64_t item = (int64_t)blockIdx.x * kTeams + team;
   if (item >= (int64_t)p.num_tokens * p.hkv) return;
   const int token = (int)(item / p.hkv), kvh = (int)(item - (int64_t)token * p.hkv);
@@ -697,7 +769,7 @@ __global__ void __launch_bounds__(256) select_choose_kernel(const SelectParams p
     const int middle = n - p.keep_first - p.keep_last;
     const uint32_t* src = p.scores + item * p.most;
     for (int i = Team<W>::rank(); i < middle; i += 32 * W) keys[i] = src[i];
-    // largest |bound|, and the largest sum of |q| of a query head; no number counts as infinite
+    // largest |bound|; no number counts as infinite
     const float* from = p.largest + ((int64_t)(token / p.together) * p.hkv + kvh) * p.chunks;
     float largest = 0.f;
     for (int i = lane; i < p.chunks; i += 32)
@@ -705,15 +777,7 @@ __global__ void __launch_bounds__(256) select_choose_kernel(const SelectParams p
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    const uint16_t* q = p.q + (int64_t)token * p.q_stride + (int64_t)kvh * p.g * SEL_D + lane * 4;
-    for (int h = 0; h < p.g; ++h) {
-      const uint2 v = *reinterpret_cast<const uint2*>(q + h * SEL_D);
-      float a = fabsf(bf16lo(v.x)) + fabsf(bf16hi(v.x)) + fabsf(bf16lo(v.y)) + fabsf(bf16hi(v.y));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-      reach = fmaxf(reach, a < INFINITY ? a : INFINITY);
-    }
-    reach *= largest;
+    reach = p.q_sum[item] * largest;
     Team<W>::sync();
   }
   choose<W>(p, token, kvh, n, p.tables + (int64_t)row * p.table_stride, keys, reach, exact, band,
@@ -724,7 +788,7 @@ __global__ void __launch_bounds__(256) select_choose_kernel(const SelectParams p
 struct SelectLayout {
   int together, chunk, chunks;
   int64_t groups;
-  size_t largest, total;              // bytes
+  size_t largest, q_sum, total;       // bytes
 };
 static SelectLayout select_layout(int64_t tokens, int hkv, int g, bool rows, int64_t most) {
   SelectLayout s;
@@ -736,11 +800,12 @@ static SelectLayout select_layout(int64_t tokens, int hkv, int g, bool rows, int
   s.groups = (tokens + s.together - 1) / s.together;
   // Long chunks for the pipeline's sake, unless that leaves SMs without work.
   s.chunk = 256;
-  while (s.chunk > 32 && s.groups * hkv * ((most + s.chunk - 1) / s.chunk) < 4ll * sm_count())
+  while (s.chunk > 64 && s.groups * hkv * ((most + s.chunk - 1) / s.chunk) < 4ll * sm_count())
     s.chunk /= 2;
   s.chunks = (int)((most + s.chunk - 1) / s.chunk);
   s.largest = ((size_t)tokens * hkv * most * 4 + 255) & ~size_t(255);
-  s.total = s.largest + (size_t)s.groups * hkv * s.chunks * 4;
+  s.q_sum = s.largest + (size_t)s.groups * hkv * s.chunks * 4;
+  s.total = s.q_sum + (size_t)tokens * hkv * 4;
   return s;
 }
 
@@ -878,22 +943,31 @@ int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, 
              workspace_bytes);
   FK_REQUIRE(w.groups * w.chunks < (1ll << 31), FK_ERR_UNSUPPORTED,
              "fk_select_blocks: too many tokens");
-  p.together = w.together; p.chunk = w.chunk; p.chunks = w.chunks;
+  p.together = w.together;
+  p.g_shift = w.together > 1 ? __builtin_ctz(p.g) : 0;
+  p.chunk = w.chunk; p.chunks = w.chunks;
   p.scores = static_cast<uint32_t*>(workspace);
   p.largest = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + w.largest);
+  p.q_sum = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + w.q_sum);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  FK_CUDA_OK(launch_kernel(select_scores_kernel,
+  const bool wide = p.g * p.together > 8;
+  auto scores = wide ? select_scores_kernel<2> : select_scores_kernel<1>;
+  static PerDeviceOnce scores_once[2];
+  FK_CUDA_OK(set_max_dynamic_smem(scores_once[wide], scores, SEL_RING_BYTES));
+  FK_CUDA_OK(launch_kernel(scores,
                            dim3((unsigned)(w.groups * w.chunks), (unsigned)num_kv_heads),
-                           dim3(32 * SEL_WARPS), (size_t)0, s, p));
+                           dim3(32 * SEL_WARPS), (size_t)SEL_RING_BYTES, s, p));
   const int64_t items = (int64_t)num_tokens * num_kv_heads;
-  const bool many = items >= 16ll * sm_count() && most <= SEL_WARP_BLOCKS;
-  static PerDeviceOnce once[2];
-  auto kernel = many ? select_choose_kernel<1> : select_choose_kernel<8>;
-  FK_CUDA_OK(set_max_dynamic_smem(once[many], kernel,
-                                  (many ? 8 * SEL_WARP_BLOCKS : SEL_MAX_BLOCKS) * 14));
-  FK_CUDA_OK(launch_kernel(kernel, dim3((unsigned)(many ? (items + 7) / 8 : items)), dim3(256),
-                           (size_t)most * 14 * (many ? 8 : 1), s, p));
-  count_launch(1);
+  const int sms = sm_count();
+  const int warps = items <= 2ll * sms ? 8 : items < 16ll * sms || most > SEL_WARP_BLOCKS ? 4 : 1;
+  const int teams = warps == 1 ? 8 : 1;
+  static PerDeviceOnce once[3];
+  auto kernel = warps == 8 ? select_choose_kernel<8>
+                           : warps == 4 ? select_choose_kernel<4> : select_choose_kernel<1>;
+  FK_CUDA_OK(set_max_dynamic_smem(once[warps == 8 ? 0 : warps == 4 ? 1 : 2], kernel,
+                                  (warps == 1 ? 8 * SEL_WARP_BLOCKS : SEL_MAX_BLOCKS) * 14));
+  FK_CUDA_OK(launch_kernel(kernel, dim3((unsigned)((items + teams - 1) / teams)),
+                           dim3(warps == 1 ? 256 : 32 * warps), (size_t)most * 14 * teams, s, p));
   count_launch(1);
   return FK_OK;
 }
