@@ -287,69 +287,107 @@ def merge_attn_states(output, prefix_output, prefix_lse, suffix_output, suffix_l
 
 
 # ------------------------------------------------- decode attention that reads less of the cache
-def _need_here(t: torch.Tensor, dtype, name: str) -> None:
-    """`_need`, and on the device whose stream the kernels go to."""
+# Checks of these calls, which are many and cost a small batch's launches as much as its kernels: one
+# comparison of type and device per tensor, and what is wrong is looked for afterwards.
+_INT32, _UINT8 = torch.int32, torch.uint8
+
+
+def _device_of(t) -> int:
+    """The current device, which the first tensor of a call has to be on."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        _refuse("the first tensor", t, t.dtype, dev if dev < 0 else torch.cuda.current_device())
+    return dev
+
+
+def _refuse(name, t, dtype, dev):
     _need(t, dtype, name)
-    if t.device.index != torch.cuda.current_device():
-        raise _lib.FkError(f"{name} is on {t.device}, the current device is "
-                           f"cuda:{torch.cuda.current_device()}")
+    raise _lib.FkError(f"{name} is on {t.device}, the current device is cuda:{dev}")
 
 
-def _need_ints(t: torch.Tensor, numel, name: str) -> None:
-    _need_here(t, torch.int32, name)
-    if t.dim() != 1 or not t.is_contiguous():
-        raise _lib.FkError(f"{name} must be a dense vector")
-    if numel is not None and t.numel() != numel:
-        raise _lib.FkError(f"{name} must have {numel} entries, got {t.numel()}")
+def _need_ints(dev, numel, name, t) -> None:
+    """A dense int32 vector of so many entries."""
+    if t.dtype is not _INT32 or t.get_device() != dev:
+        _refuse(name, t, _INT32, dev)
+    if t.dim() != 1 or not t.is_contiguous() or t.numel() != numel:
+        raise _lib.FkError(f"{name} must be a dense vector of {numel} entries")
 
 
-def _need_tables(block_tables) -> tuple[int, int, int]:
+def _need_tables(dev, t) -> tuple[int, int, int]:
     """(stride, columns, rows) of page tables; rows may be one row expanded."""
-    _need_here(block_tables, torch.int32, "block_tables")
-    if block_tables.dim() != 2 or block_tables.stride(1) != 1 and block_tables.shape[1] > 1 \
-            and block_tables.shape[0]:
-        raise _lib.FkError("block_tables must be [rows, pages] with dense rows")
-    rows, cols = block_tables.shape
-    return block_tables.stride(0) if rows > 1 else cols, cols, rows
+    if t.dtype is not _INT32 or t.get_device() != dev:
+        _refuse("block_tables", t, _INT32, dev)
+    if t.dim() != 2:
+        raise _lib.FkError("block_tables must be [rows, pages]")
+    rows, cols = t.shape
+    stride, step = t.stride()
+    if step != 1 and cols > 1 and rows:
+        raise _lib.FkError("block_tables must have dense rows")
+    return stride if rows > 1 else cols, cols, rows
 
 
-def _need_cache(cache, kv_layout, name, like=None) -> tuple[int, int, int, int, int]:
+def _need_cache(dev, cache, kv_layout, name) -> tuple[int, int, int, int, int]:
     """(pages, page size, KV heads, head size, page stride) of a paged pool."""
-    _need_here(cache, BF16, name)
-    if kv_layout not in ("NHD", "HND"):
-        raise _lib.FkError("kv_layout must be 'NHD' or 'HND'")
+    if cache.dtype is not BF16 or cache.get_device() != dev:
+        _refuse(name, cache, BF16, dev)
     if cache.dim() != 4:
         raise _lib.FkError(f"{name} must have four dimensions")
+    stride, *inner = cache.stride()
     if kv_layout == "NHD":
         pages, page, hkv, d = cache.shape
-        dense = (hkv * d, d, 1)
-    else:
+        dense = [hkv * d, d, 1]
+    elif kv_layout == "HND":
         pages, hkv, page, d = cache.shape
-        dense = (page * d, d, 1)
-    if cache.stride()[1:] != dense:
+        dense = [page * d, d, 1]
+    else:
+        raise _lib.FkError("kv_layout must be 'NHD' or 'HND'")
+    if inner != dense:
         raise _lib.FkError(f"{name} must be dense within a page")
-    if like is not None and (cache.shape != like.shape or cache.stride() != like.stride()):
+    return pages, page, hkv, d, stride if pages > 1 else page * hkv * d
+
+
+def _need_caches(dev, k_cache, v_cache, kv_layout) -> tuple[int, int, int, int, int]:
+    got = _need_cache(dev, k_cache, kv_layout, "k_cache")
+    if v_cache.dtype is not BF16 or v_cache.get_device() != dev:
+        _refuse("v_cache", v_cache, BF16, dev)
+    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
         raise _lib.FkError("cache shape mismatch")
-    return pages, page, hkv, d, cache.stride(0) if pages > 1 else page * hkv * d
+    return got
 
 
-def _need_rows(t, like, name) -> int:
-    """Token stride of q or out, [tokens, heads, D] with dense heads."""
-    _need_here(t, BF16, name)
-    if t.dim() != 3 or like is not None and t.shape != like.shape:
+def _need_rows(dev, t, name) -> tuple[int, int, int, int]:
+    """(tokens, heads, head size, token stride) of q or out with dense heads."""
+    if t.dtype is not BF16 or t.get_device() != dev:
+        _refuse(name, t, BF16, dev)
+    if t.dim() != 3:
         raise _lib.FkError(f"{name} must be [tokens, heads, D]")
     n, heads, d = t.shape
-    if n and (t.stride(2) != 1 and d > 1 or t.stride(1) != d and heads > 1):
+    stride, head, one = t.stride()
+    if n and (one != 1 and d > 1 or head != d and heads > 1):
         raise _lib.FkError(f"{name} heads must be dense")
-    return t.stride(0) if n > 1 else heads * d
+    return n, heads, d, stride if n > 1 else heads * d
 
 
-def _workspace(workspace, need: int, like) -> torch.Tensor:
+def _out_like(dev, q, out):
+    """(out, its token stride): a new one for None."""
+    if out is None:
+        n, heads, d = q.shape
+        return q.new_empty((n, heads, d)), heads * d
+    if out.shape != q.shape:
+        raise _lib.FkError("out must have the shape of q")
+    return out, _need_rows(dev, out, "out")[3]
+
+
+def _workspace(dev, workspace, need: int, like) -> tuple[int | None, int, object]:
+    """(address, bytes, the tensor to hold on to)."""
     if workspace is None:
-        return torch.empty(max(need, 1), dtype=torch.uint8, device=like.device)
-    if not workspace.is_cuda or workspace.device != like.device or not workspace.is_contiguous():
+        if need == 0:
+            return None, 0, None
+        workspace = like.new_empty(need, dtype=_UINT8)
+        return workspace.data_ptr(), need, workspace
+    if workspace.get_device() != dev or not workspace.is_contiguous():
         raise _lib.FkError("the workspace must be dense and on the device of q")
-    return workspace
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 def shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, head_dim,
@@ -364,51 +402,51 @@ def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_st
     """paged_decode_attn for a batch whose rows group_starts[g] .. group_starts[g + 1] - 1 list the
     same pages for their first prefix_lens[g] tokens: that part is read once for all of them.
 
-    group_starts int32 [groups + 1] ascends from 0 on, prefix_lens int32 [groups]; of a prefix that
-    ends inside a page the whole pages are taken together.  Rows outside of all groups have nothing
-    in common.  context_lens count all tokens of a row, the common ones too.  GQA ratios up to 16.
-    A workspace of shared_prefix_workspace_bytes holds the schedule and partial results of one call
-    at a time; without one it is allocated here."""
-    pages, page, hkv, d2, stride = _need_cache(k_cache, kv_layout, "k_cache")
-    _need_cache(v_cache, kv_layout, "v_cache", k_cache)
-    qs = _need_rows(q, None, "q")
-    b, hq, d = q.shape
+    group_starts int32 [groups + 1] ascends within the batch, prefix_lens int32 [groups]; of a
+    prefix that ends inside a page the whole pages are taken together.  Rows outside of all
+    groups have nothing in common.  context_lens count all tokens of a row, the common ones too.
+    GQA ratios up to 16.  A workspace of shared_prefix_workspace_bytes holds the schedule and
+    partial results of one call at a time; without one it is allocated here."""
+    dev = _device_of(q)
+    pages, page, hkv, d2, stride = _need_caches(dev, k_cache, v_cache, kv_layout)
+    b, hq, d, qs = _need_rows(dev, q, "q")
     if d2 != d:
         raise _lib.FkError("cache shape mismatch")
-    _need_ints(context_lens, b, "context_lens")
-    ts, cols, rows = _need_tables(block_tables)
+    _need_ints(dev, b, "context_lens", context_lens)
+    ts, cols, rows = _need_tables(dev, block_tables)
     if rows != b:
         raise _lib.FkError(f"block_tables must have {b} rows, got {rows}")
     groups = prefix_lens.numel()
-    _need_ints(prefix_lens, groups, "prefix_lens")
-    _need_ints(group_starts, groups + 1, "group_starts")
-    if out is None:
-        out = torch.empty((b, hq, d), dtype=BF16, device=q.device)
-    os_ = _need_rows(out, q, "out")
+    _need_ints(dev, groups, "prefix_lens", prefix_lens)
+    _need_ints(dev, groups + 1, "group_starts", group_starts)
+    out, os_ = _out_like(dev, q, out)
     if max_splits is None:
         max_splits = max_splits_for(cols * page)
-    workspace = _workspace(workspace, shared_prefix_workspace_bytes(b, groups, hq, hkv, d,
-                                                                    max_splits), q)
+    ws, ws_bytes, _held = _workspace(
+        dev, workspace,
+        lib.fk_shared_prefix_workspace_bytes(b, groups, hq, hkv, d, max_splits)
+        if workspace is None else 0, q)
     check(lib.fk_shared_prefix_attn(
-        _ptr(q), qs, _ptr(out), os_, _ptr(k_cache), _ptr(v_cache), pages, page, stride,
-        int(kv_layout == "HND"), _ptr(context_lens), _ptr(block_tables), ts, cols,
-        _ptr(group_starts), _ptr(prefix_lens), groups, b, hq, hkv, d, float(softmax_scale),
-        int(max_splits), _ptr(workspace), workspace.numel() * workspace.element_size(),
-        _status_ptr(status, q), _stream()), "fk_shared_prefix_attn")
+        q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
+        stride, 1 if kv_layout == "HND" else 0, context_lens.data_ptr(), block_tables.data_ptr(),
+        ts, cols, group_starts.data_ptr(), prefix_lens.data_ptr(), groups, b, hq, hkv, d,
+        softmax_scale, max_splits, ws, ws_bytes, _status_ptr(status, q), _stream()),
+        "fk_shared_prefix_attn")
     return out
 
 
 def new_key_bounds(k_cache, block, kv_layout="NHD") -> torch.Tensor:
     """Bounds of all blocks of `block` tokens of a pool, [pages, Hkv, page // block, 2, D], zeroed;
     key_bounds fills in those of the blocks that hold tokens."""
-    pages, page, hkv, d, _ = _need_cache(k_cache, kv_layout, "k_cache")
+    pages, page, hkv, d, _ = _need_cache(_device_of(k_cache), k_cache, kv_layout, "k_cache")
     if block < 1 or page % block:
         raise _lib.FkError(f"a page of {page} tokens is not a whole number of blocks of {block}")
     return torch.zeros((pages, hkv, page // block, 2, d), dtype=BF16, device=k_cache.device)
 
 
-def _need_bounds(bounds) -> None:
-    _need_here(bounds, BF16, "bounds")
+def _need_bounds(dev, bounds) -> None:
+    if bounds.dtype is not BF16 or bounds.get_device() != dev:
+        _refuse("bounds", bounds, BF16, dev)
     if bounds.dim() != 5 or bounds.shape[3] != 2 or not bounds.is_contiguous():
         raise _lib.FkError("bounds must be a contiguous [pages, Hkv, blocks of a page, 2, D]")
 
@@ -420,22 +458,23 @@ def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new
     cu_seqlens) the last cu_new[s + 1] - cu_new[s], at most max_new.  Call it after those tokens' keys
     have been stored; context_lens count them.  A block that is not full yet has the bounds of the
     keys in it.  A sequence (and so a page with new tokens) appears once in the batch."""
-    pages, page, hkv, d, stride = _need_cache(k_cache, kv_layout, "k_cache")
-    _need_bounds(bounds)
+    dev = _device_of(k_cache)
+    pages, page, hkv, d, stride = _need_cache(dev, k_cache, kv_layout, "k_cache")
+    _need_bounds(dev, bounds)
     per = bounds.shape[2]
-    if tuple(bounds.shape) != (pages, hkv, per, 2, d) or per < 1 or page % per:
+    if bounds.shape != (pages, hkv, per, 2, d) or per < 1 or page % per:
         raise _lib.FkError("bounds do not fit the cache")
     n = context_lens.numel()
-    _need_ints(context_lens, None, "context_lens")
-    ts, cols, rows = _need_tables(block_tables)
+    _need_ints(dev, n, "context_lens", context_lens)
+    ts, cols, rows = _need_tables(dev, block_tables)
     if rows != n:
         raise _lib.FkError(f"block_tables must have {n} rows, got {rows}")
     if cu_new is not None:
-        _need_ints(cu_new, n + 1, "cu_new")
+        _need_ints(dev, n + 1, "cu_new", cu_new)
     check(lib.fk_key_bounds(
-        _ptr(k_cache), pages, page, stride, int(kv_layout == "HND"), hkv, d, _ptr(bounds),
-        page // per, _ptr(context_lens), _ptr(block_tables), ts, cols, _ptr(cu_new), n,
-        int(max_new), _status_ptr(status, k_cache), _stream()), "fk_key_bounds")
+        k_cache.data_ptr(), pages, page, stride, 1 if kv_layout == "HND" else 0, hkv, d,
+        bounds.data_ptr(), page // per, context_lens.data_ptr(), block_tables.data_ptr(), ts, cols,
+        _ptr(cu_new), n, max_new, _status_ptr(status, k_cache), _stream()), "fk_key_bounds")
     return bounds
 
 
@@ -454,29 +493,33 @@ def select_blocks(q, bounds, context_lens, block_tables, block, count, keep_firs
 
     context_lens int32 [tokens]: keys that a token sees, itself among them.  table_rows int32
     [tokens]: its row of block_tables (None: its own number).  Bounds of a token's last block are
-    not read; all others before it must be there."""
-    qs = _need_rows(q, None, "q")
-    _need_bounds(bounds)
-    n, hq, d = q.shape
+    not read; all others before it must be there.  Without a workspace of
+    select_blocks_workspace_bytes one is allocated here."""
+    dev = _device_of(q)
+    n, hq, d, qs = _need_rows(dev, q, "q")
+    _need_bounds(dev, bounds)
     pages, hkv, per, _, d2 = bounds.shape
     if d2 != d:
         raise _lib.FkError("bounds do not fit q")
-    _need_ints(context_lens, n, "context_lens")
-    ts, cols, rows = _need_tables(block_tables)
+    _need_ints(dev, n, "context_lens", context_lens)
+    ts, cols, rows = _need_tables(dev, block_tables)
     if table_rows is not None:
-        _need_ints(table_rows, n, "table_rows")
+        _need_ints(dev, n, "table_rows", table_rows)
     if out is None:
-        out = torch.empty((n, hkv, count), dtype=torch.int32, device=q.device)
-    _need_here(out, torch.int32, "out")
-    if tuple(out.shape) != (n, hkv, count) or not out.is_contiguous():
-        raise _lib.FkError("out must be a contiguous [tokens, Hkv, count]")
-    workspace = _workspace(workspace, select_blocks_workspace_bytes(n, hq, hkv, per * block, block,
-                                                                    cols), q)
+        out = q.new_empty((n, hkv, count), dtype=_INT32)
+    else:
+        if out.dtype is not _INT32 or out.get_device() != dev:
+            _refuse("out", out, _INT32, dev)
+        if out.shape != (n, hkv, count) or not out.is_contiguous():
+            raise _lib.FkError("out must be a contiguous [tokens, Hkv, count]")
+    ws, ws_bytes, _held = _workspace(
+        dev, workspace,
+        lib.fk_select_blocks_workspace_bytes(n, hq, hkv, per * block, block, cols)
+        if workspace is None else 0, q)
     check(lib.fk_select_blocks(
-        _ptr(q), qs, _ptr(bounds), pages, per * block, block, _ptr(context_lens),
-        _ptr(table_rows), _ptr(block_tables), ts, cols, rows, n, hq, hkv, d, int(count),
-        int(keep_first), int(keep_last), _ptr(out), _ptr(workspace),
-        workspace.numel() * workspace.element_size(), _status_ptr(status, q), _stream()),
+        q.data_ptr(), qs, bounds.data_ptr(), pages, per * block, block, context_lens.data_ptr(),
+        _ptr(table_rows), block_tables.data_ptr(), ts, cols, rows, n, hq, hkv, d, count,
+        keep_first, keep_last, out.data_ptr(), ws, ws_bytes, _status_ptr(status, q), _stream()),
         "fk_select_blocks")
     return out
 
@@ -492,32 +535,31 @@ def selected_attn(q, k_cache, v_cache, context_lens, block_tables, selected, blo
     """Attention of each query token over the blocks in selected [tokens, Hkv, count] (int32, as
     select_blocks gives them), at positions below its context_lens.  Entries below 0 or past the
     context hold no keys, and one that is listed twice counts twice; a token without keys gets
-    zeros.  table_rows as in select_blocks; GQA ratios up to 16."""
-    pages, page, hkv, d2, stride = _need_cache(k_cache, kv_layout, "k_cache")
-    _need_cache(v_cache, kv_layout, "v_cache", k_cache)
-    qs = _need_rows(q, None, "q")
-    n, hq, d = q.shape
+    zeros.  table_rows as in select_blocks; GQA ratios up to 16.  Without a workspace of
+    selected_attn_workspace_bytes one is allocated here."""
+    dev = _device_of(q)
+    pages, page, hkv, d2, stride = _need_caches(dev, k_cache, v_cache, kv_layout)
+    n, hq, d, qs = _need_rows(dev, q, "q")
     if d2 != d:
         raise _lib.FkError("cache shape mismatch")
-    _need_ints(context_lens, n, "context_lens")
-    ts, cols, rows = _need_tables(block_tables)
+    _need_ints(dev, n, "context_lens", context_lens)
+    ts, cols, rows = _need_tables(dev, block_tables)
     if table_rows is not None:
-        _need_ints(table_rows, n, "table_rows")
-    _need_here(selected, torch.int32, "selected")
+        _need_ints(dev, n, "table_rows", table_rows)
+    if selected.dtype is not _INT32 or selected.get_device() != dev:
+        _refuse("selected", selected, _INT32, dev)
     if selected.dim() != 3 or selected.shape[:2] != (n, hkv) or not selected.is_contiguous():
         raise _lib.FkError("selected must be a contiguous [tokens, Hkv, count]")
     count = selected.shape[2]
-    if out is None:
-        out = torch.empty((n, hq, d), dtype=BF16, device=q.device)
-    os_ = _need_rows(out, q, "out")
-    workspace = _workspace(workspace, selected_attn_workspace_bytes(n, hq, hkv, d, count, block),
-                           q)
+    out, os_ = _out_like(dev, q, out)
+    ws, ws_bytes, _held = _workspace(
+        dev, workspace, lib.fk_selected_attn_workspace_bytes(n, hq, hkv, d, count, block)
+        if workspace is None else 0, q)
     check(lib.fk_selected_attn(
-        _ptr(q), qs, _ptr(out), os_, _ptr(k_cache), _ptr(v_cache), pages, page, stride,
-        int(kv_layout == "HND"), _ptr(context_lens), _ptr(table_rows), _ptr(block_tables), ts,
-        cols, rows, _ptr(selected), count, int(block), n, hq, hkv, d, float(softmax_scale),
-        _ptr(workspace), workspace.numel() * workspace.element_size(), _status_ptr(status, q),
-        _stream()), "fk_selected_attn")
+        q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
+        stride, 1 if kv_layout == "HND" else 0, context_lens.data_ptr(), _ptr(table_rows),
+        block_tables.data_ptr(), ts, cols, rows, selected.data_ptr(), count, block, n, hq, hkv, d,
+        softmax_scale, ws, ws_bytes, _status_ptr(status, q), _stream()), "fk_selected_attn")
     return out
 
 
