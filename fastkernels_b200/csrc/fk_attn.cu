@@ -441,13 +441,19 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
       const int sq = item / p.hkv;
       int L = p.context_lens[sq];
       if (L < 0) L = 0;
-      const int64_t cap = p.bt_stride * (int64_t)p.block_size;
+      const int64_t cap = p.capacity > 0 ? p.capacity : p.bt_stride * (int64_t)p.block_size;
       if ((int64_t)L > cap) {
         L = (int)cap;
         if (p.status && lane == 0) atomicOr(p.status, FK_DEV_BAD_PAGE);
       }
       return make_int4(sq, 0 | (1 << 16), 0, L);
     };
+    if (p.groups > 0 && blockIdx.x == 0) {
+      for (int i = lane; i < p.groups; i += 32)
+        if ((p.starts[i] < 0 || p.starts[i + 1] < p.starts[i] || p.starts[i + 1] > p.batch) &&
+            p.status)
+          atomicOr(p.status, FK_DEV_BAD_POSITION);
+    }
     int stage = 0;
     uint32_t phase = 0;  // parity of the `empty` phase we wait for (first pass: free)
     bool ok = true;

@@ -30,8 +30,10 @@ struct AttnParams {
   const int32_t* rows;      // table of each token, null: its own number
   int count, sel_block;
   int num_tables;
-  int64_t capacity;         // tokens that a table's row has pages for
+  int64_t capacity;         // tokens that a table's row has pages for (0: block_size * bt_stride)
   int tiles;                // 128-token tiles of `count` blocks
+  const int32_t* starts;    // groups of rows that a direct call only looks over
+  int groups;
   int64_t unit;             // tiles of all tokens and heads, one after another, that a CTA takes
 };
 

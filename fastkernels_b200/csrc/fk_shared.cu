@@ -36,39 +36,39 @@ struct RowsParams {
 // splits of a token and head joined: out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M)
 // ---------------------------------------------------------------------------
 // A lane has the (max, sum) of splits lane, lane + 32, ..., so all of them are one round of loads, and
-// four partial rows are on the way at a time.  A split without keys has a sum of zero; its row was not
-// written and is not read.
+// eight partial rows are on the way at a time.  A split without keys has a sum of zero; its row was
+// not written and is not read.
 struct JoinRow {
   float4 acc;
   float l;
 };
-__device__ __forceinline__ float join_max(const float2* ml, int n, int lane) {
+// ml(s) gives (max, sum) of split s, row(s) this lane's four channels of it
+template <typename ML>
+__device__ __forceinline__ float join_max(const ML& ml, int n, int lane) {
   float m = -INFINITY;
-  for (int s = lane; s < n; s += 32) m = fmaxf(m, ml[s].x);
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, ml(s).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
-__device__ __forceinline__ void join_add(JoinRow& r, const float* part_o, const float2* ml, int n,
-                                         float top, int lane) {
+template <typename ML, typename ROW>
+__device__ __forceinline__ void join_add(JoinRow& r, const ML& ml, const ROW& row, int n, float top,
+                                         int lane) {
   for (int s0 = 0; s0 < n; s0 += 32) {
-    const float2 mlv = s0 + lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+    const float2 mlv = s0 + lane < n ? ml(s0 + lane) : make_float2(-INFINITY, 0.f);
     const float fl = mlv.y > 0.f ? fast_exp2(mlv.x - top) : 0.f;
     const int cnt = min(32, n - s0);
-    const float4* src = reinterpret_cast<const float4*>(part_o + (int64_t)s0 * SH_D) + lane;
-    for (int s = 0; s < cnt; s += 4) {
-      float4 v[4];
-      float f[4], l[4];
+    for (int s = 0; s < cnt; s += 8) {
+      float4 v[8];
+      float f[8], l[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[i] = __shfl_sync(0xffffffffu, fl, s + i);
-        l[i] = __shfl_sync(0xffffffffu, mlv.y, s + i);
-        v[i] = s + i < cnt && l[i] > 0.f ? src[(s + i) * (SH_D / 4)]
-                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < 8; ++i) {
+        f[i] = __shfl_sync(0xffffffffu, fl, (s + i) & 31);
+        l[i] = s + i < cnt ? __shfl_sync(0xffffffffu, mlv.y, (s + i) & 31) : 0.f;
+        v[i] = l[i] > 0.f ? *row(s0 + s + i) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (s + i >= cnt) break;
+      for (int i = 0; i < 8; ++i) {
         r.l = fmaf(l[i], f[i], r.l);
         r.acc = r.acc + v[i] * f[i];
       }
@@ -88,10 +88,13 @@ __global__ void __launch_bounds__(256) selected_join_kernel(const AttnParams p) 
   selected_ctas((int64_t)token * p.hkv + head / p.g, p.tiles, p.unit, &first, &last);
   const int n = last - first + 1;
   if (n == 1) return;                        // written by the attention kernel
-  const float2* ml = p.part_ml + gw * p.max_splits;
+  auto ml = [&](int s) { return p.part_ml[gw * p.max_splits + s]; };
+  auto part = [&](int s) {
+    return reinterpret_cast<const float4*>(p.part_o + (gw * p.max_splits + s) * SH_D) + lane;
+  };
   const float top = join_max(ml, n, lane);
   JoinRow r{make_float4(0.f, 0.f, 0.f, 0.f), 0.f};
-  join_add(r, p.part_o + gw * p.max_splits * SH_D, ml, n, top == -INFINITY ? 0.f : top, lane);
+  join_add(r, ml, part, n, top == -INFINITY ? 0.f : top, lane);
   Elem<uint16_t>::store4(p.out + (int64_t)token * p.out_stride + (int64_t)head * SH_D + lane * 4,
                          r.acc * (r.l > 0.f ? 1.0f / r.l : 0.f));
 }
@@ -135,8 +138,8 @@ enum : int { PLAN_CHUNKS = 0, PLAN_COUNTER = 2, PLAN_ITEMS = 4, PLAN_TILES = 5, 
 struct SharedPlan {
   int* hdr;            // see above; chunk_start[batch + 1] behind it, as the decode kernel has it
   int* row_item;       // [batch] item that holds a row, -1: none
-  int* row_from;       // [batch] tokens of a row that its item covers
-  PrefixItem* items;   // [batch]
+  int* cta_item;       // [ctas] item of a CTA's first tile
+  PrefixItem* items;
   int4* chunks;        // chunks of what each row has for itself
 };
 
@@ -147,6 +150,8 @@ struct SharedPlanParams {
   SharedPlan plan;
   int32_t* status;
 };
+
+constexpr int PLAN_MAX_BATCH = 16384;
 
 constexpr int PLAN_THREADS = 1024;
 
@@ -185,24 +190,24 @@ __device__ __forceinline__ int plan_before(int v, int* red, int* total) {
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedPlanParams p) {
+  extern __shared__ int plan_smem[];
+  int* s_len = plan_smem;                      // [batch] tokens of a row
+  int* s_from = plan_smem + p.batch;           // [batch] of them in its item
   __shared__ int red[32];
   __shared__ int s_keys[PLAN_THREADS], s_table[PLAN_THREADS], s_item[PLAN_THREADS],
       s_start[PLAN_THREADS];
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  auto len_of = [&](int i) -> int {
-    const int64_t len = p.lens[i];
-    return len < 0 ? 0 : (int)(len > p.capacity ? p.capacity : len);
-  };
   bool cut = false;
   for (int i = tid; i < p.batch; i += PLAN_THREADS) {
-    cut |= (int64_t)p.lens[i] > p.capacity;
+    const int64_t len = p.lens[i];
+    cut |= len > p.capacity;
+    s_len[i] = len < 0 ? 0 : (int)(len > p.capacity ? p.capacity : len);
+    s_from[i] = 0;
     p.plan.row_item[i] = -1;
-    p.plan.row_from[i] = 0;
   }
   if (cut && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-  __syncthreads();
 
   // Groups into items, 1024 groups at a time: a warp looks for the longest row of a group, a thread
   // per group adds up, a warp per group writes.  Starts that do not ascend within the batch: nobody
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
       const int a = p.starts[g0 + i], b = p.starts[g0 + i + 1];
       int longest = 0, table = a;
       for (int r = a + lane; r < b; r += 32) {
-        const int n = len_of(r);
+        const int n = s_len[r];
         if (n > longest) { longest = n; table = r; }
       }
 #pragma unroll
@@ -259,16 +264,24 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
                        s_start[i] + j * tiles_i * p.hkv, tiles_i, 0, 0};
       for (int r = lane; r < n; r += 32) {
         p.plan.row_item[a + r] = s_item[i] + r / each;
-        p.plan.row_from[a + r] = keys_i;
+        s_from[a + r] = keys_i;
       }
     }
     __syncthreads();
   }
+  const int unit = max(p.min_unit, (tiles + p.ctas - 1) / p.ctas);
   __syncthreads();
+  // CTAs whose first tile is in an item
+  for (int i = tid; i < items; i += PLAN_THREADS) {
+    const PrefixItem it = p.plan.items[i];
+    const int end = it.start + it.tiles * p.hkv;
+    for (int c = (it.start + unit - 1) / unit; c < p.ctas && (int64_t)c * unit < end; ++c)
+      p.plan.cta_item[c] = i;
+  }
 
   // What each row has for itself, in chunks of one length: long ones, but enough of them for every
   // CTA, and at most max_splits a row.
-  auto rest_of = [&](int i) -> int { return max(0, len_of(i) - p.plan.row_from[i]); };
+  auto rest_of = [&](int i) -> int { return max(0, s_len[i] - s_from[i]); };
   int longest = 0;
   for (int i = tid; i < p.batch; i += PLAN_THREADS) longest = max(longest, rest_of(i));
 #pragma unroll
@@ -291,8 +304,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
   int run = 0;
   for (int i0 = 0; i0 < p.batch; i0 += PLAN_THREADS) {
     const int i = i0 + tid;
-    const int from = i < p.batch ? p.plan.row_from[i] : 0;
-    const int len = i < p.batch ? len_of(i) : 0;
+    const int from = i < p.batch ? s_from[i] : 0;
+    const int len = i < p.batch ? s_len[i] : 0;
     const int n = (max(0, len - from) + chunk - 1) / chunk;
     int all;
     const int at = run + plan_before(n, red, &all);
@@ -311,7 +324,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
     p.plan.hdr[PLAN_COUNTER] = 0;
     p.plan.hdr[PLAN_ITEMS] = items;
     p.plan.hdr[PLAN_TILES] = tiles;
-    p.plan.hdr[PLAN_UNIT] = max(p.min_unit, (tiles + p.ctas - 1) / p.ctas);
+    p.plan.hdr[PLAN_UNIT] = unit;
   }
 }
 
@@ -322,41 +335,51 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
 // another; each item and KV head in it is a split.  Rows of an item are (batch row, query head of the
 // KV head): 128 / G batch rows make a tile of query rows, and an item has one or two.
 //
-//   warp 8        TMA: query tiles, then K_0 V_0 K_1 V_1 ... through a ring of five 32 KiB slots
-//   warp 9        tensor memory and products: S_t = Q_t K_j^T into columns [128 t, 128 t + 128),
-//                 O_t += P_t V_j into [256 + 128 t, ...), P_t read from the first 64 columns of S_t.
-//                 The two tiles take turns, so that the softmax of one runs beside the
-//                 products of the other.
-//   warps 0-3, 4-7  softmax of tile 0 and 1, a thread per query row: maximum, exponentials, sum;
-//                 weights are rounded to bf16 for the product with the values (their sum is of
-//                 what was before), O is scaled when a maximum grew by more than 2^8.
+//   warps 0-7, 8-15  softmax of tile 0 and 1, two threads per query row with 64 keys each: maximum
+//                 (exchanged), exponentials, sum.  Weights are rounded to bf16 for the product with
+//                 the values (their sum is of what was before); O is scaled when a maximum grew by
+//                 more than 2^8.
+//   warp 16       TMA: query tiles, then K_0 V_0 K_1 V_1 ... through a ring of five 32 KiB slots
+//   warp 17       tensor memory and products: S_t = Q_t K_j^T into columns [128 t, 128 t + 128),
+//                 O_t += P_t V_j into [256 + 128 t, ...); P_t is read from where each half of the
+//                 keys had its S_t.  The two tiles take turns, so that the softmax of one runs
+//                 beside the products of the other.
+//
+// A tile's step is softmax, P V, next S: with one thread per row the softmax alone took as long as
+// the products of both tiles, and the tensor cores stood still half of the time.
+// Results leave through shared memory (where the query tile was) in bulk copies of 4 KiB: 32 rows of
+// 32 channels, 16-byte pieces of a row exchanged by its number so that writing them is free of
+// conflicts.
 //
 // Bounds: the bytes of the common part up to some 250 query rows a KV head, the products and
 // exponentials beyond.  Waits end after two seconds, as in the other attention kernels.
 constexpr int PX_SLOTS = 5;
 constexpr int PX_HALF_BYTES = 128 * 128;
 constexpr int PX_TILE_BYTES = 2 * PX_HALF_BYTES;
-constexpr int PX_THREADS = 320;
-constexpr int PX_WARP_TMA = 8, PX_WARP_MMA = 9;
+constexpr int PX_THREADS = 576;
+constexpr int PX_WARP_TMA = 16, PX_WARP_MMA = 17;
 constexpr int PX_OFF_Q = 0;
 constexpr int PX_OFF_KV = 2 * PX_TILE_BYTES;
 constexpr int PX_OFF_BAR = PX_OFF_KV + PX_SLOTS * PX_TILE_BYTES;
-constexpr int PX_SMEM_ALLOC = PX_OFF_BAR + 256 + 1024;
+constexpr int PX_OFF_MAX = PX_OFF_BAR + 256;
+constexpr int PX_SMEM_ALLOC = PX_OFF_MAX + 2 * 2 * 128 * 2 + 1024;
 constexpr int PX_TMEM_COLS = 512;
 constexpr float PX_RESCALE_LOG2 = 8.0f;
+constexpr int PX_SLOT_FLOATS = 2 * 128 * SH_D;   // partial rows of a split
 static_assert(PX_SMEM_ALLOC <= 232448, "shared memory budget");
 static_assert(tmem_alone(PX_SMEM_ALLOC), "two CTAs could wait for one another's tensor memory");
 
 struct PrefixParams {
-  const int* hdr; const PrefixItem* items;
+  const int* hdr; const int* cta_item; const PrefixItem* items;
   const int32_t* lens;
   const int32_t* tables; int64_t table_stride;
   int hq, hkv, g, per_tile;            // batch rows of a query tile
   int hnd, block_size, sub_tokens, num_blocks;
   float scale_log2;
-  int64_t capacity;
-  float* part_o; float2* part_ml;      // [batch, hq, splits]
-  int splits;
+  // Of the split with CTA c and item and head i at c + i, which is another for every split: partial
+  // rows [2 tiles][4 x 32 rows][2 x 64 channels][2 x 32][32 rows][32], and (maximum, sum) of both
+  // halves of the keys [2][2][128].
+  float* part_o; float2* part_ml;
   int32_t* status;
 };
 
@@ -386,6 +409,21 @@ __device__ __forceinline__ bool px_wait_warp(uint64_t* bar, uint32_t parity,
   return __all_sync(0xffffffffu, px_poll(bar, parity, abort_flag, status) ? 1 : 0) != 0;
 }
 
+// 32 lanes x 8 columns of tensor memory
+__device__ __forceinline__ void px_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void px_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+      : "memory");
+}
+
 // packed fp32 pairs and the three-input maximum
 __device__ __forceinline__ uint64_t px_pack2(float a, float b) {
   uint64_t r;
@@ -411,29 +449,29 @@ __device__ __forceinline__ float px_max3(float a, float b, float c) {
   return d;
 }
 
-// One split: tiles t0 .. t1 - 1 of an item and KV head.
+// The splits of a CTA, one after another: tiles t0 .. t1 - 1 of an item and KV head.  Little of it
+// stays in registers from one to the next.
 struct PrefixSeg {
-  int row0, rows, table, keys, kvh, t0, t1, split, two;
+  PrefixItem it;
+  int kvh, t0, t1, slot, two;
 };
-// The split that holds tile `at` of all; ends at `end` or with its item and head.
-__device__ __forceinline__ PrefixSeg px_segment(const PrefixParams& p, int items, int unit, int at,
-                                                int end) {
-  int lo = 0, hi = items;                      // the last item that starts at or before `at`
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.items[mid].start <= at) lo = mid; else hi = mid;
+struct PrefixWalk {
+  int item, at, end;
+  __device__ __forceinline__ bool next(const PrefixParams& p, PrefixSeg& s) {
+    if (at >= end) return false;
+    if (item < 0) item = p.cta_item[blockIdx.x];
+    s.it = p.items[item];
+    if (at >= s.it.start + s.it.tiles * p.hkv) s.it = p.items[++item];
+    const int in = at - s.it.start;
+    s.kvh = in / s.it.tiles;
+    s.t0 = in - s.kvh * s.it.tiles;
+    s.t1 = min(s.it.tiles, s.t0 + end - at);
+    s.slot = (int)blockIdx.x + item * p.hkv + s.kvh;
+    s.two = s.it.rows > p.per_tile ? 1 : 0;
+    at += s.t1 - s.t0;
+    return true;
   }
-  const PrefixItem it = p.items[lo];
-  PrefixSeg s;
-  s.row0 = it.row0; s.rows = it.rows; s.table = it.table; s.keys = it.keys;
-  const int in = at - it.start;
-  s.kvh = in / it.tiles;
-  s.t0 = in - s.kvh * it.tiles;
-  s.t1 = min(it.tiles, s.t0 + end - at);
-  s.split = (int)blockIdx.x - (it.start + s.kvh * it.tiles) / unit;
-  s.two = it.rows > p.per_tile ? 1 : 0;
-  return s;
-}
+};
 
 __global__ void __launch_bounds__(PX_THREADS, 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
@@ -443,15 +481,16 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(px_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + PX_OFF_BAR);
-  uint64_t* q_empty = q_full + 1;
+  uint64_t* q_empty = q_full + 1;                    // the last S product of a split has been read
   uint64_t* slot_full = q_full + 2;
   uint64_t* slot_empty = slot_full + PX_SLOTS;
   uint64_t* s_full = slot_empty + PX_SLOTS;          // [2]
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* o_empty = o_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(o_empty + 3);
+  uint64_t* staged = o_empty + 2;                    // results have left the query tile's place
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staged + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(staged + 3);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -464,9 +503,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[t], 8);
       mbar_init(&o_full[t], 1);
-      mbar_init(&o_empty[t], 4);
+      mbar_init(&o_empty[t], 8);
+      mbar_init(&staged[t], 8);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -484,42 +524,49 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
   const uint32_t tmem_got = *tmem_slot;
   constexpr uint32_t tmem_base = 0;
   pdl_wait();     // the schedule, q and the cache may come from earlier kernels
-  const int items = p.hdr[PLAN_ITEMS], unit = p.hdr[PLAN_UNIT], total = p.hdr[PLAN_TILES];
+  const int unit = p.hdr[PLAN_UNIT], total = p.hdr[PLAN_TILES];
   const int64_t from = (int64_t)blockIdx.x * unit;
   const int begin = (int)(from < total ? from : total);
   const int end = tmem_got != 0 ? begin : min(total - begin, unit) + begin;
   if (tmem_got != 0 && threadIdx.x == 0 && p.status) atomicOr(p.status, FK_DEV_TMEM_BASE);
+  PrefixWalk walk{-1, begin, end};
 
   if (warp == PX_WARP_TMA) {
     const int st = p.sub_tokens, npieces = 128 / st;
-    int kv_idx = 0, q_loads = 0;
+    int kv_idx = 0, segs = 0, before = 0;
+    uint32_t uses[2] = {0, 0};                 // splits that had query tile t
     bool ok = true;
-    for (int at = begin; ok && at < end;) {
-      const PrefixSeg sg = px_segment(p, items, unit, at, end);
-      at += sg.t1 - sg.t0;
+    PrefixSeg w;
+    while (ok && walk.next(p, w)) {
       int pass = 1;
       if (lane == 0) {
-        if (q_loads > 0)
-          pass = px_poll(q_empty, (uint32_t)(q_loads - 1) & 1u, abort_flag, p.status) ? 1 : 0;
+        if (segs > 0) {
+          pass = px_poll(q_empty, (uint32_t)(segs - 1) & 1u, abort_flag, p.status) ? 1 : 0;
+          for (int t = 0; t <= before && pass; ++t)
+            pass = px_poll(&staged[t], (uses[t] - 1) & 1u, abort_flag, p.status) ? 1 : 0;
+        }
         if (pass) {
-          mbar_arrive_expect_tx(q_full, (uint32_t)(1 + sg.two) * 2u * 128u *
+          mbar_arrive_expect_tx(q_full, (uint32_t)(1 + w.two) * 2u * 128u *
                                             (uint32_t)(p.g * p.per_tile));
-          for (int t = 0; t <= sg.two; ++t)
+          for (int t = 0; t <= w.two; ++t)
             for (int dh = 0; dh < 2; ++dh)
               tma_load_4d(smem + PX_OFF_Q + t * PX_TILE_BYTES + dh * PX_HALF_BYTES, &tmap_q, q_full,
-                          dh * 64, sg.kvh * p.g, sg.row0 + t * p.per_tile, 0);
+                          dh * 64, w.kvh * p.g, w.it.row0 + t * p.per_tile, 0);
         }
       }
       pass = __shfl_sync(0xffffffffu, pass, 0);
       if (!pass) { ok = false; break; }
-      ++q_loads;
-      const int32_t* bt = p.tables + (int64_t)sg.table * p.table_stride;
-      for (int i = 2 * sg.t0; i < 2 * sg.t1; ++i, ++kv_idx) {
+      ++segs;
+      ++uses[0];
+      if (w.two) ++uses[1];
+      before = w.two;
+      const int32_t* bt = p.tables + (int64_t)w.it.table * p.table_stride;
+      for (int i = 2 * w.t0; i < 2 * w.t1; ++i, ++kv_idx) {
         const int slot = kv_idx % PX_SLOTS;
         const uint32_t lap = (uint32_t)(kv_idx / PX_SLOTS) & 1u;
         const int tok = (i >> 1) * 128 + lane * st;
         int page = p.num_blocks;               // past the end: the copy reads the zero fill
-        if (lane < npieces && tok < sg.keys) {
+        if (lane < npieces && tok < w.it.keys) {
           page = bt[tok / p.block_size];
           if (page < 0 || page >= p.num_blocks) {
             page = p.num_blocks;
@@ -536,7 +583,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
           uint8_t* dst = smem + PX_OFF_KV + slot * PX_TILE_BYTES + lane * st * 128;
           const CUtensorMap* map = i & 1 ? &tmap_v : &tmap_k;
           const int off = tok % p.block_size;
-          const int c1 = p.hnd ? off : sg.kvh, c2 = p.hnd ? sg.kvh : off;
+          const int c1 = p.hnd ? off : w.kvh, c2 = p.hnd ? w.kvh : off;
           tma_load_4d(dst, map, &slot_full[slot], 0, c1, c2, page);
           tma_load_4d(dst + PX_HALF_BYTES, map, &slot_full[slot], 64, c1, c2, page);
         }
@@ -562,12 +609,13 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
       __syncwarp();
     };
     auto issue_pv = [&](int t, int slot, bool acc) {
+      // weights of keys 0 .. 63 in columns 0 .. 31 of S_t, of the others in columns 64 .. 95
       const uint32_t a = tmem_base + t * 128;
       const uint32_t b = kv_addr + slot * PX_TILE_BYTES;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          tc_mma_bf16_ts(tmem_base + 256 + t * SH_D, a + kk * 8,
+          tc_mma_bf16_ts(tmem_base + 256 + t * SH_D, a + (kk >> 2) * 64 + (kk & 3) * 8,
                          smem_desc_sw128_mn(b + kk * 2048, PX_HALF_BYTES, 1024), idesc_pv,
                          (acc || kk > 0) ? 1u : 0u);
       }
@@ -576,10 +624,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
     int kv_base = 0, segs = 0;
     uint32_t n_sp[2] = {0, 0}, n_o[2] = {0, 0};   // hand-overs and splits per query tile so far
     bool ok = true;
-    for (int at = begin; ok && at < end;) {
-      const PrefixSeg sg = px_segment(p, items, unit, at, end);
-      const int n = sg.t1 - sg.t0, qt = 1 + sg.two;
-      at += n;
+    PrefixSeg w;
+    while (ok && walk.next(p, w)) {
+      const int n = w.t1 - w.t0, qt = 1 + w.two;
       ok = px_wait_warp(q_full, (uint32_t)segs & 1u, abort_flag, p.status) &&
            px_wait_warp(&slot_full[kv_base % PX_SLOTS], (uint32_t)(kv_base / PX_SLOTS) & 1u,
                         abort_flag, p.status);
@@ -634,81 +681,80 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
       }
     }
   } else {
-    const int t = warp >> 2, quad = warp & 3;
-    const int row = quad * 32 + lane;
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16);
-    const uint32_t s_addr = lane_addr + t * 128;
-    const uint32_t o_addr = lane_addr + 256 + t * SH_D;
-    const float sc = p.scale_log2;
-    const uint64_t sc2 = px_pack2(sc, sc);
-    const int in_tile = row / p.g, head_in = row - in_tile * p.g;
+    const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+    const uint32_t s_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + t * 128 + half * 64;
+    const uint32_t o_addr = s_addr + 256;
+    // maxima of the two threads of a row, as bf16 rounded up: the reference value of a row's
+    // exponentials has to be the same for both, not the maximum itself
+    const uint32_t max_at = smem_u32(smem + PX_OFF_MAX) + t * 512 + (quad * 32 + lane) * 2;
+    constexpr uint32_t kGone = 0x7fffu;        // no number: this warp's wait has run out
     uint32_t n_sp = 0, n_o = 0;
     bool ok = true;
-    for (int at = begin; ok && at < end;) {
-      int n, lim, kpos;
-      int64_t part;                            // of this row's results, -1: no row
+    for (;;) {
+      int n, kpos, lim = 0, slot;
       {
-        const PrefixSeg sg = px_segment(p, items, unit, at, end);
-        n = sg.t1 - sg.t0;
-        at += n;
-        if (t > sg.two) continue;
-        const int i = t * p.per_tile + in_tile;
-        lim = 0;
-        part = -1;
-        if (in_tile < p.per_tile && i < sg.rows) {
-          const int64_t len = p.lens[sg.row0 + i];
-          lim = (int)(len < 0 ? 0 : len < sg.keys ? len : sg.keys);
-          part = ((int64_t)(sg.row0 + i) * p.hq + sg.kvh * p.g + head_in) * p.splits + sg.split;
+        PrefixSeg w;
+        if (!walk.next(p, w)) break;
+        if (t > w.two) continue;
+        n = w.t1 - w.t0;
+        kpos = w.t0 * 128 + half * 64;
+        slot = w.slot;
+        const int in_tile = (quad * 32 + lane) / p.g, i = t * p.per_tile + in_tile;
+        if (in_tile < p.per_tile && i < w.it.rows) {
+          const int64_t len = p.lens[w.it.row0 + i];
+          lim = (int)(len < 0 ? 0 : len < w.it.keys ? len : w.it.keys);
         }
-        kpos = sg.t0 * 128;
       }
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, kpos += 128) {
-        if (!px_wait_warp(&s_full[t], (n_sp + (uint32_t)j) & 1u, abort_flag, p.status)) {
-          ok = false;
-          break;
-        }
+        // Two warps have a row between them and meet at a barrier in every step: one whose wait has
+        // run out says so there, and both leave.
+        ok = ok && px_wait_warp(&s_full[t], (n_sp + (uint32_t)j) & 1u, abort_flag, p.status);
+        // (scores of a step whose wait ran out are not used)
         tc_fence_after();
-        // The row is read twice, half by half: registers for all of it at once would spill.
-        auto half_row = [&](int half, uint32_t (&v)[64]) {
-          tc_ld32(s_addr + half * 64, v);
-          tc_ld32(s_addr + half * 64 + 32, v + 32);
-          tc_wait_ld();
-          const int first = kpos + half * 64;
-          if (first + 64 > lim) {
+        uint32_t v[64];                        // scores, then weights two a word
+        tc_ld32(s_addr, v);
+        tc_ld32(s_addr + 32, v + 32);
+        tc_wait_ld();
+        if (kpos + 64 > lim) {
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (first + c >= lim) v[c] = 0xff800000u;   // -inf
-          }
-        };
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t v[64];
-          half_row(half, v);
-#pragma unroll
-          for (int c = 0; c < 64; c += 8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mx4[i] = px_max3(mx4[i], __uint_as_float(v[c + i]), __uint_as_float(v[c + 4 + i]));
-          }
-          __syncwarp();
+          for (int i = 0; i < 64; ++i)
+            if (kpos + i >= lim) v[i] = 0xff800000u;   // -inf
         }
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+        float mx = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+          mx = px_max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          m2 = px_max3(m2, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+        }
+        mx = fmaxf(mx, m2);
+        {
+          const uint32_t a = ok ? __bfloat16_as_ushort(__float2bfloat16_ru(mx)) : kGone;
+          uint32_t b;
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(max_at + half * 256), "h"((uint16_t)a)
+                       : "memory");
+          named_bar_sync(1 + t * 4 + quad, 64);
+          asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+                       : "=r"(b) : "r"(max_at + (half ^ 1) * 256) : "memory");
+          ok = a != kGone && b != kGone;       // the same for both warps: one flag for all lanes
+          mx = fmaxf(bf16_bits_to_float(a), bf16_bits_to_float(b)) * p.scale_log2;
+        }
+        if (!ok) break;
         if (j == 0) {
           m_used = mx;
         } else {
           const bool grow = mx > m_used + PX_RESCALE_LOG2;
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? fast_exp2(m_used - mx) : 1.0f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[32];
-              tc_ld32(o_addr + c * 32, o);
+            // eight columns at a time: the scores keep their registers
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[8];
+              px_ld8(o_addr + c * 8, o);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tc_st32(o_addr + c * 32, o);
+              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              px_st8(o_addr + c * 8, o);
             }
             tc_wait_st();
             if (grow) {
@@ -718,72 +764,84 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
           }
         }
         const float neg_mu = m_used == -INFINITY ? 0.f : -m_used;
-        const uint64_t nm2 = px_pack2(neg_mu, neg_mu);
+        const uint64_t nm2 = px_pack2(neg_mu, neg_mu), sc2 = px_pack2(p.scale_log2, p.scale_log2);
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t v[64];
-          half_row(half, v);
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float t0, t1, t2, t3;
-            px_unpack2(px_fma2(px_pack2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
-                               sc2, nm2), t0, t1);
-            px_unpack2(px_fma2(px_pack2(__uint_as_float(v[2 * c + 2]),
-                                        __uint_as_float(v[2 * c + 3])), sc2, nm2), t2, t3);
-            const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
-            const float e2 = fast_exp2(t2), e3 = fast_exp2(t3);
-            sum2[0] = px_add2(sum2[0], px_pack2(e0, e1));
-            sum2[1] = px_add2(sum2[1], px_pack2(e2, e3));
-            v[c] = pack_bf16(e0, e1);
-            v[c + 1] = pack_bf16(e2, e3);
-          }
-          // over columns of S that have been read
-          __syncwarp();
-          tc_st32(s_addr + half * 32, v);
+        for (int i = 0; i < 64; i += 4) {
+          float t0, t1, t2, t3;
+          px_unpack2(px_fma2(px_pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2),
+                     t0, t1);
+          px_unpack2(px_fma2(px_pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2,
+                             nm2), t2, t3);
+          const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
+          const float e2 = fast_exp2(t2), e3 = fast_exp2(t3);
+          sum2[0] = px_add2(sum2[0], px_pack2(e0, e1));
+          sum2[1] = px_add2(sum2[1], px_pack2(e2, e3));
+          v[i / 2] = pack_bf16(e0, e1);
+          v[i / 2 + 1] = pack_bf16(e2, e3);
         }
+        __syncwarp();
         {
           float a0, a1, a2, a3;
           px_unpack2(sum2[0], a0, a1);
           px_unpack2(sum2[1], a2, a3);
           l += (a0 + a1) + (a2 + a3);
         }
+        tc_st32(s_addr, v);                    // over what this warp has read
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
-      if (!px_wait_warp(&o_full[t], n_o & 1u, abort_flag, p.status)) {
-        ok = false;
-        break;
-      }
+      // a warp whose wait runs out here goes on to the next step's barrier, and says so there
+      ok = px_wait_warp(&o_full[t], n_o & 1u, abort_flag, p.status);
+      n_sp += (uint32_t)n;
+      ++n_o;
+      if (!ok) continue;
       tc_fence_after();
-      if (m_used == -INFINITY) l = 0.f;        // no key: the sum says that there is no row
-      float4* dst = reinterpret_cast<float4*>(p.part_o + part * SH_D);
+      if (m_used == -INFINITY) l = 0.f;        // no key
+      float* dst = p.part_o + (int64_t)slot * PX_SLOT_FLOATS + ((t * 4 + quad) * 2 + half) * 2048;
+      uint8_t* stage = smem + PX_OFF_Q + t * PX_TILE_BYTES + (half * 4 + quad) * 4096;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t o[32];
         tc_ld32(o_addr + c * 32, o);
         tc_wait_ld();
-        if (c == 3) {
+        if (c == 1) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&o_empty[t]);
+          if (lane == 0) {
+            mbar_arrive(&o_empty[t]);
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          }
+          __syncwarp();
         }
-        if (part >= 0 && l > 0.f) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[c * 8 + i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                         __uint_as_float(o[4 * i + 2]),
-                                         __uint_as_float(o[4 * i + 3]));
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+              make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                           dst + c * 1024),
+                       "r"(smem_u32(stage)), "r"(4096)
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
         __syncwarp();
       }
-      if (part >= 0) p.part_ml[part] = make_float2(m_used, l);
-      n_sp += (uint32_t)n;
-      ++n_o;
+      p.part_ml[(int64_t)slot * 512 + (t * 2 + half) * 128 + quad * 32 + lane] =
+          make_float2(m_used, l);
+      if (lane == 0) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        mbar_arrive(&staged[t]);
+      }
+      __syncwarp();
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -799,9 +857,9 @@ struct SharedJoinParams {
   const int* hdr; const int* row_item; const PrefixItem* items;
   int* counter;
   uint16_t* out; int64_t out_stride;
-  const float* pre_o; const float2* pre_ml; int pre_splits;
+  const float* pre_o; const float2* pre_ml;
   const float* own_o; const float2* own_ml; int own_splits;
-  int batch, hq, g;
+  int batch, hq, hkv, g, per_tile;
 };
 __global__ void __launch_bounds__(256) shared_join_kernel(const SharedJoinParams p) {
   pdl_launch_dependents();
@@ -816,19 +874,38 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const SharedJoinParams
   const int n_own = chunk_start[row + 1] - chunk_start[row];
   const int item = p.row_item[row];
   int n_pre = 0;
+  int64_t slot = 0;                            // of the first split
+  int at = 0;                                  // row among the two tiles of a split
   if (item >= 0) {
-    const int tiles = p.items[item].tiles, unit = p.hdr[PLAN_UNIT];
-    const int first = p.items[item].start + head / p.g * tiles;
-    n_pre = (first + tiles - 1) / unit - first / unit + 1;
+    const PrefixItem it = p.items[item];
+    const int unit = p.hdr[PLAN_UNIT], kvh = head / p.g;
+    const int first = it.start + kvh * it.tiles;
+    n_pre = (first + it.tiles - 1) / unit - first / unit + 1;
+    slot = first / unit + item * p.hkv + kvh;
+    const int i = row - it.row0, t = i / p.per_tile;
+    at = t * 128 + (i - t * p.per_tile) * p.g + head - kvh * p.g;
   }
   if (n_pre == 0 && n_own == 1) return;        // written by the decode kernel
-  const float2* pre_ml = p.pre_ml + gw * p.pre_splits;
-  const float2* own_ml = p.own_ml + gw * p.own_splits;
+  // the sum of a row over both halves of the keys, and this lane's piece of its channels
+  const int64_t ml_at = slot * 512 + (at >> 7) * 256 + (at & 127);
+  auto pre_ml = [&](int s) {
+    const float2 a = p.pre_ml[ml_at + (int64_t)s * 512], b = p.pre_ml[ml_at + (int64_t)s * 512 + 128];
+    return make_float2(a.x, a.y + b.y);
+  };
+  const float* pre_at = p.pre_o + slot * PX_SLOT_FLOATS + (at >> 5) * 4096 + (lane >> 3) * 1024 +
+                        (at & 31) * 32 + (((lane ^ at) & 7) << 2);
+  auto pre_row = [&](int s) {
+    return reinterpret_cast<const float4*>(pre_at + (int64_t)s * PX_SLOT_FLOATS);
+  };
+  auto own_ml = [&](int s) { return p.own_ml[gw * p.own_splits + s]; };
+  auto own_row = [&](int s) {
+    return reinterpret_cast<const float4*>(p.own_o + (gw * p.own_splits + s) * SH_D) + lane;
+  };
   float top = fmaxf(join_max(pre_ml, n_pre, lane), join_max(own_ml, n_own, lane));
   if (top == -INFINITY) top = 0.f;
   JoinRow r{make_float4(0.f, 0.f, 0.f, 0.f), 0.f};
-  join_add(r, p.pre_o + gw * p.pre_splits * SH_D, pre_ml, n_pre, top, lane);
-  join_add(r, p.own_o + gw * p.own_splits * SH_D, own_ml, n_own, top, lane);
+  join_add(r, pre_ml, pre_row, n_pre, top, lane);
+  join_add(r, own_ml, own_row, n_own, top, lane);
   Elem<uint16_t>::store4(p.out + (int64_t)row * p.out_stride + (int64_t)head * SH_D + lane * 4,
                          r.acc * (r.l > 0.f ? 1.0f / r.l : 0.f));
 }
@@ -876,14 +953,15 @@ static int get_q_map(const QMapKey& key, CUtensorMap* out) {
   return FK_OK;
 }
 
+// longest tables of a call that is one launch
+constexpr int SHARED_DIRECT_TOKENS = 2048;
 // fewest 128-key tiles of the common part that a CTA takes
 constexpr int PREFIX_MIN_UNIT = 2;
 
 struct SharedLayout {
-  size_t row_item, row_from, items, chunks, pre_o, pre_ml, own_o, own_ml, total;
-  int pre_splits;
+  size_t row_item, cta_item, items, chunks, pre_o, pre_ml, own_o, own_ml, total;
 };
-static SharedLayout shared_layout(int64_t batch, int hq, int hkv, int max_splits) {
+static SharedLayout shared_layout(int64_t batch, int groups, int hq, int hkv, int max_splits) {
   SharedLayout s;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -891,17 +969,18 @@ static SharedLayout shared_layout(int64_t batch, int hq, int hkv, int max_splits
     at = (at + bytes + 255) & ~size_t(255);
     return here;
   };
+  // an item has at least one full group's rest, or the rows of two query tiles
+  const int64_t span = 2 * (128 / (hq / hkv));
+  const int64_t items = groups < 1 ? 0 : groups + batch / span < batch ? groups + batch / span : batch;
+  const int64_t slots = items == 0 ? 0 : sm_count() + items * hkv;
   take((PLAN_HDR + batch + 1) * sizeof(int));
   s.row_item = take(batch * sizeof(int));
-  s.row_from = take(batch * sizeof(int));
-  s.items = take(batch * sizeof(PrefixItem));
+  s.cta_item = take(sm_count() * sizeof(int));
+  s.items = take(items * sizeof(PrefixItem));
   s.chunks = take((size_t)batch * max_splits * sizeof(int4));
-  // A CTA takes at least 1 / ctas of all tiles, those of all KV heads of an item among them, so that
-  // an item and head falls on at most ctas / hkv CTAs and one more on either side.
-  s.pre_splits = sm_count() / hkv + 2;
+  s.pre_o = take((size_t)slots * PX_SLOT_FLOATS * sizeof(float));
+  s.pre_ml = take((size_t)slots * 512 * sizeof(float2));
   const size_t rows = (size_t)batch * hq;
-  s.pre_o = take(rows * s.pre_splits * SH_D * sizeof(float));
-  s.pre_ml = take(rows * s.pre_splits * sizeof(float2));
   s.own_o = take(rows * max_splits * SH_D * sizeof(float));
   s.own_ml = take(rows * max_splits * sizeof(float2));
   s.total = at;
@@ -1034,9 +1113,9 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
 size_t fk_shared_prefix_workspace_bytes(int batch, int num_groups, int num_q_heads,
                                         int num_kv_heads, int head_dim, int max_splits) {
   if (batch <= 0 || num_groups < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
-      max_splits <= 0)
+      max_splits <= 0 || num_q_heads < num_kv_heads || num_q_heads / num_kv_heads > SH_MAX_G)
     return 0;
-  return shared_layout(batch, num_q_heads, num_kv_heads, max_splits).total;
+  return shared_layout(batch, num_groups, num_q_heads, num_kv_heads, max_splits).total;
 }
 
 int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
@@ -1066,7 +1145,10 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   FK_REQUIRE((int64_t)batch * num_kv_heads * ((r.capacity + ATT_TILE - 1) / ATT_TILE) <
                  (1ll << 31) - (1 << 20),
              FK_ERR_UNSUPPORTED, "fk_shared_prefix_attn: batch and tables too large");
-  const SharedLayout w = shared_layout(batch, num_q_heads, num_kv_heads, max_splits);
+  FK_REQUIRE(batch <= PLAN_MAX_BATCH, FK_ERR_UNSUPPORTED, "fk_shared_prefix_attn: more than %d rows",
+             PLAN_MAX_BATCH);
+  const SharedLayout w = shared_layout(batch, num_groups, num_q_heads, num_kv_heads,
+                                       max_splits);
   FK_REQUIRE(workspace != nullptr && workspace_bytes >= w.total &&
                  (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
              FK_ERR_WORKSPACE,
@@ -1084,7 +1166,7 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   pl.capacity = r.capacity;
   pl.plan.hdr = reinterpret_cast<int*>(ws);
   pl.plan.row_item = reinterpret_cast<int*>(ws + w.row_item);
-  pl.plan.row_from = reinterpret_cast<int*>(ws + w.row_from);
+  pl.plan.cta_item = reinterpret_cast<int*>(ws + w.cta_item);
   pl.plan.items = reinterpret_cast<PrefixItem*>(ws + w.items);
   pl.plan.chunks = reinterpret_cast<int4*>(ws + w.chunks);
   pl.status = status;
@@ -1110,17 +1192,15 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   if (rc != FK_OK) return rc;
 
   PrefixParams px{};
-  px.hdr = pl.plan.hdr; px.items = pl.plan.items;
+  px.hdr = pl.plan.hdr; px.cta_item = pl.plan.cta_item; px.items = pl.plan.items;
   px.lens = context_lens;
   px.tables = block_tables; px.table_stride = block_table_stride;
   px.hq = num_q_heads; px.hkv = num_kv_heads; px.g = g; px.per_tile = per_tile;
   px.hnd = kv_layout; px.block_size = page_size; px.sub_tokens = sub;
   px.num_blocks = (int)num_pages;
   px.scale_log2 = r.scale_log2;
-  px.capacity = r.capacity;
   px.part_o = reinterpret_cast<float*>(ws + w.pre_o);
   px.part_ml = reinterpret_cast<float2*>(ws + w.pre_ml);
-  px.splits = w.pre_splits;
   px.status = status;
 
   AttnParams a{};
@@ -1142,15 +1222,30 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   a.part_ml = reinterpret_cast<float2*>(ws + w.own_ml);
   a.status = status;
 
+  // Small calls as fk_paged_decode_attn has them: a CTA per row and KV head, which read the common part
+  // from L2, in one launch instead of four that wait for one another (8 rows of 512 common tokens
+  // and up to 200 of their own, 32/8 heads: 30.6 -> FIXME us).
+  if ((int64_t)batch * num_kv_heads <= sms && r.capacity <= SHARED_DIRECT_TOKENS) {
+    a.direct = 1;
+    a.capacity = r.capacity;
+    a.starts = group_starts; a.groups = num_groups;
+    FK_CUDA_OK(launch_decode(g > 8, false, false, batch * num_kv_heads, dk, dv, a, s));
+    count_launch(1);
+    return FK_OK;
+  }
+
   SharedJoinParams jn{};
   jn.hdr = pl.plan.hdr; jn.row_item = pl.plan.row_item; jn.items = pl.plan.items;
   jn.counter = pl.plan.hdr + PLAN_COUNTER;
   jn.out = r.out; jn.out_stride = r.out_stride;
-  jn.pre_o = px.part_o; jn.pre_ml = px.part_ml; jn.pre_splits = w.pre_splits;
+  jn.pre_o = px.part_o; jn.pre_ml = px.part_ml;
   jn.own_o = a.part_o; jn.own_ml = a.part_ml; jn.own_splits = max_splits;
-  jn.batch = batch; jn.hq = num_q_heads; jn.g = g;
+  jn.batch = batch; jn.hq = num_q_heads; jn.hkv = num_kv_heads; jn.g = g; jn.per_tile = per_tile;
 
-  FK_CUDA_OK(launch_kernel(shared_plan_kernel, dim3(1), dim3(PLAN_THREADS), (size_t)0, s, pl));
+  static PerDeviceOnce plan_once;
+  FK_CUDA_OK(set_max_dynamic_smem(plan_once, shared_plan_kernel, PLAN_MAX_BATCH * 8));
+  FK_CUDA_OK(launch_kernel(shared_plan_kernel, dim3(1), dim3(PLAN_THREADS), (size_t)batch * 8, s,
+                           pl));
   count_launch(1);
   if (num_groups > 0) {
     static PerDeviceOnce once;
