@@ -414,8 +414,10 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
   }
   pdl_launch_dependents();
   __syncthreads();
-  // everything below reads memory written by earlier kernels (plan, q, KV pool)
-  pdl_wait();
+  // Everything below reads memory written by earlier kernels (plan, q, KV pool).  Beside its
+  // predecessor the kernel waits for it when it has done its own work, so that whoever waits for this
+  // one waits for both; what it reads was there before that predecessor let it start.
+  if (!p.beside) pdl_wait();
 
   const int* plan = p.plan;
 
@@ -433,7 +435,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
       att_produce_selected(tmap_k, tmap_v, p, stages, qslots, metas, full, empty, abort_flag, lane);
       return;
     }
-    const int total_items = p.direct ? p.batch * p.hkv : plan[0] * p.hkv;
+    const int total_items = p.direct ? p.batch * p.hkv : __ldcg(plan) * p.hkv;
     int* counter = const_cast<int*>(plan) + 2;
     // direct mode: the schedule entry of item (sequence, KV head) is the whole
     // sequence as one unsplit chunk; lengths are clamped as the plan kernel does
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
     }
     int4 next_info = make_int4(0, 0, 0, 0);
     if (next < total_items)
-      next_info = p.direct ? direct_info(next) : p.chunk_info[next / p.hkv];
+      next_info = p.direct ? direct_info(next) : __ldcg(p.chunk_info + next / p.hkv);
     while (ok) {
       const int item = next;
       if (item >= total_items) break;
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
       } else {
         if (lane == 0) next = atomicAdd(counter, 1);
         next = __shfl_sync(0xffffffffu, next, 0);
-        if (next < total_items) next_info = p.chunk_info[next / p.hkv];
+        if (next < total_items) next_info = __ldcg(p.chunk_info + next / p.hkv);
       }
       const int kvh = item % p.hkv;
       const int seq = info.x;
@@ -579,6 +581,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
         mbar_arrive(&full[stage]);
       }
     }
+    if (p.beside) pdl_wait();
     return;
   }
 
@@ -848,6 +851,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
     }
     if (++stage == ATT_STAGES) { stage = 0; phase ^= 1; }
   }
+  if (p.beside) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------

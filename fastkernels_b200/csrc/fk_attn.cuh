@@ -19,6 +19,7 @@ struct AttnParams {
   float scale_log2;
   int max_splits;
   int direct;         // 1: no plan, no splits: CTA b handles (sequence, KV head) item b whole
+  int beside;         // 1: runs beside the kernel before it, which has seen the plan's kernel end
   int* plan;          // header + chunk_start[batch+1]
   int4* chunk_info;   // per chunk: {seq, split | nsplits << 16, tok_begin, tok_end}
   float* part_o;      // [batch, hq, max_splits, D]

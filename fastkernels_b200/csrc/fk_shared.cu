@@ -36,7 +36,7 @@ struct RowsParams {
 // splits of a token and head joined: out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M)
 // ---------------------------------------------------------------------------
 // A lane has the (max, sum) of splits lane, lane + 32, ..., so all of them are one round of loads, and
-// eight partial rows are on the way at a time.  A split without keys has a sum of zero; its row was
+// four partial rows are on the way at a time.  A split without keys has a sum of zero; its row was
 // not written and is not read.
 struct JoinRow {
   float4 acc;
@@ -58,17 +58,17 @@ __device__ __forceinline__ void join_add(JoinRow& r, const ML& ml, const ROW& ro
     const float2 mlv = s0 + lane < n ? ml(s0 + lane) : make_float2(-INFINITY, 0.f);
     const float fl = mlv.y > 0.f ? fast_exp2(mlv.x - top) : 0.f;
     const int cnt = min(32, n - s0);
-    for (int s = 0; s < cnt; s += 8) {
-      float4 v[8];
-      float f[8], l[8];
+    for (int s = 0; s < cnt; s += 4) {
+      float4 v[4];
+      float f[4], l[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         f[i] = __shfl_sync(0xffffffffu, fl, (s + i) & 31);
         l[i] = s + i < cnt ? __shfl_sync(0xffffffffu, mlv.y, (s + i) & 31) : 0.f;
         v[i] = l[i] > 0.f ? *row(s0 + s + i) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         r.l = fmaf(l[i], f[i], r.l);
         r.acc = r.acc + v[i] * f[i];
       }
@@ -137,7 +137,8 @@ enum : int { PLAN_CHUNKS = 0, PLAN_COUNTER = 2, PLAN_ITEMS = 4, PLAN_TILES = 5, 
 
 struct SharedPlan {
   int* hdr;            // see above; chunk_start[batch + 1] behind it, as the decode kernel has it
-  int* row_item;       // [batch] item that holds a row, -1: none
+  int4* row_part;      // [batch] start and tiles of the item that holds a row, item * hkv, its
+                       // number among the item's rows; tiles 0: none
   int* cta_item;       // [ctas] item of a CTA's first tile
   PrefixItem* items;
   int4* chunks;        // chunks of what each row has for itself
@@ -146,112 +147,105 @@ struct SharedPlan {
 struct SharedPlanParams {
   const int32_t* lens; const int32_t* starts; const int32_t* prefix;
   int batch, groups, hkv, page, per_tile, max_splits, ctas, min_unit;
+  int beside;          // the decode kernel may run beside the common part's
   int64_t capacity;
   SharedPlan plan;
   int32_t* status;
 };
 
 constexpr int PLAN_MAX_BATCH = 16384;
+constexpr int PLAN_THREADS = 512;
+constexpr int PLAN_WARPS = PLAN_THREADS / 32;
 
-constexpr int PLAN_THREADS = 1024;
-
-__device__ __forceinline__ int plan_sum(int v, int* red) {     // over the block, for all
+// Sum of the threads before this one, and of all.
+__device__ __forceinline__ int64_t plan_before(int64_t v, int64_t* red, int64_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  v = red[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-// sum of the threads before this one
-__device__ __forceinline__ int plan_before(int v, int* red, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int upto = v;
+  int64_t upto = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += u;
   }
   __syncthreads();
   if (lane == 31) red[warp] = upto;
   __syncthreads();
-  int w = red[lane], wi = w;
+  int64_t before = upto - v, all = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, wi, o);
-    if (lane >= o) wi += u;
+  for (int w = 0; w < PLAN_WARPS; ++w) {
+    if (w < warp) before += red[w];
+    all += red[w];
   }
-  *total = __shfl_sync(0xffffffffu, wi, 31);
-  return __shfl_sync(0xffffffffu, wi - w, warp) + upto - v;
+  *total = all;
+  return before;
 }
+
+// How many of the SMs take the common part: of its tiles and of those that rows have for themselves
+// (128 keys of a KV head each) one of the first takes an SM 2.2 us, one of the second 0.8 us where
+// memory does not bound it.  The other SMs start with the second kind, and take it over together
+// when the common part is through.
+constexpr int PLAN_COMMON_COST = 22, PLAN_OWN_COST = 8;
 
 __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedPlanParams p) {
   extern __shared__ int plan_smem[];
   int* s_len = plan_smem;                      // [batch] tokens of a row
   int* s_from = plan_smem + p.batch;           // [batch] of them in its item
-  __shared__ int red[32];
+  __shared__ int64_t red[PLAN_WARPS];
   __shared__ int s_keys[PLAN_THREADS], s_table[PLAN_THREADS], s_item[PLAN_THREADS],
-      s_start[PLAN_THREADS];
-  const int tid = threadIdx.x;
+      s_start[PLAN_THREADS], s_count[6];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   pdl_wait();
-  bool cut = false;
+  bool cut = false, odd = false;
   for (int i = tid; i < p.batch; i += PLAN_THREADS) {
     const int64_t len = p.lens[i];
     cut |= len > p.capacity;
     s_len[i] = len < 0 ? 0 : (int)(len > p.capacity ? p.capacity : len);
     s_from[i] = 0;
-    p.plan.row_item[i] = -1;
+    p.plan.row_part[i] = make_int4(0, 0, 0, 0);
   }
   if (cut && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+  if (tid < 6) s_count[tid] = 0;
 
-  // Groups into items, 1024 groups at a time: a warp looks for the longest row of a group, a thread
-  // per group adds up, a warp per group writes.  Starts that do not ascend within the batch: nobody
-  // has anything in common then.
-  bool odd = false;
+  // Groups into items, a round of them at a time: a warp looks for the longest row of a group, a
+  // thread per group adds up, a warp per group writes.  Starts that do not ascend within the batch:
+  // nobody has anything in common then.
   for (int g = tid; g < p.groups; g += PLAN_THREADS)
     odd |= p.starts[g] < 0 || p.starts[g + 1] < p.starts[g] || p.starts[g + 1] > p.batch;
   odd = __syncthreads_or(odd);
   if (odd && tid == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_POSITION);
   const int groups = odd ? 0 : p.groups;
-  const int warp = tid >> 5, lane = tid & 31;
+  const int span = 2 * p.per_tile;
   int items = 0, tiles = 0;                    // of the groups before
   for (int g0 = 0; g0 < groups; g0 += PLAN_THREADS) {
     const int here = min(PLAN_THREADS, groups - g0);
-    for (int i = warp; i < here; i += PLAN_THREADS / 32) {
-      const int a = p.starts[g0 + i], b = p.starts[g0 + i + 1];
+    for (int i = warp; i < here; i += PLAN_WARPS) {
+      const int a = p.starts[g0 + i], b = p.starts[g0 + i + 1], prefix = p.prefix[g0 + i];
       int longest = 0, table = a;
       for (int r = a + lane; r < b; r += 32) {
         const int n = s_len[r];
         if (n > longest) { longest = n; table = r; }
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const int n = __shfl_xor_sync(0xffffffffu, longest, o);
-        const int r = __shfl_xor_sync(0xffffffffu, table, o);
-        if (n > longest || (n == longest && r < table)) { longest = n; table = r; }
-      }
+      const int most = __reduce_max_sync(0xffffffffu, longest);
+      table = __reduce_min_sync(0xffffffffu, longest == most ? table : 0x7fffffff);
       if (lane == 0) {
-        s_keys[i] = b - a < 2 ? 0 : max(0, min(p.prefix[g0 + i], longest)) / p.page * p.page;
+        s_keys[i] = b - a < 2 ? 0 : max(0, min(prefix, most)) / p.page * p.page;
         s_table[i] = table;
       }
     }
     __syncthreads();
-    const int span = 2 * p.per_tile;
     const int keys = tid < here ? s_keys[tid] : 0;
     const int mine = keys > 0 ? (p.starts[g0 + tid + 1] - p.starts[g0 + tid] + span - 1) / span : 0;
     const int per_item = (keys + ATT_TILE - 1) / ATT_TILE;
-    int n_items, n_tiles;
-    s_item[tid] = items + plan_before(mine, red, &n_items);
-    s_start[tid] = tiles + plan_before(mine * per_item * p.hkv, red, &n_tiles);
-    items += n_items;
-    tiles += n_tiles;
+    // both sums at once: items in the upper half, tiles in the lower
+    int64_t all;
+    const int64_t before =
+        plan_before(((int64_t)mine << 32) + (int64_t)mine * per_item * p.hkv, red, &all);
+    s_item[tid] = items + (int)(before >> 32);
+    s_start[tid] = tiles + (int)(before & 0xffffffffll);
+    items += (int)(all >> 32);
+    tiles += (int)(all & 0xffffffffll);
     __syncthreads();
-    for (int i = warp; i < here; i += PLAN_THREADS / 32) {
+    for (int i = warp; i < here; i += PLAN_WARPS) {
       const int keys_i = s_keys[i];
       if (keys_i == 0) continue;
       // the rows of a group evenly over its items
@@ -263,42 +257,53 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
             PrefixItem{a + j * each, min(each, n - j * each), s_table[i], keys_i,
                        s_start[i] + j * tiles_i * p.hkv, tiles_i, 0, 0};
       for (int r = lane; r < n; r += 32) {
-        p.plan.row_item[a + r] = s_item[i] + r / each;
+        const int j = r / each;
+        p.plan.row_part[a + r] = make_int4(s_start[i] + j * tiles_i * p.hkv, tiles_i,
+                                           (s_item[i] + j) * p.hkv, r - j * each);
         s_from[a + r] = keys_i;
       }
     }
     __syncthreads();
   }
-  const int unit = max(p.min_unit, (tiles + p.ctas - 1) / p.ctas);
-  __syncthreads();
+
+  // What each row has for itself, in chunks of one length: long ones, but enough of them for every
+  // CTA, and at most max_splits a row.  Chunks of 1024, 512, 256 and 128 are counted together.
+  {
+    int longest = 0, n[4] = {0, 0, 0, 0};
+    for (int i = tid; i < p.batch; i += PLAN_THREADS) {
+      const int rest = max(0, s_len[i] - s_from[i]);
+      longest = max(longest, rest);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[k] += (rest + (1024 >> k) - 1) >> (10 - k);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0 && longest > 0) atomicMax(&s_count[4], longest);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      n[k] = __reduce_add_sync(0xffffffffu, n[k]);
+      if (lane == 0 && n[k] > 0) atomicAdd(&s_count[k], n[k]);
+    }
+    __syncthreads();
+  }
+  int chunk = 1024;
+  int64_t least = ATT_TILE;
+  while (least * p.max_splits < s_count[4]) least <<= 1;
+  if (least > chunk) chunk = (int)least;
+  for (int k = 0; k < 3 && chunk > least && (int64_t)s_count[k] * p.hkv < 4ll * p.ctas; ++k)
+    chunk >>= 1;
+  const int64_t own = (int64_t)s_count[3] * p.hkv * PLAN_OWN_COST;
+  const int64_t common = (int64_t)tiles * PLAN_COMMON_COST;
+  // SMs for the common part; its CTAs take `unit` tiles each
+  int ctas = p.ctas;
+  if (p.beside && own > 0 && common > 0)
+    ctas = max(p.ctas / 8, min(p.ctas, (int)((p.ctas * common + common + own - 1) / (common + own))));
+  const int unit = max(p.min_unit, (tiles + ctas - 1) / max(ctas, 1));
   // CTAs whose first tile is in an item
   for (int i = tid; i < items; i += PLAN_THREADS) {
     const PrefixItem it = p.plan.items[i];
     const int end = it.start + it.tiles * p.hkv;
     for (int c = (it.start + unit - 1) / unit; c < p.ctas && (int64_t)c * unit < end; ++c)
       p.plan.cta_item[c] = i;
-  }
-
-  // What each row has for itself, in chunks of one length: long ones, but enough of them for every
-  // CTA, and at most max_splits a row.
-  auto rest_of = [&](int i) -> int { return max(0, s_len[i] - s_from[i]); };
-  int longest = 0;
-  for (int i = tid; i < p.batch; i += PLAN_THREADS) longest = max(longest, rest_of(i));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  if ((tid & 31) == 0) red[tid >> 5] = longest;
-  __syncthreads();
-  longest = red[tid & 31];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  int least = ATT_TILE;
-  while ((int64_t)least * p.max_splits < longest) least <<= 1;
-  int chunk = max(1024, least);
-  for (;;) {
-    int n = 0;
-    for (int i = tid; i < p.batch; i += PLAN_THREADS) n += (rest_of(i) + chunk - 1) / chunk;
-    if (plan_sum(n, red) * p.hkv >= 4 * p.ctas || (chunk >> 1) < least) break;
-    chunk >>= 1;
   }
   int* chunk_start = p.plan.hdr + PLAN_HDR;
   int run = 0;
@@ -307,9 +312,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
     const int from = i < p.batch ? s_from[i] : 0;
     const int len = i < p.batch ? s_len[i] : 0;
     const int n = (max(0, len - from) + chunk - 1) / chunk;
-    int all;
-    const int at = run + plan_before(n, red, &all);
-    run += all;
+    int64_t all;
+    const int at = run + (int)plan_before(n, red, &all);
+    run += (int)all;
     if (i >= p.batch) continue;
     chunk_start[i] = at;
     // one chunk and nothing before it: the decode kernel writes the result itself
@@ -493,7 +498,6 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
   volatile int* abort_flag = reinterpret_cast<volatile int*>(staged + 3);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -524,6 +528,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
   const uint32_t tmem_got = *tmem_slot;
   constexpr uint32_t tmem_base = 0;
   pdl_wait();     // the schedule, q and the cache may come from earlier kernels
+  // The decode kernel starts from here on, on the SMs that have no tiles of the common part, and
+  // reads what the kernels before this one have written.
+  pdl_launch_dependents();
   const int unit = p.hdr[PLAN_UNIT], total = p.hdr[PLAN_TILES];
   const int64_t from = (int64_t)blockIdx.x * unit;
   const int begin = (int)(from < total ? from : total);
@@ -641,8 +648,11 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
       for (int j = 0; j < n && ok; ++j) {
         const int vi = kv_base + 2 * j + 1, ki = vi + 1;
         const int vslot = vi % PX_SLOTS, kslot = ki % PX_SLOTS;
+        // both tiles of this step ahead of the weights, so that P V and the next S go out together
         ok = px_wait_warp(&slot_full[vslot], (uint32_t)(vi / PX_SLOTS) & 1u, abort_flag, p.status);
-        bool k_ready = false;
+        const bool more = j + 1 < n;
+        if (ok && more)
+          ok = px_wait_warp(&slot_full[kslot], (uint32_t)(ki / PX_SLOTS) & 1u, abort_flag, p.status);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (!ok || t >= qt) break;
@@ -656,21 +666,14 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
           tc_fence_after();
           issue_pv(t, vslot, j > 0);
           if (j == n - 1) tc_commit_elect(&o_full[t]);
-          if (j + 1 < n) {
-            if (!k_ready) {
-              ok = px_wait_warp(&slot_full[kslot], (uint32_t)(ki / PX_SLOTS) & 1u, abort_flag,
-                                p.status);
-              if (!ok) break;
-              tc_fence_after();
-              k_ready = true;
-            }
+          if (more) {
             issue_s(t, kslot);
             tc_commit_elect(&s_full[t]);
           }
         }
         if (!ok) break;
         tc_commit_elect(&slot_empty[vslot]);
-        if (k_ready) tc_commit_elect(&slot_empty[kslot]);
+        if (more) tc_commit_elect(&slot_empty[kslot]);
         if (j + 2 == n) tc_commit_elect(q_empty);   // the last S products have been issued
       }
       kv_base += 2 * n;
@@ -713,40 +716,64 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
         // (scores of a step whose wait ran out are not used)
         tc_fence_after();
         uint32_t v[64];                        // scores, then weights two a word
-        tc_ld32(s_addr, v);
-        tc_ld32(s_addr + 32, v + 32);
-        tc_wait_ld();
-        if (kpos + 64 > lim) {
+        float sum;
+        // With the reference value that the row has, and again only if a maximum is far above it, as
+        // in the first step: the exponentials need not wait for the other half's maximum.
+        for (int pass = 0; pass < 2; ++pass) {
+          tc_ld32(s_addr, v);
+          tc_ld32(s_addr + 32, v + 32);
+          tc_wait_ld();
+          if (kpos + 64 > lim) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (kpos + i >= lim) v[i] = 0xff800000u;   // -inf
-        }
-        float mx = -INFINITY, m2 = -INFINITY;
+            for (int i = 0; i < 64; ++i)
+              if (kpos + i >= lim) v[i] = 0xff800000u;   // -inf
+          }
+          const float neg_mu = m_used == -INFINITY ? 0.f : -m_used;
+          const uint64_t nm2 = px_pack2(neg_mu, neg_mu),
+                         sc2 = px_pack2(p.scale_log2, p.scale_log2);
+          uint64_t sum2[2] = {0ull, 0ull};
+          float mx = -INFINITY, m2 = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          mx = px_max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-          m2 = px_max3(m2, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-        }
-        mx = fmaxf(mx, m2);
-        {
-          const uint32_t a = ok ? __bfloat16_as_ushort(__float2bfloat16_ru(mx)) : kGone;
-          uint32_t b;
-          asm volatile("st.shared.u16 [%0], %1;" ::"r"(max_at + half * 256), "h"((uint16_t)a)
-                       : "memory");
-          named_bar_sync(1 + t * 4 + quad, 64);
-          asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
-                       : "=r"(b) : "r"(max_at + (half ^ 1) * 256) : "memory");
-          ok = a != kGone && b != kGone;       // the same for both warps: one flag for all lanes
-          mx = fmaxf(bf16_bits_to_float(a), bf16_bits_to_float(b)) * p.scale_log2;
-        }
-        if (!ok) break;
-        if (j == 0) {
-          m_used = mx;
-        } else {
+          for (int i = 0; i < 64; i += 4) {
+            mx = px_max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            m2 = px_max3(m2, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+            float t0, t1, t2, t3;
+            px_unpack2(px_fma2(px_pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2),
+                       t0, t1);
+            px_unpack2(px_fma2(px_pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2,
+                               nm2), t2, t3);
+            const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
+            const float e2 = fast_exp2(t2), e3 = fast_exp2(t3);
+            sum2[0] = px_add2(sum2[0], px_pack2(e0, e1));
+            sum2[1] = px_add2(sum2[1], px_pack2(e2, e3));
+            v[i / 2] = pack_bf16(e0, e1);
+            v[i / 2 + 1] = pack_bf16(e2, e3);
+          }
+          {
+            float a0, a1, a2, a3;
+            px_unpack2(sum2[0], a0, a1);
+            px_unpack2(sum2[1], a2, a3);
+            sum = (a0 + a1) + (a2 + a3);
+          }
+          if (pass) break;
+          {
+            const uint32_t a = ok ? __bfloat16_as_ushort(__float2bfloat16_ru(fmaxf(mx, m2))) : kGone;
+            uint32_t b;
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(max_at + half * 256), "h"((uint16_t)a)
+                         : "memory");
+            named_bar_sync(1 + t * 4 + quad, 64);
+            asm volatile(
+                "{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+                : "=r"(b) : "r"(max_at + (half ^ 1) * 256) : "memory");
+            ok = a != kGone && b != kGone;     // the same for both warps: one flag for all lanes
+            mx = fmaxf(bf16_bits_to_float(a), bf16_bits_to_float(b)) * p.scale_log2;
+          }
+          if (!ok) break;
           const bool grow = mx > m_used + PX_RESCALE_LOG2;
-          if (__any_sync(0xffffffffu, grow)) {
-            const float alpha = grow ? fast_exp2(m_used - mx) : 1.0f;
-            // eight columns at a time: the scores keep their registers
+          if (!__any_sync(0xffffffffu, grow)) break;
+          const float alpha = grow ? fast_exp2(m_used - mx) : 1.0f;
+          if (j > 0) {
+            // eight columns at a time: few registers
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
               uint32_t o[8];
@@ -757,36 +784,15 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
               px_st8(o_addr + c * 8, o);
             }
             tc_wait_st();
-            if (grow) {
-              l *= alpha;
-              m_used = mx;
-            }
+          }
+          if (grow) {
+            l *= alpha;
+            m_used = mx;
           }
         }
-        const float neg_mu = m_used == -INFINITY ? 0.f : -m_used;
-        const uint64_t nm2 = px_pack2(neg_mu, neg_mu), sc2 = px_pack2(p.scale_log2, p.scale_log2);
-        uint64_t sum2[2] = {0ull, 0ull};
-#pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          float t0, t1, t2, t3;
-          px_unpack2(px_fma2(px_pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sc2, nm2),
-                     t0, t1);
-          px_unpack2(px_fma2(px_pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), sc2,
-                             nm2), t2, t3);
-          const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
-          const float e2 = fast_exp2(t2), e3 = fast_exp2(t3);
-          sum2[0] = px_add2(sum2[0], px_pack2(e0, e1));
-          sum2[1] = px_add2(sum2[1], px_pack2(e2, e3));
-          v[i / 2] = pack_bf16(e0, e1);
-          v[i / 2 + 1] = pack_bf16(e2, e3);
-        }
+        if (!ok) break;
+        l += sum;
         __syncwarp();
-        {
-          float a0, a1, a2, a3;
-          px_unpack2(sum2[0], a0, a1);
-          px_unpack2(sum2[1], a2, a3);
-          l += (a0 + a1) + (a2 + a3);
-        }
         tc_st32(s_addr, v);                    // over what this warp has read
         tc_wait_st();
         tc_fence_before();
@@ -854,7 +860,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
 
 // a warp per (row, query head): the splits of its common part, then its own
 struct SharedJoinParams {
-  const int* hdr; const int* row_item; const PrefixItem* items;
+  const int* hdr; const int4* row_part;
   int* counter;
   uint16_t* out; int64_t out_stride;
   const float* pre_o; const float2* pre_ml;
@@ -872,18 +878,18 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const SharedJoinParams
   const int row = (int)(gw / p.hq), head = (int)(gw - (int64_t)row * p.hq);
   const int* chunk_start = p.hdr + PLAN_HDR;
   const int n_own = chunk_start[row + 1] - chunk_start[row];
-  const int item = p.row_item[row];
+  const int4 in = p.row_part[row];
+  const int unit = p.hdr[PLAN_UNIT];
   int n_pre = 0;
   int64_t slot = 0;                            // of the first split
   int at = 0;                                  // row among the two tiles of a split
-  if (item >= 0) {
-    const PrefixItem it = p.items[item];
-    const int unit = p.hdr[PLAN_UNIT], kvh = head / p.g;
-    const int first = it.start + kvh * it.tiles;
-    n_pre = (first + it.tiles - 1) / unit - first / unit + 1;
-    slot = first / unit + item * p.hkv + kvh;
-    const int i = row - it.row0, t = i / p.per_tile;
-    at = t * 128 + (i - t * p.per_tile) * p.g + head - kvh * p.g;
+  if (in.y > 0) {
+    const int kvh = head / p.g, first = in.x + kvh * in.y;
+    const int cta = first / unit;
+    n_pre = (first + in.y - 1) / unit - cta + 1;
+    slot = cta + in.z + kvh;
+    const int t = in.w / p.per_tile;
+    at = t * 128 + (in.w - t * p.per_tile) * p.g + head - kvh * p.g;
   }
   if (n_pre == 0 && n_own == 1) return;        // written by the decode kernel
   // the sum of a row over both halves of the keys, and this lane's piece of its channels
@@ -959,7 +965,7 @@ constexpr int SHARED_DIRECT_TOKENS = 2048;
 constexpr int PREFIX_MIN_UNIT = 2;
 
 struct SharedLayout {
-  size_t row_item, cta_item, items, chunks, pre_o, pre_ml, own_o, own_ml, total;
+  size_t row_part, cta_item, items, chunks, pre_o, pre_ml, own_o, own_ml, total;
 };
 static SharedLayout shared_layout(int64_t batch, int groups, int hq, int hkv, int max_splits) {
   SharedLayout s;
@@ -974,7 +980,7 @@ static SharedLayout shared_layout(int64_t batch, int groups, int hq, int hkv, in
   const int64_t items = groups < 1 ? 0 : groups + batch / span < batch ? groups + batch / span : batch;
   const int64_t slots = items == 0 ? 0 : sm_count() + items * hkv;
   take((PLAN_HDR + batch + 1) * sizeof(int));
-  s.row_item = take(batch * sizeof(int));
+  s.row_part = take(batch * sizeof(int4));
   s.cta_item = take(sm_count() * sizeof(int));
   s.items = take(items * sizeof(PrefixItem));
   s.chunks = take((size_t)batch * max_splits * sizeof(int4));
@@ -1163,9 +1169,10 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   pl.batch = batch; pl.groups = num_groups; pl.hkv = num_kv_heads; pl.page = page_size;
   pl.per_tile = per_tile; pl.max_splits = max_splits; pl.ctas = sms;
   pl.min_unit = PREFIX_MIN_UNIT;
+  pl.beside = pdl_enabled();
   pl.capacity = r.capacity;
   pl.plan.hdr = reinterpret_cast<int*>(ws);
-  pl.plan.row_item = reinterpret_cast<int*>(ws + w.row_item);
+  pl.plan.row_part = reinterpret_cast<int4*>(ws + w.row_part);
   pl.plan.cta_item = reinterpret_cast<int*>(ws + w.cta_item);
   pl.plan.items = reinterpret_cast<PrefixItem*>(ws + w.items);
   pl.plan.chunks = reinterpret_cast<int4*>(ws + w.chunks);
@@ -1235,11 +1242,12 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   }
 
   SharedJoinParams jn{};
-  jn.hdr = pl.plan.hdr; jn.row_item = pl.plan.row_item; jn.items = pl.plan.items;
+  jn.hdr = pl.plan.hdr; jn.row_part = pl.plan.row_part;
   jn.counter = pl.plan.hdr + PLAN_COUNTER;
   jn.out = r.out; jn.out_stride = r.out_stride;
   jn.pre_o = px.part_o; jn.pre_ml = px.part_ml;
   jn.own_o = a.part_o; jn.own_ml = a.part_ml; jn.own_splits = max_splits;
+  a.beside = num_groups > 0;
   jn.batch = batch; jn.hq = num_q_heads; jn.hkv = num_kv_heads; jn.g = g; jn.per_tile = per_tile;
 
   static PerDeviceOnce plan_once;
