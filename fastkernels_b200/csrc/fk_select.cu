@@ -131,8 +131,9 @@ struct SelectParams {
   int together;                       // tokens of a CTA: 1, or 16 / g
   int g_shift;                        // log2 of g where that is 16 / g
   int most;                           // blocks that a table's row has pages for
+  int pitch;                          // of the scores' rows: a multiple of four
   int chunk, chunks;                  // blocks of a CTA of the scores, of those CTAs per token
-  uint32_t* scores;                   // [tokens, hkv, most], ordered
+  uint32_t* scores;                   // [tokens, hkv, pitch], ordered
   float* largest;                     // [groups of tokens, hkv, chunks] largest |bound| of a chunk
   float* q_sum;                       // [tokens, hkv] largest sum of |q| of a query head
   int32_t* selected;                  // [tokens, hkv, count]
@@ -171,34 +172,39 @@ struct Team {
   }
 };
 
-// The want-th largest of n keys (1 <= want <= n), the largest one, and how many of the keys that equal it are among the
-// want largest.  Counts of 256 parts of the range of keys leave one part, which is the range of
-// the next round, until 32 keys are left, which are ranked, or all that are left are equal.
+// The smallest and largest of all threads' values; ends behind a barrier.
 template <int W, typename KEY>
-__device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int* left, KEY* most,
-                                         Team<W>& s) {
-  const int tid = Team<W>::rank(), lane = threadIdx.x & 31;
-  constexpr int kBits = 8 * sizeof(KEY);
-  KEY lo = (KEY)~(KEY)0, hi = 0;
-  for (int i = tid; i < n; i += 32 * W) {
-    lo = min(lo, keys[i]);
-    hi = max(hi, keys[i]);
+__device__ __forceinline__ void range_of(KEY& lo, KEY& hi, Team<W>& s) {
+  if (sizeof(KEY) == 4) {
+    lo = (KEY)__reduce_min_sync(0xffffffffu, (uint32_t)lo);
+    hi = (KEY)__reduce_max_sync(0xffffffffu, (uint32_t)hi);
+  } else {
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
+  if (W > 1 && (threadIdx.x & 31) == 0) { s.lo[Team<W>::warp()] = lo; s.hi[Team<W>::warp()] = hi; }
+  Team<W>::sync();
   if (W > 1) {
-    if (lane == 0) { s.lo[Team<W>::warp()] = lo; s.hi[Team<W>::warp()] = hi; }
-    Team<W>::sync();
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       lo = min(lo, (KEY)s.lo[w]);
       hi = max(hi, (KEY)s.hi[w]);
     }
   }
-  *most = hi;
+}
+
+// The want-th largest of n keys (1 <= want <= n) between lo and hi, and how many of the keys that
+// equal it are among the want largest.  Counts of 256 parts of the range leave one part, which is
+// the range of the next round, until 32 keys are left, which are ranked, or all that are left are
+// equal.
+template <int W, typename KEY>
+__device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, KEY lo, KEY hi, int* left,
+                                         Team<W>& s) {
+  const int tid = Team<W>::rank(), lane = threadIdx.x & 31;
+  constexpr int kBits = 8 * sizeof(KEY);
   while (lo != hi) {
     const int used = kBits - (kBits == 64 ? __clzll((long long)(hi - lo)) : __clz((int)(hi - lo)));
     const int shift = max(0, used - 8);
@@ -270,60 +276,58 @@ __device__ __forceinline__ KEY border_of(const KEY* keys, int n, int want, int* 
   return lo;
 }
 
-// Score of a block in 64 bits, by eight lanes: the largest over the query heads.  Products of two bf16
-// are exact in fp32, and 128 of them all but always in a 64-bit sum.
+// Score of a block in 64 bits, by a warp: the largest over the query heads.  Products of two bf16 are
+// exact in fp32, and 128 of them all but always in a 64-bit sum.  (Code that runs once a launch
+// costs what it takes to fetch it: four heads at a time and loops, not sixteen channels a lane
+// unrolled, which took 8 us instead of 2.)
 __device__ __forceinline__ uint64_t exact_score(const SelectParams& p, int token, int kvh,
                                                 const uint16_t* at, int lane) {
-  float l[16], u[16];
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint2 a = reinterpret_cast<const uint2*>(at)[i * 8 + (lane & 7)];
-    const uint2 b = reinterpret_cast<const uint2*>(at + SEL_D)[i * 8 + (lane & 7)];
-    l[4 * i] = bf16lo(a.x); l[4 * i + 1] = bf16hi(a.x);
-    l[4 * i + 2] = bf16lo(a.y); l[4 * i + 3] = bf16hi(a.y);
-    u[4 * i] = bf16lo(b.x); u[4 * i + 1] = bf16hi(b.x);
-    u[4 * i + 2] = bf16lo(b.y); u[4 * i + 3] = bf16hi(b.y);
-  }
-  bool odd = false;                            // an infinity, or no number
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    nan |= l[i] != l[i] || u[i] != u[i];
-    odd |= !(fabsf(l[i]) < INFINITY) || !(fabsf(u[i]) < INFINITY);
-  }
-  odd = __any_sync(0xffffffffu, odd);
+  const uint2 lo = reinterpret_cast<const uint2*>(at)[lane];
+  const uint2 hi = reinterpret_cast<const uint2*>(at + SEL_D)[lane];
+  const float l[4] = {bf16lo(lo.x), bf16hi(lo.x), bf16lo(lo.y), bf16hi(lo.y)};
+  const float u[4] = {bf16lo(hi.x), bf16hi(hi.x), bf16lo(hi.y), bf16hi(hi.y)};
   const uint16_t* qp = p.q + (int64_t)token * p.q_stride + (int64_t)kvh * p.g * SEL_D;
   double best = -INFINITY;
-#pragma unroll 2
-  for (int h = 0; h < p.g; ++h) {
-    double sum[2] = {0.0, 0.0};
+  bool nan = false;
+#pragma unroll 1
+  for (int h0 = 0; h0 < p.g; h0 += 4) {
+    uint2 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint2 v = reinterpret_cast<const uint2*>(qp + h * SEL_D)[i * 8 + (lane & 7)];
-      const float q[4] = {bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y)};
+    for (int h = 0; h < 4; ++h)                // the last head again behind the last
+      v[h] = reinterpret_cast<const uint2*>(qp + min(h0 + h, p.g - 1) * SEL_D)[lane];
+    double sum[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const float q[4] = {bf16lo(v[h].x), bf16hi(v[h].x), bf16lo(v[h].y), bf16hi(v[h].y)};
+      sum[h] = 0.0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        sum[k & 1] += (double)q[k] * (double)(q[k] > 0.f ? u[4 * i + k] : l[4 * i + k]);
-        // zero times infinity is no number on either side
-        if (odd) nan |= q[k] == 0.f && (isinf(l[4 * i + k]) || isinf(u[4 * i + k]));
+        // one side of the maximum; no number, or zero times infinity, counts on either
+        sum[h] += (double)q[k] * (double)(q[k] > 0.f ? u[k] : l[k]);
+        const float other = q[k] > 0.f ? q[k] * l[k] : q[k] * u[k];
+        nan |= other != other;
       }
     }
-    double all = sum[0] + sum[1];
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    nan |= all != all;
-    best = fmax(best, all);
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      nan |= sum[h] != sum[h];
+      best = fmax(best, sum[h]);
+    }
   }
-  const uint32_t nans = __ballot_sync(0xffffffffu, nan);
-  return nans >> (lane & 24) & 255u ? ~0ull : order_of(best);
+  return __any_sync(0xffffffffu, nan) ? ~0ull : order_of(best);
 }
 
 // The choice of one token, by a team: `keys` are the scores of its n - keep_first - keep_last blocks
-// in the middle, `reach` bounds sum |q| max |bound|.  exact and band: room for those blocks.
+// in the middle, `reach` bounds sum |q| max |bound|, key_lo and key_hi are
+// the smallest and largest key.  exact and band: room for those blocks.
 template <int W>
 __device__ __forceinline__ void choose(const SelectParams& p, int token, int kvh, int n,
                                        const int32_t* table, uint32_t* keys, float reach,
-                                       uint64_t* exact, uint16_t* band, Team<W>& s) {
+                                       uint32_t key_lo, uint32_t key_hi, uint64_t* exact, uint16_t* band, Team<W>& s) {
   const int tid = Team<W>::rank(), warp = Team<W>::warp(), lane = threadIdx.x & 31;
   const uint32_t below = (1u << lane) - 1u;
   const int per = p.page / p.block;
@@ -339,18 +343,16 @@ __device__ __forceinline__ void choose(const SelectParams& p, int token, int kvh
     out[p.count - p.keep_last + i] = n - p.keep_last + i;
   if (want == 0) return;
   // scores past fp32's range, products below it, and what is no number: all in 64 bits
-  bool all = !(reach < INFINITY) || (reach > 0.f && reach < 7.9e-31f);
+  const bool all = !(reach < INFINITY) || (reach > 0.f && reach < 7.9e-31f) || key_hi == ~0u;
   uint32_t above = ~0u, least = 0u;            // keys above are taken, keys below `least` are not
   bool same = false;                           // keys between are equal in truth
   if (!all) {
     int left;
-    uint32_t most;                             // the largest key
-    const uint32_t border = border_of<W, uint32_t>(keys, middle, want, &left, &most, s);
-    all = most == ~0u;
+    const uint32_t border = border_of<W, uint32_t>(keys, middle, want, key_lo, key_hi, &left, s);
     const float v = value_of(border), e2 = reach * (2.f / 262144.f);
-    same = !all && (border == 0u || reach == 0.f);
-    above = all ? ~0u : same ? border : order_of(v + e2);
-    least = all ? 0u : same ? border : order_of(v - e2);
+    same = border == 0u || reach == 0.f;
+    above = same ? border : order_of(v + e2);
+    least = same ? border : order_of(v - e2);
   }
   // how many are above, and between; each warp has a run of blocks
   const int run = ((middle + W - 1) / W + 31) / 32 * 32;
@@ -390,14 +392,16 @@ __device__ __forceinline__ void choose(const SelectParams& p, int token, int kvh
       at += __popc(votes);
     }
     Team<W>::sync();
-    for (int c0 = warp * 4; c0 < eqs; c0 += W * 4) {
-      const int c = min(c0 + (lane >> 3), eqs - 1);
+    for (int c = warp; c < eqs; c += W) {
       const int b = p.keep_first + band[c];
-      const bool paged = keys[band[c]] != 0u;
-      const int64_t page = paged ? table[b / per] : 0;
-      const uint64_t key = exact_score(
-          p, token, kvh, p.bounds + ((page * p.hkv + kvh) * per + b % per) * 2 * SEL_D, lane);
-      if ((lane & 7) == 0 && c0 + (lane >> 3) < eqs) exact[c] = paged ? key : 0ull;
+      uint64_t key = 0ull;                     // without a page
+      if (keys[band[c]] != 0u) {
+        const int at_page = p.per_shift >= 0 ? b >> p.per_shift : b / per;
+        key = exact_score(p, token, kvh,
+                          p.bounds + (((int64_t)table[at_page] * p.hkv + kvh) * per + b -
+                                      at_page * per) * 2 * SEL_D, lane);
+      }
+      if (lane == 0) exact[c] = key;
     }
     Team<W>::sync();
     if (eqs <= 32) {
@@ -410,9 +414,14 @@ __device__ __forceinline__ void choose(const SelectParams& p, int token, int kvh
       }
       if (warp == 0 && lane < eqs) keys[band[lane]] = rank < ties ? ~0u : 0u;
     } else {
+      uint64_t lo = ~0ull, hi = 0ull;
+      for (int c = tid; c < eqs; c += 32 * W) {
+        lo = min(lo, exact[c]);
+        hi = max(hi, exact[c]);
+      }
+      range_of<W, uint64_t>(lo, hi, s);
       int left;
-      uint64_t most;
-      const uint64_t edge = border_of<W, uint64_t>(exact, eqs, ties, &left, &most, s);
+      const uint64_t edge = border_of<W, uint64_t>(exact, eqs, ties, lo, hi, &left, s);
       // equal ones in order: a warp has a run of them, as above
       const int run_c = ((eqs + W - 1) / W + 31) / 32 * 32;
       const int fc = min(warp * run_c, eqs), tc = min(fc + run_c, eqs);
@@ -673,7 +682,7 @@ select_scores_kernel(const SelectParams p) {
         asm("mov.b64 {%0, %1}, %2;" : "=f"(v[nt][0]), "=f"(v[nt][1]) : "l"(sum[nt][0]));
         asm("mov.b64 {%0, %1}, %2;" : "=f"(v[nt][2]), "=f"(v[nt][3]) : "l"(sum[nt][1]));
       }
-      uint32_t* scores = p.scores + ((int64_t)t0 * p.hkv + kvh) * p.most + b0 + r0;
+      uint32_t* scores = p.scores + ((int64_t)t0 * p.hkv + kvh) * p.pitch + b0 + r0;
       const bool in0 = b0 + r0 < end, in1 = b0 + 8 + r0 < end;
       if (p.together == 1) {
         float m0 = -INFINITY, m1 = -INFINITY;
@@ -709,7 +718,7 @@ select_scores_kernel(const SelectParams p) {
             const int col = nt * 8 + quad * 2 + i;
             const int of = col >> p.g_shift;
             if (of << p.g_shift != col || t0 + of >= t1) continue;
-            uint32_t* at = scores + (int64_t)of * p.hkv * p.most;
+            uint32_t* at = scores + (int64_t)of * p.hkv * p.pitch;
             if (in0) at[0] = ok0 ? order_of(v[nt][i]) : 0u;
             if (in1) at[8] = ok1 ? order_of(v[nt][2 + i]) : 0u;
           }
@@ -765,10 +774,21 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) select_choose_kernel(co
   uint16_t* band = reinterpret_cast<uint16_t*>(sel_smem + (size_t)kTeams * p.most * 12) +
                    team * p.most;
   float reach = 0.f;
+  uint32_t key_lo = ~0u, key_hi = 0u;
   if (n > p.count) {
     const int middle = n - p.keep_first - p.keep_last;
-    const uint32_t* src = p.scores + item * p.most;
-    for (int i = Team<W>::rank(); i < middle; i += 32 * W) keys[i] = src[i];
+    const uint4* src = reinterpret_cast<const uint4*>(p.scores + item * p.pitch);
+    for (int i = Team<W>::rank() * 4; i < middle; i += 128 * W) {
+      const uint4 v = src[i >> 2];
+      const uint32_t k[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (i + h >= middle) break;
+        keys[i + h] = k[h];
+        key_lo = min(key_lo, k[h]);
+        key_hi = max(key_hi, k[h]);
+      }
+    }
     // largest |bound|; no number counts as infinite
     const float* from = p.largest + ((int64_t)(token / p.together) * p.hkv + kvh) * p.chunks;
     float largest = 0.f;
@@ -778,15 +798,15 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) select_choose_kernel(co
     for (int o = 16; o > 0; o >>= 1)
       largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
     reach = p.q_sum[item] * largest;
-    Team<W>::sync();
+    range_of<W, uint32_t>(key_lo, key_hi, teams[team]);
   }
-  choose<W>(p, token, kvh, n, p.tables + (int64_t)row * p.table_stride, keys, reach, exact, band,
-            teams[team]);
+  choose<W>(p, token, kvh, n, p.tables + (int64_t)row * p.table_stride, keys, reach, key_lo,
+            key_hi, exact, band, teams[team]);
 }
 
 // Groups of tokens that share products, and what is in a workspace.
 struct SelectLayout {
-  int together, chunk, chunks;
+  int together, chunk, chunks, pitch;
   int64_t groups;
   size_t largest, q_sum, total;       // bytes
 };
@@ -803,7 +823,8 @@ static SelectLayout select_layout(int64_t tokens, int hkv, int g, bool rows, int
   while (s.chunk > 64 && s.groups * hkv * ((most + s.chunk - 1) / s.chunk) < 4ll * sm_count())
     s.chunk /= 2;
   s.chunks = (int)((most + s.chunk - 1) / s.chunk);
-  s.largest = ((size_t)tokens * hkv * most * 4 + 255) & ~size_t(255);
+  s.pitch = (int)((most + 3) & ~3ll);
+  s.largest = ((size_t)tokens * hkv * s.pitch * 4 + 255) & ~size_t(255);
   s.q_sum = s.largest + (size_t)s.groups * hkv * s.chunks * 4;
   s.total = s.q_sum + (size_t)tokens * hkv * 4;
   return s;
@@ -943,7 +964,7 @@ int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, 
              workspace_bytes);
   FK_REQUIRE(w.groups * w.chunks < (1ll << 31), FK_ERR_UNSUPPORTED,
              "fk_select_blocks: too many tokens");
-  p.together = w.together;
+  p.together = w.together; p.pitch = w.pitch;
   p.g_shift = w.together > 1 ? __builtin_ctz(p.g) : 0;
   p.chunk = w.chunk; p.chunks = w.chunks;
   p.scores = static_cast<uint32_t*>(workspace);
