@@ -66,7 +66,9 @@ PROTOTYPES = {
                                             _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32,
                                             _vp, _sz, _vp, _vp]),
     "fk_shared_prefix_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
-    "fk_shared_prefix_attn": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _vp,
+    "fk_shared_prefix_plan": (_i32, [_vp, _i32, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
+                                     _vp, _sz, _vp, _vp]),
+    "fk_shared_prefix_attn": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _vp,
                                      _vp, _i64, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32,
                                      _i32, _vp, _sz, _vp, _vp]),
     "fk_key_bounds": (_i32, [_vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i64,

@@ -10,7 +10,7 @@
 // every key and value is used by n G query rows, which makes a matrix product of it.
 //
 // Four launches of fk_shared_prefix_attn: shared_plan_kernel (schedule of both parts, 1 CTA),
-// prefix_attn_kernel, attn_decode_kernel, shared_join_kernel.
+// prefix_attn_kernel and beside it attn_decode_kernel, shared_join_kernel.
 #include "fk_attn.cuh"
 #include "fk_tcgen05.cuh"
 #include "fk_types.cuh"
@@ -1124,21 +1124,25 @@ size_t fk_shared_prefix_workspace_bytes(int batch, int num_groups, int num_q_hea
   return shared_layout(batch, num_groups, num_q_heads, num_kv_heads, max_splits).total;
 }
 
-int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
-                          int64_t out_stride_token, const void* k_cache, const void* v_cache,
-                          int64_t num_pages, int page_size, int64_t kv_page_stride, int kv_layout,
-                          const int32_t* context_lens, const int32_t* block_tables,
-                          int64_t block_table_stride, int64_t block_table_cols,
-                          const int32_t* group_starts, const int32_t* prefix_lens, int num_groups,
-                          int batch, int num_q_heads, int num_kv_heads, int head_dim,
-                          float softmax_scale, int max_splits, void* workspace,
-                          size_t workspace_bytes, int32_t* status, fk_stream_t stream) {
+// mode 0: schedule and attention, 1: the schedule only, 2: by the schedule in the workspace
+static int shared_impl(int mode, const void* q, int64_t q_stride_token, void* out,
+                       int64_t out_stride_token, const void* k_cache, const void* v_cache,
+                       int64_t num_pages, int page_size, int64_t kv_page_stride, int kv_layout,
+                       const int32_t* context_lens, const int32_t* block_tables,
+                       int64_t block_table_stride, int64_t block_table_cols,
+                       const int32_t* group_starts, const int32_t* prefix_lens, int num_groups,
+                       int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                       float softmax_scale, int max_splits, void* workspace,
+                       size_t workspace_bytes, int32_t* status, fk_stream_t stream) {
   FK_REQUIRE(batch >= 0 && num_groups >= 0, FK_ERR_INVALID_ARG,
              "fk_shared_prefix_attn: negative size");
   if (batch == 0) return FK_OK;
   RowsParams r{};
-  int rc = rows_args("fk_shared_prefix_attn", r, q, q_stride_token, out, out_stride_token, k_cache,
-                     v_cache, num_pages, page_size, kv_page_stride, kv_layout, context_lens,
+  // a schedule has no tensors to check
+  const void* const none = workspace;
+  int rc = rows_args("fk_shared_prefix_attn", r, mode == 1 ? none : q, q_stride_token,
+                     mode == 1 ? workspace : out, out_stride_token, mode == 1 ? none : k_cache,
+                     mode == 1 ? none : v_cache, num_pages, page_size, kv_page_stride, kv_layout, context_lens,
                      block_tables, block_table_stride, block_table_cols, num_q_heads, num_kv_heads,
                      head_dim, softmax_scale);
   if (rc != FK_OK) return rc;
@@ -1161,6 +1165,11 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
              "fk_shared_prefix_attn: workspace needs %zu bytes, 256-byte aligned (got %zu)",
              w.total, workspace_bytes);
   const int g = r.g, sms = sm_count(), per_tile = 128 / g;
+  // Small calls as fk_paged_decode_attn has them: a CTA per row and KV head, which read the common part
+  // from L2, in one launch instead of four that wait for one another (8 rows of 512 common tokens
+  // and up to 200 of their own, 32/8 heads: 30.6 -> 9.9 us).
+  const bool direct = (int64_t)batch * num_kv_heads <= sms && r.capacity <= SHARED_DIRECT_TOKENS;
+  if (direct && mode == 1) return FK_OK;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 
@@ -1177,6 +1186,15 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   pl.plan.items = reinterpret_cast<PrefixItem*>(ws + w.items);
   pl.plan.chunks = reinterpret_cast<int4*>(ws + w.chunks);
   pl.status = status;
+
+  if (mode != 2 && !direct) {
+    static PerDeviceOnce plan_once;
+    FK_CUDA_OK(set_max_dynamic_smem(plan_once, shared_plan_kernel, PLAN_MAX_BATCH * 8));
+    FK_CUDA_OK(launch_kernel(shared_plan_kernel, dim3(1), dim3(PLAN_THREADS), (size_t)batch * 8, s,
+                             pl));
+    count_launch(1);
+  }
+  if (mode == 1) return FK_OK;
 
   const int sub = page_size < ATT_BOX ? page_size : ATT_BOX;
   const int fused16 = page_size == 16;
@@ -1229,10 +1247,7 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   a.part_ml = reinterpret_cast<float2*>(ws + w.own_ml);
   a.status = status;
 
-  // Small calls as fk_paged_decode_attn has them: a CTA per row and KV head, which read the common part
-  // from L2, in one launch instead of four that wait for one another (8 rows of 512 common tokens
-  // and up to 200 of their own, 32/8 heads: 30.6 -> FIXME us).
-  if ((int64_t)batch * num_kv_heads <= sms && r.capacity <= SHARED_DIRECT_TOKENS) {
+  if (direct) {
     a.direct = 1;
     a.capacity = r.capacity;
     a.starts = group_starts; a.groups = num_groups;
@@ -1250,11 +1265,6 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
   a.beside = num_groups > 0;
   jn.batch = batch; jn.hq = num_q_heads; jn.hkv = num_kv_heads; jn.g = g; jn.per_tile = per_tile;
 
-  static PerDeviceOnce plan_once;
-  FK_CUDA_OK(set_max_dynamic_smem(plan_once, shared_plan_kernel, PLAN_MAX_BATCH * 8));
-  FK_CUDA_OK(launch_kernel(shared_plan_kernel, dim3(1), dim3(PLAN_THREADS), (size_t)batch * 8, s,
-                           pl));
-  count_launch(1);
   if (num_groups > 0) {
     static PerDeviceOnce once;
     FK_CUDA_OK(set_max_dynamic_smem(once, prefix_attn_kernel, PX_SMEM_ALLOC));
@@ -1268,6 +1278,35 @@ int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
                            (size_t)0, s, jn));
   count_launch(2);
   return FK_OK;
+}
+
+int fk_shared_prefix_attn(int planned, const void* q, int64_t q_stride_token, void* out,
+                          int64_t out_stride_token, const void* k_cache, const void* v_cache,
+                          int64_t num_pages, int page_size, int64_t kv_page_stride, int kv_layout,
+                          const int32_t* context_lens, const int32_t* block_tables,
+                          int64_t block_table_stride, int64_t block_table_cols,
+                          const int32_t* group_starts, const int32_t* prefix_lens, int num_groups,
+                          int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                          float softmax_scale, int max_splits, void* workspace,
+                          size_t workspace_bytes, int32_t* status, fk_stream_t stream) {
+  return shared_impl(planned ? 2 : 0, q, q_stride_token, out, out_stride_token, k_cache, v_cache,
+                     num_pages, page_size, kv_page_stride, kv_layout, context_lens, block_tables,
+                     block_table_stride, block_table_cols, group_starts, prefix_lens, num_groups,
+                     batch, num_q_heads, num_kv_heads, head_dim, softmax_scale, max_splits,
+                     workspace, workspace_bytes, status, stream);
+}
+
+int fk_shared_prefix_plan(const int32_t* context_lens, int page_size, int64_t block_table_cols,
+                          const int32_t* group_starts, const int32_t* prefix_lens, int num_groups,
+                          int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                          int max_splits, void* workspace, size_t workspace_bytes, int32_t* status,
+                          fk_stream_t stream) {
+  const int64_t row = (int64_t)num_q_heads * head_dim;
+  return shared_impl(1, nullptr, row, nullptr, row, nullptr, nullptr, 1, page_size,
+                     (int64_t)page_size * num_kv_heads * head_dim, 0, context_lens, context_lens, 0,
+                     block_table_cols, group_starts, prefix_lens, num_groups, batch, num_q_heads,
+                     num_kv_heads, head_dim, 1.0f, max_splits, workspace, workspace_bytes, status,
+                     stream);
 }
 
 }  // extern "C"

@@ -396,9 +396,29 @@ def shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, 
                                                     head_dim, max_splits))
 
 
+def shared_prefix_plan(context_lens, block_tables, page_size, num_q_heads, num_kv_heads, head_dim,
+                       group_starts, prefix_lens, workspace, max_splits, status=None) -> None:
+    """The schedule of a decode step, once: layers then call shared_prefix_attn(..., planned=True)
+    with the same lengths, groups, tables, workspace and max_splits."""
+    dev = _device_of(context_lens)
+    b = context_lens.numel()
+    _need_ints(dev, b, "context_lens", context_lens)
+    _, cols, rows = _need_tables(dev, block_tables)
+    if rows != b:
+        raise _lib.FkError(f"block_tables must have {b} rows, got {rows}")
+    groups = prefix_lens.numel()
+    _need_ints(dev, groups, "prefix_lens", prefix_lens)
+    _need_ints(dev, groups + 1, "group_starts", group_starts)
+    ws, ws_bytes, _held = _workspace(dev, workspace, 1, context_lens)
+    check(lib.fk_shared_prefix_plan(
+        context_lens.data_ptr(), page_size, cols, group_starts.data_ptr(), prefix_lens.data_ptr(),
+        groups, b, num_q_heads, num_kv_heads, head_dim, max_splits, ws, ws_bytes,
+        _status_ptr(status, context_lens), _stream()), "fk_shared_prefix_plan")
+
+
 def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_starts, prefix_lens,
                        softmax_scale, workspace=None, max_splits=None, out=None, status=None,
-                       kv_layout="NHD"):
+                       kv_layout="NHD", planned=False):
     """paged_decode_attn for a batch whose rows group_starts[g] .. group_starts[g + 1] - 1 list the
     same pages for their first prefix_lens[g] tokens: that part is read once for all of them.
 
@@ -406,7 +426,8 @@ def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_st
     prefix that ends inside a page the whole pages are taken together.  Rows outside of all
     groups have nothing in common.  context_lens count all tokens of a row, the common ones too.
     GQA ratios up to 16.  A workspace of shared_prefix_workspace_bytes holds the schedule and
-    partial results of one call at a time; without one it is allocated here."""
+    partial results of one call at a time; without one it is allocated here.  planned: by the
+    schedule that shared_prefix_plan has left there."""
     dev = _device_of(q)
     pages, page, hkv, d2, stride = _need_caches(dev, k_cache, v_cache, kv_layout)
     b, hq, d, qs = _need_rows(dev, q, "q")
@@ -420,6 +441,8 @@ def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_st
     _need_ints(dev, groups, "prefix_lens", prefix_lens)
     _need_ints(dev, groups + 1, "group_starts", group_starts)
     out, os_ = _out_like(dev, q, out)
+    if planned and (workspace is None or max_splits is None):
+        raise _lib.FkError("a planned call needs the plan's workspace and max_splits")
     if max_splits is None:
         max_splits = max_splits_for(cols * page)
     ws, ws_bytes, _held = _workspace(
@@ -427,7 +450,7 @@ def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_st
         lib.fk_shared_prefix_workspace_bytes(b, groups, hq, hkv, d, max_splits)
         if workspace is None else 0, q)
     check(lib.fk_shared_prefix_attn(
-        q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
+        1 if planned else 0, q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
         stride, 1 if kv_layout == "HND" else 0, context_lens.data_ptr(), block_tables.data_ptr(),
         ts, cols, group_starts.data_ptr(), prefix_lens.data_ptr(), groups, b, hq, hkv, d,
         softmax_scale, max_splits, ws, ws_bytes, _status_ptr(status, q), _stream()),

@@ -196,7 +196,12 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  * flagged FK_DEV_BAD_POSITION; no row has anything in common then.)  A row's context may
  * end inside the common part.  The table of the group's row with the longest context is
  * read for it.  max_splits: upper bound of KV splits of what each row has for itself.
- * softmax_scale above zero.  Launches: schedule, common part, own parts, join.
+ * softmax_scale above zero.  Launches: schedule, common part, own parts, join; one launch
+ * where batch * num_kv_heads fits the SMs and the tables have at most 2048 tokens.
+ * fk_shared_prefix_plan computes the schedule of a step into the workspace, and calls
+ * with `planned` go by it for any number of layers afterwards, with the same lengths,
+ * groups, sizes, head counts, table columns, max_splits and workspace.  The workspace
+ * serves one call at a time.
  *
  * fk_key_bounds: bounds[page][head][i][0 / 1][d] = smallest / largest key of
  * channel d over the cached tokens of the i-th run of `block` positions of a page,
@@ -226,7 +231,13 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
 size_t fk_shared_prefix_workspace_bytes(int batch, int num_groups, int num_q_heads,
                                         int num_kv_heads, int head_dim, int max_splits);
 
-int fk_shared_prefix_attn(const void* q, int64_t q_stride_token, void* out,
+int fk_shared_prefix_plan(const int32_t* context_lens, int page_size, int64_t block_table_cols,
+                          const int32_t* group_starts, const int32_t* prefix_lens, int num_groups,
+                          int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                          int max_splits, void* workspace, size_t workspace_bytes, int32_t* status,
+                          fk_stream_t stream);
+
+int fk_shared_prefix_attn(int planned, const void* q, int64_t q_stride_token, void* out,
                           int64_t out_stride_token, const void* k_cache, const void* v_cache,
                           int64_t num_pages, int page_size, int64_t kv_page_stride, int kv_layout,
                           const int32_t* context_lens, const int32_t* block_tables,

@@ -202,6 +202,53 @@ def test_in_a_graph_with_other_lengths(ops):
         assert (d <= S.tolerance(want, mass)).all()
 
 
+@pytest.mark.parametrize("rows", [2, 30])
+def test_planned_layers(ops, rows):
+    """One schedule, several layers with other queries and caches by it, in a graph too."""
+    case = build(11, [(640, [40 + i for i in range(rows)]), (320, [100, 900])], 64, "NHD", 16, 8)
+    q, kc, vc, lens, table, starts, prefix = case
+    b = len(lens)
+    n = ops.shared_prefix_workspace_bytes(b, 2, 16, 8, 128, 16)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    args = [ints(lens), ints(table)]
+    groups = [ints(starts), ints(prefix)]
+    layers = [(dev(S.bf16(q * f)), dev(kc), dev(S.bf16(vc * f))) for f in (1.0, 0.5, 2.0)]
+
+    def run_all():
+        ops.shared_prefix_plan(*args, 64, 16, 8, 128, *groups, ws, 16)
+        return [ops.shared_prefix_attn(*x, *args, *groups, S.SCALE, workspace=ws, max_splits=16,
+                                       planned=True) for x in layers]
+    want = [ops.shared_prefix_attn(*x, *args, *groups, S.SCALE, max_splits=16) for x in layers]
+    for a, b_ in zip(run_all(), want):
+        assert torch.equal(a, b_)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run_all()
+    for _ in range(2):
+        g.replay()
+        for a, b_ in zip(got, want):
+            assert torch.equal(a, b_)
+
+
+def test_calls_on_two_streams(ops):
+    """Two calls at once, each with a workspace of its own."""
+    cases = [build(20 + i, [(2048, [70 + 5 * i] * 12), (640, [300, 9])], 64, "NHD", 16, 4)
+             for i in range(2)]
+    want = [run(ops, c, "NHD") for c in cases]
+    side = [torch.cuda.Stream() for _ in cases]
+    tensors = [[dev(c[0]), dev(c[1]), dev(c[2])] + [ints(x) for x in c[3:]] for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, a in zip(side, tensors):
+            with torch.cuda.stream(s):
+                got.append(ops.shared_prefix_attn(*a, S.SCALE))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 def test_same_bits_every_time(ops):
     case = build(10, [(4096, [40, 50, 60, 1000] * 4), (320, [100, 900])], 64, "NHD", 8, 2)
     first = run(ops, case, "NHD")

@@ -52,10 +52,10 @@ def attend(**kw):
 
 
 def shared(**kw):
-    names = "q qs out os k v num_pages page kv_stride layout lens tables ts cols starts prefix groups " \
+    names = "planned q qs out os k v num_pages page kv_stride layout lens tables ts cols starts prefix groups " \
             "n hq hkv d scale splits ws wsb status stream".split()
     return call(L.fk_shared_prefix_attn, names,
-                dict(CACHE, q=P, qs=1024, out=P, os=1024, k=P, v=P, starts=P, prefix=P, groups=1,
+                dict(CACHE, planned=0, q=P, qs=1024, out=P, os=1024, k=P, v=P, starts=P, prefix=P, groups=1,
                      n=3, hq=8, hkv=2, d=128, scale=0.1, splits=4, ws=P, wsb=1 << 30), kw)
 
 
@@ -142,6 +142,23 @@ def test_shared_refusals():
     assert L.fk_shared_prefix_workspace_bytes(3, 1, 8, 2, 128, 0) == 0
 
 
+def test_plan_refusals():
+    def plan(**kw):
+        names = "lens page cols starts prefix groups n hq hkv d splits ws wsb status stream".split()
+        return call(L.fk_shared_prefix_plan, names,
+                    dict(CACHE, starts=P, prefix=P, groups=1, n=300, hq=8, hkv=2, d=128, splits=4, ws=P,
+                         wsb=1 << 30), kw)
+    need = L.fk_shared_prefix_workspace_bytes(300, 1, 8, 2, 128, 4)
+    assert plan(n=0) == 0 and plan(n=-1) == INVALID
+    assert plan(lens=None) == INVALID and plan(starts=None) == INVALID
+    assert plan(wsb=need - 1) == WORKSPACE and plan(ws=P + 16) == WORKSPACE
+    assert plan(d=64) == UNSUPPORTED and plan(hq=5) == INVALID and plan(splits=0) == INVALID
+    assert plan(page=48) == UNSUPPORTED and plan(cols=0) == INVALID
+    assert plan(n=16385, wsb=1 << 40) == UNSUPPORTED and "16384" in err()
+    before = L.fk_launch_count()
+    assert plan(n=3) == 0 and L.fk_launch_count() == before      # a small call needs no schedule
+
+
 def test_wrappers_refuse_cpu_tensors_and_odd_layouts():
     import torch
     from fastkernels_b200 import ops
@@ -192,6 +209,7 @@ def test_prototypes_fit_the_header():
     kinds = {"int": ctypes.c_int, "int64_t": ctypes.c_int64, "float": ctypes.c_float,
              "size_t": ctypes.c_size_t}
     for name in ("fk_key_bounds", "fk_select_blocks", "fk_selected_attn", "fk_shared_prefix_attn",
+                 "fk_shared_prefix_plan",
                  "fk_selected_attn_workspace_bytes", "fk_select_blocks_workspace_bytes",
                  "fk_shared_prefix_workspace_bytes"):
         args = re.search(rf"\b{name}\s*\(([^)]*)\)", text).group(1).split(",")
