@@ -504,8 +504,13 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
       const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
       // this lane's piece of a tile starts `lane * st` tokens into it
       const int my = lane * st;
+      // (not by way of L1 where no wait stands between the tables' last change and here)
+      auto listed = [&](int t) -> int {
+        const int32_t* at = bt + page_of(t);
+        return p.beside ? __ldcg(at) : *at;
+      };
       int pg = 0;
-      if (my < ATT_TILE && tok_begin + my < tok_end) pg = bt[page_of(tok_begin + my)];
+      if (my < ATT_TILE && tok_begin + my < tok_end) pg = listed(tok_begin + my);
       for (int tok0 = tok_begin; tok0 < tok_end; tok0 += ATT_TILE) {
         // wait until the consumers released this stage (a fresh barrier
         // passes the parity-1 test, so the first lap does not block)
@@ -568,7 +573,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
           }
         }
         const int tn = tok0 + ATT_TILE + my;  // this lane's piece of the next tile
-        if (my < ATT_TILE && tn < tok_end) pg = bt[page_of(tn)];
+        if (my < ATT_TILE && tn < tok_end) pg = listed(tn);
         if (++stage == ATT_STAGES) { stage = 0; phase ^= 1; }
       }
     }

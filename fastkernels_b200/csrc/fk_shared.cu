@@ -220,15 +220,26 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
     const int here = min(PLAN_THREADS, groups - g0);
     for (int i = warp; i < here; i += PLAN_WARPS) {
       const int a = p.starts[g0 + i], b = p.starts[g0 + i + 1], prefix = p.prefix[g0 + i];
-      int longest = 0, table = a;
+      int longest = 0, shortest = 0x7fffffff, table = a;
       for (int r = a + lane; r < b; r += 32) {
         const int n = s_len[r];
         if (n > longest) { longest = n; table = r; }
+        if (n > 0) shortest = min(shortest, n);
       }
       const int most = __reduce_max_sync(0xffffffffu, longest);
+      shortest = __reduce_min_sync(0xffffffffu, shortest);
       table = __reduce_min_sync(0xffffffffu, longest == most ? table : 0x7fffffff);
+      // Rows either see all keys of their item or have them for themselves, so that what a row does not
+      // see is not multiplied by its zeros.  The item ends where the shortest row does, unless that
+      // would leave most of the prefix to every row.
+      const int full = max(0, min(prefix, most)) / p.page * p.page;
+      const int all = min(full, shortest / p.page * p.page);
+      const int keys = all >= full / 2 ? all : full;
+      int sharing = 0;
+      for (int r = a + lane; r < b; r += 32) sharing += s_len[r] >= keys ? 1 : 0;
+      sharing = __reduce_add_sync(0xffffffffu, sharing);
       if (lane == 0) {
-        s_keys[i] = b - a < 2 ? 0 : max(0, min(prefix, most)) / p.page * p.page;
+        s_keys[i] = sharing < 2 ? 0 : keys;
         s_table[i] = table;
       }
     }
@@ -257,6 +268,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
             PrefixItem{a + j * each, min(each, n - j * each), s_table[i], keys_i,
                        s_start[i] + j * tiles_i * p.hkv, tiles_i, 0, 0};
       for (int r = lane; r < n; r += 32) {
+        if (s_len[a + r] < keys_i) continue;
         const int j = r / each;
         p.plan.row_part[a + r] = make_int4(s_start[i] + j * tiles_i * p.hkv, tiles_i,
                                            (s_item[i] + j) * p.hkv, r - j * each);
@@ -705,7 +717,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
         const int in_tile = (quad * 32 + lane) / p.g, i = t * p.per_tile + in_tile;
         if (in_tile < p.per_tile && i < w.it.rows) {
           const int64_t len = p.lens[w.it.row0 + i];
-          lim = (int)(len < 0 ? 0 : len < w.it.keys ? len : w.it.keys);
+          lim = len >= w.it.keys ? w.it.keys : 0;
         }
       }
       float m_used = -INFINITY, l = 0.f;

@@ -188,20 +188,20 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  *
  * fk_shared_prefix_attn: out as fk_paged_decode_attn, for a batch in which the
  * rows group_starts[g] .. group_starts[g + 1] - 1 list the same pages for their
- * first prefix_lens[g] tokens (whole pages of them).  That part is read once for
- * all rows of the group: their
- * query heads are the rows of one tcgen05 product per KV head.  group_starts
- * [num_groups + 1] ascends within the batch; rows outside of all groups, and groups of
- * one row, have nothing in common.  (Starts that do not ascend within the batch are
- * flagged FK_DEV_BAD_POSITION; no row has anything in common then.)  A row's context may
- * end inside the common part.  The table of the group's row with the longest context is
- * read for it.  max_splits: upper bound of KV splits of what each row has for itself.
- * softmax_scale above zero.  Launches: schedule, common part, own parts, join; one launch
- * where batch * num_kv_heads fits the SMs and the tables have at most 2048 tokens.
+ * first prefix_lens[g] tokens (whole pages of them).  That part is read once for all
+ * rows of the group, by the table of its longest row: their query heads are the rows
+ * of one tcgen05 product per KV head.  group_starts [num_groups + 1] ascends within the
+ * batch; rows outside of all groups, and groups of one row, have nothing in common.
+ * (Starts that do not ascend within the batch are flagged FK_DEV_BAD_POSITION; no row has
+ * anything in common then.)  A row whose context ends inside the common part has it for
+ * itself, or the others share no more than that row has.  max_splits: upper bound of KV
+ * splits of what each row has for itself.  softmax_scale above zero.  Launches: schedule,
+ * common part, own parts (beside it), join; one launch where batch * num_kv_heads fits the
+ * SMs and the tables have at most 2048 tokens.
  * fk_shared_prefix_plan computes the schedule of a step into the workspace, and calls
  * with `planned` go by it for any number of layers afterwards, with the same lengths,
- * groups, sizes, head counts, table columns, max_splits and workspace.  The workspace
- * serves one call at a time.
+ * groups, sizes, head counts, table columns, max_splits and workspace.  A workspace serves
+ * one call at a time (and two captured graphs only one after the other).
  *
  * fk_key_bounds: bounds[page][head][i][0 / 1][d] = smallest / largest key of
  * channel d over the cached tokens of the i-th run of `block` positions of a page,

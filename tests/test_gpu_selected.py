@@ -257,7 +257,8 @@ def attend_oracle(q, kc, vc, lens, table, sel, page, block, layout, hkv, rows):
     (64, 32, "HND", 14, 2, [900, 31, 33], 13), (32, 32, "NHD", 4, 4, [1, 2, 999], 16),
     (256, 256, "HND", 8, 1, [3000, 255], 4), (16, 16, "NHD", 16, 1, [2100], 128),
     (64, 64, "HND", 9, 3, [0, 40, 128, 0], 3), (256, 128, "NHD", 2, 2, [1100, 130, 127], 7),
-    (192, 64, "NHD", 4, 2, [600, 193], 6)])
+    (192, 64, "NHD", 4, 2, [600, 193], 6), (16, 16, "NHD", 4, 2, [1, 16, 17, 900], 1),
+    (512, 192 + 64, "NHD", 4, 1, [1500, 512], 3), (384, 192, "HND", 4, 2, [1500, 384, 191], 5)])
 @pytest.mark.parametrize("wild", [False, True])
 def test_attention_over_selected_blocks(ops, page, block, layout, hq, hkv, lens, count, wild):
     q, kc, vc, table, sel = attend_case(page + hq + count, lens, hq, hkv, page, block, layout,

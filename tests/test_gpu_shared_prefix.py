@@ -19,7 +19,13 @@ def ints(a):
     return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
 
 
-def build(seed, groups, page, layout, hq, hkv, extra_rows=()):
+def widened(table, page):
+    """With room for more than 2048 tokens, whose calls are not one launch without a schedule."""
+    extra = max(0, 2048 // page + 1 - table.shape[1])
+    return np.concatenate([table, np.full((len(table), extra), -1, np.int32)], 1)
+
+
+def build(seed, groups, page, layout, hq, hkv, extra_rows=(), wide=True):
     """groups: (prefix tokens, [tokens behind it of each row]).  Rows of a group share the whole
     pages of its prefix.  extra_rows: lengths of rows behind the last group.  What is behind
     a row's last token, and in nobody's pages, is no number."""
@@ -59,6 +65,8 @@ def build(seed, groups, page, layout, hq, hkv, extra_rows=()):
     for c in (kc, vc):
         (c if layout == "NHD" else c.swapaxes(1, 2))[~live] = np.nan
     q = S.bf16(rng.standard_normal((len(lens), hq, S.D)))
+    if wide:
+        table = widened(table, page)
     return q, kc, vc, np.array(lens, np.int32), table, starts, prefix
 
 
@@ -93,8 +101,19 @@ def test_groups_of_all_kinds(ops, page, layout, hq, hkv):
               (5 * page, [-page - 3, 2, -5 * page, 1]),  # rows that end inside it, one empty
               (2 * page + 5, [20, 30]),                  # ends inside a page
               (page - 1, [page, 9])]                     # not one whole page
-    check(ops, build(page + hq, groups, page, layout, hq, hkv, extra_rows=[70, 0, 1]), page, layout,
-          hkv)
+    for wide in (True, False):
+        check(ops, build(page + hq, groups, page, layout, hq, hkv, extra_rows=[70, 0, 1], wide=wide),
+              page, layout, hkv)
+
+
+@pytest.mark.parametrize("g", [1, 3, 4, 16])
+def test_small_calls_are_one_launch(ops, g):
+    from fastkernels_b200 import _lib
+    case = build(40 + g, [(512, [1, 200, 64]), (256, [9, -1, -256])], 64, "HND", 2 * g, 2,
+                 extra_rows=[5], wide=False)
+    before = _lib.lib.fk_launch_count()
+    check(ops, case, 64, "HND", 2)
+    assert _lib.lib.fk_launch_count() == before + 1
 
 
 @pytest.mark.parametrize("rows,hq,hkv", [(2, 2, 2), (33, 4, 1), (32, 8, 2), (40, 16, 1),
@@ -112,6 +131,57 @@ def test_lengths_of_the_common_part(ops, prefix):
     check(ops, case, 16, "HND", 2)
 
 
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("short,bad", [(100, np.nan), (700, np.inf), (1023, np.nan)])
+def test_what_a_short_row_does_not_see(ops, short, bad, wide):
+    """A row that ends inside the common part, with keys or values behind its end that are no numbers or
+    infinite: they are the others' results alone."""
+    case = build(31, [(1024, [50, 60, short - 1024, 700, -1024])], 64, "NHD", 16, 4, wide=wide)
+    q, kc, vc, lens, table, starts, prefix = case
+    kc, vc = np.nan_to_num(kc), np.nan_to_num(vc)
+    p, o = table[0, short // 64], short % 64              # the first position behind its end
+    vc[p, o, 1] = bad
+    kc[p, o, 2] = bad
+    case = (q, kc, vc, lens, table, starts, prefix)
+    got = host_f32(run(ops, case, "NHD", max_splits=4))
+    assert lens.tolist() == [1074, 1084, short, 1724, 0]
+    want, mass = S.over_positions(q[2:3], kc, vc, lens[2:3], table[2:3], 64, "NHD", 4,
+                                  lambda i, h: range(short))
+    assert (np.abs(got[2:3] - want) <= S.tolerance(want, mass)).all()
+    assert (got[4] == 0).all()
+    assert not np.isfinite(got[:2, 4:8]).any()            # the heads of the value's KV head
+    assert np.isfinite(got[:, :4]).all() and np.isfinite(got[:, 12:]).all()
+
+
+def test_pages_far_behind(ops):
+    """Pages more than 2^32 bytes into a pool."""
+    pages = 34000
+    pool = torch.zeros((pages, 64, 8, 128), dtype=torch.bfloat16, device="cuda")
+    assert pool.numel() * 2 > 2 ** 32
+    rng = np.random.default_rng(3)
+    small = S.pool(rng, 40, 64, 8, "NHD")
+    pool[-40:] = dev(small)
+    case = build(33, [(1024, [70, 300, 5])], 64, "NHD", 16, 8)
+    q, _, _, lens, table, starts, prefix = case
+    far = np.where(table >= 0, table + pages - 40, -1).astype(np.int32)
+    assert table.max() < 40
+    args = [ints(lens), ints(starts), ints(prefix)]
+    near = ops.shared_prefix_attn(dev(q), dev(small), dev(small), args[0], ints(table), *args[1:],
+                                  S.SCALE)
+    got = ops.shared_prefix_attn(dev(q), pool, pool, args[0], ints(far), *args[1:], S.SCALE)
+    assert torch.equal(got, near)
+    for block in (16, 64):
+        sel = ops.select_blocks(dev(q), dev(S.bounds_of(small, 64, block, "NHD")), args[0], ints(table),
+                                block, 9)
+        b = ops.new_key_bounds(pool, block)
+        ops.key_bounds(pool, b, args[0], ints(far), cu_new=ints(np.cumsum([0, *lens])),
+                       max_new=int(max(lens)))
+        assert torch.equal(ops.select_blocks(dev(q), b, args[0], ints(far), block, 9), sel)
+        near, got = (ops.selected_attn(dev(q), c, c, args[0], ints(t), sel, block, S.SCALE)
+                     for c, t in ((dev(small), table), (pool, far)))
+        assert torch.equal(got, near)
+
+
 def test_many_groups(ops):
     rng = np.random.default_rng(2)
     groups = [(int(rng.integers(0, 9)) * 16, [int(x) for x in rng.integers(1, 60, rng.integers(1, 5))])
@@ -120,9 +190,10 @@ def test_many_groups(ops):
 
 
 def test_no_groups_and_one_row(ops):
-    check(ops, build(1, [], 64, "NHD", 8, 2, extra_rows=[1, 700, 64, 0]), 64, "NHD", 2)
-    check(ops, build(2, [(640, [11])], 64, "NHD", 8, 2), 64, "NHD", 2)
-    check(ops, build(3, [(1280, [1, 1])], 64, "NHD", 8, 2), 64, "NHD", 2, max_splits=1)
+    for wide in (True, False):
+        check(ops, build(1, [], 64, "NHD", 8, 2, extra_rows=[1, 700, 64, 0], wide=wide), 64, "NHD", 2)
+        check(ops, build(2, [(640, [11])], 64, "NHD", 8, 2, wide=wide), 64, "NHD", 2)
+        check(ops, build(3, [(1280, [1, 1])], 64, "NHD", 8, 2, wide=wide), 64, "NHD", 2, max_splits=1)
 
 
 def test_large_scores(ops):
@@ -154,17 +225,22 @@ def test_bad_pages_are_flagged_and_left_out(ops):
     q, kc, vc, lens, table, starts, prefix = case
     good = host_f32(run(ops, case, "NHD"))
     broken = table.copy()
-    broken[0, 1], broken[4, 2] = 10 ** 6, -7
+    broken[2, 1], broken[4, 2] = 10 ** 6, -7       # the longest row's is read for its group
     st = ops.new_status("cuda")
     got = host_f32(run(ops, (q, kc, vc, lens, broken, starts, prefix), "NHD", st))
     assert int(st.item()) == 2
     assert np.isfinite(got).all() and (got[3] == good[3]).all()
+    narrow = broken[:, :7]
+    st = ops.new_status("cuda")
+    got = host_f32(run(ops, (q, kc, vc, lens, narrow, starts, prefix), "NHD", st))
+    assert int(st.item()) == 2 and np.isfinite(got).all()
 
 
-def test_groups_that_do_not_fit_the_batch(ops):
+@pytest.mark.parametrize("wide", [True, False])
+def test_groups_that_do_not_fit_the_batch(ops, wide):
     """Starts past the batch or below the one before are flagged; nobody has anything in common
     then, and all rows have their results."""
-    case = build(7, [(128, [5, 9, 70]), (64, [3, 4])], 64, "NHD", 4, 2)
+    case = build(7, [(128, [5, 9, 70]), (64, [3, 4])], 64, "NHD", 4, 2, wide=wide)
     q, kc, vc, lens, table, _, prefix = case
     good = host_f32(run(ops, case, "NHD"))
     for starts in ([0, 3, 99], [-4, 3, 5], [0, 3, 1]):
