@@ -192,10 +192,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
   __shared__ int64_t red[PLAN_WARPS];
   __shared__ int s_keys[PLAN_THREADS], s_table[PLAN_THREADS], s_item[PLAN_THREADS],
       s_start[PLAN_THREADS], s_count[6];
+  __shared__ int s_first[PLAN_THREADS + 1], s_prefix[PLAN_THREADS];   // of a round's groups
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   pdl_wait();
   bool cut = false, odd = false;
+  // a round of groups: their first rows, one more, and their prefixes
+  auto fetch = [&](int g0, int here) {
+    if (tid < here) {
+      s_first[tid] = p.starts[g0 + tid];
+      if (tid == here - 1) s_first[here] = p.starts[g0 + here];
+      s_prefix[tid] = p.prefix[g0 + tid];
+    }
+  };
+  fetch(0, min(PLAN_THREADS, p.groups));
   for (int i = tid; i < p.batch; i += PLAN_THREADS) {
     const int64_t len = p.lens[i];
     cut |= len > p.capacity;
@@ -218,8 +228,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
   int items = 0, tiles = 0;                    // of the groups before
   for (int g0 = 0; g0 < groups; g0 += PLAN_THREADS) {
     const int here = min(PLAN_THREADS, groups - g0);
+    if (g0 > 0) {
+      fetch(g0, here);
+      __syncthreads();
+    }
     for (int i = warp; i < here; i += PLAN_WARPS) {
-      const int a = p.starts[g0 + i], b = p.starts[g0 + i + 1], prefix = p.prefix[g0 + i];
+      const int a = s_first[i], b = s_first[i + 1], prefix = s_prefix[i];
       int longest = 0, shortest = 0x7fffffff, table = a;
       for (int r = a + lane; r < b; r += 32) {
         const int n = s_len[r];
@@ -245,7 +259,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
     }
     __syncthreads();
     const int keys = tid < here ? s_keys[tid] : 0;
-    const int mine = keys > 0 ? (p.starts[g0 + tid + 1] - p.starts[g0 + tid] + span - 1) / span : 0;
+    const int mine = keys > 0 ? (s_first[tid + 1] - s_first[tid] + span - 1) / span : 0;
     const int per_item = (keys + ATT_TILE - 1) / ATT_TILE;
     // both sums at once: items in the upper half, tiles in the lower
     int64_t all;
@@ -260,7 +274,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
       const int keys_i = s_keys[i];
       if (keys_i == 0) continue;
       // the rows of a group evenly over its items
-      const int a = p.starts[g0 + i], n = p.starts[g0 + i + 1] - a;
+      const int a = s_first[i], n = s_first[i + 1] - a;
       const int m = (n + span - 1) / span, each = (n + m - 1) / m;
       const int tiles_i = (keys_i + ATT_TILE - 1) / ATT_TILE;
       for (int j = lane; j < m; j += 32)
@@ -303,18 +317,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
   if (least > chunk) chunk = (int)least;
   for (int k = 0; k < 3 && chunk > least && (int64_t)s_count[k] * p.hkv < 4ll * p.ctas; ++k)
     chunk >>= 1;
-  const int64_t own = (int64_t)s_count[3] * p.hkv * PLAN_OWN_COST;
-  const int64_t common = (int64_t)tiles * PLAN_COMMON_COST;
+  const float own = (float)s_count[3] * (float)(p.hkv * PLAN_OWN_COST);
+  const float common = (float)tiles * (float)PLAN_COMMON_COST;
   // SMs for the common part; its CTAs take `unit` tiles each
   int ctas = p.ctas;
-  if (p.beside && own > 0 && common > 0)
-    ctas = max(p.ctas / 8, min(p.ctas, (int)((p.ctas * common + common + own - 1) / (common + own))));
+  if (p.beside && own > 0.f && common > 0.f)
+    ctas = max(p.ctas / 8, min(p.ctas, (int)((float)p.ctas * common / (common + own)) + 1));
   const int unit = max(p.min_unit, (tiles + ctas - 1) / max(ctas, 1));
   // CTAs whose first tile is in an item
-  for (int i = tid; i < items; i += PLAN_THREADS) {
+  for (int i = warp; i < items; i += PLAN_WARPS) {
     const PrefixItem it = p.plan.items[i];
     const int end = it.start + it.tiles * p.hkv;
-    for (int c = (it.start + unit - 1) / unit; c < p.ctas && (int64_t)c * unit < end; ++c)
+    for (int c = (it.start + unit - 1) / unit + lane; c < p.ctas && (int64_t)c * unit < end; c += 32)
       p.plan.cta_item[c] = i;
   }
   int* chunk_start = p.plan.hdr + PLAN_HDR;
