@@ -128,13 +128,13 @@ struct SelectParams {
   int num_tokens, num_tables, num_pages, page, block, hkv, g;
   int count, keep_first, keep_last;
   int per_shift;                      // log2 of the blocks of a page, -1: no power of two
-  int together;                       // tokens of a CTA: 1, or 16 / g
-  int g_shift;                        // log2 of g where that is 16 / g
+  int span;                           // tokens of a CTA of the scores
+  int cols;                           // columns of a token in a product: g up to a power of two
   int most;                           // blocks that a table's row has pages for
   int pitch;                          // of the scores' rows: a multiple of four
   int chunk, chunks;                  // blocks of a CTA of the scores, of those CTAs per token
   uint32_t* scores;                   // [tokens, hkv, pitch], ordered
-  float* largest;                     // [groups of tokens, hkv, chunks] largest |bound| of a chunk
+  float* largest;                     // [spans of tokens, hkv, chunks] largest |bound| of a chunk
   float* q_sum;                       // [tokens, hkv] largest sum of |q| of a query head
   int32_t* selected;                  // [tokens, hkv, count]
   int32_t* status;
@@ -505,20 +505,102 @@ __device__ __forceinline__ void copy16(uint4* dst, const uint16_t* src, bool hav
                : "memory");
 }
 
-// ---- scores: a CTA per token (or several of one table), KV head and chunk of blocks
-//
-// sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with the positive and negative parts of q: a
-// product of 16 blocks by 8 or 16 columns (query heads, of several tokens where they fit) by 256 on
-// the tensor cores.  A warp has 16 blocks at a time and as many on their way in shared memory; a lane
-// copies the 16-byte pieces that it uses itself, which are operands of two instructions when q's
-// channels are taken in the same order.  Sums in fp32 are off by at most e = 2^-18 sum |q| max
-// |bound|: an instruction adds 17 terms (its sum begins at zero), each off by at most 2^-23 of the
-// sum of absolute values, and a term goes through at most six further additions of 2^-24: 20 x
-// 2^-23 = 2^-18.7.
-//
-// Bounds: the bytes of the bounds, and the instructions around the products.  (Blocks as the 8
-// columns of a product, heads as its 16 rows, took twice as many of them.)
-template <int NT>                              // 8 columns each
+// ---- scores: sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with the positive and negative parts of
+// q, a product of 16 blocks by 8 query heads by 256 on the tensor cores.  A lane takes 16 bytes of a
+// row at a time, which are operands of two instructions when q's channels are taken in the same
+// order.  Sums in fp32 are off by at most e = 2^-18 sum |q| max |bound|: an instruction adds 17 terms
+// (its sum begins at zero), each off by at most 2^-23 of the sum of absolute values, and a term
+// goes through at most six further additions of 2^-24: 20 x 2^-23 = 2^-18.7.
+
+// 16 blocks (two of them with this lane's pieces: lower and upper bounds) by 8 columns; v: columns
+// 2 (lane % 4) + 0, 1 of blocks lane / 4 and lane / 4 + 8.
+__device__ __forceinline__ void score_tile(const uint4 (&l0)[4], const uint4 (&u0)[4],
+                                           const uint4 (&l1)[4], const uint4 (&u1)[4],
+                                           const uint32_t (&qp)[4][4], const uint32_t (&qm)[4][4],
+                                           float (&v)[4]) {
+  uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float c[4][4];
+    mma_from_zero(c[0], u0[j].x, u1[j].x, u0[j].y, u1[j].y, qp[j][0], qp[j][1]);
+    mma_from_zero(c[1], l0[j].x, l1[j].x, l0[j].y, l1[j].y, qm[j][0], qm[j][1]);
+    mma_from_zero(c[2], u0[j].z, u1[j].z, u0[j].w, u1[j].w, qp[j][2], qp[j][3]);
+    mma_from_zero(c[3], l0[j].z, l1[j].z, l0[j].w, l1[j].w, qm[j][2], qm[j][3]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      sum[i] = add_pair(sum[i], add_pair(add_pair(pair_of(c[0][2 * i], c[0][2 * i + 1]),
+                                                  pair_of(c[1][2 * i], c[1][2 * i + 1])),
+                                         add_pair(pair_of(c[2][2 * i], c[2][2 * i + 1]),
+                                                  pair_of(c[3][2 * i], c[3][2 * i + 1]))));
+  }
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v[0]), "=f"(v[1]) : "l"(sum[0]));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2]), "=f"(v[3]) : "l"(sum[1]));
+}
+
+// The largest upper bound and the smallest lower one, two channels at once, from below and above zero:
+// bits of bf16 as signed numbers order those above zero, and as unsigned ones those below it, the
+// most negative last.  (A bound that is no number makes a score that is none.)
+struct Extent {
+  uint32_t top = 0u, low = 0x80008000u;
+  __device__ __forceinline__ void add(const uint4& l, const uint4& u) {
+    top = __vimax3_s16x2(top, u.x, u.y); top = __vimax3_s16x2(top, u.z, u.w);
+    low = __vimax3_u16x2(low, l.x, l.y); low = __vimax3_u16x2(low, l.z, l.w);
+  }
+  // largest |bound| of a CTA's warps, as a number's bits; `scratch`: a word per warp
+  __device__ __forceinline__ uint32_t of_cta(uint32_t* scratch) const {
+    uint32_t most = max(max((top & 0xffffu) << 16, top & 0x7fff0000u),
+                        max((low & 0x7fffu) << 16, low & 0x7fff0000u));
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SEL_WARPS; ++w) most = max(most, scratch[w]);
+    return most;
+  }
+};
+
+__device__ __forceinline__ int select_length(const SelectParams& p, int token, int row) {
+  const int64_t len = p.context_lens[token];
+  if (len <= 0 || row < 0 || row >= p.num_tables) return 0;
+  return (int)(len > p.capacity ? p.capacity : len);
+}
+// blocks keep_first .. of a context that are scored
+__device__ __forceinline__ int select_scored(const SelectParams& p, int len) {
+  const int blocks = (int)(((int64_t)len + p.block - 1) / p.block);
+  return blocks > p.count ? blocks - p.keep_first - p.keep_last : 0;
+}
+// positive and negative parts of a column's channels 32 j + 8 (lane % 4) + 0 .. 7
+__device__ __forceinline__ void split_q(const uint4 (&v)[4], uint32_t (&qp)[4][4],
+                                        uint32_t (&qm)[4][4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      qp[j][i] = max2_nan(w[i], 0u);
+      qm[j][i] = min2_nan(w[i], 0u);
+    }
+  }
+}
+// sum of |q| of a column, over its four lanes; no number counts as infinite
+__device__ __forceinline__ float abs_q(const uint4 (&v)[4]) {
+  float a = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a += fabsf(bf16lo(w[i])) + fabsf(bf16hi(w[i]));
+  }
+  a += __shfl_xor_sync(0xffffffffu, a, 1);
+  a += __shfl_xor_sync(0xffffffffu, a, 2);
+  return a < INFINITY ? a : INFINITY;
+}
+
+// ---- a token for itself: a CTA per token, KV head and chunk of blocks.  A warp has 16 blocks at a time
+// and as many on their way in shared memory.  Bounds: the bytes of the bounds (64 tokens of 8192 to
+// 65536 keys, 148 MB: 31 us), and the instructions around the products.
+template <int NT>                              // 8 query heads each
 __global__ void __launch_bounds__(32 * SEL_WARPS, 3)
 select_scores_kernel(const SelectParams p) {
   extern __shared__ __align__(16) uint8_t sel_smem[];
@@ -527,39 +609,15 @@ select_scores_kernel(const SelectParams p) {
   pdl_wait();
   const int kvh = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = blockIdx.x / p.chunks, chunk = blockIdx.x - group * p.chunks;
+  const int token = blockIdx.x / p.chunks, chunk = blockIdx.x - token * p.chunks;
   const int per = p.page / p.block;
   const int r0 = lane >> 2, quad = lane & 3;
-
-  // tables and lengths of the group's tokens, a lane each
-  const int first_token = group * p.together;
-  const int tokens = min(p.together, p.num_tokens - first_token);
-  int my_row = -1, my_len = 0;
-  if (lane < tokens) {
-    my_row = p.rows ? p.rows[first_token + lane] : first_token + lane;
-    const int64_t len = p.context_lens[first_token + lane];
-    my_len = (int)(len > p.capacity ? p.capacity : len < 0 ? 0 : len);
-    if (my_row < 0 || my_row >= p.num_tables) my_len = 0;
-  }
-  // The largest upper bound and the smallest lower one, two channels at once, from below and above zero:
-  // bits of bf16 as signed numbers order those above zero, and as unsigned ones those below it, the
-  // most negative last.  (A bound that is no number makes a score that is none.)
-  uint32_t top = 0u, low = 0x80008000u;
-  // runs of tokens with one table
-  for (int i0 = 0; i0 < tokens;) {
-    const int row = __shfl_sync(0xffffffffu, my_row, i0);
-    const uint32_t others =
-        __ballot_sync(0xffffffffu, lane >= tokens || my_row != row) & (~0u << i0);
-    const int i1 = others ? __ffs(others) - 1 : 32;
-    const int t0 = first_token + i0, t1 = first_token + i1;
-    const int longest = __reduce_max_sync(0xffffffffu, lane >= i0 && lane < i1 ? my_len : 0);
-    i0 = i1;
+  const int row = token;
+  const int scored = select_scored(p, select_length(p, token, row));
+  const int begin = chunk * p.chunk, end = min(scored, begin + p.chunk);
+  Extent extent;
+  if (begin < end) {
     const int32_t* table = p.tables + (int64_t)row * p.table_stride;
-    // scores of blocks keep_first .. of the longest context; a shorter one uses fewer of them
-    const int blocks = (int)(((int64_t)longest + p.block - 1) / p.block);
-    const int scored = blocks > p.count ? blocks - p.keep_first - p.keep_last : 0;
-    const int begin = chunk * p.chunk, end = min(scored, begin + p.chunk);
-    if (begin >= end) continue;
     // pages of the two blocks that this lane copies pieces of
     auto page_of = [&](int at) -> int {
       const int b = p.keep_first + at;
@@ -591,80 +649,49 @@ select_scores_kernel(const SelectParams p) {
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
     int page0 = page_of(ahead + r0), page1 = page_of(ahead + 8 + r0);
-    // column lane / 4 of 8: a query head of a token; channels 32 j + 8 (lane % 4) + 0 .. 7
+    // column lane / 4 of 8: a query head
     uint32_t qp[NT][4][4], qm[NT][4][4];
-    float abs_sum[NT];
+    float abs_sum = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int col = nt * 8 + r0;
-      const int t = t0 + (p.together == 1 ? (col < p.g ? 0 : 1) : col >> p.g_shift);
-      const int head = p.together == 1 ? col : col & (p.g - 1);
-      abs_sum[nt] = 0.f;
+      const int head = nt * 8 + r0;
+      uint4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (t < t1)
-          v = *reinterpret_cast<const uint4*>(
-              p.q + (int64_t)t * p.q_stride + ((int64_t)kvh * p.g + head) * SEL_D + j * 32 + quad * 8);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qp[nt][j][i] = max2_nan(w[i], 0u);
-          qm[nt][j][i] = min2_nan(w[i], 0u);
-          abs_sum[nt] += fabsf(bf16lo(w[i])) + fabsf(bf16hi(w[i]));
-        }
-      }
+      for (int j = 0; j < 4; ++j)
+        v[j] = head < p.g ? *reinterpret_cast<const uint4*>(
+                                p.q + (int64_t)token * p.q_stride +
+                                ((int64_t)kvh * p.g + head) * SEL_D + j * 32 + quad * 8)
+                          : make_uint4(0u, 0u, 0u, 0u);
+      split_q(v, qp[nt], qm[nt]);
+      if (chunk == 0 && warp == 0) abs_sum = fmaxf(abs_sum, abs_q(v));
     }
     if (chunk == 0 && warp == 0) {
-      // the largest sum of |q| of each token's heads; no number counts as infinite
-      float mine[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float a = abs_sum[nt];
-        a += __shfl_xor_sync(0xffffffffu, a, 1);
-        a += __shfl_xor_sync(0xffffffffu, a, 2);
-        mine[nt] = a < INFINITY ? a : INFINITY;
-      }
-      for (int t = t0; t < t1; ++t) {
-        float best = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          if (p.together == 1 || t0 + ((nt * 8 + r0) >> p.g_shift) == t)
-            best = fmaxf(best, mine[nt]);
-        best = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(best)));
-        if (lane == 0) p.q_sum[(int64_t)t * p.hkv + kvh] = best;
-      }
+      abs_sum = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(abs_sum)));
+      if (lane == 0) p.q_sum[(int64_t)token * p.hkv + kvh] = abs_sum;
     }
     int stage = 0;
     for (int b0 = begin + warp * 16; b0 < end; b0 += kStep) {
       asm volatile("cp.async.wait_group %0;" ::"n"(SEL_STAGES - 1) : "memory");
       const uint4* src = ring + (warp * SEL_STAGES + stage) * 512 + lane;
-      uint64_t sum[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = 0ull;
+      uint4 l0[4], u0[4], l1[4], u1[4];        // blocks r0 and r0 + 8
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 l0 = src[j * 32], u0 = src[(4 + j) * 32];            // block r0
-        const uint4 l1 = src[(8 + j) * 32], u1 = src[(12 + j) * 32];     // block r0 + 8
+        l0[j] = src[j * 32]; u0[j] = src[(4 + j) * 32];
+        l1[j] = src[(8 + j) * 32]; u1[j] = src[(12 + j) * 32];
+        extent.add(l0[j], u0[j]);
+        extent.add(l1[j], u1[j]);
+      }
+      float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float c[4][4];
-          mma_from_zero(c[0], u0.x, u1.x, u0.y, u1.y, qp[nt][j][0], qp[nt][j][1]);
-          mma_from_zero(c[1], l0.x, l1.x, l0.y, l1.y, qm[nt][j][0], qm[nt][j][1]);
-          mma_from_zero(c[2], u0.z, u1.z, u0.w, u1.w, qp[nt][j][2], qp[nt][j][3]);
-          mma_from_zero(c[3], l0.z, l1.z, l0.w, l1.w, qm[nt][j][2], qm[nt][j][3]);
+      for (int nt = 0; nt < NT; ++nt) {
+        float v[4];
+        score_tile(l0, u0, l1, u1, qp[nt], qm[nt], v);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            sum[nt][i] = add_pair(
-                sum[nt][i], add_pair(add_pair(pair_of(c[0][2 * i], c[0][2 * i + 1]),
-                                              pair_of(c[1][2 * i], c[1][2 * i + 1])),
-                                     add_pair(pair_of(c[2][2 * i], c[2][2 * i + 1]),
-                                              pair_of(c[3][2 * i], c[3][2 * i + 1]))));
+        for (int i = 0; i < 2; ++i) {
+          const bool live = nt * 8 + quad * 2 + i < p.g;
+          m0 = max_nan(m0, live ? v[i] : -INFINITY);
+          m1 = max_nan(m1, live ? v[2 + i] : -INFINITY);
         }
-        top = __vimax3_s16x2(top, u0.x, u0.y); top = __vimax3_s16x2(top, u0.z, u0.w);
-        top = __vimax3_s16x2(top, u1.x, u1.y); top = __vimax3_s16x2(top, u1.z, u1.w);
-        low = __vimax3_u16x2(low, l0.x, l0.y); low = __vimax3_u16x2(low, l0.z, l0.w);
-        low = __vimax3_u16x2(low, l1.x, l1.y); low = __vimax3_u16x2(low, l1.z, l1.w);
       }
       const bool ok0 = have >> (stage * 2) & 1u, ok1 = have >> (stage * 2 + 1) & 1u;
       // the stage has been read: its next blocks
@@ -675,70 +702,143 @@ select_scores_kernel(const SelectParams p) {
       asm volatile("cp.async.commit_group;" ::: "memory");
       ahead += kStep;
       if (++stage == SEL_STAGES) stage = 0;
-      // columns 2 quad + 0, 1 of blocks r0 (v[0], v[1]) and r0 + 8: the largest of a token's
-      float v[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[nt][0]), "=f"(v[nt][1]) : "l"(sum[nt][0]));
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[nt][2]), "=f"(v[nt][3]) : "l"(sum[nt][1]));
+      for (int o = 1; o < 4; o <<= 1) {
+        m0 = max_nan(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+        m1 = max_nan(m1, __shfl_xor_sync(0xffffffffu, m1, o));
       }
-      uint32_t* scores = p.scores + ((int64_t)t0 * p.hkv + kvh) * p.pitch + b0 + r0;
-      const bool in0 = b0 + r0 < end, in1 = b0 + 8 + r0 < end;
-      if (p.together == 1) {
-        float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const bool live = nt * 8 + quad * 2 + i < p.g;
-            m0 = max_nan(m0, live ? v[nt][i] : -INFINITY);
-            m1 = max_nan(m1, live ? v[nt][2 + i] : -INFINITY);
-          }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          m0 = max_nan(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-          m1 = max_nan(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-        }
-        if (quad == 0 && in0) scores[0] = ok0 ? order_of(m0) : 0u;
-        if (quad == 0 && in1) scores[8] = ok1 ? order_of(m1) : 0u;
-      } else {
-        // a power of two of heads: next columns, then next lanes
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (p.g > 1) {
-            v[nt][0] = v[nt][1] = max_nan(v[nt][0], v[nt][1]);
-            v[nt][2] = v[nt][3] = max_nan(v[nt][2], v[nt][3]);
-          }
-          for (int o = 1; o < p.g / 2; o <<= 1) {
-            v[nt][0] = max_nan(v[nt][0], __shfl_xor_sync(0xffffffffu, v[nt][0], o));
-            v[nt][2] = max_nan(v[nt][2], __shfl_xor_sync(0xffffffffu, v[nt][2], o));
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int col = nt * 8 + quad * 2 + i;
-            const int of = col >> p.g_shift;
-            if (of << p.g_shift != col || t0 + of >= t1) continue;
-            uint32_t* at = scores + (int64_t)of * p.hkv * p.pitch;
-            if (in0) at[0] = ok0 ? order_of(v[nt][i]) : 0u;
-            if (in1) at[8] = ok1 ? order_of(v[nt][2 + i]) : 0u;
-          }
-        }
-      }
+      uint32_t* scores = p.scores + ((int64_t)token * p.hkv + kvh) * p.pitch + b0 + r0;
+      if (quad == 0 && b0 + r0 < end) scores[0] = ok0 ? order_of(m0) : 0u;
+      if (quad == 0 && b0 + 8 + r0 < end) scores[8] = ok1 ? order_of(m1) : 0u;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  uint32_t most = max(max((top & 0xffffu) << 16, top & 0x7fff0000u),
-                      max((low & 0x7fffu) << 16, low & 0x7fff0000u));
-  most = __reduce_max_sync(0xffffffffu, most);
-  uint32_t* most_of = reinterpret_cast<uint32_t*>(ring);      // which has been read
-  __syncthreads();
-  if (lane == 0) most_of[warp] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  const uint32_t most = extent.of_cta(reinterpret_cast<uint32_t*>(ring));     // which has been read
+  if (threadIdx.x == 0)
+    p.largest[((int64_t)token * p.hkv + kvh) * p.chunks + chunk] = __uint_as_float(most);
+}
+
+// ---- tokens that may have one table: a CTA per span of tokens, KV head and 64 blocks.  A warp keeps the
+// bounds of 16 blocks in registers and goes over the query heads of all tokens of the table.
+// Bounds: instructions (some 350 for 16 blocks by 8 columns) at three warps a scheduler.
+__global__ void __launch_bounds__(32 * SEL_WARPS, 3)
+select_scores_many_kernel(const SelectParams p) {
+  __shared__ uint32_t scratch[SEL_WARPS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int kvh = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = blockIdx.x / p.chunks, chunk = blockIdx.x - group * p.chunks;
+  const int per = p.page / p.block;
+  const int r0 = lane >> 2, quad = lane & 3;
+  const int shift = 31 - __clz(p.cols);
+  const int end_token = min(p.num_tokens, (group + 1) * p.span);
+  Extent extent;
+  for (int t0 = group * p.span; t0 < end_token;) {
+    // a run of tokens with one table, 32 looked at together
+    const int row = p.rows[t0];
+    int t1 = t0, longest = 0;
+    for (;;) {
+      const int t = t1 + lane;
+      const bool same = t < end_token && p.rows[t] == row;
+      const uint32_t others = ~__ballot_sync(0xffffffffu, same);
+      const int many = others ? __ffs(others) - 1 : 32;
+      longest = max(longest, __reduce_max_sync(0xffffffffu,
+                                               lane < many ? select_length(p, t, row) : 0));
+      t1 += many;
+      if (many < 32) break;
+    }
+    const int scored = select_scored(p, longest);
+    const int b0 = chunk * p.chunk + warp * 16;
+    const int first = t0;
+    t0 = t1;
+    if (b0 >= scored) continue;
+    const int32_t* table = p.tables + (int64_t)row * p.table_stride;
+    uint4 l0[4], u0[4], l1[4], u1[4];          // blocks b0 + r0 and b0 + 8 + r0
+    bool ok[2];
 #pragma unroll
-    for (int w = 1; w < SEL_WARPS; ++w) most = max(most, most_of[w]);
-    p.largest[((int64_t)group * p.hkv + kvh) * p.chunks + chunk] = __uint_as_float(most);
+    for (int half = 0; half < 2; ++half) {
+      const int at = b0 + half * 8 + r0, b = p.keep_first + at;
+      const int page = at < scored ? table[p.per_shift >= 0 ? b >> p.per_shift : b / per] : -1;
+      ok[half] = page >= 0 && page < p.num_pages;
+      if (!ok[half] && at < scored && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+      const int in = p.per_shift >= 0 ? b & (per - 1) : b % per;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          p.bounds + (ok[half] ? (((int64_t)page * p.hkv + kvh) * per + in) * 2 * SEL_D : 0) +
+          quad * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+        const uint4 l = ok[half] ? src[j * 4] : none, u = ok[half] ? src[16 + j * 4] : none;
+        if (half) { l1[j] = l; u1[j] = u; } else { l0[j] = l; u0[j] = u; }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      extent.add(l0[j], u0[j]);
+      extent.add(l1[j], u1[j]);
+    }
+    // columns: p.cols a token, the last ones of them without a head
+    const int tiles = ((t1 - first) * p.cols + 7) / 8;
+    auto column = [&](int nt, uint4 (&v)[4]) {
+      const int col = nt * 8 + r0, t = first + (col >> shift), head = col & (p.cols - 1);
+      const bool live = t < t1 && head < p.g;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          p.q + (int64_t)(live ? t : first) * p.q_stride +
+          ((int64_t)kvh * p.g + (live ? head : 0)) * SEL_D + quad * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = live ? src[j * 4] : make_uint4(0u, 0u, 0u, 0u);
+    };
+    uint4 next[4];
+    column(0, next);
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, a_max = 0.f;
+    for (int nt = 0; nt < tiles; ++nt) {
+      uint32_t qp[4][4], qm[4][4];
+      split_q(next, qp, qm);
+      float a = chunk == 0 && warp == 0 ? abs_q(next) : 0.f;
+      if (nt + 1 < tiles) column(nt + 1, next);
+      float v[4];
+      score_tile(l0, u0, l1, u1, qp, qm, v);
+      // a token's heads: columns 2 quad + 0, 1, then next lanes, then the next tile
+      const int head = (nt * 8 + quad * 2) & (p.cols - 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = head + (i & 1) < p.g ? v[i] : -INFINITY;
+      if (p.cols > 1) {
+        v[0] = v[1] = max_nan(v[0], v[1]);
+        v[2] = v[3] = max_nan(v[2], v[3]);
+      }
+      for (int o = 1; o < min(p.cols, 8) / 2; o <<= 1) {
+        v[0] = max_nan(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+        v[2] = max_nan(v[2], __shfl_xor_sync(0xffffffffu, v[2], o));
+      }
+      if (p.cols == 16) {
+        const bool more = nt & 1;              // the token's second half
+        v[0] = m[0] = more ? max_nan(m[0], v[0]) : v[0];
+        v[2] = m[2] = more ? max_nan(m[2], v[2]) : v[2];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int col = nt * 8 + quad * 2 + i, t = first + (col >> shift);
+        const int at = col & (p.cols - 1);
+        if (at != (p.cols == 16 ? 8 : 0) || t >= t1) continue;
+        uint32_t* scores = p.scores + ((int64_t)t * p.hkv + kvh) * p.pitch + b0 + r0;
+        if (b0 + r0 < scored) scores[0] = ok[0] ? order_of(v[i]) : 0u;
+        if (b0 + 8 + r0 < scored) scores[8] = ok[1] ? order_of(v[2 + i]) : 0u;
+      }
+      if (chunk == 0 && warp == 0) {
+        // the largest sum of |q| of each token's heads
+        for (int o = 1; o < min(p.cols, 8); o <<= 1)
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o * 4));
+        if (p.cols == 16) a = a_max = nt & 1 ? fmaxf(a_max, a) : a;
+        const int col = nt * 8 + r0, t = first + (col >> shift);
+        if (quad == 0 && (col & (p.cols - 1)) == (p.cols == 16 ? 8 : 0) && t < t1)
+          p.q_sum[(int64_t)t * p.hkv + kvh] = a;
+      }
+    }
   }
+  const uint32_t most = extent.of_cta(scratch);
+  if (threadIdx.x == 0)
+    p.largest[((int64_t)group * p.hkv + kvh) * p.chunks + chunk] = __uint_as_float(most);
 }
 
 // ---- the choice: a team of W warps per token and KV head, a CTA of its own or, of one warp, eight in one
@@ -790,7 +890,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) select_choose_kernel(co
       }
     }
     // largest |bound|; no number counts as infinite
-    const float* from = p.largest + ((int64_t)(token / p.together) * p.hkv + kvh) * p.chunks;
+    const float* from = p.largest + ((int64_t)(token / p.span) * p.hkv + kvh) * p.chunks;
     float largest = 0.f;
     for (int i = lane; i < p.chunks; i += 32)
       largest = fmaxf(largest, from[i] < INFINITY ? from[i] : INFINITY);
@@ -804,25 +904,31 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 32 * W) select_choose_kernel(co
             key_hi, exact, band, teams[team]);
 }
 
-// Groups of tokens that share products, and what is in a workspace.
+// Tokens of a CTA, its blocks, and what is in a workspace.
 struct SelectLayout {
-  int together, chunk, chunks, pitch;
+  int span, chunk, chunks, pitch;
   int64_t groups;
   size_t largest, q_sum, total;       // bytes
 };
-static SelectLayout select_layout(int64_t tokens, int hkv, int g, bool rows, int64_t most) {
+static SelectLayout select_layout(int64_t tokens, int hkv, bool rows, int64_t most) {
   SelectLayout s;
-  // Tokens that may have one table share the scores' products, as far as their query heads fill the
-  // 16 rows.
-  s.together = 1;
-  if (rows && (g & (g - 1)) == 0)
-    while (s.together * 2 * g <= 16) s.together *= 2;
-  s.groups = (tokens + s.together - 1) / s.together;
-  // Long chunks for the pipeline's sake, unless that leaves SMs without work.
+  const int sms = sm_count();
+  s.span = 1;
   s.chunk = 256;
-  while (s.chunk > 64 && s.groups * hkv * ((most + s.chunk - 1) / s.chunk) < 4ll * sm_count())
-    s.chunk /= 2;
-  s.chunks = (int)((most + s.chunk - 1) / s.chunk);
+  if (rows) {
+    // spans as long as leaves two rounds of work for every SM's three CTAs (1000 tokens of two
+    // prompts 66 us; one round 79, eight 73)
+    s.chunk = 64;
+    s.chunks = (int)((most + s.chunk - 1) / s.chunk);
+    s.span = 64;
+    while (s.span > 1 && (tokens + s.span - 1) / s.span * hkv * s.chunks < 6ll * sms) s.span /= 2;
+  } else {
+    // long chunks for the pipeline's sake, unless that leaves SMs without work
+    while (s.chunk > 64 && tokens * hkv * ((most + s.chunk - 1) / s.chunk) < 4ll * sms)
+      s.chunk /= 2;
+    s.chunks = (int)((most + s.chunk - 1) / s.chunk);
+  }
+  s.groups = (tokens + s.span - 1) / s.span;
   s.pitch = (int)((most + 3) & ~3ll);
   s.largest = ((size_t)tokens * hkv * s.pitch * 4 + 255) & ~size_t(255);
   s.q_sum = s.largest + (size_t)s.groups * hkv * s.chunks * 4;
@@ -900,9 +1006,8 @@ size_t fk_select_blocks_workspace_bytes(int num_tokens, int num_q_heads, int num
     return 0;
   // the larger of both ways to group tokens
   const int64_t most = block_table_cols * (page_size / block);
-  const int g = num_q_heads / num_kv_heads;
-  const size_t a = select_layout(num_tokens, num_kv_heads, g, false, most).total;
-  const size_t b = select_layout(num_tokens, num_kv_heads, g, true, most).total;
+  const size_t a = select_layout(num_tokens, num_kv_heads, false, most).total;
+  const size_t b = select_layout(num_tokens, num_kv_heads, true, most).total;
   return a > b ? a : b;
 }
 
@@ -956,7 +1061,7 @@ int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, 
   p.selected = selected;
   p.status = status;
   const SelectLayout w =
-      select_layout(num_tokens, num_kv_heads, p.g, table_rows != nullptr, most);
+      select_layout(num_tokens, num_kv_heads, table_rows != nullptr, most);
   FK_REQUIRE(workspace != nullptr && workspace_bytes >= w.total &&
                  (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
              FK_ERR_WORKSPACE,
@@ -964,20 +1069,23 @@ int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, 
              workspace_bytes);
   FK_REQUIRE(w.groups * w.chunks < (1ll << 31), FK_ERR_UNSUPPORTED,
              "fk_select_blocks: too many tokens");
-  p.together = w.together; p.pitch = w.pitch;
-  p.g_shift = w.together > 1 ? __builtin_ctz(p.g) : 0;
+  p.span = w.span; p.pitch = w.pitch;
+  p.cols = 1;
+  while (p.cols < p.g) p.cols *= 2;
   p.chunk = w.chunk; p.chunks = w.chunks;
   p.scores = static_cast<uint32_t*>(workspace);
   p.largest = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + w.largest);
   p.q_sum = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + w.q_sum);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = p.g * p.together > 8;
-  auto scores = wide ? select_scores_kernel<2> : select_scores_kernel<1>;
+  const bool wide = p.g > 8;
+  auto scores = table_rows ? select_scores_many_kernel
+                           : wide ? select_scores_kernel<2> : select_scores_kernel<1>;
+  const size_t ring = table_rows ? 0 : SEL_RING_BYTES;
   static PerDeviceOnce scores_once[2];
-  FK_CUDA_OK(set_max_dynamic_smem(scores_once[wide], scores, SEL_RING_BYTES));
+  if (ring) FK_CUDA_OK(set_max_dynamic_smem(scores_once[wide], scores, SEL_RING_BYTES));
   FK_CUDA_OK(launch_kernel(scores,
                            dim3((unsigned)(w.groups * w.chunks), (unsigned)num_kv_heads),
-                           dim3(32 * SEL_WARPS), (size_t)SEL_RING_BYTES, s, p));
+                           dim3(32 * SEL_WARPS), ring, s, p));
   const int64_t items = (int64_t)num_tokens * num_kv_heads;
   const int sms = sm_count();
   const int warps = items <= 2ll * sms ? 8 : items < 16ll * sms || most > SEL_WARP_BLOCKS ? 4 : 1;

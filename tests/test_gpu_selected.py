@@ -148,7 +148,8 @@ def test_select_rows_of_a_portion(ops):
     check_select(ops, q, bounds, lens, table, 32, 6, 1, 1, rows)
 
 
-@pytest.mark.parametrize("hq,hkv,n", [(8, 8, 301), (32, 4, 640), (10, 10, 250)])
+@pytest.mark.parametrize("hq,hkv,n", [(8, 8, 301), (32, 4, 640), (10, 10, 250), (16, 8, 300),
+                                      (48, 3, 90), (35, 5, 70), (9, 1, 130), (12, 4, 64)])
 def test_select_many_tokens(ops, hq, hkv, n):
     """As many tokens as let a warp choose for each; groups of tokens that end with a table."""
     rows = [0] * 37 + [1] * (n - 38) + [2]
