@@ -37,7 +37,7 @@ struct RowsParams {
 // ---------------------------------------------------------------------------
 // A lane has the (max, sum) of splits lane, lane + 32, ..., so all of them are one round of loads, and
 // four partial rows are on the way at a time.  A split without keys has a sum of zero; its row was
-// not written and is not read.
+// not written and is not read.  (One whose sum is no number counts.)
 struct JoinRow {
   float4 acc;
   float l;
@@ -56,7 +56,7 @@ __device__ __forceinline__ void join_add(JoinRow& r, const ML& ml, const ROW& ro
                                          int lane) {
   for (int s0 = 0; s0 < n; s0 += 32) {
     const float2 mlv = s0 + lane < n ? ml(s0 + lane) : make_float2(-INFINITY, 0.f);
-    const float fl = mlv.y > 0.f ? fast_exp2(mlv.x - top) : 0.f;
+    const float fl = mlv.y != 0.f ? fast_exp2(mlv.x - top) : 0.f;
     const int cnt = min(32, n - s0);
     for (int s = 0; s < cnt; s += 4) {
       float4 v[4];
@@ -65,7 +65,7 @@ __device__ __forceinline__ void join_add(JoinRow& r, const ML& ml, const ROW& ro
       for (int i = 0; i < 4; ++i) {
         f[i] = __shfl_sync(0xffffffffu, fl, (s + i) & 31);
         l[i] = s + i < cnt ? __shfl_sync(0xffffffffu, mlv.y, (s + i) & 31) : 0.f;
-        v[i] = l[i] > 0.f ? *row(s0 + s + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i] = l[i] != 0.f ? *row(s0 + s + i) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -737,11 +737,20 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
           lim = len >= w.it.keys ? w.it.keys : 0;
         }
       }
+      // 32 rows without one that sees keys (behind the last of an item) have nothing to do: what is
+      // in their columns stays in their rows of the products
+      const bool some = __any_sync(0xffffffffu, lim > 0);
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, kpos += 128) {
         // Two warps have a row between them and meet at a barrier in every step: one whose wait has
         // run out says so there, and both leave.
         ok = ok && px_wait_warp(&s_full[t], (n_sp + (uint32_t)j) & 1u, abort_flag, p.status);
+        if (!some) {
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&p_full[t]);
+          __syncwarp();
+          continue;
+        }
         // (scores of a step whose wait ran out are not used)
         tc_fence_after();
         uint32_t v[64];                        // scores, then weights two a word
@@ -835,11 +844,14 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
       ++n_o;
       if (!ok) continue;
       tc_fence_after();
-      if (m_used == -INFINITY) l = 0.f;        // no key
       float* dst = p.part_o + (int64_t)slot * PX_SLOT_FLOATS + ((t * 4 + quad) * 2 + half) * 2048;
       uint8_t* stage = smem + PX_OFF_Q + t * PX_TILE_BYTES + (half * 4 + quad) * 4096;
+      if (!some) {
+        tc_fence_before();
+        if (lane == 0) mbar_arrive(&o_empty[t]);
+      }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 2 && some; ++c) {
         uint32_t o[32];
         tc_ld32(o_addr + c * 32, o);
         tc_wait_ld();

@@ -309,6 +309,19 @@ def test_selected_bad_pages_are_left_out(ops):
     close(got, *attend_oracle(q, kc, vc, lens, table, sel, 64, 64, "NHD", 2, None))
 
 
+def test_selected_keys_that_are_no_numbers_are_seen(ops):
+    lens = [2000, 640]
+    q, kc, vc, table, sel = attend_case(17, lens, 4, 2, 64, 64, "NHD", 20)
+    good = host_f32(ops.selected_attn(dev(q), dev(kc), dev(vc), ints(lens), ints(table), ints(sel), 64,
+                                      S.SCALE))
+    b = int(sel[0, 1, 5])
+    kc[table[0, b], 9, 1] = np.nan
+    got = host_f32(ops.selected_attn(dev(q), dev(kc), dev(vc), ints(lens), ints(table), ints(sel), 64,
+                                     S.SCALE))
+    assert np.isnan(got[0, 2:]).all() and (got[0, :2] == good[0, :2]).all()
+    assert (got[1] == good[1]).all()
+
+
 def test_selected_large_scores(ops):
     """Scores of some hundreds: the largest key of a row alone counts, whichever block holds it."""
     q, kc, vc, table, sel = attend_case(8, [1000, 777], 8, 2, 64, 64, "NHD", 8)

@@ -151,6 +151,38 @@ def test_what_a_short_row_does_not_see(ops, short, bad, wide):
     assert (got[4] == 0).all()
     assert not np.isfinite(got[:2, 4:8]).any()            # the heads of the value's KV head
     assert np.isfinite(got[:, :4]).all() and np.isfinite(got[:, 12:]).all()
+    if np.isnan(bad):                                     # a key's: every score of its KV head's rows
+        assert np.isnan(got[:2, 8:12]).all()
+
+
+@pytest.mark.parametrize("wide", [True, False])
+def test_what_is_no_number_is_seen(ops, wide):
+    """Keys, values and queries that are no numbers, in the common part and in a row's own: the rows that see
+    them have no numbers, the others what they had."""
+    case = build(35, [(640, [50, 600, 0]), (64, [700, 3])], 64, "NHD", 8, 4, wide=wide)
+    q, kc, vc, lens, table, starts, prefix = case
+    good = host_f32(run(ops, case, "NHD"))
+
+    def changed(**kw):
+        a, b, c = (x.copy() for x in (q, kc, vc))
+        if "key" in kw:
+            row, pos, head = kw["key"]
+            b[table[row, pos // 64], pos % 64, head] = np.nan
+        if "value" in kw:
+            row, pos, head = kw["value"]
+            c[table[row, pos // 64], pos % 64, head, 7] = np.nan
+        if "query" in kw:
+            a[kw["query"]] = np.nan
+        got = host_f32(run(ops, (a, b, c, lens, table, starts, prefix), "NHD"))
+        return got, got != good
+    got, other = changed(key=(0, 300, 1))
+    assert np.isnan(got[:3, 2:4]).all() and not other[:, :2].any() and not other[3:].any()
+    got, other = changed(key=(1, 700, 2))
+    assert np.isnan(got[1, 4:6]).all() and other.sum() == 2 * 128
+    got, other = changed(value=(2, 10, 3))
+    assert np.isnan(got[:3, 6:, 7]).all() and other.sum() == 3 * 2
+    got, other = changed(query=2)                         # a row that the common part alone answers
+    assert np.isnan(got[2]).all() and not other[[0, 1, 3, 4]].any()
 
 
 def test_pages_far_behind(ops):
