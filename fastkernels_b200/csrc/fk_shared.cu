@@ -625,6 +625,15 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
         }
       }
     }
+    if (!ok && lane == 0) {
+      // given up: copies under way must land before the CTA's memory is another's
+      if (segs > 0) (void)mbar_wait(q_full, (uint32_t)(segs - 1) & 1u, 1u << 20);
+      for (int s = 0; s < PX_SLOTS && s < kv_idx; ++s) {
+        const int uses_s = (kv_idx - 1 - s) / PX_SLOTS;      // of slot s before its last one
+        (void)mbar_wait(&slot_full[s], (uint32_t)uses_s & 1u, 1u << 20);
+      }
+    }
+    __syncwarp();
   } else if (warp == PX_WARP_MMA) {
     constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) |
                                  ((uint32_t)(128 >> 4) << 24);

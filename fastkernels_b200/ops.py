@@ -295,9 +295,28 @@ _INT32, _UINT8 = torch.int32, torch.uint8
 def _device_of(t) -> int:
     """The current device, which the first tensor of a call has to be on."""
     dev = t.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
-        _refuse("the first tensor", t, t.dtype, dev if dev < 0 else torch.cuda.current_device())
+    if dev < 0 or dev != _current_device():
+        _refuse("the first tensor", t, t.dtype, dev if dev < 0 else _current_device())
     return dev
+
+
+# the current device once CUDA is up, which a CUDA tensor shows
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_STATUS_OF: dict = {}
+
+
+def _status_of(dev, status, like) -> int:
+    """Address of the status word: of the given one, or the device's own."""
+    if status is not None:
+        return status.data_ptr()
+    ptr = _STATUS_OF.get(dev)
+    if ptr is None:
+        ptr = _STATUS_OF[dev] = default_status(like.device).data_ptr()
+    return ptr
+
+
+def _stream_of(dev) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else _stream()
 
 
 def _refuse(name, t, dtype, dev):
@@ -320,6 +339,8 @@ def _need_tables(dev, t) -> tuple[int, int, int]:
     if t.dim() != 2:
         raise _lib.FkError("block_tables must be [rows, pages]")
     rows, cols = t.shape
+    if t.is_contiguous():
+        return cols, cols, rows
     stride, step = t.stride()
     if step != 1 and cols > 1 and rows:
         raise _lib.FkError("block_tables must have dense rows")
@@ -347,10 +368,21 @@ def _need_cache(dev, cache, kv_layout, name) -> tuple[int, int, int, int, int]:
 
 
 def _need_caches(dev, k_cache, v_cache, kv_layout) -> tuple[int, int, int, int, int]:
-    got = _need_cache(dev, k_cache, kv_layout, "k_cache")
     if v_cache.dtype is not BF16 or v_cache.get_device() != dev:
         _refuse("v_cache", v_cache, BF16, dev)
-    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
+    shape = k_cache.shape
+    if v_cache.shape != shape:
+        raise _lib.FkError("cache shape mismatch")
+    if k_cache.is_contiguous() and v_cache.is_contiguous() and len(shape) == 4 and \
+            k_cache.dtype is BF16 and k_cache.get_device() == dev:
+        if kv_layout == "NHD":
+            pages, page, hkv, d = shape
+            return pages, page, hkv, d, page * hkv * d
+        if kv_layout == "HND":
+            pages, hkv, page, d = shape
+            return pages, page, hkv, d, page * hkv * d
+    got = _need_cache(dev, k_cache, kv_layout, "k_cache")
+    if v_cache.stride() != k_cache.stride():
         raise _lib.FkError("cache shape mismatch")
     return got
 
@@ -362,6 +394,8 @@ def _need_rows(dev, t, name) -> tuple[int, int, int, int]:
     if t.dim() != 3:
         raise _lib.FkError(f"{name} must be [tokens, heads, D]")
     n, heads, d = t.shape
+    if t.is_contiguous():
+        return n, heads, d, heads * d
     stride, head, one = t.stride()
     if n and (one != 1 and d > 1 or head != d and heads > 1):
         raise _lib.FkError(f"{name} heads must be dense")
@@ -372,6 +406,8 @@ def _out_like(dev, q, out):
     """(out, its token stride): a new one for None."""
     if out is None:
         n, heads, d = q.shape
+        if q.is_contiguous():
+            return torch.empty_like(q), heads * d
         return q.new_empty((n, heads, d)), heads * d
     if out.shape != q.shape:
         raise _lib.FkError("out must have the shape of q")
@@ -390,6 +426,7 @@ def _workspace(dev, workspace, need: int, like) -> tuple[int | None, int, object
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
+@functools.lru_cache(maxsize=4096)
 def shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, head_dim,
                                   max_splits) -> int:
     return int(lib.fk_shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads,
@@ -413,7 +450,7 @@ def shared_prefix_plan(context_lens, block_tables, page_size, num_q_heads, num_k
     check(lib.fk_shared_prefix_plan(
         context_lens.data_ptr(), page_size, cols, group_starts.data_ptr(), prefix_lens.data_ptr(),
         groups, b, num_q_heads, num_kv_heads, head_dim, max_splits, ws, ws_bytes,
-        _status_ptr(status, context_lens), _stream()), "fk_shared_prefix_plan")
+        _status_of(dev, status, context_lens), _stream_of(dev)), "fk_shared_prefix_plan")
 
 
 def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_starts, prefix_lens,
@@ -447,13 +484,13 @@ def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_st
         max_splits = max_splits_for(cols * page)
     ws, ws_bytes, _held = _workspace(
         dev, workspace,
-        lib.fk_shared_prefix_workspace_bytes(b, groups, hq, hkv, d, max_splits)
+        shared_prefix_workspace_bytes(b, groups, hq, hkv, d, max_splits)
         if workspace is None else 0, q)
     check(lib.fk_shared_prefix_attn(
         1 if planned else 0, q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
         stride, 1 if kv_layout == "HND" else 0, context_lens.data_ptr(), block_tables.data_ptr(),
         ts, cols, group_starts.data_ptr(), prefix_lens.data_ptr(), groups, b, hq, hkv, d,
-        softmax_scale, max_splits, ws, ws_bytes, _status_ptr(status, q), _stream()),
+        softmax_scale, max_splits, ws, ws_bytes, _status_of(dev, status, q), _stream_of(dev)),
         "fk_shared_prefix_attn")
     return out
 
@@ -497,10 +534,11 @@ def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new
     check(lib.fk_key_bounds(
         k_cache.data_ptr(), pages, page, stride, 1 if kv_layout == "HND" else 0, hkv, d,
         bounds.data_ptr(), page // per, context_lens.data_ptr(), block_tables.data_ptr(), ts, cols,
-        _ptr(cu_new), n, max_new, _status_ptr(status, k_cache), _stream()), "fk_key_bounds")
+        _ptr(cu_new), n, max_new, _status_of(dev, status, k_cache), _stream_of(dev)), "fk_key_bounds")
     return bounds
 
 
+@functools.lru_cache(maxsize=4096)
 def select_blocks_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, page_size, block,
                                   table_cols) -> int:
     return int(lib.fk_select_blocks_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, page_size,
@@ -537,16 +575,17 @@ def select_blocks(q, bounds, context_lens, block_tables, block, count, keep_firs
             raise _lib.FkError("out must be a contiguous [tokens, Hkv, count]")
     ws, ws_bytes, _held = _workspace(
         dev, workspace,
-        lib.fk_select_blocks_workspace_bytes(n, hq, hkv, per * block, block, cols)
+        select_blocks_workspace_bytes(n, hq, hkv, per * block, block, cols)
         if workspace is None else 0, q)
     check(lib.fk_select_blocks(
         q.data_ptr(), qs, bounds.data_ptr(), pages, per * block, block, context_lens.data_ptr(),
         _ptr(table_rows), block_tables.data_ptr(), ts, cols, rows, n, hq, hkv, d, count,
-        keep_first, keep_last, out.data_ptr(), ws, ws_bytes, _status_ptr(status, q), _stream()),
+        keep_first, keep_last, out.data_ptr(), ws, ws_bytes, _status_of(dev, status, q), _stream_of(dev)),
         "fk_select_blocks")
     return out
 
 
+@functools.lru_cache(maxsize=4096)
 def selected_attn_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, head_dim, count,
                                   block) -> int:
     return int(lib.fk_selected_attn_workspace_bytes(num_tokens, num_q_heads, num_kv_heads,
@@ -576,13 +615,13 @@ def selected_attn(q, k_cache, v_cache, context_lens, block_tables, selected, blo
     count = selected.shape[2]
     out, os_ = _out_like(dev, q, out)
     ws, ws_bytes, _held = _workspace(
-        dev, workspace, lib.fk_selected_attn_workspace_bytes(n, hq, hkv, d, count, block)
+        dev, workspace, selected_attn_workspace_bytes(n, hq, hkv, d, count, block)
         if workspace is None else 0, q)
     check(lib.fk_selected_attn(
         q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
         stride, 1 if kv_layout == "HND" else 0, context_lens.data_ptr(), _ptr(table_rows),
         block_tables.data_ptr(), ts, cols, rows, selected.data_ptr(), count, block, n, hq, hkv, d,
-        softmax_scale, ws, ws_bytes, _status_ptr(status, q), _stream()), "fk_selected_attn")
+        softmax_scale, ws, ws_bytes, _status_of(dev, status, q), _stream_of(dev)), "fk_selected_attn")
     return out
 
 
