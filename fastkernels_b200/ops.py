@@ -517,7 +517,8 @@ def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new
     tokens of each sequence: the last one, or with cu_new (int32 [sequences + 1], as
     cu_seqlens) the last cu_new[s + 1] - cu_new[s], at most max_new.  Call it after those tokens' keys
     have been stored; context_lens count them.  A block that is not full yet has the bounds of the
-    keys in it.  A sequence (and so a page with new tokens) appears once in the batch."""
+    keys in it.  A sequence (and so a page with new tokens) appears once in the batch: of
+    sequences that share a page only the longest may have new tokens in it."""
     dev = _device_of(k_cache)
     pages, page, hkv, d, stride = _need_cache(dev, k_cache, kv_layout, "k_cache")
     _need_bounds(dev, bounds)

@@ -209,7 +209,8 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  * cu_new[s + 1] - cu_new[s] tokens of sequence s (cu_new NULL: one token each),
  * at most max_new each.  context_lens count the new tokens, whose keys are in the
  * cache already.  Bounds of other blocks stay as they are.  A sequence appears
- * once.  No-number keys give no-number bounds.
+ * once, and of sequences that share a page only the longest may have new tokens in it.
+ * No-number keys give no-number bounds.
  *
  * fk_select_blocks: for query token i and KV head, of the n = ceil(context_lens[i]
  * / block) blocks that it sees, in ascending order: the first keep_first, the last
