@@ -435,7 +435,8 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
       att_produce_selected(tmap_k, tmap_v, p, stages, qslots, metas, full, empty, abort_flag, lane);
       return;
     }
-    const int total_items = p.direct ? p.batch * p.hkv : __ldcg(plan) * p.hkv;
+    int total_items = p.direct ? p.batch * p.hkv : __ldcg(plan) * p.hkv;
+    if (p.sign != 0 && __ldcg(plan + ATT_PLAN_HDR - 1) != p.sign) total_items = 0;
     int* counter = const_cast<int*>(plan) + 2;
     // direct mode: the schedule entry of item (sequence, KV head) is the whole
     // sequence as one unsplit chunk; lengths are clamped as the plan kernel does

@@ -21,6 +21,7 @@ struct AttnParams {
   int direct;         // 1: no plan, no splits: CTA b handles (sequence, KV head) item b whole
   int beside;         // 1: runs beside the kernel before it, which has seen the plan's kernel end
   int* plan;          // header + chunk_start[batch+1]
+  int sign;           // the plan's last header word if it is of these sizes (0: not compared)
   int4* chunk_info;   // per chunk: {seq, split | nsplits << 16, tok_begin, tok_end}
   float* part_o;      // [batch, hq, max_splits, D]
   float2* part_ml;    // [batch, hq, max_splits]

@@ -133,7 +133,7 @@ struct PrefixItem {
 };
 
 enum : int { PLAN_CHUNKS = 0, PLAN_COUNTER = 2, PLAN_ITEMS = 4, PLAN_TILES = 5, PLAN_UNIT = 6,
-             PLAN_HDR = 8 };
+             PLAN_SIGN = 7, PLAN_HDR = 8 };
 
 struct SharedPlan {
   int* hdr;            // see above; chunk_start[batch + 1] behind it, as the decode kernel has it
@@ -147,6 +147,7 @@ struct SharedPlan {
 struct SharedPlanParams {
   const int32_t* lens; const int32_t* starts; const int32_t* prefix;
   int batch, groups, hkv, page, per_tile, max_splits, ctas, min_unit;
+  int sign;            // of the sizes, by which a planned call knows a schedule that is not for it
   int beside;          // the decode kernel may run beside the common part's
   int64_t capacity;
   SharedPlan plan;
@@ -356,6 +357,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) shared_plan_kernel(const SharedP
     p.plan.hdr[PLAN_ITEMS] = items;
     p.plan.hdr[PLAN_TILES] = tiles;
     p.plan.hdr[PLAN_UNIT] = unit;
+    p.plan.hdr[PLAN_SIGN] = p.sign;
   }
 }
 
@@ -404,6 +406,7 @@ static_assert(PX_SMEM_ALLOC <= 232448, "shared memory budget");
 static_assert(tmem_alone(PX_SMEM_ALLOC), "two CTAs could wait for one another's tensor memory");
 
 struct PrefixParams {
+  int sign;
   const int* hdr; const int* cta_item; const PrefixItem* items;
   const int32_t* lens;
   const int32_t* tables; int64_t table_stride;
@@ -560,7 +563,7 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
   // The decode kernel starts from here on, on the SMs that have no tiles of the common part, and
   // reads what the kernels before this one have written.
   pdl_launch_dependents();
-  const int unit = p.hdr[PLAN_UNIT], total = p.hdr[PLAN_TILES];
+  const int unit = p.hdr[PLAN_UNIT], total = p.hdr[PLAN_SIGN] == p.sign ? p.hdr[PLAN_TILES] : 0;
   const int64_t from = (int64_t)blockIdx.x * unit;
   const int begin = (int)(from < total ? from : total);
   const int end = tmem_got != 0 ? begin : min(total - begin, unit) + begin;
@@ -916,6 +919,8 @@ struct SharedJoinParams {
   const float* pre_o; const float2* pre_ml;
   const float* own_o; const float2* own_ml; int own_splits;
   int batch, hq, hkv, g, per_tile;
+  int sign;
+  int32_t* status;
 };
 __global__ void __launch_bounds__(256) shared_join_kernel(const SharedJoinParams p) {
   pdl_launch_dependents();
@@ -927,9 +932,13 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const SharedJoinParams
   if (gw >= (int64_t)p.batch * p.hq) return;
   const int row = (int)(gw / p.hq), head = (int)(gw - (int64_t)row * p.hq);
   const int* chunk_start = p.hdr + PLAN_HDR;
-  const int n_own = chunk_start[row + 1] - chunk_start[row];
-  const int4 in = p.row_part[row];
+  int n_own = chunk_start[row + 1] - chunk_start[row];
+  int4 in = p.row_part[row];
   const int unit = p.hdr[PLAN_UNIT];
+  if (p.hdr[PLAN_SIGN] != p.sign) {            // no schedule of these sizes: nothing was computed
+    n_own = in.y = 0;
+    if (gw == 0 && lane == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_POSITION);
+  }
   int n_pre = 0;
   int64_t slot = 0;                            // of the first split
   int at = 0;                                  // row among the two tiles of a split
@@ -1230,6 +1239,12 @@ static int shared_impl(int mode, const void* q, int64_t q_stride_token, void* ou
   pl.batch = batch; pl.groups = num_groups; pl.hkv = num_kv_heads; pl.page = page_size;
   pl.per_tile = per_tile; pl.max_splits = max_splits; pl.ctas = sms;
   pl.min_unit = PREFIX_MIN_UNIT;
+  uint32_t sign = 2166136261u;
+  for (const int64_t v : {(int64_t)batch, (int64_t)num_groups, (int64_t)num_q_heads,
+                          (int64_t)num_kv_heads, (int64_t)page_size, r.capacity,
+                          (int64_t)max_splits, (int64_t)sms})
+    sign = (sign ^ (uint32_t)v ^ (uint32_t)(v >> 32) * 31u) * 16777619u;
+  pl.sign = (int)(sign | 1u);
   pl.beside = pdl_enabled();
   pl.capacity = r.capacity;
   pl.plan.hdr = reinterpret_cast<int*>(ws);
@@ -1269,6 +1284,7 @@ static int shared_impl(int mode, const void* q, int64_t q_stride_token, void* ou
   if (rc != FK_OK) return rc;
 
   PrefixParams px{};
+  px.sign = pl.sign;
   px.hdr = pl.plan.hdr; px.cta_item = pl.plan.cta_item; px.items = pl.plan.items;
   px.lens = context_lens;
   px.tables = block_tables; px.table_stride = block_table_stride;
@@ -1293,14 +1309,14 @@ static int shared_impl(int mode, const void* q, int64_t q_stride_token, void* ou
   a.bs_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   a.scale_log2 = r.scale_log2;
   a.max_splits = max_splits;
-  a.plan = pl.plan.hdr;
+  a.plan = pl.plan.hdr; a.sign = pl.sign;
   a.chunk_info = pl.plan.chunks;
   a.part_o = reinterpret_cast<float*>(ws + w.own_o);
   a.part_ml = reinterpret_cast<float2*>(ws + w.own_ml);
   a.status = status;
 
   if (direct) {
-    a.direct = 1;
+    a.direct = 1; a.sign = 0;
     a.capacity = r.capacity;
     a.starts = group_starts; a.groups = num_groups;
     FK_CUDA_OK(launch_decode(g > 8, false, false, batch * num_kv_heads, dk, dv, a, s));
@@ -1309,7 +1325,7 @@ static int shared_impl(int mode, const void* q, int64_t q_stride_token, void* ou
   }
 
   SharedJoinParams jn{};
-  jn.hdr = pl.plan.hdr; jn.row_part = pl.plan.row_part;
+  jn.hdr = pl.plan.hdr; jn.row_part = pl.plan.row_part; jn.sign = pl.sign; jn.status = status;
   jn.counter = pl.plan.hdr + PLAN_COUNTER;
   jn.out = r.out; jn.out_stride = r.out_stride;
   jn.pre_o = px.part_o; jn.pre_ml = px.part_ml;

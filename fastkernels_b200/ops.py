@@ -464,7 +464,8 @@ def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_st
     groups have nothing in common.  context_lens count all tokens of a row, the common ones too.
     GQA ratios up to 16.  A workspace of shared_prefix_workspace_bytes holds the schedule and
     partial results of one call at a time; without one it is allocated here.  planned: by the
-    schedule that shared_prefix_plan has left there."""
+    schedule that shared_prefix_plan has left there; without one of these sizes the result is zeros
+    and status has DEV_BAD_POSITION."""
     dev = _device_of(q)
     pages, page, hkv, d2, stride = _need_caches(dev, k_cache, v_cache, kv_layout)
     b, hq, d, qs = _need_rows(dev, q, "q")

@@ -339,6 +339,38 @@ def test_planned_layers(ops, rows):
             assert torch.equal(a, b_)
 
 
+def test_planned_without_its_schedule(ops):
+    """A workspace without a schedule, or with that of a step of other sizes: zeros and a flag."""
+    case = build(12, [(640, [40 + i for i in range(20)]), (320, [100, 900])], 64, "NHD", 16, 8)
+    q, kc, vc, lens, table, starts, prefix = case
+    n = ops.shared_prefix_workspace_bytes(len(lens), 2, 16, 8, 128, 16)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    args, groups = [ints(lens), ints(table)], [ints(starts), ints(prefix)]
+    x = [dev(q), dev(kc), dev(vc)]
+
+    def planned():
+        status = ops.new_status("cuda")
+        out = torch.full_like(x[0], 7.0)
+        ops.shared_prefix_attn(*x, *args, *groups, S.SCALE, workspace=ws, out=out, status=status,
+                               planned=True, max_splits=16)
+        return out, int(status.item())
+    want = ops.shared_prefix_attn(*x, *args, *groups, S.SCALE, max_splits=16)
+    out, status = planned()
+    assert status == 8 and not out.any()
+    # the schedule of fewer rows, of longer tables, of other splits
+    ops.shared_prefix_plan(args[0][:20], args[1][:20], 64, 16, 8, 128, ints([0, 20]), ints([640]),
+                           ws, 16)
+    assert planned()[1] == 8
+    wide = torch.cat([args[1], torch.full_like(args[1], -1)], dim=1)
+    ops.shared_prefix_plan(args[0], wide, 64, 16, 8, 128, *groups, ws, 16)
+    assert planned()[1] == 8
+    ops.shared_prefix_plan(*args, 64, 16, 8, 128, *groups, ws, 8)
+    assert planned()[1] == 8
+    ops.shared_prefix_plan(*args, 64, 16, 8, 128, *groups, ws, 16)
+    out, status = planned()
+    assert status == 0 and torch.equal(out, want)
+
+
 def test_calls_on_two_streams(ops):
     """Two calls at once, each with a workspace of its own."""
     cases = [build(20 + i, [(2048, [70 + 5 * i] * 12), (640, [300, 9])], 64, "NHD", 16, 4)
