@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
       return;
     }
     int total_items = p.direct ? p.batch * p.hkv : __ldcg(plan) * p.hkv;
-    if (p.sign != 0 && __ldcg(plan + ATT_PLAN_HDR - 1) != p.sign) total_items = 0;
+    // no schedule of these sizes: the counter is any word too, and none of its values is an item
+    if (p.sign != 0 && __ldcg(plan + ATT_PLAN_HDR - 1) != p.sign) total_items = (int)0x80000000;
     int* counter = const_cast<int*>(plan) + 2;
     // direct mode: the schedule entry of item (sequence, KV head) is the whole
     // sequence as one unsplit chunk; lengths are clamped as the plan kernel does

@@ -563,7 +563,9 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
   // The decode kernel starts from here on, on the SMs that have no tiles of the common part, and
   // reads what the kernels before this one have written.
   pdl_launch_dependents();
-  const int unit = p.hdr[PLAN_UNIT], total = p.hdr[PLAN_SIGN] == p.sign ? p.hdr[PLAN_TILES] : 0;
+  // A workspace without a schedule of these sizes holds any words: none of them is used.
+  const bool known = p.hdr[PLAN_SIGN] == p.sign;
+  const int unit = known ? p.hdr[PLAN_UNIT] : 1, total = known ? p.hdr[PLAN_TILES] : 0;
   const int64_t from = (int64_t)blockIdx.x * unit;
   const int begin = (int)(from < total ? from : total);
   const int end = tmem_got != 0 ? begin : min(total - begin, unit) + begin;

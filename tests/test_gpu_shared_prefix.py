@@ -371,6 +371,43 @@ def test_planned_without_its_schedule(ops):
     assert status == 0 and torch.equal(out, want)
 
 
+@pytest.mark.parametrize("word", [-1, -2 ** 31, 2 ** 31 - 1, 3, "normal", "-0.5", "-0.01", "-1.5", "-3.0"])
+def test_planned_on_any_words(ops, word):
+    """Whatever a workspace holds instead of a schedule of these sizes, and behind the schedule of others:
+    zeros and a flag, and nothing but the counter is written."""
+    case = build(12, [(640, [40 + i for i in range(20)]), (320, [100, 900])], 64, "NHD", 16, 8)
+    q, kc, vc, lens, table, starts, prefix = case
+    n = ops.shared_prefix_workspace_bytes(len(lens), 2, 16, 8, 128, 16)
+    args, groups = [ints(lens), ints(table)], [ints(starts), ints(prefix)]
+    x = [dev(q), dev(kc), dev(vc)]
+    words = torch.empty(n // 4, dtype=torch.int32, device="cuda")
+    if isinstance(word, int):
+        words.fill_(word)
+    elif word == "normal":
+        torch.manual_seed(5)
+        words.copy_(torch.randn(n // 4, device="cuda").view(torch.int32))
+    else:
+        words.copy_(torch.full((n // 4,), float(word), device="cuda").view(torch.int32))
+    ws = words.view(torch.uint8)
+
+    def planned():
+        status = ops.new_status("cuda")
+        out = torch.full_like(x[0], 7.0)
+        before = words.clone()
+        ops.shared_prefix_attn(*x, *args, *groups, S.SCALE, workspace=ws, out=out, status=status,
+                               planned=True, max_splits=16)
+        assert int(status.item()) == 8 and not out.any()
+        changed = (words != before).nonzero().flatten().tolist()
+        assert changed in ([], [2])
+    planned()
+    wide = torch.cat([args[1], torch.full_like(args[1], -1)], dim=1)
+    for other in ((args[0][:20], args[1][:20], 64, 16, 8, 128, ints([0, 20]), ints([640]), ws, 16),
+                  (args[0], wide, 64, 16, 8, 128, *groups, ws, 16),
+                  (*args, 64, 16, 8, 128, *groups, ws, 8)):
+        ops.shared_prefix_plan(*other)
+        planned()
+
+
 def test_calls_on_two_streams(ops):
     """Two calls at once, each with a workspace of its own."""
     cases = [build(20 + i, [(2048, [70 + 5 * i] * 12), (640, [300, 9])], 64, "NHD", 16, 4)
