@@ -398,7 +398,8 @@ constexpr int PX_OFF_Q = 0;
 constexpr int PX_OFF_KV = 2 * PX_TILE_BYTES;
 constexpr int PX_OFF_BAR = PX_OFF_KV + PX_SLOTS * PX_TILE_BYTES;
 constexpr int PX_OFF_MAX = PX_OFF_BAR + 256;
-constexpr int PX_SMEM_ALLOC = PX_OFF_MAX + 2 * 2 * 128 * 2 + 1024;
+constexpr int PX_SMEM_BASE = 256;                 // alignment of what a launch gets, by its declaration
+constexpr int PX_SMEM_ALLOC = PX_OFF_MAX + 2 * 2 * 128 * 4 + 1024 - PX_SMEM_BASE;
 constexpr int PX_TMEM_COLS = 512;
 constexpr float PX_RESCALE_LOG2 = 8.0f;
 constexpr int PX_SLOT_FLOATS = 2 * 128 * SH_D;   // partial rows of a split
@@ -514,7 +515,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
 prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
                    const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, const PrefixParams p) {
-  extern __shared__ uint8_t px_smem_raw[];
+  extern __shared__ __align__(PX_SMEM_BASE) uint8_t px_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(px_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + PX_OFF_BAR);
@@ -730,10 +731,10 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
     const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
     const uint32_t s_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + t * 128 + half * 64;
     const uint32_t o_addr = s_addr + 256;
-    // maxima of the two threads of a row, as bf16 rounded up: the reference value of a row's
-    // exponentials has to be the same for both, not the maximum itself
-    const uint32_t max_at = smem_u32(smem + PX_OFF_MAX) + t * 512 + (quad * 32 + lane) * 2;
-    constexpr uint32_t kGone = 0x7fffu;        // no number: this warp's wait has run out
+    // maxima of the two threads of a row.  In fp32: a reference value that is off by a part of the
+    // maximum, as a rounded one is, puts all exponentials of scores past some 10^5 below fp32's range.
+    const uint32_t max_at = smem_u32(smem + PX_OFF_MAX) + t * 1024 + (quad * 32 + lane) * 4;
+    constexpr uint32_t kGone = 0x7fffffffu;    // no number: this warp's wait has run out
     uint32_t n_sp = 0, n_o = 0;
     bool ok = true;
     for (;;) {
@@ -809,16 +810,15 @@ prefix_attn_kernel(const __grid_constant__ CUtensorMap tmap_q,
           }
           if (pass) break;
           {
-            const uint32_t a = ok ? __bfloat16_as_ushort(__float2bfloat16_ru(fmaxf(mx, m2))) : kGone;
+            // (a maximum is a number: it begins at -infinity, and no-number scores are passed over)
+            const uint32_t a = ok ? __float_as_uint(fmaxf(mx, m2)) : kGone;
             uint32_t b;
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(max_at + half * 256), "h"((uint16_t)a)
-                         : "memory");
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(max_at + half * 512), "r"(a) : "memory");
             named_bar_sync(1 + t * 4 + quad, 64);
-            asm volatile(
-                "{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
-                : "=r"(b) : "r"(max_at + (half ^ 1) * 256) : "memory");
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(b) : "r"(max_at + (half ^ 1) * 512)
+                         : "memory");
             ok = a != kGone && b != kGone;     // the same for both warps: one flag for all lanes
-            mx = fmaxf(bf16_bits_to_float(a), bf16_bits_to_float(b)) * p.scale_log2;
+            mx = fmaxf(__uint_as_float(a), __uint_as_float(b)) * p.scale_log2;
           }
           if (!ok) break;
           const bool grow = mx > m_used + PX_RESCALE_LOG2;

@@ -240,6 +240,36 @@ def test_large_scores(ops):
     assert (d <= S.tolerance(out, mass) + 2 * 2.0 ** -8 * mass).all()
 
 
+@pytest.mark.parametrize("own", [0, 1, 300])
+@pytest.mark.parametrize("rise", [0, 1, 16])
+def test_scores_of_many_thousands(ops, own, rise):
+    """Logits of 10^4 to 10^5, of either sign, that differ by some units from key to key, and with
+    `rise` by tens or hundreds more from one run of 100 keys to the next.  Queries and keys are
+    whole numbers, so that scores are exact in fp32."""
+    rng = np.random.default_rng(50 + own)
+    case = build(13, [(1024, [own] * 20), (2048, [own, own + 60])], 64, "NHD", 8, 2)
+    q, kc, vc, lens, table, starts, prefix = case
+    q[:] = rng.integers(-3, 4, q.shape)
+    q[..., :64] = rng.integers(7, 70, (*q.shape[:2], 1)) * rng.choice([-1, 1], (*q.shape[:2], 1))
+    kc[:] = np.where(np.isnan(kc), kc, rng.integers(-3, 4, kc.shape))
+    kc[..., :63] = np.where(np.isnan(kc[..., :63]), np.nan, 255.0)
+    kc[..., 63] = 0.0
+    for i, n in enumerate(lens):
+        pos = np.arange(n)
+        kc[table[i, pos // 64], pos % 64, :, 63] = (pos // 100 * rise % 256)[:, None]
+    assert np.array_equal(S.bf16(q), q) and np.array_equal(S.bf16(kc), kc, equal_nan=True)
+    case = (q, kc, vc, lens, table, starts, prefix)
+    st = ops.new_status("cuda")
+    got = run(ops, case, "NHD", st)
+    out, mass = S.over_positions(q, kc, vc, lens, table, 64, "NHD", 2, lambda i, h: range(lens[i]))
+    # an exponent s log2(e) below 2^18 is off by half a step, 2^-7, where it is rounded before the
+    # maximum is taken off: a weight by a factor 2^(2^-7) < 1 + 2^-7 / ln(4), the result by twice that
+    d = np.abs(host_f32(got).astype(np.float64) - out)
+    over = d - S.tolerance(out, mass) - 2.0 ** -6 * mass
+    assert (over <= 0).all(), ((over > 0).any(-1).mean(), over.max())
+    assert int(st.item()) == 0
+
+
 def test_strided_rows_and_neighbours_of_the_result(ops):
     case = build(5, [(256, [5, 9, 70])], 64, "NHD", 8, 2)
     packed = torch.zeros((3, 12 * 128), dtype=torch.bfloat16, device="cuda")
