@@ -26,6 +26,7 @@ struct BoundsParams {
   const int32_t* cu_new;              // null: one new token each
   int64_t capacity;                   // tokens that a table's row has pages for
   int num_pages, page, block, hkv, hnd;
+  int max_new;                        // new tokens that the grid has CTAs for
   int32_t* status;
 };
 
@@ -53,7 +54,11 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
     len = p.capacity;
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
   }
-  const int64_t fresh = p.cu_new ? (int64_t)p.cu_new[seq + 1] - p.cu_new[seq] : 1;
+  int64_t fresh = p.cu_new ? (int64_t)p.cu_new[seq + 1] - p.cu_new[seq] : 1;
+  if (fresh > p.max_new) {                   // the newest ones then
+    fresh = p.max_new;
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, FK_DEV_BAD_POSITION);
+  }
   if (len <= 0 || fresh <= 0) return;
   const int64_t first = (len > fresh ? len - fresh : 0) / p.block + blockIdx.x;
   if (first * p.block >= len) return;
@@ -988,6 +993,7 @@ int fk_key_bounds(const void* k_cache, int64_t num_pages, int page_size, int64_t
   p.capacity = block_table_cols * page_size;
   p.num_pages = (int)num_pages; p.page = page_size; p.block = block; p.hkv = num_kv_heads;
   p.hnd = kv_layout;
+  p.max_new = max_new;
   p.status = status;
   // a run of max_new tokens touches at most this many blocks
   const int64_t blocks = ((int64_t)max_new - 1 + block - 1) / block + 1;

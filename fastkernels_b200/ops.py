@@ -516,8 +516,8 @@ def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new
                kv_layout="NHD", status=None):
     """Smallest and largest key per channel, in place and exact, of the blocks that hold the newest
     tokens of each sequence: the last one, or with cu_new (int32 [sequences + 1], as
-    cu_seqlens) the last cu_new[s + 1] - cu_new[s], at most max_new.  Call it after those tokens' keys
-    have been stored; context_lens count them.  A block that is not full yet has the bounds of the
+    cu_seqlens) the last cu_new[s + 1] - cu_new[s], at most max_new: of a sequence with more, the
+    newest max_new alone, and status has DEV_BAD_POSITION.  Call it after those tokens' keys have been stored; context_lens count them.  A block that is not full yet has the bounds of the
     keys in it.  A sequence (and so a page with new tokens) appears once in the batch: of
     sequences that share a page only the longest may have new tokens in it."""
     dev = _device_of(k_cache)

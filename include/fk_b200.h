@@ -208,8 +208,8 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  * channel d over the cached tokens of the i-th run of `block` positions of a page,
  * i in [0, page_size / block), for the blocks that hold the last
  * cu_new[s + 1] - cu_new[s] tokens of sequence s (cu_new NULL: one token each),
- * at most max_new each.  context_lens count the new tokens, whose keys are in the
- * cache already.  Bounds of other blocks stay as they are.  A sequence appears
+ * at most max_new each (of more, the newest max_new, and FK_DEV_BAD_POSITION is
+ * flagged).  context_lens count the new tokens, whose keys are in the cache already.  Bounds of other blocks stay as they are.  A sequence appears
  * once, and of sequences that share a page only the longest may have new tokens in it.
  * No-number keys give no-number bounds.
  *

@@ -91,6 +91,32 @@ def test_bounds_bad_pages_and_lengths_are_flagged(ops):
     assert float(b[1:].abs().sum()) == 0            # the cut context's page 0 alone was written
 
 
+@pytest.mark.parametrize("max_new", [1, 16, 17, 100])
+def test_bounds_of_more_new_tokens_than_said(ops, max_new):
+    """The newest max_new of a sequence that has more are taken, and that is flagged; the others of
+    the batch have what they had."""
+    rng = np.random.default_rng(4)
+    lens, new, page, block = [300, 64, 130, 7], [300, 1, 101, 1], 64, 16
+    kc = S.pool(rng, 12, page, 2, "NHD")
+    t = S.tables(rng, lens, page, 12)
+    want = np.full((12, 2, page // block, 2, S.D), 7.0, np.float32)
+    for i, n in enumerate(lens):
+        for b in range((n - min(new[i], max_new)) // block, -(-n // block)):
+            pos = np.arange(b * block, min(n, (b + 1) * block))
+            k = np.stack([S.rows(kc, t[i], pos, h, page, "NHD") for h in range(2)])
+            want[t[i, b * block // page], :, b * block % page // block] = np.stack([k.min(1), k.max(1)], 1)
+    got = torch.full(want.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    st = ops.new_status("cuda")
+    ops.key_bounds(dev(kc), got, ints(lens), ints(t), cu_new=ints(np.cumsum([0, *new])), max_new=max_new,
+                   status=st)
+    np.testing.assert_array_equal(host_f32(got), want)
+    assert int(st.item()) == 8
+    st = ops.new_status("cuda")                     # as many as said: no flag
+    ops.key_bounds(dev(kc), got, ints(lens), ints(t), cu_new=ints(np.cumsum([0, *new])), max_new=300,
+                   status=st)
+    assert int(st.item()) == 0
+
+
 # ------------------------------------------------------------------------------- select
 def select_case(seed, t, hq, hkv, page, block, longest, rows=None):
     rng = np.random.default_rng(seed)
