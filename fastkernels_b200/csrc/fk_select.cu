@@ -804,10 +804,13 @@ select_scores_many_kernel(const SelectParams p) {
       if (nt + 1 < tiles) column(nt + 1, next);
       float v[4];
       score_tile(l0, u0, l1, u1, qp, qm, v);
-      // a token's heads: columns 2 quad + 0, 1, then next lanes, then the next tile
-      const int head = (nt * 8 + quad * 2) & (p.cols - 1);
+      // a token's heads: columns 2 quad + 0, 1, then next lanes, then the next tile (of one head a
+      // token, every column is another token)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = head + (i & 1) < p.g ? v[i] : -INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        const int head = (nt * 8 + quad * 2 + (i & 1)) & (p.cols - 1);
+        v[i] = head < p.g ? v[i] : -INFINITY;
+      }
       if (p.cols > 1) {
         v[0] = v[1] = max_nan(v[0], v[1]);
         v[2] = v[3] = max_nan(v[2], v[3]);

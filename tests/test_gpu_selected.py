@@ -185,6 +185,31 @@ def test_select_many_tokens(ops, hq, hkv, n):
     check_select(ops, q, bounds, lens, table, 16, 9, 1, 2, rows)
 
 
+@pytest.mark.parametrize("hq,hkv,n", [(8, 8, 301), (4, 2, 90), (10, 2, 130), (16, 1, 70)])
+def test_select_scores_every_token_of_a_run(ops, hq, hkv, n):
+    """The scores that the choice starts from, [tokens, KV heads, blocks up to a multiple of four] at
+    the workspace's start as fp32 in the order of whole numbers: off by 2^-18 sum |q| max |bound| at
+    most, whatever the number of query heads of a KV head."""
+    rows = [0] * 37 + [1] * (n - 38) + [2]
+    rng, q, bounds, table = select_case(hq + n, n, hq, hkv, 64, 16, 1500, rows)
+    cols, per, g = table.shape[1], 4, hq // hkv
+    ws = torch.zeros(ops.select_blocks_workspace_bytes(n, hq, hkv, 64, 16, cols), dtype=torch.uint8,
+                     device="cuda")
+    ops.select_blocks(dev(q), dev(bounds), ints([1500] * n), ints(table), 16, 9, keep_first=1,
+                      keep_last=2, table_rows=ints(rows), workspace=ws)
+    keys = ws.view(torch.int32)[:n * hkv * cols * per].view(n, hkv, cols * per).cpu().numpy()
+    keys = keys.view(np.uint32)[:, :, :-(-1500 // 16) - 3]            # blocks 1 .. 91 of 94
+    got = np.where(keys >> 31, keys & 0x7fffffff, ~keys).astype(np.uint32).view(np.float32)
+    b = np.arange(1, 1 + got.shape[2])
+    for i in range(n):
+        of = bounds[table[rows[i], b // per], :, b % per].astype(np.float64)       # [blocks, hkv, 2, D]
+        a = q[i].reshape(hkv, g, 1, S.D).astype(np.float64)
+        want = np.maximum(a * of[:, :, 0].swapaxes(0, 1)[:, None],
+                          a * of[:, :, 1].swapaxes(0, 1)[:, None]).sum(-1).max(1)
+        reach = np.abs(a).sum(-1).max() * np.abs(of).max()
+        assert (np.abs(got[i] - want) <= 2.0 ** -18 * reach).all(), i
+
+
 @pytest.mark.parametrize("what", ["few values", "one block", "zero query", "equal blocks"])
 def test_select_takes_the_first_of_equals(ops, what):
     rng, q, bounds, table = select_case(13, 4, 8, 2, 64, 64, 64 * 700)
