@@ -1095,6 +1095,7 @@ int fk_select_blocks(const void* q, int64_t q_stride_token, const void* bounds, 
   FK_CUDA_OK(launch_kernel(scores,
                            dim3((unsigned)(w.groups * w.chunks), (unsigned)num_kv_heads),
                            dim3(32 * SEL_WARPS), ring, s, p));
+  count_launch(1);
   const int64_t items = (int64_t)num_tokens * num_kv_heads;
   const int sms = sm_count();
   const int warps = items <= 2ll * sms ? 8 : items < 16ll * sms || most > SEL_WARP_BLOCKS ? 4 : 1;

@@ -477,6 +477,29 @@ def test_chain_in_a_graph_and_on_another_stream(ops):
         close(out, *attend_oracle(a, kc, vc, lens, table, want, 64, 64, "NHD", 2, None))
 
 
+def test_launches_are_counted(ops):
+    """Two kernels choose blocks; attention over them is one, and a join where tokens are few."""
+    from fastkernels_b200 import _lib
+    rng, q, bounds, table = select_case(17, 3, 8, 2, 64, 64, 3000)
+    lens, kc = ints([3000, 700, 1]), dev(S.pool(rng, len(bounds), 64, 2, "NHD"))
+
+    def launches(f):
+        before = _lib.lib.fk_launch_count()
+        return f(), _lib.lib.fk_launch_count() - before
+    sel, n = launches(lambda: ops.select_blocks(dev(q), dev(bounds), lens, ints(table), 64, 16))
+    assert n == 2
+    _, n = launches(lambda: ops.select_blocks(dev(q), dev(bounds), lens, ints(table), 64, 16,
+                                              table_rows=ints([0, 1, 2])))
+    assert n == 2
+    for count, joined in ((16, True), (2, False)):      # 8 tiles of 128 keys a token and head; one
+        part = sel[:, :, :count].contiguous()
+        assert (ops.selected_attn_workspace_bytes(3, 8, 2, S.D, count, 64) > 0) is joined
+        _, n = launches(lambda: ops.selected_attn(dev(q), kc, kc, lens, ints(table), part, 64, S.SCALE))
+        assert n == 1 + joined
+    _, n = launches(lambda: ops.key_bounds(kc, dev(bounds), lens, ints(table)))
+    assert n == 1
+
+
 def test_nothing_to_do(ops):
     kc = dev(np.ones((2, 64, 2, 128), np.float32))
     q = torch.empty((0, 4, 128), dtype=torch.bfloat16, device="cuda")
