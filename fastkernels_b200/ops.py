@@ -427,6 +427,11 @@ def _workspace(dev, workspace, need: int, like) -> tuple[int | None, int, object
 
 
 @functools.lru_cache(maxsize=4096)
+def _bytes_on(dev, name, *sizes) -> int:
+    """A workspace's bytes on a device: they depend on the number of its SMs too."""
+    return int(getattr(lib, name)(*sizes))
+
+
 def shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, head_dim,
                                   max_splits) -> int:
     return int(lib.fk_shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads,
@@ -485,7 +490,7 @@ def shared_prefix_attn(q, k_cache, v_cache, context_lens, block_tables, group_st
         max_splits = max_splits_for(cols * page)
     ws, ws_bytes, _held = _workspace(
         dev, workspace,
-        shared_prefix_workspace_bytes(b, groups, hq, hkv, d, max_splits)
+        _bytes_on(dev, "fk_shared_prefix_workspace_bytes", b, groups, hq, hkv, d, max_splits)
         if workspace is None else 0, q)
     check(lib.fk_shared_prefix_attn(
         1 if planned else 0, q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
@@ -540,7 +545,6 @@ def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new
     return bounds
 
 
-@functools.lru_cache(maxsize=4096)
 def select_blocks_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, page_size, block,
                                   table_cols) -> int:
     return int(lib.fk_select_blocks_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, page_size,
@@ -577,7 +581,7 @@ def select_blocks(q, bounds, context_lens, block_tables, block, count, keep_firs
             raise _lib.FkError("out must be a contiguous [tokens, Hkv, count]")
     ws, ws_bytes, _held = _workspace(
         dev, workspace,
-        select_blocks_workspace_bytes(n, hq, hkv, per * block, block, cols)
+        _bytes_on(dev, "fk_select_blocks_workspace_bytes", n, hq, hkv, per * block, block, cols)
         if workspace is None else 0, q)
     check(lib.fk_select_blocks(
         q.data_ptr(), qs, bounds.data_ptr(), pages, per * block, block, context_lens.data_ptr(),
@@ -587,7 +591,6 @@ def select_blocks(q, bounds, context_lens, block_tables, block, count, keep_firs
     return out
 
 
-@functools.lru_cache(maxsize=4096)
 def selected_attn_workspace_bytes(num_tokens, num_q_heads, num_kv_heads, head_dim, count,
                                   block) -> int:
     return int(lib.fk_selected_attn_workspace_bytes(num_tokens, num_q_heads, num_kv_heads,
@@ -617,7 +620,8 @@ def selected_attn(q, k_cache, v_cache, context_lens, block_tables, selected, blo
     count = selected.shape[2]
     out, os_ = _out_like(dev, q, out)
     ws, ws_bytes, _held = _workspace(
-        dev, workspace, selected_attn_workspace_bytes(n, hq, hkv, d, count, block)
+        dev, workspace,
+        _bytes_on(dev, "fk_selected_attn_workspace_bytes", n, hq, hkv, d, count, block)
         if workspace is None else 0, q)
     check(lib.fk_selected_attn(
         q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,

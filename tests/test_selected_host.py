@@ -174,6 +174,26 @@ def test_wrappers_refuse_cpu_tensors_and_odd_layouts():
             f()
 
 
+def test_workspace_sizes_follow_the_device(monkeypatch):
+    """The bytes depend on the SMs of the current device: a size asked for on one is not another's."""
+    from types import SimpleNamespace
+    from fastkernels_b200 import ops
+    sms = [148]
+    monkeypatch.setattr(ops, "lib", SimpleNamespace(
+        **{f"fk_{n}_workspace_bytes": lambda *a: 1000 * sum(a) + sms[0]
+           for n in ("shared_prefix", "select_blocks", "selected_attn")}))
+    sizes = (1000, 1, 8, 2, 128, 4)
+    for f in (ops.shared_prefix_workspace_bytes, ops.select_blocks_workspace_bytes,
+              ops.selected_attn_workspace_bytes):
+        name = "fk_" + f.__name__
+        assert hasattr(L, name)
+        for dev, n in ((0, 148), (1, 132), (0, 148)):
+            sms[0] = n
+            assert f(*sizes) == 1000 * sum(sizes) + n
+            assert ops._bytes_on(dev, name, *sizes) == 1000 * sum(sizes) + n
+    ops._bytes_on.cache_clear()
+
+
 def test_the_bound_of_a_block_is_above_its_logits():
     rng = np.random.default_rng(1)
     kc = S.pool(rng, 6, 64, 2, "NHD")
