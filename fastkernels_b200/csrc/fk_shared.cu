@@ -155,6 +155,7 @@ struct SharedPlanParams {
 };
 
 constexpr int PLAN_MAX_BATCH = 16384;
+constexpr int64_t PLAN_MAX_TOKENS = 1ll << 30;    // of a row: positions and sums of chunks in 32 bits
 constexpr int PLAN_THREADS = 512;
 constexpr int PLAN_WARPS = PLAN_THREADS / 32;
 
@@ -1227,6 +1228,7 @@ static int shared_impl(int mode, const void* q, int64_t q_stride_token, void* ou
              FK_ERR_WORKSPACE,
              "fk_shared_prefix_attn: workspace needs %zu bytes, 256-byte aligned (got %zu)",
              w.total, workspace_bytes);
+  if (r.capacity > PLAN_MAX_TOKENS) r.capacity = PLAN_MAX_TOKENS;
   const int g = r.g, sms = sm_count(), per_tile = 128 / g;
   // Small calls as fk_paged_decode_attn has them: a CTA per row and KV head, which read the common part
   // from L2, in one launch instead of four that wait for one another (8 rows of 512 common tokens

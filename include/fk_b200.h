@@ -195,7 +195,8 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  * (Starts that do not ascend within the batch are flagged FK_DEV_BAD_POSITION; no row has
  * anything in common then.)  A row whose context ends inside the common part has it for
  * itself, or the others share no more than that row has.  max_splits: upper bound of KV
- * splits of what each row has for itself.  softmax_scale above zero.  Launches: schedule,
+ * splits of what each row has for itself.  softmax_scale above zero; contexts of at
+ * most 2^30 tokens (longer ones are cut there and flagged FK_DEV_BAD_PAGE).  Launches: schedule,
  * common part, own parts (beside it), join; one launch where batch * num_kv_heads fits the
  * SMs and the tables have at most 2048 tokens.
  * fk_shared_prefix_plan computes the schedule of a step into the workspace, and calls
@@ -209,8 +210,9 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  * i in [0, page_size / block), for the blocks that hold the last
  * cu_new[s + 1] - cu_new[s] tokens of sequence s (cu_new NULL: one token each),
  * at most max_new each (of more, the newest max_new, and FK_DEV_BAD_POSITION is
- * flagged).  context_lens count the new tokens, whose keys are in the cache already.  Bounds of other blocks stay as they are.  A sequence appears
- * once, and of sequences that share a page only the longest may have new tokens in it.
+ * flagged).  context_lens count the new tokens, whose keys are in the cache already.
+ * Bounds of other blocks stay as they are.  A sequence appears once, and of sequences
+ * that share a page only the longest may have new tokens in it.
  * No-number keys give no-number bounds.
  *
  * fk_select_blocks: for query token i and KV head, of the n = ceil(context_lens[i]

@@ -214,6 +214,29 @@ def test_pages_far_behind(ops):
         assert torch.equal(got, near)
 
 
+def test_contexts_near_two_to_31(ops):
+    """Contexts whose ends leave 32 bits no room are cut at 2^30 tokens, and that is flagged.  A table
+    lists one page again and again, so every whole number of them has one result."""
+    page, cols, splits = 1 << 16, 1 << 15, 64
+    rng = np.random.default_rng(6)
+    kc = S.bf16(rng.standard_normal((1, page, 1, S.D), dtype=np.float32) * 0.25)
+    vc = S.bf16(np.linspace(-2, 2, S.D) + 0.25 * rng.standard_normal((1, page, 1, S.D)))
+    q = S.bf16(rng.standard_normal((4, 2, S.D)))
+    lens = [2 ** 31 - 1, 2 ** 31 - 700, 2 ** 31 - 1, 300]
+    table = torch.zeros((1, cols), dtype=torch.int32, device="cuda").expand(4, cols)
+    st = ops.new_status("cuda")
+    got = ops.shared_prefix_attn(dev(q), dev(kc), dev(vc), ints(lens), table, ints([0, 2]),
+                                 ints([2 ** 31 - 1]), S.SCALE, max_splits=splits, status=st)
+    assert int(st.item()) == 2
+    out, mass = S.over_positions(q, kc, vc, lens, np.zeros((4, 1), np.int32), page, "NHD", 1,
+                                 lambda i, h: range(min(lens[i], page)))
+    d = np.abs(host_f32(got) - out)
+    # a CTA adds up 2^30 / 128 / 148 steps of 8 products into one sum, a split 2^23 / 64 of one a warp
+    steps = max(2 ** 23 / 148 * 8, 2 ** 23 / 64)
+    assert (d <= S.tolerance(out, mass) + 2 * steps * 2.0 ** -23 * mass).all(), d.max()
+    assert (d[3] <= S.tolerance(out, mass)[3]).all()
+
+
 def test_many_groups(ops):
     rng = np.random.default_rng(2)
     groups = [(int(rng.integers(0, 9)) * 16, [int(x) for x in rng.integers(1, 60, rng.integers(1, 5))])
