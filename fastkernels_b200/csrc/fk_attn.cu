@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(
     plan[1] = chunk;    // tokens per chunk
     plan[2] = 0;        // work counter
     plan[3] = maxL;
+    plan[ATT_PLAN_HDR - 1] = 0;   // what a schedule of common prefixes was here is none any more
   }
 }
 

@@ -441,7 +441,8 @@ def shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, 
 def shared_prefix_plan(context_lens, block_tables, page_size, num_q_heads, num_kv_heads, head_dim,
                        group_starts, prefix_lens, workspace, max_splits, status=None) -> None:
     """The schedule of a decode step, once: layers then call shared_prefix_attn(..., planned=True)
-    with the same lengths, groups, tables, workspace and max_splits."""
+    with the same lengths, groups, tables, workspace and max_splits.  No other call has the workspace
+    in between."""
     dev = _device_of(context_lens)
     b = context_lens.numel()
     _need_ints(dev, b, "context_lens", context_lens)
@@ -522,9 +523,10 @@ def key_bounds(k_cache, bounds, context_lens, block_tables, cu_new=None, max_new
     """Smallest and largest key per channel, in place and exact, of the blocks that hold the newest
     tokens of each sequence: the last one, or with cu_new (int32 [sequences + 1], as
     cu_seqlens) the last cu_new[s + 1] - cu_new[s], at most max_new: of a sequence with more, the
-    newest max_new alone, and status has DEV_BAD_POSITION.  Call it after those tokens' keys have been stored; context_lens count them.  A block that is not full yet has the bounds of the
-    keys in it.  A sequence (and so a page with new tokens) appears once in the batch: of
-    sequences that share a page only the longest may have new tokens in it."""
+    newest max_new alone, and status has DEV_BAD_POSITION.  Call it after those tokens' keys have
+    been stored; context_lens count them.  A block that is not full yet has the bounds of the keys in
+    it.  A sequence (and so a page with new tokens) appears once in the batch: of sequences that share
+    a page only the longest may have new tokens in it."""
     dev = _device_of(k_cache)
     pages, page, hkv, d, stride = _need_cache(dev, k_cache, kv_layout, "k_cache")
     _need_bounds(dev, bounds)

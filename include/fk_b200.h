@@ -203,7 +203,9 @@ int fk_paged_decode_attn_planned(const void* q, int64_t q_stride_token, void* ou
  * with `planned` go by it for any number of layers afterwards, with the same lengths,
  * groups, sizes, head counts, table columns, max_splits and workspace; a planned call that
  * finds no schedule of its sizes there gives zeros and flags FK_DEV_BAD_POSITION.  A workspace
- * serves one call at a time (and two captured graphs only one after the other).
+ * serves one call at a time (and two captured graphs only one after the other), and between a
+ * schedule and the calls by it no other call has it (one of fk_paged_decode_attn's takes the
+ * schedule's place).
  *
  * fk_key_bounds: bounds[page][head][i][0 / 1][d] = smallest / largest key of
  * channel d over the cached tokens of the i-th run of `block` positions of a page,

@@ -461,6 +461,36 @@ def test_planned_on_any_words(ops, word):
         planned()
 
 
+def test_planned_after_another_schedule_in_its_place(ops):
+    """paged_decode_attn in the workspace of a schedule leaves one of its own there: the planned call
+    behind it gives zeros and a flag, and after a new schedule its result."""
+    case = build(12, [(640, [40 + i for i in range(20)]), (320, [100, 900])], 64, "NHD", 16, 8)
+    q, kc, vc, lens, table, starts, prefix = case
+    args, groups = [ints(lens), ints(table)], [ints(starts), ints(prefix)]
+    x = [dev(q), dev(kc), dev(vc)]
+    ws = torch.empty(max(ops.shared_prefix_workspace_bytes(len(lens), 2, 16, 8, 128, 16),
+                         ops.attn_workspace_bytes(len(lens), 16, 128, 16)), dtype=torch.uint8, device="cuda")
+
+    def planned():
+        status = ops.new_status("cuda")
+        out = torch.full_like(x[0], 7.0)
+        ops.shared_prefix_attn(*x, *args, *groups, S.SCALE, workspace=ws, out=out, status=status,
+                               planned=True, max_splits=16)
+        return out, int(status.item())
+    want = ops.shared_prefix_attn(*x, *args, *groups, S.SCALE, max_splits=16)
+    for whole in (True, False):
+        ops.shared_prefix_plan(*args, 64, 16, 8, 128, *groups, ws, 16)
+        if whole:
+            ops.paged_decode_attn(*x, *args, S.SCALE, ws, 16)
+        else:
+            ops.paged_decode_attn_plan(*args, 64, 16, 8, 128, ws, 16)
+        out, status = planned()
+        assert status == 8 and not out.any()
+    ops.shared_prefix_plan(*args, 64, 16, 8, 128, *groups, ws, 16)
+    out, status = planned()
+    assert status == 0 and torch.equal(out, want)
+
+
 def test_calls_on_two_streams(ops):
     """Two calls at once, each with a workspace of its own."""
     cases = [build(20 + i, [(2048, [70 + 5 * i] * 12), (640, [300, 9])], 64, "NHD", 16, 4)
