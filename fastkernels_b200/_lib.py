@@ -80,6 +80,15 @@ PROTOTYPES = {
     "fk_selected_attn": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp,
                                 _vp, _i64, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
                                 _f32, _vp, _sz, _vp, _vp]),
+    "fk_q4_unit_bytes": (_i64, [_i32, _i32]),
+    "fk_store_kvcache_q4": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp,
+                                   _i32, _i64, _vp, _vp]),
+    "fk_load_kvcache_q4": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i32, _i64,
+                                  _vp, _vp]),
+    "fk_paged_decode_attn_q4_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i64]),
+    "fk_paged_decode_attn_q4": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _i64,
+                                       _i64, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp,
+                                       _i64, _vp, _sz, _vp, _vp]),
     "fk_rmsnorm": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _f32, _i64, _i64,
                           _vp]),
     "fk_fused_add_rmsnorm": (_i32, [_vp, _i64, _vp, _i64, _vp, _f32, _i64, _i64, _vp]),
@@ -202,7 +211,9 @@ PROTOTYPES = {
 # by the symbols they export; a part is there with all of them or not at all.
 COMPONENTS = {
     "decode_attn": [n for n in PROTOTYPES if n.startswith(("fk_paged_decode_attn", "fk_shared_",
-                                                           "fk_key_", "fk_select"))],
+                                                           "fk_key_", "fk_select", "fk_q4_",
+                                                           "fk_store_kvcache_q4",
+                                                           "fk_load_kvcache_q4", "fk_evict_"))],
     "delta": [n for n in PROTOTYPES if n.startswith("fk_delta_")],
     "latent": [n for n in PROTOTYPES if n.startswith("fk_latent_")],
     "mlstm": [n for n in PROTOTYPES if n.startswith("fk_mlstm_")],

@@ -1,0 +1,961 @@
+// Decode attention over a paged KV cache of 4 bits a value, which can also add up what every cached
+// token is given.
+//
+//   logit  z_t = scale (s_t q.c_t + lo_t sum q)         per group of channels, summed
+//   out    sum_t p_t (s_t c_t + lo_t) / sum_t p_t,      p_t = 2^(z_t - m)
+//   sums   of query heads (and query tokens) of p_t / sum p, added to a pool of fp32
+//
+// The codes go to the tensor cores as they are.  Four bits at the lowest end of an fp16 are the
+// number code 2^-24, four bits above them code 2^-20, exactly; so one AND makes two operands, and
+// the scales, per token, are applied to logits and to softmax weights.  Products are those of the
+// transposes, S^T = K Q^T and O^T = V^T P^T (m16n8k16), which have tokens or channels as rows and
+// the up to 8 query heads of a KV head as the 8 columns: half the matrix instructions of the
+// product with 16 rows of queries, of which most would be empty.  A warp takes 32 tokens a step;
+// S^T becomes the operand P^T by one transposing move per 16 tokens.
+//
+// Rounding to fewer bits: q to fp16 with a power of two per head taken out (exact but for channels
+// 2^-26 below the largest), the weights p s to fp16 (11 bits, where bf16 caches' decode has 8), with
+// the step's largest scale's power of two taken out.  Sums, maxima, weights' lowest-value term
+// (sum p lo) are fp32.
+//
+// Work: steps of 32 tokens of all (tokens, KV head) pairs, one after another, are cut into equal runs,
+// one for each warp of the grid.  Warps share nothing: each has a ring of steps of its own,
+// filled by bulk copies (a step is one contiguous copy of up to 4.6 KB), and no barrier between.
+// What a warp does not have whole goes to one of its two places of partial results, joined by
+// the kernel behind.  The running maximum is raised only when a logit is 8 above it (weights up to
+// 2^8 fit), so that in most steps nothing is reduced across lanes and nothing rescaled.
+#include "fk_q4.cuh"
+
+namespace fk {
+
+constexpr int QA_WARPS = 8;
+constexpr int QA_THREADS = QA_WARPS * 32;
+constexpr int QA_STEP = 32;                  // tokens of a warp's step
+constexpr float QA_SLACK = 8.f;              // logits may be this far above the maximum (log2)
+constexpr int64_t QA_LONGEST = 1ll << 30;    // tokens of a context
+
+struct Q4AttnParams {
+  const uint16_t* q; int64_t q_stride;
+  uint16_t* out; int64_t out_stride;
+  const uint8_t* pool;
+  const int32_t* lens;
+  const int32_t* cu;            // tokens of each sequence; null: one each
+  const int32_t* tables; int64_t table_stride;
+  int64_t capacity;             // tokens a table's row has pages for
+  int num_tokens, num_seqs, num_pages, page, hkv, g;
+  int block;                    // query tokens that go together
+  int cols;                     // block * g <= 8 or 16
+  float scale_log2;
+  int32_t* status;
+  int64_t* run;                 // [0] steps of a warp's run
+  int64_t* first;               // [tokens + 1] steps of one head before a token's
+  float2* part_ml;              // [2 * warps, cols]
+  float* part_o;                // [2 * warps, cols, 128]
+  float2* whole_ml;             // [tokens * hkv, cols] of pairs that one warp has
+  float* logits;                // [steps, 32, cols]
+  int64_t logit_steps;
+  float* weights;               // [pages, hkv, page]
+  const int32_t* from;          // [sequences] tokens whose sums go on
+  int chunks;                   // of a sequence's tokens, for the sums
+};
+
+__device__ __forceinline__ uint64_t qa_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+
+// A wait of 2 s at most; all lanes get the same answer.
+__device__ __forceinline__ bool qa_wait_warp(uint64_t* bar, uint32_t parity) {
+  bool got = mbar_try_wait(bar, parity);
+  if (!__all_sync(0xffffffffu, got)) {
+    const uint64_t t0 = qa_ns();
+    bool late = false;
+    do {
+      for (int i = 0; i < 64 && !got; ++i) got = mbar_try_wait(bar, parity);
+      late = qa_ns() - t0 > 2000000000ull;
+    } while (!__all_sync(0xffffffffu, got) && !__any_sync(0xffffffffu, late));
+  }
+  return __all_sync(0xffffffffu, got);
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+// Two fp32 to fp16, lo = a.
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
+// Query tokens that go together, and what they see.
+struct QaItem {
+  int row;        // table
+  int tokens;     // 0: the token is in another's block, or in no sequence
+  int len;        // keys of the longest
+  int steps;
+};
+
+__device__ __forceinline__ int qa_len(const Q4AttnParams& p, int token) {
+  const int64_t n = p.lens[token];
+  return n < 0 ? 0 : n > p.capacity ? (int)p.capacity : (int)n;
+}
+
+__device__ __forceinline__ QaItem qa_item(const Q4AttnParams& p, int token) {
+  QaItem it{token, 1, 0, 0};
+  if (p.cu) {
+    int lo = 0, hi = p.num_seqs;              // the last sequence that begins at or before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.cu[mid] <= token) lo = mid; else hi = mid;
+    }
+    const int a = p.cu[lo], b = min(p.cu[lo + 1], p.num_tokens);
+    it.row = lo;
+    if (a < 0 || token < a || token >= b || (token - a) % p.block != 0) {
+      it.tokens = 0;
+      return it;
+    }
+    it.tokens = min(p.block, b - token);
+  }
+  for (int j = 0; j < it.tokens; ++j) it.len = max(it.len, qa_len(p, token + j));
+  it.steps = (it.len + QA_STEP - 1) / QA_STEP;
+  return it;
+}
+
+// A place in the row of all steps.
+struct QaCursor {
+  int token, head, step;
+  QaItem it;
+  __device__ __forceinline__ void next(const Q4AttnParams& p) {
+    if (++step < it.steps) return;
+    step = 0;
+    if (++head < p.hkv) return;
+    head = 0;
+    do {
+      if (++token >= p.num_tokens) {          // not reached while the lengths stay as they are
+        token = 0;
+        it = QaItem{0, 0, 0, 1 << 30};
+        return;
+      }
+      it = qa_item(p, token);
+    } while (it.steps == 0);
+  }
+};
+
+template <int NG, int NT>
+struct QaShape {
+  static constexpr int kUnit = q4_unit_bytes(NG);
+  static constexpr int kStage = 2 * kUnit;
+  static constexpr int kCtas = NT == 1 ? 2 : 1;            // of an SM
+  static constexpr int kDepth = NT == 1 ? 3 : 6;           // steps of a warp's ring
+  static constexpr int kSmem = QA_WARPS * kDepth * kStage;
+};
+
+// NG groups a row; NT * 8 columns; SUMS: logits are kept for the sums of weights.
+template <int NG, int NT, bool SUMS>
+__global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
+    q4_attn_kernel(const Q4AttnParams p) {
+  using S = QaShape<NG, NT>;
+  constexpr int DEPTH = S::kDepth;
+  extern __shared__ __align__(128) uint8_t ring_all[];
+  __shared__ uint64_t bars[QA_WARPS][DEPTH];
+  __shared__ int64_t begins[QA_THREADS + 1];               // steps before each thread's tokens
+  __shared__ int64_t sums[QA_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = lane & 3, row = lane >> 2;
+  if (lane == 0) {
+    for (int i = 0; i < DEPTH; ++i) mbar_init(&bars[warp][i], 1);
+    mbar_fence_init();
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- where the run of this warp begins ----
+  const int per = (p.num_tokens + QA_THREADS - 1) / QA_THREADS;
+  {
+    const int a = min((int)threadIdx.x * per, p.num_tokens), b = min(a + per, p.num_tokens);
+    int64_t mine = 0;
+    for (int i = a; i < b; ++i) mine += qa_item(p, i).steps;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < QA_WARPS; ++w) {
+      if (w < warp) before += sums[w];
+      total += sums[w];
+    }
+    begins[threadIdx.x] = before + incl - mine;
+    if (threadIdx.x == 0) begins[QA_THREADS] = total;
+    if (blockIdx.x == 0) {
+      int64_t run = before + incl - mine;
+      for (int i = a; i < b; ++i) {
+        p.first[i] = run;
+        const QaItem it = qa_item(p, i);
+        run += it.steps;
+        if (p.status)
+          for (int j = 0; j < it.tokens; ++j)
+            if (p.lens[i + j] > p.capacity) atomicOr(p.status, FK_DEV_BAD_PAGE);
+      }
+      if (threadIdx.x == 0) p.first[p.num_tokens] = total;
+    }
+    __syncthreads();
+  }
+  const int64_t warps = (int64_t)gridDim.x * QA_WARPS;
+  const int64_t total = begins[QA_THREADS] * p.hkv;
+  const int64_t run = (total + warps - 1) / warps;
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.run[0] = run;
+  const int64_t me = (int64_t)blockIdx.x * QA_WARPS + warp;
+  const int64_t x0 = me * run, x1 = min(total, x0 + run);
+  if (x0 >= x1) return;
+
+  QaCursor now;                                            // the step that is computed
+  {
+    const int64_t at = x0 / p.hkv;
+    int lo = 0, hi = QA_THREADS;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (begins[mid] <= at) lo = mid; else hi = mid;
+    }
+    int64_t before = begins[lo];
+    int i = min(lo * per, p.num_tokens - 1);
+    now.it = qa_item(p, i);
+    while (i + 1 < p.num_tokens && before + now.it.steps <= at) {
+      before += now.it.steps;
+      now.it = qa_item(p, ++i);
+    }
+    now.token = i;
+    const int64_t in = x0 - before * p.hkv;
+    const int steps = max(now.it.steps, 1);
+    now.head = (int)(in / steps);
+    now.step = (int)(in - (int64_t)now.head * steps);
+  }
+  QaCursor ahead = now;                                    // the step that is copied
+
+  uint8_t* ring = ring_all + warp * DEPTH * S::kStage;
+  uint64_t* full = bars[warp];
+  const int units = p.page / Q4_UNIT;                      // of a page
+  // pages of 32 steps, a lane each: the page and the unit in it (pages of one unit: the next page)
+  int pg_row = -1, pg_base = 0, pg_a = -1, pg_b = -1;
+  int nx_a = -1, nx_b = -1;
+  auto look_up = [&](int base, int& a, int& b) {
+    const int64_t t = (int64_t)(base + lane) * QA_STEP;
+    a = b = -1;
+    if (t >= ahead.it.len) return;
+    const int32_t* table = p.tables + (int64_t)ahead.it.row * p.table_stride;
+    const int at = (int)t / p.page;
+    a = table[at];
+    if (units > 1) b = ((int)t - at * p.page) / Q4_UNIT;
+    else if (t + Q4_UNIT < ahead.it.len) b = table[at + 1];
+  };
+  uint32_t present = 0;                                    // two bits a slot: its units
+  auto copy = [&](int slot) {
+    const int base = ahead.step & ~31;
+    if (pg_row != ahead.token || base != pg_base) {
+      if (pg_row == ahead.token && base == pg_base + 32) {
+        pg_a = nx_a; pg_b = nx_b;
+      } else {
+        look_up(base, pg_a, pg_b);
+      }
+      pg_row = ahead.token; pg_base = base;
+      look_up(base + 32, nx_a, nx_b);
+    }
+    const int a = __shfl_sync(0xffffffffu, pg_a, ahead.step & 31);
+    const int b = __shfl_sync(0xffffffffu, pg_b, ahead.step & 31);
+    const int left = ahead.it.len - ahead.step * QA_STEP;
+    const int want = left > Q4_UNIT ? 3 : left > 0 ? 1 : 0;
+    int have = a >= 0 && a < p.num_pages ? units > 1 ? 3 : 1 : 0;
+    if (units == 1 && b >= 0 && b < p.num_pages) have |= 2;
+    have &= want;
+    present = (present & ~(3u << (2 * slot))) | (uint32_t)have << (2 * slot);
+    if (lane == 0) {
+      if (have != want && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+      mbar_arrive_expect_tx(&full[slot], __popc(have) * S::kUnit);
+      uint8_t* dst = ring + slot * S::kStage;
+      if (units > 1) {
+        if (have)
+          bulk_load(dst, p.pool + (((int64_t)a * p.hkv + ahead.head) * units + b) * S::kUnit,
+                    __popc(have) * S::kUnit, &full[slot]);
+      } else {
+        if (have & 1)
+          bulk_load(dst, p.pool + ((int64_t)a * p.hkv + ahead.head) * S::kUnit, S::kUnit,
+                    &full[slot]);
+        if (have & 2)
+          bulk_load(dst + S::kUnit, p.pool + ((int64_t)b * p.hkv + ahead.head) * S::kUnit,
+                    S::kUnit, &full[slot]);
+      }
+    }
+    __syncwarp();
+    ahead.next(p);
+  };
+  const int64_t count = x1 - x0;
+  for (int i = 0; i < DEPTH && i < count; ++i) copy(i);
+
+  // ---- state of a pair: columns 8 nt + 2 quad + {0, 1} ----
+  uint32_t qf[NT][8][2];
+  float o[8][NT][4];
+  float m[NT][2], l[NT][2], low[NG][NT][2];   // maximum, sum of weights, sum of weights' lowest
+  float factor[NT][2], qsum[NG][NT][2];       // of logits: of a product, of a token's lowest
+  int len[NT][2];
+  int shortest = 0;
+  float vref = 0.f, vinv = 0.f;
+
+  bool ok = true;
+  int slot = 0;
+  uint32_t phase = 0;
+  int64_t x = x0;
+  for (; x < x1; ++x) {
+    if (x == x0 || now.step == 0) {
+      // ---------------------------------------------------------------- a new pair
+      shortest = 0x7fffffff;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int col = nt * 8 + row;
+        const int tok = col / p.g;
+        const bool live = tok < now.it.tokens;
+        uint4 w[4];
+        float f = 0.f, sum[NG];
+        int n = 0;
+        if (live) {
+          const uint4* src = reinterpret_cast<const uint4*>(
+              p.q + (int64_t)(now.token + tok) * p.q_stride +
+              (int64_t)(now.head * p.g + col - tok * p.g) * Q4_D);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = src[4 * i + quad];
+          n = qa_len(p, now.token + tok);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        shortest = min(shortest, live ? n : 0x7fffffff);
+        float big = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) sum[gr] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = bf16lo(u[e]), b = bf16hi(u[e]);
+            big = fmaxf(big, fmaxf(fabsf(a), fabsf(b)));
+            sum[i * NG / 4] += a + b;
+          }
+        }
+#pragma unroll
+        for (int sh = 1; sh < 4; sh <<= 1) {
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], sh);
+        }
+        // 2^(13 - E) for the largest channel in [2^E, 2^(E+1))
+        const int e = max((int)(__float_as_uint(big) >> 23), 28);
+        const float up = __uint_as_float((uint32_t)(127 + 13 + 127 - e) << 23);
+        f = __uint_as_float((uint32_t)(e - 13) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // channels c, c + 4 | c + 1, c + 5, which meet codes 2^4 too large | c + 2, c + 6 | ...
+          const float c0 = bf16lo(w[i].x) * up, c1 = bf16hi(w[i].x) * up;
+          const float c2 = bf16lo(w[i].y) * up, c3 = bf16hi(w[i].y) * up;
+          const float c4 = bf16lo(w[i].z) * up, c5 = bf16hi(w[i].z) * up;
+          const float c6 = bf16lo(w[i].w) * up, c7 = bf16hi(w[i].w) * up;
+          qf[nt][2 * i][0] = pack_f16(c0, c4);
+          qf[nt][2 * i][1] = pack_f16(c1 * 0.0625f, c5 * 0.0625f);
+          qf[nt][2 * i + 1][0] = pack_f16(c2, c6);
+          qf[nt][2 * i + 1][1] = pack_f16(c3 * 0.0625f, c7 * 0.0625f);
+        }
+        f *= 16777216.f * p.scale_log2;                    // codes are 2^-24
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int from = (2 * quad + j) * 4;             // a lane of that column
+          factor[nt][j] = __shfl_sync(0xffffffffu, f, from);
+          len[nt][j] = __shfl_sync(0xffffffffu, n, from);
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr)
+            qsum[gr][nt][j] = __shfl_sync(0xffffffffu, sum[gr], from) * p.scale_log2;
+          m[nt][j] = -INFINITY;
+          l[nt][j] = 0.f;
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] = 0.f;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt)
+          o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+      }
+      shortest = __reduce_min_sync(0xffffffffu, shortest);
+      vref = vinv = 0.f;
+    }
+
+    if (!qa_wait_warp(&full[slot], phase)) {
+      if (lane == 0 && p.status) atomicOr(p.status, FK_DEV_WAIT_TIMEOUT);
+      ok = false;
+      break;
+    }
+    const uint8_t* st = ring + slot * S::kStage;
+    const uint32_t have = present >> (2 * slot) & 3u;
+    const int tok0 = now.step * QA_STEP;
+
+    // ---- logits: rows are tokens row, row + 8 of unit u ----
+    float z[2][NT][4];                                      // [unit][.][row 0: 2 columns, row 8: 2]
+    float vs[2][NG][2], vl[2][NG][2];                       // the values' scale and lowest
+    const bool edge = tok0 + QA_STEP > shortest || have != 3u;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* un = st + u * S::kUnit;
+      const uint4 ka = *reinterpret_cast<const uint4*>(un + row * Q4_ROW + quad * 16);
+      const uint4 kb = *reinterpret_cast<const uint4*>(un + (row + 8) * Q4_ROW + quad * 16);
+      uint32_t kp[2][NG], vp[2][NG];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(un + Q4_PAIRS);
+        if constexpr (NG == 2) {
+          const uint2 a = *reinterpret_cast<const uint2*>(pairs + (row + 8 * r) * 2);
+          const uint2 b = *reinterpret_cast<const uint2*>(pairs + (Q4_UNIT + row + 8 * r) * 2);
+          kp[r][0] = a.x; kp[r][1] = a.y; vp[r][0] = b.x; vp[r][1] = b.y;
+        } else {
+          kp[r][0] = pairs[row + 8 * r];
+          vp[r][0] = pairs[Q4_UNIT + row + 8 * r];
+        }
+      }
+      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+      float acc[NG][NT][4];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[gr][nt][0] = acc[gr][nt][1] = acc[gr][nt][2] = acc[gr][nt][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t ya = wa[i] >> 8, yb = wb[i] >> 8;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_f16_16816(acc[i * NG / 4][nt], wa[i] & 0x000f000fu, wb[i] & 0x000f000fu,
+                        wa[i] & 0x00f000f0u, wb[i] & 0x00f000f0u, qf[nt][2 * i][0],
+                        qf[nt][2 * i][1]);
+          mma_f16_16816(acc[i * NG / 4][nt], ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
+                        yb & 0x00f000f0u, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float t = bf16lo(kp[e >> 1][0]) * acc[0][nt][e];
+          float b = bf16hi(kp[e >> 1][0]) * qsum[0][nt][e & 1];
+          if constexpr (NG == 2) {
+            t = fmaf(bf16lo(kp[e >> 1][1]), acc[1][nt][e], t);
+            b = fmaf(bf16hi(kp[e >> 1][1]), qsum[1][nt][e & 1], b);
+          }
+          z[u][nt][e] = fmaf(t, factor[nt][e & 1], b);
+        }
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          vs[u][gr][r] = bf16lo(vp[r][gr]);
+          vl[u][gr][r] = bf16hi(vp[r][gr]);
+        }
+      if (edge) {
+        // what stands behind the context is any number, or none
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int t = tok0 + u * Q4_UNIT + row + 8 * r;
+          const bool there = (have >> u & 1u) && t < now.it.len;
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr)
+            if (!there) vs[u][gr][r] = vl[u][gr][r] = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (!there || t >= len[nt][j]) z[u][nt][2 * r + j] = -INFINITY;
+        }
+      }
+      if constexpr (SUMS) {
+        if (x < p.logit_steps) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float* dst = p.logits + (x * QA_STEP + u * Q4_UNIT + row + 8 * r) * p.cols;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const int c = nt * 8 + 2 * quad;
+              if (c + 1 < p.cols && (p.cols & 1) == 0) {
+                *reinterpret_cast<float2*>(dst + c) =
+                    make_float2(z[u][nt][2 * r], z[u][nt][2 * r + 1]);
+              } else {
+                if (c < p.cols) dst[c] = z[u][nt][2 * r];
+                if (c + 1 < p.cols) dst[c + 1] = z[u][nt][2 * r + 1];
+              }
+            }
+          }
+        }
+      }
+    }
+
+    // ---- new references, if a logit or a scale has left the old ones behind ----
+    bool beyond = false;
+    float vmax = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) vmax = fmaxf(vmax, vs[u][gr][r]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) beyond |= z[u][nt][2 * r + j] > m[nt][j] + QA_SLACK;
+      }
+    beyond |= vmax > vref;
+    if (__any_sync(0xffffffffu, beyond)) {
+#pragma unroll
+      for (int sh = 4; sh < 32; sh <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
+      float vnew = vref;
+      if (vmax > vref)                                      // the power of two above
+        vnew = fmaxf(__uint_as_float(((__float_as_uint(vmax) >> 23) + 1u) << 23), 1e-30f);
+      const float vshift = vref > 0.f ? vref / vnew : 0.f;
+      vref = vnew;
+      vinv = vnew > 0.f ? 64.f / vnew : 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float mx = fmaxf(fmaxf(z[0][nt][j], z[0][nt][2 + j]), fmaxf(z[1][nt][j], z[1][nt][2 + j]));
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+          const float old = m[nt][j], next = fmaxf(old, mx);
+          const float alpha = old == next ? 1.f : fast_exp2(old - next);
+          m[nt][j] = next;
+          l[nt][j] *= alpha;
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            o[mt][nt][j] *= alpha * vshift;
+            o[mt][nt][2 + j] *= alpha * vshift;
+          }
+        }
+    }
+
+    // ---- weights, and the operand P^T ----
+    uint32_t pt[2][NG][NT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float w[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+            w[j] = fast_exp2(z[u][nt][2 * r + j] - ref);
+            l[nt][j] += w[j];
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] = fmaf(w[j], vl[u][gr][r], low[gr][nt][j]);
+          }
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            const float f = vs[u][gr][r] * vinv;
+            pt[u][gr][nt][r] = transpose_8x8(pack_f16(w[0] * f, w[1] * f));
+          }
+        }
+
+    // ---- O^T += V^T P^T: rows are channels, of lane `row` 8 row + {0 .. 7} (+ 64) ----
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* un = st + u * S::kUnit + Q4_VALUES + row * 8;
+      const uint2 a0 = *reinterpret_cast<const uint2*>(un + (2 * quad) * Q4_ROW);
+      const uint2 a1 = *reinterpret_cast<const uint2*>(un + (2 * quad + 1) * Q4_ROW);
+      const uint2 b0 = *reinterpret_cast<const uint2*>(un + (2 * quad + 8) * Q4_ROW);
+      const uint2 b1 = *reinterpret_cast<const uint2*>(un + (2 * quad + 9) * Q4_ROW);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t wa0 = h ? a0.y : a0.x, wa1 = h ? a1.y : a1.x;
+        const uint32_t wb0 = h ? b0.y : b0.x, wb1 = h ? b1.y : b1.x;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // channels 4 half .. 4 half + 3 of the word, of two tokens side by side
+          uint32_t xa = __byte_perm(wa0, wa1, half ? 0x7632 : 0x5410);
+          uint32_t xb = __byte_perm(wb0, wb1, half ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int mt = 4 * h + 2 * half + k;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16_16816(o[mt][nt], xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu,
+                            xb & 0x00f000f0u, pt[u][h * NG / 2][nt][0], pt[u][h * NG / 2][nt][1]);
+            xa >>= 8;
+            xb >>= 8;
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (x + DEPTH < x1) copy(slot);
+    if (++slot == DEPTH) { slot = 0; phase ^= 1; }
+
+    if (now.step + 1 == now.it.steps || x + 1 == x1) {
+      // ---------------------------------------------------------------- the pair's end
+      const int64_t px = x - now.step, pe = px + now.it.steps;
+      const bool whole = px >= x0 && pe <= x1;
+      const int64_t place = 2 * me + (px > x0 ? 1 : 0);
+      const float vback = vref * (1.f / 64.f);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float sum = l[nt][j], lows[NG];
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) lows[gr] = low[gr][nt][j];
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+              lows[gr] += __shfl_xor_sync(0xffffffffu, lows[gr], sh);
+          }
+          const int col = nt * 8 + 2 * quad + j;
+          const int tok = col / p.g;
+          if (tok >= now.it.tokens) continue;
+          const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              v[c] = fmaf(o[4 * h + (c >> 1)][nt][(c & 1) * 2 + j] * vback,
+                          (c & 1) ? 1048576.f : 16777216.f, lows[h * NG / 2]);
+            if (whole) {
+              uint4 w;
+              w.x = pack_bf16(v[0] * inv, v[1] * inv);
+              w.y = pack_bf16(v[2] * inv, v[3] * inv);
+              w.z = pack_bf16(v[4] * inv, v[5] * inv);
+              w.w = pack_bf16(v[6] * inv, v[7] * inv);
+              *reinterpret_cast<uint4*>(p.out + (int64_t)(now.token + tok) * p.out_stride +
+                                        (int64_t)(now.head * p.g + col - tok * p.g) * Q4_D +
+                                        64 * h + 8 * row) = w;
+            } else {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + (place * p.cols + col) * Q4_D +
+                                                      64 * h + 8 * row);
+              dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+              dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+          }
+          if (row == 0) {
+            if (!whole) p.part_ml[place * p.cols + col] = make_float2(m[nt][j], sum);
+            else if (SUMS)
+              p.whole_ml[((int64_t)now.token * p.hkv + now.head) * p.cols + col] =
+                  make_float2(m[nt][j], sum);
+          }
+        }
+    }
+    now.next(p);
+  }
+  if (!ok) {
+    // copies still on their way end before the shared memory goes
+    for (int i = 0; i < DEPTH && i < x1 - x; ++i) {
+      (void)qa_wait_warp(&full[slot], phase);
+      if (++slot == DEPTH) { slot = 0; phase ^= 1; }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// join of partial results; sums of weights
+// ---------------------------------------------------------------------------
+// The runs that a pair's steps lie in: warps a .. b; warp a has the pair in its second place unless
+// the pair begins with the run.
+struct QaRuns {
+  int64_t px, a, b;
+  int second;
+  __device__ __forceinline__ int64_t place(int64_t w) const { return 2 * w + (w == a ? second : 0); }
+};
+__device__ __forceinline__ QaRuns qa_runs(const Q4AttnParams& p, int token, int head, int64_t steps) {
+  const int64_t run = p.run[0];
+  QaRuns r;
+  r.px = p.first[token] * p.hkv + head * steps;
+  r.a = r.px / run;
+  r.b = (r.px + steps - 1) / run;
+  r.second = r.px > r.a * run ? 1 : 0;
+  return r;
+}
+
+// (maximum, sum of weights) of a column over all parts; all lanes of a warp.
+__device__ __forceinline__ float2 qa_total(const Q4AttnParams& p, const QaRuns& r, int col) {
+  const int lane = threadIdx.x & 31;
+  float M = -INFINITY;
+  for (int64_t w = r.a + lane; w <= r.b; w += 32)
+    M = fmaxf(M, p.part_ml[r.place(w) * p.cols + col].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float Mu = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  for (int64_t w = r.a + lane; w <= r.b; w += 32) {
+    const float2 v = p.part_ml[r.place(w) * p.cols + col];
+    L += v.y * fast_exp2(v.x - Mu);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  return make_float2(Mu, L);
+}
+
+__device__ __forceinline__ void qa_join(const Q4AttnParams& p, int token, int head) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t steps = p.first[token + 1] - p.first[token];
+  if (steps == 0) {
+    const QaItem it = qa_item(p, token);
+    for (int c = warp; c < it.tokens * p.g; c += QA_WARPS) {
+      const int tok = c / p.g;
+      reinterpret_cast<uint2*>(p.out + (int64_t)(token + tok) * p.out_stride +
+                               (int64_t)(head * p.g + c - tok * p.g) * Q4_D)[lane] =
+          make_uint2(0u, 0u);
+    }
+    return;
+  }
+  const QaRuns r = qa_runs(p, token, head, steps);
+  if (r.a == r.b) return;
+  const int tokens = p.cu ? qa_item(p, token).tokens : 1;
+  for (int c = warp; c < tokens * p.g; c += QA_WARPS) {
+    const float2 all = qa_total(p, r, c);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t w0 = r.a; w0 <= r.b; w0 += 4) {
+      float4 v[4];
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t w = w0 + i <= r.b ? w0 + i : r.b;
+        const int64_t at = r.place(w) * p.cols + c;
+        v[i] = reinterpret_cast<const float4*>(p.part_o + at * Q4_D)[lane];
+        f[i] = w0 + i <= r.b ? fast_exp2(p.part_ml[at].x - all.x) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (w0 + i > r.b) break;
+        acc.x = fmaf(v[i].x, f[i], acc.x); acc.y = fmaf(v[i].y, f[i], acc.y);
+        acc.z = fmaf(v[i].z, f[i], acc.z); acc.w = fmaf(v[i].w, f[i], acc.w);
+      }
+    }
+    const float inv = all.y > 0.f ? 1.f / all.y : all.y == 0.f ? 0.f : all.y;
+    const int tok = c / p.g;
+    reinterpret_cast<uint2*>(p.out + (int64_t)(token + tok) * p.out_stride +
+                             (int64_t)(head * p.g + c - tok * p.g) * Q4_D)[lane] =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+}
+
+// One chunk of QA_THREADS cached tokens of a sequence and head: what its query tokens give each.
+__device__ __forceinline__ void qa_sums(const Q4AttnParams& p, int seq, int head, int chunk) {
+  __shared__ float2 ml[16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t0 = p.cu ? p.cu[seq] : seq;
+  const int t1 = p.cu ? min(p.cu[seq + 1], p.num_tokens) : seq + 1;
+  if (t0 < 0 || t0 >= t1) return;
+  const int key = chunk * QA_THREADS + threadIdx.x;
+  const int64_t from = p.from ? p.from[seq] : (int64_t)qa_len(p, t0) - 1;
+  float sum = 0.f;
+  bool seen = false;
+  for (int t = t0; t < t1; t += p.block) {
+    const int64_t steps = p.first[t + 1] - p.first[t];
+    if (steps * QA_STEP <= (int64_t)chunk * QA_THREADS) continue;
+    const int cols = min(p.block, t1 - t) * p.g;
+    const QaRuns r = qa_runs(p, t, head, steps);
+    __syncthreads();                         // the columns before have been read
+    for (int c = warp; c < cols; c += QA_WARPS) {
+      float2 v;
+      if (r.a == r.b) {
+        v = p.whole_ml[((int64_t)t * p.hkv + head) * p.cols + c];
+        if (v.x == -INFINITY) v.x = 0.f;
+      } else {
+        v = qa_total(p, r, c);
+      }
+      if (lane == 0) ml[c] = make_float2(v.x, v.y == 0.f ? 0.f : 1.f / v.y);
+    }
+    __syncthreads();
+    const int64_t x = r.px + key / QA_STEP;
+    if (key < steps * QA_STEP && x < p.logit_steps) {
+      seen = true;
+      const float* src = p.logits + (x * QA_STEP + key % QA_STEP) * p.cols;
+      for (int c = 0; c < cols; ++c) sum = fmaf(fast_exp2(src[c] - ml[c].x), ml[c].y, sum);
+    }
+  }
+  int most = 0;
+  for (int t = t0; t < t1; ++t) most = max(most, qa_len(p, t));
+  if (!seen || key >= most) return;
+  const int at = key / p.page;
+  const int page = p.tables[(int64_t)seq * p.table_stride + at];
+  if (page < 0 || page >= p.num_pages) return;             // flagged by the attention
+  float* w = p.weights + ((int64_t)page * p.hkv + head) * p.page + (key - at * p.page);
+  *w = key < from ? *w + sum : sum;
+}
+
+template <bool SUMS>
+__global__ void __launch_bounds__(QA_THREADS) q4_attn_join_kernel(const Q4AttnParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const unsigned joins = (unsigned)(p.num_tokens * p.hkv);
+  if (!SUMS || blockIdx.x < joins) {
+    qa_join(p, (int)blockIdx.x / p.hkv, (int)blockIdx.x % p.hkv);
+    return;
+  }
+  const unsigned b = blockIdx.x - joins;
+  const unsigned pair = b / p.chunks;
+  qa_sums(p, (int)(pair / p.hkv), (int)(pair % p.hkv), (int)(b % p.chunks));
+}
+
+struct QaLayout {
+  size_t first, part_ml, part_o, whole_ml, logits, total;
+  int64_t logit_steps;
+};
+static int qa_columns(int tokens, int seqs, int g, int* block) {
+  // query tokens of a sequence that go together: as many as 16 columns hold, and no more than
+  // there are on average
+  int n = 16 / g;
+  const int mean = seqs > 0 ? (tokens + seqs - 1) / seqs : 1;
+  if (n > mean) n = mean;
+  if (n < 1) n = 1;
+  *block = n;
+  return n * g;
+}
+static QaLayout qa_layout(int tokens, int seqs, int hkv, int g, bool sums, int64_t max_len) {
+  auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
+  int block;
+  const int cols = qa_columns(tokens, seqs, g, &block);
+  const size_t places = (size_t)sm_count() * 2 * QA_WARPS * 2;
+  QaLayout w{};
+  w.first = 256;
+  w.part_ml = w.first + up(((size_t)tokens + 1) * sizeof(int64_t));
+  w.part_o = w.part_ml + up(places * cols * sizeof(float2));
+  w.whole_ml = w.part_o + up(places * cols * Q4_D * sizeof(float));
+  w.logits = w.total = w.whole_ml;
+  if (sums) {
+    w.logits = w.whole_ml + up((size_t)tokens * hkv * cols * sizeof(float2));
+    const int64_t items = (int64_t)tokens / block + (block > 1 ? seqs : 0);
+    w.logit_steps = items * hkv * ((max_len + QA_STEP - 1) / QA_STEP);
+    w.total = w.logits + up((size_t)w.logit_steps * QA_STEP * cols * sizeof(float));
+  }
+  return w;
+}
+
+template <int NG, int NT, bool SUMS>
+static cudaError_t qa_launch(const Q4AttnParams& p, int grid, cudaStream_t s) {
+  using Shape = QaShape<NG, NT>;
+  static PerDeviceOnce once;
+  auto kernel = q4_attn_kernel<NG, NT, SUMS>;
+  const cudaError_t e = set_max_dynamic_smem(once, kernel, Shape::kSmem);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kernel, dim3(grid), dim3(QA_THREADS), (size_t)Shape::kSmem, s, p);
+}
+template <int NG, bool SUMS>
+static cudaError_t qa_launch(const Q4AttnParams& p, int sms, cudaStream_t s) {
+  return p.cols <= 8 ? qa_launch<NG, 1, SUMS>(p, sms * QaShape<NG, 1>::kCtas, s)
+                     : qa_launch<NG, 2, SUMS>(p, sms * QaShape<NG, 2>::kCtas, s);
+}
+
+}  // namespace fk
+
+using namespace fk;
+
+extern "C" {
+
+size_t fk_paged_decode_attn_q4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads,
+                                               int num_kv_heads, int head_dim, int with_weights,
+                                               int64_t max_context_len) {
+  if (num_tokens <= 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads ||
+      num_q_heads / num_kv_heads > 16 || head_dim != Q4_D || max_context_len < 0)
+    return 0;
+  return qa_layout(num_tokens, num_seqs, num_kv_heads, num_q_heads / num_kv_heads,
+                   with_weights != 0, max_context_len).total;
+}
+
+int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
+                            int64_t out_stride_token, const void* cache, int64_t num_pages,
+                            int page_size, int group, const int32_t* context_lens,
+                            const int32_t* block_tables, int64_t block_table_stride,
+                            int64_t block_table_cols, const int32_t* cu_seqlens_q, int num_seqs,
+                            int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                            float softmax_scale, float* weights, const int32_t* weights_from,
+                            int64_t max_context_len, void* workspace, size_t workspace_bytes,
+                            int32_t* status, fk_stream_t stream) {
+  static const char* what = "fk_paged_decode_attn_q4";
+  FK_REQUIRE(num_tokens >= 0 && num_seqs >= 0, FK_ERR_INVALID_ARG, "%s: negative size", what);
+  const int rc = q4_check_pool(what, cache, num_pages, page_size, num_kv_heads, head_dim, group);
+  if (rc != FK_OK) return rc;
+  if (num_tokens == 0 || num_seqs == 0) return FK_OK;
+  FK_REQUIRE(q && out && context_lens && block_tables, FK_ERR_INVALID_ARG, "%s: null pointer",
+             what);
+  FK_REQUIRE(num_q_heads > 0 && num_q_heads % num_kv_heads == 0, FK_ERR_INVALID_ARG,
+             "%s: num_q_heads must be a multiple of num_kv_heads", what);
+  const int g = num_q_heads / num_kv_heads;
+  FK_REQUIRE(g <= 16, FK_ERR_UNSUPPORTED, "%s: more than 16 query heads per KV head", what);
+  FK_REQUIRE(cu_seqlens_q != nullptr || num_seqs == num_tokens, FK_ERR_INVALID_ARG,
+             "%s: %d tokens of %d sequences need cu_seqlens_q", what, num_tokens, num_seqs);
+  FK_REQUIRE(block_table_cols > 0 && block_table_stride >= 0, FK_ERR_INVALID_ARG, "%s: bad sizes",
+             what);
+  FK_REQUIRE(q_stride_token >= (int64_t)num_q_heads * head_dim &&
+                 out_stride_token >= (int64_t)num_q_heads * head_dim,
+             FK_ERR_INVALID_ARG, "%s: token stride too small", what);
+  FK_REQUIRE(aligned16(q) && aligned16(out) && q_stride_token % 8 == 0 && out_stride_token % 8 == 0,
+             FK_ERR_ALIGNMENT, "%s: 16-byte alignment required", what);
+  FK_REQUIRE(max_context_len >= 0, FK_ERR_INVALID_ARG, "%s: negative size", what);
+  Q4AttnParams p{};
+  p.q = static_cast<const uint16_t*>(q); p.q_stride = q_stride_token;
+  p.out = static_cast<uint16_t*>(out); p.out_stride = out_stride_token;
+  p.pool = static_cast<const uint8_t*>(cache);
+  p.lens = context_lens; p.cu = cu_seqlens_q;
+  p.tables = block_tables; p.table_stride = block_table_stride;
+  p.capacity = block_table_cols < QA_LONGEST / page_size ? block_table_cols * page_size
+                                                         : QA_LONGEST;
+  p.num_tokens = num_tokens; p.num_seqs = num_seqs; p.num_pages = (int)num_pages;
+  p.page = page_size; p.hkv = num_kv_heads; p.g = g;
+  p.cols = qa_columns(num_tokens, num_seqs, g, &p.block);
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.status = status;
+  const bool sums = weights != nullptr;
+  if (sums && max_context_len < p.capacity) p.capacity = max_context_len;
+  const QaLayout w = qa_layout(num_tokens, num_seqs, num_kv_heads, g, sums, p.capacity);
+  FK_REQUIRE(workspace != nullptr && workspace_bytes >= w.total &&
+                 (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
+             FK_ERR_WORKSPACE, "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", what,
+             w.total, workspace_bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.run = reinterpret_cast<int64_t*>(ws);
+  p.first = reinterpret_cast<int64_t*>(ws + w.first);
+  p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  p.whole_ml = reinterpret_cast<float2*>(ws + w.whole_ml);
+  p.logits = reinterpret_cast<float*>(ws + w.logits);
+  p.logit_steps = w.logit_steps;
+  p.weights = weights; p.from = weights_from;
+  p.chunks = (int)((p.capacity + QA_THREADS - 1) / QA_THREADS);
+  const int64_t joins = (int64_t)num_tokens * num_kv_heads;
+  const int64_t blocks = joins + (sums ? (int64_t)num_seqs * num_kv_heads * p.chunks : 0);
+  FK_REQUIRE(blocks < (1ll << 31), FK_ERR_UNSUPPORTED, "%s: too many tokens", what);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int sms = sm_count();
+  const cudaError_t e =
+      sums ? group == 64 ? qa_launch<2, true>(p, sms, s) : qa_launch<1, true>(p, sms, s)
+           : group == 64 ? qa_launch<2, false>(p, sms, s) : qa_launch<1, false>(p, sms, s);
+  FK_CUDA_OK(e);
+  auto join = sums ? q4_attn_join_kernel<true> : q4_attn_join_kernel<false>;
+  FK_CUDA_OK(launch_kernel(join, dim3((unsigned)blocks), dim3(QA_THREADS), (size_t)0, s, p));
+  count_launch(2);
+  return FK_OK;
+}
+
+}  // extern "C"

@@ -633,6 +633,152 @@ def selected_attn(q, k_cache, v_cache, context_lens, block_tables, selected, blo
     return out
 
 
+# ----------------------------------------------------------- KV caches that take less memory
+_Q4_GROUPS = {2048 + 128 * (128 // g): g for g in (64, 128)}       # by the bytes of a unit
+
+
+def new_kvcache_q4(num_pages, page_size, num_kv_heads, head_dim=128, group=64, device="cuda"):
+    """A zeroed paged cache of 4 bits a value, uint8 [pages, Hkv, page // 16, bytes of 16 tokens];
+    keys and values share it.  `group` channels (64 or 128) have one scale: 144 or 136 bytes a token
+    and head, against 512 in bf16."""
+    unit = int(lib.fk_q4_unit_bytes(head_dim, group))
+    if unit == 0:
+        raise _lib.FkError(f"no 4-bit cache of heads of {head_dim} in groups of {group}")
+    if page_size < 16 or page_size % 16:
+        raise _lib.FkError("a page of a 4-bit cache is a multiple of 16 tokens")
+    return torch.zeros((num_pages, num_kv_heads, page_size // 16, unit), dtype=_UINT8,
+                       device=device)
+
+
+def _need_cache_q4(dev, cache) -> tuple[int, int, int, int]:
+    """(pages, page size, KV heads, group) of a 4-bit cache."""
+    if cache.dtype is not _UINT8 or cache.get_device() != dev:
+        _refuse("cache", cache, _UINT8, dev)
+    if cache.dim() != 4 or not cache.is_contiguous() or cache.shape[3] not in _Q4_GROUPS:
+        raise _lib.FkError("a 4-bit cache is a contiguous [pages, Hkv, page // 16, bytes of 16 "
+                           "tokens], as new_kvcache_q4 makes it")
+    pages, hkv, units, unit = cache.shape
+    return pages, 16 * units, hkv, _Q4_GROUPS[unit]
+
+
+def _need_slots(dev, t, numel=None) -> int:
+    """1 for int64 slots, 0 for int32."""
+    if t.dtype is not _INT32 and t.dtype is not torch.int64 or t.get_device() != dev:
+        _refuse("slot_mapping", t, _INT32, dev)
+    if t.dim() != 1 or not t.is_contiguous() or numel is not None and t.numel() != numel:
+        raise _lib.FkError("slot_mapping must be a dense vector"
+                           + (f" of {numel} entries" if numel is not None else ""))
+    return 0 if t.dtype is _INT32 else 1
+
+
+def store_kvcache_q4(key, value, cache, slot_mapping, status=None) -> None:
+    """store_kvcache into a cache of new_kvcache_q4: key / value bf16 [tokens, Hkv, 128] with dense
+    heads, slot_mapping int32 or int64, page * page_size + place, below 0 for none.  Each group of
+    channels is kept as its smallest value, a scale and 15 steps; one with a value that is not finite
+    reads back as NaN.  A slot appears once."""
+    dev = _device_of(cache)
+    pages, page, hkv, group = _need_cache_q4(dev, cache)
+    n, heads, d, ks = _need_rows(dev, key, "key")
+    if _need_rows(dev, value, "value")[:3] != (n, heads, d):
+        raise _lib.FkError("key and value differ in shape")
+    if heads != hkv:
+        raise _lib.FkError(f"the cache has {hkv} heads, key {heads}")
+    vs = _need_rows(dev, value, "value")[3]
+    wide = _need_slots(dev, slot_mapping, n)
+    check(lib.fk_store_kvcache_q4(
+        key.data_ptr(), ks, value.data_ptr(), vs, cache.data_ptr(), pages, page, hkv, d, group,
+        slot_mapping.data_ptr(), wide, n, _status_of(dev, status, cache), _stream_of(dev)),
+        "fk_store_kvcache_q4")
+
+
+def load_kvcache_q4(cache, slot_mapping, status=None):
+    """(key, value) bf16 [tokens, Hkv, 128] of slots of a 4-bit cache, zeros for a slot below 0:
+    what prefill_attn takes for a prompt whose first part is in the cache."""
+    dev = _device_of(cache)
+    pages, page, hkv, group = _need_cache_q4(dev, cache)
+    wide = _need_slots(dev, slot_mapping)
+    n = slot_mapping.numel()
+    key, value = (torch.empty((n, hkv, 128), dtype=BF16, device=cache.device) for _ in range(2))
+    check(lib.fk_load_kvcache_q4(
+        key.data_ptr(), value.data_ptr(), cache.data_ptr(), pages, page, hkv, 128, group,
+        slot_mapping.data_ptr(), wide, n, _status_of(dev, status, cache), _stream_of(dev)),
+        "fk_load_kvcache_q4")
+    return key, value
+
+
+def paged_decode_attn_q4_workspace_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                                         with_weights=False, max_context_len=0) -> int:
+    return int(lib.fk_paged_decode_attn_q4_workspace_bytes(
+        num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, int(with_weights),
+        max_context_len))
+
+
+def new_attn_weights(num_pages, page_size, num_kv_heads, device="cuda"):
+    """Zeroed sums of softmax weights of a paged pool's tokens, fp32 [pages, Hkv, page]."""
+    return torch.zeros((num_pages, num_kv_heads, page_size), dtype=torch.float32, device=device)
+
+
+def _need_weights(dev, weights, pages, hkv, page) -> None:
+    if weights.dtype is not torch.float32 or weights.get_device() != dev:
+        _refuse("weights", weights, torch.float32, dev)
+    if weights.shape != (pages, hkv, page) or not weights.is_contiguous():
+        raise _lib.FkError(f"weights must be a contiguous [{pages}, {hkv}, {page}], as "
+                           "new_attn_weights makes them")
+
+
+def _need_sequences(dev, n, cu_seqlens_q, weights_from, rows) -> int:
+    """Sequences of n query tokens: as many as tables."""
+    seqs = n if cu_seqlens_q is None else cu_seqlens_q.numel() - 1
+    if cu_seqlens_q is not None:
+        if seqs < 0:
+            raise _lib.FkError("cu_seqlens_q has the sequences' number and one more entries")
+        _need_ints(dev, seqs + 1, "cu_seqlens_q", cu_seqlens_q)
+    if weights_from is not None:
+        _need_ints(dev, seqs, "weights_from", weights_from)
+    if rows != seqs:
+        raise _lib.FkError(f"block_tables must have {seqs} rows, got {rows}")
+    return seqs
+
+
+def paged_decode_attn_q4(q, cache, context_lens, block_tables, softmax_scale, cu_seqlens_q=None,
+                         weights=None, weights_from=None, max_context_len=None, workspace=None,
+                         out=None, status=None):
+    """paged_decode_attn over a cache of new_kvcache_q4, for any GQA ratio up to 16 and one or several
+    query tokens of a sequence: tokens cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 (int32) are of the
+    sequence with row s of block_tables (None: one token a row).  context_lens int32 [tokens]: keys
+    that a token sees, itself among them.  Rows of `out` that belong to no sequence stay as they are.
+
+    weights (fp32, new_attn_weights): every token of the cache gets the softmax weights that all
+    query heads of its KV head and all query tokens here have for it added to its entry, in a fixed
+    order.  Entries from weights_from[s] (int32) on start from 0; without it, those from the first
+    query token's own on: what a new token's place held is forgotten.  A page belongs to one sequence
+    then.  evict_kvcache decides by these sums.
+
+    Without a workspace of paged_decode_attn_q4_workspace_bytes one is allocated here; with weights it
+    grows with max_context_len (default: what the tables hold), which no context may exceed."""
+    dev = _device_of(q)
+    pages, page, hkv, group = _need_cache_q4(dev, cache)
+    n, hq, d, qs = _need_rows(dev, q, "q")
+    _need_ints(dev, n, "context_lens", context_lens)
+    ts, cols, rows = _need_tables(dev, block_tables)
+    seqs = _need_sequences(dev, n, cu_seqlens_q, weights_from, rows)
+    longest = 0
+    if weights is not None:
+        _need_weights(dev, weights, pages, hkv, page)
+        longest = cols * page if max_context_len is None else min(max_context_len, cols * page)
+    out, os_ = _out_like(dev, q, out)
+    ws, ws_bytes, _held = _workspace(
+        dev, workspace,
+        _bytes_on(dev, "fk_paged_decode_attn_q4_workspace_bytes", n, seqs, hq, hkv, d,
+                  int(weights is not None), longest) if workspace is None else 0, q)
+    check(lib.fk_paged_decode_attn_q4(
+        q.data_ptr(), qs, out.data_ptr(), os_, cache.data_ptr(), pages, page, group,
+        context_lens.data_ptr(), block_tables.data_ptr(), ts, cols, _ptr(cu_seqlens_q), seqs, n, hq,
+        hkv, d, softmax_scale, _ptr(weights), _ptr(weights_from), longest, ws, ws_bytes,
+        _status_of(dev, status, q), _stream_of(dev)), "fk_paged_decode_attn_q4")
+    return out
+
+
 # --------------------------------------------------------------------------- norms
 def rmsnorm(x, weight, eps, out=None):
     """out = bf16(x * rsqrt(mean(x^2)+eps) * w); x is [..., cols], last dim dense.

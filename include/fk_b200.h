@@ -284,6 +284,70 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
                      fk_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * KV caches that take less memory (no counterpart in the reference): four bits a
+ * value, and tokens that leave.  bf16 rows, head_dim 128, page_size 16, 32 or a
+ * multiple of 64.
+ *
+ * A 4-bit cache is one pool [num_pages, num_kv_heads, page_size / 16] of units of
+ * fk_q4_unit_bytes: for 16 tokens of a head 64 bytes of codes of each key, then of
+ * each value, then for each key and each value the bf16 pair (scale, lowest) of every
+ * group of `group` (64 or 128) channels.  A 32-bit word holds 8 successive channels,
+ * the lowest in its lowest bits; word w lies at place w % 4 * 4 + w / 4 of a key's row
+ * and w % 8 * 2 + w / 8 of a value's.  Of a group with smallest value lo and largest hi
+ *   s = bf16(fp32(hi / 2 - lo / 2) / 7.5),  code = (x - lo) / s to the nearest integer
+ *   (even on ties), at most 15, 0 where s = 0;  it reads back as lo + s code,
+ * NaN throughout if one of its values is not finite.
+ *
+ * fk_store_kvcache_q4: token i's keys and values [num_tokens, num_kv_heads, 128]
+ * (heads dense) to slot slot_mapping[i] = page * page_size + place; below 0: none.
+ * fk_load_kvcache_q4: the other way, into dense rows; zeros for a slot below 0.  A slot
+ * at or past the pool's end is flagged FK_DEV_BAD_SLOT and taken as below 0.
+ *
+ * fk_paged_decode_attn_q4: attention of query token i over the first context_lens[i]
+ * tokens of its sequence, its own among them; block tables, softmax_scale and out as in
+ * fk_paged_decode_attn, up to 16 query heads per KV head.  cu_seqlens_q [num_seqs + 1]:
+ * tokens cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 are of sequence s, whose table is row
+ * s (NULL: one token each, num_seqs = num_tokens); tokens of no sequence are left out,
+ * and their rows of `out` as they were.  Tokens of one sequence share what is read, up to
+ * 16 query heads together.  A token without keys gets zeros.  Keys of a page whose id is
+ * bad are left out (FK_DEV_BAD_PAGE); a context beyond block_table_cols pages, or 2^30
+ * tokens, is cut there and flagged the same way.
+ * weights (NULL: none), fp32 [num_pages, num_kv_heads, page_size]: to the entry of
+ * every token that is seen the softmax weights of all query heads of the KV head and all
+ * query tokens of the sequence are added, in an order that does not change.  Entries from
+ * weights_from[s] on start from 0 (NULL: from the place of the sequence's first query
+ * token on, which no token before has seen).  A page is then in one table only.  Contexts
+ * of such a call are cut at max_context_len (flagged FK_DEV_BAD_PAGE); the workspace
+ * grows with it.
+ * ---------------------------------------------------------------------- */
+int64_t fk_q4_unit_bytes(int head_dim, int group);
+
+int fk_store_kvcache_q4(const void* k, int64_t k_stride_token, const void* v,
+                        int64_t v_stride_token, void* cache, int64_t num_pages, int page_size,
+                        int num_kv_heads, int head_dim, int group, const void* slot_mapping,
+                        int slots_are_int64, int64_t num_tokens, int32_t* status,
+                        fk_stream_t stream);
+
+int fk_load_kvcache_q4(void* k, void* v, const void* cache, int64_t num_pages, int page_size,
+                       int num_kv_heads, int head_dim, int group, const void* slot_mapping,
+                       int slots_are_int64, int64_t num_tokens, int32_t* status,
+                       fk_stream_t stream);
+
+size_t fk_paged_decode_attn_q4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads,
+                                               int num_kv_heads, int head_dim, int with_weights,
+                                               int64_t max_context_len);
+
+int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
+                            int64_t out_stride_token, const void* cache, int64_t num_pages,
+                            int page_size, int group, const int32_t* context_lens,
+                            const int32_t* block_tables, int64_t block_table_stride,
+                            int64_t block_table_cols, const int32_t* cu_seqlens_q, int num_seqs,
+                            int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                            float softmax_scale, float* weights, const int32_t* weights_from,
+                            int64_t max_context_len, void* workspace, size_t workspace_bytes,
+                            int32_t* status, fk_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * RMSNorm and fused residual-add + RMSNorm.
  * Replace RMSNorm.forward(x, residual=None)
  * (fastkernels/tasks/baseline/L1/rms_norm.py:153-164; kernels
