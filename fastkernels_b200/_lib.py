@@ -89,6 +89,14 @@ PROTOTYPES = {
     "fk_paged_decode_attn_q4": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _i64,
                                        _i64, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp,
                                        _i64, _vp, _sz, _vp, _vp]),
+    "fk_paged_decode_attn_weights_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i64]),
+    "fk_paged_decode_attn_weights": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32,
+                                            _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32,
+                                            _f32, _vp, _vp, _i64, _i32, _vp, _sz, _vp, _vp]),
+    "fk_evict_kvcache": (_i32, [_vp, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp,
+                                _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "fk_evict_kvcache_q4": (_i32, [_vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64,
+                                   _i64, _i32, _i32, _i32, _i32, _vp, _vp]),
     "fk_rmsnorm": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _f32, _i64, _i64,
                           _vp]),
     "fk_fused_add_rmsnorm": (_i32, [_vp, _i64, _vp, _i64, _vp, _f32, _i64, _i64, _vp]),

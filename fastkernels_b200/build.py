@@ -24,7 +24,7 @@ CORE_SOURCES = ["fk_host.cu", "fk_elementwise.cu", "fk_gemm.cu", "fk_prefill.cu"
                 "fk_gemm_large.cu", "fk_layers.cu", "fk_mixer.cu", "fk_residual.cu", "fk_group.cu",
                 "fk_plain.cu"]
 COMPONENT_SOURCES = {"decode_attn": ["fk_attn.cu", "fk_shared.cu", "fk_select.cu", "fk_q4.cu",
-                                     "fk_q4_attn.cu"],
+                                     "fk_q4_attn.cu", "fk_evict.cu"],
                      "delta": ["fk_delta.cu"],
                      "latent": ["fk_latent.cu"], "mlstm": ["fk_mlstm.cu"],
                      "experts": ["fk_moe.cu"], "comm": ["fk_comm.cu"], "block": ["fk_block.cu"]}

@@ -50,6 +50,7 @@ enum : int { TILE_FIRST = 1, TILE_LAST = 2, TILE_END = 4 };
 struct TileMeta {
   int seq, kvh, split, nsplits, n_valid, flags;
   uint32_t valid[2];        // selected blocks: valid tokens of each 16-token slab, a byte each
+                            // sums of weights: [0] the tile's first token
 };
 
 struct AttnSmem {
@@ -383,8 +384,8 @@ __device__ __forceinline__ void att_produce_selected(
 // main kernel
 // ---------------------------------------------------------------------------
 // SPLIT: the softmax weights enter P V as two bf16 parts (16 significant bits) instead
-// of one.  SEL: over selected blocks.
-template <bool G16, bool SPLIT, bool SEL>
+// of one.  SEL: over selected blocks.  SUMS: logits are kept, and every part's maximum and sum.
+template <bool G16, bool SPLIT, bool SEL, bool SUMS>
 __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
     const __grid_constant__ CUtensorMap tmap_k,
     const __grid_constant__ CUtensorMap tmap_v, const AttnParams p) {
@@ -504,7 +505,8 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
                                               (int64_t)kvh * p.g * ATT_D);
         for (int i = lane; i < p.g * ATT_D / 8; i += 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
       }
-      const int32_t* bt = p.block_tables + (int64_t)seq * p.bt_stride;
+      const int32_t* bt =
+          p.block_tables + (int64_t)(SUMS && p.rows ? p.rows[seq] : seq) * p.bt_stride;
       // this lane's piece of a tile starts `lane * st` tokens into it
       const int my = lane * st;
       // (not by way of L1 where no wait stands between the tables' last change and here)
@@ -533,7 +535,8 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
           m.seq = seq; m.kvh = kvh; m.split = split; m.nsplits = nsplits;
           m.n_valid = n_valid;
           m.flags = flags;
-          m.valid[0] = m.valid[1] = 0;
+          m.valid[0] = SUMS ? (uint32_t)tok0 : 0u;
+          m.valid[1] = 0;
           metas[stage] = m;
           uint32_t bytes = (uint32_t)ncopy * 4u * (uint32_t)st * 128u;
           if (flags & TILE_FIRST) bytes += (uint32_t)p.g * ATT_D * 2u;
@@ -687,6 +690,17 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
           const int col = nt * 8 + quad * 2 + (e & 1);
           t[nt][e] = col < nv ? s[nt][e] * p.scale_log2 : -INFINITY;
         }
+      if constexpr (SUMS) {
+        float* dst = p.logits + (((int64_t)meta.seq * p.hkv + meta.kvh) * p.logit_len +
+                                 meta.valid[0] + w * 16) * p.g;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < (G16 ? 4 : 2); ++e) {
+            const int col = nt * 8 + quad * 2 + (e & 1), r = row + 8 * (e >> 1);
+            if (col < nv && r < p.g) dst[(int64_t)col * p.g + r] = t[nt][e];
+          }
+      }
       float pa_f[2][4];
 #pragma unroll
       for (int h = 0; h < (G16 ? 2 : 1); ++h) {
@@ -844,6 +858,9 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
               for (int i = 0; i < 16; ++i)
                 dst[i * 4 + quad] =
                     pack_bf16(o[i][2 * h] * inv, o[i][2 * h + 1] * inv);
+              if (SUMS && quad == 0)
+                p.part_ml[((int64_t)meta.seq * p.hq + head) * p.max_splits] =
+                    make_float2(m_all[h], l_all[h]);
             } else {
               const int64_t pi =
                   ((int64_t)meta.seq * p.hq + head) * p.max_splits + meta.split;
@@ -868,15 +885,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
 // fastkernels/tasks/baseline/L1/triton_unified_attention.py:697-786:
 // empty total -> zeros)
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) attn_merge_kernel(const AttnParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  // the main kernel is done: clear its work counter so the same plan can serve
-  // the next layer of the step without re-running the plan kernel
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.plan[2] = 0;
-  const int gw = (int)((blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5);
-  const int lane = threadIdx.x & 31;
-  if (gw >= p.batch * p.hq) return;
+__device__ __forceinline__ void attn_merge_row(const AttnParams& p, int gw, int lane) {
   const int seq = gw / p.hq, head = gw - seq * p.hq;
   const int* chunk_start = p.plan + ATT_PLAN_HDR;
   const int n = chunk_start[seq + 1] - chunk_start[seq];
@@ -921,6 +930,98 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const AttnParams p) {
   const float inv = lt > 0.f ? 1.0f / lt : 0.f;
   *dst = make_uint2(pack_bf16(acc.x * inv, acc.y * inv),
                     pack_bf16(acc.z * inv, acc.w * inv));
+}
+__global__ void __launch_bounds__(256) attn_merge_kernel(const AttnParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  // the main kernel is done: clear its work counter so the same plan can serve
+  // the next layer of the step without re-running the plan kernel
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.plan[2] = 0;
+  const int gw = (int)((blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5);
+  if (gw >= p.batch * p.hq) return;
+  attn_merge_row(p, gw, threadIdx.x & 31);
+}
+
+// ---------------------------------------------------------------------------
+// sums of weights: what the query tokens of a sequence give each of its cached tokens,
+// sum over heads and tokens of 2^(logit - M) / sum, in the order of the tokens
+// ---------------------------------------------------------------------------
+// The table and the keys of each query token of the sequences in cu; none outside of all.
+__global__ void __launch_bounds__(256) attn_rows_kernel(const int32_t* __restrict__ cu, int num_seqs,
+                                                        const int32_t* __restrict__ context_lens,
+                                                        int batch, int32_t* rows, int32_t* lens) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= batch) return;
+  int lo = 0, hi = num_seqs;                  // the last sequence that begins at or before it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= i) lo = mid; else hi = mid;
+  }
+  const bool in = cu[lo] >= 0 && cu[lo] <= i && i < cu[lo + 1];
+  rows[i] = in ? lo : -1;
+  lens[i] = in ? context_lens[i] : 0;
+}
+
+// Rows to merge, a warp each, then chunks of 256 cached tokens of a sequence and KV head.
+__global__ void __launch_bounds__(256) attn_merge_sums_kernel(const AttnParams p, int merges) {
+  __shared__ float2 ml[16];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((int)blockIdx.x < merges) {
+    const int gw = blockIdx.x * 8 + warp;
+    // a row of no sequence stays as it is
+    if (gw < p.batch * p.hq && (!p.rows || p.rows[gw / p.hq] >= 0)) attn_merge_row(p, gw, lane);
+    return;
+  }
+  const unsigned b = blockIdx.x - merges;
+  const int chunk = (int)(b % p.sum_chunks);
+  const int pair = (int)(b / p.sum_chunks);
+  const int seq = pair / p.hkv, kvh = pair - seq * p.hkv;
+  const int t0 = p.cu ? p.cu[seq] : seq;
+  const int t1 = p.cu ? min(p.cu[seq + 1], p.batch) : seq + 1;
+  if (t0 < 0 || t0 >= t1) return;
+  const int key = chunk * 256 + threadIdx.x;
+  const int* chunk_start = p.plan + ATT_PLAN_HDR;
+  auto len_of = [&](int t) -> int64_t {
+    const int64_t n = p.context_lens[t];
+    return n < 0 ? 0 : n > p.capacity ? p.capacity : n;
+  };
+  const int64_t from = p.from ? p.from[seq] : len_of(t0) - 1;
+  float sum = 0.f;
+  bool seen = false;
+  for (int t = t0; t < t1; ++t) {
+    const int64_t len = len_of(t);
+    if (len <= (int64_t)chunk * 256) continue;
+    __syncthreads();                         // the token before has been added
+    for (int h = warp; h < p.g; h += 8) {
+      const float2* part = p.part_ml + ((int64_t)t * p.hq + kvh * p.g + h) * p.max_splits;
+      const int n = chunk_start[t + 1] - chunk_start[t];
+      float M = -INFINITY, L = 0.f;
+      for (int s = lane; s < n; s += 32) M = fmaxf(M, part[s].x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      if (M == -INFINITY) M = 0.f;
+      for (int s = lane; s < n; s += 32) L += part[s].y * fast_exp2(part[s].x - M);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      if (lane == 0) ml[h] = make_float2(M, L == 0.f ? 0.f : 1.f / L);
+    }
+    __syncthreads();
+    if (key < len) {
+      seen = true;
+      const float* z = p.logits + (((int64_t)t * p.hkv + kvh) * p.logit_len + key) * p.g;
+      for (int h = 0; h < p.g; ++h) sum = fmaf(fast_exp2(z[h] - ml[h].x), ml[h].y, sum);
+    }
+  }
+  if (!seen) return;
+  const int at = key / p.block_size;
+  const int page = p.block_tables[(int64_t)seq * p.bt_stride + at];
+  if (page < 0 || page >= p.num_blocks) return;            // flagged by the main kernel
+  float* w = p.weights + ((int64_t)page * p.hkv + kvh) * p.block_size + (key - at * p.block_size);
+  *w = key < from ? *w + sum : sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -1007,24 +1108,36 @@ int get_kv_map(const void* cache, int64_t num_blocks, int block_size, int hkv,
 
 cudaError_t launch_decode(bool g16, bool split, bool selected, int grid, const CUtensorMap& mk,
                           const CUtensorMap& mv, const AttnParams& p, cudaStream_t s) {
-  static PerDeviceOnce once[6];
+  static PerDeviceOnce once[8];
   auto go = [&](PerDeviceOnce& o, auto kernel) {
     const cudaError_t e = set_max_dynamic_smem(o, kernel, AttnSmem::kAlloc);
     if (e != cudaSuccess) return e;
     return launch_kernel(kernel, dim3(grid), dim3(ATT_THREADS), (size_t)AttnSmem::kAlloc, s, mk,
                          mv, p);
   };
-  if (selected) return g16 ? go(once[5], attn_decode_kernel<true, false, true>)
-                           : go(once[4], attn_decode_kernel<false, false, true>);
-  if (g16) return split ? go(once[3], attn_decode_kernel<true, true, false>)
-                        : go(once[1], attn_decode_kernel<true, false, false>);
-  return split ? go(once[2], attn_decode_kernel<false, true, false>)
-               : go(once[0], attn_decode_kernel<false, false, false>);
+  if (p.logits) return g16 ? go(once[7], attn_decode_kernel<true, false, false, true>)
+                           : go(once[6], attn_decode_kernel<false, false, false, true>);
+  if (selected) return g16 ? go(once[5], attn_decode_kernel<true, false, true, false>)
+                           : go(once[4], attn_decode_kernel<false, false, true, false>);
+  if (g16) return split ? go(once[3], attn_decode_kernel<true, true, false, false>)
+                        : go(once[1], attn_decode_kernel<true, false, false, false>);
+  return split ? go(once[2], attn_decode_kernel<false, true, false, false>)
+               : go(once[0], attn_decode_kernel<false, false, false, false>);
 }
 
 static size_t plan_hdr_bytes(int batch) {
   size_t b = (size_t)(ATT_PLAN_HDR + batch + 1) * sizeof(int);
   return (b + 255) & ~size_t(255);
+}
+// What sums of weights add to a call, and to its workspace.
+struct AttnSums {
+  float* weights; const int32_t* from; const int32_t* cu;
+  int num_seqs;
+  int64_t max_len;
+};
+static size_t sums_bytes(int batch, int num_q_heads, bool rows, int64_t max_len) {
+  const size_t logits = ((size_t)batch * num_q_heads * max_len * sizeof(float) + 255) & ~size_t(255);
+  return logits + (rows ? 2 * (size_t)batch * sizeof(int32_t) : 0);
 }
 static size_t plan_bytes(int batch, int max_splits) {
   size_t b = plan_hdr_bytes(batch) + (size_t)batch * max_splits * sizeof(int4);
@@ -1056,7 +1169,7 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
                          int num_q_heads, int num_kv_heads, int head_dim,
                          float softmax_scale, int max_splits, void* workspace,
                          size_t workspace_bytes, int32_t* status,
-                         fk_stream_t stream) {
+                         fk_stream_t stream, const AttnSums* sums = nullptr) {
   FK_REQUIRE(batch >= 0, FK_ERR_INVALID_ARG, "fk_paged_decode_attn: batch < 0");
   if (batch == 0) return FK_OK;
   FK_REQUIRE(context_lens && block_tables, FK_ERR_INVALID_ARG,
@@ -1092,8 +1205,12 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
   FK_REQUIRE(q_stride_token >= (int64_t)num_q_heads * head_dim &&
                  out_stride_token >= (int64_t)num_q_heads * head_dim,
              FK_ERR_INVALID_ARG, "fk_paged_decode_attn: token stride too small");
-  const size_t need = fk_paged_decode_attn_workspace_bytes(batch, num_q_heads,
-                                                           head_dim, max_splits);
+  const size_t main_bytes = (fk_paged_decode_attn_workspace_bytes(batch, num_q_heads, head_dim,
+                                                                  max_splits) + 255) & ~size_t(255);
+  const size_t need = !sums ? fk_paged_decode_attn_workspace_bytes(batch, num_q_heads, head_dim,
+                                                                   max_splits)
+                            : main_bytes + sums_bytes(batch, num_q_heads, sums->cu != nullptr,
+                                                      sums->max_len);
   FK_REQUIRE(workspace != nullptr && workspace_bytes >= need &&
                  (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
              FK_ERR_WORKSPACE,
@@ -1146,7 +1263,7 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
   // A small self-planning call (every (sequence, KV head) pair gets its own CTA and
   // no sequence is long enough to need splitting for bandwidth) runs as ONE launch:
   // no plan kernel, no partials, no merge.
-  const bool direct = mode == 0 && (int64_t)batch * num_kv_heads <= sm_count() &&
+  const bool direct = mode == 0 && !sums && (int64_t)batch * num_kv_heads <= sm_count() &&
                       block_table_stride * (int64_t)block_size <= 2048;
   p.direct = direct ? 1 : 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1159,6 +1276,27 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
   p.status = status;
 
   const int grid = sm_count();
+  int64_t capacity = block_table_stride * (int64_t)block_size;
+  if (sums) {
+    capacity = p.capacity = sums->max_len;
+    p.logits = reinterpret_cast<float*>(ws + main_bytes);
+    p.logit_len = sums->max_len;
+    p.weights = sums->weights; p.from = sums->from; p.cu = sums->cu;
+    p.num_seqs = sums->num_seqs;
+    p.sum_chunks = (int)((sums->max_len + 255) / 256);
+    FK_REQUIRE((int64_t)(batch + 7) * num_q_heads + (int64_t)p.num_seqs * num_kv_heads * p.sum_chunks <
+                   (1ll << 31),
+               FK_ERR_UNSUPPORTED, "fk_paged_decode_attn_weights: too many tokens");
+    if (sums->cu) {
+      int32_t* rows = reinterpret_cast<int32_t*>(
+          ws + main_bytes + sums_bytes(batch, num_q_heads, false, sums->max_len));
+      p.rows = rows;
+      p.context_lens = rows + batch;
+      FK_CUDA_OK(launch_kernel(attn_rows_kernel, dim3((batch + 255) / 256), dim3(256), (size_t)0, s,
+                               sums->cu, sums->num_seqs, context_lens, batch, rows, rows + batch));
+      count_launch(1);
+    }
+  }
 
   if (direct) {
     const int dgrid = batch * num_kv_heads;
@@ -1167,9 +1305,8 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
     return FK_OK;
   }
   if (mode != 2) {
-    FK_LAUNCH(attn_plan_kernel, dim3(1), dim3(1024), 0, s, context_lens, batch,
-              num_kv_heads, max_splits, grid, block_table_stride * (int64_t)block_size,
-              p.plan, p.chunk_info, status);
+    FK_LAUNCH(attn_plan_kernel, dim3(1), dim3(1024), 0, s, p.context_lens, batch,
+              num_kv_heads, max_splits, grid, capacity, p.plan, p.chunk_info, status);
     count_launch(1);
   }
   if (mode == 1) {
@@ -1178,6 +1315,14 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
   }
   FK_CUDA_OK(launch_decode(g > 8, split, false, grid, mk, mv, p, s));
   const int warps = batch * num_q_heads;
+  if (sums) {
+    const int merges = (warps + 7) / 8;
+    FK_CUDA_OK(launch_kernel(attn_merge_sums_kernel,
+                             dim3((unsigned)(merges + p.num_seqs * num_kv_heads * p.sum_chunks)),
+                             dim3(256), (size_t)0, s, p, merges));
+    count_launch(2);
+    return FK_OK;
+  }
   FK_LAUNCH(attn_merge_kernel, dim3((warps * 32 + 255) / 256), dim3(256), 0, s, p);
   count_launch(2);
   FK_CUDA_OK(cudaGetLastError());
@@ -1251,6 +1396,45 @@ int fk_paged_decode_attn_2p(int planned, const void* q, int64_t q_stride_token, 
                    v_cache, num_blocks, block_size, kv_block_stride, kv_layout, context_lens,
                    block_tables, block_table_stride, batch, num_q_heads, num_kv_heads, head_dim,
                    softmax_scale, max_splits, workspace, workspace_bytes, status, stream);
+}
+
+size_t fk_paged_decode_attn_weights_workspace_bytes(int num_tokens, int num_q_heads, int head_dim,
+                                                    int max_splits, int has_cu_seqlens,
+                                                    int64_t max_context_len) {
+  const size_t b = fk_paged_decode_attn_workspace_bytes(num_tokens, num_q_heads, head_dim,
+                                                        max_splits);
+  if (b == 0 || max_context_len < 0) return 0;
+  return ((b + 255) & ~size_t(255)) +
+         sums_bytes(num_tokens, num_q_heads, has_cu_seqlens != 0, max_context_len);
+}
+
+int fk_paged_decode_attn_weights(const void* q, int64_t q_stride_token, void* out,
+                                 int64_t out_stride_token, const void* k_cache,
+                                 const void* v_cache, int64_t num_blocks, int block_size,
+                                 int64_t kv_block_stride, int kv_layout,
+                                 const int32_t* context_lens, const int32_t* block_tables,
+                                 int64_t block_table_stride, int64_t block_table_cols,
+                                 const int32_t* cu_seqlens_q, int num_seqs, int num_tokens,
+                                 int num_q_heads, int num_kv_heads, int head_dim,
+                                 float softmax_scale, float* weights, const int32_t* weights_from,
+                                 int64_t max_context_len, int max_splits, void* workspace,
+                                 size_t workspace_bytes, int32_t* status, fk_stream_t stream) {
+  static const char* what = "fk_paged_decode_attn_weights";
+  FK_REQUIRE(num_tokens >= 0 && num_seqs >= 0 && max_context_len >= 0 && block_table_cols >= 0,
+             FK_ERR_INVALID_ARG, "%s: negative size", what);
+  if (num_tokens == 0 || num_seqs == 0) return FK_OK;
+  FK_REQUIRE(weights != nullptr, FK_ERR_INVALID_ARG, "%s: null pointer", what);
+  FK_REQUIRE(cu_seqlens_q != nullptr || num_seqs == num_tokens, FK_ERR_INVALID_ARG,
+             "%s: %d tokens of %d sequences need cu_seqlens_q", what, num_tokens, num_seqs);
+  FK_REQUIRE(block_size > 0 && block_table_cols > 0, FK_ERR_INVALID_ARG, "%s: bad sizes", what);
+  const int64_t most = 1ll << 30;
+  int64_t len = block_table_cols < most / block_size ? block_table_cols * block_size : most;
+  if (max_context_len < len) len = max_context_len;
+  const AttnSums sums{weights, weights_from, cu_seqlens_q, num_seqs, len};
+  return attn_impl(0, false, q, q_stride_token, out, out_stride_token, k_cache, v_cache, num_blocks,
+                   block_size, kv_block_stride, kv_layout, context_lens, block_tables,
+                   block_table_stride, num_tokens, num_q_heads, num_kv_heads, head_dim,
+                   softmax_scale, max_splits, workspace, workspace_bytes, status, stream, &sums);
 }
 
 }  // extern "C"

@@ -37,6 +37,13 @@ struct AttnParams {
   const int32_t* starts;    // groups of rows that a direct call only looks over
   int groups;
   int64_t unit;             // tiles of all tokens and heads, one after another, that a CTA takes
+  // sums of weights: `rows` as above; logits of every key that a token and KV head sees
+  float* logits;            // [batch, hkv, logit_len, g]
+  int64_t logit_len;
+  float* weights;           // [pages, hkv, block_size]
+  const int32_t* from;      // [sequences] first entry that starts from 0, null: the first token's own
+  const int32_t* cu;        // tokens of each sequence, null: one each
+  int num_seqs, sum_chunks;
 };
 
 

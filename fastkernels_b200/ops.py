@@ -679,11 +679,11 @@ def store_kvcache_q4(key, value, cache, slot_mapping, status=None) -> None:
     dev = _device_of(cache)
     pages, page, hkv, group = _need_cache_q4(dev, cache)
     n, heads, d, ks = _need_rows(dev, key, "key")
-    if _need_rows(dev, value, "value")[:3] != (n, heads, d):
+    *like, vs = _need_rows(dev, value, "value")
+    if like != [n, heads, d]:
         raise _lib.FkError("key and value differ in shape")
     if heads != hkv:
         raise _lib.FkError(f"the cache has {hkv} heads, key {heads}")
-    vs = _need_rows(dev, value, "value")[3]
     wide = _need_slots(dev, slot_mapping, n)
     check(lib.fk_store_kvcache_q4(
         key.data_ptr(), ks, value.data_ptr(), vs, cache.data_ptr(), pages, page, hkv, d, group,
@@ -776,6 +776,88 @@ def paged_decode_attn_q4(q, cache, context_lens, block_tables, softmax_scale, cu
         context_lens.data_ptr(), block_tables.data_ptr(), ts, cols, _ptr(cu_seqlens_q), seqs, n, hq,
         hkv, d, softmax_scale, _ptr(weights), _ptr(weights_from), longest, ws, ws_bytes,
         _status_of(dev, status, q), _stream_of(dev)), "fk_paged_decode_attn_q4")
+    return out
+
+
+def paged_decode_attn_weights_workspace_bytes(num_tokens, num_q_heads, head_dim, max_splits,
+                                              has_cu_seqlens=False, max_context_len=0) -> int:
+    return int(lib.fk_paged_decode_attn_weights_workspace_bytes(
+        num_tokens, num_q_heads, head_dim, max_splits, int(has_cu_seqlens), max_context_len))
+
+
+def paged_decode_attn_weights(q, k_cache, v_cache, context_lens, block_tables, softmax_scale, weights,
+                              cu_seqlens_q=None, weights_from=None, max_context_len=None,
+                              max_splits=None, workspace=None, out=None, status=None,
+                              kv_layout="NHD"):
+    """paged_decode_attn over bf16 pools that also adds to `weights` (new_attn_weights) what every
+    cached token is given, as paged_decode_attn_q4 does: cu_seqlens_q, weights_from, max_context_len
+    and the rows of `out` are as there.  GQA ratios 1, 2, 4, 8, 16.  Without a workspace of
+    paged_decode_attn_weights_workspace_bytes one is allocated here."""
+    dev = _device_of(q)
+    pages, page, hkv, d2, stride = _need_caches(dev, k_cache, v_cache, kv_layout)
+    n, hq, d, qs = _need_rows(dev, q, "q")
+    if d2 != d:
+        raise _lib.FkError("cache shape mismatch")
+    _need_ints(dev, n, "context_lens", context_lens)
+    ts, cols, rows = _need_tables(dev, block_tables)
+    seqs = _need_sequences(dev, n, cu_seqlens_q, weights_from, rows)
+    _need_weights(dev, weights, pages, hkv, page)
+    longest = cols * page if max_context_len is None else min(max_context_len, cols * page)
+    if max_splits is None:
+        max_splits = max_splits_for(longest)
+    out, os_ = _out_like(dev, q, out)
+    ws, ws_bytes, _held = _workspace(
+        dev, workspace,
+        _bytes_on(dev, "fk_paged_decode_attn_weights_workspace_bytes", n, hq, d, max_splits,
+                  int(cu_seqlens_q is not None), longest) if workspace is None else 0, q)
+    check(lib.fk_paged_decode_attn_weights(
+        q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
+        stride, 1 if kv_layout == "HND" else 0, context_lens.data_ptr(), block_tables.data_ptr(),
+        ts, cols, _ptr(cu_seqlens_q), seqs, n, hq, hkv, d, softmax_scale, weights.data_ptr(),
+        _ptr(weights_from), longest, max_splits, ws, ws_bytes, _status_of(dev, status, q),
+        _stream_of(dev)), "fk_paged_decode_attn_weights")
+    return out
+
+
+def evict_kvcache(caches, weights, context_lens, block_tables, budget, keep_first=0, keep_last=0,
+                  kv_layout="NHD", out=None, status=None):
+    """Cuts every sequence of more than `budget` tokens to as many, per KV head, and returns the new
+    context lengths (int32, in `out` where given).  The first keep_first and the last keep_last
+    tokens stay, and of the others those with the largest entries in `weights`, the lower place on
+    ties.  caches: (k_cache, v_cache) in bf16, or a cache of new_kvcache_q4.
+
+    Rows move within the sequence's pages, and their entries of `weights` with them: with M = budget -
+    keep_last, the i-th token that stays from place M on takes the i-th place below M that became
+    free, and the last keep_last follow in order.  Keys carry their positions, so attention does not
+    mind the order; the next token goes to place `budget`, with its true position.  A page belongs
+    to one sequence, and a sequence appears once; pages behind the budget may be given back."""
+    dev = _device_of(weights)
+    q4 = torch.is_tensor(caches)
+    if q4:
+        pages, page, hkv, group = _need_cache_q4(dev, caches)
+    else:
+        k_cache, v_cache = caches
+        pages, page, hkv, d, stride = _need_caches(dev, k_cache, v_cache, kv_layout)
+    _need_weights(dev, weights, pages, hkv, page)
+    n = context_lens.numel()
+    _need_ints(dev, n, "context_lens", context_lens)
+    ts, cols, rows = _need_tables(dev, block_tables)
+    if rows != n:
+        raise _lib.FkError(f"block_tables must have {n} rows, got {rows}")
+    if out is None:
+        out = torch.empty_like(context_lens)
+    else:
+        _need_ints(dev, n, "out", out)
+    common = (weights.data_ptr(), context_lens.data_ptr(), out.data_ptr(), block_tables.data_ptr(),
+              ts, cols, n, budget, keep_first, keep_last, _status_of(dev, status, weights),
+              _stream_of(dev))
+    if q4:
+        check(lib.fk_evict_kvcache_q4(caches.data_ptr(), pages, page, hkv, 128, group, *common),
+              "fk_evict_kvcache_q4")
+    else:
+        check(lib.fk_evict_kvcache(k_cache.data_ptr(), v_cache.data_ptr(), pages, page, stride,
+                                   1 if kv_layout == "HND" else 0, hkv, d, *common),
+              "fk_evict_kvcache")
     return out
 
 

@@ -319,6 +319,22 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
  * token on, which no token before has seen).  A page is then in one table only.  Contexts
  * of such a call are cut at max_context_len (flagged FK_DEV_BAD_PAGE); the workspace
  * grows with it.
+ *
+ * fk_paged_decode_attn_weights: the same over bf16 pools, for num_q_heads / num_kv_heads
+ * 1, 2, 4, 8 or 16; the keys of a bad page are zeros, as in fk_paged_decode_attn, and have
+ * no entry.  Launches: [tables of the tokens,] schedule, attention, merge and sums.
+ *
+ * fk_evict_kvcache (bf16 pools), fk_evict_kvcache_q4: of every sequence of more than
+ * `budget` tokens and each of its KV heads `budget` tokens stay: the first keep_first, the
+ * last keep_last, and of those between the ones with the largest entries of weights, the
+ * lower place on ties (an entry that is no number counts as -infinity).  With M = budget -
+ * keep_last: tokens that stay and are below place M stay there; the i-th of those from M on
+ * goes to the i-th place below M that became free, the last keep_last go, in order, to
+ * M .. budget - 1; entries of weights go with them.  The order of keys means nothing to
+ * attention; which place a token has may differ from head to head.  Nothing behind
+ * `budget` is changed.  new_context_lens[s] = min(context_lens[s], budget), a buffer of its
+ * own.  A page is in one table only; a token whose page id is bad counts as 0 and does not
+ * move (FK_DEV_BAD_PAGE).  One launch.
  * ---------------------------------------------------------------------- */
 int64_t fk_q4_unit_bytes(int head_dim, int group);
 
@@ -346,6 +362,36 @@ int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
                             float softmax_scale, float* weights, const int32_t* weights_from,
                             int64_t max_context_len, void* workspace, size_t workspace_bytes,
                             int32_t* status, fk_stream_t stream);
+
+size_t fk_paged_decode_attn_weights_workspace_bytes(int num_tokens, int num_q_heads, int head_dim,
+                                                    int max_splits, int has_cu_seqlens,
+                                                    int64_t max_context_len);
+
+int fk_paged_decode_attn_weights(const void* q, int64_t q_stride_token, void* out,
+                                 int64_t out_stride_token, const void* k_cache,
+                                 const void* v_cache, int64_t num_blocks, int block_size,
+                                 int64_t kv_block_stride, int kv_layout,
+                                 const int32_t* context_lens, const int32_t* block_tables,
+                                 int64_t block_table_stride, int64_t block_table_cols,
+                                 const int32_t* cu_seqlens_q, int num_seqs, int num_tokens,
+                                 int num_q_heads, int num_kv_heads, int head_dim,
+                                 float softmax_scale, float* weights, const int32_t* weights_from,
+                                 int64_t max_context_len, int max_splits, void* workspace,
+                                 size_t workspace_bytes, int32_t* status, fk_stream_t stream);
+
+int fk_evict_kvcache(void* k_cache, void* v_cache, int64_t num_pages, int page_size,
+                     int64_t kv_page_stride, int kv_layout, int num_kv_heads, int head_dim,
+                     float* weights, const int32_t* context_lens, int32_t* new_context_lens,
+                     const int32_t* block_tables, int64_t block_table_stride,
+                     int64_t block_table_cols, int num_seqs, int budget, int keep_first,
+                     int keep_last, int32_t* status, fk_stream_t stream);
+
+int fk_evict_kvcache_q4(void* cache, int64_t num_pages, int page_size, int num_kv_heads,
+                        int head_dim, int group, float* weights, const int32_t* context_lens,
+                        int32_t* new_context_lens, const int32_t* block_tables,
+                        int64_t block_table_stride, int64_t block_table_cols, int num_seqs,
+                        int budget, int keep_first, int keep_last, int32_t* status,
+                        fk_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * RMSNorm and fused residual-add + RMSNorm.
