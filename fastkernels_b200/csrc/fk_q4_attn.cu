@@ -87,6 +87,16 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same onto nothing.
+__device__ __forceinline__ void mma_f16_16816_first(float (&c)[4], uint32_t a0, uint32_t a1,
+                                                    uint32_t a2, uint32_t a3, uint32_t b0,
+                                                    uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -133,25 +143,33 @@ __device__ __forceinline__ QaItem qa_item(const Q4AttnParams& p, int token) {
   return it;
 }
 
-// A place in the row of all steps.
-struct QaCursor {
+// A step in the row of all steps.  `begins`: steps before the first of each thread's `per` tokens.
+struct QaPlace {
   int token, head, step;
   QaItem it;
-  __device__ __forceinline__ void next(const Q4AttnParams& p) {
-    if (++step < it.steps) return;
-    step = 0;
-    if (++head < p.hkv) return;
-    head = 0;
-    do {
-      if (++token >= p.num_tokens) {          // not reached while the lengths stay as they are
-        token = 0;
-        it = QaItem{0, 0, 0, 1 << 30};
-        return;
-      }
-      it = qa_item(p, token);
-    } while (it.steps == 0);
-  }
 };
+__device__ __forceinline__ QaPlace qa_locate(const Q4AttnParams& p, const int64_t* begins, int per,
+                                             int64_t x) {
+  const int64_t at = x >> 31 ? x / p.hkv : (int64_t)((uint32_t)x / (uint32_t)p.hkv);
+  int lo = 0, hi = QA_THREADS;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (begins[mid] <= at) lo = mid; else hi = mid;
+  }
+  int64_t before = begins[lo];
+  QaPlace r;
+  r.token = min(lo * per, p.num_tokens - 1);
+  r.it = qa_item(p, r.token);
+  while (r.token + 1 < p.num_tokens && before + r.it.steps <= at) {
+    before += r.it.steps;
+    r.it = qa_item(p, ++r.token);
+  }
+  const int64_t in = x - before * p.hkv;      // below steps * hkv
+  const int steps = max(r.it.steps, 1);
+  r.head = (int)(in >> 31 ? in / steps : (int64_t)((uint32_t)in / (uint32_t)steps));
+  r.step = (int)(in - (int64_t)r.head * steps);
+  return r;
+}
 
 template <int NG, int NT>
 struct QaShape {
@@ -225,105 +243,70 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
   const int64_t x0 = me * run, x1 = min(total, x0 + run);
   if (x0 >= x1) return;
 
-  QaCursor now;                                            // the step that is computed
-  {
-    const int64_t at = x0 / p.hkv;
-    int lo = 0, hi = QA_THREADS;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (begins[mid] <= at) lo = mid; else hi = mid;
-    }
-    int64_t before = begins[lo];
-    int i = min(lo * per, p.num_tokens - 1);
-    now.it = qa_item(p, i);
-    while (i + 1 < p.num_tokens && before + now.it.steps <= at) {
-      before += now.it.steps;
-      now.it = qa_item(p, ++i);
-    }
-    now.token = i;
-    const int64_t in = x0 - before * p.hkv;
-    const int steps = max(now.it.steps, 1);
-    now.head = (int)(in / steps);
-    now.step = (int)(in - (int64_t)now.head * steps);
-  }
-  QaCursor ahead = now;                                    // the step that is copied
-
   uint8_t* ring = ring_all + warp * DEPTH * S::kStage;
   uint64_t* full = bars[warp];
   const int units = p.page / Q4_UNIT;                      // of a page
-  // pages of 32 steps, a lane each: the page and the unit in it (pages of one unit: the next page)
-  int pg_row = -1, pg_base = 0, pg_a = -1, pg_b = -1;
-  int nx_a = -1, nx_b = -1;
-  auto look_up = [&](int base, int& a, int& b) {
-    const int64_t t = (int64_t)(base + lane) * QA_STEP;
-    a = b = -1;
-    if (t >= ahead.it.len) return;
-    const int32_t* table = p.tables + (int64_t)ahead.it.row * p.table_stride;
-    const int at = (int)t / p.page;
-    a = table[at];
-    if (units > 1) b = ((int)t - at * p.page) / Q4_UNIT;
-    else if (t + Q4_UNIT < ahead.it.len) b = table[at + 1];
-  };
-  uint32_t present = 0;                                    // two bits a slot: its units
-  auto copy = [&](int slot) {
-    const int base = ahead.step & ~31;
-    if (pg_row != ahead.token || base != pg_base) {
-      if (pg_row == ahead.token && base == pg_base + 32) {
-        pg_a = nx_a; pg_b = nx_b;
-      } else {
-        look_up(base, pg_a, pg_b);
-      }
-      pg_row = ahead.token; pg_base = base;
-      look_up(base + 32, nx_a, nx_b);
+  const int count = (int)(x1 - x0);
+  // Copies are looked up 32 at a time, a lane each: the step's units of the pool (-1: none), and
+  // for all lanes which are there, of these 32 steps and of those before.
+  int unit_a = -1, unit_b = -1;
+  uint32_t have_a = 0, have_b = 0, had_a = 0, had_b = 0;
+  auto look_up = [&](int k) {
+    had_a = have_a; had_b = have_b;
+    unit_a = unit_b = -1;
+    if (k + lane < count) {
+      const QaPlace r = qa_locate(p, begins, per, x0 + k + lane);
+      const int t = r.step * QA_STEP, left = r.it.len - t;
+      const int32_t* table = p.tables + (int64_t)r.it.row * p.table_stride;
+      const int at = t / p.page;
+      const int a = left > 0 ? table[at] : 0;
+      const int b = units == 1 && left > Q4_UNIT ? table[at + 1] : a;
+      if (left > 0 && a >= 0 && a < p.num_pages)
+        unit_a = (a * p.hkv + r.head) * units + (t - at * p.page) / Q4_UNIT;
+      if (left > Q4_UNIT && b >= 0 && b < p.num_pages)
+        unit_b = units == 1 ? b * p.hkv + r.head : unit_a + 1;
+      if (p.status && ((left > 0 && unit_a < 0) || (left > Q4_UNIT && unit_b < 0)))
+        atomicOr(p.status, FK_DEV_BAD_PAGE);
     }
-    const int a = __shfl_sync(0xffffffffu, pg_a, ahead.step & 31);
-    const int b = __shfl_sync(0xffffffffu, pg_b, ahead.step & 31);
-    const int left = ahead.it.len - ahead.step * QA_STEP;
-    const int want = left > Q4_UNIT ? 3 : left > 0 ? 1 : 0;
-    int have = a >= 0 && a < p.num_pages ? units > 1 ? 3 : 1 : 0;
-    if (units == 1 && b >= 0 && b < p.num_pages) have |= 2;
-    have &= want;
-    present = (present & ~(3u << (2 * slot))) | (uint32_t)have << (2 * slot);
-    if (lane == 0) {
-      if (have != want && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-      mbar_arrive_expect_tx(&full[slot], __popc(have) * S::kUnit);
+    have_a = __ballot_sync(0xffffffffu, unit_a >= 0);
+    have_b = __ballot_sync(0xffffffffu, unit_b >= 0);
+  };
+  auto copy = [&](int k, int slot) {
+    if ((k & 31) == 0) look_up(k);
+    if (lane == (k & 31)) {
       uint8_t* dst = ring + slot * S::kStage;
-      if (units > 1) {
-        if (have)
-          bulk_load(dst, p.pool + (((int64_t)a * p.hkv + ahead.head) * units + b) * S::kUnit,
-                    __popc(have) * S::kUnit, &full[slot]);
+      uint64_t* bar = &full[slot];
+      const int n = (unit_a >= 0) + (unit_b >= 0);
+      mbar_arrive_expect_tx(bar, n * S::kUnit);
+      if (n == 2 && unit_b == unit_a + 1) {                // side by side in the pool
+        bulk_load(dst, p.pool + (int64_t)unit_a * S::kUnit, 2 * S::kUnit, bar);
       } else {
-        if (have & 1)
-          bulk_load(dst, p.pool + ((int64_t)a * p.hkv + ahead.head) * S::kUnit, S::kUnit,
-                    &full[slot]);
-        if (have & 2)
-          bulk_load(dst + S::kUnit, p.pool + ((int64_t)b * p.hkv + ahead.head) * S::kUnit,
-                    S::kUnit, &full[slot]);
+        if (unit_a >= 0) bulk_load(dst, p.pool + (int64_t)unit_a * S::kUnit, S::kUnit, bar);
+        if (unit_b >= 0)
+          bulk_load(dst + S::kUnit, p.pool + (int64_t)unit_b * S::kUnit, S::kUnit, bar);
       }
     }
-    __syncwarp();
-    ahead.next(p);
   };
-  const int64_t count = x1 - x0;
-  for (int i = 0; i < DEPTH && i < count; ++i) copy(i);
+  for (int k = 0; k < DEPTH && k < count; ++k) copy(k, k);
 
   // ---- state of a pair: columns 8 nt + 2 quad + {0, 1} ----
   uint32_t qf[NT][8][2];
   float o[8][NT][4];
-  float m[NT][2], l[NT][2], low[NG][NT][2];   // maximum, sum of weights, sum of weights' lowest
+  // weights are 2^(logit - ref); logits above `limit` raise it; sums of weights, and of weights' lowest
+  float ref[NT][2], limit[NT][2], l[NT][2], low[NG][NT][2];
   float factor[NT][2], qsum[NG][NT][2];       // of logits: of a product, of a token's lowest
   int len[NT][2];
-  int shortest = 0;
   float vref = 0.f, vinv = 0.f;
 
   bool ok = true;
-  int slot = 0;
+  int slot = 0, i = 0;
   uint32_t phase = 0;
-  int64_t x = x0;
-  for (; x < x1; ++x) {
-    if (x == x0 || now.step == 0) {
-      // ---------------------------------------------------------------- a new pair
-      shortest = 0x7fffffff;
+  while (ok && i < count) {
+    // ---------------------------------------------------------------- a new pair
+    const QaPlace now = qa_locate(p, begins, per, x0 + i);
+    const int begin = i, last = i + max(1, min(now.it.steps - now.step, count - i));
+    int shortest = 0x7fffffff;
+    {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int col = nt * 8 + row;
@@ -388,8 +371,8 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr)
             qsum[gr][nt][j] = __shfl_sync(0xffffffffu, sum[gr], from) * p.scale_log2;
-          m[nt][j] = -INFINITY;
-          l[nt][j] = 0.f;
+          limit[nt][j] = -INFINITY;
+          ref[nt][j] = l[nt][j] = 0.f;
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] = 0.f;
         }
@@ -401,275 +384,286 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
       vref = vinv = 0.f;
     }
 
-    if (!qa_wait_warp(&full[slot], phase)) {
-      if (lane == 0 && p.status) atomicOr(p.status, FK_DEV_WAIT_TIMEOUT);
-      ok = false;
-      break;
-    }
-    const uint8_t* st = ring + slot * S::kStage;
-    const uint32_t have = present >> (2 * slot) & 3u;
-    const int tok0 = now.step * QA_STEP;
+    const int step0 = now.step - i;                        // of the pair, at i = 0
+    for (; i < last; ++i) {
+      if (!qa_wait_warp(&full[slot], phase)) {
+        if (lane == 0 && p.status) atomicOr(p.status, FK_DEV_WAIT_TIMEOUT);
+        ok = false;
+        break;
+      }
+      const uint8_t* st = ring + slot * S::kStage;
+      // copies are up to DEPTH steps on, perhaps among the next 32
+      const bool next = (min(i + DEPTH, count) - 1) >> 5 != i >> 5;
+      const uint32_t have = ((next ? had_a : have_a) >> (i & 31) & 1u) |
+                            ((next ? had_b : have_b) >> (i & 31) & 1u) << 1;
+      const int tok0 = (step0 + i) * QA_STEP;
+      const bool edge = tok0 + QA_STEP > shortest || have != 3u;
 
-    // ---- logits: rows are tokens row, row + 8 of unit u ----
-    float z[2][NT][4];                                      // [unit][.][row 0: 2 columns, row 8: 2]
-    float vs[2][NG][2], vl[2][NG][2];                       // the values' scale and lowest
-    const bool edge = tok0 + QA_STEP > shortest || have != 3u;
+      // ---- logits: rows are tokens row, row + 8 of unit u ----
+      float z[2][NT][4];                                    // [unit][.][row 0: 2 columns, row 8: 2]
+      float vs[2][NG][2], vl[2][NG][2];                     // the values' scale and lowest
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint8_t* un = st + u * S::kUnit;
-      const uint4 ka = *reinterpret_cast<const uint4*>(un + row * Q4_ROW + quad * 16);
-      const uint4 kb = *reinterpret_cast<const uint4*>(un + (row + 8) * Q4_ROW + quad * 16);
-      uint32_t kp[2][NG], vp[2][NG];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(un + Q4_PAIRS);
-        if constexpr (NG == 2) {
-          const uint2 a = *reinterpret_cast<const uint2*>(pairs + (row + 8 * r) * 2);
-          const uint2 b = *reinterpret_cast<const uint2*>(pairs + (Q4_UNIT + row + 8 * r) * 2);
-          kp[r][0] = a.x; kp[r][1] = a.y; vp[r][0] = b.x; vp[r][1] = b.y;
-        } else {
-          kp[r][0] = pairs[row + 8 * r];
-          vp[r][0] = pairs[Q4_UNIT + row + 8 * r];
-        }
-      }
-      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-      float acc[NG][NT][4];
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          acc[gr][nt][0] = acc[gr][nt][1] = acc[gr][nt][2] = acc[gr][nt][3] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t ya = wa[i] >> 8, yb = wb[i] >> 8;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_f16_16816(acc[i * NG / 4][nt], wa[i] & 0x000f000fu, wb[i] & 0x000f000fu,
-                        wa[i] & 0x00f000f0u, wb[i] & 0x00f000f0u, qf[nt][2 * i][0],
-                        qf[nt][2 * i][1]);
-          mma_f16_16816(acc[i * NG / 4][nt], ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
-                        yb & 0x00f000f0u, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float t = bf16lo(kp[e >> 1][0]) * acc[0][nt][e];
-          float b = bf16hi(kp[e >> 1][0]) * qsum[0][nt][e & 1];
-          if constexpr (NG == 2) {
-            t = fmaf(bf16lo(kp[e >> 1][1]), acc[1][nt][e], t);
-            b = fmaf(bf16hi(kp[e >> 1][1]), qsum[1][nt][e & 1], b);
-          }
-          z[u][nt][e] = fmaf(t, factor[nt][e & 1], b);
-        }
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          vs[u][gr][r] = bf16lo(vp[r][gr]);
-          vl[u][gr][r] = bf16hi(vp[r][gr]);
-        }
-      if (edge) {
-        // what stands behind the context is any number, or none
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* un = st + u * S::kUnit;
+        const uint4 ka = *reinterpret_cast<const uint4*>(un + row * Q4_ROW + quad * 16);
+        const uint4 kb = *reinterpret_cast<const uint4*>(un + (row + 8) * Q4_ROW + quad * 16);
+        uint32_t kp[2][NG], vp[2][NG];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int t = tok0 + u * Q4_UNIT + row + 8 * r;
-          const bool there = (have >> u & 1u) && t < now.it.len;
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr)
-            if (!there) vs[u][gr][r] = vl[u][gr][r] = 0.f;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (!there || t >= len[nt][j]) z[u][nt][2 * r + j] = -INFINITY;
+          const uint32_t* pairs = reinterpret_cast<const uint32_t*>(un + Q4_PAIRS);
+          if constexpr (NG == 2) {
+            const uint2 a = *reinterpret_cast<const uint2*>(pairs + (row + 8 * r) * 2);
+            const uint2 b = *reinterpret_cast<const uint2*>(pairs + (Q4_UNIT + row + 8 * r) * 2);
+            kp[r][0] = a.x; kp[r][1] = a.y; vp[r][0] = b.x; vp[r][1] = b.y;
+          } else {
+            kp[r][0] = pairs[row + 8 * r];
+            vp[r][0] = pairs[Q4_UNIT + row + 8 * r];
+          }
         }
-      }
-      if constexpr (SUMS) {
-        if (x < p.logit_steps) {
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        float acc[NG][NT][4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t ya = wa[w] >> 8, yb = wb[w] >> 8;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float (&c)[4] = acc[w * NG / 4][nt];
+            const uint32_t a0 = wa[w] & 0x000f000fu, a1 = wb[w] & 0x000f000fu;
+            const uint32_t a2 = wa[w] & 0x00f000f0u, a3 = wb[w] & 0x00f000f0u;
+            if (w % (4 / NG) == 0)
+              mma_f16_16816_first(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+            else
+              mma_f16_16816(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+            mma_f16_16816(c, ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
+                          yb & 0x00f000f0u, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float t = bf16lo(kp[e >> 1][0]) * acc[0][nt][e];
+            float b = bf16hi(kp[e >> 1][0]) * qsum[0][nt][e & 1];
+            if constexpr (NG == 2) {
+              t = fmaf(bf16lo(kp[e >> 1][1]), acc[1][nt][e], t);
+              b = fmaf(bf16hi(kp[e >> 1][1]), qsum[1][nt][e & 1], b);
+            }
+            z[u][nt][e] = fmaf(t, factor[nt][e & 1], b);
+          }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            vs[u][gr][r] = bf16lo(vp[r][gr]);
+            vl[u][gr][r] = bf16hi(vp[r][gr]);
+          }
+        if (edge) {
+          // what stands behind the context is any number, or none
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float* dst = p.logits + (x * QA_STEP + u * Q4_UNIT + row + 8 * r) * p.cols;
+            const int t = tok0 + u * Q4_UNIT + row + 8 * r;
+            const bool there = (have >> u & 1u) && t < now.it.len;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const int c = nt * 8 + 2 * quad;
-              if (c + 1 < p.cols && (p.cols & 1) == 0) {
-                *reinterpret_cast<float2*>(dst + c) =
-                    make_float2(z[u][nt][2 * r], z[u][nt][2 * r + 1]);
-              } else {
-                if (c < p.cols) dst[c] = z[u][nt][2 * r];
-                if (c + 1 < p.cols) dst[c + 1] = z[u][nt][2 * r + 1];
+            for (int gr = 0; gr < NG; ++gr)
+              if (!there) vs[u][gr][r] = vl[u][gr][r] = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (!there || t >= len[nt][j]) z[u][nt][2 * r + j] = -INFINITY;
+          }
+        }
+        if constexpr (SUMS) {
+          if (x0 + i < p.logit_steps) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float* dst = p.logits + ((x0 + i) * QA_STEP + u * Q4_UNIT + row + 8 * r) * p.cols;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const int c = nt * 8 + 2 * quad;
+                if (c + 1 < p.cols && (p.cols & 1) == 0) {
+                  *reinterpret_cast<float2*>(dst + c) =
+                      make_float2(z[u][nt][2 * r], z[u][nt][2 * r + 1]);
+                } else {
+                  if (c < p.cols) dst[c] = z[u][nt][2 * r];
+                  if (c + 1 < p.cols) dst[c + 1] = z[u][nt][2 * r + 1];
+                }
               }
             }
           }
         }
       }
-    }
 
-    // ---- new references, if a logit or a scale has left the old ones behind ----
-    bool beyond = false;
-    float vmax = 0.f;
+      // ---- new references, if a logit or a scale has left the old ones behind ----
+      float vmax = 0.f, top[NT][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) vmax = fmaxf(vmax, vs[u][gr][r]);
+          for (int gr = 0; gr < NG; ++gr) vmax = fmaxf(vmax, vs[u][gr][r]);
+      bool beyond = vmax > vref;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          top[nt][j] = fmaxf(fmaxf(z[0][nt][j], z[0][nt][2 + j]), fmaxf(z[1][nt][j], z[1][nt][2 + j]));
+          beyond |= top[nt][j] > limit[nt][j];
+        }
+      if (__any_sync(0xffffffffu, beyond)) {
+#pragma unroll
+        for (int sh = 4; sh < 32; sh <<= 1)
+          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
+        float vnew = vref;
+        if (vmax > vref)                                    // the power of two above
+          vnew = fmaxf(__uint_as_float(((__float_as_uint(vmax) >> 23) + 1u) << 23), 1e-30f);
+        const float vshift = vref > 0.f ? vref / vnew : 0.f;
+        vref = vnew;
+        vinv = vnew > 0.f ? 64.f / vnew : 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) beyond |= z[u][nt][2 * r + j] > m[nt][j] + QA_SLACK;
-      }
-    beyond |= vmax > vref;
-    if (__any_sync(0xffffffffu, beyond)) {
-#pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
-      float vnew = vref;
-      if (vmax > vref)                                      // the power of two above
-        vnew = fmaxf(__uint_as_float(((__float_as_uint(vmax) >> 23) + 1u) << 23), 1e-30f);
-      const float vshift = vref > 0.f ? vref / vnew : 0.f;
-      vref = vnew;
-      vinv = vnew > 0.f ? 64.f / vnew : 0.f;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float mx = fmaxf(fmaxf(z[0][nt][j], z[0][nt][2 + j]), fmaxf(z[1][nt][j], z[1][nt][2 + j]));
-#pragma unroll
-          for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-          const float old = m[nt][j], next = fmaxf(old, mx);
-          const float alpha = old == next ? 1.f : fast_exp2(old - next);
-          m[nt][j] = next;
-          l[nt][j] *= alpha;
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] *= alpha;
-#pragma unroll
-          for (int mt = 0; mt < 8; ++mt) {
-            o[mt][nt][j] *= alpha * vshift;
-            o[mt][nt][2 + j] *= alpha * vshift;
-          }
-        }
-    }
-
-    // ---- weights, and the operand P^T ----
-    uint32_t pt[2][NG][NT][2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float w[2];
-#pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
-            w[j] = fast_exp2(z[u][nt][2 * r + j] - ref);
-            l[nt][j] += w[j];
+            float mx = top[nt][j];
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] = fmaf(w[j], vl[u][gr][r], low[gr][nt][j]);
-          }
+            for (int sh = 4; sh < 32; sh <<= 1)
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+            const float old = limit[nt][j] == -INFINITY ? -INFINITY : ref[nt][j];
+            float alpha = 1.f;
+            if (mx > old) {
+              alpha = fast_exp2(old - mx);
+              ref[nt][j] = mx;
+              limit[nt][j] = mx + QA_SLACK;
+            }
+            l[nt][j] *= alpha;
 #pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-            const float f = vs[u][gr][r] * vinv;
-            pt[u][gr][nt][r] = transpose_8x8(pack_f16(w[0] * f, w[1] * f));
-          }
-        }
-
-    // ---- O^T += V^T P^T: rows are channels, of lane `row` 8 row + {0 .. 7} (+ 64) ----
+            for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] *= alpha;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint8_t* un = st + u * S::kUnit + Q4_VALUES + row * 8;
-      const uint2 a0 = *reinterpret_cast<const uint2*>(un + (2 * quad) * Q4_ROW);
-      const uint2 a1 = *reinterpret_cast<const uint2*>(un + (2 * quad + 1) * Q4_ROW);
-      const uint2 b0 = *reinterpret_cast<const uint2*>(un + (2 * quad + 8) * Q4_ROW);
-      const uint2 b1 = *reinterpret_cast<const uint2*>(un + (2 * quad + 9) * Q4_ROW);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t wa0 = h ? a0.y : a0.x, wa1 = h ? a1.y : a1.x;
-        const uint32_t wb0 = h ? b0.y : b0.x, wb1 = h ? b1.y : b1.x;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // channels 4 half .. 4 half + 3 of the word, of two tokens side by side
-          uint32_t xa = __byte_perm(wa0, wa1, half ? 0x7632 : 0x5410);
-          uint32_t xb = __byte_perm(wb0, wb1, half ? 0x7632 : 0x5410);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int mt = 4 * h + 2 * half + k;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_f16_16816(o[mt][nt], xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu,
-                            xb & 0x00f000f0u, pt[u][h * NG / 2][nt][0], pt[u][h * NG / 2][nt][1]);
-            xa >>= 8;
-            xb >>= 8;
-          }
-        }
-      }
-    }
-    __syncwarp();
-    if (x + DEPTH < x1) copy(slot);
-    if (++slot == DEPTH) { slot = 0; phase ^= 1; }
-
-    if (now.step + 1 == now.it.steps || x + 1 == x1) {
-      // ---------------------------------------------------------------- the pair's end
-      const int64_t px = x - now.step, pe = px + now.it.steps;
-      const bool whole = px >= x0 && pe <= x1;
-      const int64_t place = 2 * me + (px > x0 ? 1 : 0);
-      const float vback = vref * (1.f / 64.f);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float sum = l[nt][j], lows[NG];
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) lows[gr] = low[gr][nt][j];
-#pragma unroll
-          for (int sh = 4; sh < 32; sh <<= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, sh);
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
-              lows[gr] += __shfl_xor_sync(0xffffffffu, lows[gr], sh);
-          }
-          const int col = nt * 8 + 2 * quad + j;
-          const int tok = col / p.g;
-          if (tok >= now.it.tokens) continue;
-          const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              v[c] = fmaf(o[4 * h + (c >> 1)][nt][(c & 1) * 2 + j] * vback,
-                          (c & 1) ? 1048576.f : 16777216.f, lows[h * NG / 2]);
-            if (whole) {
-              uint4 w;
-              w.x = pack_bf16(v[0] * inv, v[1] * inv);
-              w.y = pack_bf16(v[2] * inv, v[3] * inv);
-              w.z = pack_bf16(v[4] * inv, v[5] * inv);
-              w.w = pack_bf16(v[6] * inv, v[7] * inv);
-              *reinterpret_cast<uint4*>(p.out + (int64_t)(now.token + tok) * p.out_stride +
-                                        (int64_t)(now.head * p.g + col - tok * p.g) * Q4_D +
-                                        64 * h + 8 * row) = w;
-            } else {
-              float4* dst = reinterpret_cast<float4*>(p.part_o + (place * p.cols + col) * Q4_D +
-                                                      64 * h + 8 * row);
-              dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-              dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            for (int mt = 0; mt < 8; ++mt) {
+              o[mt][nt][j] *= alpha * vshift;
+              o[mt][nt][2 + j] *= alpha * vshift;
             }
           }
-          if (row == 0) {
-            if (!whole) p.part_ml[place * p.cols + col] = make_float2(m[nt][j], sum);
-            else if (SUMS)
-              p.whole_ml[((int64_t)now.token * p.hkv + now.head) * p.cols + col] =
-                  make_float2(m[nt][j], sum);
+      }
+
+      // ---- weights, and the operand P^T ----
+      uint32_t pt[2][NG][NT][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float w[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              w[j] = fast_exp2(z[u][nt][2 * r + j] - ref[nt][j]);
+              l[nt][j] += w[j];
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr)
+                low[gr][nt][j] = fmaf(w[j], vl[u][gr][r], low[gr][nt][j]);
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+              const float f = vs[u][gr][r] * vinv;
+              pt[u][gr][nt][r] = transpose_8x8(pack_f16(w[0] * f, w[1] * f));
+            }
+          }
+
+      // ---- O^T += V^T P^T: rows are channels, of lane `row` 8 row + {0 .. 7} (+ 64) ----
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* un = st + u * S::kUnit + Q4_VALUES + row * 8;
+        const uint2 a0 = *reinterpret_cast<const uint2*>(un + (2 * quad) * Q4_ROW);
+        const uint2 a1 = *reinterpret_cast<const uint2*>(un + (2 * quad + 1) * Q4_ROW);
+        const uint2 b0 = *reinterpret_cast<const uint2*>(un + (2 * quad + 8) * Q4_ROW);
+        const uint2 b1 = *reinterpret_cast<const uint2*>(un + (2 * quad + 9) * Q4_ROW);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t wa0 = h ? a0.y : a0.x, wa1 = h ? a1.y : a1.x;
+          const uint32_t wb0 = h ? b0.y : b0.x, wb1 = h ? b1.y : b1.x;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            // channels 4 half .. 4 half + 3 of the word, of two tokens side by side
+            uint32_t xa = __byte_perm(wa0, wa1, half ? 0x7632 : 0x5410);
+            uint32_t xb = __byte_perm(wb0, wb1, half ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int mt = 4 * h + 2 * half + k;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_f16_16816(o[mt][nt], xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu,
+                              xb & 0x00f000f0u, pt[u][h * NG / 2][nt][0],
+                              pt[u][h * NG / 2][nt][1]);
+              xa >>= 8;
+              xb >>= 8;
+            }
           }
         }
+      }
+      __syncwarp();
+      if (i + DEPTH < count) copy(i + DEPTH, slot);
+      if (++slot == DEPTH) { slot = 0; phase ^= 1; }
     }
-    now.next(p);
+
+    if (!ok) break;
+    // ------------------------------------------------------------------- the pair's end
+    const bool whole = now.step == 0 && step0 + i == now.it.steps;
+    const int64_t place = 2 * me + (begin > 0 ? 1 : 0);
+    const float vback = vref * (1.f / 64.f);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = l[nt][j], lows[NG];
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) lows[gr] = low[gr][nt][j];
+#pragma unroll
+        for (int sh = 4; sh < 32; sh <<= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr)
+            lows[gr] += __shfl_xor_sync(0xffffffffu, lows[gr], sh);
+        }
+        const int col = nt * 8 + 2 * quad + j;
+        const int tok = col / p.g;
+        if (tok >= now.it.tokens) continue;
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            v[c] = fmaf(o[4 * h + (c >> 1)][nt][(c & 1) * 2 + j] * vback,
+                        (c & 1) ? 1048576.f : 16777216.f, lows[h * NG / 2]);
+          if (whole) {
+            uint4 w;
+            w.x = pack_bf16(v[0] * inv, v[1] * inv);
+            w.y = pack_bf16(v[2] * inv, v[3] * inv);
+            w.z = pack_bf16(v[4] * inv, v[5] * inv);
+            w.w = pack_bf16(v[6] * inv, v[7] * inv);
+            *reinterpret_cast<uint4*>(p.out + (int64_t)(now.token + tok) * p.out_stride +
+                                      (int64_t)(now.head * p.g + col - tok * p.g) * Q4_D + 64 * h +
+                                      8 * row) = w;
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + (place * p.cols + col) * Q4_D +
+                                                    64 * h + 8 * row);
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+          }
+        }
+        if (row == 0) {
+          const float m = limit[nt][j] == -INFINITY ? -INFINITY : ref[nt][j];
+          if (!whole) p.part_ml[place * p.cols + col] = make_float2(m, sum);
+          else if (SUMS)
+            p.whole_ml[((int64_t)now.token * p.hkv + now.head) * p.cols + col] =
+                make_float2(m, sum);
+        }
+      }
   }
   if (!ok) {
     // copies still on their way end before the shared memory goes
-    for (int i = 0; i < DEPTH && i < x1 - x; ++i) {
+    for (int k = 0; k < DEPTH && k < count - i; ++k) {
       (void)qa_wait_warp(&full[slot], phase);
       if (++slot == DEPTH) { slot = 0; phase ^= 1; }
     }
@@ -913,6 +907,8 @@ int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
   FK_REQUIRE(aligned16(q) && aligned16(out) && q_stride_token % 8 == 0 && out_stride_token % 8 == 0,
              FK_ERR_ALIGNMENT, "%s: 16-byte alignment required", what);
   FK_REQUIRE(max_context_len >= 0, FK_ERR_INVALID_ARG, "%s: negative size", what);
+  FK_REQUIRE(num_pages * num_kv_heads < (1ll << 31) / (page_size / Q4_UNIT), FK_ERR_UNSUPPORTED,
+             "%s: pool too large", what);
   Q4AttnParams p{};
   p.q = static_cast<const uint16_t*>(q); p.q_stride = q_stride_token;
   p.out = static_cast<uint16_t*>(out); p.out_stride = out_stride_token;
