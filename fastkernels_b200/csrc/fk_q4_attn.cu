@@ -81,7 +81,7 @@ __device__ __forceinline__ bool qa_wait_warp(uint64_t* bar, uint32_t parity) {
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                               uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -91,7 +91,7 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32
 __device__ __forceinline__ void mma_f16_16816_first(float (&c)[4], uint32_t a0, uint32_t a1,
                                                     uint32_t a2, uint32_t a3, uint32_t b0,
                                                     uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -99,7 +99,7 @@ __device__ __forceinline__ void mma_f16_16816_first(float (&c)[4], uint32_t a0, 
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 // Two fp32 to fp16, lo = a.
@@ -171,21 +171,26 @@ __device__ __forceinline__ QaPlace qa_locate(const Q4AttnParams& p, const int64_
   return r;
 }
 
-template <int NG, int NT>
+// Columns of a warp's products.  Of up to 4 there are two sets side by side: one for the step's
+// first 16 tokens, one for the others, so that what is done per logit is done once per 32 tokens
+// and not on empty columns.
+template <int NG, int COLS>
 struct QaShape {
+  static constexpr int kFold = COLS == 4 ? 2 : 1;          // units side by side
+  static constexpr int kTiles = COLS == 16 ? 2 : 1;        // of 8 columns
   static constexpr int kUnit = q4_unit_bytes(NG);
   static constexpr int kStage = 2 * kUnit;
-  static constexpr int kCtas = NT == 1 ? 2 : 1;            // of an SM
-  static constexpr int kDepth = NT == 1 ? 3 : 6;           // steps of a warp's ring
+  static constexpr int kCtas = COLS == 16 ? 1 : 2;         // of an SM
+  static constexpr int kDepth = COLS == 16 ? 6 : 3;        // steps of a warp's ring
   static constexpr int kSmem = QA_WARPS * kDepth * kStage;
 };
 
-// NG groups a row; NT * 8 columns; SUMS: logits are kept for the sums of weights.
-template <int NG, int NT, bool SUMS>
-__global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
+// NG groups a row; SUMS: logits are kept for the sums of weights.
+template <int NG, int COLS, bool SUMS>
+__global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
     q4_attn_kernel(const Q4AttnParams p) {
-  using S = QaShape<NG, NT>;
-  constexpr int DEPTH = S::kDepth;
+  using S = QaShape<NG, COLS>;
+  constexpr int DEPTH = S::kDepth, NT = S::kTiles, FOLD = S::kFold, SETS = 2 / FOLD;
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ uint64_t bars[QA_WARPS][DEPTH];
   __shared__ int64_t begins[QA_THREADS + 1];               // steps before each thread's tokens
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
     {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int col = nt * 8 + row;
+        const int col = nt * 8 + (FOLD == 2 ? row & 3 : row);
         const int tok = col / p.g;
         const bool live = tok < now.it.tokens;
         uint4 w[4];
@@ -399,18 +404,47 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
       const int tok0 = (step0 + i) * QA_STEP;
       const bool edge = tok0 + QA_STEP > shortest || have != 3u;
 
-      // ---- logits: rows are tokens row, row + 8 of unit u ----
-      float z[2][NT][4];                                    // [unit][.][row 0: 2 columns, row 8: 2]
-      float vs[2][NG][2], vl[2][NG][2];                     // the values' scale and lowest
+      // ---- logits: rows are tokens row, row + 8 of unit `lu` ----
+      float z[SETS][NT][4];                                 // [set][.][row: 2 columns, row + 8: 2]
+      float vs[SETS][NG][2], vl[SETS][NG][2];               // the values' scale and lowest
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint8_t* un = st + u * S::kUnit;
-        const uint4 ka = *reinterpret_cast<const uint4*>(un + row * Q4_ROW + quad * 16);
-        const uint4 kb = *reinterpret_cast<const uint4*>(un + (row + 8) * Q4_ROW + quad * 16);
+      for (int u = 0; u < SETS; ++u) {
+        const int lu = FOLD == 2 ? quad >> 1 : u;
+        float acc[2 / SETS][NG][NT][4];
+#pragma unroll
+        for (int f = 0; f < FOLD; ++f) {
+          const uint8_t* un = st + (u + f) * S::kUnit;
+          const uint4 ka = *reinterpret_cast<const uint4*>(un + row * Q4_ROW + quad * 16);
+          const uint4 kb = *reinterpret_cast<const uint4*>(un + (row + 8) * Q4_ROW + quad * 16);
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t ya = wa[w] >> 8, yb = wb[w] >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float (&c)[4] = acc[f][w * NG / 4][nt];
+              const uint32_t a0 = wa[w] & 0x000f000fu, a1 = wb[w] & 0x000f000fu;
+              const uint32_t a2 = wa[w] & 0x00f000f0u, a3 = wb[w] & 0x00f000f0u;
+              if (w % (4 / NG) == 0)
+                mma_f16_16816_first(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              else
+                mma_f16_16816(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              mma_f16_16816(c, ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
+                            yb & 0x00f000f0u, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+            }
+          }
+        }
+        if constexpr (FOLD == 2) {
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[0][gr][0][e] = lu ? acc[1][gr][0][e] : acc[0][gr][0][e];
+        }
         uint32_t kp[2][NG], vp[2][NG];
+        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(st + lu * S::kUnit + Q4_PAIRS);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t* pairs = reinterpret_cast<const uint32_t*>(un + Q4_PAIRS);
           if constexpr (NG == 2) {
             const uint2 a = *reinterpret_cast<const uint2*>(pairs + (row + 8 * r) * 2);
             const uint2 b = *reinterpret_cast<const uint2*>(pairs + (Q4_UNIT + row + 8 * r) * 2);
@@ -420,32 +454,14 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
             vp[r][0] = pairs[Q4_UNIT + row + 8 * r];
           }
         }
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-        float acc[NG][NT][4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t ya = wa[w] >> 8, yb = wb[w] >> 8;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float (&c)[4] = acc[w * NG / 4][nt];
-            const uint32_t a0 = wa[w] & 0x000f000fu, a1 = wb[w] & 0x000f000fu;
-            const uint32_t a2 = wa[w] & 0x00f000f0u, a3 = wb[w] & 0x00f000f0u;
-            if (w % (4 / NG) == 0)
-              mma_f16_16816_first(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
-            else
-              mma_f16_16816(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
-            mma_f16_16816(c, ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
-                          yb & 0x00f000f0u, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
-          }
-        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float t = bf16lo(kp[e >> 1][0]) * acc[0][nt][e];
+            float t = bf16lo(kp[e >> 1][0]) * acc[0][0][nt][e];
             float b = bf16hi(kp[e >> 1][0]) * qsum[0][nt][e & 1];
             if constexpr (NG == 2) {
-              t = fmaf(bf16lo(kp[e >> 1][1]), acc[1][nt][e], t);
+              t = fmaf(bf16lo(kp[e >> 1][1]), acc[0][1][nt][e], t);
               b = fmaf(bf16hi(kp[e >> 1][1]), qsum[1][nt][e & 1], b);
             }
             z[u][nt][e] = fmaf(t, factor[nt][e & 1], b);
@@ -461,8 +477,8 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
           // what stands behind the context is any number, or none
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int t = tok0 + u * Q4_UNIT + row + 8 * r;
-            const bool there = (have >> u & 1u) && t < now.it.len;
+            const int t = tok0 + lu * Q4_UNIT + row + 8 * r;
+            const bool there = (have >> lu & 1u) && t < now.it.len;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr)
               if (!there) vs[u][gr][r] = vl[u][gr][r] = 0.f;
@@ -477,10 +493,10 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
           if (x0 + i < p.logit_steps) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              float* dst = p.logits + ((x0 + i) * QA_STEP + u * Q4_UNIT + row + 8 * r) * p.cols;
+              float* dst = p.logits + ((x0 + i) * QA_STEP + lu * Q4_UNIT + row + 8 * r) * p.cols;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                const int c = nt * 8 + 2 * quad;
+                const int c = FOLD == 2 ? 2 * (quad & 1) : nt * 8 + 2 * quad;
                 if (c + 1 < p.cols && (p.cols & 1) == 0) {
                   *reinterpret_cast<float2*>(dst + c) =
                       make_float2(z[u][nt][2 * r], z[u][nt][2 * r + 1]);
@@ -497,7 +513,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
       // ---- new references, if a logit or a scale has left the old ones behind ----
       float vmax = 0.f, top[NT][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < SETS; ++u)
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -507,12 +523,15 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          top[nt][j] = fmaxf(fmaxf(z[0][nt][j], z[0][nt][2 + j]), fmaxf(z[1][nt][j], z[1][nt][2 + j]));
+          top[nt][j] = fmaxf(z[0][nt][j], z[0][nt][2 + j]);
+          if constexpr (SETS == 2)
+            top[nt][j] = fmaxf(top[nt][j], fmaxf(z[1][nt][j], z[1][nt][2 + j]));
           beyond |= top[nt][j] > limit[nt][j];
         }
       if (__any_sync(0xffffffffu, beyond)) {
+        constexpr int kFrom = FOLD == 2 ? 2 : 4;            // lanes of the same column, and its twin
 #pragma unroll
-        for (int sh = 4; sh < 32; sh <<= 1)
+        for (int sh = kFrom; sh < 32; sh <<= 1)
           vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
         float vnew = vref;
         if (vmax > vref)                                    // the power of two above
@@ -526,7 +545,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
           for (int j = 0; j < 2; ++j) {
             float mx = top[nt][j];
 #pragma unroll
-            for (int sh = 4; sh < 32; sh <<= 1)
+            for (int sh = kFrom; sh < 32; sh <<= 1)
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
             const float old = limit[nt][j] == -INFINITY ? -INFINITY : ref[nt][j];
             float alpha = 1.f;
@@ -549,7 +568,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
       // ---- weights, and the operand P^T ----
       uint32_t pt[2][NG][NT][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < SETS; ++u)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -566,7 +585,13 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
               const float f = vs[u][gr][r] * vinv;
-              pt[u][gr][nt][r] = transpose_8x8(pack_f16(w[0] * f, w[1] * f));
+              const uint32_t x = transpose_8x8(pack_f16(w[0] * f, w[1] * f));
+              if constexpr (FOLD == 2) {
+                pt[0][gr][nt][r] = row < 4 ? x : 0u;
+                pt[1][gr][nt][r] = row < 4 ? 0u : x;
+              } else {
+                pt[u][gr][nt][r] = x;
+              }
             }
           }
 
@@ -619,11 +644,19 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, NT>::kCtas))
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) lows[gr] = low[gr][nt][j];
 #pragma unroll
-        for (int sh = 4; sh < 32; sh <<= 1) {
+        for (int sh = FOLD == 2 ? 2 : 4; sh < 32; sh <<= 1) {
           sum += __shfl_xor_sync(0xffffffffu, sum, sh);
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr)
             lows[gr] += __shfl_xor_sync(0xffffffffu, lows[gr], sh);
+        }
+        if constexpr (FOLD == 2) {
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            o[mt][nt][j] += __shfl_xor_sync(0xffffffffu, o[mt][nt][j], 2);
+            o[mt][nt][2 + j] += __shfl_xor_sync(0xffffffffu, o[mt][nt][2 + j], 2);
+          }
+          if (quad > 1) continue;
         }
         const int col = nt * 8 + 2 * quad + j;
         const int tok = col / p.g;
@@ -846,19 +879,21 @@ static QaLayout qa_layout(int tokens, int seqs, int hkv, int g, bool sums, int64
   return w;
 }
 
-template <int NG, int NT, bool SUMS>
-static cudaError_t qa_launch(const Q4AttnParams& p, int grid, cudaStream_t s) {
-  using Shape = QaShape<NG, NT>;
+template <int NG, int COLS, bool SUMS>
+static cudaError_t qa_launch(const Q4AttnParams& p, int sms, cudaStream_t s) {
+  using Shape = QaShape<NG, COLS>;
   static PerDeviceOnce once;
-  auto kernel = q4_attn_kernel<NG, NT, SUMS>;
+  auto kernel = q4_attn_kernel<NG, COLS, SUMS>;
   const cudaError_t e = set_max_dynamic_smem(once, kernel, Shape::kSmem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(grid), dim3(QA_THREADS), (size_t)Shape::kSmem, s, p);
+  return launch_kernel(kernel, dim3(sms * Shape::kCtas), dim3(QA_THREADS), (size_t)Shape::kSmem, s,
+                       p);
 }
 template <int NG, bool SUMS>
 static cudaError_t qa_launch(const Q4AttnParams& p, int sms, cudaStream_t s) {
-  return p.cols <= 8 ? qa_launch<NG, 1, SUMS>(p, sms * QaShape<NG, 1>::kCtas, s)
-                     : qa_launch<NG, 2, SUMS>(p, sms * QaShape<NG, 2>::kCtas, s);
+  return p.cols <= 4 ? qa_launch<NG, 4, SUMS>(p, sms, s)
+                     : p.cols <= 8 ? qa_launch<NG, 8, SUMS>(p, sms, s)
+                                   : qa_launch<NG, 16, SUMS>(p, sms, s);
 }
 
 }  // namespace fk
