@@ -31,6 +31,8 @@ namespace fk {
 constexpr int QA_WARPS = 8;
 constexpr int QA_THREADS = QA_WARPS * 32;
 constexpr int QA_STEP = 32;                  // tokens of a warp's step
+constexpr int QA_AHEAD = 16;                 // steps that are looked up at a time
+constexpr float QA_NONE = -3e38f;            // reference before there is a key
 constexpr float QA_SLACK = 8.f;              // logits may be this far above the maximum (log2)
 constexpr int64_t QA_LONGEST = 1ll << 30;    // tokens of a context
 
@@ -195,6 +197,8 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
   __shared__ uint64_t bars[QA_WARPS][DEPTH];
   __shared__ int64_t begins[QA_THREADS + 1];               // steps before each thread's tokens
   __shared__ int64_t sums[QA_WARPS];
+  __shared__ int2 where[QA_WARPS][2 * QA_AHEAD];           // units of a step in the pool, -1: none
+  __shared__ QaPlace places[QA_WARPS];                     // of the pair a warp is at
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = lane & 3, row = lane >> 2;
   if (lane == 0) {
@@ -252,43 +256,39 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
   uint64_t* full = bars[warp];
   const int units = p.page / Q4_UNIT;                      // of a page
   const int count = (int)(x1 - x0);
-  // Copies are looked up 32 at a time, a lane each: the step's units of the pool (-1: none), and
-  // for all lanes which are there, of these 32 steps and of those before.
-  int unit_a = -1, unit_b = -1;
-  uint32_t have_a = 0, have_b = 0, had_a = 0, had_b = 0;
+  // Copies are looked up QA_AHEAD steps at a time, a lane for each unit.
   auto look_up = [&](int k) {
-    had_a = have_a; had_b = have_b;
-    unit_a = unit_b = -1;
-    if (k + lane < count) {
-      const QaPlace r = qa_locate(p, begins, per, x0 + k + lane);
-      const int t = r.step * QA_STEP, left = r.it.len - t;
-      const int32_t* table = p.tables + (int64_t)r.it.row * p.table_stride;
-      const int at = t / p.page;
-      const int a = left > 0 ? table[at] : 0;
-      const int b = units == 1 && left > Q4_UNIT ? table[at + 1] : a;
-      if (left > 0 && a >= 0 && a < p.num_pages)
-        unit_a = (a * p.hkv + r.head) * units + (t - at * p.page) / Q4_UNIT;
-      if (left > Q4_UNIT && b >= 0 && b < p.num_pages)
-        unit_b = units == 1 ? b * p.hkv + r.head : unit_a + 1;
-      if (p.status && ((left > 0 && unit_a < 0) || (left > Q4_UNIT && unit_b < 0)))
-        atomicOr(p.status, FK_DEV_BAD_PAGE);
+    const int step = k + (lane >> 1), second = lane & 1;
+    int unit = -1;
+    if (step < count) {
+      const QaPlace r = qa_locate(p, begins, per, x0 + step);
+      const int t = r.step * QA_STEP + second * Q4_UNIT;
+      if (t < r.it.len) {
+        const int at = t / p.page;
+        const int page = p.tables[(int64_t)r.it.row * p.table_stride + at];
+        if (page >= 0 && page < p.num_pages)
+          unit = (page * p.hkv + r.head) * units + (t - at * p.page) / Q4_UNIT;
+        else if (p.status)
+          atomicOr(p.status, FK_DEV_BAD_PAGE);
+      }
     }
-    have_a = __ballot_sync(0xffffffffu, unit_a >= 0);
-    have_b = __ballot_sync(0xffffffffu, unit_b >= 0);
+    reinterpret_cast<int*>(&where[warp][step & (2 * QA_AHEAD - 1)])[second] = unit;
+    __syncwarp();
   };
   auto copy = [&](int k, int slot) {
-    if ((k & 31) == 0) look_up(k);
-    if (lane == (k & 31)) {
+    if ((k & (QA_AHEAD - 1)) == 0) look_up(k);
+    if (lane == 0) {
+      const int2 w = where[warp][k & (2 * QA_AHEAD - 1)];
       uint8_t* dst = ring + slot * S::kStage;
       uint64_t* bar = &full[slot];
-      const int n = (unit_a >= 0) + (unit_b >= 0);
-      mbar_arrive_expect_tx(bar, n * S::kUnit);
-      if (n == 2 && unit_b == unit_a + 1) {                // side by side in the pool
-        bulk_load(dst, p.pool + (int64_t)unit_a * S::kUnit, 2 * S::kUnit, bar);
+      if (w.x >= 0 && w.y == w.x + 1) {                    // side by side in the pool
+        mbar_arrive_expect_tx(bar, 2 * S::kUnit);
+        bulk_load(dst, p.pool + (int64_t)w.x * S::kUnit, 2 * S::kUnit, bar);
       } else {
-        if (unit_a >= 0) bulk_load(dst, p.pool + (int64_t)unit_a * S::kUnit, S::kUnit, bar);
-        if (unit_b >= 0)
-          bulk_load(dst + S::kUnit, p.pool + (int64_t)unit_b * S::kUnit, S::kUnit, bar);
+        mbar_arrive_expect_tx(bar, ((w.x >= 0) + (w.y >= 0)) * S::kUnit);
+        if (w.x >= 0) bulk_load(dst, p.pool + (int64_t)w.x * S::kUnit, S::kUnit, bar);
+        if (w.y >= 0)
+          bulk_load(dst + S::kUnit, p.pool + (int64_t)w.y * S::kUnit, S::kUnit, bar);
       }
     }
   };
@@ -297,11 +297,10 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
   // ---- state of a pair: columns 8 nt + 2 quad + {0, 1} ----
   uint32_t qf[NT][8][2];
   float o[8][NT][4];
-  // weights are 2^(logit - ref); logits above `limit` raise it; sums of weights, and of weights' lowest
-  float ref[NT][2], limit[NT][2], l[NT][2], low[NG][NT][2];
+  // weights are 2^(logit - ref); their sums, and of weights times the value's lowest
+  float ref[NT][2], l[NT][2], low[NG][NT][2];
   float factor[NT][2], qsum[NG][NT][2];       // of logits: of a product, of a token's lowest
-  int len[NT][2];
-  float vref = 0.f, vinv = 0.f;
+  float vinv;                                 // 64 / (a power of two above all scales of values)
 
   bool ok = true;
   int slot = 0, i = 0;
@@ -309,7 +308,11 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
   while (ok && i < count) {
     // ---------------------------------------------------------------- a new pair
     const QaPlace now = qa_locate(p, begins, per, x0 + i);
+    __syncwarp();
+    if (lane == 0) places[warp] = now;
+    __syncwarp();
     const int begin = i, last = i + max(1, min(now.it.steps - now.step, count - i));
+    const int step0 = now.step - i;                        // of the pair, at i = 0
     int shortest = 0x7fffffff;
     {
 #pragma unroll
@@ -372,12 +375,11 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
         for (int j = 0; j < 2; ++j) {
           const int from = (2 * quad + j) * 4;             // a lane of that column
           factor[nt][j] = __shfl_sync(0xffffffffu, f, from);
-          len[nt][j] = __shfl_sync(0xffffffffu, n, from);
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr)
             qsum[gr][nt][j] = __shfl_sync(0xffffffffu, sum[gr], from) * p.scale_log2;
-          limit[nt][j] = -INFINITY;
-          ref[nt][j] = l[nt][j] = 0.f;
+          ref[nt][j] = QA_NONE;
+          l[nt][j] = 0.f;
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] = 0.f;
         }
@@ -386,10 +388,10 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
           o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
       }
       shortest = __reduce_min_sync(0xffffffffu, shortest);
-      vref = vinv = 0.f;
+      vinv = 1.2676506e30f;                                 // 2^100
     }
 
-    const int step0 = now.step - i;                        // of the pair, at i = 0
+    const int safe = shortest / QA_STEP;                   // whole steps for all columns
     for (; i < last; ++i) {
       if (!qa_wait_warp(&full[slot], phase)) {
         if (lane == 0 && p.status) atomicOr(p.status, FK_DEV_WAIT_TIMEOUT);
@@ -397,12 +399,8 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
         break;
       }
       const uint8_t* st = ring + slot * S::kStage;
-      // copies are up to DEPTH steps on, perhaps among the next 32
-      const bool next = (min(i + DEPTH, count) - 1) >> 5 != i >> 5;
-      const uint32_t have = ((next ? had_a : have_a) >> (i & 31) & 1u) |
-                            ((next ? had_b : have_b) >> (i & 31) & 1u) << 1;
-      const int tok0 = (step0 + i) * QA_STEP;
-      const bool edge = tok0 + QA_STEP > shortest || have != 3u;
+      const int2 w = where[warp][i & (2 * QA_AHEAD - 1)];
+      const bool edge = step0 + i >= safe || (w.x | w.y) < 0;
 
       // ---- logits: rows are tokens row, row + 8 of unit `lu` ----
       float z[SETS][NT][4];                                 // [set][.][row: 2 columns, row + 8: 2]
@@ -475,10 +473,19 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
           }
         if (edge) {
           // what stands behind the context is any number, or none
+          const QaPlace& at = places[warp];
+          int len[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int tok = (FOLD == 2 ? 2 * (quad & 1) + j : nt * 8 + 2 * quad + j) / p.g;
+              len[nt][j] = tok < at.it.tokens ? qa_len(p, at.token + tok) : 0;
+            }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int t = tok0 + lu * Q4_UNIT + row + 8 * r;
-            const bool there = (have >> lu & 1u) && t < now.it.len;
+            const int t = (step0 + i) * QA_STEP + lu * Q4_UNIT + row + 8 * r;
+            const bool there = (lu ? w.y : w.x) >= 0 && t < at.it.len;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr)
               if (!there) vs[u][gr][r] = vl[u][gr][r] = 0.f;
@@ -518,7 +525,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
         for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int gr = 0; gr < NG; ++gr) vmax = fmaxf(vmax, vs[u][gr][r]);
-      bool beyond = vmax > vref;
+      bool beyond = vmax * vinv > 64.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -526,19 +533,19 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
           top[nt][j] = fmaxf(z[0][nt][j], z[0][nt][2 + j]);
           if constexpr (SETS == 2)
             top[nt][j] = fmaxf(top[nt][j], fmaxf(z[1][nt][j], z[1][nt][2 + j]));
-          beyond |= top[nt][j] > limit[nt][j];
+          beyond |= top[nt][j] > ref[nt][j] + QA_SLACK;
         }
       if (__any_sync(0xffffffffu, beyond)) {
         constexpr int kFrom = FOLD == 2 ? 2 : 4;            // lanes of the same column, and its twin
 #pragma unroll
-        for (int sh = kFrom; sh < 32; sh <<= 1)
+        for (int sh = 1; sh < 32; sh <<= 1)
           vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
-        float vnew = vref;
-        if (vmax > vref)                                    // the power of two above
-          vnew = fmaxf(__uint_as_float(((__float_as_uint(vmax) >> 23) + 1u) << 23), 1e-30f);
-        const float vshift = vref > 0.f ? vref / vnew : 0.f;
-        vref = vnew;
-        vinv = vnew > 0.f ? 64.f / vnew : 0.f;
+        float shift = 1.f;
+        if (vmax * vinv > 64.f) {
+          const float old = vinv;
+          vinv = 64.f / __uint_as_float(((__float_as_uint(vmax) >> 23) + 1u) << 23);
+          shift = vinv / old;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -547,20 +554,16 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
 #pragma unroll
             for (int sh = kFrom; sh < 32; sh <<= 1)
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-            const float old = limit[nt][j] == -INFINITY ? -INFINITY : ref[nt][j];
-            float alpha = 1.f;
-            if (mx > old) {
-              alpha = fast_exp2(old - mx);
-              ref[nt][j] = mx;
-              limit[nt][j] = mx + QA_SLACK;
-            }
+            const float next = fmaxf(ref[nt][j], mx);
+            const float alpha = next > ref[nt][j] ? fast_exp2(ref[nt][j] - next) : 1.f;
+            ref[nt][j] = next;
             l[nt][j] *= alpha;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] *= alpha;
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) {
-              o[mt][nt][j] *= alpha * vshift;
-              o[mt][nt][2 + j] *= alpha * vshift;
+              o[mt][nt][j] *= alpha * shift;
+              o[mt][nt][2 + j] *= alpha * shift;
             }
           }
       }
@@ -633,9 +636,10 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
 
     if (!ok) break;
     // ------------------------------------------------------------------- the pair's end
-    const bool whole = now.step == 0 && step0 + i == now.it.steps;
+    const QaPlace done = places[warp];
+    const bool whole = done.step == 0 && step0 + i == done.it.steps;
     const int64_t place = 2 * me + (begin > 0 ? 1 : 0);
-    const float vback = vref * (1.f / 64.f);
+    const float vback = 1.f / vinv;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -660,7 +664,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
         }
         const int col = nt * 8 + 2 * quad + j;
         const int tok = col / p.g;
-        if (tok >= now.it.tokens) continue;
+        if (tok >= done.it.tokens) continue;
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -675,8 +679,8 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
             w.y = pack_bf16(v[2] * inv, v[3] * inv);
             w.z = pack_bf16(v[4] * inv, v[5] * inv);
             w.w = pack_bf16(v[6] * inv, v[7] * inv);
-            *reinterpret_cast<uint4*>(p.out + (int64_t)(now.token + tok) * p.out_stride +
-                                      (int64_t)(now.head * p.g + col - tok * p.g) * Q4_D + 64 * h +
+            *reinterpret_cast<uint4*>(p.out + (int64_t)(done.token + tok) * p.out_stride +
+                                      (int64_t)(done.head * p.g + col - tok * p.g) * Q4_D + 64 * h +
                                       8 * row) = w;
           } else {
             float4* dst = reinterpret_cast<float4*>(p.part_o + (place * p.cols + col) * Q4_D +
@@ -686,11 +690,10 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
           }
         }
         if (row == 0) {
-          const float m = limit[nt][j] == -INFINITY ? -INFINITY : ref[nt][j];
-          if (!whole) p.part_ml[place * p.cols + col] = make_float2(m, sum);
+          if (!whole) p.part_ml[place * p.cols + col] = make_float2(ref[nt][j], sum);
           else if (SUMS)
-            p.whole_ml[((int64_t)now.token * p.hkv + now.head) * p.cols + col] =
-                make_float2(m, sum);
+            p.whole_ml[((int64_t)done.token * p.hkv + done.head) * p.cols + col] =
+                make_float2(ref[nt][j], sum);
         }
       }
   }
@@ -726,20 +729,19 @@ __device__ __forceinline__ QaRuns qa_runs(const Q4AttnParams& p, int token, int 
 // (maximum, sum of weights) of a column over all parts; all lanes of a warp.
 __device__ __forceinline__ float2 qa_total(const Q4AttnParams& p, const QaRuns& r, int col) {
   const int lane = threadIdx.x & 31;
-  float M = -INFINITY;
+  float M = QA_NONE;
   for (int64_t w = r.a + lane; w <= r.b; w += 32)
     M = fmaxf(M, p.part_ml[r.place(w) * p.cols + col].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float Mu = M == -INFINITY ? 0.f : M;
   float L = 0.f;
   for (int64_t w = r.a + lane; w <= r.b; w += 32) {
     const float2 v = p.part_ml[r.place(w) * p.cols + col];
-    L += v.y * fast_exp2(v.x - Mu);
+    L += v.y * fast_exp2(v.x - M);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  return make_float2(Mu, L);
+  return make_float2(M, L);
 }
 
 __device__ __forceinline__ void qa_join(const Q4AttnParams& p, int token, int head) {
@@ -805,12 +807,8 @@ __device__ __forceinline__ void qa_sums(const Q4AttnParams& p, int seq, int head
     __syncthreads();                         // the columns before have been read
     for (int c = warp; c < cols; c += QA_WARPS) {
       float2 v;
-      if (r.a == r.b) {
-        v = p.whole_ml[((int64_t)t * p.hkv + head) * p.cols + c];
-        if (v.x == -INFINITY) v.x = 0.f;
-      } else {
-        v = qa_total(p, r, c);
-      }
+      if (r.a == r.b) v = p.whole_ml[((int64_t)t * p.hkv + head) * p.cols + c];
+      else v = qa_total(p, r, c);
       if (lane == 0) ml[c] = make_float2(v.x, v.y == 0.f ? 0.f : 1.f / v.y);
     }
     __syncthreads();
