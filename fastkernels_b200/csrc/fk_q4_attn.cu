@@ -28,7 +28,7 @@
 
 namespace fk {
 
-constexpr int QA_WARPS = 8;
+constexpr int QA_WARPS = 8;                  // of the joining kernel
 constexpr int QA_THREADS = QA_WARPS * 32;
 constexpr int QA_STEP = 32;                  // tokens of a warp's step
 constexpr int QA_AHEAD = 16;                 // steps that are looked up at a time
@@ -70,7 +70,7 @@ __device__ __forceinline__ uint64_t qa_ns() {
 // A wait of 2 s at most; all lanes get the same answer.
 __device__ __forceinline__ bool qa_wait_warp(uint64_t* bar, uint32_t parity) {
   bool got = mbar_try_wait(bar, parity);
-  if (!__all_sync(0xffffffffu, got)) {
+  if (__builtin_expect(!__all_sync(0xffffffffu, got), 0)) {
     const uint64_t t0 = qa_ns();
     bool late = false;
     do {
@@ -150,10 +150,11 @@ struct QaPlace {
   int token, head, step;
   QaItem it;
 };
+template <int THREADS>
 __device__ __forceinline__ QaPlace qa_locate(const Q4AttnParams& p, const int64_t* begins, int per,
                                              int64_t x) {
   const int64_t at = x >> 31 ? x / p.hkv : (int64_t)((uint32_t)x / (uint32_t)p.hkv);
-  int lo = 0, hi = QA_THREADS;
+  int lo = 0, hi = THREADS;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (begins[mid] <= at) lo = mid; else hi = mid;
@@ -183,22 +184,25 @@ struct QaShape {
   static constexpr int kUnit = q4_unit_bytes(NG);
   static constexpr int kStage = 2 * kUnit;
   static constexpr int kCtas = COLS == 16 ? 1 : 2;         // of an SM
-  static constexpr int kDepth = COLS == 16 ? 6 : 3;        // steps of a warp's ring
-  static constexpr int kSmem = QA_WARPS * kDepth * kStage;
+  static constexpr int kWarps = COLS == 16 ? 12 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kDepth = COLS == 16 ? 4 : 3;        // steps of a warp's ring
+  static constexpr int kSmem = kWarps * kDepth * kStage;
 };
 
 // NG groups a row; SUMS: logits are kept for the sums of weights.
 template <int NG, int COLS, bool SUMS>
-__global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
+__global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, COLS>::kCtas))
     q4_attn_kernel(const Q4AttnParams p) {
   using S = QaShape<NG, COLS>;
   constexpr int DEPTH = S::kDepth, NT = S::kTiles, FOLD = S::kFold, SETS = 2 / FOLD;
+  constexpr int WARPS = S::kWarps, THREADS = S::kThreads;
   extern __shared__ __align__(128) uint8_t ring_all[];
-  __shared__ uint64_t bars[QA_WARPS][DEPTH];
-  __shared__ int64_t begins[QA_THREADS + 1];               // steps before each thread's tokens
-  __shared__ int64_t sums[QA_WARPS];
-  __shared__ int2 where[QA_WARPS][2 * QA_AHEAD];           // units of a step in the pool, -1: none
-  __shared__ QaPlace places[QA_WARPS];                     // of the pair a warp is at
+  __shared__ uint64_t bars[WARPS][DEPTH];
+  __shared__ int64_t begins[THREADS + 1];               // steps before each thread's tokens
+  __shared__ int64_t sums[WARPS];
+  __shared__ int2 where[WARPS][2 * QA_AHEAD];           // units of a step in the pool, -1: none
+  __shared__ QaPlace places[WARPS];                     // of the pair a warp is at
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = lane & 3, row = lane >> 2;
   if (lane == 0) {
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
   pdl_wait();
 
   // ---- where the run of this warp begins ----
-  const int per = (p.num_tokens + QA_THREADS - 1) / QA_THREADS;
+  const int per = (p.num_tokens + THREADS - 1) / THREADS;
   {
     const int a = min((int)threadIdx.x * per, p.num_tokens), b = min(a + per, p.num_tokens);
     int64_t mine = 0;
@@ -224,12 +228,12 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
     __syncthreads();
     int64_t before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < QA_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) before += sums[w];
       total += sums[w];
     }
     begins[threadIdx.x] = before + incl - mine;
-    if (threadIdx.x == 0) begins[QA_THREADS] = total;
+    if (threadIdx.x == 0) begins[THREADS] = total;
     if (blockIdx.x == 0) {
       int64_t run = before + incl - mine;
       for (int i = a; i < b; ++i) {
@@ -244,11 +248,11 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
     }
     __syncthreads();
   }
-  const int64_t warps = (int64_t)gridDim.x * QA_WARPS;
-  const int64_t total = begins[QA_THREADS] * p.hkv;
+  const int64_t warps = (int64_t)gridDim.x * WARPS;
+  const int64_t total = begins[THREADS] * p.hkv;
   const int64_t run = (total + warps - 1) / warps;
   if (blockIdx.x == 0 && threadIdx.x == 0) p.run[0] = run;
-  const int64_t me = (int64_t)blockIdx.x * QA_WARPS + warp;
+  const int64_t me = (int64_t)blockIdx.x * WARPS + warp;
   const int64_t x0 = me * run, x1 = min(total, x0 + run);
   if (x0 >= x1) return;
 
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
     const int step = k + (lane >> 1), second = lane & 1;
     int unit = -1;
     if (step < count) {
-      const QaPlace r = qa_locate(p, begins, per, x0 + step);
+      const QaPlace r = qa_locate<THREADS>(p, begins, per, x0 + step);
       const int t = r.step * QA_STEP + second * Q4_UNIT;
       if (t < r.it.len) {
         const int at = t / p.page;
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
     __syncwarp();
   };
   auto copy = [&](int k, int slot) {
-    if ((k & (QA_AHEAD - 1)) == 0) look_up(k);
+    if (__builtin_expect((k & (QA_AHEAD - 1)) == 0, 0)) look_up(k);
     if (lane == 0) {
       const int2 w = where[warp][k & (2 * QA_AHEAD - 1)];
       uint8_t* dst = ring + slot * S::kStage;
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
   uint32_t phase = 0;
   while (ok && i < count) {
     // ---------------------------------------------------------------- a new pair
-    const QaPlace now = qa_locate(p, begins, per, x0 + i);
+    const QaPlace now = qa_locate<THREADS>(p, begins, per, x0 + i);
     __syncwarp();
     if (lane == 0) places[warp] = now;
     __syncwarp();
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
             vs[u][gr][r] = bf16lo(vp[r][gr]);
             vl[u][gr][r] = bf16hi(vp[r][gr]);
           }
-        if (edge) {
+        if (__builtin_expect(edge, 0)) {
           // what stands behind the context is any number, or none
           const QaPlace& at = places[warp];
           int len[NT][2];
@@ -535,7 +539,7 @@ __global__ void __launch_bounds__(QA_THREADS, (QaShape<NG, COLS>::kCtas))
             top[nt][j] = fmaxf(top[nt][j], fmaxf(z[1][nt][j], z[1][nt][2 + j]));
           beyond |= top[nt][j] > ref[nt][j] + QA_SLACK;
         }
-      if (__any_sync(0xffffffffu, beyond)) {
+      if (__builtin_expect(__any_sync(0xffffffffu, beyond), 0)) {
         constexpr int kFrom = FOLD == 2 ? 2 : 4;            // lanes of the same column, and its twin
 #pragma unroll
         for (int sh = 1; sh < 32; sh <<= 1)
@@ -861,7 +865,7 @@ static QaLayout qa_layout(int tokens, int seqs, int hkv, int g, bool sums, int64
   auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
   int block;
   const int cols = qa_columns(tokens, seqs, g, &block);
-  const size_t places = (size_t)sm_count() * 2 * QA_WARPS * 2;
+  const size_t places = (size_t)sm_count() * 16 * 2;       // two of each of at most 16 warps an SM
   QaLayout w{};
   w.first = 256;
   w.part_ml = w.first + up(((size_t)tokens + 1) * sizeof(int64_t));
@@ -884,7 +888,7 @@ static cudaError_t qa_launch(const Q4AttnParams& p, int sms, cudaStream_t s) {
   auto kernel = q4_attn_kernel<NG, COLS, SUMS>;
   const cudaError_t e = set_max_dynamic_smem(once, kernel, Shape::kSmem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(sms * Shape::kCtas), dim3(QA_THREADS), (size_t)Shape::kSmem, s,
+  return launch_kernel(kernel, dim3(sms * Shape::kCtas), dim3(Shape::kThreads), (size_t)Shape::kSmem, s,
                        p);
 }
 template <int NG, bool SUMS>
