@@ -24,14 +24,16 @@ CORE_SOURCES = ["fk_host.cu", "fk_elementwise.cu", "fk_gemm.cu", "fk_prefill.cu"
                 "fk_gemm_large.cu", "fk_layers.cu", "fk_mixer.cu", "fk_residual.cu", "fk_group.cu",
                 "fk_plain.cu"]
 COMPONENT_SOURCES = {"decode_attn": ["fk_attn.cu", "fk_shared.cu", "fk_select.cu", "fk_q4.cu",
-                                     "fk_q4_attn.cu", "fk_evict.cu"],
+                                     "fk_q4_attn.cu", "fk_sums.cu",
+                                     "fk_evict.cu"],
                      "delta": ["fk_delta.cu"],
                      "latent": ["fk_latent.cu"], "mlstm": ["fk_mlstm.cu"],
                      "experts": ["fk_moe.cu"], "comm": ["fk_comm.cu"], "block": ["fk_block.cu"]}
 SOURCES = CORE_SOURCES + [s for c in COMPONENT_SOURCES.values() for s in c]
 HEADERS = [CSRC / "fk_common.cuh", CSRC / "fk_tcgen05.cuh", CSRC / "fk_rowops.cuh",
            CSRC / "fk_types.cuh", CSRC / "fk_f32_tile.cuh", CSRC / "fk_attn.cuh",
-           CSRC / "fk_gemm_shared.cuh", CSRC / "fk_q4.cuh",
+           CSRC / "fk_gemm_shared.cuh", CSRC / "fk_q4.cuh", CSRC / "fk_runs.cuh",
+           CSRC / "fk_sums.cuh",
            PKG.parent / "include" / "fk_b200.h"]
 
 NVCC_FLAGS = [

@@ -28,6 +28,7 @@
 // once, q, out, lens, block tables) + split partials (fp32, < 4 % at the chosen
 // split sizes).
 #include "fk_attn.cuh"
+#include "fk_sums.cuh"
 
 #include <mutex>
 #include <unordered_map>
@@ -885,11 +886,19 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_decode_kernel(
 // fastkernels/tasks/baseline/L1/triton_unified_attention.py:697-786:
 // empty total -> zeros)
 // ---------------------------------------------------------------------------
+template <bool SUMS>
 __device__ __forceinline__ void attn_merge_row(const AttnParams& p, int gw, int lane) {
   const int seq = gw / p.hq, head = gw - seq * p.hq;
   const int* chunk_start = p.plan + ATT_PLAN_HDR;
   const int n = chunk_start[seq + 1] - chunk_start[seq];
-  if (n == 1) return;  // written directly by the main kernel
+  float2* total = p.part_ml + ((int64_t)seq * p.hq + head) * p.max_splits;
+  if (n == 1) {        // written directly by the main kernel
+    if (SUMS && lane == 0) {
+      const float l = total->y;
+      total->y = l == 0.f ? 0.f : 1.0f / l;
+    }
+    return;
+  }
   uint2* dst = reinterpret_cast<uint2*>(p.out + (int64_t)seq * p.out_stride +
                                         (int64_t)head * ATT_D) + lane;
   if (n == 0) {
@@ -930,6 +939,10 @@ __device__ __forceinline__ void attn_merge_row(const AttnParams& p, int gw, int 
   const float inv = lt > 0.f ? 1.0f / lt : 0.f;
   *dst = make_uint2(pack_bf16(acc.x * inv, acc.y * inv),
                     pack_bf16(acc.z * inv, acc.w * inv));
+  if (SUMS) {
+    __syncwarp();                            // all parts have been read
+    if (lane == 0) *total = make_float2(Mu, lt == 0.f ? 0.f : 1.0f / lt);
+  }
 }
 __global__ void __launch_bounds__(256) attn_merge_kernel(const AttnParams p) {
   pdl_launch_dependents();
@@ -939,12 +952,11 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const AttnParams p) {
   if (blockIdx.x == 0 && threadIdx.x == 0) p.plan[2] = 0;
   const int gw = (int)((blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5);
   if (gw >= p.batch * p.hq) return;
-  attn_merge_row(p, gw, threadIdx.x & 31);
+  attn_merge_row<false>(p, gw, threadIdx.x & 31);
 }
 
 // ---------------------------------------------------------------------------
-// sums of weights: what the query tokens of a sequence give each of its cached tokens,
-// sum over heads and tokens of 2^(logit - M) / sum, in the order of the tokens
+// with sums of weights: a row's first part becomes (maximum, 1 / sum) of all
 // ---------------------------------------------------------------------------
 // The table and the keys of each query token of the sequences in cu; none outside of all.
 __global__ void __launch_bounds__(256) attn_rows_kernel(const int32_t* __restrict__ cu, int num_seqs,
@@ -964,64 +976,13 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const int32_t* __restric
   lens[i] = in ? context_lens[i] : 0;
 }
 
-// Rows to merge, a warp each, then chunks of 256 cached tokens of a sequence and KV head.
-__global__ void __launch_bounds__(256) attn_merge_sums_kernel(const AttnParams p, int merges) {
-  __shared__ float2 ml[16];
+__global__ void __launch_bounds__(256) attn_merge_sums_kernel(const AttnParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if ((int)blockIdx.x < merges) {
-    const int gw = blockIdx.x * 8 + warp;
-    // a row of no sequence stays as it is
-    if (gw < p.batch * p.hq && (!p.rows || p.rows[gw / p.hq] >= 0)) attn_merge_row(p, gw, lane);
-    return;
-  }
-  const unsigned b = blockIdx.x - merges;
-  const int chunk = (int)(b % p.sum_chunks);
-  const int pair = (int)(b / p.sum_chunks);
-  const int seq = pair / p.hkv, kvh = pair - seq * p.hkv;
-  const int t0 = p.cu ? p.cu[seq] : seq;
-  const int t1 = p.cu ? min(p.cu[seq + 1], p.batch) : seq + 1;
-  if (t0 < 0 || t0 >= t1) return;
-  const int key = chunk * 256 + threadIdx.x;
-  const int* chunk_start = p.plan + ATT_PLAN_HDR;
-  auto len_of = [&](int t) -> int64_t {
-    const int64_t n = p.context_lens[t];
-    return n < 0 ? 0 : n > p.capacity ? p.capacity : n;
-  };
-  const int64_t from = p.from ? p.from[seq] : len_of(t0) - 1;
-  float sum = 0.f;
-  bool seen = false;
-  for (int t = t0; t < t1; ++t) {
-    const int64_t len = len_of(t);
-    if (len <= (int64_t)chunk * 256) continue;
-    __syncthreads();                         // the token before has been added
-    for (int h = warp; h < p.g; h += 8) {
-      const float2* part = p.part_ml + ((int64_t)t * p.hq + kvh * p.g + h) * p.max_splits;
-      const int n = chunk_start[t + 1] - chunk_start[t];
-      float M = -INFINITY, L = 0.f;
-      for (int s = lane; s < n; s += 32) M = fmaxf(M, part[s].x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      if (M == -INFINITY) M = 0.f;
-      for (int s = lane; s < n; s += 32) L += part[s].y * fast_exp2(part[s].x - M);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      if (lane == 0) ml[h] = make_float2(M, L == 0.f ? 0.f : 1.f / L);
-    }
-    __syncthreads();
-    if (key < len) {
-      seen = true;
-      const float* z = p.logits + (((int64_t)t * p.hkv + kvh) * p.logit_len + key) * p.g;
-      for (int h = 0; h < p.g; ++h) sum = fmaf(fast_exp2(z[h] - ml[h].x), ml[h].y, sum);
-    }
-  }
-  if (!seen) return;
-  const int at = key / p.block_size;
-  const int page = p.block_tables[(int64_t)seq * p.bt_stride + at];
-  if (page < 0 || page >= p.num_blocks) return;            // flagged by the main kernel
-  float* w = p.weights + ((int64_t)page * p.hkv + kvh) * p.block_size + (key - at * p.block_size);
-  *w = key < from ? *w + sum : sum;
+  const int gw = (int)((blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5);
+  // a row of no sequence stays as it is
+  if (gw < p.batch * p.hq && (!p.rows || p.rows[gw / p.hq] >= 0))
+    attn_merge_row<true>(p, gw, threadIdx.x & 31);
 }
 
 // ---------------------------------------------------------------------------
@@ -1281,12 +1242,6 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
     capacity = p.capacity = sums->max_len;
     p.logits = reinterpret_cast<float*>(ws + main_bytes);
     p.logit_len = sums->max_len;
-    p.weights = sums->weights; p.from = sums->from; p.cu = sums->cu;
-    p.num_seqs = sums->num_seqs;
-    p.sum_chunks = (int)((sums->max_len + 255) / 256);
-    FK_REQUIRE((int64_t)(batch + 7) * num_q_heads + (int64_t)p.num_seqs * num_kv_heads * p.sum_chunks <
-                   (1ll << 31),
-               FK_ERR_UNSUPPORTED, "fk_paged_decode_attn_weights: too many tokens");
     if (sums->cu) {
       int32_t* rows = reinterpret_cast<int32_t*>(
           ws + main_bytes + sums_bytes(batch, num_q_heads, false, sums->max_len));
@@ -1316,11 +1271,21 @@ static int attn_impl(int mode, bool split, const void* q, int64_t q_stride_token
   FK_CUDA_OK(launch_decode(g > 8, split, false, grid, mk, mv, p, s));
   const int warps = batch * num_q_heads;
   if (sums) {
-    const int merges = (warps + 7) / 8;
-    FK_CUDA_OK(launch_kernel(attn_merge_sums_kernel,
-                             dim3((unsigned)(merges + p.num_seqs * num_kv_heads * p.sum_chunks)),
-                             dim3(256), (size_t)0, s, p, merges));
-    count_launch(2);
+    FK_CUDA_OK(launch_kernel(attn_merge_sums_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256),
+                             (size_t)0, s, p));
+    SumsParams a{};
+    a.lens = p.context_lens; a.cu = sums->cu;
+    a.tables = block_tables; a.table_stride = block_table_stride;
+    a.capacity = p.capacity;
+    a.num_seqs = sums->num_seqs; a.num_tokens = batch; a.num_pages = p.num_blocks;
+    a.page = block_size; a.hkv = num_kv_heads;
+    a.block = 1; a.cols = g;
+    a.ml = p.part_ml; a.ml_pair = (int64_t)g * max_splits; a.ml_col = max_splits;
+    a.logits = p.logits; a.logit_len = p.logit_len;
+    a.logit_keys = (int64_t)batch * num_kv_heads * p.logit_len;
+    a.weights = sums->weights; a.from = sums->from;
+    FK_CUDA_OK(launch_sums(a, s));
+    count_launch(3);
     return FK_OK;
   }
   FK_LAUNCH(attn_merge_kernel, dim3((warps * 32 + 255) / 256), dim3(256), 0, s, p);

@@ -40,10 +40,6 @@ struct AttnParams {
   // sums of weights: `rows` as above; logits of every key that a token and KV head sees
   float* logits;            // [batch, hkv, logit_len, g]
   int64_t logit_len;
-  float* weights;           // [pages, hkv, block_size]
-  const int32_t* from;      // [sequences] first entry that starts from 0, null: the first token's own
-  const int32_t* cu;        // tokens of each sequence, null: one each
-  int num_seqs, sum_chunks;
 };
 
 

@@ -25,6 +25,8 @@
 // the kernel behind.  The running maximum is raised only when a logit is 8 above it (weights up to
 // 2^8 fit), so that in most steps nothing is reduced across lanes and nothing rescaled.
 #include "fk_q4.cuh"
+#include "fk_runs.cuh"
+#include "fk_sums.cuh"
 
 namespace fk {
 
@@ -53,12 +55,9 @@ struct Q4AttnParams {
   int64_t* first;               // [tokens + 1] steps of one head before a token's
   float2* part_ml;              // [2 * warps, cols]
   float* part_o;                // [2 * warps, cols, 128]
-  float2* whole_ml;             // [tokens * hkv, cols] of pairs that one warp has
+  float2* whole_ml;             // [tokens * hkv, cols] (maximum, 1 / sum)
   float* logits;                // [steps, 32, cols]
   int64_t logit_steps;
-  float* weights;               // [pages, hkv, page]
-  const int32_t* from;          // [sequences] tokens whose sums go on
-  int chunks;                   // of a sequence's tokens, for the sums
 };
 
 __device__ __forceinline__ uint64_t qa_ns() {
@@ -145,33 +144,17 @@ __device__ __forceinline__ QaItem qa_item(const Q4AttnParams& p, int token) {
   return it;
 }
 
-// A step in the row of all steps.  `begins`: steps before the first of each thread's `per` tokens.
+// A step in the row of all steps.
 struct QaPlace {
   int token, head, step;
   QaItem it;
 };
 template <int THREADS>
-__device__ __forceinline__ QaPlace qa_locate(const Q4AttnParams& p, const int64_t* begins, int per,
+__device__ __forceinline__ QaPlace qa_locate(const Q4AttnParams& p, const RunCount<THREADS>& counted,
                                              int64_t x) {
-  const int64_t at = x >> 31 ? x / p.hkv : (int64_t)((uint32_t)x / (uint32_t)p.hkv);
-  int lo = 0, hi = THREADS;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (begins[mid] <= at) lo = mid; else hi = mid;
-  }
-  int64_t before = begins[lo];
-  QaPlace r;
-  r.token = min(lo * per, p.num_tokens - 1);
-  r.it = qa_item(p, r.token);
-  while (r.token + 1 < p.num_tokens && before + r.it.steps <= at) {
-    before += r.it.steps;
-    r.it = qa_item(p, ++r.token);
-  }
-  const int64_t in = x - before * p.hkv;      // below steps * hkv
-  const int steps = max(r.it.steps, 1);
-  r.head = (int)(in >> 31 ? in / steps : (int64_t)((uint32_t)in / (uint32_t)steps));
-  r.step = (int)(in - (int64_t)r.head * steps);
-  return r;
+  const RunPlace r = find_run<THREADS>(counted, p.num_tokens, p.hkv, x,
+                                       [&](int i) { return qa_item(p, i).steps; });
+  return QaPlace{r.entry, r.head, r.step, qa_item(p, r.entry)};
 }
 
 // Columns of a warp's products.  Of up to 4 there are two sets side by side: one for the step's
@@ -199,8 +182,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   constexpr int WARPS = S::kWarps, THREADS = S::kThreads;
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ uint64_t bars[WARPS][DEPTH];
-  __shared__ int64_t begins[THREADS + 1];               // steps before each thread's tokens
-  __shared__ int64_t sums[WARPS];
+  __shared__ RunCount<THREADS> counted;
   __shared__ int2 where[WARPS][2 * QA_AHEAD];           // units of a step in the pool, -1: none
   __shared__ QaPlace places[WARPS];                     // of the pair a warp is at
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -213,44 +195,24 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   pdl_wait();
 
   // ---- where the run of this warp begins ----
-  const int per = (p.num_tokens + THREADS - 1) / THREADS;
-  {
+  int64_t before = count_runs<THREADS>(counted, p.num_tokens,
+                                       [&](int i) { return qa_item(p, i).steps; });
+  if (blockIdx.x == 0) {
+    const int per = entries_of_thread(p.num_tokens, THREADS);
     const int a = min((int)threadIdx.x * per, p.num_tokens), b = min(a + per, p.num_tokens);
-    int64_t mine = 0;
-    for (int i = a; i < b; ++i) mine += qa_item(p, i).steps;
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
+    for (int i = a; i < b; ++i) {
+      p.first[i] = before;
+      const QaItem it = qa_item(p, i);
+      before += it.steps;
+      if (p.status)
+        for (int j = 0; j < it.tokens; ++j)
+          if (p.lens[i + j] > p.capacity) atomicOr(p.status, FK_DEV_BAD_PAGE);
     }
-    if (lane == 31) sums[warp] = incl;
-    __syncthreads();
-    int64_t before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) before += sums[w];
-      total += sums[w];
-    }
-    begins[threadIdx.x] = before + incl - mine;
-    if (threadIdx.x == 0) begins[THREADS] = total;
-    if (blockIdx.x == 0) {
-      int64_t run = before + incl - mine;
-      for (int i = a; i < b; ++i) {
-        p.first[i] = run;
-        const QaItem it = qa_item(p, i);
-        run += it.steps;
-        if (p.status)
-          for (int j = 0; j < it.tokens; ++j)
-            if (p.lens[i + j] > p.capacity) atomicOr(p.status, FK_DEV_BAD_PAGE);
-      }
-      if (threadIdx.x == 0) p.first[p.num_tokens] = total;
-    }
-    __syncthreads();
+    if (threadIdx.x == 0) p.first[p.num_tokens] = counted.begins[THREADS];
   }
   const int64_t warps = (int64_t)gridDim.x * WARPS;
-  const int64_t total = begins[THREADS] * p.hkv;
-  const int64_t run = (total + warps - 1) / warps;
+  const int64_t total = counted.begins[THREADS] * p.hkv;
+  const int64_t run = run_length(total, warps);
   if (blockIdx.x == 0 && threadIdx.x == 0) p.run[0] = run;
   const int64_t me = (int64_t)blockIdx.x * WARPS + warp;
   const int64_t x0 = me * run, x1 = min(total, x0 + run);
@@ -265,7 +227,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
     const int step = k + (lane >> 1), second = lane & 1;
     int unit = -1;
     if (step < count) {
-      const QaPlace r = qa_locate<THREADS>(p, begins, per, x0 + step);
+      const QaPlace r = qa_locate<THREADS>(p, counted, x0 + step);
       const int t = r.step * QA_STEP + second * Q4_UNIT;
       if (t < r.it.len) {
         const int at = t / p.page;
@@ -311,7 +273,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   uint32_t phase = 0;
   while (ok && i < count) {
     // ---------------------------------------------------------------- a new pair
-    const QaPlace now = qa_locate<THREADS>(p, begins, per, x0 + i);
+    const QaPlace now = qa_locate<THREADS>(p, counted, x0 + i);
     __syncwarp();
     if (lane == 0) places[warp] = now;
     __syncwarp();
@@ -697,7 +659,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
           if (!whole) p.part_ml[place * p.cols + col] = make_float2(ref[nt][j], sum);
           else if (SUMS)
             p.whole_ml[((int64_t)done.token * p.hkv + done.head) * p.cols + col] =
-                make_float2(ref[nt][j], sum);
+                make_float2(ref[nt][j], inv);
         }
       }
   }
@@ -711,7 +673,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
 }
 
 // ---------------------------------------------------------------------------
-// join of partial results; sums of weights
+// join of partial results
 // ---------------------------------------------------------------------------
 // The runs that a pair's steps lie in: warps a .. b; warp a has the pair in its second place unless
 // the pair begins with the run.
@@ -748,7 +710,11 @@ __device__ __forceinline__ float2 qa_total(const Q4AttnParams& p, const QaRuns& 
   return make_float2(M, L);
 }
 
-__device__ __forceinline__ void qa_join(const Q4AttnParams& p, int token, int head) {
+template <bool SUMS>
+__global__ void __launch_bounds__(QA_THREADS) q4_attn_join_kernel(const Q4AttnParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int token = blockIdx.x / p.hkv, head = blockIdx.x - token * p.hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t steps = p.first[token + 1] - p.first[token];
   if (steps == 0) {
@@ -785,66 +751,13 @@ __device__ __forceinline__ void qa_join(const Q4AttnParams& p, int token, int he
       }
     }
     const float inv = all.y > 0.f ? 1.f / all.y : all.y == 0.f ? 0.f : all.y;
+    if (SUMS && lane == 0)
+      p.whole_ml[((int64_t)token * p.hkv + head) * p.cols + c] = make_float2(all.x, inv);
     const int tok = c / p.g;
     reinterpret_cast<uint2*>(p.out + (int64_t)(token + tok) * p.out_stride +
                              (int64_t)(head * p.g + c - tok * p.g) * Q4_D)[lane] =
         make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
   }
-}
-
-// One chunk of QA_THREADS cached tokens of a sequence and head: what its query tokens give each.
-__device__ __forceinline__ void qa_sums(const Q4AttnParams& p, int seq, int head, int chunk) {
-  __shared__ float2 ml[16];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t0 = p.cu ? p.cu[seq] : seq;
-  const int t1 = p.cu ? min(p.cu[seq + 1], p.num_tokens) : seq + 1;
-  if (t0 < 0 || t0 >= t1) return;
-  const int key = chunk * QA_THREADS + threadIdx.x;
-  const int64_t from = p.from ? p.from[seq] : (int64_t)qa_len(p, t0) - 1;
-  float sum = 0.f;
-  bool seen = false;
-  for (int t = t0; t < t1; t += p.block) {
-    const int64_t steps = p.first[t + 1] - p.first[t];
-    if (steps * QA_STEP <= (int64_t)chunk * QA_THREADS) continue;
-    const int cols = min(p.block, t1 - t) * p.g;
-    const QaRuns r = qa_runs(p, t, head, steps);
-    __syncthreads();                         // the columns before have been read
-    for (int c = warp; c < cols; c += QA_WARPS) {
-      float2 v;
-      if (r.a == r.b) v = p.whole_ml[((int64_t)t * p.hkv + head) * p.cols + c];
-      else v = qa_total(p, r, c);
-      if (lane == 0) ml[c] = make_float2(v.x, v.y == 0.f ? 0.f : 1.f / v.y);
-    }
-    __syncthreads();
-    const int64_t x = r.px + key / QA_STEP;
-    if (key < steps * QA_STEP && x < p.logit_steps) {
-      seen = true;
-      const float* src = p.logits + (x * QA_STEP + key % QA_STEP) * p.cols;
-      for (int c = 0; c < cols; ++c) sum = fmaf(fast_exp2(src[c] - ml[c].x), ml[c].y, sum);
-    }
-  }
-  int most = 0;
-  for (int t = t0; t < t1; ++t) most = max(most, qa_len(p, t));
-  if (!seen || key >= most) return;
-  const int at = key / p.page;
-  const int page = p.tables[(int64_t)seq * p.table_stride + at];
-  if (page < 0 || page >= p.num_pages) return;             // flagged by the attention
-  float* w = p.weights + ((int64_t)page * p.hkv + head) * p.page + (key - at * p.page);
-  *w = key < from ? *w + sum : sum;
-}
-
-template <bool SUMS>
-__global__ void __launch_bounds__(QA_THREADS) q4_attn_join_kernel(const Q4AttnParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const unsigned joins = (unsigned)(p.num_tokens * p.hkv);
-  if (!SUMS || blockIdx.x < joins) {
-    qa_join(p, (int)blockIdx.x / p.hkv, (int)blockIdx.x % p.hkv);
-    return;
-  }
-  const unsigned b = blockIdx.x - joins;
-  const unsigned pair = b / p.chunks;
-  qa_sums(p, (int)(pair / p.hkv), (int)(pair % p.hkv), (int)(b % p.chunks));
 }
 
 struct QaLayout {
@@ -974,10 +887,7 @@ int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
   p.whole_ml = reinterpret_cast<float2*>(ws + w.whole_ml);
   p.logits = reinterpret_cast<float*>(ws + w.logits);
   p.logit_steps = w.logit_steps;
-  p.weights = weights; p.from = weights_from;
-  p.chunks = (int)((p.capacity + QA_THREADS - 1) / QA_THREADS);
-  const int64_t joins = (int64_t)num_tokens * num_kv_heads;
-  const int64_t blocks = joins + (sums ? (int64_t)num_seqs * num_kv_heads * p.chunks : 0);
+  const int64_t blocks = (int64_t)num_tokens * num_kv_heads;
   FK_REQUIRE(blocks < (1ll << 31), FK_ERR_UNSUPPORTED, "%s: too many tokens", what);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sms = sm_count();
@@ -988,6 +898,19 @@ int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
   auto join = sums ? q4_attn_join_kernel<true> : q4_attn_join_kernel<false>;
   FK_CUDA_OK(launch_kernel(join, dim3((unsigned)blocks), dim3(QA_THREADS), (size_t)0, s, p));
   count_launch(2);
+  if (!sums) return FK_OK;
+  SumsParams a{};
+  a.lens = context_lens; a.cu = cu_seqlens_q;
+  a.tables = block_tables; a.table_stride = block_table_stride;
+  a.capacity = p.capacity;
+  a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.num_pages = p.num_pages;
+  a.page = page_size; a.hkv = num_kv_heads;
+  a.block = p.block; a.cols = p.cols;
+  a.ml = p.whole_ml; a.ml_pair = p.cols; a.ml_col = 1;
+  a.logits = p.logits; a.first = p.first; a.logit_keys = w.logit_steps * QA_STEP;
+  a.weights = weights; a.from = weights_from;
+  FK_CUDA_OK(launch_sums(a, s));
+  count_launch(1);
   return FK_OK;
 }
 
