@@ -12,7 +12,6 @@
 namespace fk {
 
 constexpr int SUMS_THREADS = 256;
-constexpr int SUMS_STEPS = 4;
 
 __device__ __forceinline__ int sums_len(const SumsParams& p, int token) {
   const int64_t n = p.lens[token];
@@ -30,7 +29,14 @@ __device__ __forceinline__ int sums_most(const SumsParams& p, int2 tokens) {
   return most;
 }
 
-__global__ void __launch_bounds__(SUMS_THREADS) attn_sums_kernel(const SumsParams p) {
+// STEPS at a time; one where there are several query tokens, whose logits are loads enough.  Each
+// grid is the CTAs that SMs hold.
+template <int STEPS>
+constexpr int sums_ctas() { return STEPS == 1 ? 4 : 3; }
+
+template <int STEPS>
+__global__ void __launch_bounds__(SUMS_THREADS, sums_ctas<STEPS>())
+    attn_sums_kernel(const SumsParams p) {
   __shared__ RunCount<SUMS_THREADS> counted;
   pdl_launch_dependents();
   pdl_wait();
@@ -40,7 +46,7 @@ __global__ void __launch_bounds__(SUMS_THREADS) attn_sums_kernel(const SumsParam
   const int64_t warps = (int64_t)gridDim.x * (SUMS_THREADS / 32);
   const int64_t total = counted.begins[SUMS_THREADS] * p.hkv;
   // (short runs would be all beginnings)
-  const int64_t run = max(run_length(total, warps), (int64_t)SUMS_STEPS);
+  const int64_t run = max(run_length(total, warps), (int64_t)STEPS);
   int64_t x = ((int64_t)blockIdx.x * (SUMS_THREADS / 32) + warp) * run;
   const int64_t x1 = min(total, x + run);
   while (x < x1) {
@@ -50,13 +56,13 @@ __global__ void __launch_bounds__(SUMS_THREADS) attn_sums_kernel(const SumsParam
     const int end = (int)min((int64_t)(most + 31) / 32, at.step + (x1 - x));
     const int64_t from = p.from ? p.from[at.entry] : (int64_t)sums_len(p, tokens.x) - 1;
     const int32_t* table = p.tables + (int64_t)at.entry * p.table_stride;
-    for (int s0 = at.step; s0 < end; s0 += SUMS_STEPS) {
-      int page[SUMS_STEPS], place[SUMS_STEPS], key[SUMS_STEPS];
-      float sum[SUMS_STEPS], old[SUMS_STEPS];
+    for (int s0 = at.step; s0 < end; s0 += STEPS) {
+      int page[STEPS], place[STEPS], key[STEPS];
+      float sum[STEPS], old[STEPS];
 #pragma unroll
-      for (int j = 0; j < SUMS_STEPS; ++j) {
+      for (int j = 0; j < STEPS; ++j) {
         key[j] = s0 + j < end ? (s0 + j) * 32 + lane : most;
-        const int i = key[j] / p.page;
+        const int i = p.page_shift >= 0 ? key[j] >> p.page_shift : key[j] / p.page;
         place[j] = key[j] - i * p.page;
         page[j] = key[j] < most ? table[i] : -1;
         sum[j] = 0.f;
@@ -75,19 +81,21 @@ __global__ void __launch_bounds__(SUMS_THREADS) attn_sums_kernel(const SumsParam
         }
         len = (int)min((int64_t)len, p.logit_keys - base);
         const float2* ml = p.ml + ((int64_t)t * p.hkv + at.head) * p.ml_pair;
-        const float* z = p.logits + base * p.cols;
+        const float* z = p.logits + (base + s0 * 32 + lane) * p.cols;
+        const int pitch = 32 * p.cols;
         // a logit that is none is -infinity
         auto add = [&](float2 m, int j, float l) {
           if (l != -INFINITY) sum[j] = fmaf(fast_exp2(l - m.x), m.y, sum[j]);
         };
         if (p.cols % 4 == 0) {
+#pragma unroll 4 / STEPS
           for (int c = 0; c < cols; c += 4) {
-            float4 v[SUMS_STEPS];
+            float4 v[STEPS];
             float2 m[4];
 #pragma unroll
-            for (int j = 0; j < SUMS_STEPS; ++j)
+            for (int j = 0; j < STEPS; ++j)
               v[j] = key[j] < len
-                         ? *reinterpret_cast<const float4*>(z + (int64_t)key[j] * p.cols + c)
+                         ? *reinterpret_cast<const float4*>(z + j * pitch + c)
                          : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -96,41 +104,46 @@ __global__ void __launch_bounds__(SUMS_THREADS) attn_sums_kernel(const SumsParam
             for (int e = 0; e < 4; ++e) {
               if (c + e >= cols) break;
 #pragma unroll
-              for (int j = 0; j < SUMS_STEPS; ++j)
+              for (int j = 0; j < STEPS; ++j)
                 add(m[e], j, e == 0 ? v[j].x : e == 1 ? v[j].y : e == 2 ? v[j].z : v[j].w);
             }
           }
         } else {
           for (int c = 0; c < cols; ++c) {
             const float2 m = ml[c * p.ml_col];
-            float v[SUMS_STEPS];
+            float v[STEPS];
 #pragma unroll
-            for (int j = 0; j < SUMS_STEPS; ++j)
-              v[j] = key[j] < len ? z[(int64_t)key[j] * p.cols + c] : -INFINITY;
+            for (int j = 0; j < STEPS; ++j)
+              v[j] = key[j] < len ? z[j * pitch + c] : -INFINITY;
 #pragma unroll
-            for (int j = 0; j < SUMS_STEPS; ++j) add(m, j, v[j]);
+            for (int j = 0; j < STEPS; ++j) add(m, j, v[j]);
           }
         }
       }
-      float* entry[SUMS_STEPS];
+      float* entry[STEPS];
 #pragma unroll
-      for (int j = 0; j < SUMS_STEPS; ++j) {
+      for (int j = 0; j < STEPS; ++j) {
         const bool there = page[j] >= 0 && page[j] < p.num_pages;     // else flagged by the attention
         entry[j] = there ? p.weights + ((int64_t)page[j] * p.hkv + at.head) * p.page + place[j]
                          : nullptr;
         old[j] = there && key[j] < from ? *entry[j] : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < SUMS_STEPS; ++j)
+      for (int j = 0; j < STEPS; ++j)
         if (entry[j]) *entry[j] = old[j] + sum[j];
     }
     x += max(1, end - at.step);
   }
 }
 
-cudaError_t launch_sums(const SumsParams& p, cudaStream_t s) {
-  // a wave of the device
-  return launch_kernel(attn_sums_kernel, dim3(sm_count() * 4), dim3(SUMS_THREADS), (size_t)0, s, p);
+template <int STEPS>
+static cudaError_t launch_steps(const SumsParams& p, cudaStream_t s) {
+  return launch_kernel(attn_sums_kernel<STEPS>, dim3(sm_count() * sums_ctas<STEPS>()),
+                       dim3(SUMS_THREADS), (size_t)0, s, p);
+}
+cudaError_t launch_sums(SumsParams p, cudaStream_t s) {
+  p.page_shift = (p.page & (p.page - 1)) == 0 ? __builtin_ctz(p.page) : -1;
+  return p.cu ? launch_steps<1>(p, s) : launch_steps<4>(p, s);
 }
 
 }  // namespace fk

@@ -11,6 +11,7 @@ struct SumsParams {
   const int32_t* tables; int64_t table_stride;
   int64_t capacity;
   int num_seqs, num_tokens, num_pages, page, hkv;
+  int page_shift;               // set by launch_sums
   int block;                    // query tokens whose logits lie side by side
   int cols;                     // logits of a key: block * query heads
   const float2* ml; int64_t ml_pair, ml_col;   // of (token, head) and column
@@ -21,6 +22,6 @@ struct SumsParams {
   const int32_t* from;
 };
 
-cudaError_t launch_sums(const SumsParams& p, cudaStream_t s);
+cudaError_t launch_sums(SumsParams p, cudaStream_t s);
 
 }  // namespace fk
