@@ -35,6 +35,7 @@ constexpr int QA_THREADS = QA_WARPS * 32;
 constexpr int QA_STEP = 32;                  // tokens of a warp's step
 constexpr int QA_AHEAD = 16;                 // steps that are looked up at a time
 constexpr float QA_NONE = -3e38f;            // reference before there is a key
+constexpr int QA_RUN = 4;                    // steps of a warp, at least
 constexpr float QA_SLACK = 8.f;              // logits may be this far above the maximum (log2)
 constexpr int64_t QA_LONGEST = 1ll << 30;    // tokens of a context
 
@@ -49,6 +50,7 @@ struct Q4AttnParams {
   int num_tokens, num_seqs, num_pages, page, hkv, g;
   int block;                    // query tokens that go together
   int cols;                     // block * g <= 8 or 16
+  int direct;                   // CTA b has pair b whole
   float scale_log2;
   int32_t* status;
   int64_t* run;                 // [0] steps of a warp's run
@@ -148,14 +150,24 @@ __device__ __forceinline__ QaItem qa_item(const Q4AttnParams& p, int token) {
 struct QaPlace {
   int token, head, step;
   QaItem it;
+  // `n` steps on
+  __device__ __forceinline__ void advance(const Q4AttnParams& p, int n) {
+    step += n;
+    while (step >= it.steps) {
+      step -= it.steps;
+      if (++head < p.hkv) continue;
+      head = 0;
+      do {
+        if (++token >= p.num_tokens) {        // behind the last: no keys
+          token = 0;
+          it = QaItem{0, 0, 0, 1 << 30};
+          return;
+        }
+        it = qa_item(p, token);
+      } while (it.steps == 0);
+    }
+  }
 };
-template <int THREADS>
-__device__ __forceinline__ QaPlace qa_locate(const Q4AttnParams& p, const RunCount<THREADS>& counted,
-                                             int64_t x) {
-  const RunPlace r = find_run<THREADS>(counted, p.num_tokens, p.hkv, x,
-                                       [&](int i) { return qa_item(p, i).steps; });
-  return QaPlace{r.entry, r.head, r.step, qa_item(p, r.entry)};
-}
 
 // Columns of a warp's products.  Of up to 4 there are two sets side by side: one for the step's
 // first 16 tokens, one for the others, so that what is done per logit is done once per 32 tokens
@@ -184,7 +196,11 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   __shared__ uint64_t bars[WARPS][DEPTH];
   __shared__ RunCount<THREADS> counted;
   __shared__ int2 where[WARPS][2 * QA_AHEAD];           // units of a step in the pool, -1: none
-  __shared__ QaPlace places[WARPS];                     // of the pair a warp is at
+  __shared__ QaPlace places[WARPS], ahead[WARPS];       // of the pair a warp is at, of its copies
+  __shared__ int ends[WARPS];
+  // (maximum, sum) of the warps' parts that become one, when runs have been counted
+  static_assert(sizeof(RunCount<THREADS>) >= sizeof(float2) * WARPS * COLS, "they share a place");
+  float2 (*part_ml)[COLS] = reinterpret_cast<float2 (*)[COLS]>(&counted);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = lane & 3, row = lane >> 2;
   if (lane == 0) {
@@ -194,40 +210,78 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   pdl_launch_dependents();
   pdl_wait();
 
-  // ---- where the run of this warp begins ----
-  int64_t before = count_runs<THREADS>(counted, p.num_tokens,
-                                       [&](int i) { return qa_item(p, i).steps; });
-  if (blockIdx.x == 0) {
-    const int per = entries_of_thread(p.num_tokens, THREADS);
-    const int a = min((int)threadIdx.x * per, p.num_tokens), b = min(a + per, p.num_tokens);
-    for (int i = a; i < b; ++i) {
-      p.first[i] = before;
-      const QaItem it = qa_item(p, i);
-      before += it.steps;
-      if (p.status)
-        for (int j = 0; j < it.tokens; ++j)
-          if (p.lens[i + j] > p.capacity) atomicOr(p.status, FK_DEV_BAD_PAGE);
-    }
-    if (threadIdx.x == 0) p.first[p.num_tokens] = counted.begins[THREADS];
-  }
-  const int64_t warps = (int64_t)gridDim.x * WARPS;
-  const int64_t total = counted.begins[THREADS] * p.hkv;
-  const int64_t run = run_length(total, warps);
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.run[0] = run;
+  // ---- the run of this warp: from a place on, every step, or of its CTA's pair every WARPS-th ----
+  QaPlace now;
+  int64_t x0 = 0;
+  int count, stride = 1;
   const int64_t me = (int64_t)blockIdx.x * WARPS + warp;
-  const int64_t x0 = me * run, x1 = min(total, x0 + run);
-  if (x0 >= x1) return;
+  if (p.direct) {
+    now.token = blockIdx.x / p.hkv;
+    now.head = blockIdx.x - now.token * p.hkv;
+    now.step = warp;
+    now.it = qa_item(p, now.token);
+    if (now.it.tokens == 0) return;
+    count = max(0, (now.it.steps - warp + WARPS - 1) / WARPS);
+    stride = WARPS;
+    if (p.status && now.head == 0 && threadIdx.x < now.it.tokens &&
+        p.lens[now.token + threadIdx.x] > p.capacity)
+      atomicOr(p.status, FK_DEV_BAD_PAGE);
+  } else {
+    auto steps = [&](int i) { return qa_item(p, i).steps; };
+    int64_t before = count_runs<THREADS>(counted, p.num_tokens, steps);
+    if (blockIdx.x == 0) {
+      const int per = entries_of_thread(p.num_tokens, THREADS);
+      const int a = min((int)threadIdx.x * per, p.num_tokens), b = min(a + per, p.num_tokens);
+      for (int i = a; i < b; ++i) {
+        p.first[i] = before;
+        const QaItem it = qa_item(p, i);
+        before += it.steps;
+        if (p.status)
+          for (int j = 0; j < it.tokens; ++j)
+            if (p.lens[i + j] > p.capacity) atomicOr(p.status, FK_DEV_BAD_PAGE);
+      }
+      if (threadIdx.x == 0) p.first[p.num_tokens] = counted.begins[THREADS];
+    }
+    const int64_t total = counted.begins[THREADS] * p.hkv;
+    // (short runs would be all beginnings, and many parts to join: but no longer than pairs are)
+    const int64_t pairs = (int64_t)p.num_tokens * p.hkv;
+    const int64_t least = total >= QA_RUN * pairs ? QA_RUN : 1;
+    const int64_t run = max(run_length(total, (int64_t)gridDim.x * WARPS), least);
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.run[0] = run;
+    x0 = me * run;
+    count = (int)max((int64_t)0, min(total, x0 + run) - x0);
+    if (count > 0) {
+      const RunPlace r = find_run<THREADS>(counted, p.num_tokens, p.hkv, x0, steps);
+      now = QaPlace{r.entry, r.head, r.step, qa_item(p, r.entry)};
+    } else {
+      now = QaPlace{-1, 0, 0, QaItem{0, 0, 0, 0}};
+    }
+  }
+  if (lane == 0) places[warp] = ahead[warp] = now;
+  // Whether all warps of the CTA are at one pair, to its run's end: their parts become one then.
+  if (lane == 0) ends[warp] = now.step + count;
+  __syncthreads();
+  bool joint = p.direct;
+  if (!p.direct) {
+    const int w = min(lane, WARPS - 1);
+    const QaPlace first = places[0], other = places[w];
+    joint = __all_sync(0xffffffffu, other.token < 0 || (other.token == first.token &&
+                                                        other.head == first.head &&
+                                                        ends[w] <= other.it.steps));
+    if (first.token < 0) return;
+  }
 
   uint8_t* ring = ring_all + warp * DEPTH * S::kStage;
   uint64_t* full = bars[warp];
   const int units = p.page / Q4_UNIT;                      // of a page
-  const int count = (int)(x1 - x0);
-  // Copies are looked up QA_AHEAD steps at a time, a lane for each unit.
+  // Copies are looked up QA_AHEAD steps at a time, a lane for each unit, from the place before.
   auto look_up = [&](int k) {
     const int step = k + (lane >> 1), second = lane & 1;
+    QaPlace r = ahead[warp];
+    __syncwarp();
     int unit = -1;
     if (step < count) {
-      const QaPlace r = qa_locate<THREADS>(p, counted, x0 + step);
+      r.advance(p, ((k > 0 ? QA_AHEAD : 0) + (lane >> 1)) * stride);
       const int t = r.step * QA_STEP + second * Q4_UNIT;
       if (t < r.it.len) {
         const int at = t / p.page;
@@ -238,6 +292,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
           atomicOr(p.status, FK_DEV_BAD_PAGE);
       }
     }
+    if (lane == 0) ahead[warp] = r;
     reinterpret_cast<int*>(&where[warp][step & (2 * QA_AHEAD - 1)])[second] = unit;
     __syncwarp();
   };
@@ -273,12 +328,16 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   uint32_t phase = 0;
   while (ok && i < count) {
     // ---------------------------------------------------------------- a new pair
-    const QaPlace now = qa_locate<THREADS>(p, counted, x0 + i);
-    __syncwarp();
-    if (lane == 0) places[warp] = now;
-    __syncwarp();
-    const int begin = i, last = i + max(1, min(now.it.steps - now.step, count - i));
-    const int step0 = now.step - i;                        // of the pair, at i = 0
+    if (i > 0) {
+      now = places[warp];
+      now.advance(p, now.it.steps - now.step);
+      __syncwarp();
+      if (lane == 0) places[warp] = now;
+      __syncwarp();
+    }
+    const int begin = i;
+    const int last = p.direct ? count : i + max(1, min(now.it.steps - now.step, count - i));
+    const int step0 = now.step - i * stride;               // of the pair, at i = 0
     int shortest = 0x7fffffff;
     {
 #pragma unroll
@@ -366,7 +425,8 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
       }
       const uint8_t* st = ring + slot * S::kStage;
       const int2 w = where[warp][i & (2 * QA_AHEAD - 1)];
-      const bool edge = step0 + i >= safe || (w.x | w.y) < 0;
+      const int step = step0 + i * stride;
+      const bool edge = step >= safe || (w.x | w.y) < 0;
 
       // ---- logits: rows are tokens row, row + 8 of unit `lu` ----
       float z[SETS][NT][4];                                 // [set][.][row: 2 columns, row + 8: 2]
@@ -450,7 +510,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
             }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int t = (step0 + i) * QA_STEP + lu * Q4_UNIT + row + 8 * r;
+            const int t = step * QA_STEP + lu * Q4_UNIT + row + 8 * r;
             const bool there = (lu ? w.y : w.x) >= 0 && t < at.it.len;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr)
@@ -603,7 +663,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
     if (!ok) break;
     // ------------------------------------------------------------------- the pair's end
     const QaPlace done = places[warp];
-    const bool whole = done.step == 0 && step0 + i == done.it.steps;
+    const bool whole = done.step == 0 && step0 + i == done.it.steps && !joint;
     const int64_t place = 2 * me + (begin > 0 ? 1 : 0);
     const float vback = 1.f / vinv;
 #pragma unroll
@@ -649,14 +709,16 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
                                       (int64_t)(done.head * p.g + col - tok * p.g) * Q4_D + 64 * h +
                                       8 * row) = w;
           } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + (place * p.cols + col) * Q4_D +
-                                                    64 * h + 8 * row);
+            float* part = joint ? reinterpret_cast<float*>(ring) + col * Q4_D
+                                : p.part_o + (place * p.cols + col) * Q4_D;
+            float4* dst = reinterpret_cast<float4*>(part + 64 * h + 8 * row);
             dst[0] = make_float4(v[0], v[1], v[2], v[3]);
             dst[1] = make_float4(v[4], v[5], v[6], v[7]);
           }
         }
         if (row == 0) {
-          if (!whole) p.part_ml[place * p.cols + col] = make_float2(ref[nt][j], sum);
+          if (joint) part_ml[warp][col] = make_float2(ref[nt][j], sum);
+          else if (!whole) p.part_ml[place * p.cols + col] = make_float2(ref[nt][j], sum);
           else if (SUMS)
             p.whole_ml[((int64_t)done.token * p.hkv + done.head) * p.cols + col] =
                 make_float2(ref[nt][j], inv);
@@ -670,94 +732,142 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
       if (++slot == DEPTH) { slot = 0; phase ^= 1; }
     }
   }
+  if (!joint) return;
+
+  // ---- parts of the CTA's warps, in their rings, become one ----
+  if (count == 0 || !ok)
+    for (int c = lane; c < COLS; c += 32) part_ml[warp][c] = make_float2(QA_NONE, 0.f);
+  __syncthreads();
+  const QaPlace done = places[0];
+  const int64_t place = 2 * (int64_t)blockIdx.x * WARPS;
+  for (int c = warp; c < done.it.tokens * p.g; c += WARPS) {
+    float M = QA_NONE, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, part_ml[w][c].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 ml = part_ml[w][c];
+      if (ml.y == 0.f) continue;
+      const float f = fast_exp2(ml.x - M);
+      const float4 v = reinterpret_cast<const float4*>(ring_all + w * DEPTH * S::kStage)[c * 32 + lane];
+      L = fmaf(ml.y, f, L);
+      acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+    }
+    if (p.direct) {
+      const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+      const int tok = c / p.g;
+      reinterpret_cast<uint2*>(p.out + (int64_t)(done.token + tok) * p.out_stride +
+                               (int64_t)(done.head * p.g + c - tok * p.g) * Q4_D)[lane] =
+          make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    } else {
+      reinterpret_cast<float4*>(p.part_o + (place * p.cols + c) * Q4_D)[lane] = acc;
+      // the first warp's part is all of them
+      if (lane < WARPS)
+        p.part_ml[(place + 2 * lane) * p.cols + c] =
+            lane == 0 ? make_float2(M, L) : make_float2(QA_NONE, 0.f);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
 // join of partial results
 // ---------------------------------------------------------------------------
-// The runs that a pair's steps lie in: warps a .. b; warp a has the pair in its second place unless
-// the pair begins with the run.
-struct QaRuns {
-  int64_t px, a, b;
-  int second;
-  __device__ __forceinline__ int64_t place(int64_t w) const { return 2 * w + (w == a ? second : 0); }
-};
-__device__ __forceinline__ QaRuns qa_runs(const Q4AttnParams& p, int token, int head, int64_t steps) {
-  const int64_t run = p.run[0];
-  QaRuns r;
-  r.px = p.first[token] * p.hkv + head * steps;
-  r.a = r.px / run;
-  r.b = (r.px + steps - 1) / run;
-  r.second = r.px > r.a * run ? 1 : 0;
-  return r;
-}
-
-// (maximum, sum of weights) of a column over all parts; all lanes of a warp.
-__device__ __forceinline__ float2 qa_total(const Q4AttnParams& p, const QaRuns& r, int col) {
-  const int lane = threadIdx.x & 31;
-  float M = QA_NONE;
-  for (int64_t w = r.a + lane; w <= r.b; w += 32)
-    M = fmaxf(M, p.part_ml[r.place(w) * p.cols + col].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float L = 0.f;
-  for (int64_t w = r.a + lane; w <= r.b; w += 32) {
-    const float2 v = p.part_ml[r.place(w) * p.cols + col];
-    L += v.y * fast_exp2(v.x - M);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  return make_float2(M, L);
-}
+// A CTA has `block_cols` columns of a pair, and as many warps for each as there are then: they take
+// its parts in turn, QA_PARTS loads of a part on their way at a time.
+constexpr int QA_PARTS = 4;
 
 template <bool SUMS>
-__global__ void __launch_bounds__(QA_THREADS) q4_attn_join_kernel(const Q4AttnParams p) {
+__global__ void __launch_bounds__(QA_THREADS) q4_attn_join_kernel(const Q4AttnParams p,
+                                                                  int block_cols) {
+  __shared__ float4 shares[QA_WARPS][32];
+  __shared__ float2 totals[QA_WARPS];
   pdl_launch_dependents();
   pdl_wait();
-  const int token = blockIdx.x / p.hkv, head = blockIdx.x - token * p.hkv;
+  const int groups = (p.cols + block_cols - 1) / block_cols;
+  const int pair = blockIdx.x / groups, group = blockIdx.x - pair * groups;
+  const int token = pair / p.hkv, head = pair - token * p.hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t steps = p.first[token + 1] - p.first[token];
+  const int slices = QA_WARPS / block_cols, slice = warp % slices;
+  const int c = group * block_cols + warp / slices;
+  const int64_t before = p.first[token], steps = p.first[token + 1] - before, run = p.run[0];
+  const QaItem it = p.cu || steps == 0 ? qa_item(p, token) : QaItem{token, 1, 0, 0};
+  const int tok = c / p.g;
+  const bool mine = tok < it.tokens;
+  uint2* out = reinterpret_cast<uint2*>(p.out + (int64_t)(token + tok) * p.out_stride +
+                                        (int64_t)(head * p.g + c - tok * p.g) * Q4_D) + lane;
   if (steps == 0) {
-    const QaItem it = qa_item(p, token);
-    for (int c = warp; c < it.tokens * p.g; c += QA_WARPS) {
-      const int tok = c / p.g;
-      reinterpret_cast<uint2*>(p.out + (int64_t)(token + tok) * p.out_stride +
-                               (int64_t)(head * p.g + c - tok * p.g) * Q4_D)[lane] =
-          make_uint2(0u, 0u);
-    }
+    if (mine && slice == 0) *out = make_uint2(0u, 0u);
     return;
   }
-  const QaRuns r = qa_runs(p, token, head, steps);
-  if (r.a == r.b) return;
-  const int tokens = p.cu ? qa_item(p, token).tokens : 1;
-  for (int c = warp; c < tokens * p.g; c += QA_WARPS) {
-    const float2 all = qa_total(p, r, c);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int64_t w0 = r.a; w0 <= r.b; w0 += 4) {
-      float4 v[4];
-      float f[4];
+  // the runs that the pair's steps lie in: a .. a + n - 1; the first has it in its second place
+  // unless the pair begins with the run
+  const int64_t px = before * p.hkv + head * steps, pe = px + steps - 1;
+  const int64_t a = pe >> 31 ? px / run : (int64_t)((uint32_t)px / (uint32_t)run);
+  const int n = (int)((pe >> 31 ? pe / run : (int64_t)((uint32_t)pe / (uint32_t)run)) - a) + 1;
+  if (n == 1) return;
+  const int second = px > a * run ? 1 : 0;
+  auto place = [&](int w) { return (2 * (a + w) + (w == 0 ? second : 0)) * p.cols + c; };
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 all = make_float2(QA_NONE, 0.f);
+  const int per = (n + slices - 1) / slices, end = min(n, (slice + 1) * per);
+  for (int w0 = slice * per; mine && w0 < end; w0 += 32) {
+    // (maximum, sum) of 32 parts, then those that are any
+    const float2 ml = w0 + lane < end ? p.part_ml[place(w0 + lane)] : make_float2(QA_NONE, 0.f);
+    float M = fmaxf(all.x, ml.x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t w = w0 + i <= r.b ? w0 + i : r.b;
-        const int64_t at = r.place(w) * p.cols + c;
-        v[i] = reinterpret_cast<const float4*>(p.part_o + at * Q4_D)[lane];
-        f[i] = w0 + i <= r.b ? fast_exp2(p.part_ml[at].x - all.x) : 0.f;
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float f = fast_exp2(ml.x - M), old = fast_exp2(all.x - M);
+    float L = ml.y * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    all = make_float2(M, fmaf(all.y, old, L));
+    acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+    uint32_t any = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    while (any) {
+      float4 v[QA_PARTS];
+      float g[QA_PARTS];
+#pragma unroll
+      for (int i = 0; i < QA_PARTS; ++i) {
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        g[i] = 0.f;
+        if (!any) continue;
+        const int w = __ffs(any) - 1;
+        any &= any - 1;
+        v[i] = reinterpret_cast<const float4*>(p.part_o + place(w0 + w) * Q4_D)[lane];
+        g[i] = __shfl_sync(0xffffffffu, f, w);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (w0 + i > r.b) break;
-        acc.x = fmaf(v[i].x, f[i], acc.x); acc.y = fmaf(v[i].y, f[i], acc.y);
-        acc.z = fmaf(v[i].z, f[i], acc.z); acc.w = fmaf(v[i].w, f[i], acc.w);
+      for (int i = 0; i < QA_PARTS; ++i) {
+        acc.x = fmaf(v[i].x, g[i], acc.x); acc.y = fmaf(v[i].y, g[i], acc.y);
+        acc.z = fmaf(v[i].z, g[i], acc.z); acc.w = fmaf(v[i].w, g[i], acc.w);
       }
     }
-    const float inv = all.y > 0.f ? 1.f / all.y : all.y == 0.f ? 0.f : all.y;
-    if (SUMS && lane == 0)
-      p.whole_ml[((int64_t)token * p.hkv + head) * p.cols + c] = make_float2(all.x, inv);
-    const int tok = c / p.g;
-    reinterpret_cast<uint2*>(p.out + (int64_t)(token + tok) * p.out_stride +
-                             (int64_t)(head * p.g + c - tok * p.g) * Q4_D)[lane] =
-        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
   }
+  if (slices > 1) {
+    shares[warp][lane] = acc;
+    if (lane == 0) totals[warp] = all;
+    __syncthreads();
+    if (slice != 0) return;
+    float M = all.x;
+    for (int i = 1; i < slices; ++i) M = fmaxf(M, totals[warp + i].x);
+    const float old = fast_exp2(all.x - M);
+    acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+    all = make_float2(M, all.y * old);
+    for (int i = 1; i < slices; ++i) {
+      const float2 t = totals[warp + i];
+      const float4 v = shares[warp + i][lane];
+      const float f = fast_exp2(t.x - M);
+      all.y = fmaf(t.y, f, all.y);
+      acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+    }
+  }
+  if (!mine) return;
+  const float inv = all.y > 0.f ? 1.f / all.y : all.y == 0.f ? 0.f : all.y;
+  if (SUMS && lane == 0) p.whole_ml[(int64_t)pair * p.cols + c] = make_float2(all.x, inv);
+  *out = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
 struct QaLayout {
@@ -801,7 +911,8 @@ static cudaError_t qa_launch(const Q4AttnParams& p, int sms, cudaStream_t s) {
   auto kernel = q4_attn_kernel<NG, COLS, SUMS>;
   const cudaError_t e = set_max_dynamic_smem(once, kernel, Shape::kSmem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(sms * Shape::kCtas), dim3(Shape::kThreads), (size_t)Shape::kSmem, s,
+  const int grid = p.direct ? p.num_tokens * p.hkv : sms * Shape::kCtas;
+  return launch_kernel(kernel, dim3(grid), dim3(Shape::kThreads), (size_t)Shape::kSmem, s,
                        p);
 }
 template <int NG, bool SUMS>
@@ -887,17 +998,30 @@ int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
   p.whole_ml = reinterpret_cast<float2*>(ws + w.whole_ml);
   p.logits = reinterpret_cast<float*>(ws + w.logits);
   p.logit_steps = w.logit_steps;
-  const int64_t blocks = (int64_t)num_tokens * num_kv_heads;
+  // A small call -- each pair has a CTA of its own at once, and tables of at most 2048 tokens leave
+  // the CTA's warps little to do each -- is one launch, without runs, parts or join (1 x 500
+  // tokens: 7 us, 13).
+  const int64_t pairs = (int64_t)num_tokens * num_kv_heads;
+  const int sms = sm_count();
+  p.direct = !sums && pairs <= (p.cols <= 8 ? 2 : 1) * sms && p.capacity <= 2048;
+  // Few pairs have many parts each: then all of a joining CTA's warps take one column.
+  int block_cols = 1;
+  while (block_cols < 8 && block_cols < p.cols &&
+         pairs * ((p.cols + 2 * block_cols - 1) / (2 * block_cols)) >= 2 * sms)
+    block_cols *= 2;
+  const int64_t blocks = pairs * ((p.cols + block_cols - 1) / block_cols);
   FK_REQUIRE(blocks < (1ll << 31), FK_ERR_UNSUPPORTED, "%s: too many tokens", what);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int sms = sm_count();
   const cudaError_t e =
       sums ? group == 64 ? qa_launch<2, true>(p, sms, s) : qa_launch<1, true>(p, sms, s)
            : group == 64 ? qa_launch<2, false>(p, sms, s) : qa_launch<1, false>(p, sms, s);
   FK_CUDA_OK(e);
+  count_launch(1);
+  if (p.direct) return FK_OK;
   auto join = sums ? q4_attn_join_kernel<true> : q4_attn_join_kernel<false>;
-  FK_CUDA_OK(launch_kernel(join, dim3((unsigned)blocks), dim3(QA_THREADS), (size_t)0, s, p));
-  count_launch(2);
+  FK_CUDA_OK(launch_kernel(join, dim3((unsigned)blocks), dim3(QA_THREADS), (size_t)0, s, p,
+                           block_cols));
+  count_launch(1);
   if (!sums) return FK_OK;
   SumsParams a{};
   a.lens = context_lens; a.cu = cu_seqlens_q;

@@ -56,17 +56,19 @@ struct RunPlace {
   int entry, head, step;
 };
 
-// Place of step x, which is below the number of all.
+// Place of step x, which is below the number of all; by all lanes of a warp, for the same x.
 template <int THREADS, class Steps>
 __device__ __forceinline__ RunPlace find_run(const RunCount<THREADS>& c, int n, int heads, int64_t x,
                                              Steps steps) {
   // (32-bit divisions where they do)
   const int64_t at = x >> 31 ? x / heads : (int64_t)((uint32_t)x / (uint32_t)heads);
-  int lo = 0, hi = THREADS;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (c.begins[mid] <= at) lo = mid; else hi = mid;
-  }
+  // the last thread that begins at or before it, in two rounds of a look by every lane
+  constexpr int PER = THREADS / 32;
+  const int lane = threadIdx.x & 31;
+  const uint32_t group = __ballot_sync(0xffffffffu, c.begins[lane * PER] <= at);
+  const int g = (31 - __clz(group)) * PER;
+  const uint32_t in_group = __ballot_sync(0xffffffffu, lane < PER && c.begins[g + lane] <= at);
+  const int lo = g + 31 - __clz(in_group);
   int64_t before = c.begins[lo];
   RunPlace r;
   r.entry = min(lo * entries_of_thread(n, THREADS), n - 1);
