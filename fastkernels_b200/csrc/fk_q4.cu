@@ -36,6 +36,33 @@ __device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b) {
   return r;
 }
 
+// Two fp32 side by side.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both_of(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Unit of a slot's token for a head, and the token's place in it; null where there is none.
 __device__ __forceinline__ uint8_t* q4_unit(const Q4MoveParams& p, int64_t row, int head,
                                             int unit_bytes, int* token) {
@@ -52,25 +79,16 @@ __device__ __forceinline__ uint8_t* q4_unit(const Q4MoveParams& p, int64_t row, 
   return p.pool + ((page * p.hkv + head) * (p.page / Q4_UNIT) + at / Q4_UNIT) * unit_bytes;
 }
 
-// Nearest integer of (x - lo) / s to 15, exactly, from halves of lo and s (exact, and no difference
-// of finite values overflows).  The quotient's own error (three roundings, below 2^-18 of 16) is
-// far below 2^-12, so a quotient that is not that close to a half is on the right side of it; others
-// are compared with (k + 1/2) s, which fp32 holds exactly, as is the difference of two numbers that
-// close, and the rounding of x - lo is made up for.
-__device__ __forceinline__ uint32_t q4_code(float x, float lo_half, float s_half, float inv,
-                                            bool tiny) {
-  const float d = fmaf(x, 0.5f, -lo_half);
-  const float y = fminf(tiny ? d / s_half : d * inv, 15.f);
-  const float k = floorf(y);
-  if (fabsf(y - k - 0.5f) < 0.000244140625f) {
-    const float x_half = x * 0.5f;
-    const float back = d - x_half;                   // two-sum: x / 2 - lo / 2 = d + e
-    const float e = (x_half - (d - back)) + (-lo_half - back);
-    const float over = (d - (k + 0.5f) * s_half) + e;
-    const int ki = (int)k;
-    return (uint32_t)(over > 0.f || (over == 0.f && (ki & 1)) ? ki + 1 : ki);
-  }
-  return __float_as_uint(y + 8388608.f) & 15u;       // to nearest
+// The code of x in a group whose step is near the ends of fp32's range, where 1 / s or x - lo may
+// not be a number: from halves, by division.  Only such groups come here.
+__device__ __noinline__ uint32_t q4_code_far(float x, float lo, float s) {
+  const float h = s * 0.5f, d = fmaf(x, 0.5f, -lo * 0.5f);
+  const float y = fminf(d / h, 15.f), k = floorf(y);
+  const float back = d - x * 0.5f;                   // two-sum: x / 2 - lo / 2 = d + e
+  const float e = (x * 0.5f - (d - back)) + (-lo * 0.5f - back);
+  // (near a half the products and differences are exact)
+  const float over = fabsf(y - k - 0.5f) < 0.000244140625f ? (d - (k + 0.5f) * h) + e : y - k - 0.5f;
+  return (uint32_t)k + (over > 0.f || (over == 0.f && ((int)k & 1)));
 }
 
 // One row: the lane's 8 channels into a word, with the pair of its group.
@@ -93,15 +111,47 @@ __device__ __forceinline__ uint32_t q4_pack(const uint4& x, uint32_t* pair) {
   }
   *pair = (__float_as_uint(s) >> 16) | (__float_as_uint(lo) & 0xffff0000u);
   if (s == 0.f) return 0u;
-  const bool tiny = s < 1e-30f;                      // 1 / s might not be finite
-  const float lo_half = lo * 0.5f, s_half = s * 0.5f;
-  const float inv = tiny ? 0.f : 1.0f / s_half;
+  // The plain way, where 1 / s is a number and x - lo too, two channels at a time: three roundings
+  // and the reciprocal's put the quotient less than 2^-18 off, so that one that is 2^-17 from a
+  // half is on the right side of it.
+  constexpr float kWhole = 8388608.f;                // its sum with a code is a whole number
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t word = 0u;
+  const float inv = rcp_approx(s);
+  const uint64_t inv2 = pair_of(inv, inv), low2 = pair_of(-lo, -lo);
+  const uint64_t up = pair_of(kWhole, kWhole), down = pair_of(-kWhole, -kWhole);
+  const uint64_t one = pair_of(-1.f, -1.f);
+  float far = s > 1e-30f && s < 1e30f ? 0.f : 1.f;   // largest distance from a code
+  float2 r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    word |= q4_code(bf16lo(w[i]), lo_half, s_half, inv, tiny) << (8 * i);
-    word |= q4_code(bf16hi(w[i]), lo_half, s_half, inv, tiny) << (8 * i + 4);
+    const uint64_t d = add2(pair_of(bf16lo(w[i]), bf16hi(w[i])), low2);
+    const uint64_t c = add2(fma2(d, inv2, up), down);          // to nearest, even on ties
+    const float2 e = both_of(fma2(d, inv2, fma2(c, one, 0ull)));
+    far = fmaxf(far, fmaxf(fabsf(e.x), fabsf(e.y)));
+    r[i] = both_of(c);
+  }
+  // 16 bits of four codes, a number that fp32 holds
+  const float half0 = fmaf(r[1].y, 4096.f, fmaf(r[1].x, 256.f, fmaf(r[0].y, 16.f, r[0].x)));
+  const float half1 = fmaf(r[3].y, 4096.f, fmaf(r[3].x, 256.f, fmaf(r[2].y, 16.f, r[2].x)));
+  uint32_t word = __byte_perm(__float_as_uint(half0 + kWhole), __float_as_uint(half1 + kWhole), 0x5410);
+  if (far >= 0.5f - 7.62939453125e-06f) {
+    // Closer: what is left of x - lo = d + e (two-sum) beyond code c is exact, and compared with
+    // s / 2.  Halves are frequent: keys and values are bf16, as is s.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = i & 1 ? bf16hi(w[i >> 1]) : bf16lo(w[i >> 1]);
+      if (far == 1.f) {
+        word = (word & ~(15u << (4 * i))) | q4_code_far(v, lo, s) << (4 * i);
+        continue;
+      }
+      const float c = i & 1 ? r[i >> 1].y : r[i >> 1].x;
+      const float d = v - lo, left = fmaf(-c, s, d), over = fabsf(left) - 0.5f * s;
+      if (over < s * -7.62939453125e-06f) continue;
+      const float back = d - v, e = (v - (d - back)) + (-lo - back);
+      const float more = over + (left > 0.f ? e : -e);
+      if (more > 0.f || (more == 0.f && ((word >> (4 * i)) & 1u)))
+        word += left > 0.f ? 1u << (4 * i) : ~0u << (4 * i);
+    }
   }
   return word;
 }
@@ -118,27 +168,32 @@ __device__ __forceinline__ uint4 q4_unpack(uint32_t word, uint32_t pair) {
 }
 
 constexpr int Q4_MOVE_THREADS = 256;
-constexpr int Q4_MOVE_HEADS = 2;             // (token, head) pairs of a lane, key and value each
+constexpr int Q4_MOVE_HEADS = 2;             // heads of a lane's token, key and value each
+
+// A CTA takes Q4_MOVE_HEADS heads of 16 tokens, so that successive tokens fill a unit from one place.
+__device__ __forceinline__ bool q4_place(const Q4MoveParams& p, int u, int64_t* row, int* head) {
+  const int groups = (p.hkv + Q4_MOVE_HEADS - 1) / Q4_MOVE_HEADS;
+  const int64_t tile = blockIdx.x / groups;
+  *row = tile * 16 + (threadIdx.x >> 4);
+  *head = (int)(blockIdx.x - tile * groups) * Q4_MOVE_HEADS + u;
+  return *row < p.rows && *head < p.hkv;
+}
 
 template <int NG>
 __global__ void __launch_bounds__(Q4_MOVE_THREADS) q4_store_kernel(const Q4MoveParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 15;
-  const int64_t total = p.rows * p.hkv;
-  const int64_t first = (int64_t)blockIdx.x * (Q4_MOVE_THREADS / 16) * Q4_MOVE_HEADS +
-                        (threadIdx.x >> 4);
   uint4 x[Q4_MOVE_HEADS][2];
   uint8_t* unit[Q4_MOVE_HEADS];
   int token[Q4_MOVE_HEADS];
 #pragma unroll
   for (int u = 0; u < Q4_MOVE_HEADS; ++u) {
-    const int64_t i = first + u * (Q4_MOVE_THREADS / 16);
+    int64_t row;
+    int head;
     unit[u] = nullptr;
     x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (i < total) {
-      const int64_t row = i / p.hkv;
-      const int head = (int)(i - row * p.hkv);
+    if (q4_place(p, u, &row, &head)) {
       x[u][0] = p.k[row * p.k_stride + head * 16 + lane];
       x[u][1] = p.v[row * p.v_stride + head * 16 + lane];
       unit[u] = q4_unit(p, row, head, q4_unit_bytes(NG), &token[u]);
@@ -164,18 +219,14 @@ __global__ void __launch_bounds__(Q4_MOVE_THREADS) q4_load_kernel(const Q4MovePa
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 15;
-  const int64_t total = p.rows * p.hkv;
-  const int64_t first = (int64_t)blockIdx.x * (Q4_MOVE_THREADS / 16) * Q4_MOVE_HEADS +
-                        (threadIdx.x >> 4);
   uint32_t word[Q4_MOVE_HEADS][2], pair[Q4_MOVE_HEADS][2];
 #pragma unroll
   for (int u = 0; u < Q4_MOVE_HEADS; ++u) {
-    const int64_t i = first + u * (Q4_MOVE_THREADS / 16);
+    int64_t row;
+    int head, token;
     word[u][0] = word[u][1] = pair[u][0] = pair[u][1] = 0u;
-    if (i < total) {
-      const int64_t row = i / p.hkv;
-      int token;
-      const uint8_t* unit = q4_unit(p, row, (int)(i - row * p.hkv), q4_unit_bytes(NG), &token);
+    if (q4_place(p, u, &row, &head)) {
+      const uint8_t* unit = q4_unit(p, row, head, q4_unit_bytes(NG), &token);
       if (unit)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -189,8 +240,10 @@ __global__ void __launch_bounds__(Q4_MOVE_THREADS) q4_load_kernel(const Q4MovePa
   }
 #pragma unroll
   for (int u = 0; u < Q4_MOVE_HEADS; ++u) {
-    const int64_t i = first + u * (Q4_MOVE_THREADS / 16);
-    if (i >= total) break;
+    int64_t row;
+    int head;
+    if (!q4_place(p, u, &row, &head)) break;
+    const int64_t i = row * p.hkv + head;
     p.k_out[i * 16 + lane] = q4_unpack<NG>(word[u][0], pair[u][0]);
     p.v_out[i * 16 + lane] = q4_unpack<NG>(word[u][1], pair[u][1]);
   }
@@ -212,9 +265,9 @@ static int q4_move(const char* what, bool store, const void* k, int64_t k_stride
   FK_REQUIRE(store ? aligned16(k) && aligned16(v) && k_stride % 8 == 0 && v_stride % 8 == 0
                    : aligned16(k_out) && aligned16(v_out),
              FK_ERR_ALIGNMENT, "%s: 16-byte alignment required", what);
-  const int64_t per = (Q4_MOVE_THREADS / 16) * Q4_MOVE_HEADS;
-  FK_REQUIRE(rows < (1ll << 31) && (rows * hkv + per - 1) / per < (1ll << 31), FK_ERR_UNSUPPORTED,
-             "%s: too many tokens", what);
+  const int64_t blocks = (rows + 15) / 16 * ((hkv + Q4_MOVE_HEADS - 1) / Q4_MOVE_HEADS);
+  FK_REQUIRE(rows < (1ll << 31) && blocks < (1ll << 31), FK_ERR_UNSUPPORTED, "%s: too many tokens",
+             what);
   Q4MoveParams p{};
   p.k = static_cast<const uint4*>(k); p.k_stride = k_stride / 8;
   p.v = static_cast<const uint4*>(v); p.v_stride = v_stride / 8;
@@ -225,7 +278,7 @@ static int q4_move(const char* what, bool store, const void* k, int64_t k_stride
   p.hkv = hkv; p.page = page;
   p.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
   p.status = status;
-  const dim3 grid((unsigned)((rows * hkv + per - 1) / per));
+  const dim3 grid((unsigned)blocks);
   auto kernel = store ? group == 64 ? q4_store_kernel<2> : q4_store_kernel<1>
                       : group == 64 ? q4_load_kernel<2> : q4_load_kernel<1>;
   FK_CUDA_OK(launch_kernel(kernel, grid, dim3(Q4_MOVE_THREADS), (size_t)0, s, p));
