@@ -156,7 +156,6 @@ __device__ __forceinline__ uint32_t q4_pack(const uint4& x, uint32_t* pair) {
   return word;
 }
 
-template <int NG>
 __device__ __forceinline__ uint4 q4_unpack(uint32_t word, uint32_t pair) {
   const float s = bf16lo(pair), lo = bf16hi(pair);
   uint32_t out[4];
@@ -171,32 +170,36 @@ constexpr int Q4_MOVE_THREADS = 256;
 constexpr int Q4_MOVE_HEADS = 2;             // heads of a lane's token, key and value each
 
 // A CTA takes Q4_MOVE_HEADS heads of 16 tokens, so that successive tokens fill a unit from one place.
-__device__ __forceinline__ bool q4_place(const Q4MoveParams& p, int u, int64_t* row, int* head) {
-  const int groups = (p.hkv + Q4_MOVE_HEADS - 1) / Q4_MOVE_HEADS;
-  const int64_t tile = blockIdx.x / groups;
-  *row = tile * 16 + (threadIdx.x >> 4);
-  *head = (int)(blockIdx.x - tile * groups) * Q4_MOVE_HEADS + u;
-  return *row < p.rows && *head < p.hkv;
-}
+struct Q4Place {
+  int64_t row;
+  int head, heads;             // the first of so many; none: no row
+  uint8_t* unit;               // of the first head; null: no slot
+  int64_t next;                // bytes to the next head's
+  int token;
+  __device__ __forceinline__ Q4Place(const Q4MoveParams& p, int unit_bytes) {
+    const int groups = (p.hkv + Q4_MOVE_HEADS - 1) / Q4_MOVE_HEADS;
+    const int tile = blockIdx.x / groups;
+    row = (int64_t)tile * 16 + (threadIdx.x >> 4);
+    head = (int)(blockIdx.x - tile * groups) * Q4_MOVE_HEADS;
+    heads = row < p.rows ? min(Q4_MOVE_HEADS, p.hkv - head) : 0;
+    next = (int64_t)(p.page / Q4_UNIT) * unit_bytes;
+    unit = heads > 0 ? q4_unit(p, row, head, unit_bytes, &token) : nullptr;
+  }
+};
 
 template <int NG>
 __global__ void __launch_bounds__(Q4_MOVE_THREADS) q4_store_kernel(const Q4MoveParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 15;
+  const Q4Place at(p, q4_unit_bytes(NG));
   uint4 x[Q4_MOVE_HEADS][2];
-  uint8_t* unit[Q4_MOVE_HEADS];
-  int token[Q4_MOVE_HEADS];
 #pragma unroll
   for (int u = 0; u < Q4_MOVE_HEADS; ++u) {
-    int64_t row;
-    int head;
-    unit[u] = nullptr;
     x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (q4_place(p, u, &row, &head)) {
-      x[u][0] = p.k[row * p.k_stride + head * 16 + lane];
-      x[u][1] = p.v[row * p.v_stride + head * 16 + lane];
-      unit[u] = q4_unit(p, row, head, q4_unit_bytes(NG), &token[u]);
+    if (u < at.heads) {
+      x[u][0] = p.k[at.row * p.k_stride + (at.head + u) * 16 + lane];
+      x[u][1] = p.v[at.row * p.v_stride + (at.head + u) * 16 + lane];
     }
   }
 #pragma unroll
@@ -205,12 +208,13 @@ __global__ void __launch_bounds__(Q4_MOVE_THREADS) q4_store_kernel(const Q4MoveP
     for (int kv = 0; kv < 2; ++kv) {
       uint32_t pair;
       const uint32_t word = q4_pack<NG>(x[u][kv], &pair);
-      if (!unit[u]) continue;
+      if (!at.unit || u >= at.heads) continue;
+      uint8_t* unit = at.unit + u * at.next;
       const int place = kv ? q4_value_place(lane) : q4_key_place(lane);
-      reinterpret_cast<uint32_t*>(unit[u] + kv * Q4_VALUES + token[u] * Q4_ROW)[place] = word;
+      reinterpret_cast<uint32_t*>(unit + kv * Q4_VALUES + at.token * Q4_ROW)[place] = word;
       if (lane % (16 / NG) == 0)
-        reinterpret_cast<uint32_t*>(unit[u] + Q4_PAIRS)[(kv * Q4_UNIT + token[u]) * NG +
-                                                        lane / (16 / NG)] = pair;
+        reinterpret_cast<uint32_t*>(unit + Q4_PAIRS)[(kv * Q4_UNIT + at.token) * NG +
+                                                     lane / (16 / NG)] = pair;
     }
 }
 
@@ -219,33 +223,27 @@ __global__ void __launch_bounds__(Q4_MOVE_THREADS) q4_load_kernel(const Q4MovePa
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 15;
+  const Q4Place at(p, q4_unit_bytes(NG));
   uint32_t word[Q4_MOVE_HEADS][2], pair[Q4_MOVE_HEADS][2];
 #pragma unroll
-  for (int u = 0; u < Q4_MOVE_HEADS; ++u) {
-    int64_t row;
-    int head, token;
-    word[u][0] = word[u][1] = pair[u][0] = pair[u][1] = 0u;
-    if (q4_place(p, u, &row, &head)) {
-      const uint8_t* unit = q4_unit(p, row, head, q4_unit_bytes(NG), &token);
-      if (unit)
+  for (int u = 0; u < Q4_MOVE_HEADS; ++u)
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int place = kv ? q4_value_place(lane) : q4_key_place(lane);
-          word[u][kv] = reinterpret_cast<const uint32_t*>(unit + kv * Q4_VALUES +
-                                                          token * Q4_ROW)[place];
-          pair[u][kv] = reinterpret_cast<const uint32_t*>(
-              unit + Q4_PAIRS)[(kv * Q4_UNIT + token) * NG + lane / (16 / NG)];
-        }
+    for (int kv = 0; kv < 2; ++kv) {
+      word[u][kv] = pair[u][kv] = 0u;
+      if (!at.unit || u >= at.heads) continue;
+      const uint8_t* unit = at.unit + u * at.next;
+      const int place = kv ? q4_value_place(lane) : q4_key_place(lane);
+      word[u][kv] = reinterpret_cast<const uint32_t*>(unit + kv * Q4_VALUES +
+                                                      at.token * Q4_ROW)[place];
+      pair[u][kv] = reinterpret_cast<const uint32_t*>(
+          unit + Q4_PAIRS)[(kv * Q4_UNIT + at.token) * NG + lane / (16 / NG)];
     }
-  }
 #pragma unroll
   for (int u = 0; u < Q4_MOVE_HEADS; ++u) {
-    int64_t row;
-    int head;
-    if (!q4_place(p, u, &row, &head)) break;
-    const int64_t i = row * p.hkv + head;
-    p.k_out[i * 16 + lane] = q4_unpack<NG>(word[u][0], pair[u][0]);
-    p.v_out[i * 16 + lane] = q4_unpack<NG>(word[u][1], pair[u][1]);
+    if (u >= at.heads) break;
+    const int64_t i = at.row * p.hkv + at.head + u;
+    p.k_out[i * 16 + lane] = q4_unpack(word[u][0], pair[u][0]);
+    p.v_out[i * 16 + lane] = q4_unpack(word[u][1], pair[u][1]);
   }
 }
 
