@@ -7,23 +7,21 @@
 // budget - 1.  Sources of the first kind of move lie behind all of its destinations, so these moves
 // run side by side; those of the second kind run in ascending tiles, read before written.
 //
-// One CTA has a sequence and KV head.  The border weight is found by counting: the range of keys
-// (weights as integers of the same order) is cut into 2048 parts, the part with the border into 2048
-// again, so that two or three passes over the keys suffice whatever their distribution; ties go to
-// the lowest places.  The keys of the first tokens are kept in shared memory, those beyond are
-// read again.  Bound by latency (a chain of about ten passes and barriers) until there are rows
-// enough to move; the bytes are 4 a token to decide and each moved row twice.
+// One CTA has a sequence and KV head; its warps have a stretch of the tokens each, a lane every
+// 32nd.  Keys (weights as integers of the same order) of the first EV_KEYS tokens stay in shared
+// memory, those beyond are read again.  The border weight is found by counting: the range of keys is cut into
+// 2048 parts, the part with the border into 2048 again, so that two or three passes suffice whatever
+// their distribution; ties go to the lowest places.  Bound by latency (a chain of loads, passes and
+// barriers) until there are rows enough to move; the bytes are 4 a token to decide and each moved
+// row twice.
 #include "fk_q4.cuh"
 
 namespace fk {
 
-constexpr int EV_THREADS = 512;
-constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;
-constexpr int EV_KEYS = 12288;               // tokens whose keys are kept
+constexpr int EV_KEYS = 14336;               // tokens whose keys are kept
 constexpr int EV_LIST = 2048;                // moves of a round
 constexpr int EV_ROWS = 4;                   // rows that 16 lanes move at a time
-constexpr int EV_TILE = EV_THREADS / 16 * EV_ROWS;
 
 struct EvictParams {
   uint8_t* k;                 // bf16 keys, or the 4-bit pool
@@ -48,15 +46,13 @@ __device__ __forceinline__ uint32_t ev_key(float w) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Place of a token: its page, checked, and the place in it.
-__device__ __forceinline__ int ev_page(const EvictParams& p, const int32_t* table, int token,
-                                       int* at) {
+// (page, place in it) of a token; page -1 if its id is bad.
+__device__ __forceinline__ int2 ev_place(const EvictParams& p, const int32_t* table, int token) {
   const int i = p.page_shift >= 0 ? token >> p.page_shift : token / p.page;
-  *at = token - i * p.page;
   const int page = table[i];
-  if (page >= 0 && page < p.num_pages) return page;
+  if (page >= 0 && page < p.num_pages) return make_int2(page, token - i * p.page);
   if (p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
-  return -1;
+  return make_int2(-1, 0);
 }
 
 // What one of the 16 lanes of a row moves of it.
@@ -70,28 +66,25 @@ struct EvRow {
   uint8_t* a;        // 16 bytes; 4-bit: lanes 0-3 keys, 4-7 values
   uint8_t* b;        // bf16: the value's; 4-bit: lanes 8, 9 the pairs of the key, the value
   float* w;          // lane 0 (bf16), 10
-  __device__ __forceinline__ EvRow(const EvictParams& p, const int32_t* table, int head, int token,
-                                   bool live) {
+  __device__ __forceinline__ EvRow(const EvictParams& p, int head, int2 place) {
     const int lane = threadIdx.x & 15;
     a = b = nullptr;
     w = nullptr;
-    if (!live) return;
-    int at;
-    const int64_t page = ev_page(p, table, token, &at);
-    if (page < 0) return;
+    if (place.x < 0) return;
+    const int at = place.y;
     if constexpr (Q4) {
       const int ng = p.group_pairs;
-      uint8_t* unit = p.k + ((page * p.hkv + head) * (p.page / Q4_UNIT) + at / Q4_UNIT) *
+      uint8_t* unit = p.k + ((int64_t)(place.x * p.hkv + head) * (p.page / Q4_UNIT) + at / Q4_UNIT) *
                                 q4_unit_bytes(ng);
       const int t = at % Q4_UNIT;
       if (lane < 8) a = unit + (lane >> 2) * Q4_VALUES + t * Q4_ROW + (lane & 3) * 16;
       else if (lane < 10) b = unit + Q4_PAIRS + ((lane - 8) * Q4_UNIT + t) * 4 * ng;
-      if (lane == 10) w = p.weights + (page * p.hkv + head) * p.page + at;
+      if (lane == 10) w = p.weights + (int64_t)(place.x * p.hkv + head) * p.page + at;
     } else {
-      const int64_t off = page * p.page_bytes + at * p.token_bytes + head * p.head_bytes + lane * 16;
+      const int64_t off = place.x * p.page_bytes + at * p.token_bytes + head * p.head_bytes + lane * 16;
       a = p.k + off;
       b = p.v + off;
-      if (lane == 0) w = p.weights + (page * p.hkv + head) * p.page + at;
+      if (lane == 0) w = p.weights + (int64_t)(place.x * p.hkv + head) * p.page + at;
     }
   }
   __device__ __forceinline__ void load(const EvictParams& p, EvPiece& x) const {
@@ -114,39 +107,39 @@ struct EvRow {
   }
 };
 
-// Sum over the CTA before this thread, and the total; `red` holds EV_WARPS words.
-__device__ __forceinline__ int ev_scan(int v, int* red, int* total) {
+template <int THREADS>
+struct EvShared {
+  int bins[EV_BINS];
+  int2 from[EV_LIST], to[EV_LIST];             // (page, place)
+  int red[2][THREADS / 32];
+  uint32_t range[2][THREADS / 32];
+  int pick[3];
+};
+
+// Sums over the warps before this one of two numbers that lanes agree on, and the totals.
+template <int THREADS>
+__device__ __forceinline__ int2 ev_before(EvShared<THREADS>& sh, int a, int b, int2* all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 31) red[warp] = incl;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < EV_WARPS; ++w) {
-    if (w < warp) before += red[w];
-    all += red[w];
+  if (lane == 0) {
+    sh.red[0][warp] = a;
+    sh.red[1][warp] = b;
   }
   __syncthreads();
-  *total = all;
-  return before + incl - v;
+  const int x = lane < THREADS / 32 ? sh.red[0][lane] : 0;
+  const int y = lane < THREADS / 32 ? sh.red[1][lane] : 0;
+  const int2 r = make_int2(__reduce_add_sync(0xffffffffu, lane < warp ? x : 0),
+                           __reduce_add_sync(0xffffffffu, lane < warp ? y : 0));
+  *all = make_int2(__reduce_add_sync(0xffffffffu, x), __reduce_add_sync(0xffffffffu, y));
+  __syncthreads();
+  return r;
 }
 
-template <bool Q4>
-__global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictParams p) {
-  extern __shared__ uint32_t kept[];                      // keys of tokens 0 .. p.keys - 1
-  __shared__ int bins[EV_BINS];
-  __shared__ int from_list[EV_LIST], to_list[EV_LIST];
-  __shared__ int red[EV_WARPS];
-  __shared__ uint32_t range[2 * EV_WARPS];
-  __shared__ int pick[3];
+template <bool Q4, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const EvictParams p) {
+  extern __shared__ uint32_t kept[];                       // keys of tokens 0 .. p.keys - 1
+  __shared__ EvShared<THREADS> sh;
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seq = blockIdx.x / p.hkv, head = blockIdx.x - seq * p.hkv;
   const int64_t len = p.lens[seq];
   const int n = len < 0 ? 0 : len > p.capacity ? (int)p.capacity : (int)len;
@@ -156,184 +149,203 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictParams p) 
   }
   if (n <= p.budget) return;
   const int32_t* table = p.tables + (int64_t)seq * p.table_stride;
-  const int M = p.budget - p.last, end = n - p.last;      // candidates: first .. end - 1
-  auto read_key = [&](int i) -> uint32_t {
-    int at;
-    const int64_t page = ev_page(p, table, i, &at);
-    return page < 0 ? 0u : ev_key(p.weights[(page * p.hkv + head) * p.page + at]);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int WARPS = THREADS / 32;
+  const int M = p.budget - p.last, end = n - p.last;       // candidates: first .. end - 1
+  const int stretch = ((end + WARPS - 1) / WARPS + 31) & ~31;
+  const int w0 = min(warp * stretch, end), w1 = min(w0 + stretch, end);
+  const float* weights = p.weights + (int64_t)head * p.page;
+  auto read_key = [&](int t) -> uint32_t {
+    if (t < p.first || t >= w1) return 0u;
+    const int i = p.page_shift >= 0 ? t >> p.page_shift : t / p.page;
+    const int page = table[i];
+    if (page < 0 || page >= p.num_pages) {
+      if (p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
+      return 0u;
+    }
+    return ev_key(weights[(int64_t)page * p.hkv * p.page + (t - i * p.page)]);
   };
-  auto key = [&](int i) -> uint32_t { return i < p.keys ? kept[i] : read_key(i); };
+  // every 32 tokens of the stretch, with this lane's token and key
+  auto each_read = [&](auto f) {
+#pragma unroll 4
+    for (int i = w0; i < w1; i += 32) f(i + lane, read_key(i + lane));
+  };
+  auto each = [&](auto f) {
+    const int w = min(w1, max(w0, p.keys & ~31));
+#pragma unroll 4
+    for (int i = w0; i < w; i += 32) f(i + lane, kept[i + lane]);
+#pragma unroll 1
+    for (int i = w; i < w1; i += 32) f(i + lane, read_key(i + lane));
+  };
 
-  // ---- keys, and their range ----
+  // ---- the range of the candidates' keys ----
   uint32_t lo = ~0u, hi = 0u;
-  for (int i = p.first + threadIdx.x; i < end; i += EV_THREADS) {
-    const uint32_t k = read_key(i);
-    if (i < p.keys) kept[i] = k;
+#pragma unroll 8
+  for (int i = w0; i < w1; i += 32) {
+    const int t = i + lane;
+    const uint32_t k = read_key(t);
+    if (i + 32 <= p.keys) kept[t] = k;
+    if (t < p.first || t >= w1) continue;
     lo = min(lo, k);
     hi = max(hi, k);
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   if (lane == 0) {
-    range[warp] = lo;
-    range[EV_WARPS + warp] = hi;
+    sh.range[0][warp] = lo;
+    sh.range[1][warp] = hi;
   }
+  for (int i = threadIdx.x; i < EV_BINS; i += THREADS) sh.bins[i] = 0;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < EV_WARPS; ++w) {
-    lo = min(lo, range[w]);
-    hi = max(hi, range[EV_WARPS + w]);
-  }
+  lo = __reduce_min_sync(0xffffffffu, lane < WARPS ? sh.range[0][lane] : ~0u);
+  hi = __reduce_max_sync(0xffffffffu, lane < WARPS ? sh.range[1][lane] : 0u);
 
   // ---- the border: `want` of the keys at it stay, all above, none below ----
   int want = M - p.first;
   uint32_t border = hi;
+  bool whole = false;            // all at the border and above stay
   if (want > 0) {
     for (int pass = 0; pass < 3; ++pass) {                 // 32 bits in parts of 11
       const int bits = 32 - __clz(hi - lo);                // 0 when all are one key
       const int shift = bits > 11 ? bits - 11 : 0;
-      for (int i = threadIdx.x; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
-      __syncthreads();
-      for (int i = p.first + threadIdx.x; i < end; i += EV_THREADS) {
-        const uint32_t k = key(i);
-        if (k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> shift], 1);
+      if (pass > 0) {
+        for (int i = threadIdx.x; i < EV_BINS; i += THREADS) sh.bins[i] = 0;
+        __syncthreads();
       }
+      each([&](int t, uint32_t k) {
+        if (t >= p.first && t < w1 && k >= lo && k <= hi) atomicAdd(&sh.bins[(k - lo) >> shift], 1);
+      });
       __syncthreads();
       // from the top: the bin in which the sum reaches `want`
-      constexpr int PER = EV_BINS / EV_THREADS;
+      constexpr int PER = EV_BINS / THREADS;
       int mine[PER], sum = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum += mine[i] = bins[EV_BINS - 1 - (threadIdx.x * PER + i)];
-      int all;
-      int above = ev_scan(sum, red, &all);
+      for (int i = 0; i < PER; ++i) sum += mine[i] = sh.bins[EV_BINS - 1 - (threadIdx.x * PER + i)];
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      int2 all;
+      int above = ev_before<THREADS>(sh, __shfl_sync(0xffffffffu, incl, 31), 0, &all).x + incl - sum;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         if (above < want && above + mine[i] >= want) {
-          pick[0] = EV_BINS - 1 - (threadIdx.x * PER + i);
-          pick[1] = want - above;
-          pick[2] = mine[i];
+          sh.pick[0] = EV_BINS - 1 - (threadIdx.x * PER + i);
+          sh.pick[1] = want - above;
+          sh.pick[2] = mine[i];
         }
         above += mine[i];
       }
       __syncthreads();
-      want = pick[1];
-      const int in_bin = pick[2];
-      const uint32_t at = lo + ((uint32_t)pick[0] << shift);
-      __syncthreads();
-      if (shift == 0 || in_bin == want) {
-        // one key, or the whole bin stays: from its lowest key on
-        border = at;
-        if (shift != 0) want = 0x7fffffff;
-        break;
-      }
-      lo = at;
-      const uint32_t top = at + ((1u << shift) - 1u);
-      hi = top < hi && top >= at ? top : hi;
+      want = sh.pick[1];
+      border = lo + ((uint32_t)sh.pick[0] << shift);
+      whole = sh.pick[2] == want;
+      if (shift == 0 || whole) break;
+      lo = border;
+      const uint32_t top = border + ((1u << shift) - 1u);
+      hi = top < hi && top >= border ? top : hi;
     }
   }
-  // A bin that stays whole: everything from `border` on.  Else keys above it, and `want` at it.
-  const bool whole = want == 0x7fffffff;
 
-  // ---- moves: each warp a stretch of the tokens, in order ----
-  const int stretch = ((end + EV_WARPS - 1) / EV_WARPS + 31) & ~31;
-  const int w0 = min(warp * stretch, end), w1 = min(w0 + stretch, end);
-  int ties = 0;
-  if (!whole) {
-    for (int i = w0; i < w1; i += 32) {
-      const int t = i + lane;
-      ties += __popc(__ballot_sync(0xffffffffu, t >= p.first && t < w1 && key(t) == border));
+  // ---- of the keys at the border those of the first `want` places stay, those below `cut` ----
+  int cut = whole ? 0x7fffffff : 0;
+  int2 all;
+  if (!whole && want > 0) {
+    int here = 0;
+    each([&](int t, uint32_t k) {
+      here += __popc(__ballot_sync(0xffffffffu, t >= p.first && t < w1 && k == border));
+    });
+    int before = ev_before<THREADS>(sh, here, 0, &all).x;
+    if (before < want && before + here >= want) {
+      each([&](int t, uint32_t k) {
+        const uint32_t at = __ballot_sync(0xffffffffu, t >= p.first && t < w1 && k == border);
+        if ((at >> lane & 1u) && before + __popc(at & ((1u << lane) - 1u)) == want - 1)
+          sh.pick[0] = t + 1;
+        before += __popc(at);
+      });
     }
-    if (lane == 0) red[warp] = ties;
     __syncthreads();
-    ties = 0;
-    for (int w = 0; w < warp; ++w) ties += red[w];
-    __syncthreads();
+    cut = sh.pick[0];
   }
-  // stayers of a stretch of 32, given the ties before it
-  auto stays = [&](int i, int& tied) -> uint32_t {
-    const int t = i + lane;
-    bool s = false, tie = false;
-    if (t < w1) {
-      if (t < p.first) {
-        s = true;
-      } else {
-        const uint32_t k = key(t);
-        s = whole ? k >= border : k > border;
-        tie = !whole && k == border;
-      }
-    }
-    if (!whole) {
-      const uint32_t at = __ballot_sync(0xffffffffu, tie);
-      if (tie) s = tied + __popc(at & ((1u << lane) - 1u)) < want;
-      tied += __popc(at);
-    }
-    return __ballot_sync(0xffffffffu, s);
+  // (a place that a moved token has taken counts as one that stays, if it is looked at again)
+  auto stays = [&](int t, uint32_t k) {
+    return t < p.first || k > border || (k == border && t < cut);
   };
-  int free_here = 0, move_here = 0;
-  {
-    int tied = ties;
-    for (int i = w0; i < w1; i += 32) {
-      const uint32_t s = stays(i, tied);
-      const int t = i + lane;
-      free_here += __popc(__ballot_sync(0xffffffffu, t < min(w1, M) && !(s >> lane & 1u)));
-      move_here += __popc(__ballot_sync(0xffffffffu, t < w1 && t >= M && (s >> lane & 1u)));
-    }
-  }
-  int moves, frees;
-  const int free_before = ev_scan(lane == 0 ? free_here : 0, red, &frees);
-  const int move_before = ev_scan(lane == 0 ? move_here : 0, red, &moves);
-  moves = min(moves, frees);                               // they are equal
+  auto freed = [&](int t, uint32_t k) {
+    return __ballot_sync(0xffffffffu, t < min(w1, M) && !stays(t, k));
+  };
+  auto moved = [&](int t, uint32_t k) {
+    return __ballot_sync(0xffffffffu, t < w1 && t >= M && stays(t, k));
+  };
+
+  // ---- moves, in order: lists of them, then the rows ----
   const int half = threadIdx.x >> 4;
-  for (int r0 = 0; r0 < moves; r0 += EV_LIST) {
-    int f = __shfl_sync(0xffffffffu, free_before, 0) - r0;
-    int m = __shfl_sync(0xffffffffu, move_before, 0) - r0;
-    int tied = ties;
-    for (int i = w0; i < w1; i += 32) {
-      const uint32_t s = stays(i, tied);
-      const int t = i + lane;
-      const uint32_t below = (1u << lane) - 1u;
-      const uint32_t fr = __ballot_sync(0xffffffffu, t < min(w1, M) && !(s >> lane & 1u));
-      const uint32_t mv = __ballot_sync(0xffffffffu, t < w1 && t >= M && (s >> lane & 1u));
-      const int fi = f + __popc(fr & below), mi = m + __popc(mv & below);
-      if ((fr >> lane & 1u) && fi >= 0 && fi < EV_LIST) to_list[fi] = t;
-      if ((mv >> lane & 1u) && mi >= 0 && mi < EV_LIST) from_list[mi] = t;
-      f += __popc(fr);
-      m += __popc(mv);
-    }
+  constexpr int TILE = THREADS / 16 * EV_ROWS;
+  const int2 none = make_int2(-1, 0);
+  auto round = [&](int done, auto over) {
+    int2 here = make_int2(0, 0);
+    over([&](int t, uint32_t k) {
+      here.x += __popc(freed(t, k));
+      here.y += __popc(moved(t, k));
+    });
+    here = ev_before<THREADS>(sh, here.x, here.y, &all);
+    here.y -= done;
+    over([&](int t, uint32_t k) {
+      const uint32_t fr = freed(t, k), mv = moved(t, k), below = (1u << lane) - 1u;
+      const int fi = here.x + __popc(fr & below), mi = here.y + __popc(mv & below);
+      if ((fr >> lane & 1u) && fi < EV_LIST) sh.to[fi] = ev_place(p, table, t);
+      if ((mv >> lane & 1u) && mi >= 0 && mi < EV_LIST) sh.from[mi] = ev_place(p, table, t);
+      here.x += __popc(fr);
+      here.y += __popc(mv);
+    });
     __syncthreads();
-    const int count = min(EV_LIST, moves - r0);
-    for (int j0 = 0; j0 < count; j0 += EV_TILE) {
+    const int count = min(EV_LIST, min(all.x, all.y - done));
+    for (int j0 = 0; j0 < count; j0 += TILE) {
       EvPiece x[EV_ROWS];
 #pragma unroll
       for (int u = 0; u < EV_ROWS; ++u) {
-        const int j = j0 + u * (EV_THREADS / 16) + half;
-        const int t = j < count ? from_list[j] : -1;
-        EvRow<Q4>(p, table, head, t, (unsigned)t < (unsigned)n).load(p, x[u]);
+        const int j = j0 + u * (THREADS / 16) + half;
+        EvRow<Q4>(p, head, j < count ? sh.from[j] : none).load(p, x[u]);
       }
 #pragma unroll
       for (int u = 0; u < EV_ROWS; ++u) {
-        const int j = j0 + u * (EV_THREADS / 16) + half;
-        const int t = j < count ? to_list[j] : -1;
-        EvRow<Q4>(p, table, head, t, (unsigned)t < (unsigned)n).store(p, x[u]);
+        const int j = j0 + u * (THREADS / 16) + half;
+        EvRow<Q4>(p, head, j < count && sh.from[j].x >= 0 ? sh.to[j] : none).store(p, x[u]);
       }
     }
     __syncthreads();
-  }
+    return all.y;
+  };
+  const int moves = round(0, each);
+  for (int done = EV_LIST; done < moves; done += EV_LIST) round(done, each_read);
   // ---- the newest ----
-  for (int j0 = 0; j0 < p.last; j0 += EV_TILE) {
+  const bool apart = n - p.budget >= p.last;               // places and sources are
+  for (int j0 = 0; j0 < p.last; j0 += TILE) {
     EvPiece x[EV_ROWS];
+    int2 from[EV_ROWS], to[EV_ROWS];
 #pragma unroll
     for (int u = 0; u < EV_ROWS; ++u) {
-      const int j = j0 + u * (EV_THREADS / 16) + half;
-      EvRow<Q4>(p, table, head, end + j, j < p.last).load(p, x[u]);
+      const int j = j0 + u * (THREADS / 16) + half;
+      from[u] = j < p.last ? ev_place(p, table, end + j) : none;
+      to[u] = from[u].x >= 0 ? ev_place(p, table, M + j) : none;
     }
-    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < EV_ROWS; ++u) {
-      const int j = j0 + u * (EV_THREADS / 16) + half;
-      EvRow<Q4>(p, table, head, M + j, j < p.last).store(p, x[u]);
-    }
+    for (int u = 0; u < EV_ROWS; ++u) EvRow<Q4>(p, head, from[u]).load(p, x[u]);
+    if (!apart) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < EV_ROWS; ++u) EvRow<Q4>(p, head, to[u]).store(p, x[u]);
   }
+}
+
+template <bool Q4, int THREADS>
+static cudaError_t ev_launch(const EvictParams& p, int64_t pairs, cudaStream_t s) {
+  static PerDeviceOnce once;
+  auto kernel = evict_kernel<Q4, THREADS>;
+  const cudaError_t e = set_max_dynamic_smem(once, kernel, EV_KEYS * 4);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kernel, dim3((unsigned)pairs), dim3(THREADS), (size_t)p.keys * 4, s, p);
 }
 
 static int evict(const char* what, EvictParams& p, bool q4, int64_t num_pages, int page,
@@ -351,6 +363,7 @@ static int evict(const char* what, EvictParams& p, bool q4, int64_t num_pages, i
   FK_REQUIRE(table_cols > 0 && table_stride >= 0, FK_ERR_INVALID_ARG, "%s: bad sizes", what);
   FK_REQUIRE((int64_t)num_seqs * hkv < (1ll << 31), FK_ERR_UNSUPPORTED, "%s: too many sequences",
              what);
+  FK_REQUIRE(num_pages * hkv < (1ll << 31), FK_ERR_UNSUPPORTED, "%s: pool too large", what);
   p.weights = weights; p.lens = lens; p.new_lens = new_lens;
   p.tables = tables; p.table_stride = table_stride;
   const int64_t longest = 1ll << 30;
@@ -358,13 +371,14 @@ static int evict(const char* what, EvictParams& p, bool q4, int64_t num_pages, i
   p.num_pages = (int)num_pages; p.page = page; p.hkv = hkv;
   p.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
   p.budget = budget; p.first = first; p.last = last;
-  p.keys = (int)(p.capacity < EV_KEYS ? p.capacity : EV_KEYS);
+  // whole rounds of 32, up to what the tables can hold
+  p.keys = (int)(p.capacity < EV_KEYS ? (p.capacity + 31) & ~31 : EV_KEYS);
   p.status = status;
-  static PerDeviceOnce once[2];
-  auto kernel = q4 ? evict_kernel<true> : evict_kernel<false>;
-  FK_CUDA_OK(set_max_dynamic_smem(once[q4 ? 1 : 0], kernel, EV_KEYS * 4));
-  FK_CUDA_OK(launch_kernel(kernel, dim3((unsigned)(num_seqs * hkv)), dim3(EV_THREADS),
-                           (size_t)p.keys * 4, s, p));
+  // With a CTA per SM or fewer, 1024 threads each: what one has to pass over and to move is the time.
+  const int64_t pairs = (int64_t)num_seqs * hkv;
+  FK_CUDA_OK(pairs <= sm_count()
+                 ? (q4 ? ev_launch<true, 1024>(p, pairs, s) : ev_launch<false, 1024>(p, pairs, s))
+                 : (q4 ? ev_launch<true, 512>(p, pairs, s) : ev_launch<false, 512>(p, pairs, s)));
   count_launch(1);
   return FK_OK;
 }
