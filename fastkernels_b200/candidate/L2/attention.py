@@ -76,6 +76,19 @@ class LlamaAttention(nn.Module):
         q_size = self.num_heads * self.head_dim
         kv_size = self.num_kv_heads * self.head_dim
         rope = rotary_emb if rotary_emb is not None else self.rotary_emb
+        if self.fused and rope is not None and self.attn.cache_q4 is not None \
+                and hasattr(rope, "activation_cache"):
+            ops.qkv_rope_store(
+                qkv, self.num_heads, self.num_kv_heads, self.head_dim, positions,
+                rope.activation_cache(qkv.dtype, qkv.device),
+                self.q_norm.weight if self.q_norm is not None else None,
+                self.k_norm.weight if self.k_norm is not None else None,
+                self.rms_norm_eps, None, None, None)
+            q = qkv[:, :q_size].view(n, self.num_heads, self.head_dim)
+            k = qkv[:, q_size:q_size + kv_size].view(n, self.num_kv_heads, self.head_dim)
+            v = qkv[:, q_size + kv_size:].view(n, self.num_kv_heads, self.head_dim)
+            self.attn.store_q4(k, v)
+            return self.o_proj(self.attn.attend_q4(q, k, v).reshape(n, q_size))
         if self.fused and rope is not None and self.attn.k_cache.numel() \
                 and hasattr(rope, "activation_cache"):
             ctx = get_context()

@@ -14,6 +14,10 @@ Features of the reference layer this path does not carry raise at construction
 route) or at the call (mixed prefill + decode batches, tree verification); none
 of them is used by the Llama / Qwen3 dense decoders.
 
+`cache_q4`, where the engine has installed one instead of `k_cache` / `v_cache`, is a cache of 4
+bits a value (ops.new_kvcache_q4): tokens are stored to it, decode attends over it, and a prefill
+with block tables over what it gives back.
+
 Page size and pool layout: the two keyword-only arguments win; without them the
 layer follows the backend configuration of the reference engine it is running
 in (HND / 16 on Blackwell), and outside the reference it defaults to NHD / 256.
@@ -23,7 +27,8 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from fastkernels_b200.infra.context import get_context, reference_attn_backend
+from fastkernels_b200 import ops
+from fastkernels_b200.infra.context import get_context, key_slots, reference_attn_backend
 from fastkernels_b200.candidate.L1.flash_attn_decode import FlashAttnDecode
 from fastkernels_b200.candidate.L1.flash_attn_prefill import FlashAttnPrefill
 from fastkernels_b200.candidate.L1.flashinfer_decode import TRTLLMDecode
@@ -55,6 +60,7 @@ class Attention(nn.Module):
         self.sinks = None
         self.attention_chunk_size = None
         self.k_cache = self.v_cache = torch.tensor([])
+        self.cache_q4 = self.q4_workspace = self.q4_status = None
         if block_size is None or kv_layout is None:
             ref = reference_attn_backend()
             ref_block, ref_layout = ref if ref is not None else (256, "NHD")
@@ -112,6 +118,29 @@ class Attention(nn.Module):
                               max_seq_len=ctx.max_context_len,
                               plan_ready=getattr(ctx, "attn_plan_ready", False))
 
+    def store_q4(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        ops.store_kvcache_q4(k, v, self.cache_q4, get_context().slot_mapping,
+                             status=self.q4_status)
+
+    def attend_q4(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """attend() over the cache of 4 bits."""
+        ctx = get_context()
+        if getattr(ctx, "is_mixed", False) or getattr(ctx, "is_tree_verify", False):
+            raise NotImplementedError(
+                "mixed prefill + decode batches and tree verification are not on this path")
+        if not ctx.is_prefill:
+            return ops.paged_decode_attn_q4(q, self.cache_q4, ctx.context_lens, ctx.block_tables,
+                                            self.scale, workspace=self.q4_workspace,
+                                            status=self.q4_status)
+        if ctx.block_tables is not None:
+            # a prompt sees what later tokens will see of it, however it is cut into portions
+            k, v = ops.load_kvcache_q4(self.cache_q4, key_slots(ctx, self._block_size),
+                                       status=self.q4_status)
+        return self.prefill_op(q, k, v, cu_seqlens_q=ctx.cu_seqlens_q,
+                               cu_seqlens_k=ctx.cu_seqlens_k, max_seqlen_q=ctx.max_seqlen_q,
+                               max_seqlen_k=ctx.max_seqlen_k, softmax_scale=self.scale,
+                               causal=True)
+
     def decode_only(self, q: torch.Tensor) -> torch.Tensor:
         return self.attend(q)
 
@@ -121,6 +150,9 @@ class Attention(nn.Module):
         q = query.view(n, self.num_heads, self.head_size)
         k = key.view(n, self.num_kv_heads, self.head_size)
         v = value.view(n, self.num_kv_heads, self.head_size)
+        if self.cache_q4 is not None:
+            self.store_q4(k, v)
+            return self.attend_q4(q, k, v).reshape(n, self.num_heads * self.head_size)
         if self.k_cache.numel() and self.v_cache.numel():
             self.store_kvcache(k, v, self.k_cache, self.v_cache, ctx.slot_mapping)
         o = self.attend(q, k, v)

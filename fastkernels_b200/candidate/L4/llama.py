@@ -48,6 +48,9 @@ class LlamaConfig:
     qk_norm: bool = False
     kv_block_size: int = 256
     kv_layout: str = "NHD"     # "HND" = the reference's B200 default (page size 16)
+    # bits of a cached value: 16, or 4 with one scale for `kv_group` channels (64 or 128)
+    kv_bits: int = 16
+    kv_group: int = 64
     fused_attention_prologue: bool = True
     # decode batches of up to 128 rows on one GPU: run everything between two
     # attention calls as one persistent kernel (fk_decode_block).  Off by default:

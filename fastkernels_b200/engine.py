@@ -135,10 +135,14 @@ class DecodeEngine:
 
     @classmethod
     def from_folder(cls, folder, *, max_tokens: int, max_num_seqs: int, dtype=torch.bfloat16,
-                    **kw):
+                    kv_bits: int = 16, **kw):
         """Engine for the model in a folder (config.json, safetensors), with pages for
-        max_tokens live tokens in all."""
+        max_tokens live tokens in all.  kv_bits=4: a KV cache of 4 bits a value."""
         config, source = load_folder(folder, dtype)
+        if kv_bits != 16:
+            if not hasattr(config, "kv_bits"):
+                raise ValueError(f"{type(config).__name__}: the cache is not kept in {kv_bits} bits")
+            config.kv_bits = kv_bits
         eng = cls(config, init_scale=None, max_num_seqs=max_num_seqs,
                   max_model_len=max_tokens + 1,
                   num_kv_blocks=cls.pages_for(config, max_tokens, max_num_seqs), **kw)
@@ -175,7 +179,19 @@ class DecodeEngine:
         pools = self.kv_cache if isinstance(self.kv_cache, (list, tuple)) \
             else [self.kv_cache[:, li] for li in range(self.kv_cache.shape[1])]
         for pool in pools:
-            pool.normal_(0.0, scale, generator=g)
+            if pool.dtype == torch.uint8:                  # 4 bits a value
+                self._fill_q4_random(pool, scale, g)
+            else:
+                pool.normal_(0.0, scale, generator=g)
+
+    def _fill_q4_random(self, pool, scale, g) -> None:
+        pages, hkv, units, _ = pool.shape
+        slots, piece = pages * units * 16, 1 << 16
+        for a in range(0, slots, piece):
+            at = torch.arange(a, min(slots, a + piece), device=self.device)
+            k, v = (torch.empty((len(at), hkv, 128), dtype=torch.bfloat16, device=self.device)
+                    .normal_(0.0, scale, generator=g) for _ in range(2))
+            ops.store_kvcache_q4(k, v, pool, at)
 
     # ------------------------------------------------------------------ buffers
     def _init_buffers(self) -> None:

@@ -89,6 +89,21 @@ def reference_attn_backend():
     return int(cfg.block_size), ("HND" if cfg.use_trtllm else "NHD")
 
 
+def key_slots(ctx, page_size) -> torch.Tensor:
+    """Cache slots of all keys of a prefill with block tables, in the order of cu_seqlens_k; made once
+    a forward, on the device."""
+    slots = getattr(ctx, "_key_slots", None)
+    if slots is None:
+        ends = ctx.cu_seqlens_k.long()
+        total = ctx.spans[0].total_k if getattr(ctx, "spans", None) else int(ends[-1])
+        t = torch.arange(total, device=ends.device)
+        seq = torch.searchsorted(ends, t, right=True) - 1
+        pos = t - ends[seq]
+        slots = ctx._key_slots = ctx.block_tables[seq, pos // page_size].long() * page_size + \
+            pos % page_size
+    return slots
+
+
 def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0,
                 max_seqlen_k=0, slot_mapping=None, context_lens=None, block_tables=None,
                 max_context_len=0, spans=None, state_slots=None, cu_portions=None,

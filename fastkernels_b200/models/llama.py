@@ -13,6 +13,16 @@ class ServedLlama(LlamaForCausalLM, ServedModel):
     def __init__(self, config: LlamaConfig):
         if config.dtype != torch.bfloat16:
             raise ValueError("the Llama / Qwen3 decoders run in bf16 only")
+        if config.kv_bits not in (16, 4):
+            raise ValueError(f"a cached value has 16 or 4 bits, not {config.kv_bits}")
+        if config.kv_bits == 4:
+            page = config.kv_block_size
+            if config.head_dim != 128 or config.kv_group not in (64, 128) or \
+                    not (page in (16, 32) or page >= 64 and page % 64 == 0) or \
+                    config.num_attention_heads > 16 * config.num_key_value_heads:
+                raise ValueError("a cache of 4 bits takes heads of 128 channels in groups of 64 or "
+                                 "128, pages of 16, 32 or a multiple of 64 tokens, and up to 16 "
+                                 "query heads per KV head")
         super().__init__(config)
 
     # ------------------------------------------------------------------ weights
@@ -92,6 +102,12 @@ class ServedLlama(LlamaForCausalLM, ServedModel):
         c = self.config
         hkv = self.model.layers[0].self_attn.num_kv_heads
         nb = num_blocks[0]
+        if c.kv_bits == 4:          # a pool per layer, keys and values in one
+            pools = []
+            for layer in self.model.layers:
+                pools.append(ops.new_kvcache_q4(nb, block_size, hkv, c.head_dim, c.kv_group, device))
+                layer.self_attn.attn.cache_q4 = pools[-1]
+            return pools
         shape = (nb, hkv, block_size, c.head_dim) if c.kv_layout == "HND" \
             else (nb, block_size, hkv, c.head_dim)
         kv = torch.zeros((2, c.num_hidden_layers, *shape), dtype=c.dtype, device=device)
@@ -103,6 +119,17 @@ class ServedLlama(LlamaForCausalLM, ServedModel):
     def preallocate(self, max_num_seqs, max_model_len, device, max_splits):
         """One split-KV workspace serves every layer (they run back to back on one
         stream)."""
+        if self.config.kv_bits == 4:
+            a = self.model.layers[0].self_attn.attn
+            need = ops.paged_decode_attn_q4_workspace_bytes(max_num_seqs, max_num_seqs, a.num_heads,
+                                                            a.num_kv_heads, a.head_size)
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            status = ops.new_status(device)
+            for layer in self.model.layers:
+                layer.self_attn.attn.q4_workspace = workspace
+                layer.self_attn.attn.q4_status = status
+            self.attn_workspace = workspace
+            return status
         for layer in self.model.layers:
             layer.self_attn.attn.decode_op._max_splits = max_splits
         first = self.model.layers[0].self_attn.attn.decode_op
@@ -117,7 +144,10 @@ class ServedLlama(LlamaForCausalLM, ServedModel):
 
     # -------------------------------------------------------------------- steps
     def begin_decode(self, ctx):
-        """One split-KV schedule per step, shared by every layer."""
+        """One split-KV schedule per step, shared by every layer (over a cache of 4 bits each call
+        makes its own)."""
+        if self.config.kv_bits == 4:
+            return
         att = self.model.layers[0].self_attn.attn
         op = att.decode_op
         ops.paged_decode_attn_plan(ctx.context_lens, ctx.block_tables, self.config.kv_block_size,

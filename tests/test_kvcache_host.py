@@ -221,3 +221,52 @@ def test_ctypes_take_large_sizes():
     assert isinstance(L.fk_q4_unit_bytes(128, 64), int) and L.fk_q4_unit_bytes(128, 64) == 2304
     assert L.fk_q4_unit_bytes(128, 128) == 2176 and L.fk_q4_unit_bytes(64, 64) == 0
     assert ctypes.sizeof(ctypes.c_size_t) == 8
+
+
+# ------------------------------------------------------------------------------- the engine
+def test_configurations_that_have_no_4_bit_cache():
+    from fastkernels_b200.candidate.L4.llama import LlamaConfig
+    from fastkernels_b200.models.llama import ServedLlama
+    small = dict(hidden_size=256, intermediate_size=256, num_hidden_layers=1, num_attention_heads=4,
+                 num_key_value_heads=2, vocab_size=128, max_position_embeddings=64)
+    for kw in (dict(kv_bits=8), dict(kv_bits=4, head_dim=64), dict(kv_bits=4, kv_group=32),
+               dict(kv_bits=4, kv_block_size=48), dict(kv_bits=4, num_attention_heads=34)):
+        with pytest.raises(ValueError):
+            ServedLlama(LlamaConfig(**dict(small, **kw)))
+
+
+def test_slots_of_all_keys_of_a_prefill():
+    from types import SimpleNamespace
+
+    from fastkernels_b200.infra.context import key_slots
+    lens, page = [5, 0, 130, 64], 64
+    tables = torch.tensor([[3, -1, -1], [-1, -1, -1], [7, 1, 0], [2, -1, -1]], dtype=torch.int32)
+    cu = torch.tensor(np.cumsum([0, *lens]), dtype=torch.int32)
+    want = np.concatenate([S.slots_of(t, n, page) for t, n in zip(tables.numpy(), lens)])
+    ctx = SimpleNamespace(cu_seqlens_k=cu, block_tables=tables, spans=None)
+    got = key_slots(ctx, page)
+    np.testing.assert_array_equal(got.numpy(), want)
+    assert key_slots(ctx, page) is got                 # once a forward
+    ctx = SimpleNamespace(cu_seqlens_k=cu, block_tables=tables,
+                          spans=[SimpleNamespace(total_k=sum(lens))])
+    np.testing.assert_array_equal(key_slots(ctx, page).numpy(), want)
+
+
+def test_command_line_and_folder_options():
+    from fastkernels_b200 import engine, generate
+    assert generate.parse_args(["--model", "d", "--prompt", "1"]).kv_bits == 16
+    assert generate.parse_args(["--model", "d", "--prompt", "1", "--kv-bits", "4"]).kv_bits == 4
+    with pytest.raises(SystemExit):
+        generate.parse_args(["--model", "d", "--prompt", "1", "--kv-bits", "8"])
+    plain = SimpleConfig()
+    old = engine.load_folder
+    engine.load_folder = lambda folder, dtype: (plain, None)
+    try:
+        with pytest.raises(ValueError, match="4 bits"):
+            engine.DecodeEngine.from_folder("d", max_tokens=8, max_num_seqs=1, kv_bits=4)
+    finally:
+        engine.load_folder = old
+
+
+class SimpleConfig:
+    """A configuration of a model whose cache is kept in its own type."""
