@@ -179,10 +179,15 @@ struct QaShape {
   static constexpr int kUnit = q4_unit_bytes(NG);
   static constexpr int kStage = 2 * kUnit;
   static constexpr int kCtas = COLS == 16 ? 1 : 2;         // of an SM
-  static constexpr int kWarps = COLS == 16 ? 12 : 8;
+  // 16 columns of two groups need the registers of 8 warps (4 windows of 32 tokens: 158 us, 181
+  // with 12), of one group they do with those of 12 (256 x 64 heads: 114 us, 126 with 8)
+  static constexpr int kWarps = COLS == 16 && NG == 1 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kDepth = COLS == 16 ? 4 : 3;        // steps of a warp's ring
-  static constexpr int kSmem = kWarps * kDepth * kStage;
+  static constexpr int kDepth = 3;                         // steps of a warp's ring
+  // the operand Q^T in registers, or in shared memory: 4 KB a warp
+  static constexpr bool kSharedQ = COLS == 16;
+  static constexpr int kRing = kWarps * kDepth * kStage;
+  static constexpr int kSmem = kRing + (kSharedQ ? kWarps * 4096 : 0);
 };
 
 // NG groups a row; SUMS: logits are kept for the sums of weights.
@@ -316,7 +321,8 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   for (int k = 0; k < DEPTH && k < count; ++k) copy(k, k);
 
   // ---- state of a pair: columns 8 nt + 2 quad + {0, 1} ----
-  uint32_t qf[NT][8][2];
+  uint32_t qf[S::kSharedQ ? 1 : NT][8][2];
+  uint4* qs = reinterpret_cast<uint4*>(ring_all + S::kRing) + warp * 256 + lane;
   float o[8][NT][4];
   // weights are 2^(logit - ref); their sums, and of weights times the value's lowest
   float ref[NT][2], l[NT][2], low[NG][NT][2];
@@ -390,10 +396,16 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
           const float c2 = bf16lo(w[i].y) * up, c3 = bf16hi(w[i].y) * up;
           const float c4 = bf16lo(w[i].z) * up, c5 = bf16hi(w[i].z) * up;
           const float c6 = bf16lo(w[i].w) * up, c7 = bf16hi(w[i].w) * up;
-          qf[nt][2 * i][0] = pack_f16(c0, c4);
-          qf[nt][2 * i][1] = pack_f16(c1 * 0.0625f, c5 * 0.0625f);
-          qf[nt][2 * i + 1][0] = pack_f16(c2, c6);
-          qf[nt][2 * i + 1][1] = pack_f16(c3 * 0.0625f, c7 * 0.0625f);
+          const uint4 q = make_uint4(pack_f16(c0, c4), pack_f16(c1 * 0.0625f, c5 * 0.0625f),
+                                     pack_f16(c2, c6), pack_f16(c3 * 0.0625f, c7 * 0.0625f));
+          if constexpr (S::kSharedQ) {
+            qs[(i * NT + nt) * 32] = q;
+          } else {
+            qf[nt][2 * i][0] = q.x;
+            qf[nt][2 * i][1] = q.y;
+            qf[nt][2 * i + 1][0] = q.z;
+            qf[nt][2 * i + 1][1] = q.w;
+          }
         }
         f *= 16777216.f * p.scale_log2;                    // codes are 2^-24
 #pragma unroll
@@ -447,14 +459,16 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               float (&c)[4] = acc[f][w * NG / 4][nt];
+              uint4 q;
+              if constexpr (S::kSharedQ) q = qs[(w * NT + nt) * 32];
+              else q = make_uint4(qf[nt][2 * w][0], qf[nt][2 * w][1], qf[nt][2 * w + 1][0],
+                                  qf[nt][2 * w + 1][1]);
               const uint32_t a0 = wa[w] & 0x000f000fu, a1 = wb[w] & 0x000f000fu;
               const uint32_t a2 = wa[w] & 0x00f000f0u, a3 = wb[w] & 0x00f000f0u;
-              if (w % (4 / NG) == 0)
-                mma_f16_16816_first(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
-              else
-                mma_f16_16816(c, a0, a1, a2, a3, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              if (w % (4 / NG) == 0) mma_f16_16816_first(c, a0, a1, a2, a3, q.x, q.y);
+              else mma_f16_16816(c, a0, a1, a2, a3, q.x, q.y);
               mma_f16_16816(c, ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
-                            yb & 0x00f000f0u, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+                            yb & 0x00f000f0u, q.z, q.w);
             }
           }
         }
@@ -884,12 +898,20 @@ static int qa_columns(int tokens, int seqs, int g, int* block) {
   *block = n;
   return n * g;
 }
+// A small call -- each pair has a CTA of its own at once, and tables of at most 2048 tokens leave the
+// CTA's warps little to do each -- is one launch, without runs, parts, join or workspace (1 x 500
+// tokens: 7 us, 13).
+static bool qa_direct(int tokens, int hkv, int cols, bool sums, int64_t max_len) {
+  return !sums && max_len > 0 && max_len <= 2048 &&
+         (int64_t)tokens * hkv <= (int64_t)(cols <= 8 ? 2 : 1) * sm_count();
+}
 static QaLayout qa_layout(int tokens, int seqs, int hkv, int g, bool sums, int64_t max_len) {
   auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
   int block;
   const int cols = qa_columns(tokens, seqs, g, &block);
   const size_t places = (size_t)sm_count() * 16 * 2;       // two of each of at most 16 warps an SM
   QaLayout w{};
+  if (qa_direct(tokens, hkv, cols, sums, max_len)) return w;
   w.first = 256;
   w.part_ml = w.first + up(((size_t)tokens + 1) * sizeof(int64_t));
   w.part_o = w.part_ml + up(places * cols * sizeof(float2));
@@ -986,8 +1008,8 @@ int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
   const bool sums = weights != nullptr;
   if (sums && max_context_len < p.capacity) p.capacity = max_context_len;
   const QaLayout w = qa_layout(num_tokens, num_seqs, num_kv_heads, g, sums, p.capacity);
-  FK_REQUIRE(workspace != nullptr && workspace_bytes >= w.total &&
-                 (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
+  FK_REQUIRE(w.total == 0 || (workspace != nullptr && workspace_bytes >= w.total &&
+                              (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0),
              FK_ERR_WORKSPACE, "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", what,
              w.total, workspace_bytes);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -998,12 +1020,9 @@ int fk_paged_decode_attn_q4(const void* q, int64_t q_stride_token, void* out,
   p.whole_ml = reinterpret_cast<float2*>(ws + w.whole_ml);
   p.logits = reinterpret_cast<float*>(ws + w.logits);
   p.logit_steps = w.logit_steps;
-  // A small call -- each pair has a CTA of its own at once, and tables of at most 2048 tokens leave
-  // the CTA's warps little to do each -- is one launch, without runs, parts or join (1 x 500
-  // tokens: 7 us, 13).
   const int64_t pairs = (int64_t)num_tokens * num_kv_heads;
   const int sms = sm_count();
-  p.direct = !sums && pairs <= (p.cols <= 8 ? 2 : 1) * sms && p.capacity <= 2048;
+  p.direct = qa_direct(num_tokens, num_kv_heads, p.cols, sums, p.capacity);
   // Few pairs have many parts each: then all of a joining CTA's warps take one column.
   int block_cols = 1;
   while (block_cols < 8 && block_cols < p.cols &&

@@ -698,7 +698,7 @@ def load_kvcache_q4(cache, slot_mapping, status=None):
     pages, page, hkv, group = _need_cache_q4(dev, cache)
     wide = _need_slots(dev, slot_mapping)
     n = slot_mapping.numel()
-    key, value = (torch.empty((n, hkv, 128), dtype=BF16, device=cache.device) for _ in range(2))
+    key, value = cache.new_empty((2, n, hkv, 128), dtype=BF16).unbind()
     check(lib.fk_load_kvcache_q4(
         key.data_ptr(), value.data_ptr(), cache.data_ptr(), pages, page, hkv, 128, group,
         slot_mapping.data_ptr(), wide, n, _status_of(dev, status, cache), _stream_of(dev)),
@@ -762,10 +762,11 @@ def paged_decode_attn_q4(q, cache, context_lens, block_tables, softmax_scale, cu
     _need_ints(dev, n, "context_lens", context_lens)
     ts, cols, rows = _need_tables(dev, block_tables)
     seqs = _need_sequences(dev, n, cu_seqlens_q, weights_from, rows)
-    longest = 0
+    longest = cols * page
     if weights is not None:
         _need_weights(dev, weights, pages, hkv, page)
-        longest = cols * page if max_context_len is None else min(max_context_len, cols * page)
+        if max_context_len is not None:
+            longest = min(max_context_len, longest)
     out, os_ = _out_like(dev, q, out)
     ws, ws_bytes, _held = _workspace(
         dev, workspace,

@@ -318,7 +318,9 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
  * weights_from[s] on start from 0 (NULL: from the place of the sequence's first query
  * token on, which no token before has seen).  A page is then in one table only.  Contexts
  * of such a call are cut at max_context_len (flagged FK_DEV_BAD_PAGE); the workspace
- * grows with it.
+ * grows with it.  Without weights max_context_len is not read by the call; the workspace
+ * of any tables is that for 0, and for the tokens that tables hold it may be less: none
+ * for few sequences with tables of up to 2048 tokens.
  *
  * fk_paged_decode_attn_weights: the same over bf16 pools, for num_q_heads / num_kv_heads
  * 1, 2, 4, 8 or 16; the keys of a bad page are zeros, as in fk_paged_decode_attn, and have

@@ -103,8 +103,8 @@ def test_pools_that_no_cache_has(fn):
     (attend, dict(qs=1016), INVALID), (attend, dict(os=1028), ALIGNMENT),
     (attend, dict(q=P + 2), ALIGNMENT), (attend, dict(cols=0), INVALID),
     (attend, dict(ts=-1), INVALID), (attend, dict(longest=-1), INVALID),
-    (attend, dict(ws=None), WORKSPACE), (attend, dict(wsb=1000), WORKSPACE),
-    (attend, dict(ws=P + 16), WORKSPACE),
+    (attend, dict(ws=None, cols=64), WORKSPACE), (attend, dict(wsb=1000, cols=64), WORKSPACE),
+    (attend, dict(ws=P + 16, cols=64), WORKSPACE), (attend, dict(ws=None, weights=P), WORKSPACE),
     (attend_bf16, dict(weights=None), INVALID), (attend_bf16, dict(hq=6, qs=768, os=768), UNSUPPORTED),
     (attend_bf16, dict(seqs=2), INVALID), (attend_bf16, dict(layout=2), INVALID),
     (attend_bf16, dict(wsb=1000), WORKSPACE), (attend_bf16, dict(longest=-1), INVALID),
@@ -139,12 +139,13 @@ def test_workspaces():
         return ops.paged_decode_attn_q4_workspace_bytes(n, s, hq, hkv, d, w, longest)
     assert q4() > 0 and q4(n=0) == 0 and q4(hq=200) == 0 and q4(d=64) == 0 and q4(longest=-1) == 0
     assert q4(longest=10 ** 6) == q4()                 # only sums of weights grow with it
+    assert q4(longest=2048) == 0 and q4(longest=2049) == q4() and q4(w=1, longest=2048) > q4()
     assert q4(w=1, longest=8192) - q4(w=1) == 4 * 8 * 8192 * 4 * 4
     assert q4(n=64, s=4) > q4(n=4, s=4)
     need = ops.paged_decode_attn_weights_workspace_bytes(3, 8, 128, 4, False, 256)
     assert attend_bf16(wsb=need - 1) == WORKSPACE and need % 256 == 0
     need = q4(3, 3, 8, 2)
-    assert attend(wsb=need - 1) == WORKSPACE
+    assert attend(wsb=need - 1, cols=64) == WORKSPACE
 
 
 def test_calls_refuse_tensors_on_the_host():
