@@ -183,7 +183,7 @@ struct QaShape {
   // with 12), of one group they do with those of 12 (256 x 64 heads: 114 us, 126 with 8)
   static constexpr int kWarps = COLS == 16 && NG == 1 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kDepth = 3;                         // steps of a warp's ring
+  static constexpr int kDepth = 2;                         // steps of a warp's ring
   // the operand Q^T in registers, or in shared memory: 4 KB a warp
   static constexpr bool kSharedQ = COLS == 16;
   static constexpr int kRing = kWarps * kDepth * kStage;
