@@ -112,6 +112,21 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return r;
 }
 
+// bulk_load of what is read once: it leaves L2 first.
+__device__ __forceinline__ uint64_t qa_policy() {
+  uint64_t r;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(r));
+  return r;
+}
+__device__ __forceinline__ void qa_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar,
+                                        uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
 // Query tokens that go together, and what they see.
 struct QaItem {
   int row;        // table
@@ -307,14 +322,15 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
       const int2 w = where[warp][k & (2 * QA_AHEAD - 1)];
       uint8_t* dst = ring + slot * S::kStage;
       uint64_t* bar = &full[slot];
+      const uint64_t policy = qa_policy();
       if (w.x >= 0 && w.y == w.x + 1) {                    // side by side in the pool
         mbar_arrive_expect_tx(bar, 2 * S::kUnit);
-        bulk_load(dst, p.pool + (int64_t)w.x * S::kUnit, 2 * S::kUnit, bar);
+        qa_load(dst, p.pool + (int64_t)w.x * S::kUnit, 2 * S::kUnit, bar, policy);
       } else {
         mbar_arrive_expect_tx(bar, ((w.x >= 0) + (w.y >= 0)) * S::kUnit);
-        if (w.x >= 0) bulk_load(dst, p.pool + (int64_t)w.x * S::kUnit, S::kUnit, bar);
+        if (w.x >= 0) qa_load(dst, p.pool + (int64_t)w.x * S::kUnit, S::kUnit, bar, policy);
         if (w.y >= 0)
-          bulk_load(dst + S::kUnit, p.pool + (int64_t)w.y * S::kUnit, S::kUnit, bar);
+          qa_load(dst + S::kUnit, p.pool + (int64_t)w.y * S::kUnit, S::kUnit, bar, policy);
       }
     }
   };
