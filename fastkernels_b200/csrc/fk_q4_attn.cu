@@ -285,7 +285,8 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   if (!p.direct) {
     const int w = min(lane, WARPS - 1);
     const QaPlace first = places[0], other = places[w];
-    joint = __all_sync(0xffffffffu, other.token < 0 || (other.token == first.token &&
+    // (a pair that one run has whole is not joined: two warps have to be at it)
+    joint = places[1].token >= 0 && __all_sync(0xffffffffu, other.token < 0 || (other.token == first.token &&
                                                         other.head == first.head &&
                                                         ends[w] <= other.it.steps));
     if (first.token < 0) return;

@@ -644,8 +644,8 @@ def new_kvcache_q4(num_pages, page_size, num_kv_heads, head_dim=128, group=64, d
     unit = int(lib.fk_q4_unit_bytes(head_dim, group))
     if unit == 0:
         raise _lib.FkError(f"no 4-bit cache of heads of {head_dim} in groups of {group}")
-    if page_size < 16 or page_size % 16:
-        raise _lib.FkError("a page of a 4-bit cache is a multiple of 16 tokens")
+    if page_size not in (16, 32) and (page_size < 64 or page_size % 64):
+        raise _lib.FkError("a page of a 4-bit cache has 16, 32 or a multiple of 64 tokens")
     return torch.zeros((num_pages, num_kv_heads, page_size // 16, unit), dtype=_UINT8,
                        device=device)
 

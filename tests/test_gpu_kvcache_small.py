@@ -182,6 +182,23 @@ def test_attention_split_and_whole(ops, lens):
     check(ops, Batch(rng, lens, 8, 2, 64, 64), False)
 
 
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (8, 1), (16, 1), (2, 2)])
+@pytest.mark.parametrize("lens", [[100], [128], [129], [33, 0], [257], [1025], [5, 4000]])
+def test_few_pairs_under_wide_tables(ops, hq, hkv, lens):
+    """Runs of the fewest steps: pairs that one warp has whole, a CTA has alone, or several have."""
+    rng = np.random.default_rng(sum(lens) + hq)
+    b = Batch(rng, lens, hq, hkv, 64, 64)
+    wide = np.full((len(lens), 40), -1, np.int32)
+    wide[:, :min(40, b.tables.shape[1])] = b.tables[:, :40]
+    if max(lens) <= 2048:
+        b.tables = wide
+    check(ops, b, False)
+    w = ops.new_attn_weights(b.tables.max() + 4, 64, hkv)
+    ops.paged_decode_attn_q4(dev(b.q), b.cache(ops), ints(b.q_lens), ints(b.tables), b.scale, weights=w)
+    _, _, reach, sums = b.expect()
+    check_sums(b, w, reach, sums, None)
+
+
 @pytest.mark.parametrize("hq,hkv,group,page", [(8, 2, 64, 64), (5, 5, 128, 16), (16, 1, 64, 32),
                                                (9, 3, 128, 256), (12, 2, 64, 16)])
 @pytest.mark.parametrize("counts", [[1, 4, 1, 7], [0, 40, 0, 3], [2, 2, 2, 2], [1, 1, 1, 1],
