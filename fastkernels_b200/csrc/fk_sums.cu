@@ -29,13 +29,12 @@ __device__ __forceinline__ int sums_most(const SumsParams& p, int2 tokens) {
   return most;
 }
 
-// STEPS at a time; one where there are several query tokens, whose logits are loads enough.  Each
-// grid is the CTAs that SMs hold.
-template <int STEPS>
-constexpr int sums_ctas() { return STEPS == 1 ? 4 : 3; }
+constexpr int SUMS_CTAS = 3;                 // of an SM, all there are
+
+// STEPS at a time; one where there are several query tokens, whose logits are loads enough.
 
 template <int STEPS>
-__global__ void __launch_bounds__(SUMS_THREADS, sums_ctas<STEPS>())
+__global__ void __launch_bounds__(SUMS_THREADS, SUMS_CTAS)
     attn_sums_kernel(const SumsParams p) {
   __shared__ RunCount<SUMS_THREADS> counted;
   pdl_launch_dependents();
@@ -67,7 +66,40 @@ __global__ void __launch_bounds__(SUMS_THREADS, sums_ctas<STEPS>())
         page[j] = key[j] < most ? table[i] : -1;
         sum[j] = 0.f;
       }
-      for (int t = tokens.x; t < tokens.y; t += p.block) {
+      int t = tokens.x;
+      if constexpr (STEPS == 1) {
+        // blocks of 16 columns, two at a time
+        if (p.first && p.cols == 16 && p.ml_col == 1) {
+          for (; t + 2 * p.block <= tokens.y; t += 2 * p.block) {
+            float4 v[2][4], m[2][8];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int u = t + b * p.block;
+              const int64_t before = p.first[u], n = p.first[u + 1] - before;
+              const int64_t row = (before * p.hkv + at.head * n) * 32 + key[0];
+              const bool live = key[0] < n * 32 && row < p.logit_keys;
+              const float4* z = reinterpret_cast<const float4*>(p.logits + row * 16);
+              const float4* ml = reinterpret_cast<const float4*>(
+                  p.ml + ((int64_t)u * p.hkv + at.head) * p.ml_pair);
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                v[b][c] = live ? z[c] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) m[b][c] = ml[c];
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const float x = c & 1 ? v[b][c / 2].z : v[b][c / 2].x;
+                const float y = c & 1 ? v[b][c / 2].w : v[b][c / 2].y;
+                if (x != -INFINITY) sum[0] = fmaf(fast_exp2(x - m[b][c].x), m[b][c].y, sum[0]);
+                if (y != -INFINITY) sum[0] = fmaf(fast_exp2(y - m[b][c].z), m[b][c].w, sum[0]);
+              }
+          }
+        }
+      }
+      for (; t < tokens.y; t += p.block) {
         const int cols = p.cols / p.block * min(p.block, tokens.y - t);
         int64_t base;
         int len;
@@ -138,12 +170,12 @@ __global__ void __launch_bounds__(SUMS_THREADS, sums_ctas<STEPS>())
 
 template <int STEPS>
 static cudaError_t launch_steps(const SumsParams& p, cudaStream_t s) {
-  return launch_kernel(attn_sums_kernel<STEPS>, dim3(sm_count() * sums_ctas<STEPS>()),
+  return launch_kernel(attn_sums_kernel<STEPS>, dim3(sm_count() * SUMS_CTAS),
                        dim3(SUMS_THREADS), (size_t)0, s, p);
 }
 cudaError_t launch_sums(SumsParams p, cudaStream_t s) {
   p.page_shift = (p.page & (p.page - 1)) == 0 ? __builtin_ctz(p.page) : -1;
-  return p.cu ? launch_steps<1>(p, s) : launch_steps<4>(p, s);
+  return p.num_tokens > p.num_seqs ? launch_steps<1>(p, s) : launch_steps<4>(p, s);
 }
 
 }  // namespace fk
