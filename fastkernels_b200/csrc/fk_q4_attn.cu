@@ -22,8 +22,14 @@
 // one for each warp of the grid.  Warps share nothing: each has a ring of steps of its own,
 // filled by bulk copies (a step is one contiguous copy of up to 4.6 KB), and no barrier between.
 // What a warp does not have whole goes to one of its two places of partial results, joined by
-// the kernel behind.  The running maximum is raised only when a logit is 8 above it (weights up to
-// 2^8 fit), so that in most steps nothing is reduced across lanes and nothing rescaled.
+// the kernel behind; where all warps of a CTA are at one pair their parts become one first.  The
+// running maximum is raised only when a logit is 8 above it (weights up to 2^8 fit), so that in
+// most steps nothing is reduced across lanes and nothing rescaled.
+//
+// What bounds it: long contexts of up to 8 columns run at 0.94 of the copy rate once they run (64 x 4096
+// to 64 x 8192 tokens, 32 / 8 heads: 62.5 to 110 us for 302 MB more); the beginning of the runs
+// takes some 9 us, the join 5.  A step is some 490 warp instructions at half of the issue slots.
+// 16 columns are bound by instructions (256 sequences, 64 / 4 heads: 109 us, 2.9 TB/s).
 #include "fk_q4.cuh"
 #include "fk_runs.cuh"
 #include "fk_sums.cuh"
@@ -82,27 +88,37 @@ __device__ __forceinline__ bool qa_wait_warp(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, got);
 }
 
+// KEPT: at its place in the program, as instructions of whole warps whose results lanes choose among
+// have to be; else where the compiler likes (3 % of the time with 16 columns).
+#define FK_QA_MMA(ASM)                                                                          \
+  ASM("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "                                      \
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                                   \
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                          \
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+template <bool KEPT>
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                               uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (KEPT) FK_QA_MMA(asm volatile);
+  else FK_QA_MMA(asm);
 }
+#undef FK_QA_MMA
+#define FK_QA_MMA(ASM)                                                                          \
+  ASM("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "                                      \
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"                               \
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                          \
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f))
 // The same onto nothing.
+template <bool KEPT>
 __device__ __forceinline__ void mma_f16_16816_first(float (&c)[4], uint32_t a0, uint32_t a1,
                                                     uint32_t a2, uint32_t a3, uint32_t b0,
                                                     uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  if constexpr (KEPT) FK_QA_MMA(asm volatile);
+  else FK_QA_MMA(asm);
 }
+#undef FK_QA_MMA
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 // Two fp32 to fp16, lo = a.
@@ -212,6 +228,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   using S = QaShape<NG, COLS>;
   constexpr int DEPTH = S::kDepth, NT = S::kTiles, FOLD = S::kFold, SETS = 2 / FOLD;
   constexpr int WARPS = S::kWarps, THREADS = S::kThreads;
+  constexpr bool KEPT = COLS != 16;
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ uint64_t bars[WARPS][DEPTH];
   __shared__ RunCount<THREADS> counted;
@@ -286,7 +303,8 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
     const int w = min(lane, WARPS - 1);
     const QaPlace first = places[0], other = places[w];
     // (a pair that one run has whole is not joined: two warps have to be at it)
-    joint = places[1].token >= 0 && __all_sync(0xffffffffu, other.token < 0 || (other.token == first.token &&
+    joint = places[1].token >= 0 &&
+            __all_sync(0xffffffffu, other.token < 0 || (other.token == first.token &&
                                                         other.head == first.head &&
                                                         ends[w] <= other.it.steps));
     if (first.token < 0) return;
@@ -482,9 +500,9 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
                                   qf[nt][2 * w + 1][1]);
               const uint32_t a0 = wa[w] & 0x000f000fu, a1 = wb[w] & 0x000f000fu;
               const uint32_t a2 = wa[w] & 0x00f000f0u, a3 = wb[w] & 0x00f000f0u;
-              if (w % (4 / NG) == 0) mma_f16_16816_first(c, a0, a1, a2, a3, q.x, q.y);
-              else mma_f16_16816(c, a0, a1, a2, a3, q.x, q.y);
-              mma_f16_16816(c, ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
+              if (w % (4 / NG) == 0) mma_f16_16816_first<KEPT>(c, a0, a1, a2, a3, q.x, q.y);
+              else mma_f16_16816<KEPT>(c, a0, a1, a2, a3, q.x, q.y);
+              mma_f16_16816<KEPT>(c, ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u,
                             yb & 0x00f000f0u, q.z, q.w);
             }
           }
@@ -677,7 +695,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
               const int mt = 4 * h + 2 * half + k;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma_f16_16816(o[mt][nt], xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu,
+                mma_f16_16816<KEPT>(o[mt][nt], xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu,
                               xb & 0x00f000f0u, pt[u][h * NG / 2][nt][0],
                               pt[u][h * NG / 2][nt][1]);
               xa >>= 8;
