@@ -698,7 +698,8 @@ def load_kvcache_q4(cache, slot_mapping, status=None):
     pages, page, hkv, group = _need_cache_q4(dev, cache)
     wide = _need_slots(dev, slot_mapping)
     n = slot_mapping.numel()
-    key, value = cache.new_empty((2, n, hkv, 128), dtype=BF16).unbind()
+    key = cache.new_empty((n, hkv, 128), dtype=BF16)
+    value = torch.empty_like(key)
     check(lib.fk_load_kvcache_q4(
         key.data_ptr(), value.data_ptr(), cache.data_ptr(), pages, page, hkv, 128, group,
         slot_mapping.data_ptr(), wide, n, _status_of(dev, status, cache), _stream_of(dev)),

@@ -120,3 +120,37 @@ def test_pool_is_smaller_and_filled_at_random():
     small.fill_kv_random(1)
     small.add_sequences([200, 90], [1, 2])
     assert len(small.step(sync=True)) == 2 and small.device_status() == 0
+
+
+def test_command_line_of_a_llama_folder(tmp_path):
+    import io
+    import json
+    import pinuvik_oracle
+    from fastkernels_b200 import generate
+    c = dict(architectures=["LlamaForCausalLM"], hidden_size=256, intermediate_size=256,
+             num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=128,
+             vocab_size=320, max_position_embeddings=512, rms_norm_eps=1e-6, rope_theta=1e4)
+    rng = np.random.default_rng(0)
+
+    def m(*shape):
+        return (rng.standard_normal(shape) * 0.1).astype(np.float32)
+    w = {"model.embed_tokens.weight": m(320, 256), "model.norm.weight": np.ones(256, np.float32)}
+    for i in range(2):
+        h = f"model.layers.{i}."
+        for n in ("input_layernorm", "post_attention_layernorm"):
+            w[h + n + ".weight"] = np.ones(256, np.float32)
+        for n, rows in (("q", 512), ("k", 256), ("v", 256)):
+            w[f"{h}self_attn.{n}_proj.weight"] = m(rows, 256)
+        w[h + "self_attn.o_proj.weight"] = m(256, 512)
+        for n in ("gate", "up", "down"):
+            w[f"{h}mlp.{n}_proj.weight"] = m(256, 256)
+    pinuvik_oracle.write_folder(tmp_path, c, w)
+    assert json.loads((tmp_path / "config.json").read_text())["vocab_size"] == 320
+    outs = []
+    for bits in ("16", "4"):
+        out = io.StringIO()
+        args = ["--model", str(tmp_path), "--prompt", "5,17,3", "--prompt", "9,8,7,6,5,4",
+                "--max-new-tokens", "12", "--kv-bits", bits]
+        assert generate.main(args, stdout=out) == 0
+        outs.append([[int(t) for t in line.split(",")] for line in out.getvalue().split()])
+    assert all(len(line) == 12 for o in outs for line in o) and len(outs[1]) == 2
