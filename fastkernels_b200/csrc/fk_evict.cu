@@ -8,20 +8,34 @@
 // run side by side; those of the second kind run in ascending tiles, read before written.
 //
 // One CTA has a sequence and KV head; its warps have a stretch of the tokens each, a lane every
-// 32nd.  Keys (weights as integers of the same order) of the first EV_KEYS tokens stay in shared
-// memory, those beyond are read again.  The border weight is found by counting: the range of keys is cut into
+// 32nd.  Keys (weights as integers of the same order) stay in shared memory as far as there is room,
+// others are read again.  The border weight is found by counting: the range of keys is cut into
 // 2048 parts, the part with the border into 2048 again, so that two or three passes suffice whatever
 // their distribution; ties go to the lowest places.  Bound by latency (a chain of loads, passes and
-// barriers) until there are rows enough to move; the bytes are 4 a token to decide and each moved
-// row twice.
+// barriers, 11 us for 1100 tokens, then 1 us for 1024 more) until there are rows enough to move; the
+// bytes are 4 a token to decide and each moved row twice.
+//
+// Where there are fewer pairs than half the SMs a cluster of up to 8 CTAs has one: counts, sums and
+// lists go between them by their shared memory, and rows are moved by all.  8 pairs of 12 000 tokens
+// take 20.3 us (alone 22.7), of 40 000 24.4 (52), of 100 000 36 (282).  Barriers and peers' loads cost
+// some 6 us.
 #include "fk_q4.cuh"
+#include "fk_tcgen05.cuh"
 
 namespace fk {
 
 constexpr int EV_BINS = 2048;
-constexpr int EV_KEYS = 14336;               // tokens whose keys are kept
 constexpr int EV_LIST = 2048;                // moves of a round
 constexpr int EV_ROWS = 4;                   // rows that 16 lanes move at a time
+constexpr int EV_RANKS = 8;                  // CTAs of a sequence and head, at most
+// Up to so many CTAs each reads the counts of all; of more one adds up a part for all (8 CTAs: 21.5 us
+// for 32, 3: 24.0 for 23.0).
+constexpr int EV_GATHER = 4;
+// Tokens up to which one CTA of a cluster has them all, and that tables have to hold for clusters
+// (a cluster's launch costs 2.5 us more).
+constexpr int EV_ALONE = 6144, EV_CLUSTER = 10240;
+// Tokens whose keys a CTA keeps: two CTAs of 512 threads are on an SM, or one of 1024.
+__host__ __device__ constexpr int ev_keys(int threads) { return threads == 512 ? 14336 : 43008; }
 
 struct EvictParams {
   uint8_t* k;                 // bf16 keys, or the 4-bit pool
@@ -35,7 +49,8 @@ struct EvictParams {
   int64_t capacity;
   int num_pages, page, page_shift, hkv;
   int budget, first, last;
-  int keys;                   // kept in shared memory
+  int keys;                   // of a CTA's tokens kept in shared memory
+  int ranks;                  // CTAs of a sequence and head: a cluster
   int32_t* status;
 };
 
@@ -107,53 +122,101 @@ struct EvRow {
   }
 };
 
-template <int THREADS>
+__device__ __forceinline__ uint32_t ev_peer(const void* x, int rank) {
+  return cluster_map(smem_u32(x), (uint32_t)rank);
+}
+// (no memory clobber: loads of several peers are on their way together; barriers have one)
+__device__ __forceinline__ int2 ev_peer_load(const int2* x, int rank) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];"
+               : "=r"(v.x), "=r"(v.y)
+               : "r"(ev_peer(x, rank)));
+  return v;
+}
+__device__ __forceinline__ void ev_peer_store(void* x, int rank, int v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(ev_peer(x, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void ev_peer_store(void* x, int rank, int2 v) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(ev_peer(x, rank)), "r"(v.x),
+               "r"(v.y)
+               : "memory");
+}
+
+// `red` and `red_of` are used in turn, with a barrier in each turn: what one holds is read before it is
+// written again.  The same holds for `bins` and, of few CTAs, `sums`.
+template <int THREADS, bool CLUSTER>
 struct EvShared {
-  int bins[EV_BINS];
-  int2 from[EV_LIST], to[EV_LIST];             // (page, place)
-  int red[2][THREADS / 32];
-  uint32_t range[2][THREADS / 32];
+  static constexpr int LIST = CLUSTER ? EV_LIST / 2 : EV_LIST;
+  alignas(8) int bins[EV_BINS];                // of this CTA's keys
+  alignas(8) int sums[CLUSTER ? EV_BINS : 2];  // of all CTAs', each written by one; of every other pass
+  int2 from[LIST], to[LIST];                   // (page, place)
+  int2 red[2][THREADS / 32];
+  int2 range[THREADS / 32];
+  int2 red_of[2][EV_RANKS], range_of[EV_RANKS];            // of each CTA, written by it
   int pick[3];
 };
 
-// Sums over the warps before this one of two numbers that lanes agree on, and the totals.
-template <int THREADS>
-__device__ __forceinline__ int2 ev_before(EvShared<THREADS>& sh, int a, int b, int2* all) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) {
-    sh.red[0][warp] = a;
-    sh.red[1][warp] = b;
-  }
-  __syncthreads();
-  const int x = lane < THREADS / 32 ? sh.red[0][lane] : 0;
-  const int y = lane < THREADS / 32 ? sh.red[1][lane] : 0;
-  const int2 r = make_int2(__reduce_add_sync(0xffffffffu, lane < warp ? x : 0),
-                           __reduce_add_sync(0xffffffffu, lane < warp ? y : 0));
-  *all = make_int2(__reduce_add_sync(0xffffffffu, x), __reduce_add_sync(0xffffffffu, y));
-  __syncthreads();
-  return r;
-}
-
-template <bool Q4, int THREADS>
+template <bool Q4, int THREADS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const EvictParams p) {
-  extern __shared__ uint32_t kept[];                       // keys of tokens 0 .. p.keys - 1
-  __shared__ EvShared<THREADS> sh;
+  extern __shared__ uint32_t kept[];                       // keys of this CTA's first p.keys tokens
+  __shared__ EvShared<THREADS, CLUSTER> sh;
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.x / p.hkv, head = blockIdx.x - seq * p.hkv;
+  const int pair = CLUSTER ? blockIdx.x / p.ranks : blockIdx.x;
+  const int rank = CLUSTER ? blockIdx.x - pair * p.ranks : 0;
+  const int seq = pair / p.hkv, head = pair - seq * p.hkv;
   const int64_t len = p.lens[seq];
   const int n = len < 0 ? 0 : len > p.capacity ? (int)p.capacity : (int)len;
-  if (head == 0 && threadIdx.x == 0) {
+  if (head == 0 && rank == 0 && threadIdx.x == 0) {
     p.new_lens[seq] = min(n, p.budget);
     if (len > p.capacity && p.status) atomicOr(p.status, FK_DEV_BAD_PAGE);
   }
-  if (n <= p.budget) return;
+  const int ranks = CLUSTER && n > EV_ALONE ? p.ranks : 1;
+  if (n <= p.budget || rank >= ranks) return;
+  if (CLUSTER && ranks > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  }
   const int32_t* table = p.tables + (int64_t)seq * p.table_stride;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int WARPS = THREADS / 32;
+  static_assert(!CLUSTER || WARPS == 32, "a lane reads a warp's entry of each CTA");
   const int M = p.budget - p.last, end = n - p.last;       // candidates: first .. end - 1
-  const int stretch = ((end + WARPS - 1) / WARPS + 31) & ~31;
-  const int w0 = min(warp * stretch, end), w1 = min(w0 + stretch, end);
+  const int stretch = ((end + ranks * WARPS - 1) / (ranks * WARPS) + 31) & ~31;
+  const int base = rank * WARPS * stretch;
+  const int w0 = min(base + warp * stretch, end), w1 = min(w0 + stretch, end);
+  auto sync = [&] {
+    if (CLUSTER && ranks > 1) {
+      __syncwarp();
+      cluster_barrier_sync();
+    } else {
+      __syncthreads();
+    }
+  };
+  // Sums, over the pair's (or only `here` this CTA's) warps before this one, of two numbers that a
+  // warp's lanes agree on, and the totals.
+  int turn = 0;
+  auto before_me = [&](int a, int b, int2* all, bool here) {
+    turn ^= 1;
+    if (lane == 0) sh.red[turn][warp] = make_int2(a, b);
+    __syncthreads();
+    int2 v = lane < WARPS ? sh.red[turn][lane] : make_int2(0, 0);
+    auto add = [&](bool which) {
+      return make_int2(__reduce_add_sync(0xffffffffu, which ? v.x : 0),
+                       __reduce_add_sync(0xffffffffu, which ? v.y : 0));
+    };
+    int2 before = add(lane < warp);
+    *all = add(true);
+    if (CLUSTER && !here && ranks > 1) {
+      if (warp == 0 && lane < ranks) ev_peer_store(&sh.red_of[turn][rank], lane, *all);
+      sync();
+      v = lane < ranks ? sh.red_of[turn][lane] : make_int2(0, 0);
+      const int2 more = add(lane < rank);
+      before = make_int2(before.x + more.x, before.y + more.y);
+      *all = add(true);
+    }
+    return before;
+  };
   const float* weights = p.weights + (int64_t)head * p.page;
   auto read_key = [&](int t) -> uint32_t {
     if (t < p.first || t >= w1) return 0u;
@@ -171,9 +234,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
     for (int i = w0; i < w1; i += 32) f(i + lane, read_key(i + lane));
   };
   auto each = [&](auto f) {
-    const int w = min(w1, max(w0, p.keys & ~31));
+    const int w = min(w1, max(w0, base + p.keys));
 #pragma unroll 4
-    for (int i = w0; i < w; i += 32) f(i + lane, kept[i + lane]);
+    for (int i = w0; i < w; i += 32) f(i + lane, kept[i - base + lane]);
 #pragma unroll 1
     for (int i = w; i < w1; i += 32) f(i + lane, read_key(i + lane));
   };
@@ -184,21 +247,27 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
   for (int i = w0; i < w1; i += 32) {
     const int t = i + lane;
     const uint32_t k = read_key(t);
-    if (i + 32 <= p.keys) kept[t] = k;
+    if (i + 32 <= base + p.keys) kept[t - base] = k;
     if (t < p.first || t >= w1) continue;
     lo = min(lo, k);
     hi = max(hi, k);
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  if (lane == 0) {
-    sh.range[0][warp] = lo;
-    sh.range[1][warp] = hi;
-  }
+  if (lane == 0) sh.range[warp] = make_int2((int)lo, (int)hi);
   for (int i = threadIdx.x; i < EV_BINS; i += THREADS) sh.bins[i] = 0;
   __syncthreads();
-  lo = __reduce_min_sync(0xffffffffu, lane < WARPS ? sh.range[0][lane] : ~0u);
-  hi = __reduce_max_sync(0xffffffffu, lane < WARPS ? sh.range[1][lane] : 0u);
+  auto widest = [&](int2 v) {
+    lo = __reduce_min_sync(0xffffffffu, (uint32_t)v.x);
+    hi = __reduce_max_sync(0xffffffffu, (uint32_t)v.y);
+  };
+  widest(lane < WARPS ? sh.range[lane] : make_int2(-1, 0));
+  if (CLUSTER && ranks > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // all have begun
+    if (warp == 0 && lane < ranks) ev_peer_store(&sh.range_of[rank], lane, make_int2((int)lo, (int)hi));
+    sync();
+    widest(lane < ranks ? sh.range_of[lane] : make_int2(-1, 0));
+  }
 
   // ---- the border: `want` of the keys at it stay, all above, none below ----
   int want = M - p.first;
@@ -208,19 +277,53 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
     for (int pass = 0; pass < 3; ++pass) {                 // 32 bits in parts of 11
       const int bits = 32 - __clz(hi - lo);                // 0 when all are one key
       const int shift = bits > 11 ? bits - 11 : 0;
+      const bool gather = CLUSTER && ranks <= EV_GATHER;
+      int* bins = gather && (pass & 1) ? sh.sums : sh.bins;
       if (pass > 0) {
-        for (int i = threadIdx.x; i < EV_BINS; i += THREADS) sh.bins[i] = 0;
+        for (int i = threadIdx.x; i < EV_BINS; i += THREADS) bins[i] = 0;
         __syncthreads();
       }
       each([&](int t, uint32_t k) {
-        if (t >= p.first && t < w1 && k >= lo && k <= hi) atomicAdd(&sh.bins[(k - lo) >> shift], 1);
+        if (t >= p.first && t < w1 && k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> shift], 1);
       });
-      __syncthreads();
+      sync();
       // from the top: the bin in which the sum reaches `want`
       constexpr int PER = EV_BINS / THREADS;
       int mine[PER], sum = 0;
+      const int at = EV_BINS - (threadIdx.x + 1) * PER;
+      if constexpr (CLUSTER) {
+        // of few CTAs each adds up all bins, two a thread; of more a part that it gives to all
+        const int part = gather ? THREADS : (EV_BINS / 2 + ranks - 1) / ranks;
+        const int q = gather ? at / 2 : rank * part + threadIdx.x;
+        int2 v[EV_RANKS];
+        if (threadIdx.x < part && q < EV_BINS / 2) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum += mine[i] = sh.bins[EV_BINS - 1 - (threadIdx.x * PER + i)];
+          for (int r = 0; r < EV_RANKS; ++r)
+            v[r] = r < ranks && ranks > 1
+                       ? ev_peer_load(reinterpret_cast<const int2*>(bins) + q, r)
+                       : make_int2(0, 0);
+          if (ranks == 1) v[0] = reinterpret_cast<const int2*>(bins)[q];
+#pragma unroll
+          for (int r = 1; r < EV_RANKS; ++r) {
+            v[0].x += v[r].x;
+            v[0].y += v[r].y;
+          }
+          if (!gather)
+            for (int r = 0; r < ranks; ++r)
+              ev_peer_store(reinterpret_cast<int2*>(sh.sums) + q, r, v[0]);
+        }
+        if (!gather) {
+          sync();
+          v[0] = *reinterpret_cast<const int2*>(&sh.sums[at]);
+        }
+        static_assert(!CLUSTER || PER == 2, "two bins a thread");
+        mine[0] = v[0].y;
+        mine[1] = v[0].x;
+        sum = v[0].x + v[0].y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum += mine[i] = bins[at + PER - 1 - i];
+      }
       int incl = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -228,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
         if (lane >= o) incl += up;
       }
       int2 all;
-      int above = ev_before<THREADS>(sh, __shfl_sync(0xffffffffu, incl, 31), 0, &all).x + incl - sum;
+      int above = before_me(__shfl_sync(0xffffffffu, incl, 31), 0, &all, true).x + incl - sum;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         if (above < want && above + mine[i] >= want) {
@@ -257,16 +360,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
     each([&](int t, uint32_t k) {
       here += __popc(__ballot_sync(0xffffffffu, t >= p.first && t < w1 && k == border));
     });
-    int before = ev_before<THREADS>(sh, here, 0, &all).x;
+    int before = before_me(here, 0, &all, false).x;
     if (before < want && before + here >= want) {
       each([&](int t, uint32_t k) {
         const uint32_t at = __ballot_sync(0xffffffffu, t >= p.first && t < w1 && k == border);
         if ((at >> lane & 1u) && before + __popc(at & ((1u << lane) - 1u)) == want - 1)
-          sh.pick[0] = t + 1;
+          for (int r = 0; r < ranks; ++r) {
+            if (CLUSTER) ev_peer_store(&sh.pick[0], r, t + 1);
+            else sh.pick[0] = t + 1;
+          }
         before += __popc(at);
       });
     }
-    __syncthreads();
+    sync();
     cut = sh.pick[0];
   }
   // (a place that a moved token has taken counts as one that stays, if it is looked at again)
@@ -280,49 +386,62 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
     return __ballot_sync(0xffffffffu, t < w1 && t >= M && stays(t, k));
   };
 
-  // ---- moves, in order: lists of them, then the rows ----
+  // ---- moves, in order: lists of them, a CTA every ranks-th tile, then the rows ----
   const int half = threadIdx.x >> 4;
   constexpr int TILE = THREADS / 16 * EV_ROWS;
   const int2 none = make_int2(-1, 0);
+  const int most = EvShared<THREADS, CLUSTER>::LIST * ranks;
+  auto list = [&](int2* at, int i, int t) {
+    const int2 place = ev_place(p, table, t);
+    if (CLUSTER && ranks > 1) {
+      const int tile = i / TILE, turns = tile / ranks;
+      ev_peer_store(&at[turns * TILE + i % TILE], tile - turns * ranks, place);
+    } else {
+      at[i] = place;
+    }
+  };
   auto round = [&](int done, auto over) {
     int2 here = make_int2(0, 0);
     over([&](int t, uint32_t k) {
       here.x += __popc(freed(t, k));
       here.y += __popc(moved(t, k));
     });
-    here = ev_before<THREADS>(sh, here.x, here.y, &all);
+    here = before_me(here.x, here.y, &all, false);
     here.y -= done;
     over([&](int t, uint32_t k) {
       const uint32_t fr = freed(t, k), mv = moved(t, k), below = (1u << lane) - 1u;
       const int fi = here.x + __popc(fr & below), mi = here.y + __popc(mv & below);
-      if ((fr >> lane & 1u) && fi < EV_LIST) sh.to[fi] = ev_place(p, table, t);
-      if ((mv >> lane & 1u) && mi >= 0 && mi < EV_LIST) sh.from[mi] = ev_place(p, table, t);
+      if ((fr >> lane & 1u) && fi < most) list(sh.to, fi, t);
+      if ((mv >> lane & 1u) && mi >= 0 && mi < most) list(sh.from, mi, t);
       here.x += __popc(fr);
       here.y += __popc(mv);
     });
-    __syncthreads();
-    const int count = min(EV_LIST, min(all.x, all.y - done));
-    for (int j0 = 0; j0 < count; j0 += TILE) {
+    sync();                                  // all have decided, and their lists are here
+    const int count = min(most, min(all.x, all.y - done));
+    for (int mine = 0, j0 = rank * TILE; j0 < count; mine += TILE, j0 += TILE * ranks) {
       EvPiece x[EV_ROWS];
 #pragma unroll
       for (int u = 0; u < EV_ROWS; ++u) {
-        const int j = j0 + u * (THREADS / 16) + half;
-        EvRow<Q4>(p, head, j < count ? sh.from[j] : none).load(p, x[u]);
+        const int j = u * (THREADS / 16) + half;
+        EvRow<Q4>(p, head, j0 + j < count ? sh.from[mine + j] : none).load(p, x[u]);
       }
 #pragma unroll
       for (int u = 0; u < EV_ROWS; ++u) {
-        const int j = j0 + u * (THREADS / 16) + half;
-        EvRow<Q4>(p, head, j < count && sh.from[j].x >= 0 ? sh.to[j] : none).store(p, x[u]);
+        const int j = u * (THREADS / 16) + half;
+        const bool moves = j0 + j < count && sh.from[mine + j].x >= 0;
+        EvRow<Q4>(p, head, moves ? sh.to[mine + j] : none).store(p, x[u]);
       }
     }
-    __syncthreads();
+    sync();
     return all.y;
   };
   const int moves = round(0, each);
-  for (int done = EV_LIST; done < moves; done += EV_LIST) round(done, each_read);
+  for (int done = most; done < moves; done += most) round(done, each_read);
   // ---- the newest ----
   const bool apart = n - p.budget >= p.last;               // places and sources are
-  for (int j0 = 0; j0 < p.last; j0 += TILE) {
+  if (!apart && rank > 0) return;
+  const int by = apart ? TILE * ranks : TILE;
+  for (int j0 = rank * TILE; j0 < p.last; j0 += by) {
     EvPiece x[EV_ROWS];
     int2 from[EV_ROWS], to[EV_ROWS];
 #pragma unroll
@@ -339,13 +458,42 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
   }
 }
 
-template <bool Q4, int THREADS>
-static cudaError_t ev_launch(const EvictParams& p, int64_t pairs, cudaStream_t s) {
+template <bool Q4, int THREADS, bool CLUSTER>
+static cudaError_t ev_launch(EvictParams p, int64_t pairs, cudaStream_t s) {
   static PerDeviceOnce once;
-  auto kernel = evict_kernel<Q4, THREADS>;
-  const cudaError_t e = set_max_dynamic_smem(once, kernel, EV_KEYS * 4);
+  auto kernel = evict_kernel<Q4, THREADS, CLUSTER>;
+  const cudaError_t e = set_max_dynamic_smem(once, kernel, ev_keys(THREADS) * 4);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3((unsigned)pairs), dim3(THREADS), (size_t)p.keys * 4, s, p);
+  // what a CTA can have of the tables' tokens: its warps' stretches are whole rounds of 32
+  const int64_t alone = p.capacity < EV_ALONE ? p.capacity : EV_ALONE, part = p.capacity / p.ranks;
+  const int64_t most = (part > alone ? part : alone) + THREADS;
+  p.keys = (int)(most < ev_keys(THREADS) ? most & ~31 : ev_keys(THREADS));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(pairs * p.ranks));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = (size_t)p.keys * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (CLUSTER) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)p.ranks;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+template <bool Q4>
+static cudaError_t ev_launch(const EvictParams& p, int64_t pairs, cudaStream_t s) {
+  if (p.ranks > 1) return ev_launch<Q4, 1024, true>(p, pairs, s);
+  return pairs <= sm_count() ? ev_launch<Q4, 1024, false>(p, pairs, s)
+                             : ev_launch<Q4, 512, false>(p, pairs, s);
 }
 
 static int evict(const char* what, EvictParams& p, bool q4, int64_t num_pages, int page,
@@ -358,8 +506,8 @@ static int evict(const char* what, EvictParams& p, bool q4, int64_t num_pages, i
              budget, first, last);
   if (num_seqs == 0) return FK_OK;
   FK_REQUIRE(weights && lens && new_lens && tables, FK_ERR_INVALID_ARG, "%s: null pointer", what);
-  FK_REQUIRE(lens != new_lens, FK_ERR_INVALID_ARG, "%s: the new lengths need a place of their own",
-             what);
+  FK_REQUIRE(lens + num_seqs <= new_lens || new_lens + num_seqs <= lens, FK_ERR_INVALID_ARG,
+             "%s: the new lengths need a place of their own", what);
   FK_REQUIRE(table_cols > 0 && table_stride >= 0, FK_ERR_INVALID_ARG, "%s: bad sizes", what);
   FK_REQUIRE((int64_t)num_seqs * hkv < (1ll << 31), FK_ERR_UNSUPPORTED, "%s: too many sequences",
              what);
@@ -371,14 +519,12 @@ static int evict(const char* what, EvictParams& p, bool q4, int64_t num_pages, i
   p.num_pages = (int)num_pages; p.page = page; p.hkv = hkv;
   p.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
   p.budget = budget; p.first = first; p.last = last;
-  // whole rounds of 32, up to what the tables can hold
-  p.keys = (int)(p.capacity < EV_KEYS ? (p.capacity + 31) & ~31 : EV_KEYS);
   p.status = status;
-  // With a CTA per SM or fewer, 1024 threads each: what one has to pass over and to move is the time.
   const int64_t pairs = (int64_t)num_seqs * hkv;
-  FK_CUDA_OK(pairs <= sm_count()
-                 ? (q4 ? ev_launch<true, 1024>(p, pairs, s) : ev_launch<false, 1024>(p, pairs, s))
-                 : (q4 ? ev_launch<true, 512>(p, pairs, s) : ev_launch<false, 512>(p, pairs, s)));
+  // (clusters find room where an eighth of the SMs may stay empty)
+  const int64_t ranks = sm_count() * 7 / 8 / pairs;
+  p.ranks = p.capacity <= EV_CLUSTER || ranks < 2 ? 1 : (int)(ranks < EV_RANKS ? ranks : EV_RANKS);
+  FK_CUDA_OK(q4 ? ev_launch<true>(p, pairs, s) : ev_launch<false>(p, pairs, s));
   count_launch(1);
   return FK_OK;
 }

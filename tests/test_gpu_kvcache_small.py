@@ -625,6 +625,24 @@ def test_eviction_of_long_contexts(ops, kind, n, budget, first, last):
               cols=-(-n // 256) + 30)
 
 
+@pytest.mark.parametrize("name", ["spread", "equal", "few values"])
+@pytest.mark.parametrize("kind,lens,hkv,budget,first,last", [
+    ("NHD", [13000, 10241, 100, 10240], 2, 700, 4, 20),
+    ("q4", [10500, 12000, 10240, 11000], 5, 2500, 0, 300),
+    ("HND", [10500, 11200, 3000, 10241, 14000], 8, 300, 5, 64), ("q4", [10400] * 7, 8, 1024, 0, 0),
+    ("NHD", [70000], 1, 40000, 16, 100), ("q4", [400000], 1, 900, 0, 1),
+    ("q4", [11000, 10800, 10801], 2, 10800, 4, 1000), ("HND", [20000], 1, 1, 0, 0)])
+def test_eviction_of_few_long_contexts(ops, kind, lens, hkv, budget, first, last, name):
+    """A sequence and head is cut by several CTAs: 8, 6, 3, 2 of them, with ties in all."""
+    rng = np.random.default_rng(len(lens) + budget)
+
+    def weights(n):
+        if name == "spread":
+            return spread_weights(rng, hkv)(n)
+        return np.floor(rng.random((hkv, n)) * (3 if name == "few values" else 1)).astype(np.float32)
+    run_evict(ops, rng, lens, budget, first, last, weights, 64, hkv, kind)
+
+
 def test_eviction_flags_bad_pages_and_long_contexts(ops):
     w = ops.new_attn_weights(6, 16, 1)
     cache = ops.new_kvcache_q4(6, 16, 1)

@@ -111,7 +111,8 @@ def test_pools_that_no_cache_has(fn):
     (attend_bf16, dict(stride=100), INVALID), (attend_bf16, dict(page=48), UNSUPPORTED),
     (attend_bf16, dict(k=None), INVALID), (attend_bf16, dict(cols=0), INVALID),
     (evict, dict(k=None), INVALID), (evict, dict(weights=None), INVALID), (evict, dict(new=None), INVALID),
-    (evict, dict(new=P), INVALID), (evict, dict(lens=None), INVALID), (evict, dict(d=64), UNSUPPORTED),
+    (evict, dict(new=P), INVALID), (evict, dict(new=P + 8), INVALID), (evict_q4, dict(new=P - 8), INVALID),
+    (evict, dict(lens=None), INVALID), (evict, dict(d=64), UNSUPPORTED),
     (evict, dict(layout=2), INVALID), (evict, dict(stride=100), INVALID),
     (evict, dict(v=P + 8), ALIGNMENT), (evict, dict(page=0), INVALID), (evict, dict(cols=0), INVALID)])
 def test_refusals(fn, kw, code):
