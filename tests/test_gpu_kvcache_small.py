@@ -643,6 +643,64 @@ def test_eviction_of_few_long_contexts(ops, kind, lens, hkv, budget, first, last
     run_evict(ops, rng, lens, budget, first, last, weights, 64, hkv, kind)
 
 
+def test_evictions_side_by_side_and_captured(ops):
+    """Few long sequences on two streams at once, and in a graph whose lengths change: the same bits as
+    one after another."""
+    rng = np.random.default_rng(17)
+    pages, hkv, budget, lens = 200, 2, 700, [12000, 300, 6144, 6145, 700, 701, 0, 12800]
+    start = [torch.from_numpy(rng.integers(0, 256, (pages, hkv, 4, 2304), dtype=np.uint8)).cuda(),
+             raw(rng.random((pages, hkv, 64)).astype(np.float32))]
+    t = ints([rng.permutation(pages)])
+
+    def cut(state, n, out=None):
+        return ops.evict_kvcache(state[0], state[1], n, t, budget, 4, 100, out=out)
+    want = []
+    for n in lens:
+        state = [x.clone() for x in start]
+        want.append((state, cut(state, ints([n])).tolist()))
+    torch.cuda.synchronize()
+    states, news = [[x.clone() for x in start] for _ in lens], [ints([-1]) for _ in lens]
+    sizes = [ints([n]) for n in lens]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, n in enumerate(sizes):
+        with torch.cuda.stream(streams[i % 2]):
+            cut(states[i], n, news[i])
+    torch.cuda.synchronize()
+    state, n, new = [x.clone() for x in start], ints([lens[0]]), ints([-1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cut(state, n, new)
+    for i, (ref, length) in enumerate(want):
+        for x, y in zip(states[i], ref):
+            assert torch.equal(x, y)
+        for x, y in zip(state, start):
+            x.copy_(y)
+        n.fill_(lens[i])
+        graph.replay()
+        for x, y in zip(state, ref):
+            assert torch.equal(x, y)
+        assert news[i].tolist() == new.tolist() == length == [min(lens[i], budget)]
+
+
+def test_bad_pages_of_few_long_contexts(ops):
+    """Their tokens count as the smallest and do not move; others' do, whichever CTA has them."""
+    pages, n, budget = 210, 13000, 1000
+    table = np.arange(204, dtype=np.int32)
+    table[[3, 150]] = -1, pages
+    w = ops.new_attn_weights(pages, 64, 1)
+    w[100:110] = 1.0                            # 640 tokens that stay, behind the budget
+    cache = ops.new_kvcache_q4(pages, 64, 1)
+    cache[100:110] = 7
+    st = ops.new_status("cuda")
+    assert ops.evict_kvcache(cache, w, ints([n]), ints([table]), budget, status=st).tolist() == [budget]
+    assert int(st.item()) == 2
+    # the first 360 of good pages stay, below place 424; the places of the fourth page take nothing
+    want = torch.zeros(pages * 64)
+    want[424:1000] = want[6400:7040] = 1
+    assert torch.equal(w.cpu().flatten(), want)
+
+
 def test_eviction_flags_bad_pages_and_long_contexts(ops):
     w = ops.new_attn_weights(6, 16, 1)
     cache = ops.new_kvcache_q4(6, 16, 1)
