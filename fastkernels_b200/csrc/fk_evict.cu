@@ -28,8 +28,8 @@ constexpr int EV_BINS = 2048;
 constexpr int EV_LIST = 2048;                // moves of a round
 constexpr int EV_ROWS = 4;                   // rows that 16 lanes move at a time
 constexpr int EV_RANKS = 8;                  // CTAs of a sequence and head, at most
-// Up to so many CTAs each reads the counts of all; of more one adds up a part for all (8 CTAs: 21.5 us
-// for 32, 3: 24.0 for 23.0).
+// Up to so many CTAs each reads the counts of all; of more, one adds up a part and gives it to all
+// (12 000 tokens: 8 CTAs 28.8 us this way and 32.3 that way, 3 CTAs 24.0 and 23.0).
 constexpr int EV_GATHER = 4;
 // Tokens up to which one CTA of a cluster has them all, and that tables have to hold for clusters
 // (a cluster's launch costs 2.5 us more).
