@@ -30,6 +30,9 @@ __device__ __forceinline__ int sums_most(const SumsParams& p, int2 tokens) {
 }
 
 constexpr int SUMS_CTAS = 3;                 // of an SM, all there are
+// Place of a step behind the run's: beyond all lengths, those rounded up to whole steps among them, so
+// that nothing is loaded for it.
+constexpr int SUMS_NONE = 0x7fffffff;
 
 // STEPS at a time; one where there are several query tokens, whose logits are loads enough.
 
@@ -60,7 +63,7 @@ __global__ void __launch_bounds__(SUMS_THREADS, SUMS_CTAS)
       float sum[STEPS], old[STEPS];
 #pragma unroll
       for (int j = 0; j < STEPS; ++j) {
-        key[j] = s0 + j < end ? (s0 + j) * 32 + lane : most;
+        key[j] = s0 + j < end ? (s0 + j) * 32 + lane : SUMS_NONE;
         const int i = p.page_shift >= 0 ? key[j] >> p.page_shift : key[j] / p.page;
         place[j] = key[j] - i * p.page;
         page[j] = key[j] < most ? table[i] : -1;
