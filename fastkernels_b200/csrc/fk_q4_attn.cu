@@ -307,6 +307,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
             __all_sync(0xffffffffu, other.token < 0 || (other.token == first.token &&
                                                         other.head == first.head &&
                                                         ends[w] <= other.it.steps));
+    __syncthreads();                                       // a warp's next pair takes its place there
     if (first.token < 0) return;
   }
 

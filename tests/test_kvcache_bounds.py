@@ -44,3 +44,17 @@ def test_sums_load_no_logits_behind_a_run():
                                     if eval(guard.replace("&&", " and ").strip(), {}, names):
                                         assert 0 <= base + (s0 + j) * 32 + lane < rows, (hkv, lens, run)
                     x += max(1, end - at)
+
+
+def test_warps_have_read_all_places_before_one_changes():
+    """Whether a CTA's parts become one is each warp's own reading of all warps' places, and decides who
+    meets at the barriers behind: a warp that goes on to its next pair changes its place, so a
+    barrier stands between the last such reading and the first change."""
+    text = code("fk_q4_attn.cu")
+    text = text[text.index("    q4_attn_kernel("):]
+    last = max(m.start() for m in re.finditer(r"places\[(?:0|1|w)\]|ends\[w\]",
+                                              text[:text.index("auto look_up")]))
+    change = text.index("places[warp] = now", last)
+    between = text[last:change]
+    assert "__syncthreads();" in between
+    assert "return" not in between[:between.index("__syncthreads();")]
