@@ -563,8 +563,17 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
             const int t = step * QA_STEP + lu * Q4_UNIT + row + 8 * r;
             const bool there = (lu ? w.y : w.x) >= 0 && t < at.it.len;
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
-              if (!there) vs[u][gr][r] = vl[u][gr][r] = 0.f;
+            for (int gr = 0; gr < NG; ++gr) {
+              if (there && fabsf(vs[u][gr][r]) < INFINITY && fabsf(vl[u][gr][r]) < INFINITY) continue;
+              // no weight makes nothing of a value that is no number: columns that see it have none
+              // as their sum, the others are not told
+              vs[u][gr][r] = vl[u][gr][r] = 0.f;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                  if (there && t < len[nt][j]) low[gr][nt][j] = NAN;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
