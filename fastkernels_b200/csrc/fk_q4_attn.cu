@@ -14,16 +14,17 @@
 // S^T becomes the operand P^T by one transposing move per 16 tokens.
 //
 // Rounding to fewer bits: q to fp16 with a power of two per head taken out (exact but for channels
-// 2^-26 below the largest), the weights p s to fp16 (11 bits, where bf16 caches' decode has 8), with
-// the step's largest scale's power of two taken out.  Sums, maxima, weights' lowest-value term
-// (sum p lo) are fp32.
+// 2^-26 below the largest), the weights p s to fp16 (11 bits, where bf16 caches' decode has 8), taken by
+// a power of two that the largest p s so far of the column and group decides: a scale counts by its
+// weight, and what lies 2^-19 below the largest has fewer than 11 bits.  Sums, maxima, weights'
+// lowest-value term (sum p lo) are fp32.
 //
 // Work: steps of 32 tokens of all (tokens, KV head) pairs, one after another, are cut into equal runs,
 // one for each warp of the grid.  Warps share nothing: each has a ring of steps of its own,
 // filled by bulk copies (a step is one contiguous copy of up to 4.6 KB), and no barrier between.
 // What a warp does not have whole goes to one of its two places of partial results, joined by
 // the kernel behind; where all warps of a CTA are at one pair their parts become one first.  The
-// running maximum is raised only when a logit is 8 above it (weights up to 2^8 fit), so that in
+// running maximum is raised only when a logit is 4 above it (weights up to 2^4 fit), so that in
 // most steps nothing is reduced across lanes and nothing rescaled.
 //
 // What bounds it: long contexts of up to 8 columns run at 0.94 of the copy rate once they run (64 x 4096
@@ -42,7 +43,13 @@ constexpr int QA_STEP = 32;                  // tokens of a warp's step
 constexpr int QA_AHEAD = 16;                 // steps that are looked up at a time
 constexpr float QA_NONE = -3e38f;            // reference before there is a key
 constexpr int QA_RUN = 4;                    // steps of a warp, at least
-constexpr float QA_SLACK = 8.f;              // logits may be this far above the maximum (log2)
+// Logits may be this far above the reference (log2).
+constexpr float QA_SLACK = 4.f;
+// Weights times scales are taken by powers of two into fp16, each group of a column by its own.  Where a
+// step's scale would be taken above 2^11, and so a product above 2^15, the step is looked at by its
+// weights too, and its largest product taken to 2^6 at most.  So 2^5 is the least that the largest of
+// all that has been summed is taken to, unless 2^118 makes less of it.
+constexpr int QA_LARGE = 11, QA_PRODUCT = 5, QA_MOST = 118;
 constexpr int64_t QA_LONGEST = 1ll << 30;    // tokens of a context
 
 struct Q4AttnParams {
@@ -121,6 +128,13 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
+__device__ __forceinline__ uint32_t max_bf16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// 2^(e - 127)
+__device__ __forceinline__ float power_of_2(int e) { return __int_as_float(e << 23); }
 // Two fp32 to fp16, lo = a.
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   uint32_t r;
@@ -217,6 +231,9 @@ struct QaShape {
   static constexpr int kDepth = 2;                         // steps of a warp's ring
   // the operand Q^T in registers, or in shared memory: 4 KB a warp
   static constexpr bool kSharedQ = COLS == 16;
+  // what weights are taken by in shared memory, where there are the fewest registers (256 x 64 heads:
+  // 109.3 us, 111.1 in registers; 4 windows of 32 tokens, with 8 warps: 140.0 and 138.3)
+  static constexpr bool kSharedTaken = COLS == 16 && NG == 1;
   static constexpr int kRing = kWarps * kDepth * kStage;
   static constexpr int kSmem = kRing + (kSharedQ ? kWarps * 4096 : 0);
 };
@@ -235,6 +252,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   __shared__ int2 where[WARPS][2 * QA_AHEAD];           // units of a step in the pool, -1: none
   __shared__ QaPlace places[WARPS], ahead[WARPS];       // of the pair a warp is at, of its copies
   __shared__ int ends[WARPS];
+  __shared__ float2 taken_all[S::kSharedTaken ? WARPS : 1][NG][8];
   // (maximum, sum) of the warps' parts that become one, when runs have been counted
   static_assert(sizeof(RunCount<THREADS>) >= sizeof(float2) * WARPS * COLS, "they share a place");
   float2 (*part_ml)[COLS] = reinterpret_cast<float2 (*)[COLS]>(&counted);
@@ -363,7 +381,13 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
   // weights are 2^(logit - ref); their sums, and of weights times the value's lowest
   float ref[NT][2], l[NT][2], low[NG][NT][2];
   float factor[NT][2], qsum[NG][NT][2];       // of logits: of a product, of a token's lowest
-  float vinv;                                 // 64 / (a power of two above all scales of values)
+  // what weights times scales of values are taken by
+  float2 taken_own[NG][NT];
+  auto taken = [&](int gr, int nt) -> float2& {
+    if constexpr (S::kSharedTaken) return taken_all[warp][gr][nt * 4 + quad];
+    else return taken_own[gr][nt];
+  };
+  float large[NG];                            // the scale that the largest of them takes to 2^QA_LARGE
 
   bool ok = true;
   int slot = 0, i = 0;
@@ -459,9 +483,13 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt)
           o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+          taken(gr, nt) = make_float2(power_of_2(127 + QA_MOST), power_of_2(127 + QA_MOST));
       }
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) large[gr] = power_of_2(127 + QA_LARGE - QA_MOST);
       shortest = __reduce_min_sync(0xffffffffu, shortest);
-      vinv = 1.2676506e30f;                                 // 2^100
     }
 
     const int safe = shortest / QA_STEP;                   // whole steps for all columns
@@ -531,14 +559,20 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float t = bf16lo(kp[e >> 1][0]) * acc[0][0][nt][e];
-            float b = bf16hi(kp[e >> 1][0]) * qsum[0][nt][e & 1];
+          for (int r = 0; r < 2; ++r) {
+            auto product = [&](int gr) {
+              return pair_of(acc[0][gr][nt][2 * r], acc[0][gr][nt][2 * r + 1]);
+            };
+            auto q_sum = [&](int gr) { return pair_of(qsum[gr][nt][0], qsum[gr][nt][1]); };
+            uint64_t t = mul2(pair_of(bf16lo(kp[r][0])), product(0));
+            uint64_t b = mul2(pair_of(bf16hi(kp[r][0])), q_sum(0));
             if constexpr (NG == 2) {
-              t = fmaf(bf16lo(kp[e >> 1][1]), acc[0][1][nt][e], t);
-              b = fmaf(bf16hi(kp[e >> 1][1]), qsum[1][nt][e & 1], b);
+              t = fma2(pair_of(bf16lo(kp[r][1])), product(1), t);
+              b = fma2(pair_of(bf16hi(kp[r][1])), q_sum(1), b);
             }
-            z[u][nt][e] = fmaf(t, factor[nt][e & 1], b);
+            const float2 both = both_of(fma2(t, pair_of(factor[nt][0], factor[nt][1]), b));
+            z[u][nt][2 * r] = both.x;
+            z[u][nt][2 * r + 1] = both.y;
           }
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -603,14 +637,14 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
       }
 
       // ---- new references, if a logit or a scale has left the old ones behind ----
-      float vmax = 0.f, top[NT][2];
+      float top[NT][2];
+      bool beyond = false;
 #pragma unroll
-      for (int u = 0; u < SETS; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) vmax = fmaxf(vmax, vs[u][gr][r]);
-      bool beyond = vmax * vinv > 64.f;
+      for (int gr = 0; gr < NG; ++gr) {
+        float most = fmaxf(vs[0][gr][0], vs[0][gr][1]);
+        if constexpr (SETS == 2) most = fmaxf(most, fmaxf(vs[1][gr][0], vs[1][gr][1]));
+        beyond |= most > large[gr];
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -622,35 +656,66 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
         }
       if (__builtin_expect(__any_sync(0xffffffffu, beyond), 0)) {
         constexpr int kFrom = FOLD == 2 ? 2 : 4;            // lanes of the same column, and its twin
+        int most[NG];
 #pragma unroll
-        for (int sh = 1; sh < 32; sh <<= 1)
-          vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, sh));
-        float shift = 1.f;
-        if (vmax * vinv > 64.f) {
-          const float old = vinv;
-          vinv = 64.f / __uint_as_float(((__float_as_uint(vmax) >> 23) + 1u) << 23);
-          shift = vinv / old;
-        }
+        for (int gr = 0; gr < NG; ++gr) most[gr] = 0;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          float up[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float mx = top[nt][j];
 #pragma unroll
             for (int sh = kFrom; sh < 32; sh <<= 1)
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-            const float next = fmaxf(ref[nt][j], mx);
-            const float alpha = next > ref[nt][j] ? fast_exp2(ref[nt][j] - next) : 1.f;
+            const float next = fmaxf(ref[nt][j], ceilf(mx));
+            up[j] = next - ref[nt][j];                       // whole, or all there is
+            const float alpha = fast_exp2(-up[j]);
             ref[nt][j] = next;
             l[nt][j] *= alpha;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) low[gr][nt][j] *= alpha;
-#pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
-              o[mt][nt][j] *= alpha * shift;
-              o[mt][nt][2 + j] *= alpha * shift;
-            }
           }
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            float m[2] = {0.f, 0.f};                         // the largest product
+#pragma unroll
+            for (int u = 0; u < SETS; ++u)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                  m[j] = fmaxf(m[j], fast_exp2(z[u][nt][2 * r + j] - ref[nt][j]) * vs[u][gr][r]);
+            uint32_t both = pack_bf16(m[0], m[1]);
+#pragma unroll
+            for (int sh = kFrom; sh < 32; sh <<= 1)
+              both = max_bf16(both, __shfl_xor_sync(0xffffffffu, both, sh));
+            float2 by = taken(gr, nt);
+            if constexpr (S::kSharedTaken) __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              // (what has been summed stays as it is where weights are taken by as much more as the
+              // reference is higher)
+              const float rise = (float)(__float_as_int(j ? by.y : by.x) >> 23) + up[j];
+              const int at_most = min(127 + QA_MOST, 127 + QA_PRODUCT + 127 -
+                                                         (int)(both >> (16 * j + 7) & 0xffu));
+              const float e = fminf(rise, (float)at_most), back = fast_exp2(e - rise);
+              (j ? by.y : by.x) = power_of_2((int)e);
+              most[gr] = max(most[gr], (int)e);
+#pragma unroll
+              for (int mt = 0; mt < 8; ++mt)
+                if (mt * NG / 8 == gr) {
+                  o[mt][nt][j] *= back;
+                  o[mt][nt][2 + j] *= back;
+                }
+            }
+            taken(gr, nt) = by;
+            if constexpr (S::kSharedTaken) __syncwarp();
+          }
+        }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+          large[gr] = power_of_2(min(127 + QA_LARGE + 127 - most[gr], 254));
       }
 
       // ---- weights, and the operand P^T ----
@@ -661,19 +726,24 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float w[2];
+            const uint64_t w = pair_of(fast_exp2(z[u][nt][2 * r] - ref[nt][0]),
+                                       fast_exp2(z[u][nt][2 * r + 1] - ref[nt][1]));
+            auto add_to = [](float (&to)[2], uint64_t v) {
+              const float2 both = both_of(v);
+              to[0] = both.x;
+              to[1] = both.y;
+            };
+            add_to(l[nt], add2(pair_of(l[nt][0], l[nt][1]), w));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              w[j] = fast_exp2(z[u][nt][2 * r + j] - ref[nt][j]);
-              l[nt][j] += w[j];
-#pragma unroll
-              for (int gr = 0; gr < NG; ++gr)
-                low[gr][nt][j] = fmaf(w[j], vl[u][gr][r], low[gr][nt][j]);
+            for (int gr = 0; gr < NG; ++gr) {
+              float (&sum)[2] = low[gr][nt];
+              add_to(sum, fma2(w, pair_of(vl[u][gr][r]), pair_of(sum[0], sum[1])));
             }
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-              const float f = vs[u][gr][r] * vinv;
-              const uint32_t x = transpose_8x8(pack_f16(w[0] * f, w[1] * f));
+              const float2 by = taken(gr, nt);
+              const float2 ws = both_of(mul2(mul2(w, pair_of(by.x, by.y)), pair_of(vs[u][gr][r])));
+              const uint32_t x = transpose_8x8(pack_f16(ws.x, ws.y));
               if constexpr (FOLD == 2) {
                 pt[0][gr][nt][r] = row < 4 ? x : 0u;
                 pt[1][gr][nt][r] = row < 4 ? 0u : x;
@@ -724,7 +794,6 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
     const QaPlace done = places[warp];
     const bool whole = done.step == 0 && step0 + i == done.it.steps && !joint;
     const int64_t place = 2 * me + (begin > 0 ? 1 : 0);
-    const float vback = 1.f / vinv;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -753,11 +822,14 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          const float2 by = taken(h * NG / 2, nt);
+          const float back = __fdividef(1.f, j ? by.y : by.x);
           float v[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c)
-            v[c] = fmaf(o[4 * h + (c >> 1)][nt][(c & 1) * 2 + j] * vback,
-                        (c & 1) ? 1048576.f : 16777216.f, lows[h * NG / 2]);
+            v[c] = fmaf(o[4 * h + (c >> 1)][nt][(c & 1) * 2 + j] *
+                            ((c & 1) ? 1048576.f : 16777216.f),
+                        back, lows[h * NG / 2]);
           if (whole) {
             uint4 w;
             w.x = pack_bf16(v[0] * inv, v[1] * inv);

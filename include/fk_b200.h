@@ -309,7 +309,11 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
  * tokens cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 are of sequence s, whose table is row
  * s (NULL: one token each, num_seqs = num_tokens); tokens of no sequence are left out,
  * and their rows of `out` as they were.  Tokens of one sequence share what is read, up to
- * 16 query heads together.  A token without keys gets zeros.  Keys of a page whose id is
+ * 16 query heads together.  A token without keys gets zeros.  What a query token does not
+ * see, whatever it holds, has no part in it.  Softmax weights times scales are rounded to
+ * fp16 relative to the largest such product that a query head has met in that group of
+ * channels, all else is fp32: a large scale counts by its weight, values may be as large as
+ * 2^100, and of scales below 2^-113 fewer bits are left.  Keys of a page whose id is
  * bad are left out (FK_DEV_BAD_PAGE); a context beyond block_table_cols pages, or 2^30
  * tokens, is cut there and flagged the same way.
  * weights (NULL: none), fp32 [num_pages, num_kv_heads, page_size]: to the entry of

@@ -1,4 +1,4 @@
-"""4-bit caches on the GPU: values that are no numbers."""
+"""4-bit caches on the GPU: values that are no numbers, scales far apart."""
 import numpy as np
 import pytest
 
@@ -20,8 +20,9 @@ def near(got, b):
     """Against 64 bits, element by element, where neither is no number; which are has to agree.  Relative
     to what the weights give, not to the largest scale of all: bf16 of the result; per key the
     weight's error (weight_error) and, of the codes' part, fp16's (2^-11) or, below fp16's numbers,
-    2^-25 where the largest weight times scale is 2^5 at least; sums of products in fp32, 2^-22 of the
-    whole each."""
+    2^-25 where the largest weight times scale is 2^4 at least (of scales so small that this takes
+    more than 2^118: 2^-25 of 2^-118); sums of products in fp32, 2^-22 of the whole each; half of
+    bf16's smallest step, 2^-134."""
     kv = [[S.values(x, b.group) for x in side] for side in (b.k, b.v)]
     out, _, reach, sums = S.attention(b.q, *kv, b.q_lens, b.seq_of, b.scale)
 
@@ -33,7 +34,8 @@ def near(got, b):
     step = 15 * given([S.quantise(x, b.group)[1] for x in b.v])
     keys = max(b.lens)
     rel = weight_error(reach)[..., None] + (keys / 16 + 8) * 2.0 ** -22
-    tol = np.abs(out) * 2.0 ** -8 + low * rel + step * (2.0 ** -11 + rel + keys * 2.0 ** -30)
+    tol = np.abs(out) * 2.0 ** -8 + low * rel + step * (2.0 ** -11 + rel + keys * 2.0 ** -29) + \
+        keys * 15 * 2.0 ** -143 + 2.0 ** -134
     got = host_f32(got).astype(np.float64)
     np.testing.assert_array_equal(np.isnan(got), np.isnan(out))
     d = np.where(np.isnan(out), 0, np.abs(got - out) - tol)
@@ -65,3 +67,85 @@ def test_tokens_see_no_value_of_later_ones(ops, hq, hkv, page, group, lens, coun
         assert not np.isnan(out[:seen]).any() and np.isnan(out[seen:counts[0]]).any()
         if sums and what != "key":
             check_sums(b, w, reach, want, None)
+
+
+# -------------------------------------------------------------------------------- scales far apart
+def steered(rng, lens, hkv, group, levels, v, slopes, counts=None):
+    """A batch whose logits are slopes[head] * levels[token], in units of e: the keys' first channel says
+    the level, the queries' first channel the slope."""
+    hq = len(slopes)
+    k = []
+    for n in lens:
+        x = S.randn(rng, n, hkv, D, scale=0.01) * np.float32(0.02)
+        x[:, :, 0] = levels(n)[:, None]
+        k.append(S.bf16(x))
+    b = Batch(rng, lens, hq, hkv, group, 64, counts, k=k, v=v)
+    b.q[...] = S.bf16(rng.standard_normal(b.q.shape).astype(np.float32) * np.float32(0.01))
+    b.q[:, :, 0] = np.asarray(slopes, np.float32) * np.float32(8.0)
+    b.scale = 0.125
+    return b
+
+
+@pytest.mark.parametrize("hq,hkv,group,counts", [(4, 4, 64, None), (8, 2, 64, None), (8, 2, 128, None),
+                                                 (8, 1, 64, None), (16, 1, 128, None),
+                                                 (16, 1, 64, None), (8, 2, 64, [3, 4]),
+                                                 (5, 1, 128, [1, 6])])
+@pytest.mark.parametrize("far", [22, 28, 60, 100])
+def test_a_large_scale_counts_by_its_weight(ops, hq, hkv, group, counts, far):
+    """One token's values are 2^far times the others' and its weight is less than 2^-far: what the others
+    give is as exact as without it, wherever it stands, and for the heads that look at nothing else
+    it is exact too."""
+    rng = np.random.default_rng(far + hq)
+    deep = far * 0.6931 + 14.0
+    lens = [300, 2500]
+    for place in (0, 20, 150, 290):
+        v = [S.randn(rng, n, hkv, D) for n in lens]
+        for x in v:
+            x[place] = S.bf16(x[place] * np.float32(2.0 ** far))
+
+        def levels(n):
+            at = rng.uniform(-2, 0, n).astype(np.float32)
+            at[place] = -deep
+            return at
+        # of every KV head's, the last query head looks the other way
+        slopes = np.ones(hq)
+        g = hq // hkv
+        if g > 1:
+            slopes[g - 1::g] = -1.0
+        b = steered(rng, lens, hkv, group, levels, v, slopes, counts)
+        got = ops.paged_decode_attn_q4(dev(b.q), b.cache(ops), ints(b.q_lens), ints(b.tables), b.scale,
+                                       cu_seqlens_q=ints(b.cu) if counts else None)
+        near(got, b)
+
+
+@pytest.mark.parametrize("hq,hkv,group", [(4, 4, 64), (8, 2, 128), (8, 1, 64), (16, 1, 64), (16, 1, 128)])
+def test_scales_that_fall_while_logits_rise(ops, hq, hkv, group):
+    """The largest weight times scale so far shrinks from step to step, and one group of channels is far
+    below the other."""
+    rng = np.random.default_rng(hq)
+    lens = [400, 90]
+    v = []
+    for n in lens:
+        x = S.randn(rng, n, hkv, D) * np.exp2(-np.arange(n) / 8.0 + 30)[:, None, None]
+        x[:, :, 64:] *= 2.0 ** -40
+        v.append(S.bf16(x.astype(np.float32)))
+
+    def levels(n):
+        return (np.arange(n) / 6.0).astype(np.float32) - 30
+    near(*both(ops, steered(rng, lens, hkv, group, levels, v, np.ones(hq))))
+    near(*both(ops, steered(rng, lens, hkv, group, levels, v, -np.ones(hq))))
+
+
+@pytest.mark.parametrize("hq,hkv,group", [(4, 4, 64), (8, 1, 128), (16, 1, 64)])
+@pytest.mark.parametrize("size", [-126, -100, 100])
+def test_values_near_the_ends_of_the_type(ops, hq, hkv, group, size):
+    rng = np.random.default_rng(hq)
+    lens = [200, 33]
+    v = [S.bf16((S.randn(rng, n, hkv, D).astype(np.float64) * 2.0 ** size).astype(np.float32))
+         for n in lens]
+    b = Batch(rng, lens, hq, hkv, group, 64, v=v)
+    near(*both(ops, b))
+
+
+def both(ops, b):
+    return ops.paged_decode_attn_q4(dev(b.q), b.cache(ops), ints(b.q_lens), ints(b.tables), b.scale), b
