@@ -19,6 +19,8 @@
 // lists go between them by their shared memory, and rows are moved by all.  8 pairs of 12 000 tokens
 // take 20.3 us (alone 22.7), of 40 000 24.4 (52), of 100 000 36 (282).  Barriers and peers' loads cost
 // some 6 us.
+#include <type_traits>
+
 #include "fk_q4.cuh"
 #include "fk_tcgen05.cuh"
 
@@ -154,6 +156,7 @@ struct EvShared {
   int2 range[THREADS / 32];
   int2 red_of[2][EV_RANKS], range_of[EV_RANKS];            // of each CTA, written by it
   int pick[3];
+  int next_turn[2];            // behind the last place of the lists before, and of these
 };
 
 template <bool Q4, int THREADS, bool CLUSTER>
@@ -375,12 +378,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
     sync();
     cut = sh.pick[0];
   }
-  // (a place that a moved token has taken counts as one that stays, if it is looked at again)
   auto stays = [&](int t, uint32_t k) {
     return t < p.first || k > border || (k == border && t < cut);
   };
-  auto freed = [&](int t, uint32_t k) {
-    return __ballot_sync(0xffffffffu, t < min(w1, M) && !stays(t, k));
+  // Places whose turn has been are not looked at again: a moved token's weight is there now, or, where a
+  // page id is bad, the old one.
+  auto freed = [&](int t, uint32_t k, auto later) {
+    bool turn = t < min(w1, M) && !stays(t, k);
+    if constexpr (later) turn = turn && t >= sh.next_turn[0];
+    return __ballot_sync(0xffffffffu, turn);
   };
   auto moved = [&](int t, uint32_t k) {
     return __ballot_sync(0xffffffffu, t < w1 && t >= M && stays(t, k));
@@ -400,18 +406,25 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
       at[i] = place;
     }
   };
-  auto round = [&](int done, auto over) {
+  auto round = [&](int done, auto over, auto later) {
     int2 here = make_int2(0, 0);
     over([&](int t, uint32_t k) {
-      here.x += __popc(freed(t, k));
+      here.x += __popc(freed(t, k, later));
       here.y += __popc(moved(t, k));
     });
     here = before_me(here.x, here.y, &all, false);
     here.y -= done;
     over([&](int t, uint32_t k) {
-      const uint32_t fr = freed(t, k), mv = moved(t, k), below = (1u << lane) - 1u;
+      const uint32_t fr = freed(t, k, later), mv = moved(t, k), below = (1u << lane) - 1u;
       const int fi = here.x + __popc(fr & below), mi = here.y + __popc(mv & below);
-      if ((fr >> lane & 1u) && fi < most) list(sh.to, fi, t);
+      if ((fr >> lane & 1u) && fi < most) {
+        list(sh.to, fi, t);
+        if (fi == most - 1)
+          for (int r = 0; r < ranks; ++r) {
+            if (CLUSTER) ev_peer_store(&sh.next_turn[1], r, t + 1);
+            else sh.next_turn[1] = t + 1;
+          }
+      }
       if ((mv >> lane & 1u) && mi >= 0 && mi < most) list(sh.from, mi, t);
       here.x += __popc(fr);
       here.y += __popc(mv);
@@ -435,8 +448,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) evict_kernel(const Ev
     sync();
     return all.y;
   };
-  const int moves = round(0, each);
-  for (int done = most; done < moves; done += most) round(done, each_read);
+  const int moves = round(0, each, std::false_type{});
+  for (int done = most; done < moves; done += most) {
+    if (threadIdx.x == 0) sh.next_turn[0] = sh.next_turn[1];
+    __syncthreads();
+    round(done, each_read, std::true_type{});
+  }
   // ---- the newest ----
   const bool apart = n - p.budget >= p.last;               // places and sources are
   if (!apart && rank > 0) return;

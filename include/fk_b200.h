@@ -340,7 +340,8 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
  * attention; which place a token has may differ from head to head.  Nothing behind
  * `budget` is changed.  new_context_lens[s] = min(context_lens[s], budget), a buffer of its
  * own.  A page is in one table only; a token whose page id is bad counts as the smallest
- * and does not move (FK_DEV_BAD_PAGE).  One launch.
+ * and does not move, and its place takes nothing: the turn of either passes
+ * (FK_DEV_BAD_PAGE).  One launch.
  * ---------------------------------------------------------------------- */
 int64_t fk_q4_unit_bytes(int head_dim, int group);
 

@@ -1,10 +1,11 @@
-"""4-bit caches on the GPU: values that are no numbers, scales far apart."""
+"""4-bit caches on the GPU: values that are no numbers, scales far apart, bad pages of long evictions."""
 import numpy as np
 import pytest
+import torch
 
 import kvcache_oracle as S
 from gpu_util import dev, host_f32
-from test_gpu_kvcache_small import Batch, check_sums, ints, weight_error
+from test_gpu_kvcache_small import Batch, check_sums, ints, raw, weight_error
 
 pytestmark = pytest.mark.gpu
 D = 128
@@ -149,3 +150,50 @@ def test_values_near_the_ends_of_the_type(ops, hq, hkv, group, size):
 
 def both(ops, b):
     return ops.paged_decode_attn_q4(dev(b.q), b.cache(ops), ints(b.q_lens), ints(b.tables), b.scale), b
+
+
+# ---------------------------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("n,budget,first,last,cols", [(10000, 6000, 4, 100, 0), (10000, 9000, 0, 0, 0),
+                                                      (40000, 24000, 16, 300, 30)])
+@pytest.mark.parametrize("many", [False, True])
+def test_bad_pages_of_evictions_with_many_moves(ops, n, budget, first, last, cols, many):
+    """More moves than a list holds, and places among the first that take nothing: the i-th token that
+    stays still goes to the i-th place that became free, or nowhere.  many: so many bad pages that
+    tokens of them stay."""
+    rng = np.random.default_rng(n + budget)
+    pages = -(-n // 64) + 2
+    table = np.full(-(-n // 64) + cols, -1, np.int32)
+    table[:-(-n // 64)] = rng.permutation(pages)[:-(-n // 64)]
+    live = -(-(n - last) // 64) - 1
+    bad = np.sort(rng.permutation(np.arange(first // 64 + 1, live))[:(n - budget) // 64 + 8 if many else 5])
+    if not many:
+        bad[:2] = first // 64 + 1, first // 64 + 3                # places that the first round fills
+    table[bad] = np.where(np.arange(len(bad)) % 2, -1, pages)
+    at = np.arange(n)
+    there = ~np.isin(at // 64, bad)
+    slot = np.where(there, table[at // 64].astype(np.int64) * 64 + at % 64, 0)
+    # most of what stays stands behind the budget
+    key = rng.random(n).astype(np.float32) + (at > 0.45 * n)
+    w = np.full(pages * 64, -5.0, np.float32)
+    w[slot[there]] = key[there]
+    rows = rng.integers(0, 2 ** 15, (pages * 64, 2, D), dtype=np.int16)
+    middle = budget - last
+    order = sorted(range(first, n - last), key=lambda i: (-(key[i] if there[i] else -np.inf), i))
+    stay = np.zeros(n, bool)
+    stay[:first] = True
+    stay[order[:middle - first]] = True
+    movers = np.flatnonzero(stay & (at >= middle) & (at < n - last))
+    free = np.flatnonzero(~stay[:middle])
+    assert len(movers) == len(free) and len(movers) > (8192 if cols else min(1500, n - budget - 300))
+    moves = list(zip(movers, free)) + [(n - last + i, middle + i) for i in range(last)]
+    want_w, want = w.copy(), rows.copy()
+    for a, b in moves:
+        if there[a] and there[b]:
+            want_w[slot[b]], want[slot[b]] = w[slot[a]], rows[slot[a]]
+    pools = [raw(rows[:, i].reshape(pages, 64, 1, D)).view(torch.bfloat16) for i in range(2)]
+    dw, st = raw(w.reshape(pages, 1, 64)), ops.new_status("cuda")
+    new = ops.evict_kvcache(tuple(pools), dw, ints([n]), ints([table]), budget, first, last, status=st)
+    assert new.tolist() == [budget] and int(st.item()) == 2
+    np.testing.assert_array_equal(dw.cpu().numpy().reshape(-1), want_w)
+    for i, x in enumerate(pools):
+        np.testing.assert_array_equal(x.view(torch.int16).cpu().numpy().reshape(-1, D), want[:, i])
