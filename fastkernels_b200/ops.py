@@ -846,6 +846,9 @@ def evict_kvcache(caches, weights, context_lens, block_tables, budget, keep_firs
     ts, cols, rows = _need_tables(dev, block_tables)
     if rows != n:
         raise _lib.FkError(f"block_tables must have {n} rows, got {rows}")
+    for name, x in (("budget", budget), ("keep_first", keep_first), ("keep_last", keep_last)):
+        if not -2 ** 31 <= x < 2 ** 31:
+            raise _lib.FkError(f"{name} {x} is beyond 32 bits")
     if out is None:
         out = torch.empty_like(context_lens)
     else:

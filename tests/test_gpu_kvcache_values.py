@@ -197,3 +197,13 @@ def test_bad_pages_of_evictions_with_many_moves(ops, n, budget, first, last, col
     np.testing.assert_array_equal(dw.cpu().numpy().reshape(-1), want_w)
     for i, x in enumerate(pools):
         np.testing.assert_array_equal(x.view(torch.int16).cpu().numpy().reshape(-1, D), want[:, i])
+
+
+def test_budgets_beyond_32_bits_are_refused(ops):
+    from fastkernels_b200._lib import FkError
+    w, cache = ops.new_attn_weights(4, 16, 1), ops.new_kvcache_q4(4, 16, 1)
+    lens, t = ints([60]), ints([[0, 1, 2, 3]])
+    for args in ((2 ** 32 + 20,), (2 ** 31,), (40, 2 ** 32 + 1), (40, 0, 2 ** 32 + 1), (-2 ** 32 + 20,)):
+        with pytest.raises(FkError, match="32 bits"):
+            ops.evict_kvcache(cache, w, lens, t, *args)
+    assert ops.evict_kvcache(cache, w, lens, t, 2 ** 31 - 1).tolist() == [60]
