@@ -16,9 +16,9 @@
 // bytes are 4 a token to decide and each moved row twice.
 //
 // Where there are fewer pairs than half the SMs a cluster of up to 8 CTAs has one: counts, sums and
-// lists go between them by their shared memory, and rows are moved by all.  8 pairs of 12 000 tokens
-// take 20.3 us (alone 22.7), of 40 000 24.4 (52), of 100 000 36 (282).  Barriers and peers' loads cost
-// some 6 us.
+// lists go between them by their shared memory, and rows are moved by all.  8 pairs of 12 000 tokens of
+// a 4-bit cache cut to 1024 take 20.7 us (one CTA each 22.7), of bf16 21.6; bf16 of 40 000 24.4 (52), of
+// 100 000 cut to 4096 36.6 (282).  Barriers and peers' loads cost some 6 us.
 #include <type_traits>
 
 #include "fk_q4.cuh"
@@ -30,11 +30,14 @@ constexpr int EV_BINS = 2048;
 constexpr int EV_LIST = 2048;                // moves of a round
 constexpr int EV_ROWS = 4;                   // rows that 16 lanes move at a time
 constexpr int EV_RANKS = 8;                  // CTAs of a sequence and head, at most
-// Up to so many CTAs each reads the counts of all; of more, one adds up a part and gives it to all
-// (12 000 tokens: 8 CTAs 28.8 us this way and 32.3 that way, 3 CTAs 24.0 and 23.0).
+// Up to so many CTAs each reads the counts of all; of more, each adds up a part and gives it to all.  4-bit
+// caches of 12 000 tokens cut to 1024: 3 CTAs (40 pairs) 21.8 us by reading all and 22.8 by parts, 8 CTAs
+// (8 pairs) 24.7 and 20.7.
 constexpr int EV_GATHER = 4;
-// Tokens up to which one CTA of a cluster has them all, and that tables have to hold for clusters
-// (a cluster's launch costs 2.5 us more).
+// Tokens up to which one CTA of a cluster has them all, and that tables have to hold for clusters, whose
+// launch costs 2.5 us more.  8 pairs of a 4-bit cache, one CTA each and 8: 8000 tokens 18.2 us and 19.4,
+// 10 000 20.7 and 20.7, 12 000 22.7 and 20.7; under tables that hold 12 800, one CTA of a cluster and all:
+// 5000 tokens 17.7 us and 19.2, 6000 18.9 and 19.3, 7000 by all 19.4.
 constexpr int EV_ALONE = 6144, EV_CLUSTER = 10240;
 // Tokens whose keys a CTA keeps: two CTAs of 512 threads are on an SM, or one of 1024.
 __host__ __device__ constexpr int ev_keys(int threads) { return threads == 512 ? 14336 : 43008; }

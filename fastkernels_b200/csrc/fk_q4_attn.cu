@@ -27,10 +27,13 @@
 // running maximum is raised only when a logit is 4 above it (weights up to 2^4 fit), so that in
 // most steps nothing is reduced across lanes and nothing rescaled.
 //
-// What bounds it: long contexts of up to 8 columns run at 0.94 of the copy rate once they run (64 x 4096
-// to 64 x 8192 tokens, 32 / 8 heads: 62.5 to 110 us for 302 MB more); the beginning of the runs
-// takes some 9 us, the join 5.  A step is some 490 warp instructions at half of the issue slots.
-// 16 columns are bound by instructions (256 sequences, 64 / 4 heads: 109 us, 2.9 TB/s).
+// What bounds it: long contexts of up to 8 columns run at 0.99 of the copy rate once they run (64 x 4096
+// to 64 x 8192 tokens, 32 / 8 heads: 62.4 to 109.1 us for 302 MB more); the beginning of the runs
+// takes some 9 us, the join 5.  A step is some 480 warp instructions at half of the issue slots.
+// 16 columns are bound by waiting (256 sequences, 64 / 4 heads: 109.7 us, 2.9 TB/s): the registers leave
+// 3 warps a scheduler, each a chain of copy, product, exponential, transpose and product; 0.45 of the
+// issue slots are used, and a warp waits 1.9 times an instruction for the one before, 0.8 times each
+// for a pipe and for instructions to be fetched.
 #include "fk_q4.cuh"
 #include "fk_runs.cuh"
 #include "fk_sums.cuh"
@@ -142,7 +145,9 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return r;
 }
 
-// bulk_load of what is read once: it leaves L2 first.
+// A bulk load whose lines leave L2 first, so that logits and parts stay.  Also where several blocks of
+// query tokens read a cache one after another (256 x 64 heads 109.7 us, 115.5 with lines that stay as
+// long as others; drafts of 5 tokens 107 and 112; 4 windows of 32 tokens 136.5 and 137.4).
 __device__ __forceinline__ uint64_t qa_policy() {
   uint64_t r;
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(r));
@@ -224,15 +229,15 @@ struct QaShape {
   static constexpr int kUnit = q4_unit_bytes(NG);
   static constexpr int kStage = 2 * kUnit;
   static constexpr int kCtas = COLS == 16 ? 1 : 2;         // of an SM
-  // 16 columns of two groups need the registers of 8 warps (4 windows of 32 tokens: 158 us, 181
-  // with 12), of one group they do with those of 12 (256 x 64 heads: 114 us, 126 with 8)
+  // 16 columns of two groups need the registers of 8 warps (4 windows of 32 tokens with sums: 137 us,
+  // 163 with 12), of one group they do with those of 12 (256 x 64 heads: 109.7 us, 121.8 with 8)
   static constexpr int kWarps = COLS == 16 && NG == 1 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kDepth = 2;                         // steps of a warp's ring
   // the operand Q^T in registers, or in shared memory: 4 KB a warp
   static constexpr bool kSharedQ = COLS == 16;
   // what weights are taken by in shared memory, where there are the fewest registers (256 x 64 heads:
-  // 109.3 us, 111.1 in registers; 4 windows of 32 tokens, with 8 warps: 140.0 and 138.3)
+  // 109.3 us, 111.1 in registers; 4 windows of 32 tokens, of two groups and 8 warps: 140.0 and 138.3)
   static constexpr bool kSharedTaken = COLS == 16 && NG == 1;
   static constexpr int kRing = kWarps * kDepth * kStage;
   static constexpr int kSmem = kRing + (kSharedQ ? kWarps * 4096 : 0);
@@ -1006,8 +1011,10 @@ struct QaLayout {
   int64_t logit_steps;
 };
 static int qa_columns(int tokens, int seqs, int g, int* block) {
-  // query tokens of a sequence that go together: as many as 16 columns hold, and no more than
-  // there are on average
+  // Query tokens of a sequence that go together: as many as 16 columns hold, and no more than there are
+  // on average, since empty columns cost what full ones do.  Against as many as 16 columns hold, 4 query
+  // heads, contexts of 4000: 64 x 1 token 66 us (101), 64 x 2 77 (108), 31 x 1 and one of 32 tokens
+  // 56 (76); but 56 x 1 and 8 of 16 tokens 160 (143).
   int n = 16 / g;
   const int mean = seqs > 0 ? (tokens + seqs - 1) / seqs : 1;
   if (n > mean) n = mean;
@@ -1017,7 +1024,7 @@ static int qa_columns(int tokens, int seqs, int g, int* block) {
 }
 // A small call -- each pair has a CTA of its own at once, and tables of at most 2048 tokens leave the
 // CTA's warps little to do each -- is one launch, without runs, parts, join or workspace (1 x 500
-// tokens: 7 us, 13).
+// tokens: 7.4 us; 13 by runs).
 static bool qa_direct(int tokens, int hkv, int cols, bool sums, int64_t max_len) {
   return !sums && max_len > 0 && max_len <= 2048 &&
          (int64_t)tokens * hkv <= (int64_t)(cols <= 8 ? 2 : 1) * sm_count();

@@ -34,8 +34,9 @@ constexpr int SUMS_CTAS = 3;                 // of an SM, all there are
 // that nothing is loaded for it.
 constexpr int SUMS_NONE = 0x7fffffff;
 
-// STEPS at a time; one where there are several query tokens, whose logits are loads enough.
-
+// STEPS at a time: four where each sequence has one query token (64 sequences of 1024 to 5000: 72.5 us
+// with the attention before, 85 by one), one where there are several, whose logits are loads enough (4
+// windows of 32 tokens: 137 us, 161 by four; a bf16 pool and 8 x 4 tokens: 110 and 105).
 template <int STEPS>
 __global__ void __launch_bounds__(SUMS_THREADS, SUMS_CTAS)
     attn_sums_kernel(const SumsParams p) {
@@ -71,7 +72,8 @@ __global__ void __launch_bounds__(SUMS_THREADS, SUMS_CTAS)
       }
       int t = tokens.x;
       if constexpr (STEPS == 1) {
-        // blocks of 16 columns, two at a time
+        // blocks of 16 columns, two at a time (4 windows of 32 tokens: 137 us, 150 by the loop below,
+        // which takes all others)
         if (p.first && p.cols == 16 && p.ml_col == 1) {
           for (; t + 2 * p.block <= tokens.y; t += 2 * p.block) {
             float4 v[2][4], m[2][8];

@@ -326,9 +326,10 @@ int fk_selected_attn(const void* q, int64_t q_stride_token, void* out, int64_t o
  * of any tables is that for 0, and for the tokens that tables hold it may be less: none
  * for few sequences with tables of up to 2048 tokens.
  *
- * fk_paged_decode_attn_weights: the same over bf16 pools, for num_q_heads / num_kv_heads
- * 1, 2, 4, 8 or 16; the keys of a bad page are zeros, as in fk_paged_decode_attn, and have
- * no entry.  Launches: [tables of the tokens,] schedule, attention, merge and sums.
+ * fk_paged_decode_attn_weights: the same sums over bf16 pools, for num_q_heads /
+ * num_kv_heads 1, 2, 4, 8 or 16.  Here each query token reads its keys for itself; the keys
+ * of a bad page are zeros, as in fk_paged_decode_attn, and have no entry.  Launches: [tables
+ * of the tokens,] schedule, attention, merge and sums.
  *
  * fk_evict_kvcache (bf16 pools), fk_evict_kvcache_q4: of every sequence of more than
  * `budget` tokens and each of its KV heads `budget` tokens stay: the first keep_first, the
