@@ -494,6 +494,7 @@ __global__ void __launch_bounds__((QaShape<NG, COLS>::kThreads), (QaShape<NG, CO
       }
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) large[gr] = power_of_2(127 + QA_LARGE - QA_MOST);
+      if constexpr (S::kSharedTaken) __syncwarp();
       shortest = __reduce_min_sync(0xffffffffu, shortest);
     }
 
